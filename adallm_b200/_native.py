@@ -29,6 +29,7 @@ ADA_ERR_TIMEOUT = 6
 ADA_ERR_CUDA = 7
 
 DT = {torch.bfloat16: 0, torch.float16: 1}
+DT_LOGITS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # the sampling entries
 
 P, I32, I64, F32, INT, SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_int, C.c_size_t
 PP, U32 = C.POINTER(C.c_void_p), C.c_uint32
@@ -70,6 +71,15 @@ _SIGS = {
     "ada_argmax_workspace_size": (SZ, [I64, I64]),
     "ada_argmax": (INT, [P, I64, I64, I64, INT, P, P, SZ, P]),
     "ada_argmax_noalloc": (INT, [P, I64, I64, I64, INT, P, P]),
+    "ada_fp8_shared_prefix_decode_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32]),
+    "ada_fp8_shared_prefix_decode": (INT, [P, INT, I64, I64, P, P, I64, I64, I64, I64, P, I64, I32, P, P, I32, P, I64,
+                                           I32, P, P, I32, I32, I32, I32, I32, I32, F32, F32, F32, I32, P, INT, I64,
+                                           I64, P, SZ, P, P]),
+    "ada_sample_workspace_size": (SZ, [I64, I64]),
+    "ada_sample": (INT, [P, INT, I64, I64, I64, P, P, I64, P, P, P, P, SZ, P]),
+    "ada_verify_drafts_workspace_size": (SZ, [I32, I32, I64]),
+    "ada_verify_drafts": (INT, [P, INT, I64, I32, I64, P, P, I32, I32, P, P, I64, P, I64, P, I64, I64, P, I64, I64, P,
+                                P, P, P, SZ, P]),
     "ada_nvfp4_sf_bytes": (SZ, [I64, I64]),
     "ada_nvfp4_prepack_scales": (INT, [P, INT, I64, I64, I64, P, P]),
     "ada_nvfp4_linear_workspace_size": (SZ, [I64, I64, I64, INT]),
@@ -168,7 +178,8 @@ _ERROR_BITS = [(0x1, "GEMM producer waited for a free pipeline stage"),
 _ERROR_CODES = {0x50: "a peer's partial planes never arrived (tensor-parallel inbox wait)",
                 0x60: "an expert id outside [0, num_experts)",
                 0x70: "a prefill attention tile load never completed",
-                0x80: "a router logit never arrived (fused MoE router wait)"}
+                0x80: "a router logit never arrived (fused MoE router wait)",
+                0x90: "a shared-prefix attention tile never completed"}
 
 
 def describe_error_word(code: int) -> str:

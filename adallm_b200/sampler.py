@@ -1,0 +1,128 @@
+"""Sampling at a temperature and verification of drafted tokens (B200 kernels).
+
+  * sample: the reference's Sampler.forward (adallm/ops/sampler.py:10-15: softmax(logits / T)
+    divided by Exp(1) noise, argmax) with the noise given, and the log-normaliser of every row
+  * verify_drafts: acceptance of drafted tokens against the target's probabilities, given the
+    draft's logits and their log-normalisers (what ``sample`` returned when it drew them)
+  * Sampler: the reference's module on these kernels
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from . import _native as N
+
+
+def _rows(t: torch.Tensor, name: str, dtypes, dim: int = 2) -> torch.Tensor:
+    if t.dim() != dim or t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {dim}-D, one of {[str(d) for d in dtypes]}")
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[-1])
+
+
+def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
+    if t.dtype != dtype or t.numel() != n:
+        raise ValueError(f"{name} must be {dtype} with {n} entries")
+    return t.contiguous()
+
+
+def _workspace(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor:
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace
+
+
+def sample(logits: torch.Tensor, temperatures: torch.Tensor, noise: torch.Tensor,
+           workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """One token per row of logits [R, V] (bf16/fp16/fp32; rows may be strided).
+
+    temperatures fp32 [R] (<= 1e-10: greedy); noise fp32 [R, V]: Exp(1) draws.
+    Returns (tokens int64 [R], logprobs fp32 [R], lse fp32 [R]): the draw, its log-probability
+    and the row's log-normaliser, both at the row's temperature (1 where greedy).  A row whose
+    logits are all -inf gives -1, 0 and -inf."""
+    N.require_cuda(logits, temperatures, noise, workspace, what="sample")
+    logits = _rows(logits, "logits", N.DT_LOGITS)
+    noise = _rows(noise, "noise", (torch.float32,))
+    r, v = logits.shape
+    temperatures = _vector(temperatures, "temperatures", torch.float32, r)
+    if noise.shape != logits.shape:
+        raise ValueError("noise must have one entry per logit")
+    d = logits.device
+    tokens = torch.empty(r, dtype=torch.int64, device=d)
+    logprobs = torch.empty(r, dtype=torch.float32, device=d)
+    lse = torch.empty(r, dtype=torch.float32, device=d)
+    if r == 0:
+        return tokens, logprobs, lse
+    lib = N.lib()
+    need = lib.ada_sample_workspace_size(r, v)
+    ws = _workspace(workspace, need, d)
+    st = lib.ada_sample(logits.data_ptr(), N.DT_LOGITS[logits.dtype], _ld(logits), r, v, temperatures.data_ptr(),
+                        noise.data_ptr(), _ld(noise), tokens.data_ptr(), logprobs.data_ptr(), lse.data_ptr(),
+                        ws.data_ptr(), need, N.stream_ptr(d))
+    N.check(st, "sampling kernel")
+    return tokens, logprobs, lse
+
+
+def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                  temperatures: torch.Tensor, uniforms: torch.Tensor, noise: torch.Tensor,
+                  draft_logits: torch.Tensor | None = None, draft_lse: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Accepts each sequence's drafted tokens up to the first refusal and draws the token after them.
+
+    target_logits [N, V] (bf16/fp16/fp32): the target's logits of the rows input_ids int64 [N];
+    cu_seqlens_q int32 [B + 1]: sequence b's rows are its last known token and then its drafts;
+    temperatures fp32 [B] (<= 1e-10: greedy); uniforms fp32 [B, D] in [0, 1); noise fp32 [B, V]
+    Exp(1); draft_logits [B, D, V] (target's dtype, any strides with unit stride in V) and
+    draft_lse fp32 [B, D]: the logits each draft was drawn from and their log-normaliser at the
+    sequence's temperature (``sample`` returns it); both None for drafts without a distribution.
+    Returns (tokens int64 [B, D + 1], accepted int32 [B], logprobs fp32 [B, D + 1]): the accepted
+    drafts and the drawn token with their log-probabilities under the target, then -1 and 0."""
+    N.require_cuda(target_logits, input_ids, cu_seqlens_q, temperatures, uniforms, noise, draft_logits, draft_lse,
+                   workspace, what="verify_drafts")
+    target_logits = _rows(target_logits, "target_logits", N.DT_LOGITS)
+    noise = _rows(noise, "noise", (torch.float32,))
+    uniforms = _rows(uniforms, "uniforms", (torch.float32,))
+    (n, v), (b, most) = target_logits.shape, uniforms.shape
+    temperatures = _vector(temperatures, "temperatures", torch.float32, b)
+    input_ids = _vector(input_ids, "input_ids", torch.int64, n)
+    cu_seqlens_q = _vector(cu_seqlens_q, "cu_seqlens_q", torch.int32, b + 1)
+    if noise.shape != (b, v):
+        raise ValueError("noise must be [batch, vocab]")
+    if (draft_logits is None) != (draft_lse is None):
+        raise ValueError("draft_logits and draft_lse come together")
+    strides = (0, 0, 0, 0)
+    if draft_logits is not None:
+        draft_logits = _rows(draft_logits, "draft_logits", (target_logits.dtype,), 3)
+        if draft_logits.shape != (b, most, v) or draft_lse.shape != (b, most) or draft_lse.dtype != torch.float32:
+            raise ValueError("draft_logits must be [batch, drafts, vocab] and draft_lse fp32 [batch, drafts]")
+        strides = (draft_logits.stride(0), draft_logits.stride(1), draft_lse.stride(0), draft_lse.stride(1))
+    d = target_logits.device
+    tokens = torch.empty((b, most + 1), dtype=torch.int64, device=d)
+    logprobs = torch.empty((b, most + 1), dtype=torch.float32, device=d)
+    accepted = torch.empty(b, dtype=torch.int32, device=d)
+    if b == 0:
+        return tokens, accepted, logprobs
+    lib = N.lib()
+    need = lib.ada_verify_drafts_workspace_size(b, most, v)
+    ws = _workspace(workspace, need, d)
+    st = lib.ada_verify_drafts(
+        target_logits.data_ptr(), N.DT_LOGITS[target_logits.dtype], _ld(target_logits) if n else v, n, v,
+        input_ids.data_ptr(), cu_seqlens_q.data_ptr(), b, most, temperatures.data_ptr(), uniforms.data_ptr(),
+        _ld(uniforms), noise.data_ptr(), _ld(noise), N.ptr(draft_logits), strides[0], strides[1], N.ptr(draft_lse),
+        strides[2], strides[3], tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), need,
+        N.stream_ptr(d))
+    N.check(st, "draft verification kernel")
+    return tokens, accepted, logprobs
+
+
+class Sampler(nn.Module):
+    """Drop-in for adallm.ops.sampler.Sampler: one token per row at its temperature (the reference
+    refuses greedy rows; here a temperature of 0 takes the first maximum)."""
+
+    def forward(self, logits: torch.Tensor, temperatures: torch.Tensor) -> torch.Tensor:
+        noise = torch.empty(logits.shape, dtype=torch.float32, device=logits.device).exponential_(1.0)
+        return sample(logits, temperatures.float(), noise)[0]

@@ -1,0 +1,85 @@
+"""Decode attention for batches that share prompt prefixes, on the FP8 paged cache.
+
+``shared_prefix_decode`` reads the keys and values of a prefix once for all the sequences behind
+it (parallel samples of a prompt, a common system prompt), joins them with each sequence's own
+pages, and takes one or several query rows a sequence (the rows of drafted tokens).  The
+reference has no such form: its decode reads a cached prefix once per sequence
+(adallm/ops/attention.py:359-414)."""
+from __future__ import annotations
+
+import torch
+
+from . import _native as N
+
+
+def shared_prefix_workspace_bytes(total_q: int, num_groups: int, batch: int, num_heads: int, num_kv_heads: int,
+                                  head_dim: int) -> int:
+    return int(N.lib().ada_fp8_shared_prefix_decode_workspace_size(total_q, num_groups, batch, num_heads,
+                                                                   num_kv_heads, head_dim))
+
+
+def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_tables: torch.Tensor,
+                         prefix_lens: torch.Tensor, cu_groups: torch.Tensor | None, block_tables: torch.Tensor,
+                         context_lens: torch.Tensor, scale: float, cu_seqlens_q: torch.Tensor | None = None,
+                         window: int = 0, k_scale: float = 1.0, v_scale: float = 1.0,
+                         out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                         err: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each sequence's newest tokens over its group's prefix and its own keys.
+
+    q [N, Hq, 128] bf16/fp16; k_cache/v_cache [num_pages, page, Hkv, 128] e4m3;
+    prefix_tables int32 [G, pages], prefix_lens int32 [G]: the prefix pages of each group;
+    cu_groups int32 [G + 1]: group g is sequences cu_groups[g]..cu_groups[g+1] (None: one group
+    of all); block_tables int32 [B, pages], context_lens int32 [B]: each sequence's own keys
+    behind the prefix, its new tokens included (store_kvcache runs first);
+    cu_seqlens_q int32 [B + 1]: sequence b's rows of q are its newest tokens (None: one each).
+    Row i of t attends to positions <= prefix + context - t + i, with window W > 0 to the last W
+    of them.  Rows that see no key are zeros.
+    Returns [N, Hq, 128] in q.dtype.  err: optional int32 [1] device word; 0x90 is OR-ed in if a
+    tile wait ran out."""
+    N.require_cuda(q, k_cache, v_cache, prefix_tables, prefix_lens, block_tables, context_lens, cu_groups,
+                   cu_seqlens_q, out, workspace, err, what="shared_prefix_decode")
+    if q.dim() != 3 or k_cache.dim() != 4 or prefix_tables.dim() != 2 or block_tables.dim() != 2:
+        raise ValueError("shared_prefix_decode expects q [N, Hq, D], caches [pages, page, Hkv, D] and 2-D page tables")
+    total_q, hq, d = q.shape
+    pages, page, hkv, dk = k_cache.shape
+    if q.dtype not in N.DT or (out is not None and out.dtype not in N.DT):
+        raise ValueError("q and out must be bf16 or fp16")
+    if dk != d or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride() or k_cache.stride(-1) != 1:
+        raise ValueError("k_cache and v_cache must share a [pages, page, Hkv, D] layout with q's head size")
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError("the shared-prefix decode reads a float8_e4m3fn cache")
+    for t, name in ((prefix_tables, "prefix_tables"), (prefix_lens, "prefix_lens"), (cu_groups, "cu_groups"),
+                    (block_tables, "block_tables"), (context_lens, "context_lens"), (cu_seqlens_q, "cu_seqlens_q")):
+        if t is not None and (t.dtype != torch.int32 or (t.numel() > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{name} must be int32 with unit stride")
+    groups, batch = prefix_lens.numel(), context_lens.numel()
+    if prefix_tables.shape[0] != groups or block_tables.shape[0] != batch:
+        raise ValueError("page tables must have one row per prefix and per sequence")
+    if (cu_groups is None and groups > 1) or (cu_groups is not None and cu_groups.numel() != groups + 1):
+        raise ValueError("cu_groups must hold the first sequence of each group and the end (None for one group)")
+    if cu_seqlens_q.numel() != batch + 1 if cu_seqlens_q is not None else total_q != batch:
+        raise ValueError("cu_seqlens_q must have batch + 1 entries (None for one row per sequence)")
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((total_q, hq, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.stride(-1) != 1:
+        raise ValueError("out must have q's shape and unit stride in the head dimension")
+    if total_q == 0:
+        return out
+    if batch == 0:
+        return out.zero_()
+    lib = N.lib()
+    need = lib.ada_fp8_shared_prefix_decode_workspace_size(total_q, groups, batch, hq, hkv, d)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    st = lib.ada_fp8_shared_prefix_decode(
+        q.data_ptr(), N.DT[q.dtype], q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), pages, prefix_tables.data_ptr(),
+        prefix_tables.stride(0), prefix_tables.shape[1], prefix_lens.data_ptr(), N.ptr(cu_groups), groups,
+        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
+        N.ptr(cu_seqlens_q), batch, total_q, hq, hkv, d, page, float(scale), float(k_scale), float(v_scale),
+        int(window), out.data_ptr(), N.DT[out.dtype], out.stride(0), out.stride(1), workspace.data_ptr(), need,
+        N.ptr(err), N.stream_ptr(q.device))
+    N.check(st, "shared-prefix decode attention")
+    return out

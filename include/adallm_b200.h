@@ -8,7 +8,8 @@
  *   - Pointers are device pointers unless stated; sizes and strides are in
  *     elements of the pointed-to type.  `stream` is a cudaStream_t passed as
  *     void* so this header needs no CUDA include.
- *   - dtype codes: ADA_DT_BF16 = 0, ADA_DT_F16 = 1.
+ *   - dtype codes: ADA_DT_BF16 = 0, ADA_DT_F16 = 1; the sampling entries also take
+ *     ADA_DT_F32 = 2.
  *   - No entry point allocates or frees memory: outputs and workspaces are
  *     owned by the caller (the reference's ops allocate with torch.empty,
  *     adallm/ops/nvfp4_gemm.py:479, adallm/ops/attention.py:367; the Python
@@ -45,7 +46,7 @@ enum {
   ADA_ERR_CUDA = 7          /* other CUDA runtime / driver failure           */
 };
 
-enum { ADA_DT_BF16 = 0, ADA_DT_F16 = 1 };
+enum { ADA_DT_BF16 = 0, ADA_DT_F16 = 1, ADA_DT_F32 = 2 };
 
 /* Human-readable text for a status code (static storage). */
 ADA_API const char* ada_status_string(int status);
@@ -565,6 +566,89 @@ ADA_API int ada_argmax(const void* logits, int64_t ld, int64_t rows, int64_t col
  * device race. */
 ADA_API int ada_argmax_noalloc(const void* logits, int64_t ld, int64_t rows, int64_t cols, int dtype,
                                int64_t* out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Decode attention for batches that share prompt prefixes (FP8 paged cache)
+ * No counterpart in the reference, whose decode reads a cached prefix once per sequence
+ * (adallm/ops/attention.py:359-414); for parallel samples of a prompt, a common system prompt,
+ * and the rows of drafted tokens.
+ *
+ * Sequences cu_groups[g] .. cu_groups[g+1] - 1 share the first prefix_lens[g] keys of the pages
+ * prefix_tables[g]; sequence b has context_lens[b] keys of its own in block_tables[b], starting
+ * at row 0 of its first page, its new tokens included (store them first).  Rows cu_seqlens_q[b]
+ * .. cu_seqlens_q[b+1] - 1 of q are its t_b newest tokens: query i stands at position
+ * pos = prefix_len + context_len - t_b + i of the joined keys and sees keys j <= pos, with
+ * window W > 0 only the last W of them (the meaning of the decode entry's window).
+ *
+ * q, out   [total_q, num_heads, head_dim], token and head strides given, unit stride in D
+ * k_cache, v_cache, num_pages, page_size, k_scale, v_scale: as the decode entry; table entries
+ *          outside [0, num_pages) are holes
+ * prefix_tables int32 [num_groups, >= max_prefix_pages] (row stride pt_stride), block_tables
+ *          int32 [batch, >= max_pages] (bt_stride); lengths past a table's reach are cut off
+ * cu_groups int32 [num_groups + 1] ascending; NULL: one group of all sequences.  A sequence in
+ *          no group (num_groups 0, or outside [cu_groups[0], cu_groups[num_groups])) has no prefix
+ * cu_seqlens_q int32 [batch + 1] ascending; NULL: one row per sequence (total_q == batch).  Rows
+ *          of no sequence, and rows that see no key, are written as zeros
+ * err      optional uint32 word: 0x90 is OR-ed in if a tile wait ran out (~2 s)
+ * Implemented: head_dim 128, num_heads / num_kv_heads <= 128, page_size % 16 == 0,
+ * scale * k_scale > 0.  workspace: ada_fp8_shared_prefix_decode_workspace_size bytes, 256-byte
+ * aligned, no initial value; calls that share one must be ordered.
+ * ---------------------------------------------------------------------- */
+ADA_API size_t ada_fp8_shared_prefix_decode_workspace_size(int32_t total_q, int32_t num_groups, int32_t batch,
+                                                           int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+ADA_API int ada_fp8_shared_prefix_decode(
+    const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* k_cache, const uint8_t* v_cache,
+    int64_t kv_stride_page, int64_t kv_stride_tok, int64_t kv_stride_head, int64_t num_pages,
+    const int32_t* prefix_tables, int64_t pt_stride, int32_t max_prefix_pages, const int32_t* prefix_lens,
+    const int32_t* cu_groups, int32_t num_groups, const int32_t* block_tables, int64_t bt_stride, int32_t max_pages,
+    const int32_t* context_lens, const int32_t* cu_seqlens_q, int32_t batch, int32_t total_q, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, float k_scale, float v_scale,
+    int32_t window, void* out, int out_dtype, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+    size_t workspace_bytes, unsigned int* err, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Sampling at a temperature with given random numbers
+ * Replaces Sampler.forward (adallm/ops/sampler.py:10-15): softmax(logits / T) / Exp(1), argmax.
+ * logits [rows, vocab] (bf16 / f16 / f32, row stride ld), temperatures fp32 [rows], noise fp32
+ * [rows, vocab] (row stride ld_noise): independent Exp(1) draws, read as max(e, 1e-10).
+ * z = logits / T;  lse[r] = ln sum exp(z);  tokens[r] = the lowest index of the largest
+ * exp(z - lse) / noise;  logprobs[r] = z[token] - lse.  T <= 1e-10: greedy, tokens[r] = the first
+ * maximum, lse and logprobs at temperature 1.  -inf and NaN logits have probability 0, +inf is
+ * read as the largest float; a row with no possible token gives token -1, logprob 0, lse -inf.
+ * logprobs, lse: either may be NULL.  workspace: ada_sample_workspace_size bytes, 256-byte
+ * aligned, no initial value.
+ * ---------------------------------------------------------------------- */
+ADA_API size_t ada_sample_workspace_size(int64_t rows, int64_t vocab);
+ADA_API int ada_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab,
+                       const float* temperatures, const float* noise, int64_t ld_noise, int64_t* tokens,
+                       float* logprobs, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Verification of drafted tokens against the target's probabilities (no reference counterpart)
+ * target [total_q, vocab] (dtype, row stride ld): the target's logits for the rows of input_ids
+ * int64 [total_q]; sequence b owns rows cu_seqlens_q[b] .. cu_seqlens_q[b+1] - 1, the first its
+ * last known token and the others its d_b drafts (at most max_drafts are looked at; an empty
+ * sequence gets no token).  draft_logits (dtype, element (b, i, v) at b * draft_stride_b +
+ * i * draft_stride_d + v) and draft_lse (fp32, strides lse_stride_*): the logits draft i + 1 was
+ * drawn from and their log-normaliser at the sequence's temperature (ada_sample's lse); both
+ * NULL: drafts without a distribution, taken as certain.  uniforms [batch, max_drafts] in [0, 1)
+ * (row stride ld_u), noise [batch, vocab] Exp(1) (ld_noise), temperatures [batch].
+ * Draft x after row i is accepted while uniform * q(x) < p_i(x); the first refused position draws
+ * from max(p_i - q, 0) (p_i if that is zero everywhere), the row after d acceptances from p_d.
+ * Greedy sequences (T <= 1e-10) accept x if it is row i's first maximum, and end with the first
+ * maximum.  tokens int64 and logprobs fp32 [batch, max_drafts + 1]: the accepted drafts and the
+ * drawn token with their log-probabilities under p, then -1 and 0; accepted int32 [batch].
+ * Logits are read as in ada_sample; where no token is possible the drawn one is -1.
+ * workspace: ada_verify_drafts_workspace_size bytes, 256-byte aligned, no initial value.
+ * ---------------------------------------------------------------------- */
+ADA_API size_t ada_verify_drafts_workspace_size(int32_t batch, int32_t max_drafts, int64_t vocab);
+ADA_API int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t total_q, int64_t vocab,
+                              const int64_t* input_ids, const int32_t* cu_seqlens_q, int32_t batch,
+                              int32_t max_drafts, const float* temperatures, const float* uniforms, int64_t ld_u,
+                              const float* noise, int64_t ld_noise, const void* draft_logits, int64_t draft_stride_b,
+                              int64_t draft_stride_d, const float* draft_lse, int64_t lse_stride_b,
+                              int64_t lse_stride_d, int64_t* tokens, int32_t* accepted, float* logprobs,
+                              void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
