@@ -30,21 +30,15 @@ def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Ten
     return t.contiguous()
 
 
-def _workspace(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor:
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    return workspace
-
-
-def sample(logits: torch.Tensor, temperatures: torch.Tensor, noise: torch.Tensor,
-           workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def sample(logits: torch.Tensor, temperatures: torch.Tensor,
+           noise: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """One token per row of logits [R, V] (bf16/fp16/fp32; rows may be strided).
 
     temperatures fp32 [R] (<= 1e-10: greedy); noise fp32 [R, V]: Exp(1) draws.
     Returns (tokens int64 [R], logprobs fp32 [R], lse fp32 [R]): the draw, its log-probability
     and the row's log-normaliser, both at the row's temperature (1 where greedy).  A row whose
     logits are all -inf gives -1, 0 and -inf."""
-    N.require_cuda(logits, temperatures, noise, workspace, what="sample")
+    N.require_cuda(logits, temperatures, noise, what="sample")
     logits = _rows(logits, "logits", N.DT_LOGITS)
     noise = _rows(noise, "noise", (torch.float32,))
     r, v = logits.shape
@@ -57,20 +51,17 @@ def sample(logits: torch.Tensor, temperatures: torch.Tensor, noise: torch.Tensor
     lse = torch.empty(r, dtype=torch.float32, device=d)
     if r == 0:
         return tokens, logprobs, lse
-    lib = N.lib()
-    need = lib.ada_sample_workspace_size(r, v)
-    ws = _workspace(workspace, need, d)
-    st = lib.ada_sample(logits.data_ptr(), N.DT_LOGITS[logits.dtype], _ld(logits), r, v, temperatures.data_ptr(),
-                        noise.data_ptr(), _ld(noise), tokens.data_ptr(), logprobs.data_ptr(), lse.data_ptr(),
-                        ws.data_ptr(), need, N.stream_ptr(d))
+    st = N.lib().ada_sample(logits.data_ptr(), N.DT_LOGITS[logits.dtype], _ld(logits), r, v, temperatures.data_ptr(),
+                            noise.data_ptr(), _ld(noise), tokens.data_ptr(), logprobs.data_ptr(), lse.data_ptr(),
+                            N.stream_ptr(d))
     N.check(st, "sampling kernel")
     return tokens, logprobs, lse
 
 
 def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqlens_q: torch.Tensor,
                   temperatures: torch.Tensor, uniforms: torch.Tensor, noise: torch.Tensor,
-                  draft_logits: torch.Tensor | None = None, draft_lse: torch.Tensor | None = None,
-                  workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                  draft_logits: torch.Tensor | None = None, draft_lse: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Accepts each sequence's drafted tokens up to the first refusal and draws the token after them.
 
     target_logits [N, V] (bf16/fp16/fp32): the target's logits of the rows input_ids int64 [N];
@@ -82,7 +73,7 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     Returns (tokens int64 [B, D + 1], accepted int32 [B], logprobs fp32 [B, D + 1]): the accepted
     drafts and the drawn token with their log-probabilities under the target, then -1 and 0."""
     N.require_cuda(target_logits, input_ids, cu_seqlens_q, temperatures, uniforms, noise, draft_logits, draft_lse,
-                   workspace, what="verify_drafts")
+                   what="verify_drafts")
     target_logits = _rows(target_logits, "target_logits", N.DT_LOGITS)
     noise = _rows(noise, "noise", (torch.float32,))
     uniforms = _rows(uniforms, "uniforms", (torch.float32,))
@@ -106,15 +97,11 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     accepted = torch.empty(b, dtype=torch.int32, device=d)
     if b == 0:
         return tokens, accepted, logprobs
-    lib = N.lib()
-    need = lib.ada_verify_drafts_workspace_size(b, most, v)
-    ws = _workspace(workspace, need, d)
-    st = lib.ada_verify_drafts(
+    st = N.lib().ada_verify_drafts(
         target_logits.data_ptr(), N.DT_LOGITS[target_logits.dtype], _ld(target_logits) if n else v, n, v,
         input_ids.data_ptr(), cu_seqlens_q.data_ptr(), b, most, temperatures.data_ptr(), uniforms.data_ptr(),
         _ld(uniforms), noise.data_ptr(), _ld(noise), N.ptr(draft_logits), strides[0], strides[1], N.ptr(draft_lse),
-        strides[2], strides[3], tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), need,
-        N.stream_ptr(d))
+        strides[2], strides[3], tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), N.stream_ptr(d))
     N.check(st, "draft verification kernel")
     return tokens, accepted, logprobs
 

@@ -615,13 +615,11 @@ ADA_API int ada_fp8_shared_prefix_decode(
  * exp(z - lse) / noise;  logprobs[r] = z[token] - lse.  T <= 1e-10: greedy, tokens[r] = the first
  * maximum, lse and logprobs at temperature 1.  -inf and NaN logits have probability 0, +inf is
  * read as the largest float; a row with no possible token gives token -1, logprob 0, lse -inf.
- * logprobs, lse: either may be NULL.  workspace: ada_sample_workspace_size bytes, 256-byte
- * aligned, no initial value.
+ * logprobs, lse: either may be NULL.  One launch, no workspace.
  * ---------------------------------------------------------------------- */
-ADA_API size_t ada_sample_workspace_size(int64_t rows, int64_t vocab);
 ADA_API int ada_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab,
                        const float* temperatures, const float* noise, int64_t ld_noise, int64_t* tokens,
-                       float* logprobs, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+                       float* logprobs, float* lse, void* stream);
 
 /* ------------------------------------------------------------------------
  * Verification of drafted tokens against the target's probabilities (no reference counterpart)
@@ -639,16 +637,15 @@ ADA_API int ada_sample(const void* logits, int dtype, int64_t ld, int64_t rows, 
  * maximum.  tokens int64 and logprobs fp32 [batch, max_drafts + 1]: the accepted drafts and the
  * drawn token with their log-probabilities under p, then -1 and 0; accepted int32 [batch].
  * Logits are read as in ada_sample; where no token is possible the drawn one is -1.
- * workspace: ada_verify_drafts_workspace_size bytes, 256-byte aligned, no initial value.
+ * One launch, no workspace.
  * ---------------------------------------------------------------------- */
-ADA_API size_t ada_verify_drafts_workspace_size(int32_t batch, int32_t max_drafts, int64_t vocab);
 ADA_API int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t total_q, int64_t vocab,
                               const int64_t* input_ids, const int32_t* cu_seqlens_q, int32_t batch,
                               int32_t max_drafts, const float* temperatures, const float* uniforms, int64_t ld_u,
                               const float* noise, int64_t ld_noise, const void* draft_logits, int64_t draft_stride_b,
                               int64_t draft_stride_d, const float* draft_lse, int64_t lse_stride_b,
                               int64_t lse_stride_d, int64_t* tokens, int32_t* accepted, float* logprobs,
-                              void* workspace, size_t workspace_bytes, void* stream);
+                              void* stream);
 
 #ifdef __cplusplus
 }

@@ -54,48 +54,39 @@ def test_shared_prefix_argument_errors(lib):
 
 
 def test_sample_argument_errors(lib):
-    need = lib.ada_sample_workspace_size(4, 1000)
-    assert need > 0 and lib.ada_sample_workspace_size(0, 1000) == 0
-
     def call(**kw):
         a = dict(x=P, dtype=0, ld=1000, rows=4, vocab=1000, temps=P, noise=P, ld_noise=1000, tokens=P, lp=P, lse=P,
-                 ws=P, ws_bytes=need, stream=None)
+                 stream=None)
         a.update(kw)
         return lib.ada_sample(*a.values())
 
     assert call(rows=0) == 0
-    for name in ("x", "temps", "noise", "tokens", "ws"):
+    for name in ("x", "temps", "noise", "tokens"):
         assert call(**{name: None}) == N.ADA_ERR_INVALID_ARG, name
     assert call(vocab=0) == N.ADA_ERR_INVALID_ARG and call(rows=-1) == N.ADA_ERR_INVALID_ARG
     assert call(ld=999) == N.ADA_ERR_INVALID_ARG and call(ld_noise=999) == N.ADA_ERR_INVALID_ARG
     assert call(dtype=3) == N.ADA_ERR_INVALID_ARG
-    assert call(rows=(1 << 20) + 1, ws_bytes=1 << 40) == N.ADA_ERR_UNSUPPORTED
+    assert call(rows=(1 << 20) + 1) == N.ADA_ERR_UNSUPPORTED
     assert call(x=P + 1) == N.ADA_ERR_ALIGNMENT and call(x=P + 2, dtype=2) == N.ADA_ERR_ALIGNMENT
     assert call(noise=P + 2) == N.ADA_ERR_ALIGNMENT and call(tokens=P + 4) == N.ADA_ERR_ALIGNMENT
-    assert call(ws=P + 64) == N.ADA_ERR_ALIGNMENT
-    assert call(ws_bytes=need - 1) == N.ADA_ERR_WORKSPACE
 
 
 def test_verify_argument_errors(lib):
-    need = lib.ada_verify_drafts_workspace_size(4, 3, 1000)
-    assert need > 0 and lib.ada_verify_drafts_workspace_size(0, 3, 1000) == 0
-
     def call(**kw):
         a = dict(x=P, dtype=0, ld=1000, total=10, vocab=1000, ids=P, cu=P, batch=4, most=3, temps=P, u=P, ld_u=3,
                  noise=P, ld_noise=1000, draft=P, d_sb=3000, d_sd=1000, lse=P, l_sb=3, l_sd=1, tokens=P, acc=P, lp=P,
-                 ws=P, ws_bytes=need, stream=None)
+                 stream=None)
         a.update(kw)
         return lib.ada_verify_drafts(*a.values())
 
     assert call(batch=0) == 0
-    for name in ("x", "ids", "cu", "temps", "u", "noise", "tokens", "acc", "lp", "ws"):
+    for name in ("x", "ids", "cu", "temps", "u", "noise", "tokens", "acc", "lp"):
         assert call(**{name: None}) == N.ADA_ERR_INVALID_ARG, name
     assert call(draft=None) == N.ADA_ERR_INVALID_ARG and call(lse=None) == N.ADA_ERR_INVALID_ARG
     assert call(d_sd=-1) == N.ADA_ERR_INVALID_ARG
     assert call(ld_u=2) == N.ADA_ERR_INVALID_ARG and call(dtype=4) == N.ADA_ERR_INVALID_ARG
-    assert call(most=1025, ld_u=1025, ws_bytes=1 << 40) == N.ADA_ERR_UNSUPPORTED
+    assert call(most=1025, ld_u=1025) == N.ADA_ERR_UNSUPPORTED
     assert call(draft=P + 1) == N.ADA_ERR_ALIGNMENT and call(ids=P + 4) == N.ADA_ERR_ALIGNMENT
-    assert call(ws_bytes=need - 1) == N.ADA_ERR_WORKSPACE
 
 
 def test_python_layer_needs_cuda_tensors():
