@@ -76,8 +76,9 @@ _SIGS = {
                                            I32, P, P, I32, I32, I32, I32, I32, I32, F32, F32, F32, I32, P, INT, I64,
                                            I64, P, SZ, P, P]),
     "ada_sample": (INT, [P, INT, I64, I64, I64, P, P, I64, P, P, P, P]),
+    "ada_verify_drafts_workspace_size": (SZ, [I32, I64, INT]),
     "ada_verify_drafts": (INT, [P, INT, I64, I32, I64, P, P, I32, I32, P, P, I64, P, I64, P, I64, I64, P, I64, I64, P,
-                                P, P, P]),
+                                P, P, P, SZ, P]),
     "ada_nvfp4_sf_bytes": (SZ, [I64, I64]),
     "ada_nvfp4_prepack_scales": (INT, [P, INT, I64, I64, I64, P, P]),
     "ada_nvfp4_linear_workspace_size": (SZ, [I64, I64, I64, INT]),
@@ -196,7 +197,9 @@ def raise_on_error_word(code: int, what: str) -> None:
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle (the raw look-up: building a Stream object costs 2 us a call)."""
+    index = device.index if device is not None else None
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -17,12 +17,12 @@
 // target's own.  Greedy sequences accept a draft that is the target's first maximum and end with
 // the first maximum.
 //
-// Bound: HBM (a logit costs 2 or 4 bytes and about ten instructions).  One thread-block cluster
-// takes one row (or one sequence's rows), each CTA a contiguous share of the vocabulary, so a call is
-// one launch without a workspace: the CTAs exchange their partial results through distributed
-// shared memory.  A thread keeps a running maximum m of its raw logits and its sum of
-// 2^((x - m) c), c = log2(e) / T; x - m is exact or nearly so where the weight matters, so the
-// statistics do not pay for the size of x.
+// Bound: HBM (a logit costs 2 or 4 bytes and about ten instructions).  A row is read once: a warp
+// keeps a running maximum m of its raw logits and each lane its sum of 2^((x - m) c),
+// c = log2(e) / T; x - m is exact or nearly so where the weight matters, so the statistics do not pay
+// for the size of x.  Sampling takes one thread-block cluster per row, each CTA a share of the
+// vocabulary; the CTAs meet in distributed shared memory, so a call is one launch without a
+// workspace.
 #include <float.h>
 
 #include <type_traits>
@@ -119,19 +119,15 @@ struct Scale {
   }
 };
 
-// Maximum and sum of the logits a thread (warp, CTA, cluster) has seen: s = sum 2^((x - m) c).
+// Maximum and sum of a set of logits: s = sum 2^((x - m) c); at = the index of the first maximum
+// (greedy rows).
 struct Stats {
   float m, s;
-  int at;  // a thread's packet that first held the maximum, then the index of the first maximum
-  __device__ __forceinline__ void init() {
-    m = -FLT_MAX;
-    s = 0.f;
-    at = NONE;
-  }
+  int at;
   __device__ __forceinline__ void merge(float m2, float s2, int at2, const Scale& sc) {
     const float top = fmaxf(m, m2);
     at = m == m2 ? min(at, at2) : (m > m2 ? at : at2);
-    s = s * sc.weight(fmaxf(m - top, sc.least)) + s2 * sc.weight(fmaxf(m2 - top, sc.least));
+    s = s * sc.weight(sc.diff(m, top)) + s2 * sc.weight(sc.diff(m2, top));
     m = top;
   }
   __device__ __forceinline__ void merge_warp(const Scale& sc) {
@@ -142,42 +138,81 @@ struct Stats {
       merge(m2, s2, at2, sc);
     }
   }
-  __device__ __forceinline__ bool any() const { return s > 0.f; }
 };
-// Fold packet k (values v) in; returns whether the maximum moved.
-template <int N>
-__device__ __forceinline__ bool fold(Stats& st, const float* v, int k, const Scale& sc) {
-  float top = v[0];
+__device__ __forceinline__ Stats no_stats() { return Stats{-FLT_MAX, 0.f, NONE}; }
+
+__device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
-  const bool moved = top > st.m || (st.at == NONE && top == -FLT_MAX);
-  if (moved) {
-    top = fminf(top, FLT_MAX);
-    st.s *= sc.weight(fmaxf(st.m - top, sc.least));
-    st.m = top;
-    st.at = k;
-  }
-  float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    s0 += sc.weight(sc.diff(v[i], st.m));
-    s1 += sc.weight(sc.diff(v[i + 1], st.m));
-  }
-  st.s += s0 + s1;
-  return moved;
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
-// A thread's packet of the first maximum -> the index of that maximum.
-template <typename T, bool VEC>
-__device__ __forceinline__ int first_maximum(const T* x, const Stats& st, int n) {
-  if (st.at == NONE) return NONE;
-  float v[pack_n<T>()];
-  unpack<T>(load_pack<T, VEC>(x, st.at, n), v);
-  int at = NONE;
+
+// A warp's statistics while it reads a row.  The maximum is the warp's (it moves a handful of times
+// a row, found by one vote a packet), so a logit costs a maximum, a difference, a clamp (which
+// also takes -inf and NaN to weight 0), a product, an ex2 and an add.
+struct Fold {
+  float m, s;    // warp maximum; this lane's sum against it
+  float top;     // this lane's own maximum and the packet that first held it (greedy rows)
+  int top_pack;
+  __device__ __forceinline__ void init() {
+    m = -FLT_MAX;
+    s = 0.f;
+    top = -INFINITY;
+    top_pack = NONE;
+  }
+  // Fold packet k in; every lane of the warp calls.  w: the packet's weights against m.  Returns
+  // whether m moved.
+  template <int N>
+  __device__ __forceinline__ bool add(float* v, int k, const Scale& sc, float* w) {
+    float most = v[0];
 #pragma unroll
-  for (int i = pack_n<T>() - 1; i >= 0; --i)
-    if (v[i] >= st.m) at = pack_index<T, VEC>(st.at, i);
-  return at;
-}
+    for (int i = 1; i < N; ++i) most = fmaxf(most, v[i]);
+    if (most > top) {
+      top = most;
+      top_pack = k;
+    }
+    const bool moved = __any_sync(0xffffffffu, most > m);
+    if (moved) {
+      float to = warp_max(most);
+      if (to > FLT_MAX) {  // +inf among them: read as the largest float (such a packet always gets here)
+        to = FLT_MAX;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] > FLT_MAX ? FLT_MAX : v[i];
+      }
+      s *= sc.weight(sc.diff(m, to));
+      m = to;
+    }
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      w[i] = sc.weight(fmaxf(v[i] - m, sc.least));
+      w[i + 1] = sc.weight(fmaxf(v[i + 1] - m, sc.least));
+      s0 += w[i];
+      s1 += w[i + 1];
+    }
+    s += s0 + s1;
+    return moved;
+  }
+  // The warp's statistics, in every lane.
+  template <typename T, bool VEC>
+  __device__ __forceinline__ Stats finish(const T* x, int n, const Scale& sc) const {
+    Stats st{m, s, NONE};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+    if (sc.greedy) {
+      if (top_pack != NONE && top >= m) {  // (top may be +inf, m not)
+        float v[pack_n<T>()];
+        unpack<T>(load_pack<T, VEC>(x, top_pack, n), v);
+#pragma unroll
+        for (int i = pack_n<T>() - 1; i >= 0; --i)
+          if (v[i] >= m) st.at = pack_index<T, VEC>(top_pack, i);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) st.at = min(st.at, __shfl_xor_sync(0xffffffffu, st.at, o));
+    }
+    return st;
+  }
+};
 
 // The winner of a race: the largest w / e, lowest index on ties.  Compared crosswise, so no
 // division: w1 / e1 > w2 / e2 as w1 e2 > w2 e1.
@@ -206,7 +241,20 @@ struct Best {
     }
   }
 };
+// How far a score that filters candidates is lowered: above the roundings of the weights it is made of.
+constexpr float SLACK = 1.f - 1.f / 16384.f;
+__device__ __forceinline__ unsigned long long pack2(float a, float b) {
+  return ((unsigned long long)__float_as_uint(b) << 32) | __float_as_uint(a);
+}
+__device__ __forceinline__ float2 unpack2(unsigned long long v) {
+  return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
+}
 __device__ __forceinline__ float exponential(float e) { return fmaxf(e, 1e-10f); }
+
+// Probability of a draft's logit given its row's log-normaliser (NaN: 0, +inf: the largest float).
+__device__ __forceinline__ float draft_prob(float x, const Scale& sc, float lse) {
+  return x == x ? expf(fminf(x, FLT_MAX) / sc.t - lse) : 0.f;
+}
 
 // This CTA's packets [k0, k1) of a row of n elements, in shares of whole warps.
 template <typename T> __device__ __forceinline__ void share(int n, int rank, int ranks, int& k0, int& k1) {
@@ -229,12 +277,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     sample_kernel(const T* __restrict__ logits, int64_t ld, int n, const float* __restrict__ temps,
                   const float* __restrict__ noise, int64_t ld_noise, int64_t* tokens, float* logprobs, float* lse) {
   constexpr int N = pack_n<T>(), WARPS = NT / 32, U = 2;
-  __shared__ float wm[WARPS], wsum[WARPS], we[WARPS], wx[WARPS];
-  __shared__ int wat[WARPS], wfirst[WARPS];
-  __shared__ SampleWord words[MAX_CLUSTER];
+  __shared__ SampleWord mine[WARPS], words[MAX_CLUSTER];
+  __shared__ unsigned long long bound;  // (maximum, score): see below
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cl::ctarank(), ranks = (int)cl::nctarank();
   cl::cluster_arrive_relaxed();
+  if (threadIdx.x == 0) bound = pack2(-FLT_MAX, 0.f);
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
   const int64_t r = blockIdx.x / ranks;
@@ -244,98 +293,77 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   int k0, k1;
   share<T>(n, rank, ranks, k0, k1);
 
-  Stats st;
-  st.init();
-  float bx = -INFINITY, be = 1.f, bw = 0.f;  // the thread's candidate: logit, noise, weight against st.m
+  // The race.  A lane keeps its best (logit, noise), with its weight against the warp's maximum;
+  // the CTA shares a score that some lane has reached, with the maximum that it is against, so only
+  // a few packets a row hold anything that could still win and are looked at element by element.
+  Fold f;
+  f.init();
+  float bx = -INFINITY, be = 1.f, bw = 0.f;
   int bat = NONE;
-  for (int base = k0 + warp * 32; base < k1; base += NT * U) {  // warp-uniform
-    uint4 raw[U];
-    float ns[U][N];
+  // U packets a lane are in flight: each is asked for again as soon as it has been used
+  uint4 raw[U];
+  float ns[U][N];
+  auto load = [&](int u, int base) {
+    if (base >= k1) return;
+    raw[u] = load_pack<T, VEC>(x, base + lane, n);
+    if (!sc.greedy) load_noise<T, VEC>(e, base + lane, n, ns[u]);
+  };
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = base + u * NT + lane;
-      if (base + u * NT < k1) {
-        raw[u] = load_pack<T, VEC>(x, k, n);
-        if (!sc.greedy) load_noise<T, VEC>(e, k, n, ns[u]);
-      }
-    }
+  for (int u = 0; u < U; ++u) load(u, k0 + warp * 32 + u * NT);
+  for (int base = k0 + warp * 32; base < k1; base += NT * U) {  // warp-uniform
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (base + u * NT >= k1) break;
       const int k = base + u * NT + lane;
-      float v[N];
+      float v[N], w[N];
       unpack<T>(raw[u], v);
-      if (sc.greedy) {
-        fold<N>(st, v, k, sc);
-        continue;
-      }
-      float top = v[0];
+      const bool moved = f.add<N>(v, k, sc, w);
+      if (!sc.greedy) {
+        if (moved) bw = sc.weight(sc.diff(bx, f.m));
+        const float2 known = unpack2(*const_cast<volatile unsigned long long*>(&bound));
+        const float score = known.y * sc.weight(known.x - f.m);  // against f.m
+        const float least = score * SLACK;
+        bool hit = false;
 #pragma unroll
-      for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
-      if (top > st.m || (st.at == NONE && top == -FLT_MAX)) {
-        top = fminf(top, FLT_MAX);
-        st.s *= sc.weight(fmaxf(st.m - top, sc.least));
-        st.m = top;
-        st.at = k;
-        bw = sc.weight_exact(sc.diff(bx, top));
-      }
+        for (int i = 0; i < N; ++i) hit |= !(w[i] <= least * ns[u][i]);
+        if (__any_sync(0xffffffffu, hit)) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float w = sc.weight_exact(sc.diff(v[i], st.m)), ei = exponential(ns[u][i]);
-        st.s += w;
-        if (w * be > bw * ei) {
-          bw = w;
-          bx = v[i];
-          be = ei;
-          bat = pack_index<T, VEC>(k, i);
+          for (int i = 0; i < N; ++i) {
+            const float ei = exponential(ns[u][i]);
+            if (w[i] * be > bw * ei) {
+              bw = w[i];
+              bx = v[i];
+              be = ei;
+              bat = pack_index<T, VEC>(k, i);
+            }
+          }
+          const float reached = warp_max(bw / be);
+          if (lane == 0 && reached > score) *const_cast<volatile unsigned long long*>(&bound) = pack2(f.m, reached);
         }
       }
+      load(u, base + (u + U) * NT);
     }
   }
-  int first = sc.greedy ? first_maximum<T, VEC>(x, st, n) : NONE;
-  // the CTA's maximum, then everything against it
-  st.at = first;
-  st.merge_warp(sc);
-  Best b;
-  b.w = bat != NONE ? sc.weight_exact(sc.diff(bx, st.m)) : 0.f;
-  b.e = be;
-  b.at = bat;
-  b.merge_warp();
-  // the winning lane's logit travels with it
-  const unsigned who = __ballot_sync(0xffffffffu, bat == b.at);
-  const float x_best = __shfl_sync(0xffffffffu, bx, __ffs(who) - 1);
-  if (lane == 0) {
-    wm[warp] = st.m;
-    wsum[warp] = st.s;
-    wfirst[warp] = st.at;
-    wx[warp] = x_best;
-    we[warp] = b.e;
-    wat[warp] = b.at;
+  // entries (statistics, candidate) of a warp's lanes -> their merge, in every lane
+  auto reduce = [&](SampleWord w) {
+    Stats a{w.m, w.s, w.first};
+    a.merge_warp(sc);
+    Best c{w.at != NONE ? sc.weight(sc.diff(w.x, a.m)) : 0.f, w.e, w.at};
+    c.merge_warp();
+    const unsigned hit = __ballot_sync(0xffffffffu, w.at == c.at);
+    return SampleWord{a.m, a.s, __shfl_sync(0xffffffffu, w.x, __ffs(hit) - 1), c.e, c.at, a.at, {0, 0}};
+  };
+  {
+    const Stats st = f.finish<T, VEC>(x, n, sc);
+    SampleWord w{st.m, lane == 0 ? st.s : 0.f, bx, be, bat, st.at, {0, 0}};
+    w = reduce(w);
+    if (lane == 0) mine[warp] = w;
   }
   __syncthreads();
   cl::cluster_wait();  // every CTA of the cluster runs
-  auto reduce = [&](int count, auto get) {  // lanes hold entries; result in every lane
-    SampleWord w = get(lane < count ? lane : 0);
-    if (lane >= count) {
-      w.s = 0.f;
-      w.m = -FLT_MAX;
-      w.at = w.first = NONE;
-    }
-    Stats a{w.m, w.s, w.first};
-    a.merge_warp(sc);
-    Best c{w.at != NONE ? sc.weight_exact(sc.diff(w.x, a.m)) : 0.f, w.e, w.at};
-    c.merge_warp();
-    const unsigned hit = __ballot_sync(0xffffffffu, w.at == c.at);
-    w.x = __shfl_sync(0xffffffffu, w.x, __ffs(hit) - 1);
-    w.m = a.m;
-    w.s = a.s;
-    w.first = a.at;
-    w.e = c.e;
-    w.at = c.at;
-    return w;
-  };
+  const SampleWord nothing{-FLT_MAX, 0.f, -INFINITY, 1.f, NONE, NONE, {0, 0}};
   if (warp == 0) {
-    const SampleWord w = reduce(WARPS, [&](int i) { return SampleWord{wm[i], wsum[i], wx[i], we[i], wat[i], wfirst[i], {0, 0}}; });
+    const SampleWord w = reduce(lane < WARPS ? mine[lane] : nothing);
     if (lane == 0) {
       const uint32_t to = cl::mapa(&words[rank], 0);
       cl::st_cluster_v4(to, w.m, w.s, w.x, w.e);
@@ -344,25 +372,27 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   }
   cl::cluster_sync();
   if (rank != 0 || warp != 0) return;
-  const SampleWord w = reduce(ranks, [&](int i) { return words[i]; });
+  const SampleWord w = reduce(lane < ranks ? words[lane] : nothing);
   if (lane != 0) return;
-  const bool any = w.s > 0.f && (sc.greedy || w.at != NONE);
-  const float ln_s = logf(w.s);
-  const float xt = sc.greedy ? w.m : w.x;
   const int at = sc.greedy ? w.first : w.at;
-  tokens[r] = any ? at : -1;
-  if (logprobs) logprobs[r] = any ? sc.diff(xt, w.m) / sc.t - ln_s : 0.f;
+  const bool any = w.s > 0.f;
+  const float ln_s = logf(w.s);
+  tokens[r] = any && at != NONE ? at : -1;
+  if (logprobs) logprobs[r] = any ? sc.diff(sc.greedy ? w.m : w.x, w.m) / sc.t - ln_s : 0.f;
   if (lse) lse[r] = any ? w.m / sc.t + ln_s : -INFINITY;
 }
 
-// ---- verification: one cluster per sequence -----------------------------------------------------
+// ---- verification ---------------------------------------------------------------------------------
+// Two kernels: the statistics of every target row (any CTA takes any share of any row, so ragged
+// numbers of drafts cost no balance), then one cluster per sequence that judges its drafts and
+// draws from one row, which is in L2 by then.
 struct VerifyParams {
   const void* target;
   int64_t ld;
   int n;  // vocabulary
   const int64_t* ids;
   const int32_t* cu_q;
-  int32_t total_q, max_drafts;
+  int32_t batch, total_q, max_drafts;
   const float* temps;
   const float* uniforms;
   int64_t ld_u;
@@ -375,31 +405,88 @@ struct VerifyParams {
   int64_t* tokens;
   int32_t* accepted;
   float* logprobs;
+  float4* part;  // [total_q][chunks]: maximum, sum, first maximum
+  int32_t chunks, chunk_packs;
 };
+constexpr int STAT_THREADS = 256;
 
-constexpr int TILE_ROWS = 16;  // rows whose statistics are taken before their drafts are judged
+// Warp-wide: how many entries of the ascending list cu[0..count) are <= x, 32 probes at a time.
+__device__ __forceinline__ int count_up_to(const int32_t* cu, int count, int x) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, end = count;
+  while (lo < end) {
+    const int step = (end - lo + 31) / 32;
+    const int at = lo + lane * step;
+    const bool below = at < end && __ldg(cu + min(at + step, end) - 1) <= x;
+    const int blocks = __popc(__ballot_sync(0xffffffffu, below));
+    lo = min(lo + blocks * step, end);
+    if (step == 1) break;
+    end = min(lo + step, end);
+  }
+  return lo;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(STAT_THREADS, 4) row_stats_kernel(VerifyParams P) {
+  constexpr int N = pack_n<T>(), WARPS = STAT_THREADS / 32, U = 4;
+  __shared__ Stats mine[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  const int row = blockIdx.x / P.chunks, chunk = blockIdx.x % P.chunks;
+  const T* x = reinterpret_cast<const T*>(P.target) + (int64_t)row * P.ld;
+  const int k0 = chunk * P.chunk_packs, k1 = k0 + P.chunk_packs;  // packets past the row's end are -inf
+  uint4 raw[U];
+  auto load = [&](int u, int base) {
+    if (base < k1) raw[u] = load_pack<T, VEC>(x, base + lane, P.n);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) load(u, k0 + warp * 32 + u * STAT_THREADS);
+  const int seq = count_up_to(P.cu_q, P.batch + 1, row) - 1;
+  if (seq < 0 || seq >= P.batch || row - __ldg(P.cu_q + seq) > P.max_drafts) return;  // no one asks for this row
+  const Scale sc(P.temps[seq]);
+  Fold f;
+  f.init();
+  for (int base = k0 + warp * 32; base < k1; base += STAT_THREADS * U) {  // warp-uniform
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (base + u * STAT_THREADS >= k1) break;
+      float v[N], w[N];
+      unpack<T>(raw[u], v);
+      f.add<N>(v, base + u * STAT_THREADS + lane, sc, w);
+      load(u, base + (u + U) * STAT_THREADS);
+    }
+  }
+  const Stats st = f.finish<T, VEC>(x, P.n, sc);
+  if (lane == 0) mine[warp] = st;
+  __syncthreads();
+  if (warp == 0) {
+    Stats a = lane < WARPS ? mine[lane] : no_stats();
+    a.merge_warp(sc);
+    if (lane == 0) P.part[blockIdx.x] = make_float4(a.m, a.s, __int_as_float(a.at), 0.f);
+  }
+}
+
+constexpr int TILE_ROWS = 16;  // rows judged at a time
 
 template <typename T, bool VEC, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) verify_kernel(VerifyParams P) {
-  constexpr int N = pack_n<T>(), WARPS = NT / 32, U = 4;
-  __shared__ float wm[WARPS][TILE_ROWS], wsum[WARPS][TILE_ROWS];
-  __shared__ int wfirst[WARPS][TILE_ROWS];
-  __shared__ float cm[TILE_ROWS][MAX_CLUSTER], cs[TILE_ROWS][MAX_CLUSTER];
-  __shared__ int cfirst[TILE_ROWS][MAX_CLUSTER];
-  __shared__ float rm[TILE_ROWS], rs[TILE_ROWS];  // the rows' statistics over the whole vocabulary
-  __shared__ int rfirst[TILE_ROWS];
-  __shared__ float id_x[TILE_ROWS], id_q[TILE_ROWS];  // target logit and draft probability of each draft
+__global__ void __launch_bounds__(NT, 1024 / NT) judge_kernel(VerifyParams P) {
+  constexpr int N = pack_n<T>(), WARPS = NT / 32, U = 2;
+  __shared__ Stats rows_s[TILE_ROWS];  // over the whole vocabulary
+  __shared__ float id_x[TILE_ROWS], id_q[TILE_ROWS], id_u[TILE_ROWS];  // of each draft: target logit, q, uniform
   __shared__ int id_at[TILE_ROWS];
   __shared__ float bw[WARPS], be[WARPS];
   __shared__ int bat[WARPS];
   __shared__ float cw[2][MAX_CLUSTER], ce[2][MAX_CLUSTER];
   __shared__ int cat[2][MAX_CLUSTER];
   __shared__ int s_count, s_winner;
+  __shared__ int s_bound[2];  // bits of a score that the CTA's race has reached (scores are >= 0)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cl::ctarank(), ranks = (int)cl::nctarank();
   cl::cluster_arrive_relaxed();
-  pdl_wait();
-  pdl_trigger();
+  if (tid < 2) s_bound[tid] = 0;
+  // The kernel before this one (the row statistics) has waited for its predecessors before it let
+  // this one start: all inputs are settled, only its own results are waited for below.
   const int64_t b = blockIdx.x / ranks;
   const int begin = max(0, __ldg(P.cu_q + b)), end = min(P.total_q, __ldg(P.cu_q + b + 1));
   const int drafts = min(end - begin - 1, P.max_drafts);  // -1: an empty sequence
@@ -409,135 +496,82 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_kernel(VerifyParams P) {
   share<T>(n, rank, ranks, k0, k1);
   int64_t* tokens = P.tokens + b * (P.max_drafts + 1);
   float* logprobs = P.logprobs + b * (P.max_drafts + 1);
-  cl::cluster_wait();  // every CTA of the cluster runs
+  bool waited = false;
 
-  int count = 0;  // accepted drafts; cluster-uniform from here on
+  int count = 0;  // accepted drafts; cluster-uniform
   for (int i0 = 0; i0 <= drafts; i0 += TILE_ROWS) {
     const int rows = min(TILE_ROWS, drafts + 1 - i0);
     const T* x0 = reinterpret_cast<const T*>(P.target) + (int64_t)(begin + i0) * P.ld;
-    // what the judgement needs of each draft, asked for before the statistics are taken
     if (tid < rows) {
       const int i = i0 + tid;
       int at = -1;
-      float xv = -INFINITY, q = 1.f;
+      float xv = -INFINITY, q = 1.f, un = 0.f;
       if (i < drafts) {
         const int64_t id = P.ids[begin + i + 1];
+        un = P.uniforms[b * P.ld_u + i];
         if (id >= 0 && id < n) {
           at = (int)id;
           xv = as_f32(x0[(int64_t)tid * P.ld + at]);
-          if (P.draft) {
-            const float xd = as_f32(reinterpret_cast<const T*>(P.draft)[b * P.d_sb + i * P.d_sd + at]);
-            const float d = fminf(xd, FLT_MAX) / sc.t - P.draft_lse[b * P.l_sb + i * P.l_sd];
-            q = xd == xd ? expf(d) : 0.f;
-          }
+          if (P.draft)
+            q = draft_prob(as_f32(reinterpret_cast<const T*>(P.draft)[b * P.d_sb + i * P.d_sd + at]), sc,
+                           P.draft_lse[b * P.l_sb + i * P.l_sd]);
         }
       }
       id_at[tid] = at;
       id_x[tid] = xv;
       id_q[tid] = q;
+      id_u[tid] = un;
     }
-    // ---- statistics of the tile's rows over this CTA's share, U packets in flight a thread
-    const int np = k0 + warp * 32 < k1 ? (k1 - (k0 + warp * 32) + NT - 1) / NT : 0;  // warp-uniform
-    const int total = rows * np;
-    Stats st;
-    st.init();
-    int row = 0, p = 0, lrow = 0, lp = 0;
-    auto flush = [&]() {
-      if (sc.greedy) st.at = first_maximum<T, VEC>(x0 + (int64_t)row * P.ld, st, n);
-      st.merge_warp(sc);
-      if (lane == 0) {
-        wm[warp][row] = st.m;
-        wsum[warp][row] = st.s;
-        wfirst[warp][row] = st.at;
-      }
-      st.init();
-      ++row;
-      p = 0;
-    };
-    for (int t = 0; t < total; t += U) {
-      uint4 raw[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (t + u < total) {
-          raw[u] = load_pack<T, VEC>(x0 + (int64_t)lrow * P.ld, k0 + warp * 32 + lane + lp * NT, n);
-          if (++lp == np) {
-            lp = 0;
-            ++lrow;
-          }
-        }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (t + u < total) {
-          float v[N];
-          unpack<T>(raw[u], v);
-          fold<N>(st, v, k0 + warp * 32 + lane + p * NT, sc);
-          if (++p == np) flush();
-        }
+    if (!waited) {
+      pdl_wait();
+      pdl_trigger();
+      waited = true;
     }
-    while (row < rows) flush();  // warps without packets
-    __syncthreads();
-    // warp w merges rows w, w + WARPS, ... over the CTA's warps and tells every CTA
     for (int i = warp; i < rows; i += WARPS) {
-      Stats a;
-      a.init();
-      if (lane < WARPS) a = Stats{wm[lane][i], wsum[lane][i], wfirst[lane][i]};
-      a.merge_warp(sc);
-      if (lane < ranks) {
-        cl::st_cluster_f32(cl::mapa(&cm[i][rank], lane), a.m);
-        cl::st_cluster_f32(cl::mapa(&cs[i][rank], lane), a.s);
-        cl::st_cluster_f32(cl::mapa(&cfirst[i][rank], lane), __int_as_float(a.at));
+      Stats a = no_stats();
+      const float4* part = P.part + (int64_t)(begin + i0 + i) * P.chunks;
+      for (int c = lane; c < P.chunks; c += 32) {
+        const float4 w = part[c];
+        a.merge(w.x, w.y, __float_as_int(w.z), sc);
       }
-    }
-    cl::cluster_sync();
-    for (int i = warp; i < rows; i += WARPS) {
-      Stats a;
-      a.init();
-      if (lane < ranks) a = Stats{cm[i][lane], cs[i][lane], cfirst[i][lane]};
       a.merge_warp(sc);
-      if (lane == 0) {
-        rm[i] = a.m;
-        rs[i] = a.s;
-        rfirst[i] = a.at;
-      }
+      if (lane == 0) rows_s[i] = a;
     }
     __syncthreads();
     // ---- judge the tile's drafts: lane = draft; the first refusal ends the run of acceptances
     if (warp == 0) {
       bool ok = false;
-      float lp_id = 0.f;
+      float lp = 0.f;
       if (lane < rows && i0 + lane < drafts) {
         const int at = id_at[lane];
-        const bool any = rs[lane] > 0.f;
-        const float d = sc.diff(id_x[lane], rm[lane]);
-        if (sc.greedy)
-          ok = any && at == rfirst[lane];
-        else
-          ok = any && at >= 0 &&
-               P.uniforms[b * P.ld_u + i0 + lane] * id_q[lane] < sc.weight_exact(d) / rs[lane];
-        lp_id = d / sc.t - logf(rs[lane]);
+        const Stats st = rows_s[lane];
+        const float d = sc.diff(id_x[lane], st.m);
+        ok = st.s > 0.f && at >= 0 &&
+             (sc.greedy ? at == st.at : id_u[lane] * id_q[lane] < sc.weight_exact(d) / st.s);
+        lp = d / sc.t - logf(st.s);
       }
       const unsigned good = __ballot_sync(0xffffffffu, ok);
       const int run = __ffs(~good) - 1;  // rows <= 16 < 32: a zero bit exists
       if (rank == 0 && lane < run) {
         tokens[i0 + lane] = id_at[lane];
-        logprobs[i0 + lane] = lp_id;
+        logprobs[i0 + lane] = lp;
       }
       if (lane == 0) s_count = run;
     }
     __syncthreads();
     const int run = s_count;
     count += run;
-    if (run == TILE_ROWS && i0 + TILE_ROWS <= drafts) {
-      cl::cluster_sync();  // the exchange words are read before the next tile overwrites them
+    if (run == TILE_ROWS) {  // every row's draft was accepted: the next tile (it exists)
+      __syncthreads();
       continue;
     }
     // ---- the token after the accepted drafts, from row `run` of the tile
     const int i = i0 + run;
     const T* x = x0 + (int64_t)run * P.ld;
-    const float m = rm[run], s = rs[run];
+    const float m = rows_s[run].m, s = rows_s[run].s;
     int winner = NONE;
     if (sc.greedy) {
-      winner = s > 0.f ? rfirst[run] : NONE;
+      winner = s > 0.f ? rows_s[run].at : NONE;
     } else if (s > 0.f) {
       const T* dr = P.draft && i < drafts ? reinterpret_cast<const T*>(P.draft) + b * P.d_sb + i * P.d_sd : nullptr;
       const float dl = dr ? P.draft_lse[b * P.l_sb + i * P.l_sd] : 0.f;
@@ -547,31 +581,47 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_kernel(VerifyParams P) {
       for (int attempt = 0; attempt < 2; ++attempt) {  // the second draws from p: nothing was left
         Best best;
         best.init();
-        for (int k = k0 + tid; k < k1; k += NT) {
-          float v[N], ns[N];
-          const uint4 raw = load_pack<T, VEC>(x, k, n);
-          uint4 rawd;
-          if (dr) rawd = load_pack<T, VEC>(dr, k, n);
-          load_noise<T, VEC>(e, k, n, ns);
-          unpack<T>(raw, v);
-          float w[N];
+        // p bounds what is left of it, so a packet in which no p / e reaches a score that the CTA
+        // already has is done with; only the others look at the draft's logits.  About 1 / (1 - a)
+        // of a row's tokens do, where a is the chance that the draft was accepted.
+        uint4 raw[U];
+        float ns[U][N];
+        auto load = [&](int u, int base) {
+          if (base >= k1) return;
+          raw[u] = load_pack<T, VEC>(x, base + lane, n);
+          load_noise<T, VEC>(e, base + lane, n, ns[u]);
+        };
 #pragma unroll
-          for (int c = 0; c < N; ++c) w[c] = sc.weight_exact(sc.diff(v[c], m)) * inv;
-          if (attempt == 0 && dr) {
-            float d[N];
-            unpack<T>(rawd, d);
+        for (int u = 0; u < U; ++u) load(u, k0 + warp * 32 + u * NT);
+        for (int base = k0 + warp * 32; base < k1; base += NT * U) {  // warp-uniform
 #pragma unroll
-            for (int c = 0; c < N; ++c) {
-              const float q = d[c] == d[c] ? expf(fminf(d[c], FLT_MAX) / sc.t - dl) : 0.f;
-              w[c] = fmaxf(w[c] - q, 0.f);
+          for (int u = 0; u < U; ++u) {
+            if (base + u * NT >= k1) break;
+            const int k = base + u * NT + lane;
+            const float score = __int_as_float(*const_cast<volatile int*>(&s_bound[attempt]));
+            const float least = score * SLACK;
+            float v[N];
+            unpack<T>(raw[u], v);
+            bool hit = false;
+#pragma unroll
+            for (int c = 0; c < N; ++c) hit |= !(sc.weight(sc.diff(v[c], m)) * inv <= least * ns[u][c]);
+            if (__any_sync(0xffffffffu, hit)) {
+              const bool left = attempt == 0 && dr;
+              uint4 rawd;
+              if (left) rawd = load_pack<T, VEC>(dr, k, n);
+#pragma unroll
+              for (int c = 0; c < N; ++c) {
+                const int at = pack_index<T, VEC>(k, c);
+                float w = sc.weight_exact(sc.diff(v[c], m)) * inv;
+                if (left) w = fmaxf(w - draft_prob(as_f32(reinterpret_cast<const T*>(&rawd)[c]), sc, dl), 0.f);
+                if (attempt == 0 && at == struck) w = fmaxf(w - 1.f, 0.f);
+                const float ei = exponential(ns[u][c]);
+                if (w * best.e > best.w * ei) best = Best{w, ei, at};
+              }
+              const float reached = warp_max(best.w / best.e);
+              if (lane == 0 && reached > score) atomicMax(&s_bound[attempt], __float_as_int(reached));
             }
-          }
-#pragma unroll
-          for (int c = 0; c < N; ++c) {
-            const int at = pack_index<T, VEC>(k, c);
-            if (attempt == 0 && at == struck) w[c] = fmaxf(w[c] - 1.f, 0.f);
-            const float ei = exponential(ns[c]);
-            if (w[c] * best.e > best.w * ei) best = Best{w[c], ei, at};
+            load(u, base + (u + U) * NT);
           }
         }
         best.merge_warp();
@@ -581,6 +631,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_kernel(VerifyParams P) {
           bat[warp] = best.at;
         }
         __syncthreads();
+        if (attempt == 0) cl::cluster_wait();  // every CTA of the cluster runs
         if (warp == 0) {
           best.init();
           if (lane < WARPS) best = Best{bw[lane], be[lane], bat[lane]};
@@ -609,6 +660,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_kernel(VerifyParams P) {
     }
     break;
   }
+  if (!waited) {
+    pdl_wait();
+    pdl_trigger();
+  }
   if (rank == 0) {
     const int written = drafts < 0 ? 0 : count + 1;
     for (int i = written + tid; i <= P.max_drafts; i += NT) {
@@ -620,17 +675,28 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_kernel(VerifyParams P) {
 }
 
 // ---- launch ------------------------------------------------------------------------------------
-// CTAs per row: as many as fill the SMs' 2,048 resident threads once (592 CTAs of 256), so that few
-// rows still pull from all of HBM, but no less than 2,048 logits a CTA (below that the exchange
-// costs more than the reading saves).  Up to 148 CTAs in all take 1,024 threads each.
+// CTAs per row or sequence: as many as fill the SMs' threads once (592 CTAs of 256; 512 in clusters of
+// 16, which have to fit a GPC), so that few rows still pull from all of HBM, but no less than 2,048
+// logits a CTA (below that the exchange costs more than the reading saves).  Up to 148 CTAs in all
+// take 1,024 threads each.
 struct Split {
   int ctas;
   bool wide;
 };
 inline Split split_for(int64_t rows, int64_t vocab) {
   int c = 1;
-  while (c < MAX_CLUSTER && rows * (2 * c) <= (c < 8 ? 592 : 148) && vocab >= 2048 * 2 * c) c *= 2;
+  while (c < MAX_CLUSTER && rows * (2 * c) <= (c < 8 ? 592 : 512) && vocab >= 2048 * 2 * c) c *= 2;
   return {c, rows * c <= 148};
+}
+
+// Shares of a target row in the statistics kernel: 16 packets a thread, halved while the CTAs would
+// not fill the SMs twice.
+inline void stat_chunks(int64_t rows, int64_t vocab, int pack, int* chunks, int* packs) {
+  const int64_t all = cdiv(vocab, 32 * pack) * 32;
+  int per = 16;
+  while (per > 1 && rows * cdiv(all, per * STAT_THREADS) < 2 * 592) per /= 2;
+  *packs = per * STAT_THREADS;
+  *chunks = (int)cdiv(all, *packs);
 }
 
 template <auto Kernel, typename... Args>
@@ -662,10 +728,14 @@ int sample_typed(int64_t rows, int64_t vocab, cudaStream_t st, const void* logit
                  : launch<sample_kernel<T, VEC, 256>>(rows, sp, st, (const T*)logits, args...);
 }
 template <typename T, bool VEC>
-int verify_typed(int64_t batch, const VerifyParams& P, cudaStream_t st) {
-  const Split sp = split_for(batch, P.n);
-  return sp.wide ? launch<verify_kernel<T, VEC, 1024>>(batch, sp, st, P)
-                 : launch<verify_kernel<T, VEC, 256>>(batch, sp, st, P);
+int verify_typed(VerifyParams P, cudaStream_t st) {
+  if (P.total_q > 0) {
+    (void)ada::launch_k(row_stats_kernel<T, VEC>, dim3((unsigned)P.total_q * P.chunks), dim3(STAT_THREADS), 0, st, P);
+    ADA_CHECK_LAUNCH();
+  }
+  const Split sp = split_for(P.batch, P.n);
+  return sp.wide ? launch<judge_kernel<T, VEC, 1024>>(P.batch, sp, st, P)
+                 : launch<judge_kernel<T, VEC, 256>>(P.batch, sp, st, P);
 }
 
 }  // namespace smp
@@ -696,35 +766,44 @@ extern "C" int ada_sample(const void* logits, int dtype, int64_t ld, int64_t row
 #undef ADA_SAMPLE
 }
 
+extern "C" size_t ada_verify_drafts_workspace_size(int32_t total_q, int64_t vocab, int dtype) {
+  if (total_q <= 0 || vocab <= 0 || !smp::dtype_ok(dtype)) return 0;
+  int chunks, packs;
+  smp::stat_chunks(total_q, vocab, 16 / smp::dtype_size(dtype), &chunks, &packs);
+  return (size_t)total_q * chunks * sizeof(float4);
+}
+
 extern "C" int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t total_q, int64_t vocab,
                                  const int64_t* input_ids, const int32_t* cu_seqlens_q, int32_t batch,
                                  int32_t max_drafts, const float* temperatures, const float* uniforms, int64_t ld_u,
                                  const float* noise, int64_t ld_noise, const void* draft_logits,
                                  int64_t draft_stride_b, int64_t draft_stride_d, const float* draft_lse,
                                  int64_t lse_stride_b, int64_t lse_stride_d, int64_t* tokens, int32_t* accepted,
-                                 float* logprobs, void* stream) {
+                                 float* logprobs, void* workspace, size_t workspace_bytes, void* stream) {
   if (batch < 0 || total_q < 0 || max_drafts < 0 || vocab <= 0 || ld < vocab || ld_noise < vocab ||
       ld_u < max_drafts || !smp::dtype_ok(dtype))
     return ADA_ERR_INVALID_ARG;
   if (batch == 0) return ADA_OK;
   if ((!target && total_q > 0) || (!input_ids && total_q > 0) || !cu_seqlens_q || !temperatures || !noise || !tokens ||
-      !accepted || !logprobs || (!uniforms && max_drafts > 0))
+      !accepted || !logprobs || (!uniforms && max_drafts > 0) || (!workspace && total_q > 0))
     return ADA_ERR_INVALID_ARG;
   if ((draft_logits == nullptr) != (draft_lse == nullptr)) return ADA_ERR_INVALID_ARG;
   if (draft_logits && (draft_stride_b < 0 || draft_stride_d < 0 || lse_stride_b < 0 || lse_stride_d < 0))
     return ADA_ERR_INVALID_ARG;
-  if (vocab > (1 << 30) || batch > (1 << 20) || max_drafts > 1024) return ADA_ERR_UNSUPPORTED;
+  if (vocab > (1 << 30) || batch > (1 << 20) || max_drafts > 1024 || (int64_t)total_q * vocab > (1LL << 42)) return ADA_ERR_UNSUPPORTED;
   if (smp::misaligned(target, dtype) || smp::misaligned(draft_logits, dtype) || ((uintptr_t)noise & 3) ||
       ((uintptr_t)temperatures & 3) || ((uintptr_t)uniforms & 3) || ((uintptr_t)draft_lse & 3) ||
       ((uintptr_t)input_ids & 7) || ((uintptr_t)cu_seqlens_q & 3) || ((uintptr_t)tokens & 7) ||
-      ((uintptr_t)accepted & 3) || ((uintptr_t)logprobs & 3))
+      ((uintptr_t)accepted & 3) || ((uintptr_t)logprobs & 3) || ((uintptr_t)workspace & 15))
     return ADA_ERR_ALIGNMENT;
+  if (workspace_bytes < ada_verify_drafts_workspace_size(total_q, vocab, dtype)) return ADA_ERR_WORKSPACE;
   smp::VerifyParams P;
   P.target = target;
   P.ld = ld;
   P.n = (int)vocab;
   P.ids = input_ids;
   P.cu_q = cu_seqlens_q;
+  P.batch = batch;
   P.total_q = total_q;
   P.max_drafts = max_drafts;
   P.temps = temperatures;
@@ -741,14 +820,16 @@ extern "C" int ada_verify_drafts(const void* target, int dtype, int64_t ld, int3
   P.tokens = tokens;
   P.accepted = accepted;
   P.logprobs = logprobs;
+  P.part = reinterpret_cast<float4*>(workspace);
+  smp::stat_chunks(total_q, vocab, 16 / smp::dtype_size(dtype), &P.chunks, &P.chunk_packs);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int size = smp::dtype_size(dtype);
   const bool vec = smp::on16(target, ld * size) && smp::on16(noise, ld_noise * 4) &&
                    (!draft_logits || smp::on16(draft_logits, (draft_stride_b | draft_stride_d) * size));
   if (dtype == ADA_DT_BF16)
-    return vec ? smp::verify_typed<__nv_bfloat16, true>(batch, P, st)
-               : smp::verify_typed<__nv_bfloat16, false>(batch, P, st);
+    return vec ? smp::verify_typed<__nv_bfloat16, true>(P, st)
+               : smp::verify_typed<__nv_bfloat16, false>(P, st);
   if (dtype == ADA_DT_F16)
-    return vec ? smp::verify_typed<__half, true>(batch, P, st) : smp::verify_typed<__half, false>(batch, P, st);
-  return vec ? smp::verify_typed<float, true>(batch, P, st) : smp::verify_typed<float, false>(batch, P, st);
+    return vec ? smp::verify_typed<__half, true>(P, st) : smp::verify_typed<__half, false>(P, st);
+  return vec ? smp::verify_typed<float, true>(P, st) : smp::verify_typed<float, false>(P, st);
 }

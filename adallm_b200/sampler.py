@@ -14,20 +14,20 @@ from torch import nn
 from . import _native as N
 
 
-def _rows(t: torch.Tensor, name: str, dtypes, dim: int = 2) -> torch.Tensor:
-    if t.dim() != dim or t.dtype not in dtypes:
-        raise ValueError(f"{name} must be {dim}-D, one of {[str(d) for d in dtypes]}")
+def _rows(t: torch.Tensor, name: str, dim: int = 2) -> torch.Tensor:
+    if t.dim() != dim:
+        raise ValueError(f"{name} must have {dim} dimensions")
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[-1])
+def _ld(t: torch.Tensor, rows: int, cols: int) -> int:
+    return t.stride(0) if rows > 1 else max(t.stride(0), cols)
 
 
 def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
     if t.dtype != dtype or t.numel() != n:
         raise ValueError(f"{name} must be {dtype} with {n} entries")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def sample(logits: torch.Tensor, temperatures: torch.Tensor,
@@ -39,29 +39,33 @@ def sample(logits: torch.Tensor, temperatures: torch.Tensor,
     and the row's log-normaliser, both at the row's temperature (1 where greedy).  A row whose
     logits are all -inf gives -1, 0 and -inf."""
     N.require_cuda(logits, temperatures, noise, what="sample")
-    logits = _rows(logits, "logits", N.DT_LOGITS)
-    noise = _rows(noise, "noise", (torch.float32,))
+    logits, noise = _rows(logits, "logits"), _rows(noise, "noise")
     r, v = logits.shape
+    code = N.DT_LOGITS.get(logits.dtype)
+    if code is None or noise.dtype != torch.float32 or noise.shape != logits.shape:
+        raise ValueError("logits must be bf16, fp16 or fp32, and noise fp32 with one entry per logit")
     temperatures = _vector(temperatures, "temperatures", torch.float32, r)
-    if noise.shape != logits.shape:
-        raise ValueError("noise must have one entry per logit")
     d = logits.device
     tokens = torch.empty(r, dtype=torch.int64, device=d)
     logprobs = torch.empty(r, dtype=torch.float32, device=d)
     lse = torch.empty(r, dtype=torch.float32, device=d)
     if r == 0:
         return tokens, logprobs, lse
-    st = N.lib().ada_sample(logits.data_ptr(), N.DT_LOGITS[logits.dtype], _ld(logits), r, v, temperatures.data_ptr(),
-                            noise.data_ptr(), _ld(noise), tokens.data_ptr(), logprobs.data_ptr(), lse.data_ptr(),
-                            N.stream_ptr(d))
+    st = N.lib().ada_sample(logits.data_ptr(), code, _ld(logits, r, v), r, v, temperatures.data_ptr(),
+                            noise.data_ptr(), _ld(noise, r, v), tokens.data_ptr(), logprobs.data_ptr(),
+                            lse.data_ptr(), N.stream_ptr(d))
     N.check(st, "sampling kernel")
     return tokens, logprobs, lse
 
 
+def verify_workspace_bytes(total_q: int, vocab: int, dtype: torch.dtype) -> int:
+    return int(N.lib().ada_verify_drafts_workspace_size(total_q, vocab, N.DT_LOGITS[dtype]))
+
+
 def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqlens_q: torch.Tensor,
                   temperatures: torch.Tensor, uniforms: torch.Tensor, noise: torch.Tensor,
-                  draft_logits: torch.Tensor | None = None, draft_lse: torch.Tensor | None = None
-                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                  draft_logits: torch.Tensor | None = None, draft_lse: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Accepts each sequence's drafted tokens up to the first refusal and draws the token after them.
 
     target_logits [N, V] (bf16/fp16/fp32): the target's logits of the rows input_ids int64 [N];
@@ -73,35 +77,43 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     Returns (tokens int64 [B, D + 1], accepted int32 [B], logprobs fp32 [B, D + 1]): the accepted
     drafts and the drawn token with their log-probabilities under the target, then -1 and 0."""
     N.require_cuda(target_logits, input_ids, cu_seqlens_q, temperatures, uniforms, noise, draft_logits, draft_lse,
-                   what="verify_drafts")
-    target_logits = _rows(target_logits, "target_logits", N.DT_LOGITS)
-    noise = _rows(noise, "noise", (torch.float32,))
-    uniforms = _rows(uniforms, "uniforms", (torch.float32,))
+                   workspace, what="verify_drafts")
+    target_logits, noise = _rows(target_logits, "target_logits"), _rows(noise, "noise")
+    uniforms = _rows(uniforms, "uniforms")
     (n, v), (b, most) = target_logits.shape, uniforms.shape
+    dtype = target_logits.dtype
+    code = N.DT_LOGITS.get(dtype)
+    if code is None or noise.dtype != torch.float32 or uniforms.dtype != torch.float32 or noise.shape != (b, v):
+        raise ValueError("target_logits must be bf16, fp16 or fp32, uniforms and noise [batch, vocab] fp32")
     temperatures = _vector(temperatures, "temperatures", torch.float32, b)
     input_ids = _vector(input_ids, "input_ids", torch.int64, n)
     cu_seqlens_q = _vector(cu_seqlens_q, "cu_seqlens_q", torch.int32, b + 1)
-    if noise.shape != (b, v):
-        raise ValueError("noise must be [batch, vocab]")
     if (draft_logits is None) != (draft_lse is None):
         raise ValueError("draft_logits and draft_lse come together")
     strides = (0, 0, 0, 0)
     if draft_logits is not None:
-        draft_logits = _rows(draft_logits, "draft_logits", (target_logits.dtype,), 3)
-        if draft_logits.shape != (b, most, v) or draft_lse.shape != (b, most) or draft_lse.dtype != torch.float32:
-            raise ValueError("draft_logits must be [batch, drafts, vocab] and draft_lse fp32 [batch, drafts]")
-        strides = (draft_logits.stride(0), draft_logits.stride(1), draft_lse.stride(0), draft_lse.stride(1))
+        draft_logits = _rows(draft_logits, "draft_logits", 3)
+        if (draft_logits.dtype != dtype or draft_logits.shape != (b, most, v) or draft_lse.shape != (b, most)
+                or draft_lse.dtype != torch.float32):
+            raise ValueError("draft_logits must be [batch, drafts, vocab] like the target's, draft_lse fp32 "
+                             "[batch, drafts]")
+        strides = draft_logits.stride()[:2] + draft_lse.stride()
     d = target_logits.device
     tokens = torch.empty((b, most + 1), dtype=torch.int64, device=d)
     logprobs = torch.empty((b, most + 1), dtype=torch.float32, device=d)
     accepted = torch.empty(b, dtype=torch.int32, device=d)
     if b == 0:
         return tokens, accepted, logprobs
-    st = N.lib().ada_verify_drafts(
-        target_logits.data_ptr(), N.DT_LOGITS[target_logits.dtype], _ld(target_logits) if n else v, n, v,
-        input_ids.data_ptr(), cu_seqlens_q.data_ptr(), b, most, temperatures.data_ptr(), uniforms.data_ptr(),
-        _ld(uniforms), noise.data_ptr(), _ld(noise), N.ptr(draft_logits), strides[0], strides[1], N.ptr(draft_lse),
-        strides[2], strides[3], tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), N.stream_ptr(d))
+    lib = N.lib()
+    need = lib.ada_verify_drafts_workspace_size(n, v, code)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=d)
+    st = lib.ada_verify_drafts(
+        target_logits.data_ptr(), code, _ld(target_logits, n, v), n, v, input_ids.data_ptr(),
+        cu_seqlens_q.data_ptr(), b, most, temperatures.data_ptr(), uniforms.data_ptr(), _ld(uniforms, b, most),
+        noise.data_ptr(), _ld(noise, b, v), N.ptr(draft_logits), strides[0], strides[1], N.ptr(draft_lse), strides[2],
+        strides[3], tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), workspace.data_ptr(), need,
+        N.stream_ptr(d))
     N.check(st, "draft verification kernel")
     return tokens, accepted, logprobs
 

@@ -637,15 +637,17 @@ ADA_API int ada_sample(const void* logits, int dtype, int64_t ld, int64_t rows, 
  * maximum.  tokens int64 and logprobs fp32 [batch, max_drafts + 1]: the accepted drafts and the
  * drawn token with their log-probabilities under p, then -1 and 0; accepted int32 [batch].
  * Logits are read as in ada_sample; where no token is possible the drawn one is -1.
- * One launch, no workspace.
+ * workspace: ada_verify_drafts_workspace_size bytes, 16-byte aligned, no initial value; calls that
+ * share one must be ordered.  Two launches.
  * ---------------------------------------------------------------------- */
+ADA_API size_t ada_verify_drafts_workspace_size(int32_t total_q, int64_t vocab, int dtype);
 ADA_API int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t total_q, int64_t vocab,
                               const int64_t* input_ids, const int32_t* cu_seqlens_q, int32_t batch,
                               int32_t max_drafts, const float* temperatures, const float* uniforms, int64_t ld_u,
                               const float* noise, int64_t ld_noise, const void* draft_logits, int64_t draft_stride_b,
                               int64_t draft_stride_d, const float* draft_lse, int64_t lse_stride_b,
                               int64_t lse_stride_d, int64_t* tokens, int32_t* accepted, float* logprobs,
-                              void* stream);
+                              void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

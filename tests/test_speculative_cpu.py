@@ -72,20 +72,24 @@ def test_sample_argument_errors(lib):
 
 
 def test_verify_argument_errors(lib):
+    need = lib.ada_verify_drafts_workspace_size(10, 1000, 0)
+    assert need > 0 and lib.ada_verify_drafts_workspace_size(0, 1000, 0) == 0
+
     def call(**kw):
         a = dict(x=P, dtype=0, ld=1000, total=10, vocab=1000, ids=P, cu=P, batch=4, most=3, temps=P, u=P, ld_u=3,
                  noise=P, ld_noise=1000, draft=P, d_sb=3000, d_sd=1000, lse=P, l_sb=3, l_sd=1, tokens=P, acc=P, lp=P,
-                 stream=None)
+                 ws=P, ws_bytes=need, stream=None)
         a.update(kw)
         return lib.ada_verify_drafts(*a.values())
 
     assert call(batch=0) == 0
-    for name in ("x", "ids", "cu", "temps", "u", "noise", "tokens", "acc", "lp"):
+    for name in ("x", "ids", "cu", "temps", "u", "noise", "tokens", "acc", "lp", "ws"):
         assert call(**{name: None}) == N.ADA_ERR_INVALID_ARG, name
     assert call(draft=None) == N.ADA_ERR_INVALID_ARG and call(lse=None) == N.ADA_ERR_INVALID_ARG
     assert call(d_sd=-1) == N.ADA_ERR_INVALID_ARG
     assert call(ld_u=2) == N.ADA_ERR_INVALID_ARG and call(dtype=4) == N.ADA_ERR_INVALID_ARG
     assert call(most=1025, ld_u=1025) == N.ADA_ERR_UNSUPPORTED
+    assert call(ws_bytes=need - 1) == N.ADA_ERR_WORKSPACE and call(ws=P + 8) == N.ADA_ERR_ALIGNMENT
     assert call(draft=P + 1) == N.ADA_ERR_ALIGNMENT and call(ids=P + 4) == N.ADA_ERR_ALIGNMENT
 
 
