@@ -76,7 +76,7 @@ _SIGS = {
                                            I32, P, P, I32, I32, I32, I32, I32, I32, F32, F32, F32, I32, P, INT, I64,
                                            I64, P, SZ, P, P]),
     "ada_sample": (INT, [P, INT, I64, I64, I64, P, P, I64, P, P, P, P]),
-    "ada_verify_drafts_workspace_size": (SZ, [I32, I64, INT]),
+    "ada_verify_drafts_workspace_size": (SZ, [I32, I32, I64, INT]),
     "ada_verify_drafts": (INT, [P, INT, I64, I32, I64, P, P, I32, I32, P, P, I64, P, I64, P, I64, I64, P, I64, I64, P,
                                 P, P, P, SZ, P]),
     "ada_nvfp4_sf_bytes": (SZ, [I64, I64]),

@@ -65,10 +65,53 @@ __device__ __forceinline__ uint4 load_pack(const T* __restrict__ x, int k, int n
   }
   return u;
 }
-template <typename T> __device__ __forceinline__ void unpack(const uint4& u, float* f) {
-  const T* h = reinterpret_cast<const T*>(&u);
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// A packet's values with NaN replaced by -inf (a maximum takes the operand that is a number), and
+// their maximum.
+template <typename H2> __device__ __forceinline__ float unpack_halves(const uint4& u, H2 low, float* f) {
+  H2 h[4];
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < pack_n<T>(); ++i) f[i] = as_f32(h[i]);
+  for (int i = 0; i < 4; ++i) h[i] = __hmax2(*reinterpret_cast<const H2*>(&w[i]), low);
+  const H2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = as_f32(h[i].x);
+    f[2 * i + 1] = as_f32(h[i].y);
+  }
+  return fmaxf(as_f32(m.x), as_f32(m.y));
+}
+template <typename T> __device__ __forceinline__ float unpack(const uint4& u, float* f) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return unpack_halves(u, __halves2bfloat162(minus_inf<T>(), minus_inf<T>()), f);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    return unpack_halves(u, __halves2half2(minus_inf<T>(), minus_inf<T>()), f);
+  } else {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = fmaxf(__uint_as_float(w[i]), -INFINITY);
+    return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+  }
+}
+// Raw element i of a packet.
+template <typename T> __device__ __forceinline__ float element(const uint4& u, int i) {
+  return as_f32(reinterpret_cast<const T*>(&u)[i]);
 }
 // The noise beside packet k of a T row.
 template <typename T, bool VEC>
@@ -99,11 +142,11 @@ struct Scale {
   bool greedy;
   float t;
   __device__ __forceinline__ explicit Scale(float temp) {
+    constexpr float L = 1.4426950408889634f, L_LO = (float)(1.4426950408889634 - (double)1.4426950408889634f);
     greedy = !(temp > 1e-10f);
     t = greedy ? 1.f : temp;
-    const double cd = 1.4426950408889634 / (double)t;
-    c = (float)cd;
-    c_lo = (float)(cd - (double)c);
+    c = L / t;
+    c_lo = (fmaf(-c, t, L) + L_LO) / t;
     least = -200.f / c;
   }
   // x - m, at most 0: -inf and NaN give `least` (weight 0), +inf gives 0.
@@ -148,25 +191,23 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 
 // A warp's statistics while it reads a row.  The maximum is the warp's (it moves a handful of times
-// a row, found by one vote a packet), so a logit costs a maximum, a difference, a clamp (which
-// also takes -inf and NaN to weight 0), a product, an ex2 and an add.
+// a row, found by one vote a packet), so a logit costs half a cleaning and half a maximum (packed
+// 16-bit), its widening, half a difference and half a product (f32x2), an ex2 and half an add.
 struct Fold {
-  float m, s;    // warp maximum; this lane's sum against it
+  float m;       // the warp's maximum
+  float2 s;      // this lane's sum against it, in two parts
   float top;     // this lane's own maximum and the packet that first held it (greedy rows)
   int top_pack;
   __device__ __forceinline__ void init() {
     m = -FLT_MAX;
-    s = 0.f;
+    s = make_float2(0.f, 0.f);
     top = -INFINITY;
     top_pack = NONE;
   }
-  // Fold packet k in; every lane of the warp calls.  w: the packet's weights against m.  Returns
-  // whether m moved.
+  // Fold packet k with values v and maximum `most` in; every lane of the warp calls.  w: the
+  // packet's weights against m.  Returns whether m moved.
   template <int N>
-  __device__ __forceinline__ bool add(float* v, int k, const Scale& sc, float* w) {
-    float most = v[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) most = fmaxf(most, v[i]);
+  __device__ __forceinline__ bool add(float* v, float most, int k, const Scale& sc, float* w) {
     if (most > top) {
       top = most;
       top_pack = k;
@@ -177,26 +218,26 @@ struct Fold {
       if (to > FLT_MAX) {  // +inf among them: read as the largest float (such a packet always gets here)
         to = FLT_MAX;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = v[i] > FLT_MAX ? FLT_MAX : v[i];
+        for (int i = 0; i < N; ++i) v[i] = fminf(v[i], FLT_MAX);
       }
-      s *= sc.weight(sc.diff(m, to));
+      const float by = sc.weight(sc.diff(m, to));
+      s = mul2(s, make_float2(by, by));
       m = to;
     }
-    float s0 = 0.f, s1 = 0.f;
+    const float2 off = make_float2(-m, -m), c2 = make_float2(sc.c, sc.c);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      w[i] = sc.weight(fmaxf(v[i] - m, sc.least));
-      w[i + 1] = sc.weight(fmaxf(v[i + 1] - m, sc.least));
-      s0 += w[i];
-      s1 += w[i + 1];
+      const float2 y = mul2(add2(make_float2(v[i], v[i + 1]), off), c2);  // -inf stays -inf: weight 0
+      w[i] = fast_exp2(y.x);
+      w[i + 1] = fast_exp2(y.y);
+      s = add2(s, make_float2(w[i], w[i + 1]));
     }
-    s += s0 + s1;
     return moved;
   }
   // The warp's statistics, in every lane.
   template <typename T, bool VEC>
   __device__ __forceinline__ Stats finish(const T* x, int n, const Scale& sc) const {
-    Stats st{m, s, NONE};
+    Stats st{m, s.x + s.y, NONE};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
     if (sc.greedy) {
@@ -316,8 +357,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
       if (base + u * NT >= k1) break;
       const int k = base + u * NT + lane;
       float v[N], w[N];
-      unpack<T>(raw[u], v);
-      const bool moved = f.add<N>(v, k, sc, w);
+      const float most = unpack<T>(raw[u], v);
+      const bool moved = f.add<N>(v, most, k, sc, w);
       if (!sc.greedy) {
         if (moved) bw = sc.weight(sc.diff(bx, f.m));
         const float2 known = unpack2(*const_cast<volatile unsigned long long*>(&bound));
@@ -325,7 +366,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
         const float least = score * SLACK;
         bool hit = false;
 #pragma unroll
-        for (int i = 0; i < N; ++i) hit |= !(w[i] <= least * ns[u][i]);
+        for (int i = 0; i < N; i += 2) {
+          const float2 t = mul2(make_float2(ns[u][i], ns[u][i + 1]), make_float2(least, least));
+          hit |= !(w[i] <= t.x) | !(w[i + 1] <= t.y);
+        }
         if (__any_sync(0xffffffffu, hit)) {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -383,9 +427,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 }
 
 // ---- verification ---------------------------------------------------------------------------------
-// Two kernels: the statistics of every target row (any CTA takes any share of any row, so ragged
-// numbers of drafts cost no balance), then one cluster per sequence that judges its drafts and
-// draws from one row, which is in L2 by then.
+// Two kernels: the statistics of every target row, then the draw from one row of every sequence
+// (by then in L2).  In both any CTA takes any share of any row, so ragged numbers of drafts cost no
+// balance; in the second each CTA judges its sequence's drafts for itself (a few words) and the
+// shares meet in one 64-bit atomic maximum of (score, lowest index), whose order does not matter.
 struct VerifyParams {
   const void* target;
   int64_t ld;
@@ -407,6 +452,9 @@ struct VerifyParams {
   float* logprobs;
   float4* part;  // [total_q][chunks]: maximum, sum, first maximum
   int32_t chunks, chunk_packs;
+  unsigned long long* best;  // [batch]: score bits << 32 | ~index; 0: no candidate yet
+  unsigned int* done;        // [batch]: shares drawn
+  int32_t draw_chunks, draw_packs;
 };
 constexpr int STAT_THREADS = 256;
 
@@ -433,7 +481,13 @@ __global__ void __launch_bounds__(STAT_THREADS, 4) row_stats_kernel(VerifyParams
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
+  if (blockIdx.x == 0)  // the draw's words, for the kernel after this one
+    for (int i = threadIdx.x; i < P.batch; i += STAT_THREADS) {
+      P.best[i] = 0;
+      P.done[i] = 0;
+    }
   const int row = blockIdx.x / P.chunks, chunk = blockIdx.x % P.chunks;
+  if (row >= P.total_q) return;  // a call without rows
   const T* x = reinterpret_cast<const T*>(P.target) + (int64_t)row * P.ld;
   const int k0 = chunk * P.chunk_packs, k1 = k0 + P.chunk_packs;  // packets past the row's end are -inf
   uint4 raw[U];
@@ -452,8 +506,8 @@ __global__ void __launch_bounds__(STAT_THREADS, 4) row_stats_kernel(VerifyParams
     for (int u = 0; u < U; ++u) {
       if (base + u * STAT_THREADS >= k1) break;
       float v[N], w[N];
-      unpack<T>(raw[u], v);
-      f.add<N>(v, base + u * STAT_THREADS + lane, sc, w);
+      const float most = unpack<T>(raw[u], v);
+      f.add<N>(v, most, base + u * STAT_THREADS + lane, sc, w);
       load(u, base + (u + U) * STAT_THREADS);
     }
   }
@@ -467,38 +521,97 @@ __global__ void __launch_bounds__(STAT_THREADS, 4) row_stats_kernel(VerifyParams
   }
 }
 
-constexpr int TILE_ROWS = 16;  // rows judged at a time
-
+// A share of the race for one token: the candidates of packets [k0, k1) of a row, weights
+// max(p - q, 0), returned as (score bits << 32 | ~index) in every lane of the warp; 0: none.  `known`
+// is a score that some share has reached.  p bounds what is left of it, so a packet in which no p / e
+// reaches that score is done with; the others (about 1 / (1 - a) of a row's tokens, where a is the
+// chance that the draft was accepted, and each warp's first) take q into account.
 template <typename T, bool VEC, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) judge_kernel(VerifyParams P) {
-  constexpr int N = pack_n<T>(), WARPS = NT / 32, U = 2;
+__device__ __forceinline__ unsigned long long draw_share(const T* x, const T* dr, const float* e, int n, int k0, int k1,
+                                                         const Scale& sc, float m, float s, float dl, int struck,
+                                                         volatile int* known) {
+  constexpr int N = pack_n<T>(), U = 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float inv = 1.f / s;
+  Best best;
+  best.init();
+  uint4 raw[U], rawd[U];
+  float ns[U][N];
+  auto load = [&](int u, int base) {
+    if (base >= k1) return;
+    raw[u] = load_pack<T, VEC>(x, base + lane, n);
+    if (dr) rawd[u] = load_pack<T, VEC>(dr, base + lane, n);
+    load_noise<T, VEC>(e, base + lane, n, ns[u]);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) load(u, k0 + warp * 32 + u * NT);
+  for (int base = k0 + warp * 32; base < k1; base += NT * U) {  // warp-uniform
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (base + u * NT >= k1) break;
+      const int k = base + u * NT + lane;
+      const float score = __int_as_float(*known);
+      const float least = score * SLACK * s;  // against s p
+      float v[N];
+      unpack<T>(raw[u], v);
+      bool hit = false;
+#pragma unroll
+      for (int c = 0; c < N; c += 2) {
+        const float2 t = mul2(make_float2(ns[u][c], ns[u][c + 1]), make_float2(least, least));
+        hit |= !(sc.weight(sc.diff(v[c], m)) <= t.x) | !(sc.weight(sc.diff(v[c + 1], m)) <= t.y);
+      }
+      if (__any_sync(0xffffffffu, hit)) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const int at = pack_index<T, VEC>(k, c);
+          float w = sc.weight_exact(sc.diff(v[c], m)) * inv;
+          if (dr) w = fmaxf(w - draft_prob(element<T>(rawd[u], c), sc, dl), 0.f);
+          if (at == struck) w = fmaxf(w - 1.f, 0.f);
+          const float ei = exponential(ns[u][c]);
+          if (w * best.e > best.w * ei) best = Best{w, ei, at};
+        }
+        const float reached = warp_max(best.w / best.e);
+        if (lane == 0 && reached > score) atomicMax(const_cast<int*>(known), __float_as_int(reached));
+      }
+      load(u, base + (u + U) * NT);
+    }
+  }
+  unsigned long long word =
+      best.at == NONE ? 0ull : ((unsigned long long)__float_as_uint(best.w / best.e) << 32) | (unsigned)~best.at;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long other = __shfl_xor_sync(0xffffffffu, word, o);
+    word = other > word ? other : word;
+  }
+  return word;
+}
+
+constexpr int TILE_ROWS = 16;  // rows judged at a time
+constexpr int DRAW_THREADS = 256;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(DRAW_THREADS, 3) draw_kernel(VerifyParams P) {
+  constexpr int WARPS = DRAW_THREADS / 32;
   __shared__ Stats rows_s[TILE_ROWS];  // over the whole vocabulary
   __shared__ float id_x[TILE_ROWS], id_q[TILE_ROWS], id_u[TILE_ROWS];  // of each draft: target logit, q, uniform
   __shared__ int id_at[TILE_ROWS];
-  __shared__ float bw[WARPS], be[WARPS];
-  __shared__ int bat[WARPS];
-  __shared__ float cw[2][MAX_CLUSTER], ce[2][MAX_CLUSTER];
-  __shared__ int cat[2][MAX_CLUSTER];
-  __shared__ int s_count, s_winner;
-  __shared__ int s_bound[2];  // bits of a score that the CTA's race has reached (scores are >= 0)
+  __shared__ unsigned long long words[WARPS];
+  __shared__ int s_count, s_last;
+  __shared__ int s_known;  // bits of a score that the race has reached (scores are >= 0)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = (int)cl::ctarank(), ranks = (int)cl::nctarank();
-  cl::cluster_arrive_relaxed();
-  if (tid < 2) s_bound[tid] = 0;
   // The kernel before this one (the row statistics) has waited for its predecessors before it let
   // this one start: all inputs are settled, only its own results are waited for below.
-  const int64_t b = blockIdx.x / ranks;
+  const int64_t b = blockIdx.x / P.draw_chunks;
+  const int chunk = blockIdx.x % P.draw_chunks;
   const int begin = max(0, __ldg(P.cu_q + b)), end = min(P.total_q, __ldg(P.cu_q + b + 1));
   const int drafts = min(end - begin - 1, P.max_drafts);  // -1: an empty sequence
   const Scale sc(P.temps[b]);
-  const int n = P.n;
-  int k0, k1;
-  share<T>(n, rank, ranks, k0, k1);
   int64_t* tokens = P.tokens + b * (P.max_drafts + 1);
   float* logprobs = P.logprobs + b * (P.max_drafts + 1);
   bool waited = false;
 
-  int count = 0;  // accepted drafts; cluster-uniform
+  int count = 0;  // accepted drafts
+  int run = 0;
   for (int i0 = 0; i0 <= drafts; i0 += TILE_ROWS) {
     const int rows = min(TILE_ROWS, drafts + 1 - i0);
     const T* x0 = reinterpret_cast<const T*>(P.target) + (int64_t)(begin + i0) * P.ld;
@@ -509,7 +622,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) judge_kernel(VerifyParams P) {
       if (i < drafts) {
         const int64_t id = P.ids[begin + i + 1];
         un = P.uniforms[b * P.ld_u + i];
-        if (id >= 0 && id < n) {
+        if (id >= 0 && id < P.n) {
           at = (int)id;
           xv = as_f32(x0[(int64_t)tid * P.ld + at]);
           if (P.draft)
@@ -551,134 +664,81 @@ __global__ void __launch_bounds__(NT, 1024 / NT) judge_kernel(VerifyParams P) {
         lp = d / sc.t - logf(st.s);
       }
       const unsigned good = __ballot_sync(0xffffffffu, ok);
-      const int run = __ffs(~good) - 1;  // rows <= 16 < 32: a zero bit exists
-      if (rank == 0 && lane < run) {
+      const int ran = __ffs(~good) - 1;  // rows <= 16 < 32: a zero bit exists
+      if (chunk == 0 && lane < ran) {
         tokens[i0 + lane] = id_at[lane];
         logprobs[i0 + lane] = lp;
       }
-      if (lane == 0) s_count = run;
+      if (lane == 0) s_count = ran;
     }
     __syncthreads();
-    const int run = s_count;
+    run = s_count;
     count += run;
-    if (run == TILE_ROWS) {  // every row's draft was accepted: the next tile (it exists)
-      __syncthreads();
-      continue;
-    }
-    // ---- the token after the accepted drafts, from row `run` of the tile
-    const int i = i0 + run;
-    const T* x = x0 + (int64_t)run * P.ld;
-    const float m = rows_s[run].m, s = rows_s[run].s;
-    int winner = NONE;
-    if (sc.greedy) {
-      winner = s > 0.f ? rows_s[run].at : NONE;
-    } else if (s > 0.f) {
-      const T* dr = P.draft && i < drafts ? reinterpret_cast<const T*>(P.draft) + b * P.d_sb + i * P.d_sd : nullptr;
-      const float dl = dr ? P.draft_lse[b * P.l_sb + i * P.l_sd] : 0.f;
-      const float* e = P.noise + b * P.ld_noise;
-      const int struck = !P.draft && i < drafts ? id_at[run] : -1;  // a certain draft: q = 1 there
-      const float inv = 1.f / s;
-      for (int attempt = 0; attempt < 2; ++attempt) {  // the second draws from p: nothing was left
-        Best best;
-        best.init();
-        // p bounds what is left of it, so a packet in which no p / e reaches a score that the CTA
-        // already has is done with; only the others look at the draft's logits.  About 1 / (1 - a)
-        // of a row's tokens do, where a is the chance that the draft was accepted.
-        uint4 raw[U];
-        float ns[U][N];
-        auto load = [&](int u, int base) {
-          if (base >= k1) return;
-          raw[u] = load_pack<T, VEC>(x, base + lane, n);
-          load_noise<T, VEC>(e, base + lane, n, ns[u]);
-        };
-#pragma unroll
-        for (int u = 0; u < U; ++u) load(u, k0 + warp * 32 + u * NT);
-        for (int base = k0 + warp * 32; base < k1; base += NT * U) {  // warp-uniform
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            if (base + u * NT >= k1) break;
-            const int k = base + u * NT + lane;
-            const float score = __int_as_float(*const_cast<volatile int*>(&s_bound[attempt]));
-            const float least = score * SLACK;
-            float v[N];
-            unpack<T>(raw[u], v);
-            bool hit = false;
-#pragma unroll
-            for (int c = 0; c < N; ++c) hit |= !(sc.weight(sc.diff(v[c], m)) * inv <= least * ns[u][c]);
-            if (__any_sync(0xffffffffu, hit)) {
-              const bool left = attempt == 0 && dr;
-              uint4 rawd;
-              if (left) rawd = load_pack<T, VEC>(dr, k, n);
-#pragma unroll
-              for (int c = 0; c < N; ++c) {
-                const int at = pack_index<T, VEC>(k, c);
-                float w = sc.weight_exact(sc.diff(v[c], m)) * inv;
-                if (left) w = fmaxf(w - draft_prob(as_f32(reinterpret_cast<const T*>(&rawd)[c]), sc, dl), 0.f);
-                if (attempt == 0 && at == struck) w = fmaxf(w - 1.f, 0.f);
-                const float ei = exponential(ns[u][c]);
-                if (w * best.e > best.w * ei) best = Best{w, ei, at};
-              }
-              const float reached = warp_max(best.w / best.e);
-              if (lane == 0 && reached > score) atomicMax(&s_bound[attempt], __float_as_int(reached));
-            }
-            load(u, base + (u + U) * NT);
-          }
-        }
-        best.merge_warp();
-        if (lane == 0) {
-          bw[warp] = best.w;
-          be[warp] = best.e;
-          bat[warp] = best.at;
-        }
-        __syncthreads();
-        if (attempt == 0) cl::cluster_wait();  // every CTA of the cluster runs
-        if (warp == 0) {
-          best.init();
-          if (lane < WARPS) best = Best{bw[lane], be[lane], bat[lane]};
-          best.merge_warp();
-          if (lane < ranks) {
-            cl::st_cluster_f32(cl::mapa(&cw[attempt][rank], lane), best.w);
-            cl::st_cluster_f32(cl::mapa(&ce[attempt][rank], lane), best.e);
-            cl::st_cluster_f32(cl::mapa(&cat[attempt][rank], lane), __int_as_float(best.at));
-          }
-        }
-        cl::cluster_sync();
-        if (warp == 0) {
-          best.init();
-          if (lane < ranks) best = Best{cw[attempt][lane], ce[attempt][lane], cat[attempt][lane]};
-          best.merge_warp();
-          if (lane == 0) s_winner = best.at;
-        }
-        __syncthreads();
-        winner = s_winner;
-        if (winner != NONE) break;
-      }
-    }
-    if (rank == 0 && tid == 0) {
-      tokens[i] = winner != NONE ? winner : -1;
-      logprobs[i] = winner != NONE ? sc.diff(as_f32(x[winner]), m) / sc.t - logf(s) : 0.f;
-    }
-    break;
+    if (run < TILE_ROWS) break;
+    __syncthreads();  // every row's draft was accepted: the next tile (it exists)
   }
   if (!waited) {
     pdl_wait();
     pdl_trigger();
   }
-  if (rank == 0) {
-    const int written = drafts < 0 ? 0 : count + 1;
-    for (int i = written + tid; i <= P.max_drafts; i += NT) {
+  if (chunk == 0) {
+    for (int i = (drafts < 0 ? 0 : count + 1) + tid; i <= P.max_drafts; i += DRAW_THREADS) {
       tokens[i] = -1;
       logprobs[i] = 0.f;
     }
     if (tid == 0) P.accepted[b] = count;
   }
+  if (drafts < 0) return;
+  // ---- the token after the accepted drafts: row `count`, row `run` of the last tile
+  const T* x = reinterpret_cast<const T*>(P.target) + (int64_t)(begin + count) * P.ld;
+  const Stats st = rows_s[run];
+  auto finish = [&](int winner) {
+    tokens[count] = winner != NONE ? winner : -1;
+    logprobs[count] = winner != NONE ? sc.diff(as_f32(x[winner]), st.m) / sc.t - logf(st.s) : 0.f;
+  };
+  if (sc.greedy || !(st.s > 0.f)) {
+    if (chunk == 0 && tid == 0) finish(st.s > 0.f ? st.at : NONE);
+    return;
+  }
+  const bool refused = count < drafts;
+  const T* dr = P.draft && refused ? reinterpret_cast<const T*>(P.draft) + b * P.d_sb + count * P.d_sd : nullptr;
+  const float dl = dr ? P.draft_lse[b * P.l_sb + count * P.l_sd] : 0.f;
+  const float* e = P.noise + b * P.ld_noise;
+  const int struck = !P.draft && refused ? id_at[run] : -1;  // a certain draft: q = 1 there
+  const int k0 = chunk * P.draw_packs;
+  if (tid == 0) s_known = (int)(*const_cast<volatile unsigned long long*>(P.best + b) >> 32);
+  __syncthreads();
+  unsigned long long word =
+      draw_share<T, VEC, DRAW_THREADS>(x, dr, e, P.n, k0, k0 + P.draw_packs, sc, st.m, st.s, dl, struck, &s_known);
+  if (lane == 0) words[warp] = word;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < WARPS; ++i) word = words[i] > word ? words[i] : word;
+    if (word) atomicMax(P.best + b, word);
+    __threadfence();
+    s_last = atomicAdd(P.done + b, 1u) == (unsigned)P.draw_chunks - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  word = *const_cast<volatile unsigned long long*>(P.best + b);
+  if (!word && refused) {  // nothing was left anywhere: the token is drawn from p
+    if (tid == 0) s_known = 0;
+    __syncthreads();
+    word = draw_share<T, VEC, DRAW_THREADS>(x, nullptr, e, P.n, 0, (int)cdiv(P.n, 32 * pack_n<T>()) * 32, sc, st.m, st.s,
+                                            0.f, -1, &s_known);
+    if (lane == 0) words[warp] = word;
+    __syncthreads();
+    for (int i = 0; i < WARPS; ++i) word = words[i] > word ? words[i] : word;
+  }
+  if (tid == 0) finish(word ? (int)~(unsigned)word : NONE);
 }
 
 // ---- launch ------------------------------------------------------------------------------------
-// CTAs per row or sequence: as many as fill the SMs' threads once (592 CTAs of 256; 512 in clusters of
-// 16, which have to fit a GPC), so that few rows still pull from all of HBM, but no less than 2,048
-// logits a CTA (below that the exchange costs more than the reading saves).  Up to 148 CTAs in all
-// take 1,024 threads each.
+// CTAs per row of the sampling kernel: as many as fill the SMs' threads once (592 CTAs of 256; 512 in
+// clusters of 16, which have to fit a GPC), so that few rows still pull from all of HBM, but no less
+// than 2,048 logits a CTA (below that the exchange costs more than the reading saves).  Up to 148
+// CTAs in all take 1,024 threads each.
 struct Split {
   int ctas;
   bool wide;
@@ -689,14 +749,28 @@ inline Split split_for(int64_t rows, int64_t vocab) {
   return {c, rows * c <= 148};
 }
 
-// Shares of a target row in the statistics kernel: 16 packets a thread, halved while the CTAs would
-// not fill the SMs twice.
-inline void stat_chunks(int64_t rows, int64_t vocab, int pack, int* chunks, int* packs) {
-  const int64_t all = cdiv(vocab, 32 * pack) * 32;
-  int per = 16;
-  while (per > 1 && rows * cdiv(all, per * STAT_THREADS) < 2 * 592) per /= 2;
-  *packs = per * STAT_THREADS;
-  *chunks = (int)cdiv(all, *packs);
+// Shares of a row in the verification kernels (256 threads, `resident` CTAs on the card at once): the
+// fewest waves that fill at least nine tenths of their CTAs, up to four, else the fullest; at least
+// one packet a thread.
+inline void row_shares(int64_t rows, int64_t vocab, int pack, int64_t resident, int* chunks, int* packs) {
+  const int64_t units = cdiv(vocab, 256 * pack);  // packets a thread of a lone CTA
+  int64_t best = 1;
+  double best_fill = 0;
+  for (int w = 1; w <= 4; ++w) {
+    int64_t c = rows > 0 ? w * resident / rows : 1;
+    c = c < 1 ? 1 : (c > units ? units : c);
+    const int64_t per = cdiv(units, c);
+    c = cdiv(units, per);
+    const double fill = (double)(rows * units) / (double)(cdiv(rows * c, resident) * resident * per);
+    if (fill > best_fill * 1.02) {
+      best_fill = fill;
+      best = c;
+    }
+    if (fill >= 0.9) break;
+  }
+  const int64_t per = cdiv(units, best);
+  *packs = (int)per * 256;
+  *chunks = (int)cdiv(units, per);
 }
 
 template <auto Kernel, typename... Args>
@@ -729,13 +803,24 @@ int sample_typed(int64_t rows, int64_t vocab, cudaStream_t st, const void* logit
 }
 template <typename T, bool VEC>
 int verify_typed(VerifyParams P, cudaStream_t st) {
-  if (P.total_q > 0) {
-    (void)ada::launch_k(row_stats_kernel<T, VEC>, dim3((unsigned)P.total_q * P.chunks), dim3(STAT_THREADS), 0, st, P);
-    ADA_CHECK_LAUNCH();
-  }
-  const Split sp = split_for(P.batch, P.n);
-  return sp.wide ? launch<judge_kernel<T, VEC, 1024>>(P.batch, sp, st, P)
-                 : launch<judge_kernel<T, VEC, 256>>(P.batch, sp, st, P);
+  const unsigned stat_ctas = (unsigned)P.total_q * P.chunks;
+  (void)ada::launch_k(row_stats_kernel<T, VEC>, dim3(stat_ctas ? stat_ctas : 1), dim3(STAT_THREADS), 0, st, P);
+  ADA_CHECK_LAUNCH();
+  (void)ada::launch_k(draw_kernel<T, VEC>, dim3((unsigned)P.batch * P.draw_chunks), dim3(DRAW_THREADS), 0, st, P);
+  ADA_CHECK_LAUNCH();
+  return ADA_OK;
+}
+
+// Workspace: the row statistics, then the draw's words.
+inline size_t verify_layout(VerifyParams& P, int64_t total_q, int64_t batch, int64_t vocab, int dtype, void* ws) {
+  const int pack = 16 / dtype_size(dtype);
+  row_shares(total_q, vocab, pack, 4 * 148, &P.chunks, &P.chunk_packs);
+  row_shares(batch, vocab, pack, 3 * 148, &P.draw_chunks, &P.draw_packs);
+  const size_t part = (size_t)total_q * P.chunks * sizeof(float4);
+  P.part = reinterpret_cast<float4*>(ws);
+  P.best = reinterpret_cast<unsigned long long*>(reinterpret_cast<char*>(ws) + part);
+  P.done = reinterpret_cast<unsigned int*>(P.best + batch);
+  return part + (size_t)batch * 12;
 }
 
 }  // namespace smp
@@ -766,11 +851,10 @@ extern "C" int ada_sample(const void* logits, int dtype, int64_t ld, int64_t row
 #undef ADA_SAMPLE
 }
 
-extern "C" size_t ada_verify_drafts_workspace_size(int32_t total_q, int64_t vocab, int dtype) {
-  if (total_q <= 0 || vocab <= 0 || !smp::dtype_ok(dtype)) return 0;
-  int chunks, packs;
-  smp::stat_chunks(total_q, vocab, 16 / smp::dtype_size(dtype), &chunks, &packs);
-  return (size_t)total_q * chunks * sizeof(float4);
+extern "C" size_t ada_verify_drafts_workspace_size(int32_t total_q, int32_t batch, int64_t vocab, int dtype) {
+  if (total_q < 0 || batch <= 0 || vocab <= 0 || !smp::dtype_ok(dtype)) return 0;
+  smp::VerifyParams P;
+  return smp::verify_layout(P, total_q, batch, vocab, dtype, nullptr);
 }
 
 extern "C" int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t total_q, int64_t vocab,
@@ -785,19 +869,21 @@ extern "C" int ada_verify_drafts(const void* target, int dtype, int64_t ld, int3
     return ADA_ERR_INVALID_ARG;
   if (batch == 0) return ADA_OK;
   if ((!target && total_q > 0) || (!input_ids && total_q > 0) || !cu_seqlens_q || !temperatures || !noise || !tokens ||
-      !accepted || !logprobs || (!uniforms && max_drafts > 0) || (!workspace && total_q > 0))
+      !accepted || !logprobs || (!uniforms && max_drafts > 0) || !workspace)
     return ADA_ERR_INVALID_ARG;
   if ((draft_logits == nullptr) != (draft_lse == nullptr)) return ADA_ERR_INVALID_ARG;
   if (draft_logits && (draft_stride_b < 0 || draft_stride_d < 0 || lse_stride_b < 0 || lse_stride_d < 0))
     return ADA_ERR_INVALID_ARG;
-  if (vocab > (1 << 30) || batch > (1 << 20) || max_drafts > 1024 || (int64_t)total_q * vocab > (1LL << 42)) return ADA_ERR_UNSUPPORTED;
+  if (vocab > (1 << 30) || batch > (1 << 20) || max_drafts > 1024) return ADA_ERR_UNSUPPORTED;
   if (smp::misaligned(target, dtype) || smp::misaligned(draft_logits, dtype) || ((uintptr_t)noise & 3) ||
       ((uintptr_t)temperatures & 3) || ((uintptr_t)uniforms & 3) || ((uintptr_t)draft_lse & 3) ||
       ((uintptr_t)input_ids & 7) || ((uintptr_t)cu_seqlens_q & 3) || ((uintptr_t)tokens & 7) ||
       ((uintptr_t)accepted & 3) || ((uintptr_t)logprobs & 3) || ((uintptr_t)workspace & 15))
     return ADA_ERR_ALIGNMENT;
-  if (workspace_bytes < ada_verify_drafts_workspace_size(total_q, vocab, dtype)) return ADA_ERR_WORKSPACE;
   smp::VerifyParams P;
+  if (workspace_bytes < smp::verify_layout(P, total_q, batch, vocab, dtype, workspace)) return ADA_ERR_WORKSPACE;
+  if ((int64_t)total_q * P.chunks > 0x7fffffff || (int64_t)batch * P.draw_chunks > 0x7fffffff)
+    return ADA_ERR_UNSUPPORTED;
   P.target = target;
   P.ld = ld;
   P.n = (int)vocab;
@@ -820,8 +906,6 @@ extern "C" int ada_verify_drafts(const void* target, int dtype, int64_t ld, int3
   P.tokens = tokens;
   P.accepted = accepted;
   P.logprobs = logprobs;
-  P.part = reinterpret_cast<float4*>(workspace);
-  smp::stat_chunks(total_q, vocab, 16 / smp::dtype_size(dtype), &P.chunks, &P.chunk_packs);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int size = smp::dtype_size(dtype);
   const bool vec = smp::on16(target, ld * size) && smp::on16(noise, ld_noise * 4) &&

@@ -58,8 +58,8 @@ def sample(logits: torch.Tensor, temperatures: torch.Tensor,
     return tokens, logprobs, lse
 
 
-def verify_workspace_bytes(total_q: int, vocab: int, dtype: torch.dtype) -> int:
-    return int(N.lib().ada_verify_drafts_workspace_size(total_q, vocab, N.DT_LOGITS[dtype]))
+def verify_workspace_bytes(total_q: int, batch: int, vocab: int, dtype: torch.dtype) -> int:
+    return int(N.lib().ada_verify_drafts_workspace_size(total_q, batch, vocab, N.DT_LOGITS[dtype]))
 
 
 def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -105,7 +105,7 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     if b == 0:
         return tokens, accepted, logprobs
     lib = N.lib()
-    need = lib.ada_verify_drafts_workspace_size(n, v, code)
+    need = lib.ada_verify_drafts_workspace_size(n, b, v, code)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=d)
     st = lib.ada_verify_drafts(

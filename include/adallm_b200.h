@@ -640,7 +640,7 @@ ADA_API int ada_sample(const void* logits, int dtype, int64_t ld, int64_t rows, 
  * workspace: ada_verify_drafts_workspace_size bytes, 16-byte aligned, no initial value; calls that
  * share one must be ordered.  Two launches.
  * ---------------------------------------------------------------------- */
-ADA_API size_t ada_verify_drafts_workspace_size(int32_t total_q, int64_t vocab, int dtype);
+ADA_API size_t ada_verify_drafts_workspace_size(int32_t total_q, int32_t batch, int64_t vocab, int dtype);
 ADA_API int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t total_q, int64_t vocab,
                               const int64_t* input_ids, const int32_t* cu_seqlens_q, int32_t batch,
                               int32_t max_drafts, const float* temperatures, const float* uniforms, int64_t ld_u,

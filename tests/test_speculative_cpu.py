@@ -72,8 +72,8 @@ def test_sample_argument_errors(lib):
 
 
 def test_verify_argument_errors(lib):
-    need = lib.ada_verify_drafts_workspace_size(10, 1000, 0)
-    assert need > 0 and lib.ada_verify_drafts_workspace_size(0, 1000, 0) == 0
+    need = lib.ada_verify_drafts_workspace_size(10, 4, 1000, 0)
+    assert need > 0 and lib.ada_verify_drafts_workspace_size(10, 0, 1000, 0) == 0
 
     def call(**kw):
         a = dict(x=P, dtype=0, ld=1000, total=10, vocab=1000, ids=P, cu=P, batch=4, most=3, temps=P, u=P, ld_u=3,
