@@ -8,20 +8,28 @@
 //   out = v_scale * sum_j p_j V_j,  p = softmax_j(scale * k_scale * q . K_j),
 //   j <= pos and (window W > 0) j > pos - W, holes of the block tables left out;
 // a row that sees no key is zeros.
+//
+// Work is cut into segments (a group's prefix, a sequence's own keys), a segment's (token, head of
+// the GQA group) rows into blocks, its keys into splits, and each piece gives a partial softmax
+// (maximum, sum, sum over V) in the workspace; a merge kernel joins a row's pieces.  What lies in a
+// piece is worked out on the device from the lengths, so a call can be captured in a graph and
+// follows the lengths it finds when it runs.
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace ada {
 namespace sp {
 
 constexpr int D = 128;
+constexpr int TILE = 16;              // keys of a tile: 16 rows of one page
+constexpr int TILE_BYTES = TILE * D;  // 16 keys x 128 e4m3 bytes
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr unsigned int ERR_TILE_WAIT = 0x90;
 
 struct Params {
   const void* q;
   int64_t q_st, q_sh;
-  const uint8_t* k;
-  const uint8_t* v;
-  int64_t s_page, s_tok, s_head, num_pages;
+  int64_t num_pages;
   const int32_t* pt;  // [groups][max_prefix_pages]
   int64_t pt_stride;
   int32_t max_prefix_pages;
@@ -33,14 +41,34 @@ struct Params {
   int32_t max_pages;
   const int32_t* ctx;
   const int32_t* cu_q;  // null: one row per sequence
-  int32_t batch, total_q, num_heads, group, page, window;
+  int32_t batch, total_q, num_heads, num_kv_heads, group, page, window;
   float scale_log2, v_scale;
   void* out;
   int64_t o_st, o_sh;
+  unsigned int* err;
+  // workspace
+  int32_t* plan;       // [0] tiles of a split, [1] splits before each segment ...
+  float* o_part;       // [piece][rows][D]
+  float2* ml_part;     // [piece][rows]: maximum (log2 units), sum
+  int32_t max_pieces;
 };
 
-// Number of entries of the ascending list cu[0..n] that are <= x, minus one: the interval
-// [cu[i], cu[i + 1]) that holds x (-1: before the first; n: past the last).
+// ---- metadata (lengths are cut to what the tables reach, row ranges to the rows there are) ----
+__device__ __forceinline__ int q_begin(const Params& P, int b) {
+  return P.cu_q ? max(0, min(__ldg(P.cu_q + b), P.total_q)) : b;
+}
+__device__ __forceinline__ int own_len(const Params& P, int b) {
+  return max(0, min(__ldg(P.ctx + b), P.max_pages * P.page));
+}
+__device__ __forceinline__ int prefix_len(const Params& P, int g) {
+  return max(0, min(__ldg(P.prefix_lens + g), P.max_prefix_pages * P.page));
+}
+__device__ __forceinline__ int group_begin(const Params& P, int g) {  // first sequence
+  return P.cu_groups ? max(0, min(__ldg(P.cu_groups + g), P.batch)) : g * P.batch;
+}
+
+// The interval [cu[i], cu[i + 1]) of the ascending list cu[0..n] that holds x (-1: before the first;
+// n: past the last).
 __device__ __forceinline__ int interval_of(const int32_t* cu, int n, int x) {
   int lo = 0, hi = n + 1;
   while (lo < hi) {
@@ -49,82 +77,519 @@ __device__ __forceinline__ int interval_of(const int32_t* cu, int n, int x) {
   }
   return lo - 1;
 }
+__device__ __forceinline__ int sequence_of(const Params& P, int n) {  // row n's, or -1
+  if (!P.cu_q) return n < P.batch ? n : -1;
+  const int b = interval_of(P.cu_q, P.batch, n);
+  return b < P.batch ? b : -1;
+}
+__device__ __forceinline__ int group_of(const Params& P, int b) {  // sequence b's, or -1
+  if (!P.cu_groups) return P.num_groups > 0 ? 0 : -1;
+  const int g = interval_of(P.cu_groups, P.num_groups, b);
+  return g < P.num_groups ? g : -1;
+}
 
-// One warp per (row, query head): 32 keys at a time, lane = key for the scores, lane = four
-// dimensions for the sum over V.
-template <typename TQ, typename TO>
-__global__ void __launch_bounds__(128) rows_kernel(Params P) {
+// A segment: rows [tok0, tok0 + tokens) x group heads over keys [k0, len) of a page list.
+struct Segment {
+  int tok0, tokens, k0, len;
+  __device__ __forceinline__ int tiles() const { return len > k0 ? (len - k0 + TILE - 1) / TILE : 0; }
+};
+__device__ __forceinline__ Segment prefix_segment(const Params& P, int g) {
+  Segment s;
+  const int b0 = group_begin(P, g), b1 = max(b0, group_begin(P, g + 1));
+  s.tok0 = q_begin(P, b0);
+  s.tokens = max(0, q_begin(P, b1) - s.tok0);
+  s.len = prefix_len(P, g);
+  // with a window: no row of the group stands before len - tokens, so none sees keys before this
+  s.k0 = P.window > 0 ? (max(0, s.len - s.tokens - P.window + 1) & ~(TILE - 1)) : 0;
+  if (s.tokens == 0) s.len = s.k0 = 0;
+  return s;
+}
+__device__ __forceinline__ Segment own_segment(const Params& P, int b) {
+  Segment s;
+  s.tok0 = q_begin(P, b);
+  s.tokens = max(0, q_begin(P, b + 1) - s.tok0);
+  s.len = own_len(P, b);
+  s.k0 = P.window > 0 ? (max(0, s.len - s.tokens - P.window + 1) & ~(TILE - 1)) : 0;
+  if (s.tokens == 0) s.len = s.k0 = 0;
+  return s;
+}
+
+// ---- pieces of few rows: one warp each, warp-level MMA --------------------------------------------
+// Bound: HBM.  A warp takes one piece (segment, block of 8 * NB rows, split, KV head) at a time, KV
+// head fastest, so that neighbouring warps read the heads of the same pages together.  It streams the
+// piece's tiles through its own ring of RING slots (TMA, 128-byte swizzle, one mbarrier a slot) and
+// computes S^T = K . Q^T (mma.m16n8k16, keys on M, rows on N), an online softmax per row and
+// O^T += V^T . P^T: the e4m3 tile is widened once for all NB row blocks.  Queries are taken as fp16
+// (bf16 values of 2^-14 to 65504 are exact), probabilities rounded to fp16 for P . V, statistics fp32.
+// For the K operand the head dimension is permuted so that lane (g, c) needs bytes [32c, 32c + 32) of
+// keys g and g + 8 (Q likewise); for V the output dimension so that it needs bytes [16g, 16g + 16) of
+// keys 2c, 2c + 1, 2c + 8, 2c + 9: 16-byte shared-memory reads, conflict-free through the swizzle.
+constexpr int RING = 4;
+constexpr int WARPS = 4;
+constexpr int MIN_TILES = 4;  // of a split: below, a piece's fixed cost outweighs its keys
+constexpr int RING_BYTES = RING * 2 * TILE_BYTES;
+
+__device__ __forceinline__ uint4 tile_ld16(const uint8_t* tile, int row, int chunk) {
+  return *reinterpret_cast<const uint4*>(tile + row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+
+// Tiles of a split: the fewest (>= MIN_TILES) with which the pieces do not exceed P.max_pieces, which
+// is one piece for every warp of the grid, or twice the (segment, row block, head) units where those
+// are more.  seg[s] = (tiles, row blocks).  Warp-wide.
+__device__ __forceinline__ int split_tiles(const int2* seg, int segs, int num_kv_heads, int max_pieces) {
+  const int lane = threadIdx.x & 31;
+  int most = 0;
+  for (int s = lane; s < segs; s += 32) most = max(most, seg[s].x);
+  most = __reduce_max_sync(0xffffffffu, most);
+  int lo = MIN_TILES, hi = max(most, MIN_TILES);  // hi fits: one split a unit
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    int64_t n = 0;
+    for (int s = lane; s < segs; s += 32) n += (int64_t)((seg[s].x + mid - 1) / mid) * seg[s].y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (n * num_kv_heads <= max_pieces) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
+template <typename TQ, int NB>
+__global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
+    pieces_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, Params P) {
+  using namespace sm100;
+  constexpr int ROWS = 8 * NB;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = base + warp * RING_BYTES;
+  const int segs = P.num_groups + P.batch;
+  int2* seg = reinterpret_cast<int2*>(base + WARPS * RING_BYTES);  // (tiles, row blocks) of each segment
+  int* first = reinterpret_cast<int*>(seg + segs);                 // splits before it
+  __shared__ uint64_t bars[WARPS][RING];
+  __shared__ __align__(16) __half p_s[WARPS][NB][8][16];
+  __shared__ int abort_flag, s_tiles, s_cut;
+  uint64_t* bar = bars[warp];
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    s_cut = P.window > 0;
+  }
+  if (lane < RING) mbar_init(&bar[lane], 1);
+  fence_mbar_init();
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
-  __shared__ float qs[4][D];
+
+  // ---- the plan, the same in every CTA
+  for (int s = threadIdx.x; s < segs; s += WARPS * 32) {
+    const Segment x = s < P.num_groups ? prefix_segment(P, s) : own_segment(P, s - P.num_groups);
+    seg[s] = make_int2(x.tiles(), (x.tokens * P.group + ROWS - 1) / ROWS);
+    if (s >= P.num_groups && x.len < x.tokens) s_cut = 1;  // rows inside the prefix: it needs a mask too
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const int ct = split_tiles(seg, segs, P.num_kv_heads, P.max_pieces);
+    int sum = 0;
+    for (int s0 = 0; s0 < segs; s0 += 32) {
+      const int s = s0 + lane;
+      const int n = s < segs ? (seg[s].x + ct - 1) / ct * seg[s].y : 0;
+      int acc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, acc, o);
+        if (lane >= o) acc += up;
+      }
+      if (s < segs) first[s] = sum + acc - n;
+      sum += __shfl_sync(0xffffffffu, acc, 31);
+    }
+    if (lane == 0) {
+      first[segs] = sum;
+      s_tiles = ct;
+    }
+  }
+  __syncthreads();
+  const int ct = s_tiles;
+  const bool cut = s_cut != 0;
+  if (blockIdx.x == 0) {  // for the merge
+    if (threadIdx.x == 0) P.plan[0] = ct;
+    for (int s = threadIdx.x; s <= segs; s += WARPS * 32) P.plan[1 + s] = first[s];
+  }
+  // (group lists that overlap could name more than the workspace holds)
+  const int64_t pieces = min((int64_t)first[segs] * P.num_kv_heads, (int64_t)P.max_pieces);
+  uint32_t uses = 0;  // tiles through the ring (slot = uses % RING, parity = (uses / RING) & 1)
+  for (int64_t piece = (int64_t)blockIdx.x * WARPS + warp; piece < pieces; piece += (int64_t)gridDim.x * WARPS) {
+    const int kvh = (int)(piece % P.num_kv_heads), flat = (int)(piece / P.num_kv_heads);
+    int lo_s = 0, hi_s = segs;  // the last segment with first[s] <= flat: it is not empty
+    while (hi_s - lo_s > 1) {
+      const int mid = (lo_s + hi_s) >> 1;
+      if (first[mid] <= flat) lo_s = mid; else hi_s = mid;
+    }
+    const int s = lo_s;
+    const bool pre = s < P.num_groups;
+    const Segment x = pre ? prefix_segment(P, s) : own_segment(P, s - P.num_groups);
+    const int splits = (seg[s].x + ct - 1) / ct;
+    const int rb = (flat - first[s]) / splits, sp = (flat - first[s]) % splits;
+    const int t_begin = x.k0 + sp * ct * TILE, t_end = min(x.len, t_begin + ct * TILE);
+    const int nt = (t_end - t_begin + TILE - 1) / TILE;
+    const int32_t* table = pre ? P.pt + (int64_t)s * P.pt_stride : P.bt + (int64_t)(s - P.num_groups) * P.bt_stride;
+
+    int my_block = -1, my_row0 = 0;  // lane j: page of tile j (mod 32), refilled every 32 tiles
+    auto look_up = [&](int from) {
+      my_block = -1;
+      if (from + lane < nt) {
+        const int key = t_begin + TILE * (from + lane);
+        const int at = key / P.page;
+        my_row0 = key - at * P.page;
+        my_block = __ldg(table + at);
+        if (my_block >= P.num_pages) my_block = -1;
+      }
+    };
+    auto issue = [&](int k, int blk, int row0) {
+      if (lane == 0) {
+        const uint32_t use = uses + k;
+        const int slot = use % RING;
+        if (blk >= 0) {
+          mbar_arrive_expect_tx(&bar[slot], 2 * TILE_BYTES);
+          tma_load_4d(ring + slot * 2 * TILE_BYTES, &tmk, &bar[slot], 0, kvh, row0, blk);
+          tma_load_4d(ring + slot * 2 * TILE_BYTES + TILE_BYTES, &tmv, &bar[slot], 0, kvh, row0, blk);
+        } else {
+          mbar_arrive_plain(&bar[slot]);  // a hole: nothing to load
+        }
+      }
+    };
+    look_up(0);
+    uint32_t ok_mask = __ballot_sync(0xffffffffu, my_block >= 0);  // of the 32 tiles looked up last
+    int looked = 0;
+    for (int k = 0; k < RING && k < nt; ++k)
+      issue(k, __shfl_sync(0xffffffffu, my_block, k), __shfl_sync(0xffffffffu, my_row0, k));
+
+    // ---- the rows: queries as the B operand (lane: row g of each block of 8, d in [32c, 32c + 32)),
+    // and the key range [lo, hi) of the rows 2c, 2c + 1 that this lane's scores belong to
+    uint32_t qf[NB][16];
+    int lo[NB][2], hi[NB][2], lo_max = 0, hi_min = 0x7fffffff;
+    const int rows = x.tokens * P.group;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int r = rb * ROWS + nb * 8 + g;
+      if (r < rows) {
+        const TQ* qp = reinterpret_cast<const TQ*>(P.q) + (int64_t)(x.tok0 + r / P.group) * P.q_st +
+                       (int64_t)(kvh * P.group + r % P.group) * P.q_sh + 32 * c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[8];
+          unpack8<TQ>(*reinterpret_cast<const uint4*>(qp + 8 * i), f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) qf[nb][4 * i + j] = pack_half2(f[2 * j], f[2 * j + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) qf[nb][i] = 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int re = rb * ROWS + nb * 8 + 2 * c + e;
+        int from = 0, to = x.len;
+        if (re < rows && (!pre || cut)) {
+          const int n = x.tok0 + re / P.group;
+          int pos;  // of the row, in this segment's key coordinates
+          if (pre) {
+            const int b = sequence_of(P, n);
+            pos = x.len + own_len(P, b) - (q_begin(P, b + 1) - n);
+          } else {
+            pos = x.len - (x.tok0 + x.tokens - n);
+          }
+          to = min(to, pos + 1);
+          if (P.window > 0) from = max(0, pos - P.window + 1);
+        }
+        lo[nb][e] = from;
+        hi[nb][e] = to;
+        lo_max = max(lo_max, from);
+        hi_min = min(hi_min, to);
+      }
+    }
+    lo_max = __reduce_max_sync(0xffffffffu, lo_max);
+    hi_min = __reduce_min_sync(0xffffffffu, hi_min);
+
+    float acc[NB][8][4], m[NB][2], l[NB][2];  // O^T fragments: d = 16g + 2mt (+1), rows 2c / 2c + 1
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[nb][i][0] = acc[nb][i][1] = acc[nb][i][2] = acc[nb][i][3] = 0.f;
+      m[nb][0] = m[nb][1] = -INFINITY;
+      l[nb][0] = l[nb][1] = 0.f;
+    }
+    bool failed = false;
+    for (int k = 0; k < nt; ++k) {
+      const uint32_t use = uses + k;
+      const int slot = use % RING;
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bar[slot], (use / RING) & 1, &abort_flag, P.err, ERR_TILE_WAIT))) {
+        failed = true;
+        break;
+      }
+      const bool there = (ok_mask >> (k & 31)) & 1;
+      const int tt = t_begin + TILE * k;
+      const uint8_t* kt = ring + slot * 2 * TILE_BYTES;
+      const uint8_t* vt = kt + TILE_BYTES;
+      uint4 kk[4], vv[4];
+      kk[0] = tile_ld16(kt, g, 2 * c);
+      kk[1] = tile_ld16(kt, g, 2 * c + 1);
+      kk[2] = tile_ld16(kt, g + 8, 2 * c);
+      kk[3] = tile_ld16(kt, g + 8, 2 * c + 1);
+      const int keys[4] = {2 * c, 2 * c + 1, 2 * c + 8, 2 * c + 9};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // rows of a hole or past the end may hold NaN: their weight is 0, V must be finite
+        vv[i] = (there && tt + keys[i] < x.len) ? tile_ld16(vt, keys[i], g) : make_uint4(0, 0, 0, 0);
+
+      float sc[NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+      const uint32_t* kg = reinterpret_cast<const uint32_t*>(kk);
+      const uint32_t* kg8 = reinterpret_cast<const uint32_t*>(kk + 2);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        uint32_t a[4];
+        a[0] = e4m3x2_to_f16x2((uint16_t)(kg[ks] & 0xFFFFu));
+        a[1] = e4m3x2_to_f16x2((uint16_t)(kg8[ks] & 0xFFFFu));
+        a[2] = e4m3x2_to_f16x2((uint16_t)(kg[ks] >> 16));
+        a[3] = e4m3x2_to_f16x2((uint16_t)(kg8[ks] >> 16));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma_16816_f16(sc[nb], a, &qf[nb][2 * ks]);
+      }
+      const bool whole = there && tt >= lo_max && tt + TILE <= hi_min;  // warp-uniform
+      const int tg = tt + g, tg8 = tt + g + 8;
+      uint32_t bp[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float s0 = sc[nb][0] * P.scale_log2, s1 = sc[nb][1] * P.scale_log2;    // key g,     rows 2c, 2c + 1
+        float s2 = sc[nb][2] * P.scale_log2, s3 = sc[nb][3] * P.scale_log2;    // key g + 8
+        if (!whole) {
+          s0 = there && tg >= lo[nb][0] && tg < hi[nb][0] ? s0 : -INFINITY;
+          s1 = there && tg >= lo[nb][1] && tg < hi[nb][1] ? s1 : -INFINITY;
+          s2 = there && tg8 >= lo[nb][0] && tg8 < hi[nb][0] ? s2 : -INFINITY;
+          s3 = there && tg8 >= lo[nb][1] && tg8 < hi[nb][1] ? s3 : -INFINITY;
+        }
+        float x0 = fmaxf(s0, s2), x1 = fmaxf(s1, s3);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
+        }
+        x0 = fmaxf(m[nb][0], x0);
+        x1 = fmaxf(m[nb][1], x1);
+        // nothing visible so far: against 0, so that no weight is NaN
+        const float z0 = x0 == -INFINITY ? 0.f : x0, z1 = x1 == -INFINITY ? 0.f : x1;
+        const float al0 = fast_exp2(m[nb][0] - z0), al1 = fast_exp2(m[nb][1] - z1);
+        const float p0 = fast_exp2(s0 - z0), p1 = fast_exp2(s1 - z1);
+        const float p2 = fast_exp2(s2 - z0), p3 = fast_exp2(s3 - z1);
+        m[nb][0] = x0;
+        m[nb][1] = x1;
+        l[nb][0] = l[nb][0] * al0 + (p0 + p2);
+        l[nb][1] = l[nb][1] * al1 + (p1 + p3);
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+          acc[nb][mt][0] *= al0;
+          acc[nb][mt][1] *= al1;
+          acc[nb][mt][2] *= al0;
+          acc[nb][mt][3] *= al1;
+        }
+        __half(*ps)[16] = p_s[warp][nb];  // P through shared memory: the B operand wants (key pairs, row g)
+        ps[2 * c][g] = __float2half_rn(p0);
+        ps[2 * c + 1][g] = __float2half_rn(p1);
+        ps[2 * c][g + 8] = __float2half_rn(p2);
+        ps[2 * c + 1][g + 8] = __float2half_rn(p3);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        bp[nb][0] = *reinterpret_cast<const uint32_t*>(&p_s[warp][nb][g][2 * c]);
+        bp[nb][1] = *reinterpret_cast<const uint32_t*>(&p_s[warp][nb][g][2 * c + 8]);
+      }
+      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0]);
+      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1]);
+      const uint32_t* v8 = reinterpret_cast<const uint32_t*>(&vv[2]);
+      const uint32_t* v9 = reinterpret_cast<const uint32_t*>(&vv[3]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t sel = half ? 0x7362u : 0x5140u;
+          const uint32_t lo01 = prmt(v0[j], v1[j], sel);
+          const uint32_t lo89 = prmt(v8[j], v9[j], sel);
+          uint32_t a[4];
+          a[0] = e4m3x2_to_f16x2((uint16_t)(lo01 & 0xFFFFu));
+          a[1] = e4m3x2_to_f16x2((uint16_t)(lo01 >> 16));
+          a[2] = e4m3x2_to_f16x2((uint16_t)(lo89 & 0xFFFFu));
+          a[3] = e4m3x2_to_f16x2((uint16_t)(lo89 >> 16));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma_16816_f16(acc[nb][2 * j + half], a, bp[nb]);
+        }
+      }
+      // every lane is done with the slot and with P: refill the slot with tile k + RING
+      __syncwarp();
+      const int nx = k + RING;
+      if (nx < nt) {
+        if ((nx & 31) == 0) look_up(nx);
+        const int blk = __shfl_sync(0xffffffffu, my_block, nx & 31);
+        const int row0 = __shfl_sync(0xffffffffu, my_row0, nx & 31);
+        if ((nx & 31) == 0) looked = nx;
+        if (lane == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        issue(nx, blk, row0);
+      }
+      // the mask of the next tile's block of 32 (its look-up is RING tiles old by then)
+      if (((k + 1) & 31) == 0 && looked == k + 1) ok_mask = __ballot_sync(0xffffffffu, my_block >= 0);
+    }
+    uses += nt;
+    const float poison = failed ? __int_as_float(0x7fc00000) : 0.f;  // a tile never came: the result is not valid
+
+    float2* ml = P.ml_part + piece * ROWS;
+    float* op = P.o_part + piece * ROWS * D;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float l0 = l[nb][0], l1 = l[nb][1];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+      }
+      const int r0 = nb * 8 + 2 * c;
+      if (rb * ROWS + r0 < rows) {
+        if (g == 0) ml[r0] = make_float2(m[nb][0] + poison, l0 + poison);
+        if (m[nb][0] != -INFINITY)
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt)
+            *reinterpret_cast<float2*>(op + r0 * D + 16 * g + 2 * mt) = make_float2(acc[nb][mt][0], acc[nb][mt][2]);
+      }
+      if (rb * ROWS + r0 + 1 < rows) {
+        if (g == 0) ml[r0 + 1] = make_float2(m[nb][1] + poison, l1 + poison);
+        if (m[nb][1] != -INFINITY)
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt)
+            *reinterpret_cast<float2*>(op + (r0 + 1) * D + 16 * g + 2 * mt) =
+                make_float2(acc[nb][mt][1], acc[nb][mt][3]);
+      }
+    }
+    if (failed) break;
+  }
+}
+
+// ---- merge: one warp per (row, head), four dimensions a lane --------------------------------------
+template <typename TO>
+__global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
+  pdl_wait();
+  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * 4 + warp;
   if (item >= (int64_t)P.total_q * P.num_heads) return;
   const int n = (int)(item / P.num_heads), h = (int)(item % P.num_heads);
   const int kvh = h / P.group;
-  const int b = P.cu_q ? interval_of(P.cu_q, P.batch, n) : n;
-  const bool live = b >= 0 && b < P.batch;
-  const int g = !live ? -1 : (P.cu_groups ? interval_of(P.cu_groups, P.num_groups, b) : 0);
-  const int len_p =
-      g >= 0 && g < P.num_groups ? max(0, min(__ldg(P.prefix_lens + g), P.max_prefix_pages * P.page)) : 0;
-  const int len_c = live ? max(0, min(__ldg(P.ctx + b), P.max_pages * P.page)) : 0;
-  const int pos = live ? len_p + len_c - (P.cu_q ? __ldg(P.cu_q + b + 1) - n : 1) : -1;
-  const int lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
-
-  const TQ* qp = reinterpret_cast<const TQ*>(P.q) + (int64_t)n * P.q_st + (int64_t)h * P.q_sh;
-  for (int d = lane; d < D; d += 32) qs[warp][d] = to_f32(qp[d]) * P.scale_log2;
-  __syncwarp();
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = lo; j0 <= pos; j0 += 32) {
-    const int j = j0 + lane;
-    int64_t at = -1;  // byte offset of key j's row, -1: not visible
-    if (j <= pos) {
-      const bool pre = j < len_p;
-      const int jj = pre ? j : j - len_p;
-      const int32_t* tab = pre ? P.pt + (int64_t)g * P.pt_stride : P.bt + (int64_t)b * P.bt_stride;
-      const int blk = __ldg(tab + jj / P.page);
-      if (blk >= 0 && blk < P.num_pages) at = blk * P.s_page + (jj % P.page) * P.s_tok + kvh * P.s_head;
-    }
-    float s = -INFINITY;
-    if (at >= 0) {
-      s = 0.f;
-      for (int c = 0; c < 8; ++c) {
-        const uint4 e = *reinterpret_cast<const uint4*>(P.k + at + 16 * c);
-        const uint32_t w[4] = {e.x, e.y, e.z, e.w};
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t f = e4m3x2_to_f16x2((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
-          const float2 kv = __half22float2(*reinterpret_cast<const __half2*>(&f));
-          s = fmaf(qs[warp][16 * c + 2 * i], kv.x, s);
-          s = fmaf(qs[warp][16 * c + 2 * i + 1], kv.y, s);
+  const int b = sequence_of(P, n);
+  const int g = b >= 0 ? group_of(P, b) : -1;
+  float M = -INFINITY, L = 0.f;
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  // pieces of segment s that hold this row, in order of their splits
+  auto join = [&](int s, const Segment& x) {
+    const int ct = P.plan[0], tiles = x.tiles();
+    const int splits = (tiles + ct - 1) / ct;
+    const int r = (n - x.tok0) * P.group + h % P.group;
+    const int64_t piece0 = ((int64_t)P.plan[1 + s] + (int64_t)(r / piece_rows) * splits) * P.num_kv_heads + kvh;
+    for (int s0 = 0; s0 < splits; s0 += 32) {
+      float2 ml = make_float2(-INFINITY, 0.f);
+      const int64_t mine = (piece0 + (int64_t)(s0 + lane) * P.num_kv_heads) * piece_rows + r % piece_rows;
+      if (s0 + lane < splits && mine < (int64_t)P.max_pieces * piece_rows) ml = P.ml_part[mine];
+      float most = ml.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      const float to = fmaxf(M, most);
+      if (to == -INFINITY && !__any_sync(0xffffffffu, ml.y != ml.y)) continue;
+      const float by = M == -INFINITY ? 0.f : fast_exp2(M - to);
+      M = to;
+      L *= by;
+      O.x *= by, O.y *= by, O.z *= by, O.w *= by;
+      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - to);
+      float add = ml.y * w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+      L += add;
+      const int count = min(32, splits - s0);
+#pragma unroll 4
+      for (int j = 0; j < count; ++j) {
+        const float wj = __shfl_sync(0xffffffffu, w, j);
+        const int64_t at = (piece0 + (int64_t)(s0 + j) * P.num_kv_heads) * piece_rows + r % piece_rows;
+        if (wj != 0.f) {  // (0 for a piece without a visible key, which holds no sum)
+          const float4 v = *reinterpret_cast<const float4*>(P.o_part + at * D + 4 * lane);
+          O.x = fmaf(v.x, wj, O.x);
+          O.y = fmaf(v.y, wj, O.y);
+          O.z = fmaf(v.z, wj, O.z);
+          O.w = fmaf(v.w, wj, O.w);
         }
       }
     }
-    float mx = s;
-    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    const float mn = fmaxf(m, mx);
-    if (mn == -INFINITY) continue;  // nothing visible so far
-    const float al = exp2f(m - mn), p = exp2f(s - mn);
-    m = mn;
-    l = l * al + p;
-    for (int i = 0; i < 4; ++i) o[i] *= al;
-    for (int t = 0; t < 32; ++t) {
-      const int64_t a = __shfl_sync(0xffffffffu, at, t);
-      const float pt = __shfl_sync(0xffffffffu, p, t);
-      if (a < 0) continue;
-      const uint32_t e = *reinterpret_cast<const uint32_t*>(P.v + a + 4 * lane);
-      const uint32_t f0 = e4m3x2_to_f16x2((uint16_t)e), f1 = e4m3x2_to_f16x2((uint16_t)(e >> 16));
-      const float2 v0 = __half22float2(*reinterpret_cast<const __half2*>(&f0));
-      const float2 v1 = __half22float2(*reinterpret_cast<const __half2*>(&f1));
-      o[0] = fmaf(pt, v0.x, o[0]);
-      o[1] = fmaf(pt, v0.y, o[1]);
-      o[2] = fmaf(pt, v1.x, o[2]);
-      o[3] = fmaf(pt, v1.y, o[3]);
-    }
+  };
+  if (b >= 0) {
+    if (g >= 0) join(g, prefix_segment(P, g));
+    join(P.num_groups + b, own_segment(P, b));
   }
-  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-  const float inv = l > 0.f ? P.v_scale / l : 0.f;
-  TO* op = reinterpret_cast<TO*>(P.out) + (int64_t)n * P.o_st + (int64_t)h * P.o_sh;
-  for (int i = 0; i < 4; ++i) op[4 * lane + i] = from_f32<TO>(o[i] * inv);
+  const float inv = L > 0.f ? P.v_scale / L : (L != L ? L : 0.f);  // a poisoned piece stays visible
+  TO* op = reinterpret_cast<TO*>(P.out) + (int64_t)n * P.o_st + (int64_t)h * P.o_sh + 4 * lane;
+  TO v[4] = {from_f32<TO>(O.x * inv), from_f32<TO>(O.y * inv), from_f32<TO>(O.z * inv), from_f32<TO>(O.w * inv)};
+  *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(v);
+}
+
+// ---- launch -----------------------------------------------------------------------------------------
+inline int sm_count() {
+  static std::atomic<int> sms[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = sms[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 0;
+    sms[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+template <auto Kernel>
+inline bool smem_ready(int bytes) {
+  static std::atomic<int> done[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (done[dev] >= bytes) return true;
+  if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared) !=
+          cudaSuccess)
+    return false;
+  done[dev] = bytes;
+  return true;
+}
+
+// Blocks of 8 rows that a warp takes together: what a sequence's rows fill on average, up to four.
+inline int row_blocks(int64_t total_q, int64_t batch, int64_t group) {
+  const int64_t rows = cdiv(total_q * group, batch);
+  return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4);
+}
+
+constexpr int MAX_SEGMENTS = 4096;
+constexpr int PIECES_PER_SM = 3 * WARPS;
+
+struct Layout {
+  int nb;
+  int64_t pieces;
+  size_t plan, ml, o, bytes;  // offsets of the workspace's parts, its size
+};
+inline Layout layout(int64_t total_q, int64_t groups, int64_t batch, int64_t heads, int64_t kv_heads) {
+  Layout y;
+  const int64_t group = heads / kv_heads;
+  y.nb = row_blocks(total_q, batch, group);
+  const int64_t rows = 8 * y.nb;
+  // every row lies in at most two segments (its prefix and its own keys)
+  const int64_t units = (2 * cdiv(total_q * group, rows) + groups + batch) * kv_heads;
+  y.pieces = units * 2 > 148 * PIECES_PER_SM ? units * 2 : 148 * PIECES_PER_SM;
+  auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
+  y.plan = 0;
+  y.ml = up((size_t)(groups + batch + 2) * sizeof(int32_t));
+  y.o = up(y.ml + (size_t)y.pieces * rows * sizeof(float2));
+  y.bytes = y.o + (size_t)y.pieces * rows * D * sizeof(float);
+  return y;
 }
 
 }  // namespace sp
@@ -135,8 +600,10 @@ using namespace ada;
 extern "C" size_t ada_fp8_shared_prefix_decode_workspace_size(int32_t total_q, int32_t num_groups, int32_t batch,
                                                               int32_t num_heads, int32_t num_kv_heads,
                                                               int32_t head_dim) {
-  if (total_q <= 0 || num_groups < 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
-  return 256;
+  if (total_q <= 0 || num_groups < 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      num_heads % num_kv_heads != 0)
+    return 0;
+  return sp::layout(total_q, num_groups, batch, num_heads, num_kv_heads).bytes;
 }
 
 extern "C" int ada_fp8_shared_prefix_decode(
@@ -161,6 +628,7 @@ extern "C" int ada_fp8_shared_prefix_decode(
   if (window < 0 || bt_stride < max_pages || pt_stride < max_prefix_pages || num_pages <= 0) return ADA_ERR_INVALID_ARG;
   if (!(scale * k_scale > 0.f)) return ADA_ERR_INVALID_ARG;  // row maxima are taken on unscaled scores
   if (head_dim != sp::D || page_size % 16 != 0 || num_heads / num_kv_heads > 128) return ADA_ERR_UNSUPPORTED;
+  if ((int64_t)num_groups + batch > sp::MAX_SEGMENTS) return ADA_ERR_UNSUPPORTED;
   if (((int64_t)max_pages + max_prefix_pages) * page_size > (1LL << 30)) return ADA_ERR_UNSUPPORTED;
   if ((int64_t)total_q * num_heads > (1LL << 30)) return ADA_ERR_UNSUPPORTED;
   if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return ADA_ERR_ALIGNMENT;
@@ -168,19 +636,13 @@ extern "C" int ada_fp8_shared_prefix_decode(
   if (((uintptr_t)q & 15) || (q_stride_t & 7) || (q_stride_h & 7)) return ADA_ERR_ALIGNMENT;
   if (((uintptr_t)out & 15) || (out_stride_t & 7) || (out_stride_h & 7)) return ADA_ERR_ALIGNMENT;
   if (((uintptr_t)workspace & 255) || ((uintptr_t)err & 3)) return ADA_ERR_ALIGNMENT;
-  if (workspace_bytes < ada_fp8_shared_prefix_decode_workspace_size(total_q, num_groups, batch, num_heads,
-                                                                    num_kv_heads, head_dim))
-    return ADA_ERR_WORKSPACE;
+  const sp::Layout y = sp::layout(total_q, num_groups, batch, num_heads, num_kv_heads);
+  if (workspace_bytes < y.bytes) return ADA_ERR_WORKSPACE;
 
   sp::Params P;
   P.q = q;
   P.q_st = q_stride_t;
   P.q_sh = q_stride_h;
-  P.k = k_cache;
-  P.v = v_cache;
-  P.s_page = kv_stride_page;
-  P.s_tok = kv_stride_tok;
-  P.s_head = kv_stride_head;
   P.num_pages = num_pages;
   P.pt = prefix_tables;
   P.pt_stride = pt_stride;
@@ -196,6 +658,7 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.batch = batch;
   P.total_q = total_q;
   P.num_heads = num_heads;
+  P.num_kv_heads = num_kv_heads;
   P.group = num_heads / num_kv_heads;
   P.page = page_size;
   P.window = window;
@@ -204,19 +667,45 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.out = out;
   P.o_st = out_stride_t;
   P.o_sh = out_stride_h;
-  const dim3 grid((unsigned)cdiv((int64_t)total_q * num_heads, 4));
+  P.err = err;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  P.plan = reinterpret_cast<int32_t*>(ws + y.plan);
+  P.ml_part = reinterpret_cast<float2*>(ws + y.ml);
+  P.o_part = reinterpret_cast<float*>(ws + y.o);
+  P.max_pieces = (int32_t)(y.pieces < 0x7fffffff ? y.pieces : 0x7fffffff);
+
+  // K / V caches as 4-D byte tensors [num_pages][page][Hkv][D] -> TMA box of 16 rows x 128 B
+  CUtensorMap tmk, tmv;
+  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)num_kv_heads, (cuuint64_t)page_size,
+                              (cuuint64_t)num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)kv_stride_head, (cuuint64_t)kv_stride_tok, (cuuint64_t)kv_stride_page};
+  const cuuint32_t box[4] = {(cuuint32_t)head_dim, 1, (cuuint32_t)sp::TILE, 1};
+  if (!sm100::encode_bytes(&tmk, k_cache, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !sm100::encode_bytes(&tmv, v_cache, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+    return ADA_ERR_CUDA;
+  const int sms = sp::sm_count();
+  if (!sms) return ADA_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int segs = num_groups + batch;
+  const int smem = 1024 + sp::WARPS * sp::RING_BYTES + segs * 12 + 4;
+#define ADA_SP(TQ, NB)                                                                                              \
+  do {                                                                                                              \
+    if (!sp::smem_ready<sp::pieces_kernel<TQ, NB>>(smem)) return ADA_ERR_CUDA;                                      \
+    (void)ada::launch_k(sp::pieces_kernel<TQ, NB>, dim3((unsigned)(sms * (NB == 4 ? 2 : 3))), dim3(sp::WARPS * 32), \
+                        smem, st, tmk, tmv, P);                                                                     \
+  } while (0)
   if (q_dtype == ADA_DT_BF16) {
-    if (out_dtype == ADA_DT_BF16)
-      (void)ada::launch_k(sp::rows_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, st, P);
-    else
-      (void)ada::launch_k(sp::rows_kernel<__nv_bfloat16, __half>, grid, dim3(128), 0, st, P);
+    if (y.nb == 1) ADA_SP(__nv_bfloat16, 1); else if (y.nb == 2) ADA_SP(__nv_bfloat16, 2); else ADA_SP(__nv_bfloat16, 4);
   } else {
-    if (out_dtype == ADA_DT_BF16)
-      (void)ada::launch_k(sp::rows_kernel<__half, __nv_bfloat16>, grid, dim3(128), 0, st, P);
-    else
-      (void)ada::launch_k(sp::rows_kernel<__half, __half>, grid, dim3(128), 0, st, P);
+    if (y.nb == 1) ADA_SP(__half, 1); else if (y.nb == 2) ADA_SP(__half, 2); else ADA_SP(__half, 4);
   }
+#undef ADA_SP
+  ADA_CHECK_LAUNCH();
+  const dim3 grid((unsigned)cdiv((int64_t)total_q * num_heads, 4));
+  if (out_dtype == ADA_DT_BF16)
+    (void)ada::launch_k(sp::merge_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, P, 8 * y.nb);
+  else
+    (void)ada::launch_k(sp::merge_kernel<__half>, grid, dim3(128), 0, st, P, 8 * y.nb);
   ADA_CHECK_LAUNCH();
   return ADA_OK;
 }
