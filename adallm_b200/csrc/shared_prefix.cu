@@ -51,6 +51,11 @@ struct Params {
   float* o_part;       // [piece][rows][D]
   float2* ml_part;     // [piece][rows]: maximum (log2 units), sum
   int32_t max_pieces;
+  int32_t prefix_tc;   // prefixes are taken by tc::prefix_kernel, not by pieces_kernel
+  int64_t* tc_plan;    // [0] blocks, [1] CTAs, then per group: blocks and units before it
+  float* tc_o;         // [unit + CTA][256 rows][D]
+  float2* tc_ml;       // [unit + CTA][256 rows]
+  int64_t tc_rows;     // rows of the two
 };
 
 // ---- metadata (lengths are cut to what the tables reach, row ranges to the rows there are) ----
@@ -177,13 +182,16 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
   if (lane < RING) mbar_init(&bar[lane], 1);
   fence_mbar_init();
   __syncthreads();
-  pdl_wait();
+  // Behind prefix_kernel, which has waited for its predecessors before it let this kernel start, all
+  // inputs are settled and nothing of prefix_kernel's is read: its end is waited for at the end.
+  if (!P.prefix_tc) pdl_wait();
   pdl_trigger();
 
   // ---- the plan, the same in every CTA
   for (int s = threadIdx.x; s < segs; s += WARPS * 32) {
     const Segment x = s < P.num_groups ? prefix_segment(P, s) : own_segment(P, s - P.num_groups);
-    seg[s] = make_int2(x.tiles(), (x.tokens * P.group + ROWS - 1) / ROWS);
+    const bool mine = s >= P.num_groups || !P.prefix_tc;
+    seg[s] = mine ? make_int2(x.tiles(), (x.tokens * P.group + ROWS - 1) / ROWS) : make_int2(0, 0);
     if (s >= P.num_groups && x.len < x.tokens) s_cut = 1;  // rows inside the prefix: it needs a mask too
   }
   __syncthreads();
@@ -470,7 +478,671 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
     }
     if (failed) break;
   }
+  if (P.prefix_tc) pdl_wait();  // so that the merge, which waits for this kernel, finds both done
 }
+
+// ---- prefixes under many rows: tcgen05 ---------------------------------------------------------------
+// Bound: the tensor cores, 4 * 128 flops for every (row, key).  A unit is 256 rows (two 128-row
+// tiles, the TMEM lanes) of one prefix and KV head over blocks of 128 keys; the blocks of all units are
+// laid end to end and every CTA takes an equal range, so a range covers the end of one unit, whole
+// ones and the start of another, each giving one partial (piece = unit + CTA index: one of the two
+// moves on from each piece to the next).
+//   S_t = Q_t . K^T  kind::f8f6f4 on the e4m3 bytes as they lie in the cache.  A query row is scaled by
+//     a power of two to a maximum in [128, 256) and written as a sum of e4m3 terms: a term keeps 4
+//     significant bits and what it leaves is exact, so two terms hold every bf16 value down to 2^-10 of
+//     the row's maximum exactly (three hold fp16), smaller ones to 2^-18 of it.  K is never widened
+//     and the terms cost what the fp16 product would.
+//   P  = 2^(S c - m) in fp16, written over S in TMEM, the A operand of
+//   O_t += P_t . V  kind::f16; V is widened to fp16 by four warps, once for both tiles.
+// Roles (14 warps): 0-3 widen V; 4-7 and 8-11 take tile 0's and tile 1's rows (thread = row: queries to
+// terms, softmax, O to the workspace); 12 loads (TMA, eight 16-key tiles a block for K and V each);
+// 13 issues the MMAs.  P.V of a block and S of the next are issued together for a tile, so one tile's
+// MMAs run under the other tile's softmax.  All tcgen05 operations come from one thread in order, so
+// s_full of block j + 1 also says that P.V of block j is complete: O may be rescaled.
+// Barriers, phase = use: k_full/k_empty (K slots), e_full/e_empty (e4m3 V slots), v_full/v_empty (fp16 V
+// slots), s_full[t], p_full[t] (a block's S, P of tile t), q_full[t], o_full[t] (a piece's Q, O).  A
+// tile's next S and its next P.V wait for q_full and p_full, which its warps give after they have
+// written the piece before.  Every wait is bounded and ends all roles through the abort flag.
+namespace tc {
+constexpr int BM = 128, BN = 128, TILES = 2, ROWS = TILES * BM;
+constexpr int THREADS = 14 * 32;
+constexpr int NE = 2, NV = 2;
+template <int TERMS> struct Smem {
+  static constexpr int NK = TERMS == 2 ? 3 : 2;
+  static constexpr int Q = 0;                            // [tile][term][128 rows][128 B]
+  static constexpr int K = Q + TILES * TERMS * 16384;    // e4m3 K slots [128 keys][128 B]
+  static constexpr int E = K + NK * 16384;               // e4m3 V slots
+  static constexpr int V = E + NE * 16384;               // fp16 V slots [2 halves of d][128 keys][128 B]
+  static constexpr int BAR = V + NV * 32768;
+  static constexpr int NBAR = 2 * NK + 2 * NE + 2 * NV + 4 * TILES + 1;
+  static constexpr int END = BAR + NBAR * 8 + NE * 4 + 8;
+  static constexpr int BYTES = 1024 + END;
+};
+static_assert(Smem<2>::BYTES <= 232448 && Smem<3>::BYTES <= 232448, "shared memory per CTA");
+constexpr uint32_t TMEM_COLS = 512;  // O of tile t at 128 t, S (then P) at 256 + 128 t
+constexpr float RESCALE_LOG2 = 8.f;  // move a row's reference only when its maximum grew by more than this
+constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);  // e4m3, f32 out
+constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(IDESC_S), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(IDESC_PV), "r"(accumulate)
+      : "memory");
+}
+// 32 consecutive fp32 columns of this thread's TMEM lane; valid after ld_wait.
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Wait for this thread's loads, then pin the registers behind the wait.
+__device__ __forceinline__ void ld_wait32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store8(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
+// try_wait with a suspend-time hint: waiting roles leave the issue slots to the working ones.
+__device__ __forceinline__ bool try_sleep(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(sm100::smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_b(uint64_t* bar, uint32_t use, volatile int* abort_v, unsigned int* err) {
+  const uint32_t parity = use & 1;
+  if (try_sleep(bar, parity)) return true;
+  const uint64_t t0 = sm100::globaltimer();
+  for (;;) {
+    if (try_sleep(bar, parity)) return true;
+    if (*abort_v) return false;
+    if (sm100::globaltimer() - t0 > 2000000000ull) {
+      *abort_v = 1;
+      if (err) atomicOr(err, ERR_TILE_WAIT);
+      return false;
+    }
+  }
+}
+// The same outcome in all lanes (the tcgen05 operations that follow are warp-collective).
+__device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t use, volatile int* abort_v, unsigned int* err) {
+  return __all_sync(0xffffffffu, wait_b(bar, use, abort_v, err));
+}
+
+// The blocks of one group: units (row block, KV head; head fastest) of `blocks` blocks each.
+__device__ __forceinline__ void group_shape(const Params& P, int g, Segment& x, int64_t& units, int& blocks) {
+  x = prefix_segment(P, g);
+  blocks = x.len > x.k0 ? (x.len - x.k0 + BN - 1) / BN : 0;
+  units = blocks ? cdiv((int64_t)x.tokens * P.group, ROWS) * P.num_kv_heads : 0;
+}
+
+// Walks a CTA's range of blocks piece by piece; every warp walks for itself, warp-wide.  32 groups at a
+// time are held in the lanes.
+struct Walk {
+  int64_t pos, end;        // blocks
+  int g0;                  // first group in the lanes
+  int64_t base, units0;    // blocks, units before it
+  int64_t size, before;    // this lane's group: blocks, blocks before it
+  int64_t units, ubefore;  // units, units before it
+  int blocks, tok0, tokens, k0, len;
+  // the piece
+  int g, rb, kvh, blk, n;
+  int64_t unit;
+
+  __device__ __forceinline__ void fill(const Params& P) {
+    const int lane = threadIdx.x & 31;
+    Segment x{0, 0, 0, 0};
+    units = 0;
+    blocks = 0;
+    if (g0 + lane < P.num_groups) group_shape(P, g0 + lane, x, units, blocks);
+    tok0 = x.tok0;
+    tokens = x.tokens;
+    k0 = x.k0;
+    len = x.len;
+    size = units * blocks;
+    before = size;
+    ubefore = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t a = __shfl_up_sync(0xffffffffu, before, o), b = __shfl_up_sync(0xffffffffu, ubefore, o);
+      if (lane >= o) {
+        before += a;
+        ubefore += b;
+      }
+    }
+    before += base - size;
+    ubefore += units0 - units;
+  }
+  __device__ __forceinline__ void begin(const Params& P) {
+    g0 = 0;
+    base = units0 = 0;
+    fill(P);
+  }
+  __device__ __forceinline__ void forward(const Params& P) {  // the next 32 groups
+    base = __shfl_sync(0xffffffffu, before + size, 31);
+    units0 = __shfl_sync(0xffffffffu, ubefore + units, 31);
+    g0 += 32;
+    fill(P);
+  }
+  // The next piece of [pos, end), or false.
+  __device__ __forceinline__ bool next(const Params& P, Segment& x) {
+    if (pos >= end) return false;
+    while (pos >= __shfl_sync(0xffffffffu, before + size, 31)) {
+      if (g0 >= P.num_groups) return false;
+      forward(P);
+    }
+    const int at = __ffs(__ballot_sync(0xffffffffu, pos < before + size)) - 1;
+    g = g0 + at;
+    const int64_t off = pos - __shfl_sync(0xffffffffu, before, at);
+    const int nb = __shfl_sync(0xffffffffu, blocks, at);
+    const int u = (int)(off / nb);
+    blk = (int)(off - (int64_t)u * nb);
+    n = (int)min((int64_t)(nb - blk), end - pos);
+    rb = u / P.num_kv_heads;
+    kvh = u - rb * P.num_kv_heads;
+    unit = __shfl_sync(0xffffffffu, ubefore, at) + u;
+    x.tok0 = __shfl_sync(0xffffffffu, tok0, at);
+    x.tokens = __shfl_sync(0xffffffffu, tokens, at);
+    x.k0 = __shfl_sync(0xffffffffu, k0, at);
+    x.len = __shfl_sync(0xffffffffu, len, at);
+    pos += n;
+    return true;
+  }
+};
+// CTA c of `ctas` takes blocks [c * total / ctas, (c + 1) * total / ctas).
+__device__ __forceinline__ int64_t range_begin(int64_t total, int64_t ctas, int64_t c) { return c * total / ctas; }
+__device__ __forceinline__ int64_t cta_of(int64_t total, int64_t ctas, int64_t block) {
+  return ((block + 1) * ctas - 1) / total;
+}
+
+template <typename TQ, int TERMS>
+__global__ void __launch_bounds__(THREADS, 1)
+    prefix_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, Params P) {
+  using namespace sm100;
+  using L = Smem<TERMS>;
+  constexpr int NK = L::NK;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(base + L::BAR);
+  uint64_t* k_empty = k_full + NK;
+  uint64_t* e_full = k_empty + NK;
+  uint64_t* e_empty = e_full + NE;
+  uint64_t* v_full = e_empty + NE;
+  uint64_t* v_empty = v_full + NV;
+  uint64_t* s_full = v_empty + NV;
+  uint64_t* p_full = s_full + TILES;
+  uint64_t* q_full = p_full + TILES;
+  uint64_t* o_full = q_full + TILES;
+  uint64_t* fin = o_full + TILES;
+  int* e_ok = reinterpret_cast<int*>(fin + 1);  // which of a V slot's page tiles are there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(e_ok + NE);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* abort_v = abort_flag;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < NE; ++i) {
+      mbar_init(&e_full[i], 1);
+      mbar_init(&e_empty[i], 4);
+    }
+    for (int i = 0; i < NV; ++i) {
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int t = 0; t < TILES; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&q_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    mbar_init(fin, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 13) tmem_alloc(tmem_slot, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  Walk w;
+  w.begin(P);
+  int64_t total, ctas;
+  {  // all blocks; the walk's lanes end up at the last 32 groups, so it starts again below
+    while (w.g0 + 32 < P.num_groups) w.forward(P);
+    total = __shfl_sync(0xffffffffu, w.before + w.size, 31);
+    ctas = min((int64_t)gridDim.x, total);
+    if (w.g0 > 0) w.begin(P);
+  }
+  if (blockIdx.x == 0) {  // for the merge: units and blocks before each group
+    if (threadIdx.x == 0) {
+      P.tc_plan[0] = total;
+      P.tc_plan[1] = ctas;
+    }
+    if (warp == 0) {
+      Walk a = w;
+      for (;;) {
+        if (a.g0 + lane < P.num_groups) {
+          P.tc_plan[2 + 2 * (a.g0 + lane)] = a.before;
+          P.tc_plan[3 + 2 * (a.g0 + lane)] = a.ubefore;
+        }
+        if (a.g0 + 32 >= P.num_groups) break;
+        a.forward(P);
+      }
+    }
+  }
+  const bool work = (int64_t)blockIdx.x < ctas;
+  w.pos = work ? range_begin(total, ctas, blockIdx.x) : 0;
+  w.end = work ? range_begin(total, ctas, blockIdx.x + 1) : 0;
+  Segment x;
+
+  if (warp < 4) {  // ---------------- V: e4m3 -> fp16 ----------------
+    const int ct = threadIdx.x;
+    uint32_t j = 0;
+    bool ok = true;
+    while (ok && w.next(P, x)) {
+      for (int i = 0; i < w.n; ++i, ++j) {
+        const int se = j % NE, sv = j % NV;
+        if (!wait_w(&e_full[se], j / NE, abort_v, P.err) ||
+            (j >= NV && !wait_w(&v_empty[sv], j / NV - 1, abort_v, P.err))) {
+          ok = false;
+          break;
+        }
+        const int key0 = x.k0 + (w.blk + i) * BN, there = e_ok[se];
+        const uint8_t* src = base + L::E + se * 16384;
+        uint8_t* dst = base + L::V + sv * 32768;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int id = ct + 128 * u, key = id >> 3, ch = id & 7;
+          uint4 e = *reinterpret_cast<const uint4*>(src + key * 128 + ((ch ^ (key & 7)) << 4));
+          // a hole or a row past the end may hold NaN: its weight is 0, V must be finite
+          if (!((there >> (key >> 4)) & 1) || key0 + key >= x.len) e = make_uint4(0, 0, 0, 0);
+          uint4 lo, hi;
+          lo.x = e4m3x2_to_f16x2((uint16_t)(e.x & 0xFFFFu));
+          lo.y = e4m3x2_to_f16x2((uint16_t)(e.x >> 16));
+          lo.z = e4m3x2_to_f16x2((uint16_t)(e.y & 0xFFFFu));
+          lo.w = e4m3x2_to_f16x2((uint16_t)(e.y >> 16));
+          hi.x = e4m3x2_to_f16x2((uint16_t)(e.z & 0xFFFFu));
+          hi.y = e4m3x2_to_f16x2((uint16_t)(e.z >> 16));
+          hi.z = e4m3x2_to_f16x2((uint16_t)(e.w & 0xFFFFu));
+          hi.w = e4m3x2_to_f16x2((uint16_t)(e.w >> 16));
+          uint8_t* d = dst + (ch >> 2) * 16384 + key * 128;
+          const int c0 = (ch & 3) * 2;
+          *reinterpret_cast<uint4*>(d + ((c0 ^ (key & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(d + (((c0 + 1) ^ (key & 7)) << 4)) = hi;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_plain(&v_full[sv]);
+          mbar_arrive_plain(&e_empty[se]);
+        }
+      }
+    }
+  } else if (warp < 12) {  // ---------------- rows: Q terms, softmax, O ----------------
+    const int t = (warp - 4) >> 2;
+    const int r = 32 * (warp & 3) + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_addr = tmem + lane_off + 256u + 128u * t, o_addr = tmem + lane_off + 128u * t;
+    uint32_t j = 0, piece = 0;
+    bool ok = true;
+    while (ok && w.next(P, x)) {
+      const int row = w.rb * ROWS + t * BM + r, rows = x.tokens * P.group;
+      if (w.rb * ROWS + t * BM >= rows) continue;  // the unit has no rows in this tile
+      const bool valid = row < rows;
+      const int n = x.tok0 + row / P.group;
+      // ---- the row's queries as e4m3 terms
+      float c = P.scale_log2;
+      {
+        uint4 raw[16];
+        const TQ* qp = reinterpret_cast<const TQ*>(P.q) + (int64_t)n * P.q_st +
+                       (int64_t)(w.kvh * P.group + row % P.group) * P.q_sh;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          raw[i] = valid ? *reinterpret_cast<const uint4*>(qp + 8 * i) : make_uint4(0, 0, 0, 0);
+        uint32_t most = 0;  // bits of the largest magnitude; infinities and NaN are the largest
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float f[8];
+          unpack8<TQ>(raw[i], f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) most = max(most, __float_as_uint(f[k]) & 0x7FFFFFFFu);
+        }
+        // 2^s with most * 2^s in [128, 256); tiny rows stop at 2^126
+        const int sh = most ? min(134 - (int)(most >> 23), 126) : 0;
+        const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
+        c = most < 0x7F800000u ? c * __uint_as_float((uint32_t)(127 - sh) << 23) : __int_as_float(0x7fc00000);
+        uint8_t* qd = base + L::Q + t * TERMS * 16384 + r * 128;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // 16 elements
+          float f[16];
+          unpack8<TQ>(raw[2 * i], f);
+          unpack8<TQ>(raw[2 * i + 1], f + 8);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) f[k] *= up;
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term) {
+            uint32_t out[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t a = f32x2_to_e4m3x2(f[4 * k], f[4 * k + 1]), b = f32x2_to_e4m3x2(f[4 * k + 2], f[4 * k + 3]);
+              out[k] = a | (b << 16);
+              if (term + 1 < TERMS) {
+                const uint32_t ha = e4m3x2_to_f16x2((uint16_t)a), hb = e4m3x2_to_f16x2((uint16_t)b);
+                const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&ha));
+                const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
+                f[4 * k] -= fa.x;
+                f[4 * k + 1] -= fa.y;
+                f[4 * k + 2] -= fb.x;
+                f[4 * k + 3] -= fb.y;
+              }
+            }
+            *reinterpret_cast<uint4*>(qd + term * 16384 + ((i ^ (r & 7)) << 4)) =
+                make_uint4(out[0], out[1], out[2], out[3]);
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_plain(&q_full[t]);
+      // ---- the keys that the row sees
+      int lo = 0, hi = 0;
+      if (valid) {
+        const int b = sequence_of(P, n);
+        const int pos = x.len + own_len(P, b) - (q_begin(P, b + 1) - n);
+        hi = min(x.len, pos + 1);
+        lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
+      }
+      const int32_t* table = P.pt + (int64_t)w.g * P.pt_stride;
+      const int tile0 = w.blk * (BN / TILE);  // of the piece's first block, from k0
+      auto entry = [&](int tile) {           // is the page of this lane's key tile there?
+        const int key = x.k0 + (tile0 + tile) * TILE;
+        if (tile >= w.n * (BN / TILE) || key >= x.len) return 0;
+        const int blk = __ldg(table + key / P.page);
+        return blk >= 0 && blk < P.num_pages ? 1 : 0;
+      };
+      int coming = entry(lane);
+      uint32_t there = 0;
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < w.n; ++i, ++j) {
+        if ((i & 3) == 0) {  // 32 key tiles = 4 blocks
+          there = __ballot_sync(0xffffffffu, coming != 0);
+          coming = entry(32 * (i / 4 + 1) + lane);
+        }
+        const uint32_t okb = (there >> (8 * (i & 3))) & 0xFFu;
+        const int key0 = x.k0 + (w.blk + i) * BN;
+        const int a = lo - key0, e = hi - key0;  // the row sees columns [a, e) of pages that are there
+        const bool whole = __all_sync(0xffffffffu, !valid || (okb == 0xFFu && a <= 0 && e >= BN));
+        if (!wait_w(&s_full[t], j, abort_v, P.err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float mx = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t sr[32];
+          ld32(s_addr + 32 * q, sr);
+          ld_wait32(sr);
+          float m0 = -INFINITY, m1 = -INFINITY;
+          if (whole) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              m0 = fmaxf(m0, __uint_as_float(sr[k]));
+              m1 = fmaxf(m1, __uint_as_float(sr[k + 1]));
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int col = 32 * q + k;
+              const bool vis = (col >= a) & (col < e) & (((okb >> (col >> 4)) & 1u) != 0);
+              m0 = fmaxf(m0, vis ? __uint_as_float(sr[k]) : -INFINITY);
+            }
+          }
+          mx = fmaxf(mx, fmaxf(m0, m1));
+        }
+        mx *= c;
+        // The reference of a row's O and l follows its maximum only when that grew by more than
+        // 2^RESCALE_LOG2: weights stay <= 2^8, exact enough in fp16, and O / l does not change.
+        float alpha = 1.f;
+        if (mx > m + RESCALE_LOG2 || (m == -INFINITY && mx != -INFINITY)) {
+          alpha = fast_exp2(m - mx);
+          m = mx;
+        }
+        const float ref = m != -INFINITY ? m : 0.f;
+        if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            uint32_t o[32];
+            ld32(o_addr + 32 * q, o);
+            ld_wait32(o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            st16(o_addr + 32 * q, o);
+            st16(o_addr + 32 * q + 16, o + 16);
+          }
+        }
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t sr[32], pk[16];
+          ld32(s_addr + 32 * q, sr);
+          ld_wait32(sr);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            float s0 = __uint_as_float(sr[k]), s1 = __uint_as_float(sr[k + 1]);
+            if (!whole) {
+              const int col = 32 * q + k;
+              const bool pg = ((okb >> (col >> 4)) & 1u) != 0;
+              s0 = ((col >= a) & (col < e) & pg) ? s0 : -INFINITY;
+              s1 = ((col + 1 >= a) & (col + 1 < e) & pg) ? s1 : -INFINITY;
+            }
+            const float p0 = fast_exp2(fmaf(s0, c, -ref)), p1 = fast_exp2(fmaf(s1, c, -ref));
+            l0 += p0;
+            l1 += p1;
+            pk[k >> 1] = pack_half2(p0, p1);
+          }
+          st16(s_addr + 16 * q, pk);  // over columns already read
+        }
+        l = l * alpha + (l0 + l1);
+        st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_plain(&p_full[t]);
+      }
+      // ---- the piece's partial
+      if (ok) ok = wait_w(&o_full[t], piece, abort_v, P.err);
+      ++piece;
+      tc_fence_after();
+      const int64_t at = (w.unit + blockIdx.x) * ROWS + t * BM + r;
+      if (at < P.tc_rows) {
+        if (valid) P.tc_ml[at] = ok ? make_float2(m, l) : make_float2(__int_as_float(0x7fc00000), 0.f);
+        float* op = P.tc_o + at * D;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          uint32_t o[32];
+          ld32(o_addr + 32 * q, o);
+          ld_wait32(o);
+          if (valid)
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) store8(op + 32 * q + k, reinterpret_cast<const float*>(o + k));
+        }
+      }
+      tc_fence_before();
+    }
+  } else if (warp == 12) {  // ---------------- loads ----------------
+    uint32_t j = 0;
+    bool ok = true;
+    while (ok && w.next(P, x)) {
+      const int32_t* table = P.pt + (int64_t)w.g * P.pt_stride;
+      const int tile0 = w.blk * (BN / TILE), tiles = w.n * (BN / TILE);
+      int blk = -1, row0 = 0, blk_n = -1, row_n = 0;  // lane: key tile of the current and the next 4 blocks
+      auto entry = [&](int tile, int& b, int& r) {
+        const int key = x.k0 + (tile0 + tile) * TILE;
+        b = -1;
+        r = 0;
+        if (tile >= tiles || key >= x.len) return;
+        const int at = key / P.page;
+        r = key - at * P.page;
+        b = __ldg(table + at);
+        if (b >= P.num_pages) b = -1;
+      };
+      entry(lane, blk_n, row_n);
+      for (int i = 0; i < w.n; ++i, ++j) {
+        if ((i & 3) == 0) {
+          blk = blk_n;
+          row0 = row_n;
+          entry(32 * (i / 4 + 1) + lane, blk_n, row_n);
+        }
+        const uint32_t there = (__ballot_sync(0xffffffffu, blk >= 0) >> (8 * (i & 3))) & 0xFFu;
+        const int sk = j % NK, se = j % NE;
+        int go = 1;
+        if (lane == 0)
+          go = !*abort_v && (j < NK || wait_b(&k_empty[sk], j / NK - 1, abort_v, P.err));
+        go = __shfl_sync(0xffffffffu, go, 0);
+        if (go) {
+          if (lane == 0) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive_expect_tx(&k_full[sk], __popc(there) * TILE_BYTES);
+          }
+          __syncwarp();
+          const int tile = lane - 8 * (i & 3);
+          if (tile >= 0 && tile < 8 && blk >= 0)
+            tma_load_4d(base + L::K + sk * 16384 + tile * TILE_BYTES, &tmk, &k_full[sk], 0, w.kvh, row0, blk);
+          if (lane == 0) go = j < NE || wait_b(&e_empty[se], j / NE - 1, abort_v, P.err);
+          go = __shfl_sync(0xffffffffu, go, 0);
+          if (go) {
+            if (lane == 0) {
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              e_ok[se] = (int)there;  // published by the arrive below
+              mbar_arrive_expect_tx(&e_full[se], __popc(there) * TILE_BYTES);
+            }
+            __syncwarp();
+            if (tile >= 0 && tile < 8 && blk >= 0)
+              tma_load_4d(base + L::E + se * 16384 + tile * TILE_BYTES, &tmv, &e_full[se], 0, w.kvh, row0, blk);
+          }
+        }
+        if (!go) {
+          ok = false;
+          break;
+        }
+      }
+    }
+    if (lane == 0 && *abort_v) {  // leave no copy in flight: wait (bounded) for the last uses of every slot
+      const uint64_t t0 = globaltimer();
+      for (int i = 0; i < NK + NE; ++i) {
+        uint64_t* bar = i < NK ? &k_full[i] : &e_full[i - NK];
+        const uint32_t ns = i < NK ? NK : NE, slot = i < NK ? i : i - NK;
+        if (j <= slot) continue;
+        const uint32_t use = (j - 1 - slot) / ns;
+        while (!mbar_try_wait(bar, use & 1) && globaltimer() - t0 < 1000000000ull) {
+        }
+      }
+    }
+  } else {  // ---------------- MMA (warp 13) ----------------
+    const uint32_t q_addr = smem_u32(base + L::Q), k_addr = smem_u32(base + L::K), v_addr = smem_u32(base + L::V);
+    uint32_t j = 0, piece[TILES] = {0, 0}, sj[TILES] = {0, 0};
+    bool ok = true;
+    auto issue_s = [&](int t, uint32_t jj) {
+      const uint32_t d = tmem + 256u + 128u * t, kb = k_addr + (jj % NK) * 16384u;
+#pragma unroll
+      for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_f8(d, desc_kmajor_sw128(q_addr + (t * TERMS + term) * 16384u + kk * 32u), desc_kmajor_sw128(kb + kk * 32u),
+                 term + kk > 0 ? 1u : 0u);
+      tc_commit(&s_full[t]);
+    };
+    while (ok && w.next(P, x)) {
+      const int tiles = w.rb * ROWS + BM < x.tokens * P.group ? 2 : 1;
+      if (lane == 0) {
+        ok = wait_b(&k_full[j % NK], j / NK, abort_v, P.err);
+        for (int t = 0; ok && t < tiles; ++t) {
+          ok = wait_b(&q_full[t], piece[t], abort_v, P.err);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(t, j);
+        }
+        if (ok) tc_commit(&k_empty[j % NK]);
+        for (int i = 0; ok && i < w.n; ++i, ++j) {
+          const bool more = i + 1 < w.n;
+          ok = (!more || wait_b(&k_full[(j + 1) % NK], (j + 1) / NK, abort_v, P.err)) &&
+               wait_b(&v_full[j % NV], j / NV, abort_v, P.err);
+          const uint32_t vb = v_addr + (j % NV) * 32768u;
+          for (int t = 0; ok && t < tiles; ++t) {
+            ok = wait_b(&p_full[t], sj[t], abort_v, P.err);
+            if (!ok) break;
+            ++sj[t];
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys each; V MN-major: d-halves 16 KB apart, 8-key groups 1 KB
+              mma_pv(tmem + 128u * t, tmem + 256u + 128u * t + 8u * kk, smem_desc(vb + kk * 2048u, 16384, 1024, SWZ_128B),
+                     (i > 0 || kk > 0) ? 1u : 0u);
+            if (more)
+              issue_s(t, j + 1);
+            else
+              tc_commit(&o_full[t]);
+          }
+          if (ok) {
+            tc_commit(&v_empty[j % NV]);
+            if (more) tc_commit(&k_empty[(j + 1) % NK]);
+          }
+        }
+        for (int t = 0; t < tiles; ++t) ++piece[t];
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      j = __shfl_sync(0xffffffffu, j, 0);
+    }
+    if (lane == 0) {  // everything issued has completed before the teardown
+      tc_commit(fin);
+      const uint64_t t0 = globaltimer();
+      while (!mbar_try_wait(fin, 0) && globaltimer() - t0 < 2000000000ull) {
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 13) tmem_dealloc(tmem, TMEM_COLS);
+}
+}  // namespace tc
 
 // ---- merge: one warp per (row, head), four dimensions a lane --------------------------------------
 template <typename TO>
@@ -486,21 +1158,17 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
   const int g = b >= 0 ? group_of(P, b) : -1;
   float M = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-  // pieces of segment s that hold this row, in order of their splits
-  auto join = [&](int s, const Segment& x) {
-    const int ct = P.plan[0], tiles = x.tiles();
-    const int splits = (tiles + ct - 1) / ct;
-    const int r = (n - x.tok0) * P.group + h % P.group;
-    const int64_t piece0 = ((int64_t)P.plan[1 + s] + (int64_t)(r / piece_rows) * splits) * P.num_kv_heads + kvh;
-    for (int s0 = 0; s0 < splits; s0 += 32) {
+  // `count` partials of this row, `step` rows apart from row0 on, in order
+  auto gather = [&](int count, int64_t row0, int64_t step, const float2* mls, const float* os, int64_t limit) {
+    for (int s0 = 0; s0 < count; s0 += 32) {
       float2 ml = make_float2(-INFINITY, 0.f);
-      const int64_t mine = (piece0 + (int64_t)(s0 + lane) * P.num_kv_heads) * piece_rows + r % piece_rows;
-      if (s0 + lane < splits && mine < (int64_t)P.max_pieces * piece_rows) ml = P.ml_part[mine];
+      const int64_t mine = row0 + (s0 + lane) * step;
+      if (s0 + lane < count && mine < limit) ml = mls[mine];
       float most = ml.x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       const float to = fmaxf(M, most);
-      if (to == -INFINITY && !__any_sync(0xffffffffu, ml.y != ml.y)) continue;
+      if (to == -INFINITY && !__any_sync(0xffffffffu, ml.x != ml.x)) continue;
       const float by = M == -INFINITY ? 0.f : fast_exp2(M - to);
       M = to;
       L *= by;
@@ -510,13 +1178,12 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
       L += add;
-      const int count = min(32, splits - s0);
+      const int here = min(32, count - s0);
 #pragma unroll 4
-      for (int j = 0; j < count; ++j) {
+      for (int j = 0; j < here; ++j) {
         const float wj = __shfl_sync(0xffffffffu, w, j);
-        const int64_t at = (piece0 + (int64_t)(s0 + j) * P.num_kv_heads) * piece_rows + r % piece_rows;
         if (wj != 0.f) {  // (0 for a piece without a visible key, which holds no sum)
-          const float4 v = *reinterpret_cast<const float4*>(P.o_part + at * D + 4 * lane);
+          const float4 v = *reinterpret_cast<const float4*>(os + (row0 + (s0 + j) * step) * D + 4 * lane);
           O.x = fmaf(v.x, wj, O.x);
           O.y = fmaf(v.y, wj, O.y);
           O.z = fmaf(v.z, wj, O.z);
@@ -525,8 +1192,30 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
       }
     }
   };
+  // the pieces of segment s that hold this row
+  auto join = [&](int s, const Segment& x) {
+    const int ct = P.plan[0], splits = (x.tiles() + ct - 1) / ct;
+    const int r = (n - x.tok0) * P.group + h % P.group;
+    const int64_t piece0 = ((int64_t)P.plan[1 + s] + (int64_t)(r / piece_rows) * splits) * P.num_kv_heads + kvh;
+    gather(splits, piece0 * piece_rows + r % piece_rows, (int64_t)P.num_kv_heads * piece_rows, P.ml_part, P.o_part,
+           (int64_t)P.max_pieces * piece_rows);
+  };
   if (b >= 0) {
-    if (g >= 0) join(g, prefix_segment(P, g));
+    if (g >= 0) {
+      const Segment x = prefix_segment(P, g);
+      if (!P.prefix_tc) {
+        join(g, x);
+      } else if (x.len > x.k0) {
+        const int blocks = (x.len - x.k0 + tc::BN - 1) / tc::BN;
+        const int r = (n - x.tok0) * P.group + h % P.group;
+        const int64_t total = P.tc_plan[0], ctas = P.tc_plan[1];
+        const int64_t unit = (int64_t)(r / tc::ROWS) * P.num_kv_heads + kvh;
+        const int64_t from = P.tc_plan[2 + 2 * g] + unit * blocks;
+        const int64_t c0 = tc::cta_of(total, ctas, from), c1 = tc::cta_of(total, ctas, from + blocks - 1);
+        const int64_t row0 = (P.tc_plan[3 + 2 * g] + unit + c0) * tc::ROWS + r % tc::ROWS;
+        gather((int)(c1 - c0 + 1), row0, tc::ROWS, P.tc_ml, P.tc_o, P.tc_rows);
+      }
+    }
     join(P.num_groups + b, own_segment(P, b));
   }
   const float inv = L > 0.f ? P.v_scale / L : (L != L ? L : 0.f);  // a poisoned piece stays visible
@@ -571,10 +1260,14 @@ inline int row_blocks(int64_t total_q, int64_t batch, int64_t group) {
 constexpr int MAX_SEGMENTS = 4096;
 constexpr int PIECES_PER_SM = 3 * WARPS;
 
+// Rows of a prefix and KV head from which the tensor-core kernel takes the prefixes.
+constexpr int64_t TC_ROWS = 33;
+
 struct Layout {
   int nb;
-  int64_t pieces;
-  size_t plan, ml, o, bytes;  // offsets of the workspace's parts, its size
+  bool tc;
+  int64_t pieces, tc_pieces;
+  size_t plan, tc_plan, ml, o, tc_ml, tc_o, bytes;  // offsets of the workspace's parts, its size
 };
 inline Layout layout(int64_t total_q, int64_t groups, int64_t batch, int64_t heads, int64_t kv_heads) {
   Layout y;
@@ -585,10 +1278,15 @@ inline Layout layout(int64_t total_q, int64_t groups, int64_t batch, int64_t hea
   const int64_t units = (2 * cdiv(total_q * group, rows) + groups + batch) * kv_heads;
   y.pieces = units * 2 > 148 * PIECES_PER_SM ? units * 2 : 148 * PIECES_PER_SM;
   auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
+  y.tc = groups > 0 && total_q * group >= TC_ROWS * groups;
+  y.tc_pieces = y.tc ? (cdiv(total_q * group, tc::ROWS) + groups) * kv_heads + 148 : 0;
   y.plan = 0;
-  y.ml = up((size_t)(groups + batch + 2) * sizeof(int32_t));
+  y.tc_plan = up((size_t)(groups + batch + 2) * sizeof(int32_t));
+  y.ml = up(y.tc_plan + (size_t)(2 * groups + 2) * sizeof(int64_t));
   y.o = up(y.ml + (size_t)y.pieces * rows * sizeof(float2));
-  y.bytes = y.o + (size_t)y.pieces * rows * D * sizeof(float);
+  y.tc_ml = up(y.o + (size_t)y.pieces * rows * D * sizeof(float));
+  y.tc_o = up(y.tc_ml + (size_t)y.tc_pieces * tc::ROWS * sizeof(float2));
+  y.bytes = y.tc_o + (size_t)y.tc_pieces * tc::ROWS * D * sizeof(float);
   return y;
 }
 
@@ -673,6 +1371,11 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.ml_part = reinterpret_cast<float2*>(ws + y.ml);
   P.o_part = reinterpret_cast<float*>(ws + y.o);
   P.max_pieces = (int32_t)(y.pieces < 0x7fffffff ? y.pieces : 0x7fffffff);
+  P.prefix_tc = y.tc ? 1 : 0;
+  P.tc_plan = reinterpret_cast<int64_t*>(ws + y.tc_plan);
+  P.tc_ml = reinterpret_cast<float2*>(ws + y.tc_ml);
+  P.tc_o = reinterpret_cast<float*>(ws + y.tc_o);
+  P.tc_rows = y.tc_pieces * sp::tc::ROWS;
 
   // K / V caches as 4-D byte tensors [num_pages][page][Hkv][D] -> TMA box of 16 rows x 128 B
   CUtensorMap tmk, tmv;
@@ -686,6 +1389,19 @@ extern "C" int ada_fp8_shared_prefix_decode(
   const int sms = sp::sm_count();
   if (!sms) return ADA_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (y.tc) {
+    const dim3 grid((unsigned)(sms < 148 ? sms : 148)), block(sp::tc::THREADS);
+    if (q_dtype == ADA_DT_BF16) {
+      constexpr int bytes = sp::tc::Smem<2>::BYTES;
+      if (!sp::smem_ready<sp::tc::prefix_kernel<__nv_bfloat16, 2>>(bytes)) return ADA_ERR_CUDA;
+      (void)ada::launch_k(sp::tc::prefix_kernel<__nv_bfloat16, 2>, grid, block, bytes, st, tmk, tmv, P);
+    } else {
+      constexpr int bytes = sp::tc::Smem<3>::BYTES;
+      if (!sp::smem_ready<sp::tc::prefix_kernel<__half, 3>>(bytes)) return ADA_ERR_CUDA;
+      (void)ada::launch_k(sp::tc::prefix_kernel<__half, 3>, grid, block, bytes, st, tmk, tmv, P);
+    }
+    ADA_CHECK_LAUNCH();
+  }
   const int segs = num_groups + batch;
   const int smem = 1024 + sp::WARPS * sp::RING_BYTES + segs * 12 + 4;
 #define ADA_SP(TQ, NB)                                                                                              \
