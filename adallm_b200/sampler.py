@@ -8,6 +8,8 @@
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import nn
 
@@ -51,13 +53,16 @@ def sample(logits: torch.Tensor, temperatures: torch.Tensor,
     lse = torch.empty(r, dtype=torch.float32, device=d)
     if r == 0:
         return tokens, logprobs, lse
+    stream = N.stream_ptr(d)
     st = N.lib().ada_sample(logits.data_ptr(), code, _ld(logits, r, v), r, v, temperatures.data_ptr(),
                             noise.data_ptr(), _ld(noise, r, v), tokens.data_ptr(), logprobs.data_ptr(),
-                            lse.data_ptr(), N.stream_ptr(d))
-    N.check(st, "sampling kernel")
+                            lse.data_ptr(), stream)
+    if st:
+        N.check(st, "sampling kernel")
     return tokens, logprobs, lse
 
 
+@functools.lru_cache(maxsize=512)
 def verify_workspace_bytes(total_q: int, batch: int, vocab: int, dtype: torch.dtype) -> int:
     return int(N.lib().ada_verify_drafts_workspace_size(total_q, batch, vocab, N.DT_LOGITS[dtype]))
 
@@ -74,6 +79,7 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     Exp(1); draft_logits [B, D, V] (target's dtype, any strides with unit stride in V) and
     draft_lse fp32 [B, D]: the logits each draft was drawn from and their log-normaliser at the
     sequence's temperature (``sample`` returns it); both None for drafts without a distribution.
+    workspace: at least verify_workspace_bytes(...) bytes (default: one kept per stream).
     Returns (tokens int64 [B, D + 1], accepted int32 [B], logprobs fp32 [B, D + 1]): the accepted
     drafts and the drawn token with their log-probabilities under the target, then -1 and 0."""
     N.require_cuda(target_logits, input_ids, cu_seqlens_q, temperatures, uniforms, noise, draft_logits, draft_lse,
@@ -104,17 +110,17 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     accepted = torch.empty(b, dtype=torch.int32, device=d)
     if b == 0:
         return tokens, accepted, logprobs
-    lib = N.lib()
-    need = lib.ada_verify_drafts_workspace_size(n, b, v, code)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=d)
-    st = lib.ada_verify_drafts(
+    stream = N.stream_ptr(d)
+    if workspace is None:
+        workspace = N.workspace(d, stream, verify_workspace_bytes(n, b, v, dtype))
+    st = N.lib().ada_verify_drafts(
         target_logits.data_ptr(), code, _ld(target_logits, n, v), n, v, input_ids.data_ptr(),
         cu_seqlens_q.data_ptr(), b, most, temperatures.data_ptr(), uniforms.data_ptr(), _ld(uniforms, b, most),
         noise.data_ptr(), _ld(noise, b, v), N.ptr(draft_logits), strides[0], strides[1], N.ptr(draft_lse), strides[2],
-        strides[3], tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), workspace.data_ptr(), need,
-        N.stream_ptr(d))
-    N.check(st, "draft verification kernel")
+        strides[3], tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), stream)
+    if st:
+        N.check(st, "draft verification kernel")
     return tokens, accepted, logprobs
 
 

@@ -7,15 +7,23 @@ reference has no such form: its decode reads a cached prefix once per sequence
 (adallm/ops/attention.py:359-414)."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native as N
 
 
+@functools.lru_cache(maxsize=512)
 def shared_prefix_workspace_bytes(total_q: int, num_groups: int, batch: int, num_heads: int, num_kv_heads: int,
                                   head_dim: int) -> int:
     return int(N.lib().ada_fp8_shared_prefix_decode_workspace_size(total_q, num_groups, batch, num_heads,
                                                                    num_kv_heads, head_dim))
+
+
+def _check_int32(t: torch.Tensor | None, name: str) -> None:
+    if t is not None and (t.dtype is not torch.int32 or (t.numel() > 1 and t.stride(-1) != 1)):
+        raise ValueError(f"{name} must be int32 with unit stride")
 
 
 def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_tables: torch.Tensor,
@@ -34,52 +42,59 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     cu_seqlens_q int32 [B + 1]: sequence b's rows of q are its newest tokens (None: one each).
     Row i of t attends to positions <= prefix + context - t + i, with window W > 0 to the last W
     of them.  Rows that see no key are zeros.
-    Returns [N, Hq, 128] in q.dtype.  err: optional int32 [1] device word; 0x90 is OR-ed in if a
+    Returns [N, Hq, 128] in q.dtype.  workspace: at least shared_prefix_workspace_bytes(...) bytes
+    (default: one kept per stream).  err: optional int32 [1] device word; 0x90 is OR-ed in if a
     tile wait ran out."""
     N.require_cuda(q, k_cache, v_cache, prefix_tables, prefix_lens, block_tables, context_lens, cu_groups,
                    cu_seqlens_q, out, workspace, err, what="shared_prefix_decode")
-    if q.dim() != 3 or k_cache.dim() != 4 or prefix_tables.dim() != 2 or block_tables.dim() != 2:
-        raise ValueError("shared_prefix_decode expects q [N, Hq, D], caches [pages, page, Hkv, D] and 2-D page tables")
     total_q, hq, d = q.shape
-    pages, page, hkv, dk = k_cache.shape
-    if q.dtype not in N.DT or (out is not None and out.dtype not in N.DT):
-        raise ValueError("q and out must be bf16 or fp16")
-    if dk != d or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride() or k_cache.stride(-1) != 1:
-        raise ValueError("k_cache and v_cache must share a [pages, page, Hkv, D] layout with q's head size")
-    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
-        raise ValueError("the shared-prefix decode reads a float8_e4m3fn cache")
-    for t, name in ((prefix_tables, "prefix_tables"), (prefix_lens, "prefix_lens"), (cu_groups, "cu_groups"),
-                    (block_tables, "block_tables"), (context_lens, "context_lens"), (cu_seqlens_q, "cu_seqlens_q")):
-        if t is not None and (t.dtype != torch.int32 or (t.numel() > 1 and t.stride(-1) != 1)):
-            raise ValueError(f"{name} must be int32 with unit stride")
-    groups, batch = prefix_lens.numel(), context_lens.numel()
-    if prefix_tables.shape[0] != groups or block_tables.shape[0] != batch:
-        raise ValueError("page tables must have one row per prefix and per sequence")
-    if (cu_groups is None and groups > 1) or (cu_groups is not None and cu_groups.numel() != groups + 1):
-        raise ValueError("cu_groups must hold the first sequence of each group and the end (None for one group)")
-    if cu_seqlens_q.numel() != batch + 1 if cu_seqlens_q is not None else total_q != batch:
-        raise ValueError("cu_seqlens_q must have batch + 1 entries (None for one row per sequence)")
+    pages, page, hkv, dk = shape = k_cache.shape
     if q.stride(-1) != 1:
         q = q.contiguous()
+    qs, ks = q.stride(), k_cache.stride()
+    code = N.DT.get(q.dtype)
+    if code is None or (out is not None and out.dtype not in N.DT):
+        raise ValueError("q and out must be bf16 or fp16")
+    if dk != d or shape != v_cache.shape or ks != v_cache.stride() or ks[3] != 1:
+        raise ValueError("k_cache and v_cache must share a [pages, page, Hkv, D] layout with q's head size")
+    if k_cache.dtype is not torch.float8_e4m3fn or v_cache.dtype is not torch.float8_e4m3fn:
+        raise ValueError("the shared-prefix decode reads a float8_e4m3fn cache")
+    _check_int32(prefix_tables, "prefix_tables")
+    _check_int32(prefix_lens, "prefix_lens")
+    _check_int32(cu_groups, "cu_groups")
+    _check_int32(block_tables, "block_tables")
+    _check_int32(context_lens, "context_lens")
+    _check_int32(cu_seqlens_q, "cu_seqlens_q")
+    groups, batch = prefix_lens.numel(), context_lens.numel()
+    (pt_rows, pt_pages), (bt_rows, bt_pages) = prefix_tables.shape, block_tables.shape
+    if pt_rows != groups or bt_rows != batch:
+        raise ValueError("page tables must have one row per prefix and per sequence")
+    if groups > 1 if cu_groups is None else cu_groups.numel() != groups + 1:
+        raise ValueError("cu_groups must hold the first sequence of each group and the end (None for one group)")
+    if total_q != batch if cu_seqlens_q is None else cu_seqlens_q.numel() != batch + 1:
+        raise ValueError("cu_seqlens_q must have batch + 1 entries (None for one row per sequence)")
+    device = q.device
     if out is None:
-        out = torch.empty((total_q, hq, d), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.stride(-1) != 1:
-        raise ValueError("out must have q's shape and unit stride in the head dimension")
+        out = torch.empty((total_q, hq, d), dtype=q.dtype, device=device)
+        os, out_code = (hq * d, d), code
+    else:
+        os, out_code = out.stride(), N.DT[out.dtype]
+        if out.shape != q.shape or os[2] != 1:
+            raise ValueError("out must have q's shape and unit stride in the head dimension")
     if total_q == 0:
         return out
     if batch == 0:
         return out.zero_()
-    lib = N.lib()
-    need = lib.ada_fp8_shared_prefix_decode_workspace_size(total_q, groups, batch, hq, hkv, d)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    st = lib.ada_fp8_shared_prefix_decode(
-        q.data_ptr(), N.DT[q.dtype], q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
-        k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), pages, prefix_tables.data_ptr(),
-        prefix_tables.stride(0), prefix_tables.shape[1], prefix_lens.data_ptr(), N.ptr(cu_groups), groups,
-        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
-        N.ptr(cu_seqlens_q), batch, total_q, hq, hkv, d, page, float(scale), float(k_scale), float(v_scale),
-        int(window), out.data_ptr(), N.DT[out.dtype], out.stride(0), out.stride(1), workspace.data_ptr(), need,
-        N.ptr(err), N.stream_ptr(q.device))
-    N.check(st, "shared-prefix decode attention")
+    stream = N.stream_ptr(device)
+    need = shared_prefix_workspace_bytes(total_q, groups, batch, hq, hkv, d)
+    if workspace is None:
+        workspace = N.workspace(device, stream, need)
+    st = N.lib().ada_fp8_shared_prefix_decode(
+        q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], pages,
+        prefix_tables.data_ptr(), prefix_tables.stride(0), pt_pages, prefix_lens.data_ptr(), N.ptr(cu_groups), groups,
+        block_tables.data_ptr(), block_tables.stride(0), bt_pages, context_lens.data_ptr(), N.ptr(cu_seqlens_q), batch,
+        total_q, hq, hkv, d, page, scale, k_scale, v_scale, window, out.data_ptr(), out_code, os[0], os[1],
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), N.ptr(err), stream)
+    if st:
+        N.check(st, "shared-prefix decode attention")
     return out
