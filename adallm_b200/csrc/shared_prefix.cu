@@ -494,19 +494,28 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
 //     and the terms cost what the fp16 product would.
 //   P  = 2^(S c - m) in fp16, written over S in TMEM, the A operand of
 //   O_t += P_t . V  kind::f16; V is widened to fp16 by four warps, once for both tiles.
-// Roles (14 warps): 0-3 widen V; 4-7 and 8-11 take tile 0's and tile 1's rows (thread = row: queries to
+// Roles (16 warps): 0-3 widen V; 4-7 and 8-11 take tile 0's and tile 1's rows (thread = row: queries to
 // terms, softmax, O to the workspace); 12 loads (TMA, eight 16-key tiles a block for K and V each);
-// 13 issues the MMAs.  P.V of a block and S of the next are issued together for a tile, so one tile's
+// 13 issues the MMAs; 14 walks the CTA's range and hands out its pieces.  The row warps take 192
+// registers a thread (a row of S at once), the others 64.  P.V of a block and S of the next are issued together for a tile, so one tile's
 // MMAs run under the other tile's softmax.  All tcgen05 operations come from one thread in order, so
 // s_full of block j + 1 also says that P.V of block j is complete: O may be rescaled.
-// Barriers, phase = use: k_full/k_empty (K slots), e_full/e_empty (e4m3 V slots), v_full/v_empty (fp16 V
-// slots), s_full[t], p_full[t] (a block's S, P of tile t), q_full[t], o_full[t] (a piece's Q, O).  A
+// Barriers, phase = use: d_full/d_empty (pieces), k_full/k_empty (K slots), e_full/e_empty (e4m3 V
+// slots), v_full/v_empty (fp16 V slots), s_full[t], p_full[t] (a block's S, P of tile t), q_full[t], o_full[t] (a piece's Q, O).  A
 // tile's next S and its next P.V wait for q_full and p_full, which its warps give after they have
 // written the piece before.  Every wait is bounded and ends all roles through the abort flag.
 namespace tc {
 constexpr int BM = 128, BN = 128, TILES = 2, ROWS = TILES * BM;
-constexpr int THREADS = 14 * 32;
-constexpr int NE = 2, NV = 2;
+constexpr int THREADS = 16 * 32;
+constexpr int NE = 2, NV = 2, ND = 2;
+constexpr int REGS_LAUNCH = 128, REGS_ROWS = 192, REGS_REST = 64;  // a thread: 4 * 128 = 2 * 192 + 2 * 64
+static_assert(2 * REGS_ROWS + 2 * REGS_REST <= 4 * REGS_LAUNCH, "registers of the block");
+// A piece: blocks [blk, blk + n) of a unit; n = 0: no more.
+struct Piece {
+  int tok0, tokens, k0, len;
+  int g, rb, kvh, blk;
+  int n, unit;
+};
 template <int TERMS> struct Smem {
   static constexpr int NK = TERMS == 2 ? 3 : 2;
   static constexpr int Q = 0;                            // [tile][term][128 rows][128 B]
@@ -514,8 +523,8 @@ template <int TERMS> struct Smem {
   static constexpr int E = K + NK * 16384;               // e4m3 V slots
   static constexpr int V = E + NE * 16384;               // fp16 V slots [2 halves of d][128 keys][128 B]
   static constexpr int BAR = V + NV * 32768;
-  static constexpr int NBAR = 2 * NK + 2 * NE + 2 * NV + 4 * TILES + 1;
-  static constexpr int END = BAR + NBAR * 8 + NE * 4 + 8;
+  static constexpr int NBAR = 2 * ND + 2 * NK + 2 * NE + 2 * NV + 4 * TILES + 1;
+  static constexpr int END = BAR + NBAR * 8 + ND * (int)sizeof(Piece) + NE * 4 + 8;
   static constexpr int BYTES = 1024 + END;
 };
 static_assert(Smem<2>::BYTES <= 232448 && Smem<3>::BYTES <= 232448, "shared memory per CTA");
@@ -571,6 +580,23 @@ __device__ __forceinline__ void store8(float* p, const float* v) {
                : "memory");
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
 // try_wait with a suspend-time hint: waiting roles leave the issue slots to the working ones.
 __device__ __forceinline__ bool try_sleep(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -607,8 +633,7 @@ __device__ __forceinline__ void group_shape(const Params& P, int g, Segment& x, 
   units = blocks ? cdiv((int64_t)x.tokens * P.group, ROWS) * P.num_kv_heads : 0;
 }
 
-// Walks a CTA's range of blocks piece by piece; every warp walks for itself, warp-wide.  32 groups at a
-// time are held in the lanes.
+// Walks a CTA's range of blocks piece by piece, warp-wide; 32 groups at a time are held in the lanes.
 struct Walk {
   int64_t pos, end;        // blocks
   int g0;                  // first group in the lanes
@@ -616,9 +641,6 @@ struct Walk {
   int64_t size, before;    // this lane's group: blocks, blocks before it
   int64_t units, ubefore;  // units, units before it
   int blocks, tok0, tokens, k0, len;
-  // the piece
-  int g, rb, kvh, blk, n;
-  int64_t unit;
 
   __device__ __forceinline__ void fill(const Params& P) {
     const int lane = threadIdx.x & 31;
@@ -655,35 +677,43 @@ struct Walk {
     g0 += 32;
     fill(P);
   }
-  // The next piece of [pos, end), or false.
-  __device__ __forceinline__ bool next(const Params& P, Segment& x) {
-    if (pos >= end) return false;
+  // The next piece of [pos, end).
+  __device__ __forceinline__ Piece next(const Params& P) {
+    Piece d{0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    if (pos >= end) return d;
     while (pos >= __shfl_sync(0xffffffffu, before + size, 31)) {
-      if (g0 >= P.num_groups) return false;
+      if (g0 >= P.num_groups) return d;
       forward(P);
     }
     const int at = __ffs(__ballot_sync(0xffffffffu, pos < before + size)) - 1;
-    g = g0 + at;
     const int64_t off = pos - __shfl_sync(0xffffffffu, before, at);
     const int nb = __shfl_sync(0xffffffffu, blocks, at);
     const int u = (int)(off / nb);
-    blk = (int)(off - (int64_t)u * nb);
-    n = (int)min((int64_t)(nb - blk), end - pos);
-    rb = u / P.num_kv_heads;
-    kvh = u - rb * P.num_kv_heads;
-    unit = __shfl_sync(0xffffffffu, ubefore, at) + u;
-    x.tok0 = __shfl_sync(0xffffffffu, tok0, at);
-    x.tokens = __shfl_sync(0xffffffffu, tokens, at);
-    x.k0 = __shfl_sync(0xffffffffu, k0, at);
-    x.len = __shfl_sync(0xffffffffu, len, at);
-    pos += n;
-    return true;
+    d.g = g0 + at;
+    d.blk = (int)(off - (int64_t)u * nb);
+    d.n = (int)min((int64_t)(nb - d.blk), end - pos);
+    d.rb = u / P.num_kv_heads;
+    d.kvh = u - d.rb * P.num_kv_heads;
+    d.unit = (int)__shfl_sync(0xffffffffu, ubefore, at) + u;
+    d.tok0 = __shfl_sync(0xffffffffu, tok0, at);
+    d.tokens = __shfl_sync(0xffffffffu, tokens, at);
+    d.k0 = __shfl_sync(0xffffffffu, k0, at);
+    d.len = __shfl_sync(0xffffffffu, len, at);
+    pos += d.n;
+    return d;
   }
 };
 // CTA c of `ctas` takes blocks [c * total / ctas, (c + 1) * total / ctas).
 __device__ __forceinline__ int64_t range_begin(int64_t total, int64_t ctas, int64_t c) { return c * total / ctas; }
 __device__ __forceinline__ int64_t cta_of(int64_t total, int64_t ctas, int64_t block) {
   return ((block + 1) * ctas - 1) / total;
+}
+
+template <int N> __device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 template <typename TQ, int TERMS>
@@ -695,7 +725,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(base + L::BAR);
+  uint64_t* d_full = reinterpret_cast<uint64_t*>(base + L::BAR);
+  uint64_t* d_empty = d_full + ND;
+  uint64_t* k_full = d_empty + ND;
   uint64_t* k_empty = k_full + NK;
   uint64_t* e_full = k_empty + NK;
   uint64_t* e_empty = e_full + NE;
@@ -706,11 +738,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* q_full = p_full + TILES;
   uint64_t* o_full = q_full + TILES;
   uint64_t* fin = o_full + TILES;
-  int* e_ok = reinterpret_cast<int*>(fin + 1);  // which of a V slot's page tiles are there
+  Piece* pieces = reinterpret_cast<Piece*>(fin + 1);
+  int* e_ok = reinterpret_cast<int*>(pieces + ND);  // which of a V slot's page tiles are there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(e_ok + NE);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* abort_v = abort_flag;
   if (threadIdx.x == 0) {
+    for (int i = 0; i < ND; ++i) {
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 14);
+    }
     for (int i = 0; i < NK; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -741,53 +778,36 @@ __global__ void __launch_bounds__(THREADS, 1)
   pdl_wait();
   pdl_trigger();
 
-  Walk w;
-  w.begin(P);
-  int64_t total, ctas;
-  {  // all blocks; the walk's lanes end up at the last 32 groups, so it starts again below
-    while (w.g0 + 32 < P.num_groups) w.forward(P);
-    total = __shfl_sync(0xffffffffu, w.before + w.size, 31);
-    ctas = min((int64_t)gridDim.x, total);
-    if (w.g0 > 0) w.begin(P);
-  }
-  if (blockIdx.x == 0) {  // for the merge: units and blocks before each group
-    if (threadIdx.x == 0) {
-      P.tc_plan[0] = total;
-      P.tc_plan[1] = ctas;
-    }
-    if (warp == 0) {
-      Walk a = w;
-      for (;;) {
-        if (a.g0 + lane < P.num_groups) {
-          P.tc_plan[2 + 2 * (a.g0 + lane)] = a.before;
-          P.tc_plan[3 + 2 * (a.g0 + lane)] = a.ubefore;
-        }
-        if (a.g0 + 32 >= P.num_groups) break;
-        a.forward(P);
-      }
-    }
-  }
-  const bool work = (int64_t)blockIdx.x < ctas;
-  w.pos = work ? range_begin(total, ctas, blockIdx.x) : 0;
-  w.end = work ? range_begin(total, ctas, blockIdx.x + 1) : 0;
-  Segment x;
+  // The next piece (number `d`) for a role's warp; n = 0 at the end or after an abort.
+  auto take = [&](uint32_t d) {
+    Piece x;
+    x.n = 0;
+    if (!wait_w(&d_full[d % ND], d / ND, abort_v, P.err)) return x;
+    x = pieces[d % ND];
+    __syncwarp();
+    if (lane == 0) mbar_arrive_plain(&d_empty[d % ND]);
+    return x;
+  };
 
   if (warp < 4) {  // ---------------- V: e4m3 -> fp16 ----------------
+    regs_down<REGS_REST>();
     const int ct = threadIdx.x;
     uint32_t j = 0;
     bool ok = true;
-    while (ok && w.next(P, x)) {
-      for (int i = 0; i < w.n; ++i, ++j) {
+    for (uint32_t d = 0; ok; ++d) {
+      const Piece x = take(d);
+      if (!x.n) break;
+      for (int i = 0; i < x.n; ++i, ++j) {
         const int se = j % NE, sv = j % NV;
         if (!wait_w(&e_full[se], j / NE, abort_v, P.err) ||
             (j >= NV && !wait_w(&v_empty[sv], j / NV - 1, abort_v, P.err))) {
           ok = false;
           break;
         }
-        const int key0 = x.k0 + (w.blk + i) * BN, there = e_ok[se];
+        const int key0 = x.k0 + (x.blk + i) * BN, there = e_ok[se];
         const uint8_t* src = base + L::E + se * 16384;
         uint8_t* dst = base + L::V + sv * 32768;
-#pragma unroll
+#pragma unroll 4
         for (int u = 0; u < 8; ++u) {
           const int id = ct + 128 * u, key = id >> 3, ch = id & 7;
           uint4 e = *reinterpret_cast<const uint4*>(src + key * 128 + ((ch ^ (key & 7)) << 4));
@@ -802,10 +822,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           hi.y = e4m3x2_to_f16x2((uint16_t)(e.z >> 16));
           hi.z = e4m3x2_to_f16x2((uint16_t)(e.w & 0xFFFFu));
           hi.w = e4m3x2_to_f16x2((uint16_t)(e.w >> 16));
-          uint8_t* d = dst + (ch >> 2) * 16384 + key * 128;
+          uint8_t* dd = dst + (ch >> 2) * 16384 + key * 128;
           const int c0 = (ch & 3) * 2;
-          *reinterpret_cast<uint4*>(d + ((c0 ^ (key & 7)) << 4)) = lo;
-          *reinterpret_cast<uint4*>(d + (((c0 + 1) ^ (key & 7)) << 4)) = hi;
+          *reinterpret_cast<uint4*>(dd + ((c0 ^ (key & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(dd + (((c0 + 1) ^ (key & 7)) << 4)) = hi;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -816,15 +836,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp < 12) {  // ---------------- rows: Q terms, softmax, O ----------------
+    regs_up<REGS_ROWS>();
     const int t = (warp - 4) >> 2;
     const int r = 32 * (warp & 3) + lane;  // row of the tile = TMEM lane
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t s_addr = tmem + lane_off + 256u + 128u * t, o_addr = tmem + lane_off + 128u * t;
-    uint32_t j = 0, piece = 0;
+    uint32_t j = 0, done = 0;
     bool ok = true;
-    while (ok && w.next(P, x)) {
-      const int row = w.rb * ROWS + t * BM + r, rows = x.tokens * P.group;
-      if (w.rb * ROWS + t * BM >= rows) continue;  // the unit has no rows in this tile
+    for (uint32_t d = 0; ok; ++d) {
+      const Piece x = take(d);
+      if (!x.n) break;
+      const int row = x.rb * ROWS + t * BM + r, rows = x.tokens * P.group;
+      if (x.rb * ROWS + t * BM >= rows) continue;  // the unit has no rows in this tile
       const bool valid = row < rows;
       const int n = x.tok0 + row / P.group;
       // ---- the row's queries as e4m3 terms
@@ -832,7 +855,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       {
         uint4 raw[16];
         const TQ* qp = reinterpret_cast<const TQ*>(P.q) + (int64_t)n * P.q_st +
-                       (int64_t)(w.kvh * P.group + row % P.group) * P.q_sh;
+                       (int64_t)(x.kvh * P.group + row % P.group) * P.q_sh;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           raw[i] = valid ? *reinterpret_cast<const uint4*>(qp + 8 * i) : make_uint4(0, 0, 0, 0);
@@ -889,24 +912,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         hi = min(x.len, pos + 1);
         lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
       }
-      const int32_t* table = P.pt + (int64_t)w.g * P.pt_stride;
-      const int tile0 = w.blk * (BN / TILE);  // of the piece's first block, from k0
-      auto entry = [&](int tile) {           // is the page of this lane's key tile there?
+      const int32_t* table = P.pt + (int64_t)x.g * P.pt_stride;
+      const int tile0 = x.blk * (BN / TILE);  // of the piece's first block, from k0
+      auto entry = [&](int tile) {            // is the page of this lane's key tile there?
         const int key = x.k0 + (tile0 + tile) * TILE;
-        if (tile >= w.n * (BN / TILE) || key >= x.len) return 0;
+        if (tile >= x.n * (BN / TILE) || key >= x.len) return 0;
         const int blk = __ldg(table + key / P.page);
         return blk >= 0 && blk < P.num_pages ? 1 : 0;
       };
       int coming = entry(lane);
       uint32_t there = 0;
       float m = -INFINITY, l = 0.f;
-      for (int i = 0; i < w.n; ++i, ++j) {
+      for (int i = 0; i < x.n; ++i, ++j) {
         if ((i & 3) == 0) {  // 32 key tiles = 4 blocks
           there = __ballot_sync(0xffffffffu, coming != 0);
           coming = entry(32 * (i / 4 + 1) + lane);
         }
         const uint32_t okb = (there >> (8 * (i & 3))) & 0xFFu;
-        const int key0 = x.k0 + (w.blk + i) * BN;
+        const int key0 = x.k0 + (x.blk + i) * BN;
         const int a = lo - key0, e = hi - key0;  // the row sees columns [a, e) of pages that are there
         const bool whole = __all_sync(0xffffffffu, !valid || (okb == 0xFFu && a <= 0 && e >= BN));
         if (!wait_w(&s_full[t], j, abort_v, P.err)) {
@@ -914,30 +937,31 @@ __global__ void __launch_bounds__(THREADS, 1)
           break;
         }
         tc_fence_after();
-        float mx = -INFINITY;
+        uint32_t sr[128];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ld32(s_addr + 32 * q, sr + 32 * q);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 128; ++k) asm volatile("" : "+r"(sr[k]));
+        if (!whole) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            // bit k: column 32 q + k is visible
+            const int from = min(max(a - 32 * q, 0), 32), to = min(max(e - 32 * q, 0), 32);
+            uint32_t vis = (to >= 32 ? 0xFFFFFFFFu : (1u << to) - 1u) & (from >= 32 ? 0u : 0xFFFFFFFFu << from);
+            vis &= ((okb >> (2 * q)) & 1u ? 0xFFFFu : 0u) | ((okb >> (2 * q + 1)) & 1u ? 0xFFFF0000u : 0u);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) sr[32 * q + k] = (vis >> k) & 1u ? sr[32 * q + k] : 0xFF800000u;
+          }
+        }
+        float mq[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint32_t sr[32];
-          ld32(s_addr + 32 * q, sr);
-          ld_wait32(sr);
-          float m0 = -INFINITY, m1 = -INFINITY;
-          if (whole) {
+          mq[q] = __uint_as_float(sr[q]);
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              m0 = fmaxf(m0, __uint_as_float(sr[k]));
-              m1 = fmaxf(m1, __uint_as_float(sr[k + 1]));
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int col = 32 * q + k;
-              const bool vis = (col >= a) & (col < e) & (((okb >> (col >> 4)) & 1u) != 0);
-              m0 = fmaxf(m0, vis ? __uint_as_float(sr[k]) : -INFINITY);
-            }
-          }
-          mx = fmaxf(mx, fmaxf(m0, m1));
+          for (int k = 4; k < 128; k += 4) mq[q] = fmaxf(mq[q], __uint_as_float(sr[k + q]));
         }
-        mx *= c;
+        const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * c;
         // The reference of a row's O and l follows its maximum only when that grew by more than
         // 2^RESCALE_LOG2: weights stay <= 2^8, exact enough in fp16, and O / l does not change.
         float alpha = 1.f;
@@ -946,6 +970,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           m = mx;
         }
         const float ref = m != -INFINITY ? m : 0.f;
+        const float2 c2 = make_float2(c, c), off = make_float2(-ref, -ref);
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float2 y =
+                fma2(make_float2(__uint_as_float(sr[32 * q + k]), __uint_as_float(sr[32 * q + k + 1])), c2, off);
+            const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+            sum = add2(sum, p);
+            pk[k >> 1] = pack_half2(p.x, p.y);
+          }
+          st16(s_addr + 16 * q, pk);  // over S, which is in registers
+        }
+        l = l * alpha + (sum.x + sum.y);
         if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
           for (int q = 0; q < 4; ++q) {
@@ -958,39 +998,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             st16(o_addr + 32 * q + 16, o + 16);
           }
         }
-        float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t sr[32], pk[16];
-          ld32(s_addr + 32 * q, sr);
-          ld_wait32(sr);
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            float s0 = __uint_as_float(sr[k]), s1 = __uint_as_float(sr[k + 1]);
-            if (!whole) {
-              const int col = 32 * q + k;
-              const bool pg = ((okb >> (col >> 4)) & 1u) != 0;
-              s0 = ((col >= a) & (col < e) & pg) ? s0 : -INFINITY;
-              s1 = ((col + 1 >= a) & (col + 1 < e) & pg) ? s1 : -INFINITY;
-            }
-            const float p0 = fast_exp2(fmaf(s0, c, -ref)), p1 = fast_exp2(fmaf(s1, c, -ref));
-            l0 += p0;
-            l1 += p1;
-            pk[k >> 1] = pack_half2(p0, p1);
-          }
-          st16(s_addr + 16 * q, pk);  // over columns already read
-        }
-        l = l * alpha + (l0 + l1);
         st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_plain(&p_full[t]);
       }
       // ---- the piece's partial
-      if (ok) ok = wait_w(&o_full[t], piece, abort_v, P.err);
-      ++piece;
+      if (ok) ok = wait_w(&o_full[t], done, abort_v, P.err);
+      ++done;
       tc_fence_after();
-      const int64_t at = (w.unit + blockIdx.x) * ROWS + t * BM + r;
+      const int64_t at = ((int64_t)x.unit + blockIdx.x) * ROWS + t * BM + r;
       if (at < P.tc_rows) {
         if (valid) P.tc_ml[at] = ok ? make_float2(m, l) : make_float2(__int_as_float(0x7fc00000), 0.f);
         float* op = P.tc_o + at * D;
@@ -1006,141 +1023,181 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       tc_fence_before();
     }
-  } else if (warp == 12) {  // ---------------- loads ----------------
-    uint32_t j = 0;
-    bool ok = true;
-    while (ok && w.next(P, x)) {
-      const int32_t* table = P.pt + (int64_t)w.g * P.pt_stride;
-      const int tile0 = w.blk * (BN / TILE), tiles = w.n * (BN / TILE);
-      int blk = -1, row0 = 0, blk_n = -1, row_n = 0;  // lane: key tile of the current and the next 4 blocks
-      auto entry = [&](int tile, int& b, int& r) {
-        const int key = x.k0 + (tile0 + tile) * TILE;
-        b = -1;
-        r = 0;
-        if (tile >= tiles || key >= x.len) return;
-        const int at = key / P.page;
-        r = key - at * P.page;
-        b = __ldg(table + at);
-        if (b >= P.num_pages) b = -1;
-      };
-      entry(lane, blk_n, row_n);
-      for (int i = 0; i < w.n; ++i, ++j) {
-        if ((i & 3) == 0) {
-          blk = blk_n;
-          row0 = row_n;
-          entry(32 * (i / 4 + 1) + lane, blk_n, row_n);
-        }
-        const uint32_t there = (__ballot_sync(0xffffffffu, blk >= 0) >> (8 * (i & 3))) & 0xFFu;
-        const int sk = j % NK, se = j % NE;
-        int go = 1;
-        if (lane == 0)
-          go = !*abort_v && (j < NK || wait_b(&k_empty[sk], j / NK - 1, abort_v, P.err));
-        go = __shfl_sync(0xffffffffu, go, 0);
-        if (go) {
+  } else {
+    regs_down<REGS_REST>();
+    if (warp == 12) {  // ---------------- loads ----------------
+      uint32_t j = 0;
+      bool ok = true;
+      for (uint32_t d = 0; ok; ++d) {
+        const Piece x = take(d);
+        if (!x.n) break;
+        const int32_t* table = P.pt + (int64_t)x.g * P.pt_stride;
+        const int tile0 = x.blk * (BN / TILE), tiles = x.n * (BN / TILE);
+        int blk = -1, row0 = 0, blk_n = -1, row_n = 0;  // lane: key tile of the current and the next 4 blocks
+        auto entry = [&](int tile, int& b, int& rr) {
+          const int key = x.k0 + (tile0 + tile) * TILE;
+          b = -1;
+          rr = 0;
+          if (tile >= tiles || key >= x.len) return;
+          const int at = key / P.page;
+          rr = key - at * P.page;
+          b = __ldg(table + at);
+          if (b >= P.num_pages) b = -1;
+        };
+        entry(lane, blk_n, row_n);
+        for (int i = 0; i < x.n; ++i, ++j) {
+          if ((i & 3) == 0) {
+            blk = blk_n;
+            row0 = row_n;
+            entry(32 * (i / 4 + 1) + lane, blk_n, row_n);
+          }
+          const uint32_t there = (__ballot_sync(0xffffffffu, blk >= 0) >> (8 * (i & 3))) & 0xFFu;
+          const int sk = j % NK, se = j % NE, tile = lane - 8 * (i & 3);
+          const bool mine = tile >= 0 && tile < 8 && blk >= 0;
+          ok = j < NK || wait_w(&k_empty[sk], j / NK - 1, abort_v, P.err);
+          if (!ok) break;
           if (lane == 0) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive_expect_tx(&k_full[sk], __popc(there) * TILE_BYTES);
           }
           __syncwarp();
-          const int tile = lane - 8 * (i & 3);
-          if (tile >= 0 && tile < 8 && blk >= 0)
-            tma_load_4d(base + L::K + sk * 16384 + tile * TILE_BYTES, &tmk, &k_full[sk], 0, w.kvh, row0, blk);
-          if (lane == 0) go = j < NE || wait_b(&e_empty[se], j / NE - 1, abort_v, P.err);
-          go = __shfl_sync(0xffffffffu, go, 0);
-          if (go) {
-            if (lane == 0) {
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              e_ok[se] = (int)there;  // published by the arrive below
-              mbar_arrive_expect_tx(&e_full[se], __popc(there) * TILE_BYTES);
-            }
-            __syncwarp();
-            if (tile >= 0 && tile < 8 && blk >= 0)
-              tma_load_4d(base + L::E + se * 16384 + tile * TILE_BYTES, &tmv, &e_full[se], 0, w.kvh, row0, blk);
-          }
-        }
-        if (!go) {
-          ok = false;
-          break;
-        }
-      }
-    }
-    if (lane == 0 && *abort_v) {  // leave no copy in flight: wait (bounded) for the last uses of every slot
-      const uint64_t t0 = globaltimer();
-      for (int i = 0; i < NK + NE; ++i) {
-        uint64_t* bar = i < NK ? &k_full[i] : &e_full[i - NK];
-        const uint32_t ns = i < NK ? NK : NE, slot = i < NK ? i : i - NK;
-        if (j <= slot) continue;
-        const uint32_t use = (j - 1 - slot) / ns;
-        while (!mbar_try_wait(bar, use & 1) && globaltimer() - t0 < 1000000000ull) {
-        }
-      }
-    }
-  } else {  // ---------------- MMA (warp 13) ----------------
-    const uint32_t q_addr = smem_u32(base + L::Q), k_addr = smem_u32(base + L::K), v_addr = smem_u32(base + L::V);
-    uint32_t j = 0, piece[TILES] = {0, 0}, sj[TILES] = {0, 0};
-    bool ok = true;
-    auto issue_s = [&](int t, uint32_t jj) {
-      const uint32_t d = tmem + 256u + 128u * t, kb = k_addr + (jj % NK) * 16384u;
-#pragma unroll
-      for (int term = 0; term < TERMS; ++term)
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          mma_f8(d, desc_kmajor_sw128(q_addr + (t * TERMS + term) * 16384u + kk * 32u), desc_kmajor_sw128(kb + kk * 32u),
-                 term + kk > 0 ? 1u : 0u);
-      tc_commit(&s_full[t]);
-    };
-    while (ok && w.next(P, x)) {
-      const int tiles = w.rb * ROWS + BM < x.tokens * P.group ? 2 : 1;
-      if (lane == 0) {
-        ok = wait_b(&k_full[j % NK], j / NK, abort_v, P.err);
-        for (int t = 0; ok && t < tiles; ++t) {
-          ok = wait_b(&q_full[t], piece[t], abort_v, P.err);
+          if (mine) tma_load_4d(base + L::K + sk * 16384 + tile * TILE_BYTES, &tmk, &k_full[sk], 0, x.kvh, row0, blk);
+          ok = j < NE || wait_w(&e_empty[se], j / NE - 1, abort_v, P.err);
           if (!ok) break;
-          tc_fence_after();
-          issue_s(t, j);
+          if (lane == 0) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            e_ok[se] = (int)there;  // published by the arrive below
+            mbar_arrive_expect_tx(&e_full[se], __popc(there) * TILE_BYTES);
+          }
+          __syncwarp();
+          if (mine) tma_load_4d(base + L::E + se * 16384 + tile * TILE_BYTES, &tmv, &e_full[se], 0, x.kvh, row0, blk);
         }
-        if (ok) tc_commit(&k_empty[j % NK]);
-        for (int i = 0; ok && i < w.n; ++i, ++j) {
-          const bool more = i + 1 < w.n;
-          ok = (!more || wait_b(&k_full[(j + 1) % NK], (j + 1) / NK, abort_v, P.err)) &&
-               wait_b(&v_full[j % NV], j / NV, abort_v, P.err);
-          const uint32_t vb = v_addr + (j % NV) * 32768u;
-          for (int t = 0; ok && t < tiles; ++t) {
-            ok = wait_b(&p_full[t], sj[t], abort_v, P.err);
-            if (!ok) break;
-            ++sj[t];
-            tc_fence_after();
+      }
+      if (lane == 0 && *abort_v) {  // leave no copy in flight: wait (bounded) for the last use of every slot
+        const uint64_t t0 = globaltimer();
+        for (int i = 0; i < NK + NE; ++i) {
+          uint64_t* bar = i < NK ? &k_full[i] : &e_full[i - NK];
+          const uint32_t ns = i < NK ? NK : NE, slot = i < NK ? i : i - NK;
+          if (j <= slot) continue;
+          const uint32_t use = (j - 1 - slot) / ns;
+          while (!mbar_try_wait(bar, use & 1) && globaltimer() - t0 < 1000000000ull) {
+          }
+        }
+      }
+    } else if (warp == 13) {  // ---------------- MMA ----------------
+      const uint32_t q_addr = smem_u32(base + L::Q), k_addr = smem_u32(base + L::K), v_addr = smem_u32(base + L::V);
+      uint32_t j = 0, piece[TILES] = {0, 0}, sj[TILES] = {0, 0};
+      bool ok = true;
+      auto issue_s = [&](int t, uint32_t jj) {
+        const uint32_t dd = tmem + 256u + 128u * t, kb = k_addr + (jj % NK) * 16384u;
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys each; V MN-major: d-halves 16 KB apart, 8-key groups 1 KB
-              mma_pv(tmem + 128u * t, tmem + 256u + 128u * t + 8u * kk, smem_desc(vb + kk * 2048u, 16384, 1024, SWZ_128B),
-                     (i > 0 || kk > 0) ? 1u : 0u);
-            if (more)
-              issue_s(t, j + 1);
-            else
-              tc_commit(&o_full[t]);
+        for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8(dd, desc_kmajor_sw128(q_addr + (t * TERMS + term) * 16384u + kk * 32u),
+                   desc_kmajor_sw128(kb + kk * 32u), term + kk > 0 ? 1u : 0u);
+        tc_commit(&s_full[t]);
+      };
+      for (uint32_t d = 0; ok; ++d) {
+        const Piece x = take(d);
+        if (!x.n) break;
+        const int tiles = x.rb * ROWS + BM < x.tokens * P.group ? 2 : 1;
+        if (lane == 0) {
+          ok = wait_b(&k_full[j % NK], j / NK, abort_v, P.err);
+          for (int t = 0; ok && t < tiles; ++t) {
+            ok = wait_b(&q_full[t], piece[t], abort_v, P.err);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(t, j);
           }
-          if (ok) {
-            tc_commit(&v_empty[j % NV]);
-            if (more) tc_commit(&k_empty[(j + 1) % NK]);
+          if (ok) tc_commit(&k_empty[j % NK]);
+          for (int i = 0; ok && i < x.n; ++i, ++j) {
+            const bool more = i + 1 < x.n;
+            ok = (!more || wait_b(&k_full[(j + 1) % NK], (j + 1) / NK, abort_v, P.err)) &&
+                 wait_b(&v_full[j % NV], j / NV, abort_v, P.err);
+            const uint32_t vb = v_addr + (j % NV) * 32768u;
+            for (int t = 0; ok && t < tiles; ++t) {
+              ok = wait_b(&p_full[t], sj[t], abort_v, P.err);
+              if (!ok) break;
+              ++sj[t];
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys; V MN-major: d-halves 16 KB apart, 8-key groups 1 KB
+                mma_pv(tmem + 128u * t, tmem + 256u + 128u * t + 8u * kk,
+                       smem_desc(vb + kk * 2048u, 16384, 1024, SWZ_128B), (i > 0 || kk > 0) ? 1u : 0u);
+              if (more)
+                issue_s(t, j + 1);
+              else
+                tc_commit(&o_full[t]);
+            }
+            if (ok) {
+              tc_commit(&v_empty[j % NV]);
+              if (more) tc_commit(&k_empty[(j + 1) % NK]);
+            }
           }
+          for (int t = 0; t < tiles; ++t) ++piece[t];
         }
-        for (int t = 0; t < tiles; ++t) ++piece[t];
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      j = __shfl_sync(0xffffffffu, j, 0);
-    }
-    if (lane == 0) {  // everything issued has completed before the teardown
-      tc_commit(fin);
-      const uint64_t t0 = globaltimer();
-      while (!mbar_try_wait(fin, 0) && globaltimer() - t0 < 2000000000ull) {
+      if (lane == 0) {  // everything issued has completed before the teardown
+        tc_commit(fin);
+        const uint64_t t0 = globaltimer();
+        while (!mbar_try_wait(fin, 0) && globaltimer() - t0 < 2000000000ull) {
+        }
+      }
+      __syncwarp();
+    } else if (warp == 14) {  // ---------------- pieces ----------------
+      Walk w;
+      w.begin(P);
+      while (w.g0 + 32 < P.num_groups) w.forward(P);
+      const int64_t total = __shfl_sync(0xffffffffu, w.before + w.size, 31);
+      const int64_t ctas = min((int64_t)gridDim.x, total);
+      if (w.g0 > 0) w.begin(P);
+      const bool work = (int64_t)blockIdx.x < ctas;
+      w.pos = work ? range_begin(total, ctas, blockIdx.x) : 0;
+      w.end = work ? range_begin(total, ctas, blockIdx.x + 1) : 0;
+      for (uint32_t d = 0;; ++d) {
+        const Piece x = w.next(P);
+        if (d >= ND && !wait_w(&d_empty[d % ND], d / ND - 1, abort_v, P.err)) break;
+        if (lane == 0) {
+          pieces[d % ND] = x;
+          mbar_arrive_plain(&d_full[d % ND]);
+        }
+        if (!x.n) break;
+      }
+      if (blockIdx.x == 0) {  // for the merge: blocks, CTAs, and before each group blocks and units
+        if (lane == 0) {
+          P.tc_plan[0] = total;
+          P.tc_plan[1] = ctas;
+        }
+        for (w.begin(P);; w.forward(P)) {
+          if (w.g0 + lane < P.num_groups) {
+            P.tc_plan[2 + 2 * (w.g0 + lane)] = w.before;
+            P.tc_plan[3 + 2 * (w.g0 + lane)] = w.ubefore;
+          }
+          if (w.g0 + 32 >= P.num_groups) break;
+        }
       }
     }
-    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == 13) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// The row warps wait for registers that the others give back: only what the block was launched with is
+// there, so the compiled kernel has to come with REGS_LAUNCH a thread.
+template <auto Kernel>
+inline bool registers_ready() {
+  static std::atomic<int> ok{-1};
+  int v = ok;
+  if (v < 0) {
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, Kernel) != cudaSuccess) return false;
+    ok = v = a.numRegs >= REGS_LAUNCH ? 1 : 0;
+  }
+  return v == 1;
 }
 }  // namespace tc
 
@@ -1393,10 +1450,12 @@ extern "C" int ada_fp8_shared_prefix_decode(
     const dim3 grid((unsigned)(sms < 148 ? sms : 148)), block(sp::tc::THREADS);
     if (q_dtype == ADA_DT_BF16) {
       constexpr int bytes = sp::tc::Smem<2>::BYTES;
+      if (!sp::tc::registers_ready<sp::tc::prefix_kernel<__nv_bfloat16, 2>>()) return ADA_ERR_UNSUPPORTED;
       if (!sp::smem_ready<sp::tc::prefix_kernel<__nv_bfloat16, 2>>(bytes)) return ADA_ERR_CUDA;
       (void)ada::launch_k(sp::tc::prefix_kernel<__nv_bfloat16, 2>, grid, block, bytes, st, tmk, tmv, P);
     } else {
       constexpr int bytes = sp::tc::Smem<3>::BYTES;
+      if (!sp::tc::registers_ready<sp::tc::prefix_kernel<__half, 3>>()) return ADA_ERR_UNSUPPORTED;
       if (!sp::smem_ready<sp::tc::prefix_kernel<__half, 3>>(bytes)) return ADA_ERR_CUDA;
       (void)ada::launch_k(sp::tc::prefix_kernel<__half, 3>, grid, block, bytes, st, tmk, tmv, P);
     }
