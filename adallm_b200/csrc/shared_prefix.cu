@@ -533,18 +533,21 @@ constexpr float RESCALE_LOG2 = 8.f;  // move a row's reference only when its max
 constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);  // e4m3, f32 out
 constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+// Descriptors are passed by their low words (address and leading offset); the high words are the same
+// for all operands here (1024 bytes between 8-row groups, 128-byte swizzle).
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | ((uint32_t)sm100::SWZ_128B << 29);
+template <bool ACC> __device__ __forceinline__ void mma_f8(uint32_t d, uint32_t a_lo, uint32_t b_lo) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(IDESC_S), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(DESC_HI), "r"(IDESC_S), "n"(ACC ? 1 : 0)
       : "memory");
 }
-__device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t accumulate) {
+template <bool ACC> __device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a_tmem, uint32_t b_lo) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "l"(b), "r"(IDESC_PV), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(DESC_HI), "r"(IDESC_PV), "n"(ACC ? 1 : 0)
       : "memory");
 }
 // 32 consecutive fp32 columns of this thread's TMEM lane; valid after ld_wait.
@@ -597,22 +600,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
-// try_wait with a suspend-time hint: waiting roles leave the issue slots to the working ones.
-__device__ __forceinline__ bool try_sleep(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(sm100::smem_u32(bar)), "r"(parity), "r"(1000000u)
-      : "memory");
-  return ok != 0;
-}
 __device__ __forceinline__ bool wait_b(uint64_t* bar, uint32_t use, volatile int* abort_v, unsigned int* err) {
   const uint32_t parity = use & 1;
-  if (try_sleep(bar, parity)) return true;
+  if (sm100::mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = sm100::globaltimer();
-  for (;;) {
-    if (try_sleep(bar, parity)) return true;
+  for (uint32_t n = 1;; ++n) {
+    if (sm100::mbar_try_wait(bar, parity)) return true;
+    if (n & 63u) continue;
     if (*abort_v) return false;
     if (sm100::globaltimer() - t0 > 2000000000ull) {
       *abort_v = 1;
@@ -624,6 +618,12 @@ __device__ __forceinline__ bool wait_b(uint64_t* bar, uint32_t use, volatile int
 // The same outcome in all lanes (the tcgen05 operations that follow are warp-collective).
 __device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t use, volatile int* abort_v, unsigned int* err) {
   return __all_sync(0xffffffffu, wait_b(bar, use, abort_v, err));
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // The blocks of one group: units (row block, KV head; head fastest) of `blocks` blocks each.
@@ -1085,61 +1085,88 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
     } else if (warp == 13) {  // ---------------- MMA ----------------
-      const uint32_t q_addr = smem_u32(base + L::Q), k_addr = smem_u32(base + L::K), v_addr = smem_u32(base + L::V);
-      uint32_t j = 0, piece[TILES] = {0, 0}, sj[TILES] = {0, 0};
+      // low descriptor words: address >> 4, and the leading offset >> 4 (K-major: unused, 1; V: 16 KB
+      // between its halves of d)
+      const uint32_t q_lo = (smem_u32(base + L::Q) >> 4) | (1u << 16), k_lo = (smem_u32(base + L::K) >> 4) | (1u << 16);
+      const uint32_t v_lo = (smem_u32(base + L::V) >> 4) | ((16384u >> 4) << 16);
+      // The whole warp runs this loop, its values uniform, and one elected lane issues: the operands of
+      // the tcgen05 instructions then stay in uniform registers (issued from a divergent lane, an MMA
+      // took about 100 cycles to issue, longer than the 64 it runs).
+      const bool leader = elect_one();
+      const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
+      uint32_t j = 0, sk = 0, sv = 0, s0 = 0, s1 = 0, p0 = 0, p1 = 0;  // blocks, slots, P and pieces by tile
       bool ok = true;
-      auto issue_s = [&](int t, uint32_t jj) {
-        const uint32_t dd = tmem + 256u + 128u * t, kb = k_addr + (jj % NK) * 16384u;
+      auto issue_s = [&](int t, uint32_t slot) {
+        const uint32_t dd = tm + 256u + 128u * t, q = q_lo + t * (TERMS * 1024u), k = k_lo + slot * 1024u;
+        if (leader) {
+          mma_f8<false>(dd, q, k);
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term)
+          for (int kk = 1; kk < 4 * TERMS; ++kk)
+            mma_f8<true>(dd, q + (kk / 4) * 1024u + (kk % 4) * 2u, k + (kk % 4) * 2u);
+          tc_commit(&s_full[t]);
+        }
+        __syncwarp();
+      };
+      auto issue_pv = [&](int t, uint32_t v, bool first, bool last) {
+        const uint32_t o = tm + 128u * t, pt = tm + 256u + 128u * t;
+        if (leader) {
+          if (first)
+            mma_pv<false>(o, pt, v);
+          else
+            mma_pv<true>(o, pt, v);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f8(dd, desc_kmajor_sw128(q_addr + (t * TERMS + term) * 16384u + kk * 32u),
-                   desc_kmajor_sw128(kb + kk * 32u), term + kk > 0 ? 1u : 0u);
-        tc_commit(&s_full[t]);
+          for (int kk = 1; kk < BN / 16; ++kk) mma_pv<true>(o, pt + 8u * kk, v + kk * 128u);  // 16 keys each
+          if (last) tc_commit(&o_full[t]);
+        }
+        __syncwarp();
       };
       for (uint32_t d = 0; ok; ++d) {
         const Piece x = take(d);
-        if (!x.n) break;
-        const int tiles = x.rb * ROWS + BM < x.tokens * P.group ? 2 : 1;
-        if (lane == 0) {
-          ok = wait_b(&k_full[j % NK], j / NK, abort_v, P.err);
-          for (int t = 0; ok && t < tiles; ++t) {
-            ok = wait_b(&q_full[t], piece[t], abort_v, P.err);
+        const int n = __reduce_max_sync(0xffffffffu, x.n);
+        if (!n) break;
+        const bool two = __any_sync(0xffffffffu, x.rb * ROWS + BM < x.tokens * P.group);
+        // V of a block and K of the next are waited for under the MMAs of the block before
+        auto operands = [&](bool more) {
+          const uint32_t next = sk + 1 == NK ? 0 : sk + 1;
+          return (!more || wait_w(&k_full[next], (j + 1) / NK, abort_v, P.err)) &&
+                 wait_w(&v_full[sv], j / NV, abort_v, P.err);
+        };
+        ok = wait_w(&k_full[sk], j / NK, abort_v, P.err) && wait_w(&q_full[0], p0++, abort_v, P.err) &&
+             (!two || wait_w(&q_full[1], p1++, abort_v, P.err));
+        if (!ok) break;
+        tc_fence_after();
+        issue_s(0, sk);
+        if (two) issue_s(1, sk);
+        if (leader) tc_commit(&k_empty[sk]);
+        __syncwarp();
+        ok = operands(n > 1);
+        for (int i = 0; ok && i < n; ++i) {
+          const bool more = i + 1 < n;
+          const uint32_t v = v_lo + sv * 2048u, next = sk + 1 == NK ? 0 : sk + 1;
+          ok = wait_w(&p_full[0], s0++, abort_v, P.err);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(0, v, i == 0, !more);
+          if (more) issue_s(0, next);
+          if (two) {
+            ok = wait_w(&p_full[1], s1++, abort_v, P.err);
             if (!ok) break;
             tc_fence_after();
-            issue_s(t, j);
+            issue_pv(1, v, i == 0, !more);
+            if (more) issue_s(1, next);
           }
-          if (ok) tc_commit(&k_empty[j % NK]);
-          for (int i = 0; ok && i < x.n; ++i, ++j) {
-            const bool more = i + 1 < x.n;
-            ok = (!more || wait_b(&k_full[(j + 1) % NK], (j + 1) / NK, abort_v, P.err)) &&
-                 wait_b(&v_full[j % NV], j / NV, abort_v, P.err);
-            const uint32_t vb = v_addr + (j % NV) * 32768u;
-            for (int t = 0; ok && t < tiles; ++t) {
-              ok = wait_b(&p_full[t], sj[t], abort_v, P.err);
-              if (!ok) break;
-              ++sj[t];
-              tc_fence_after();
-#pragma unroll
-              for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys; V MN-major: d-halves 16 KB apart, 8-key groups 1 KB
-                mma_pv(tmem + 128u * t, tmem + 256u + 128u * t + 8u * kk,
-                       smem_desc(vb + kk * 2048u, 16384, 1024, SWZ_128B), (i > 0 || kk > 0) ? 1u : 0u);
-              if (more)
-                issue_s(t, j + 1);
-              else
-                tc_commit(&o_full[t]);
-            }
-            if (ok) {
-              tc_commit(&v_empty[j % NV]);
-              if (more) tc_commit(&k_empty[(j + 1) % NK]);
-            }
+          if (leader) {
+            tc_commit(&v_empty[sv]);
+            if (more) tc_commit(&k_empty[next]);
           }
-          for (int t = 0; t < tiles; ++t) ++piece[t];
+          __syncwarp();
+          ++j;
+          sk = next;
+          sv = sv + 1 == NV ? 0 : sv + 1;
+          if (more) ok = operands(i + 2 < n);
         }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
-      if (lane == 0) {  // everything issued has completed before the teardown
+      if (leader) {  // everything issued has completed before the teardown
         tc_commit(fin);
         const uint64_t t0 = globaltimer();
         while (!mbar_try_wait(fin, 0) && globaltimer() - t0 < 2000000000ull) {
