@@ -26,8 +26,8 @@ constexpr int TILE_BYTES = TILE * D;  // 16 keys x 128 e4m3 bytes
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr unsigned int ERR_TILE_WAIT = 0x90;
 
-// A token's partials.  Own keys: `own_splits` pieces from (own_first + row block * own_splits) * KV heads
-// on, row own_row + head of the segment; prefix likewise, or with prefix_kernel the pieces of the
+// A token's partials.  Own keys: `own_splits` pieces, KV heads apart, from own_first + row block *
+// own_splits * KV heads + KV head on, row own_row + head of the segment; prefix likewise, or with prefix_kernel the pieces of the
 // `blocks` blocks from block `tc_from` + unit * blocks on (units: tc_units before the group).
 struct RowPlan {
   int own_first, own_splits, own_row, pre_row;
@@ -107,9 +107,6 @@ __device__ __forceinline__ int group_of(const Params& P, int b) {  // sequence b
 struct Segment {
   int tok0, tokens, k0, len;
   __device__ __forceinline__ int tiles() const { return len > k0 ? (len - k0 + TILE - 1) / TILE : 0; }
-  template <int ROWS> __device__ __forceinline__ int row_blocks(int group) const {
-    return (tokens * group + ROWS - 1) / ROWS;
-  }
 };
 __device__ __forceinline__ Segment prefix_segment(const Params& P, int g) {
   Segment s;
@@ -142,15 +139,62 @@ __device__ __forceinline__ int64_t tc_units(const Segment& x, const Params& P) {
 }
 
 // ---- pieces of few rows: one warp each, warp-level MMA --------------------------------------------
-// Bound: HBM.  A warp takes one piece (segment, block of 8 * NB rows, split, KV head) at a time, KV
-// head fastest, so that neighbouring warps read the heads of the same pages together.  It streams the
-// piece's tiles through its own ring of RING slots (TMA, 128-byte swizzle, one mbarrier a slot) and
-// computes S^T = K . Q^T (mma.m16n8k16, keys on M, rows on N), an online softmax per row and
-// O^T += V^T . P^T: the e4m3 tile is widened once for all NB row blocks.  Queries are taken as fp16
-// (bf16 values of 2^-14 to 65504 are exact), probabilities rounded to fp16 for P . V, statistics fp32.
-// For the K operand the head dimension is permuted so that lane (g, c) needs bytes [32c, 32c + 32) of
-// keys g and g + 8 (Q likewise); for V the output dimension so that it needs bytes [16g, 16g + 16) of
-// keys 2c, 2c + 1, 2c + 8, 2c + 9: 16-byte shared-memory reads, conflict-free through the swizzle.
+// Bound: HBM by its bytes; measured, the instructions of a tile.  A warp takes one piece (segment, block
+// of 8 * NB rows, split, KV head) at a time, KV head fastest, so that neighbouring warps read the heads
+// of the same pages together.  It streams the piece's 16-key tiles through its own ring of RING slots
+// (TMA, 128-byte swizzle, one mbarrier a slot) and takes two tiles a step, so the steps' serial parts
+// (waits, maxima, the way of P through shared memory) are paid once for 32 keys:
+//   S^T = K . Q^T  mma.m16n8k32 on the e4m3 bytes as they lie (keys on M, rows on N), the queries as
+//     sums of e4m3 terms (see term_scale): K costs no conversion.  The head dimension is permuted so that
+//     lane (g, c) needs bytes [32c, 32c + 32) of keys g and g + 8, Q likewise.
+//   O^T += V^T . P^T  mma.m16n8k16 with V widened to fp16 and P rounded to fp16; the output dimension is
+//     permuted so that the lane needs bytes [16g, 16g + 16) of keys 2c, 2c + 1, 2c + 8, 2c + 9.
+// All shared-memory reads are 16 bytes a lane, conflict-free through the swizzle.  Statistics fp32; the
+// sums are rescaled only when a row's maximum moved.
+// Queries as sums of e4m3 terms.  A row is scaled by a power of two to a maximum in [128, 256); a term
+// keeps 4 significant bits and what it leaves is exact, so two terms hold every bf16 value down to 2^-10
+// of the row's maximum exactly (three hold fp16), smaller ones to 2^-18 of it.
+template <typename TQ> struct Terms;
+template <> struct Terms<__nv_bfloat16> { static constexpr int N = 2; };
+template <> struct Terms<__half> { static constexpr int N = 3; };
+// From the packed 16-bit maxima of |q| over a row's even and odd elements: the scale, and its inverse
+// (NaN for a row with infinities or NaN).
+template <typename TQ> __device__ __forceinline__ void term_scale(uint32_t top, float& up, float& down) {
+  const uint16_t top16 = (uint16_t)max(top & 0xFFFFu, top >> 16);
+  const uint32_t most = __float_as_uint(to_f32(*reinterpret_cast<const TQ*>(&top16)));
+  const int sh = most ? min(134 - (int)(most >> 23), 126) : 0;  // tiny rows stop at 2^126
+  up = __uint_as_float((uint32_t)(sh + 127) << 23);
+  down = most < 0x7F800000u ? __uint_as_float((uint32_t)(127 - sh) << 23) : __int_as_float(0x7fc00000);
+}
+__device__ __forceinline__ uint32_t top_of(uint32_t top, const uint4& u) {
+  top = __vmaxu2(top, u.x & 0x7FFF7FFFu);
+  top = __vmaxu2(top, u.y & 0x7FFF7FFFu);
+  top = __vmaxu2(top, u.z & 0x7FFF7FFFu);
+  return __vmaxu2(top, u.w & 0x7FFF7FFFu);
+}
+// The next term of 4 values (packed), which are left with the rest.
+__device__ __forceinline__ uint32_t next_term(float* f, bool last) {
+  const uint32_t a = f32x2_to_e4m3x2(f[0], f[1]), b = f32x2_to_e4m3x2(f[2], f[3]);
+  if (!last) {
+    const uint32_t ha = e4m3x2_to_f16x2((uint16_t)a), hb = e4m3x2_to_f16x2((uint16_t)b);
+    const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&ha));
+    const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
+    f[0] -= fa.x;
+    f[1] -= fa.y;
+    f[2] -= fb.x;
+    f[3] -= fb.y;
+  }
+  return a | (b << 16);
+}
+// D(16x8, f32) += A(16x32, e4m3, row) * B(32x8, e4m3, col)
+__device__ __forceinline__ void mma_16832_e4m3(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 constexpr int RING = 4;
 constexpr int WARPS = 4;
 constexpr int MIN_TILES = 4;  // of a split: below, a piece's fixed cost outweighs its keys
@@ -162,31 +206,45 @@ __device__ __forceinline__ uint4 tile_ld16(const uint8_t* tile, int row, int chu
 
 // Tiles of a split: the fewest (>= MIN_TILES) with which the pieces do not exceed max_pieces, which is
 // one piece for every warp of the grid, or twice the (segment, row block, head) units where those are
-// more.  Warp-wide.
-template <int ROWS>
-__device__ __forceinline__ int split_tiles(const Segment* seg, int segs, int group, int num_kv_heads, int max_pieces) {
+// more.  work[s] = (tiles, row blocks * heads).  Each lane tries a length, from the bound that the tiles
+// alone give upwards; lengths past those (or of more segments than are worth trying) come from
+// pieces <= tiles / length + units.  Warp-wide.
+__device__ __forceinline__ int ceil_div_small(int a, float inverse) {  // a < 2^21: the half keeps it off the edges
+  return (int)(((float)a - 0.5f) * inverse) + (a > 0);
+}
+__device__ __forceinline__ int split_tiles(const int2* work, int segs, int max_pieces) {
   const int lane = threadIdx.x & 31;
-  int most = 0;
-  for (int s = lane; s < segs; s += 32) most = max(most, seg[s].tiles());
-  most = __reduce_max_sync(0xffffffffu, most);
-  int lo = MIN_TILES, hi = max(most, MIN_TILES);  // hi fits: one split a unit
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    int64_t n = 0;
-    for (int s = lane; s < segs; s += 32)
-      n += (int64_t)((seg[s].tiles() + mid - 1) / mid) * seg[s].row_blocks<ROWS>(group);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (n * num_kv_heads <= max_pieces) hi = mid; else lo = mid + 1;
+  int64_t all = 0;
+  int units = 0, most = 0;
+  for (int s = lane; s < segs; s += 32) {
+    all += (int64_t)work[s].x * work[s].y;
+    units += work[s].x ? work[s].y : 0;
+    most = max(most, work[s].x);
   }
-  return lo;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  units = __reduce_add_sync(0xffffffffu, units);
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int least = (int)min(all / max_pieces + 1, (int64_t)most);
+  const int ct = max(MIN_TILES, least) + lane;
+  bool fits = false;
+  if (segs <= 256 && most < (1 << 21)) {
+    const float inverse = 1.f / (float)ct;
+    int n = 0;
+#pragma unroll 4
+    for (int s = 0; s < segs; ++s) n += ceil_div_small(work[s].x, inverse) * work[s].y;
+    fits = n <= max_pieces && n >= 0;
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, fits);
+  if (who) return __shfl_sync(0xffffffffu, ct, __ffs(who) - 1);
+  return (int)max((int64_t)MIN_TILES, all / max(1, max_pieces - units) + 1);
 }
 
 template <typename TQ, int NB>
-__global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
+__global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
     pieces_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, Params P) {
   using namespace sm100;
-  constexpr int ROWS = 8 * NB;
+  constexpr int ROWS = 8 * NB, TERMS = Terms<TQ>::N;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   extern __shared__ uint8_t smem_raw[];
@@ -194,9 +252,10 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
   uint8_t* ring = base + warp * RING_BYTES;
   const int segs = P.num_groups + P.batch;
   Segment* seg = reinterpret_cast<Segment*>(base + WARPS * RING_BYTES);
-  int* first = reinterpret_cast<int*>(seg + segs);  // splits before each segment
+  int2* work = reinterpret_cast<int2*>(seg + segs);  // tiles, row blocks * heads (0: not this kernel's)
+  int* first = reinterpret_cast<int*>(work + segs);  // pieces before each segment, by heads
   __shared__ uint64_t bars[WARPS][RING];
-  __shared__ __align__(16) __half p_s[WARPS][NB][8][16];
+  __shared__ __align__(16) __half p_s[WARPS][NB][8][40];  // 32 keys a row; padded against bank conflicts
   __shared__ int abort_flag, s_tiles, s_cut;
   uint64_t* bar = bars[warp];
   if (threadIdx.x == 0) {
@@ -216,15 +275,16 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
   for (int s = threadIdx.x; s < segs; s += WARPS * 32) {
     const Segment x = s < P.num_groups ? prefix_segment(P, s) : own_segment(P, s - P.num_groups);
     seg[s] = x;
+    work[s] = make_int2(s >= skip ? x.tiles() : 0, (x.tokens * P.group + ROWS - 1) / ROWS * P.num_kv_heads);
     if (s >= P.num_groups && x.len < x.tokens) s_cut = 1;  // rows inside the prefix: it needs a mask too
   }
   __syncthreads();
   if (warp == 0) {
-    const int ct = split_tiles<ROWS>(seg + skip, segs - skip, P.group, P.num_kv_heads, P.max_pieces);
+    const int ct = split_tiles(work + skip, segs - skip, P.max_pieces);
     int sum = 0;
     for (int s0 = 0; s0 < segs; s0 += 32) {
       const int s = s0 + lane;
-      const int n = s >= skip && s < segs ? (seg[s].tiles() + ct - 1) / ct * seg[s].row_blocks<ROWS>(P.group) : 0;
+      const int n = s < segs ? (work[s].x + ct - 1) / ct * work[s].y : 0;
       int acc = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -286,20 +346,20 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
       if (n < from || n >= to) P.plan[n] = none;
   }
   // (group lists that overlap could name more than the workspace holds)
-  const int64_t pieces = min((int64_t)first[segs] * P.num_kv_heads, (int64_t)P.max_pieces);
+  const int pieces = first[segs] < 0 ? P.max_pieces : min(first[segs], P.max_pieces);
   uint32_t uses = 0;  // tiles through the ring (slot = uses % RING, parity = (uses / RING) & 1)
-  for (int64_t piece = (int64_t)blockIdx.x * WARPS + warp; piece < pieces; piece += (int64_t)gridDim.x * WARPS) {
-    const int kvh = (int)(piece % P.num_kv_heads), flat = (int)(piece / P.num_kv_heads);
-    int lo_s = 0, hi_s = segs;  // the last segment with first[s] <= flat: it is not empty
+  for (int piece = blockIdx.x * WARPS + warp; piece < pieces; piece += gridDim.x * WARPS) {
+    int lo_s = 0, hi_s = segs;  // the last segment with first[s] <= piece: it is not empty
     while (hi_s - lo_s > 1) {
       const int mid = (lo_s + hi_s) >> 1;
-      if (first[mid] <= flat) lo_s = mid; else hi_s = mid;
+      if (first[mid] <= piece) lo_s = mid; else hi_s = mid;
     }
     const int s = lo_s;
     const bool pre = s < P.num_groups;
     const Segment x = seg[s];
-    const int splits = (x.tiles() + ct - 1) / ct;
-    const int rb = (flat - first[s]) / splits, sp = (flat - first[s]) % splits;
+    const int splits = (work[s].x + ct - 1) / ct, off = piece - first[s];
+    const int flat = off / P.num_kv_heads, kvh = off - flat * P.num_kv_heads;
+    const int rb = flat / splits, sp = flat - rb * splits;
     const int t_begin = x.k0 + sp * ct * TILE, t_end = min(x.len, t_begin + ct * TILE);
     const int nt = (t_end - t_begin + TILE - 1) / TILE;
     const int32_t* table = pre ? P.pt + (int64_t)s * P.pt_stride : P.bt + (int64_t)(s - P.num_groups) * P.bt_stride;
@@ -329,33 +389,55 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
       }
     };
     look_up(0);
+    const int rows = x.tokens * P.group;
+    uint4 raw[NB][4];  // queries of row g of each block of 8, d in [32c, 32c + 32)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int r = rb * ROWS + nb * 8 + g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[nb][i] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int tok = r / P.group;
+        const uint4* qp = reinterpret_cast<const uint4*>(
+            reinterpret_cast<const TQ*>(P.q) + (int64_t)(x.tok0 + tok) * P.q_st +
+            (int64_t)(kvh * P.group + r - tok * P.group) * P.q_sh + 32 * c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[nb][i] = qp[i];
+      }
+    }
     uint32_t ok_mask = __ballot_sync(0xffffffffu, my_block >= 0);  // of the 32 tiles looked up last
     int looked = 0;
     for (int k = 0; k < RING && k < nt; ++k)
       issue(k, __shfl_sync(0xffffffffu, my_block, k), __shfl_sync(0xffffffffu, my_row0, k));
 
-    // ---- the rows: queries as the B operand (lane: row g of each block of 8, d in [32c, 32c + 32)),
-    // and the key range [lo, hi) of the rows 2c, 2c + 1 that this lane's scores belong to
-    uint32_t qf[NB][16];
+    // ---- the rows: queries as the B operand (lane: row g of each block of 8, d in [32c, 32c + 32)), and
+    // for the rows 2c, 2c + 1 that this lane's scores belong to their scale and key range [lo, hi)
+    uint32_t qf[NB][TERMS][8];
+    float cs[NB][2];
     int lo[NB][2], hi[NB][2], lo_max = 0, hi_min = 0x7fffffff;
-    const int rows = x.tokens * P.group;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int r = rb * ROWS + nb * 8 + g;
-      if (r < rows) {
-        const TQ* qp = reinterpret_cast<const TQ*>(P.q) + (int64_t)(x.tok0 + r / P.group) * P.q_st +
-                       (int64_t)(kvh * P.group + r % P.group) * P.q_sh + 32 * c;
+      uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float f[8];
-          unpack8<TQ>(*reinterpret_cast<const uint4*>(qp + 8 * i), f);
+      for (int i = 0; i < 4; ++i) top = top_of(top, raw[nb][i]);
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      float up, down;
+      term_scale<TQ>(top, up, down);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) qf[nb][4 * i + j] = pack_half2(f[2 * j], f[2 * j + 1]);
+      for (int i = 0; i < 4; ++i) {
+        float f[8];
+        unpack8<TQ>(raw[nb][i], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= up;
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) {
+          qf[nb][term][2 * i] = next_term(f, term + 1 == TERMS);
+          qf[nb][term][2 * i + 1] = next_term(f + 4, term + 1 == TERMS);
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) qf[nb][i] = 0u;
       }
+      cs[nb][0] = P.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * c);
+      cs[nb][1] = P.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * c + 4);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int re = rb * ROWS + nb * 8 + 2 * c + e;
@@ -363,9 +445,14 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
         if (re < rows && (!pre || cut)) {
           const int n = x.tok0 + re / P.group;
           int pos;  // of the row, in this segment's key coordinates
-          if (pre) {
-            const int b = sequence_of(P, n);
-            pos = x.len + own_len(P, b) - (q_begin(P, b + 1) - n);
+          if (pre) {  // the last sequence that begins at or before row n (empty ones begin there too)
+            int bl = 0, bh = P.batch;
+            while (bh - bl > 1) {
+              const int mid = (bl + bh) >> 1;
+              if (seg[P.num_groups + mid].tok0 <= n) bl = mid; else bh = mid;
+            }
+            const Segment own = seg[P.num_groups + bl];
+            pos = x.len + own.len - (own.tok0 + own.tokens - n);
           } else {
             pos = x.len - (x.tok0 + x.tokens - n);
           }
@@ -390,56 +477,65 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
       l[nb][0] = l[nb][1] = 0.f;
     }
     bool failed = false;
-    for (int k = 0; k < nt; ++k) {
-      const uint32_t use = uses + k;
-      const int slot = use % RING;
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bar[slot], (use / RING) & 1, &abort_flag, P.err, ERR_TILE_WAIT))) {
+    for (int k = 0; k < nt; k += 2) {
+      const bool two = k + 1 < nt;
+      bool came = true;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (u == 0 || two)
+          came &= mbar_wait_bounded(&bar[(uses + k + u) % RING], ((uses + k + u) / RING) & 1, &abort_flag, P.err,
+                                    ERR_TILE_WAIT);
+      if (!__all_sync(0xffffffffu, came)) {
         failed = true;
         break;
       }
-      const bool there = (ok_mask >> (k & 31)) & 1;
       const int tt = t_begin + TILE * k;
-      const uint8_t* kt = ring + slot * 2 * TILE_BYTES;
-      const uint8_t* vt = kt + TILE_BYTES;
-      uint4 kk[4], vv[4];
-      kk[0] = tile_ld16(kt, g, 2 * c);
-      kk[1] = tile_ld16(kt, g, 2 * c + 1);
-      kk[2] = tile_ld16(kt, g + 8, 2 * c);
-      kk[3] = tile_ld16(kt, g + 8, 2 * c + 1);
-      const int keys[4] = {2 * c, 2 * c + 1, 2 * c + 8, 2 * c + 9};
+      const uint32_t ok2 = (ok_mask >> (k & 31)) & (two ? 3u : 1u);  // which of the two tiles are there
+      float sc[NB][2][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)  // rows of a hole or past the end may hold NaN: their weight is 0, V must be finite
-        vv[i] = (there && tt + keys[i] < x.len) ? tile_ld16(vt, keys[i], g) : make_uint4(0, 0, 0, 0);
-
-      float sc[NB][4];
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-      const uint32_t* kg = reinterpret_cast<const uint32_t*>(kk);
-      const uint32_t* kg8 = reinterpret_cast<const uint32_t*>(kk + 2);
+        for (int nb = 0; nb < NB; ++nb) sc[nb][u][0] = sc[nb][u][1] = sc[nb][u][2] = sc[nb][u][3] = 0.f;
+        if (u == 1 && !two) break;
+        const uint8_t* kt = ring + ((uses + k + u) % RING) * 2 * TILE_BYTES;
+        uint4 kk[4];
+        kk[0] = tile_ld16(kt, g, 2 * c);
+        kk[1] = tile_ld16(kt, g, 2 * c + 1);
+        kk[2] = tile_ld16(kt, g + 8, 2 * c);
+        kk[3] = tile_ld16(kt, g + 8, 2 * c + 1);
+        const uint32_t* kg = reinterpret_cast<const uint32_t*>(kk);
+        const uint32_t* kg8 = reinterpret_cast<const uint32_t*>(kk + 2);
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        uint32_t a[4];
-        a[0] = e4m3x2_to_f16x2((uint16_t)(kg[ks] & 0xFFFFu));
-        a[1] = e4m3x2_to_f16x2((uint16_t)(kg8[ks] & 0xFFFFu));
-        a[2] = e4m3x2_to_f16x2((uint16_t)(kg[ks] >> 16));
-        a[3] = e4m3x2_to_f16x2((uint16_t)(kg8[ks] >> 16));
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma_16816_f16(sc[nb], a, &qf[nb][2 * ks]);
+          for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              mma_16832_e4m3(sc[nb][u], kg[2 * ks], kg8[2 * ks], kg[2 * ks + 1], kg8[2 * ks + 1], qf[nb][term][2 * ks],
+                             qf[nb][term][2 * ks + 1]);
       }
-      const bool whole = there && tt >= lo_max && tt + TILE <= hi_min;  // warp-uniform
-      const int tg = tt + g, tg8 = tt + g + 8;
-      uint32_t bp[NB][2];
+      const bool whole = ok2 == 3u && tt >= lo_max && tt + 2 * TILE <= hi_min;  // warp-uniform
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        float s0 = sc[nb][0] * P.scale_log2, s1 = sc[nb][1] * P.scale_log2;    // key g,     rows 2c, 2c + 1
-        float s2 = sc[nb][2] * P.scale_log2, s3 = sc[nb][3] * P.scale_log2;    // key g + 8
-        if (!whole) {
-          s0 = there && tg >= lo[nb][0] && tg < hi[nb][0] ? s0 : -INFINITY;
-          s1 = there && tg >= lo[nb][1] && tg < hi[nb][1] ? s1 : -INFINITY;
-          s2 = there && tg8 >= lo[nb][0] && tg8 < hi[nb][0] ? s2 : -INFINITY;
-          s3 = there && tg8 >= lo[nb][1] && tg8 < hi[nb][1] ? s3 : -INFINITY;
+        float v[2][4];  // [row 2c, 2c + 1][keys g, g + 8 of both tiles]
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          v[0][2 * u] = sc[nb][u][0] * cs[nb][0];
+          v[1][2 * u] = sc[nb][u][1] * cs[nb][1];
+          v[0][2 * u + 1] = sc[nb][u][2] * cs[nb][0];
+          v[1][2 * u + 1] = sc[nb][u][3] * cs[nb][1];
         }
-        float x0 = fmaxf(s0, s2), x1 = fmaxf(s1, s3);
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = tt + g + 8 * i;
+            const bool there = (ok2 >> (i >> 1)) & 1u;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) v[e][i] = there && key >= lo[nb][e] && key < hi[nb][e] ? v[e][i] : -INFINITY;
+          }
+        }
+        float x0 = fmaxf(fmaxf(v[0][0], v[0][1]), fmaxf(v[0][2], v[0][3]));
+        float x1 = fmaxf(fmaxf(v[1][0], v[1][1]), fmaxf(v[1][2], v[1][3]));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
@@ -449,71 +545,93 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
         x1 = fmaxf(m[nb][1], x1);
         // nothing visible so far: against 0, so that no weight is NaN
         const float z0 = x0 == -INFINITY ? 0.f : x0, z1 = x1 == -INFINITY ? 0.f : x1;
-        const float al0 = fast_exp2(m[nb][0] - z0), al1 = fast_exp2(m[nb][1] - z1);
-        const float p0 = fast_exp2(s0 - z0), p1 = fast_exp2(s1 - z1);
-        const float p2 = fast_exp2(s2 - z0), p3 = fast_exp2(s3 - z1);
-        m[nb][0] = x0;
-        m[nb][1] = x1;
-        l[nb][0] = l[nb][0] * al0 + (p0 + p2);
-        l[nb][1] = l[nb][1] * al1 + (p1 + p3);
+        if (__any_sync(0xffffffffu, x0 != m[nb][0] || x1 != m[nb][1])) {
+          const float al0 = fast_exp2(m[nb][0] - z0), al1 = fast_exp2(m[nb][1] - z1);
+          m[nb][0] = x0;
+          m[nb][1] = x1;
+          l[nb][0] *= al0;
+          l[nb][1] *= al1;
 #pragma unroll
-        for (int mt = 0; mt < 8; ++mt) {
-          acc[nb][mt][0] *= al0;
-          acc[nb][mt][1] *= al1;
-          acc[nb][mt][2] *= al0;
-          acc[nb][mt][3] *= al1;
+          for (int mt = 0; mt < 8; ++mt) {
+            acc[nb][mt][0] *= al0;
+            acc[nb][mt][1] *= al1;
+            acc[nb][mt][2] *= al0;
+            acc[nb][mt][3] *= al1;
+          }
         }
-        __half(*ps)[16] = p_s[warp][nb];  // P through shared memory: the B operand wants (key pairs, row g)
-        ps[2 * c][g] = __float2half_rn(p0);
-        ps[2 * c + 1][g] = __float2half_rn(p1);
-        ps[2 * c][g + 8] = __float2half_rn(p2);
-        ps[2 * c + 1][g + 8] = __float2half_rn(p3);
+        __half(*ps)[40] = p_s[warp][nb];  // P through shared memory: the B operand wants (key pairs, row g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = fast_exp2(v[0][i] - z0), p1 = fast_exp2(v[1][i] - z1);
+          l[nb][0] += p0;
+          l[nb][1] += p1;
+          ps[2 * c][g + 8 * i] = __float2half_rn(p0);
+          ps[2 * c + 1][g + 8 * i] = __float2half_rn(p1);
+        }
       }
       __syncwarp();
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        bp[nb][0] = *reinterpret_cast<const uint32_t*>(&p_s[warp][nb][g][2 * c]);
-        bp[nb][1] = *reinterpret_cast<const uint32_t*>(&p_s[warp][nb][g][2 * c + 8]);
-      }
-      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0]);
-      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1]);
-      const uint32_t* v8 = reinterpret_cast<const uint32_t*>(&vv[2]);
-      const uint32_t* v9 = reinterpret_cast<const uint32_t*>(&vv[3]);
+      for (int u = 0; u < 2; ++u) {
+        if (u == 1 && !two) break;
+        const uint8_t* vt = ring + ((uses + k + u) % RING) * 2 * TILE_BYTES + TILE_BYTES;
+        uint4 vv[4];
+        const int keys[4] = {2 * c, 2 * c + 1, 2 * c + 8, 2 * c + 9};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+        for (int i = 0; i < 4; ++i) {  // rows of a hole or past the end may hold NaN: their weight is 0, V must be finite
+          vv[i] = tile_ld16(vt, keys[i], g);
+          if (!whole && !(((ok2 >> u) & 1u) && tt + TILE * u + keys[i] < x.len)) vv[i] = make_uint4(0, 0, 0, 0);
+        }
+        uint32_t bp[NB][2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362u : 0x5140u;
-          const uint32_t lo01 = prmt(v0[j], v1[j], sel);
-          const uint32_t lo89 = prmt(v8[j], v9[j], sel);
-          uint32_t a[4];
-          a[0] = e4m3x2_to_f16x2((uint16_t)(lo01 & 0xFFFFu));
-          a[1] = e4m3x2_to_f16x2((uint16_t)(lo01 >> 16));
-          a[2] = e4m3x2_to_f16x2((uint16_t)(lo89 & 0xFFFFu));
-          a[3] = e4m3x2_to_f16x2((uint16_t)(lo89 >> 16));
+        for (int nb = 0; nb < NB; ++nb) {
+          bp[nb][0] = *reinterpret_cast<const uint32_t*>(&p_s[warp][nb][g][TILE * u + 2 * c]);
+          bp[nb][1] = *reinterpret_cast<const uint32_t*>(&p_s[warp][nb][g][TILE * u + 2 * c + 8]);
+        }
+        const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0]);
+        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1]);
+        const uint32_t* v8 = reinterpret_cast<const uint32_t*>(&vv[2]);
+        const uint32_t* v9 = reinterpret_cast<const uint32_t*>(&vv[3]);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma_16816_f16(acc[nb][2 * j + half], a, bp[nb]);
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362u : 0x5140u;
+            const uint32_t lo01 = prmt(v0[i], v1[i], sel);
+            const uint32_t lo89 = prmt(v8[i], v9[i], sel);
+            uint32_t a[4];
+            a[0] = e4m3x2_to_f16x2((uint16_t)(lo01 & 0xFFFFu));
+            a[1] = e4m3x2_to_f16x2((uint16_t)(lo01 >> 16));
+            a[2] = e4m3x2_to_f16x2((uint16_t)(lo89 & 0xFFFFu));
+            a[3] = e4m3x2_to_f16x2((uint16_t)(lo89 >> 16));
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) mma_16816_f16(acc[nb][2 * i + half], a, bp[nb]);
+          }
         }
       }
-      // every lane is done with the slot and with P: refill the slot with tile k + RING
+      // every lane is done with the slots and with P: refill the slots with tiles k + RING, k + RING + 1
       __syncwarp();
-      const int nx = k + RING;
-      if (nx < nt) {
-        if ((nx & 31) == 0) look_up(nx);
-        const int blk = __shfl_sync(0xffffffffu, my_block, nx & 31);
-        const int row0 = __shfl_sync(0xffffffffu, my_row0, nx & 31);
-        if ((nx & 31) == 0) looked = nx;
+      if (k + RING < nt) {
+        const int nx = k + RING;
+        if ((nx & 31) == 0) {
+          look_up(nx);
+          looked = nx;
+        }
         if (lane == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        issue(nx, blk, row0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int blk = __shfl_sync(0xffffffffu, my_block, (nx + u) & 31);
+          const int row0 = __shfl_sync(0xffffffffu, my_row0, (nx + u) & 31);
+          if (nx + u < nt) issue(nx + u, blk, row0);
+        }
       }
-      // the mask of the next tile's block of 32 (its look-up is RING tiles old by then)
-      if (((k + 1) & 31) == 0 && looked == k + 1) ok_mask = __ballot_sync(0xffffffffu, my_block >= 0);
+      // the mask of the next step's block of 32 (its look-up is RING tiles old by then)
+      if (((k + 2) & 31) == 0 && looked == k + 2) ok_mask = __ballot_sync(0xffffffffu, my_block >= 0);
     }
     uses += nt;
     const float poison = failed ? __int_as_float(0x7fc00000) : 0.f;  // a tile never came: the result is not valid
 
-    float2* ml = P.ml_part + piece * ROWS;
-    float* op = P.o_part + piece * ROWS * D;
+    float2* ml = P.ml_part + (int64_t)piece * ROWS;
+    float* op = P.o_part + (int64_t)piece * ROWS * D;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       float l0 = l[nb][0], l1 = l[nb][1];
@@ -550,11 +668,8 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 4 ? 2 : 3)
 // laid end to end and every CTA takes an equal range, so a range covers the end of one unit, whole
 // ones and the start of another, each giving one partial (piece = unit + CTA index: one of the two
 // moves on from each piece to the next).
-//   S_t = Q_t . K^T  kind::f8f6f4 on the e4m3 bytes as they lie in the cache.  A query row is scaled by
-//     a power of two to a maximum in [128, 256) and written as a sum of e4m3 terms: a term keeps 4
-//     significant bits and what it leaves is exact, so two terms hold every bf16 value down to 2^-10 of
-//     the row's maximum exactly (three hold fp16), smaller ones to 2^-18 of it.  K is never widened
-//     and the terms cost what the fp16 product would.
+//   S_t = Q_t . K^T  kind::f8f6f4 on the e4m3 bytes as they lie in the cache, the queries as sums of e4m3
+//     terms (see Terms): K is never widened and the terms cost what the fp16 product would.
 //   P  = 2^(S c - m) in fp16, written over S in TMEM, the A operand of
 //   O_t += P_t . V  kind::f16; V is widened to fp16 by four warps, once for both tiles.
 // Roles (16 warps): 0-3 widen V; 4-7 and 8-11 take tile 0's and tile 1's rows (thread = row: queries to
@@ -950,22 +1065,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint8_t* row_at = qt + rl * 128;
           const uint4 raw[2] = {*reinterpret_cast<const uint4*>(row_at + 16 * (lane & 7)),
                                 *reinterpret_cast<const uint4*>(row_at + 16384 + 16 * (lane & 7))};
-          uint32_t top = 0;  // bits of the largest magnitudes of the even and the odd elements
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            top = __vmaxu2(top, raw[h].x & 0x7FFF7FFFu);
-            top = __vmaxu2(top, raw[h].y & 0x7FFF7FFFu);
-            top = __vmaxu2(top, raw[h].z & 0x7FFF7FFFu);
-            top = __vmaxu2(top, raw[h].w & 0x7FFF7FFFu);
-          }
+          uint32_t top = top_of(top_of(0, raw[0]), raw[1]);
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const uint16_t top16 = (uint16_t)max(top & 0xFFFFu, top >> 16);
-          const uint32_t most = __float_as_uint(to_f32(*reinterpret_cast<const TQ*>(&top16)));
-          // 2^s with most * 2^s in [128, 256); tiny rows stop at 2^126; infinities and NaN make the row NaN
-          const int sh = most ? min(134 - (int)(most >> 23), 126) : 0;
-          const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
-          const float down = most < 0x7F800000u ? __uint_as_float((uint32_t)(127 - sh) << 23) : __int_as_float(0x7fc00000);
+          float up, down;
+          term_scale<TQ>(top, up, down);
           const float mine = __shfl_sync(0xffffffffu, down, 8 * (lane & 3));
           if (lane >> 2 == k) c *= mine;  // lane = row 4 k + (lane & 3)
           __syncwarp();                   // the row has been read
@@ -978,19 +1082,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int term = 0; term < TERMS; ++term) {
             uint32_t out[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t a = f32x2_to_e4m3x2(f[4 * e], f[4 * e + 1]), b = f32x2_to_e4m3x2(f[4 * e + 2], f[4 * e + 3]);
-              out[e] = a | (b << 16);
-              if (term + 1 < TERMS) {
-                const uint32_t ha = e4m3x2_to_f16x2((uint16_t)a), hb = e4m3x2_to_f16x2((uint16_t)b);
-                const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&ha));
-                const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
-                f[4 * e] -= fa.x;
-                f[4 * e + 1] -= fa.y;
-                f[4 * e + 2] -= fb.x;
-                f[4 * e + 3] -= fb.y;
-              }
-            }
+            for (int e = 0; e < 4; ++e) out[e] = next_term(f + 4 * e, term + 1 == TERMS);
             *reinterpret_cast<uint4*>(row_at + term * 16384 + (((lane & 7) ^ (rl & 7)) << 4)) =
                 make_uint4(out[0], out[1], out[2], out[3]);
           }
@@ -1385,7 +1477,7 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
   }
   // the pieces of a segment that hold row r, in order of their splits
   auto join = [&](int first, int splits, int r) {
-    const int64_t piece0 = ((int64_t)first + (int64_t)(r / piece_rows) * splits) * P.num_kv_heads + kvh;
+    const int64_t piece0 = first + (int64_t)(r / piece_rows) * splits * P.num_kv_heads + kvh;
     gather(splits, piece0 * piece_rows + r % piece_rows, (int64_t)P.num_kv_heads * piece_rows, P.ml_part, P.o_part,
            (int64_t)P.max_pieces * piece_rows);
   };
@@ -1424,9 +1516,9 @@ inline bool smem_ready(int bytes) {
   return true;
 }
 
-// Blocks of 8 rows that a warp takes together: what the rows of a sequence fill on average, up to four
+// Blocks of 8 rows that a warp takes together: what the rows of a sequence fill on average, up to two
 // (a prefix of 16 rows ran faster as two blocks of 8 than as one of 16: 54 against 72 us for 8 x 8 samples).
-inline int row_blocks(int64_t rows) { return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4); }
+inline int row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 constexpr int MAX_SEGMENTS = 4096;
 constexpr int PIECES_PER_SM = 3 * WARPS;
@@ -1575,17 +1667,17 @@ extern "C" int ada_fp8_shared_prefix_decode(
     ADA_CHECK_LAUNCH();
   }
   const int segs = num_groups + batch;
-  const int smem = 1024 + sp::WARPS * sp::RING_BYTES + segs * ((int)sizeof(sp::Segment) + 4) + 4;
+  const int smem = 1024 + sp::WARPS * sp::RING_BYTES + segs * ((int)sizeof(sp::Segment) + 12) + 4;
 #define ADA_SP(TQ, NB)                                                                                              \
   do {                                                                                                              \
     if (!sp::smem_ready<sp::pieces_kernel<TQ, NB>>(smem)) return ADA_ERR_CUDA;                                      \
-    (void)ada::launch_k(sp::pieces_kernel<TQ, NB>, dim3((unsigned)(sms * (NB == 4 ? 2 : 3))), dim3(sp::WARPS * 32), \
+    (void)ada::launch_k(sp::pieces_kernel<TQ, NB>, dim3((unsigned)(sms * (NB == 1 ? 3 : 2))), dim3(sp::WARPS * 32), \
                         smem, st, tmk, tmv, P);                                                                     \
   } while (0)
   if (q_dtype == ADA_DT_BF16) {
-    if (y.nb == 1) ADA_SP(__nv_bfloat16, 1); else if (y.nb == 2) ADA_SP(__nv_bfloat16, 2); else ADA_SP(__nv_bfloat16, 4);
+    if (y.nb == 1) ADA_SP(__nv_bfloat16, 1); else ADA_SP(__nv_bfloat16, 2);
   } else {
-    if (y.nb == 1) ADA_SP(__half, 1); else if (y.nb == 2) ADA_SP(__half, 2); else ADA_SP(__half, 4);
+    if (y.nb == 1) ADA_SP(__half, 1); else ADA_SP(__half, 2);
   }
 #undef ADA_SP
   ADA_CHECK_LAUNCH();
