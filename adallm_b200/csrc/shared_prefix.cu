@@ -26,6 +26,24 @@ constexpr int TILE_BYTES = TILE * D;  // 16 keys x 128 e4m3 bytes
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr unsigned int ERR_TILE_WAIT = 0x90;
 
+// Division of 0 <= n < 2^31 by a number fixed per launch: multiply and shift (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994): m = ceil(2^(31 + s) / d), s = ceil(log2 d).
+struct Divisor {
+  uint32_t m;
+  int32_t shift, d;
+  __host__ static Divisor of(int32_t d) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s, d};
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> shift); }
+  __device__ __forceinline__ int divmod(int n, int& rest) const {
+    const int q = div(n);
+    rest = n - q * d;
+    return q;
+  }
+};
+
 // A token's partials.  Own keys: `own_splits` pieces, KV heads apart, from own_first + row block *
 // own_splits * KV heads + KV head on, row own_row + head of the segment; prefix likewise, or with prefix_kernel the pieces of the
 // `blocks` blocks from block `tc_from` + unit * blocks on (units: tc_units before the group).
@@ -52,6 +70,7 @@ struct Params {
   const int32_t* ctx;
   const int32_t* cu_q;  // null: one row per sequence
   int32_t batch, total_q, num_heads, num_kv_heads, group, page, window;
+  Divisor by_group, by_page, by_kv_heads, by_heads;
   float scale_log2, v_scale;
   void* out;
   int64_t o_st, o_sh;
@@ -349,16 +368,17 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
   const int pieces = first[segs] < 0 ? P.max_pieces : min(first[segs], P.max_pieces);
   uint32_t uses = 0;  // tiles through the ring (slot = uses % RING, parity = (uses / RING) & 1)
   for (int piece = blockIdx.x * WARPS + warp; piece < pieces; piece += gridDim.x * WARPS) {
-    int lo_s = 0, hi_s = segs;  // the last segment with first[s] <= piece: it is not empty
-    while (hi_s - lo_s > 1) {
-      const int mid = (lo_s + hi_s) >> 1;
-      if (first[mid] <= piece) lo_s = mid; else hi_s = mid;
+    int s = 0;  // the last segment with first[s] <= piece (it is not empty), 32 probes at a time
+    for (int step = segs <= 32 ? 1 : (segs <= 1024 ? 32 : 1024);; step >>= 5) {
+      const int at = s + lane * step;
+      s += (__popc(__ballot_sync(0xffffffffu, at < segs && first[at] <= piece)) - 1) * step;
+      if (step == 1) break;
     }
-    const int s = lo_s;
     const bool pre = s < P.num_groups;
     const Segment x = seg[s];
     const int splits = (work[s].x + ct - 1) / ct, off = piece - first[s];
-    const int flat = off / P.num_kv_heads, kvh = off - flat * P.num_kv_heads;
+    int kvh;
+    const int flat = P.by_kv_heads.divmod(off, kvh);
     const int rb = flat / splits, sp = flat - rb * splits;
     const int t_begin = x.k0 + sp * ct * TILE, t_end = min(x.len, t_begin + ct * TILE);
     const int nt = (t_end - t_begin + TILE - 1) / TILE;
@@ -369,7 +389,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
       my_block = -1;
       if (from + lane < nt) {
         const int key = t_begin + TILE * (from + lane);
-        const int at = key / P.page;
+        const int at = P.by_page.div(key);
         my_row0 = key - at * P.page;
         my_block = __ldg(table + at);
         if (my_block >= P.num_pages) my_block = -1;
@@ -397,10 +417,11 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
 #pragma unroll
       for (int i = 0; i < 4; ++i) raw[nb][i] = make_uint4(0, 0, 0, 0);
       if (r < rows) {
-        const int tok = r / P.group;
+        int head;
+        const int tok = P.by_group.divmod(r, head);
         const uint4* qp = reinterpret_cast<const uint4*>(
             reinterpret_cast<const TQ*>(P.q) + (int64_t)(x.tok0 + tok) * P.q_st +
-            (int64_t)(kvh * P.group + r - tok * P.group) * P.q_sh + 32 * c);
+            (int64_t)(kvh * P.group + head) * P.q_sh + 32 * c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) raw[nb][i] = qp[i];
       }
@@ -443,7 +464,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
         const int re = rb * ROWS + nb * 8 + 2 * c + e;
         int from = 0, to = x.len;
         if (re < rows && (!pre || cut)) {
-          const int n = x.tok0 + re / P.group;
+          const int n = x.tok0 + P.by_group.div(re);
           int pos;  // of the row, in this segment's key coordinates
           if (pre) {  // the last sequence that begins at or before row n (empty ones begin there too)
             int bl = 0, bh = P.batch;
@@ -1037,7 +1058,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int row = x.rb * ROWS + t * BM + r, rows = x.tokens * P.group;
       if (x.rb * ROWS + t * BM >= rows) continue;  // the unit has no rows in this tile
       const bool valid = row < rows;
-      const int n = x.tok0 + row / P.group;
+      const int n = x.tok0 + P.by_group.div(row);
       // ---- the warp's 32 rows of queries as e4m3 terms, eight lanes a row.  The rows are copied into the
       // place of their first two terms and converted there; the loop is kept short, since this runs once
       // a piece and fetching unrolled code took longer than running it.
@@ -1049,8 +1070,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int rl = 32 * (warp & 3) + 4 * k + (lane >> 3), rr = x.rb * ROWS + t * BM + rl;
           uint8_t* to = qt + rl * 128 + 16 * (lane & 7);
           if (rr < rows) {
-            const TQ* qp = reinterpret_cast<const TQ*>(P.q) + (int64_t)(x.tok0 + rr / P.group) * P.q_st +
-                           (int64_t)(x.kvh * P.group + rr % P.group) * P.q_sh + 16 * (lane & 7);
+            int head;
+            const int tok = P.by_group.divmod(rr, head);
+            const TQ* qp = reinterpret_cast<const TQ*>(P.q) + (int64_t)(x.tok0 + tok) * P.q_st +
+                           (int64_t)(x.kvh * P.group + head) * P.q_sh + 16 * (lane & 7);
             copy16(to, qp);
             copy16(to + 16384, qp + 8);
           } else {
@@ -1105,7 +1128,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       auto entry = [&](int tile) {            // is the page of this lane's key tile there?
         const int key = x.k0 + (tile0 + tile) * TILE;
         if (tile >= x.n * (BN / TILE) || key >= x.len) return 0;
-        const int blk = __ldg(table + key / P.page);
+        const int blk = __ldg(table + P.by_page.div(key));
         return blk >= 0 && blk < P.num_pages ? 1 : 0;
       };
       int coming = entry(lane);
@@ -1232,7 +1255,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           b = -1;
           rr = 0;
           if (tile >= tiles || key >= x.len) return;
-          const int at = key / P.page;
+          const int at = P.by_page.div(key);
           rr = key - at * P.page;
           b = __ldg(table + at);
           if (b >= P.num_pages) b = -1;
@@ -1426,10 +1449,10 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + warp;
-  if (item >= (int64_t)P.total_q * P.num_heads) return;
-  const int n = (int)(item / P.num_heads), h = (int)(item % P.num_heads);
-  const int kvh = h / P.group, hg = h % P.group;
+  const int item = blockIdx.x * 4 + warp;
+  if (item >= P.total_q * P.num_heads) return;
+  int h, hg;
+  const int n = P.by_heads.divmod(item, h), kvh = P.by_group.divmod(h, hg);
   const RowPlan plan = P.plan[n];
   float M = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1621,6 +1644,10 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.num_kv_heads = num_kv_heads;
   P.group = num_heads / num_kv_heads;
   P.page = page_size;
+  P.by_group = sp::Divisor::of(P.group);
+  P.by_page = sp::Divisor::of(page_size);
+  P.by_kv_heads = sp::Divisor::of(num_kv_heads);
+  P.by_heads = sp::Divisor::of(num_heads);
   P.window = window;
   P.scale_log2 = scale * k_scale * sp::LOG2E;
   P.v_scale = v_scale;
