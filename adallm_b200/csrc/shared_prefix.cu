@@ -1133,7 +1133,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       int coming = entry(lane);
       uint32_t there = 0;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, m_raw = 0.f, l = 0.f;  // reference, scaled and as a raw score; sum
       for (int i = 0; i < x.n; ++i, ++j) {
         if ((i & 3) == 0) {  // 32 key tiles = 4 blocks
           there = __ballot_sync(0xffffffffu, coming != 0);
@@ -1174,16 +1174,26 @@ __global__ void __launch_bounds__(THREADS, 1)
             mq[q] = fmaxf(fmaxf(mq[q], __uint_as_float(sr[k + q])), __uint_as_float(sr[k + 8 + q]));
           mq[q] = fmaxf(mq[q], __uint_as_float(sr[120 + q]));
         }
-        const float mx = fmaxf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])),
-                               fmaxf(fmaxf(mq[4], mq[5]), fmaxf(mq[6], mq[7]))) * c;
+        const float raw = fmaxf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])),
+                                fmaxf(fmaxf(mq[4], mq[5]), fmaxf(mq[6], mq[7])));
+        const float mx = raw * c;
         // The reference of a row's O and l follows its maximum only when that grew by more than
         // 2^RESCALE_LOG2: weights stay <= 2^8, exact enough in fp16, and O / l does not change.
         float alpha = 1.f;
         if (mx > m + RESCALE_LOG2 || (m == -INFINITY && mx != -INFINITY)) {
           alpha = fast_exp2(m - mx);
           m = mx;
+          m_raw = raw;
         }
-        const float ref = m != -INFINITY ? m : 0.f;
+        // Weights are 2^(s c - m) by one fma, m carrying a rounding of 2^-24 |m|; where that could be seen,
+        // the maximum is taken off s first.
+        const bool huge = fabsf(m) > 16384.f && m != -INFINITY;
+        if (__any_sync(0xffffffffu, huge)) {
+#pragma unroll
+          for (int k = 0; k < 128; ++k)
+            if (huge) sr[k] = __float_as_uint(__uint_as_float(sr[k]) - m_raw);
+        }
+        const float ref = m != -INFINITY && !huge ? m : 0.f;
         if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {  // P.V of the block before is complete: see s_full
 #pragma unroll 1
           for (int q = 0; q < 4; ++q) {
@@ -1466,7 +1476,7 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       const float to = fmaxf(M, most);
-      if (to == -INFINITY && !__any_sync(0xffffffffu, ml.x != ml.x)) continue;
+      if (to == -INFINITY && !__any_sync(0xffffffffu, ml.x != ml.x || ml.y != ml.y)) continue;
       const float by = M == -INFINITY ? 0.f : fast_exp2(M - to);
       M = to;
       L *= by;
@@ -1546,12 +1556,16 @@ inline int row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 constexpr int MAX_SEGMENTS = 4096;
 constexpr int PIECES_PER_SM = 3 * WARPS;
 
-// Rows of a prefix and KV head from which the tensor-core kernel takes the prefixes.
-constexpr int64_t TC_ROWS = 33;
+// prefix_kernel takes the prefixes from 33 rows a prefix and KV head on (with fewer, its 128-row tiles stay
+// emptier than the pieces' blocks of 8), where (rows) x (keys that the prefix tables reach) x (KV heads)
+// is at least 2^21: its launch, set-up and partials cost about 10 us, which the pieces need for that much.
+// 64 rows x 8 heads behind 2,048 keys: 24 us by pieces, 30 us with it; behind 32,768 keys the pieces' share
+// alone is 16 times as long.
+constexpr int64_t TC_ROWS = 33, TC_WORK = 1 << 21;
 
 struct Layout {
   int nb;
-  bool tc;
+  bool tc;  // enough rows for prefix_kernel
   int64_t pieces, tc_pieces;
   size_t plan, ml, o, tc_ml, tc_o, bytes;  // offsets of the workspace's parts, its size
 };
@@ -1660,7 +1674,8 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.ml_part = reinterpret_cast<float2*>(ws + y.ml);
   P.o_part = reinterpret_cast<float*>(ws + y.o);
   P.max_pieces = (int32_t)(y.pieces < 0x7fffffff ? y.pieces : 0x7fffffff);
-  P.prefix_tc = y.tc ? 1 : 0;
+  const int64_t reach = (int64_t)max_prefix_pages * page_size;
+  P.prefix_tc = y.tc && total_q * (int64_t)P.group * num_kv_heads * reach >= sp::TC_WORK ? 1 : 0;
   P.tc_ml = reinterpret_cast<float2*>(ws + y.tc_ml);
   P.tc_o = reinterpret_cast<float*>(ws + y.tc_o);
   P.tc_rows = y.tc_pieces * sp::tc::ROWS;
@@ -1678,7 +1693,7 @@ extern "C" int ada_fp8_shared_prefix_decode(
   if (!sms) return ADA_ERR_CUDA;
   P.tc_ctas = sms < 148 ? sms : 148;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (y.tc) {
+  if (P.prefix_tc) {
     const dim3 grid((unsigned)P.tc_ctas), block(sp::tc::THREADS);
     if (q_dtype == ADA_DT_BF16) {
       constexpr int bytes = sp::tc::Smem<2>::BYTES;

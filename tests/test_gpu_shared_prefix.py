@@ -17,11 +17,28 @@ from tests.gpu_util import dev, rel_l2
 pytestmark = pytest.mark.gpu
 
 REL = {torch.bfloat16: 2 ** -8.5, torch.float16: 2 ** -10}
-ULP = {torch.bfloat16: 2 ** -9, torch.float16: 2 ** -12}
+ULP = {torch.bfloat16: 2 ** -8, torch.float16: 2 ** -11}
+
+
+REACH = 0
+
+
+@pytest.fixture(params=[0, 1 << 18], ids=["", "wide"], autouse=True)
+def reach(request):
+    """Every test also with prefix tables padded to a long reach: from 33 rows a prefix on, the
+    library then takes the tensor-core kernel for the prefixes whatever their lengths."""
+    global REACH
+    REACH = request.param
+    yield
+    REACH = 0
 
 
 def _to_gpu(case):
-    return {k: v.to(dev()) if isinstance(v, torch.Tensor) else v for k, v in case.items()}
+    c = {k: v.to(dev()) if isinstance(v, torch.Tensor) else v for k, v in case.items()}
+    pad = REACH // c["k_cache"].shape[1] - c["prefix_tables"].shape[1]
+    if pad > 0:
+        c["prefix_tables"] = torch.nn.functional.pad(c["prefix_tables"], (0, pad), value=-1)
+    return c
 
 
 def _args(c, **kw):
@@ -62,8 +79,9 @@ def test_heads_and_pages(hq, hkv, page, dtype):
 
 
 @pytest.mark.parametrize("prefix", [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 257, 1000])
-def test_prefix_lengths(prefix):
-    _run(osp.make_shared_prefix_case(2, [prefix], [3], [1, 2, 40], [1, 1, 1], 32, 8, 16))
+@pytest.mark.parametrize("rows", [[1, 1, 1], [9, 3, 1], [30, 35, 2]])
+def test_prefix_lengths(prefix, rows):
+    _run(osp.make_shared_prefix_case(2, [prefix], [3], [9, 2, 40], rows, 32, 8, 16))
 
 
 @pytest.mark.parametrize("own", [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 400])
@@ -88,8 +106,9 @@ def test_more_rows_than_own_keys():
                                             ([2, 2, 2], [0, 513, 0])])
 def test_groups(sizes, prefixes):
     n = 8
-    _run(osp.make_shared_prefix_case(6, prefixes, sizes, [5, 30, 64, 1, 129, 17, 70, 16], [1, 2, 1, 1, 3, 1, 1, 2],
-                                     32, 8, 16) | {"n": n})
+    for rows in ([1, 2, 1, 1, 3, 1, 1, 2], [17, 20, 40, 1, 9, 30, 3, 16]):
+        _run(osp.make_shared_prefix_case(6, prefixes, sizes, [5, 30, 64, 1, 129, 17, 70, 16], rows, 32, 8, 16)
+             | {"n": n})
 
 
 def test_many_groups_and_sequences():
@@ -109,16 +128,17 @@ def test_wide_batches_fill_several_row_blocks():
 
 
 @pytest.mark.parametrize("window", [1, 2, 17, 64, 130, 1024])
-@pytest.mark.parametrize("rows", [[1, 1, 1], [4, 2, 5]])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [4, 2, 5], [30, 9, 40]])
 def test_window(window, rows):
     """Windows inside the own keys, across the prefix's end and over everything."""
     _run(osp.make_shared_prefix_case(9, [200], [3], [5, 60, 150], rows, 32, 16, 16), window=window)
 
 
-def test_holes_in_the_tables():
-    for seed in range(3):
-        _run(osp.make_shared_prefix_case(10 + seed, [130, 40], [2, 2], [20, 70, 0, 33], [1, 2, 1, 3], 32, 8, 16,
-                                         holes=6))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_holes_in_the_tables(dtype):
+    for seed, rows in enumerate(([1, 2, 1, 3], [20, 2, 1, 3], [12, 30, 9, 30])):
+        _run(osp.make_shared_prefix_case(10 + seed, [430, 340], [2, 2], [20, 70, 0, 33], rows, 32, 8, 16, dtype,
+                                         holes=12))
     # every page a hole: nothing to see, zeros
     case = osp.make_shared_prefix_case(14, [40], [2], [20, 30], [1, 2], 32, 8, 16)
     case["prefix_tables"].fill_(-1)
@@ -131,9 +151,10 @@ def test_lengths_past_the_tables_are_cut_off():
     case["prefix_tables"] = case["prefix_tables"][:, :4].contiguous()
     case["block_tables"] = case["block_tables"][:, :2].contiguous()
     full = _run(case)
-    case["prefix_lens"] += 1000
+    if not REACH:
+        case["prefix_lens"] += 1000
     case["context_lens"] += 5000
-    assert torch.equal(_run(case), full)
+    assert torch.equal(_to_gpu_run(case), full)
     case["prefix_lens"].fill_(-5)
     case["context_lens"].fill_(-5)
     assert not bool(_to_gpu_run(case).any())
@@ -146,17 +167,19 @@ def _to_gpu_run(case, **kw):
     return out
 
 
-def test_peaked_and_flat_scores():
+@pytest.mark.parametrize("rows", [[2, 1, 1], [20, 11, 3]])
+def test_peaked_and_flat_scores(rows):
     """Large scores (one key takes all the weight; rising maxima along the keys) and none (q = 0)."""
-    case = osp.make_shared_prefix_case(16, [500], [3], [40, 80, 3], [2, 1, 1], 32, 8, 16, q_gain=12.0)
+    case = osp.make_shared_prefix_case(16, [500], [3], [40, 80, 3], rows, 32, 8, 16, q_gain=12.0)
     _run(case)
     case["q"].zero_()
     _run(case)
-    rising = osp.make_shared_prefix_case(17, [512], [2], [64, 10], [1, 1], 8, 8, 16)
+    rising = osp.make_shared_prefix_case(17, [512], [2], [64, 10], [30, 9] if rows[0] > 2 else [1, 1], 8, 8, 16)
     order = rising["prefix_tables"][0]
     k = rising["k_cache"].float()
     for j in range(512):  # scores grow steadily: the running maximum moves in every tile
         k[order[j // 16], j % 16] = rising["q"][0].float() * (0.02 * j - 4.0) / 8.0
+    rising["q"][1:] = rising["q"][:1] * torch.linspace(0.5, 1.0, len(rising["q"]) - 1)[:, None, None]
     rising["k_cache"] = k.to(torch.float8_e4m3fn)
     _run(rising)
 
@@ -283,6 +306,28 @@ def test_agrees_with_the_decode_and_prefill_entries():
     many = paged_prefill(case["q"], case["k_cache"], case["v_cache"], joined, case["cu_seqlens_q"], cu_k, 5,
                          case["scale"])
     assert rel_l2(out, many) < 2 * REL[torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_queries_of_any_size(dtype):
+    """Rows scaled from the smallest normal numbers to the largest, and rows with one large element."""
+    case = osp.make_shared_prefix_case(26, [200], [3], [20, 33, 40], [20, 16, 9], 32, 8, 16, dtype)
+    top = 1e30 if dtype == torch.bfloat16 else 6e4
+    gain = torch.logspace(-4.0, 0.0, 45)
+    case["q"] = (case["q"].float() * gain[:, None, None]).to(dtype)
+    case["q"][3, :, 5] = 30.0
+    case["q"][7, :, 77] = -200.0
+    _run(case)
+    case["q"][0] = top / 8 * torch.sign(case["q"][0].float() + 1e-9).to(dtype)  # one key takes it all
+    a, k = _args(_to_gpu(case))
+    out = shared_prefix_decode(*a, **k)
+    assert bool(torch.isfinite(out[0].float()).all())
+    case["q"][1, 2, 3] = float("inf")
+    case["q"][2, 4, 100] = float("nan")
+    a, k = _args(_to_gpu(case))
+    out = shared_prefix_decode(*a, **k).float().cpu()
+    assert bool(torch.isnan(out[1, 2]).all()) and bool(torch.isnan(out[2, 4]).all())
+    assert int(torch.isnan(out).any(-1).sum()) == 2  # and no other row
 
 
 def test_empty_calls():
