@@ -147,7 +147,7 @@ struct Scale {
     t = greedy ? 1.f : temp;
     c = L / t;
     c_lo = (fmaf(-c, t, L) + L_LO) / t;
-    least = -200.f / c;
+    least = -138.62944f * t;  // -200 ln 2 T
   }
   // x - m, at most 0: -inf and NaN give `least` (weight 0), +inf gives 0.
   __device__ __forceinline__ float diff(float x, float m) const { return fminf(fmaxf(x - m, least), 0.f); }

@@ -16,18 +16,16 @@ from torch import nn
 from . import _native as N
 
 
-def _rows(t: torch.Tensor, name: str, dim: int = 2) -> torch.Tensor:
-    if t.dim() != dim:
-        raise ValueError(f"{name} must have {dim} dimensions")
+F32 = torch.float32
+
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    """t with unit stride in its last dimension."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _ld(t: torch.Tensor, rows: int, cols: int) -> int:
-    return t.stride(0) if rows > 1 else max(t.stride(0), cols)
-
-
-def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
-    if t.dtype != dtype or t.numel() != n:
+def _dense(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
+    if t.dtype is not dtype or t.numel() != n:
         raise ValueError(f"{name} must be {dtype} with {n} entries")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -40,23 +38,22 @@ def sample(logits: torch.Tensor, temperatures: torch.Tensor,
     Returns (tokens int64 [R], logprobs fp32 [R], lse fp32 [R]): the draw, its log-probability
     and the row's log-normaliser, both at the row's temperature (1 where greedy).  A row whose
     logits are all -inf gives -1, 0 and -inf."""
-    N.require_cuda(logits, temperatures, noise, what="sample")
-    logits, noise = _rows(logits, "logits"), _rows(noise, "noise")
+    if not (logits.is_cuda and temperatures.is_cuda and noise.is_cuda):
+        raise RuntimeError("sample requires CUDA tensors")
     r, v = logits.shape
     code = N.DT_LOGITS.get(logits.dtype)
-    if code is None or noise.dtype != torch.float32 or noise.shape != logits.shape:
+    if code is None or noise.dtype is not F32 or noise.shape != logits.shape:
         raise ValueError("logits must be bf16, fp16 or fp32, and noise fp32 with one entry per logit")
-    temperatures = _vector(temperatures, "temperatures", torch.float32, r)
-    d = logits.device
-    tokens = torch.empty(r, dtype=torch.int64, device=d)
-    logprobs = torch.empty(r, dtype=torch.float32, device=d)
-    lse = torch.empty(r, dtype=torch.float32, device=d)
+    logits, noise = _unit(logits), _unit(noise)
+    temperatures = _dense(temperatures, "temperatures", F32, r)
+    tokens = temperatures.new_empty(r, dtype=torch.int64)
+    logprobs, lse = temperatures.new_empty(r), temperatures.new_empty(r)
     if r == 0:
         return tokens, logprobs, lse
-    stream = N.stream_ptr(d)
-    st = N.lib().ada_sample(logits.data_ptr(), code, _ld(logits, r, v), r, v, temperatures.data_ptr(),
-                            noise.data_ptr(), _ld(noise, r, v), tokens.data_ptr(), logprobs.data_ptr(),
-                            lse.data_ptr(), stream)
+    # (a single row may have any stride)
+    ld, ld_noise = (logits.stride(0), noise.stride(0)) if r > 1 else (v, v)
+    st = N.lib().ada_sample(logits.data_ptr(), code, ld, r, v, temperatures.data_ptr(), noise.data_ptr(), ld_noise,
+                            tokens.data_ptr(), logprobs.data_ptr(), lse.data_ptr(), N.stream_ptr(logits.device))
     if st:
         N.check(st, "sampling kernel")
     return tokens, logprobs, lse
@@ -82,43 +79,50 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     workspace: at least verify_workspace_bytes(...) bytes (default: one kept per stream).
     Returns (tokens int64 [B, D + 1], accepted int32 [B], logprobs fp32 [B, D + 1]): the accepted
     drafts and the drawn token with their log-probabilities under the target, then -1 and 0."""
-    N.require_cuda(target_logits, input_ids, cu_seqlens_q, temperatures, uniforms, noise, draft_logits, draft_lse,
-                   workspace, what="verify_drafts")
-    target_logits, noise = _rows(target_logits, "target_logits"), _rows(noise, "noise")
-    uniforms = _rows(uniforms, "uniforms")
+    drafter = draft_logits is not None
+    if not (target_logits.is_cuda and input_ids.is_cuda and cu_seqlens_q.is_cuda and temperatures.is_cuda
+            and uniforms.is_cuda and noise.is_cuda):
+        raise RuntimeError("verify_drafts requires CUDA tensors")
     (n, v), (b, most) = target_logits.shape, uniforms.shape
     dtype = target_logits.dtype
     code = N.DT_LOGITS.get(dtype)
-    if code is None or noise.dtype != torch.float32 or uniforms.dtype != torch.float32 or noise.shape != (b, v):
+    if code is None or noise.dtype is not F32 or uniforms.dtype is not F32 or noise.shape != (b, v):
         raise ValueError("target_logits must be bf16, fp16 or fp32, uniforms and noise [batch, vocab] fp32")
-    temperatures = _vector(temperatures, "temperatures", torch.float32, b)
-    input_ids = _vector(input_ids, "input_ids", torch.int64, n)
-    cu_seqlens_q = _vector(cu_seqlens_q, "cu_seqlens_q", torch.int32, b + 1)
-    if (draft_logits is None) != (draft_lse is None):
+    target_logits, noise, uniforms = _unit(target_logits), _unit(noise), _unit(uniforms)
+    temperatures = _dense(temperatures, "temperatures", F32, b)
+    input_ids = _dense(input_ids, "input_ids", torch.int64, n)
+    cu_seqlens_q = _dense(cu_seqlens_q, "cu_seqlens_q", torch.int32, b + 1)
+    if drafter != (draft_lse is not None):
         raise ValueError("draft_logits and draft_lse come together")
-    strides = (0, 0, 0, 0)
-    if draft_logits is not None:
-        draft_logits = _rows(draft_logits, "draft_logits", 3)
-        if (draft_logits.dtype != dtype or draft_logits.shape != (b, most, v) or draft_lse.shape != (b, most)
-                or draft_lse.dtype != torch.float32):
+    if drafter:
+        if not (draft_logits.is_cuda and draft_lse.is_cuda):
+            raise RuntimeError("verify_drafts requires CUDA tensors")
+        if (draft_logits.dtype is not dtype or draft_logits.shape != (b, most, v) or draft_lse.shape != (b, most)
+                or draft_lse.dtype is not F32):
             raise ValueError("draft_logits must be [batch, drafts, vocab] like the target's, draft_lse fp32 "
                              "[batch, drafts]")
-        strides = draft_logits.stride()[:2] + draft_lse.stride()
-    d = target_logits.device
-    tokens = torch.empty((b, most + 1), dtype=torch.int64, device=d)
-    logprobs = torch.empty((b, most + 1), dtype=torch.float32, device=d)
-    accepted = torch.empty(b, dtype=torch.int32, device=d)
+        draft_logits = _unit(draft_logits)
+        (db, dd, _), (lb, ld) = draft_logits.stride(), draft_lse.stride()
+        draft, lse = draft_logits.data_ptr(), draft_lse.data_ptr()
+    else:
+        db = dd = lb = ld = 0
+        draft = lse = None
+    tokens = temperatures.new_empty((b, most + 1), dtype=torch.int64)
+    logprobs = temperatures.new_empty((b, most + 1))
+    accepted = cu_seqlens_q.new_empty(b)
     if b == 0:
         return tokens, accepted, logprobs
-    stream = N.stream_ptr(d)
+    device = target_logits.device
+    stream = N.stream_ptr(device)
     if workspace is None:
-        workspace = N.workspace(d, stream, verify_workspace_bytes(n, b, v, dtype))
+        workspace = N.workspace(device, stream, verify_workspace_bytes(n, b, v, dtype))
+    # (a single row may have any stride)
+    ld_u, ld_noise = (uniforms.stride(0), noise.stride(0)) if b > 1 else (most, v)
     st = N.lib().ada_verify_drafts(
-        target_logits.data_ptr(), code, _ld(target_logits, n, v), n, v, input_ids.data_ptr(),
-        cu_seqlens_q.data_ptr(), b, most, temperatures.data_ptr(), uniforms.data_ptr(), _ld(uniforms, b, most),
-        noise.data_ptr(), _ld(noise, b, v), N.ptr(draft_logits), strides[0], strides[1], N.ptr(draft_lse), strides[2],
-        strides[3], tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), stream)
+        target_logits.data_ptr(), code, target_logits.stride(0) if n > 1 else v, n, v, input_ids.data_ptr(),
+        cu_seqlens_q.data_ptr(), b, most, temperatures.data_ptr(), uniforms.data_ptr(), ld_u, noise.data_ptr(),
+        ld_noise, draft, db, dd, lse, lb, ld, tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(),
+        workspace.data_ptr(), workspace.nbytes, stream)
     if st:
         N.check(st, "draft verification kernel")
     return tokens, accepted, logprobs

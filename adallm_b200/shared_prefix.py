@@ -21,9 +21,13 @@ def shared_prefix_workspace_bytes(total_q: int, num_groups: int, batch: int, num
                                                                    num_kv_heads, head_dim))
 
 
-def _check_int32(t: torch.Tensor | None, name: str) -> None:
-    if t is not None and (t.dtype is not torch.int32 or (t.numel() > 1 and t.stride(-1) != 1)):
+I32 = torch.int32
+
+
+def _lengths(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dtype is not I32 or not t.is_contiguous():
         raise ValueError(f"{name} must be int32 with unit stride")
+    return t
 
 
 def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_tables: torch.Tensor,
@@ -45,13 +49,14 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     Returns [N, Hq, 128] in q.dtype.  workspace: at least shared_prefix_workspace_bytes(...) bytes
     (default: one kept per stream).  err: optional int32 [1] device word; 0x90 is OR-ed in if a
     tile wait ran out."""
-    N.require_cuda(q, k_cache, v_cache, prefix_tables, prefix_lens, block_tables, context_lens, cu_groups,
-                   cu_seqlens_q, out, workspace, err, what="shared_prefix_decode")
+    if not (q.is_cuda and k_cache.is_cuda and v_cache.is_cuda and prefix_tables.is_cuda and prefix_lens.is_cuda
+            and block_tables.is_cuda and context_lens.is_cuda):
+        raise RuntimeError("shared_prefix_decode requires CUDA tensors")
     total_q, hq, d = q.shape
     pages, page, hkv, dk = shape = k_cache.shape
     if q.stride(-1) != 1:
         q = q.contiguous()
-    qs, ks = q.stride(), k_cache.stride()
+    qs, ks, pts, bts = q.stride(), k_cache.stride(), prefix_tables.stride(), block_tables.stride()
     code = N.DT.get(q.dtype)
     if code is None or (out is not None and out.dtype not in N.DT):
         raise ValueError("q and out must be bf16 or fp16")
@@ -59,12 +64,17 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError("k_cache and v_cache must share a [pages, page, Hkv, D] layout with q's head size")
     if k_cache.dtype is not torch.float8_e4m3fn or v_cache.dtype is not torch.float8_e4m3fn:
         raise ValueError("the shared-prefix decode reads a float8_e4m3fn cache")
-    _check_int32(prefix_tables, "prefix_tables")
-    _check_int32(prefix_lens, "prefix_lens")
-    _check_int32(cu_groups, "cu_groups")
-    _check_int32(block_tables, "block_tables")
-    _check_int32(context_lens, "context_lens")
-    _check_int32(cu_seqlens_q, "cu_seqlens_q")
+    if prefix_tables.dtype is not I32 or block_tables.dtype is not I32 or pts[1] != 1 or bts[1] != 1:
+        raise ValueError("prefix_tables and block_tables must be int32 with unit stride")
+    _lengths(prefix_lens, "prefix_lens")
+    _lengths(context_lens, "context_lens")
+    cu_g = cu_q = None
+    if cu_groups is not None:
+        N.require_cuda(cu_groups, what="shared_prefix_decode")
+        cu_g = _lengths(cu_groups, "cu_groups").data_ptr()
+    if cu_seqlens_q is not None:
+        N.require_cuda(cu_seqlens_q, what="shared_prefix_decode")
+        cu_q = _lengths(cu_seqlens_q, "cu_seqlens_q").data_ptr()
     groups, batch = prefix_lens.numel(), context_lens.numel()
     (pt_rows, pt_pages), (bt_rows, bt_pages) = prefix_tables.shape, block_tables.shape
     if pt_rows != groups or bt_rows != batch:
@@ -75,9 +85,10 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError("cu_seqlens_q must have batch + 1 entries (None for one row per sequence)")
     device = q.device
     if out is None:
-        out = torch.empty((total_q, hq, d), dtype=q.dtype, device=device)
+        out = q.new_empty((total_q, hq, d))
         os, out_code = (hq * d, d), code
     else:
+        N.require_cuda(out, what="shared_prefix_decode")
         os, out_code = out.stride(), N.DT[out.dtype]
         if out.shape != q.shape or os[2] != 1:
             raise ValueError("out must have q's shape and unit stride in the head dimension")
@@ -91,10 +102,10 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         workspace = N.workspace(device, stream, need)
     st = N.lib().ada_fp8_shared_prefix_decode(
         q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], pages,
-        prefix_tables.data_ptr(), prefix_tables.stride(0), pt_pages, prefix_lens.data_ptr(), N.ptr(cu_groups), groups,
-        block_tables.data_ptr(), block_tables.stride(0), bt_pages, context_lens.data_ptr(), N.ptr(cu_seqlens_q), batch,
-        total_q, hq, hkv, d, page, scale, k_scale, v_scale, window, out.data_ptr(), out_code, os[0], os[1],
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), N.ptr(err), stream)
+        prefix_tables.data_ptr(), pts[0], pt_pages, prefix_lens.data_ptr(), cu_g, groups,
+        block_tables.data_ptr(), bts[0], bt_pages, context_lens.data_ptr(), cu_q, batch,
+        total_q, hq, hkv, d, page, float(scale), float(k_scale), float(v_scale), int(window), out.data_ptr(), out_code, os[0], os[1],
+        workspace.data_ptr(), workspace.nbytes, N.ptr(err), stream)
     if st:
         N.check(st, "shared-prefix decode attention")
     return out
