@@ -523,9 +523,9 @@ __global__ void __launch_bounds__(STAT_THREADS, 4) row_stats_kernel(VerifyParams
 
 // A share of the race for one token: the candidates of packets [k0, k1) of a row, weights
 // max(p - q, 0), returned as (score bits << 32 | ~index) in every lane of the warp; 0: none.  `known`
-// is a score that some share has reached.  p bounds what is left of it, so a packet in which no p / e
-// reaches that score is done with; the others (about 1 / (1 - a) of a row's tokens, where a is the
-// chance that the draft was accepted, and each warp's first) take q into account.
+// is a score that some share has reached.  p bounds what is left of it, so elements whose p / e does not
+// reach that score are done with; the others (about 1 / (1 - a) of a row's tokens, where a is the chance
+// that the draft was accepted) take q into account.  Every thread of the CTA calls.
 template <typename T, bool VEC, int NT>
 __device__ __forceinline__ unsigned long long draw_share(const T* x, const T* dr, const float* e, int n, int k0, int k1,
                                                          const Scale& sc, float m, float s, float dl, int struck,
@@ -543,8 +543,39 @@ __device__ __forceinline__ unsigned long long draw_share(const T* x, const T* dr
     if (dr) rawd[u] = load_pack<T, VEC>(dr, base + lane, n);
     load_noise<T, VEC>(e, base + lane, n, ns[u]);
   };
+  auto consider = [&](float v, float d, float noise, int at) {
+    float w = sc.weight_exact(sc.diff(v, m)) * inv;
+    if (dr) w = fmaxf(w - draft_prob(d, sc, dl), 0.f);
+    if (at == struck) w = fmaxf(w - 1.f, 0.f);
+    const float ei = exponential(noise);
+    if (w * best.e > best.w * ei) best = Best{w, ei, at};
+  };
+  auto publish = [&](float score) {
+    const float reached = warp_max(best.w / best.e);
+    if (lane == 0 && reached > score) atomicMax(const_cast<int*>(known), __float_as_int(reached));
+  };
 #pragma unroll
   for (int u = 0; u < U; ++u) load(u, k0 + warp * 32 + u * NT);
+  // A first bound: of each lane's first packet the element with the largest p / e.
+  if (k0 + warp * 32 < k1) {
+    float v[N], most = -1.f, mv = 0.f, md = 0.f, me = 1.f;
+    int mi = 0;
+    unpack<T>(raw[0], v);
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const float r = __fdividef(sc.weight(sc.diff(v[c], m)), exponential(ns[0][c]));
+      if (r > most) {
+        most = r;
+        mv = v[c];
+        md = dr ? element<T>(rawd[0], c) : 0.f;
+        me = ns[0][c];
+        mi = c;
+      }
+    }
+    consider(mv, md, me, pack_index<T, VEC>(k0 + warp * 32 + lane, mi));
+    publish(0.f);
+  }
+  __syncthreads();
   for (int base = k0 + warp * 32; base < k1; base += NT * U) {  // warp-uniform
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -554,24 +585,20 @@ __device__ __forceinline__ unsigned long long draw_share(const T* x, const T* dr
       const float least = score * SLACK * s;  // against s p
       float v[N];
       unpack<T>(raw[u], v);
-      bool hit = false;
+      unsigned hits = 0;
 #pragma unroll
       for (int c = 0; c < N; c += 2) {
         const float2 t = mul2(make_float2(ns[u][c], ns[u][c + 1]), make_float2(least, least));
-        hit |= !(sc.weight(sc.diff(v[c], m)) <= t.x) | !(sc.weight(sc.diff(v[c + 1], m)) <= t.y);
+        hits |= !(sc.weight(sc.diff(v[c], m)) <= t.x) ? 1u << c : 0u;
+        hits |= !(sc.weight(sc.diff(v[c + 1], m)) <= t.y) ? 2u << c : 0u;
       }
-      if (__any_sync(0xffffffffu, hit)) {
+      const unsigned any = __reduce_or_sync(0xffffffffu, hits);
+      if (any) {
 #pragma unroll
-        for (int c = 0; c < N; ++c) {
-          const int at = pack_index<T, VEC>(k, c);
-          float w = sc.weight_exact(sc.diff(v[c], m)) * inv;
-          if (dr) w = fmaxf(w - draft_prob(element<T>(rawd[u], c), sc, dl), 0.f);
-          if (at == struck) w = fmaxf(w - 1.f, 0.f);
-          const float ei = exponential(ns[u][c]);
-          if (w * best.e > best.w * ei) best = Best{w, ei, at};
-        }
-        const float reached = warp_max(best.w / best.e);
-        if (lane == 0 && reached > score) atomicMax(const_cast<int*>(known), __float_as_int(reached));
+        for (int c = 0; c < N; ++c)
+          if ((any >> c) & 1u)  // warp-uniform: the few places where some lane has a candidate
+            consider(v[c], dr ? element<T>(rawd[u], c) : 0.f, ns[u][c], pack_index<T, VEC>(k, c));
+        publish(score);
       }
       load(u, base + (u + U) * NT);
     }
