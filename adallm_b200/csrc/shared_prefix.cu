@@ -1540,7 +1540,7 @@ inline bool smem_ready(int bytes) {
   static std::atomic<int> done[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-  if (done[dev] >= bytes) return true;
+  if (done[dev] == bytes) return true;
   if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
       cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared) !=
           cudaSuccess)
@@ -1553,7 +1553,11 @@ inline bool smem_ready(int bytes) {
 // (a prefix of 16 rows ran faster as two blocks of 8 than as one of 16: 54 against 72 us for 8 x 8 samples).
 inline int row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
+// pieces_kernel keeps the segments in shared memory behind its rings; its limit is set once, for the most
+// there may be, so that calls of different batches on different threads cannot lower it under one another.
 constexpr int MAX_SEGMENTS = 4096;
+constexpr int pieces_smem(int segs) { return 1024 + WARPS * RING_BYTES + segs * ((int)sizeof(Segment) + 12) + 4; }
+static_assert(pieces_smem(MAX_SEGMENTS) + 8 * 1024 <= 227 * 1024, "the segments have to fit beside the rings");
 constexpr int PIECES_PER_SM = 3 * WARPS;
 
 // prefix_kernel takes the prefixes from 33 rows a prefix and KV head on (with fewer, its 128-row tiles stay
@@ -1708,11 +1712,10 @@ extern "C" int ada_fp8_shared_prefix_decode(
     }
     ADA_CHECK_LAUNCH();
   }
-  const int segs = num_groups + batch;
-  const int smem = 1024 + sp::WARPS * sp::RING_BYTES + segs * ((int)sizeof(sp::Segment) + 12) + 4;
+  const int smem = sp::pieces_smem(num_groups + batch);
 #define ADA_SP(TQ, NB)                                                                                              \
   do {                                                                                                              \
-    if (!sp::smem_ready<sp::pieces_kernel<TQ, NB>>(smem)) return ADA_ERR_CUDA;                                      \
+    if (!sp::smem_ready<sp::pieces_kernel<TQ, NB>>(sp::pieces_smem(sp::MAX_SEGMENTS))) return ADA_ERR_CUDA;         \
     (void)ada::launch_k(sp::pieces_kernel<TQ, NB>, dim3((unsigned)(sms * (NB == 1 ? 3 : 2))), dim3(sp::WARPS * 32), \
                         smem, st, tmk, tmv, P);                                                                     \
   } while (0)

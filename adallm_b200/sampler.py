@@ -116,6 +116,8 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     stream = N.stream_ptr(device)
     if workspace is None:
         workspace = N.workspace(device, stream, verify_workspace_bytes(n, b, v, dtype))
+    else:
+        N.require_cuda(workspace, what="verify_drafts")
     # (a single row may have any stride)
     ld_u, ld_noise = (uniforms.stride(0), noise.stride(0)) if b > 1 else (most, v)
     st = N.lib().ada_verify_drafts(

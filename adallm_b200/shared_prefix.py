@@ -47,7 +47,7 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     Row i of t attends to positions <= prefix + context - t + i, with window W > 0 to the last W
     of them.  Rows that see no key are zeros.
     Returns [N, Hq, 128] in q.dtype.  workspace: at least shared_prefix_workspace_bytes(...) bytes
-    (default: one kept per stream).  err: optional int32 [1] device word; 0x90 is OR-ed in if a
+    (default: one kept per stream).  At most 4096 prefixes and sequences together.  err: optional int32 [1] device word; 0x90 is OR-ed in if a
     tile wait ran out."""
     if not (q.is_cuda and k_cache.is_cuda and v_cache.is_cuda and prefix_tables.is_cuda and prefix_lens.is_cuda
             and block_tables.is_cuda and context_lens.is_cuda):
@@ -100,12 +100,16 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     need = shared_prefix_workspace_bytes(total_q, groups, batch, hq, hkv, d)
     if workspace is None:
         workspace = N.workspace(device, stream, need)
+    else:
+        N.require_cuda(workspace, what="shared_prefix_decode")
+    if err is not None:
+        N.require_cuda(err, what="shared_prefix_decode")
     st = N.lib().ada_fp8_shared_prefix_decode(
         q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], pages,
         prefix_tables.data_ptr(), pts[0], pt_pages, prefix_lens.data_ptr(), cu_g, groups,
         block_tables.data_ptr(), bts[0], bt_pages, context_lens.data_ptr(), cu_q, batch,
-        total_q, hq, hkv, d, page, float(scale), float(k_scale), float(v_scale), int(window), out.data_ptr(), out_code, os[0], os[1],
-        workspace.data_ptr(), workspace.nbytes, N.ptr(err), stream)
+        total_q, hq, hkv, d, page, float(scale), float(k_scale), float(v_scale), int(window), out.data_ptr(), out_code,
+        os[0], os[1], workspace.data_ptr(), workspace.nbytes, N.ptr(err), stream)
     if st:
         N.check(st, "shared-prefix decode attention")
     return out

@@ -591,7 +591,7 @@ ADA_API int ada_argmax_noalloc(const void* logits, int64_t ld, int64_t rows, int
  *          of no sequence, and rows that see no key, are written as zeros
  * err      optional uint32 word: 0x90 is OR-ed in if a tile wait ran out (~2 s)
  * Implemented: head_dim 128, num_heads / num_kv_heads <= 128, page_size % 16 == 0,
- * scale * k_scale > 0.  workspace: ada_fp8_shared_prefix_decode_workspace_size bytes, 256-byte
+ * num_groups + batch <= 4096, scale * k_scale > 0.  workspace: ada_fp8_shared_prefix_decode_workspace_size bytes, 256-byte
  * aligned, no initial value; calls that share one must be ordered.
  * ---------------------------------------------------------------------- */
 ADA_API size_t ada_fp8_shared_prefix_decode_workspace_size(int32_t total_q, int32_t num_groups, int32_t batch,

@@ -314,3 +314,30 @@ def test_same_result_twice_on_another_stream_and_in_a_graph():
         graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, first))
+
+
+def test_refusals():
+    x = torch.zeros((3, 50), device=dev())
+    t, e = torch.ones(3, device=dev()), torch.ones((3, 50), device=dev())
+    for a in ((x.double(), t, e), (x, t, e.half()), (x, t, e[:, :49]), (x, t[:2], e), (x, t.double(), e)):
+        with pytest.raises(ValueError):
+            sample(*a)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        sample(x, t.cpu(), e)
+    good = dict(target_logits=x, input_ids=torch.zeros(3, dtype=torch.int64, device=dev()),
+                cu_seqlens_q=torch.tensor([0, 3], dtype=torch.int32, device=dev()), temperatures=t[:1],
+                uniforms=torch.zeros((1, 2), device=dev()), noise=e[:1], draft_logits=x[None, :2],
+                draft_lse=torch.zeros((1, 2), device=dev()))
+    wrong = [dict(target_logits=x.double()), dict(input_ids=good["input_ids"].int()), dict(input_ids=good["input_ids"][:2]),
+             dict(cu_seqlens_q=good["cu_seqlens_q"][:1]), dict(cu_seqlens_q=good["cu_seqlens_q"].long()),
+             dict(temperatures=t), dict(uniforms=good["uniforms"].half()), dict(noise=e), dict(draft_lse=None),
+             dict(draft_logits=None), dict(draft_logits=x[None]), dict(draft_logits=x[None, :2].half()),
+             dict(draft_lse=torch.zeros((1, 3), device=dev())),
+             dict(workspace=torch.empty(16, dtype=torch.uint8, device=dev()))]
+    for kw in wrong:
+        with pytest.raises(ValueError):
+            verify_drafts(**{**good, **kw})
+    for name in good:
+        with pytest.raises(RuntimeError, match="CUDA"):
+            verify_drafts(**{**good, name: good[name].cpu()})
+    verify_drafts(**good)

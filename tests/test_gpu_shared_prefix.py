@@ -2,8 +2,8 @@
 
 Tolerances.  Inputs are exact on both sides (bf16/fp16 queries, e4m3 cache); what is left is the
 fp32 score (relative 2^-20 or so), probabilities held in no fewer than 11 bits for P.V (at most
-2^-11 of each weight) and the output's own rounding (at most 2^-9 relative for bf16, 2^-12 fp16).
-Element-wise: 2^-9 (2^-12) of the element plus 2^-10 of the largest |v| of the case (weights sum to
+2^-11 of each weight) and the output's own rounding (at most 2^-8 relative for bf16, 2^-11 fp16).
+Element-wise: 2^-8 (2^-11) of the element plus 2^-10 of the largest |v| of the case (weights sum to
 one, so their rounding moves an element by at most 2^-11 max|v|; doubled for the row sum and the
 scores).  Over all elements: roundings are spread evenly below their bounds, so the relative
 2-norm is below 2^-8.5 (bf16) and 2^-10 (fp16)."""
@@ -336,3 +336,39 @@ def test_empty_calls():
     k = {"cu_seqlens_q": torch.zeros(3, dtype=torch.int32, device=dev())}
     assert shared_prefix_decode(case["q"][:0], *a[1:], **k).shape == (0, 32, 128)
     assert not bool(shared_prefix_decode(*a, **k).any())  # rows, but none of them owned
+
+
+def test_as_many_sequences_as_there_may_be():
+    """4,095 sequences behind one prefix; one more is refused."""
+    n = 4095
+    case = osp.make_shared_prefix_case(26, [20], [n], [1 + i % 3 for i in range(n)], [1] * n, 2, 2, 16)
+    out = _run(case)
+    c = _to_gpu(case)
+    with pytest.raises(ValueError):
+        shared_prefix_decode(out[:1].expand(n + 1, -1, -1), c["k_cache"], c["v_cache"], c["prefix_tables"],
+                             c["prefix_lens"], None, c["block_tables"][:1].expand(n + 1, -1),
+                             c["context_lens"][:1].repeat(n + 1), 1.0)
+
+
+def test_refusals():
+    case = _to_gpu(osp.make_shared_prefix_case(27, [20], [2], [5, 6], [1, 1], 32, 8, 16))
+    good = dict(zip(("q", "k_cache", "v_cache", "prefix_tables", "prefix_lens", "cu_groups", "block_tables",
+                     "context_lens", "scale"), _args(case)[0]))
+    need = shared_prefix_workspace_bytes(2, 1, 2, 32, 8, 128)
+    q, k, v = good["q"], good["k_cache"], good["v_cache"]
+    wrong = [dict(q=q.float()), dict(q=q[..., :64]), dict(q=q[:1]), dict(q=q[:, :30]), dict(k_cache=k.view(torch.uint8)),
+             dict(v_cache=v[:, :, :4]), dict(prefix_tables=good["prefix_tables"].long()),
+             dict(prefix_lens=good["prefix_lens"].long()), dict(prefix_lens=good["prefix_lens"].repeat(2)),
+             dict(cu_groups=good["cu_groups"][:1]), dict(block_tables=good["block_tables"][:1]),
+             dict(context_lens=good["context_lens"].float()), dict(scale=0.0), dict(scale=float("nan")),
+             dict(scale=-1.0), dict(window=-1), dict(cu_seqlens_q=torch.zeros(2, dtype=torch.int32, device=dev())),
+             dict(out=q.float()), dict(out=q[:1]), dict(workspace=torch.empty(need - 256, dtype=torch.uint8, device=dev()))]
+    for kw in wrong:
+        with pytest.raises(ValueError):
+            shared_prefix_decode(**{**good, **kw})
+    for name in ("q", "k_cache", "v_cache", "prefix_tables", "prefix_lens", "block_tables", "context_lens", "cu_groups"):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            shared_prefix_decode(**{**good, name: good[name].cpu()})
+    with pytest.raises(RuntimeError, match="CUDA"):
+        shared_prefix_decode(**good, workspace=torch.empty(need, dtype=torch.uint8))
+    assert bool(torch.isfinite(shared_prefix_decode(**good).float()).all())

@@ -45,6 +45,7 @@ def test_shared_prefix_argument_errors(lib):
     assert call(total_q=-1) == N.ADA_ERR_INVALID_ARG and call(num_pages=0) == N.ADA_ERR_INVALID_ARG
     assert call(d=64) == N.ADA_ERR_UNSUPPORTED and call(page=24) == N.ADA_ERR_UNSUPPORTED
     assert call(hq=256, hkv=1) == N.ADA_ERR_UNSUPPORTED
+    assert call(batch=4096, total_q=4096) == N.ADA_ERR_UNSUPPORTED     # 4,097 prefixes and sequences
     assert call(max_pp=1 << 27, pt_stride=1 << 27) == N.ADA_ERR_UNSUPPORTED
     assert call(q=P + 8) == N.ADA_ERR_ALIGNMENT and call(k=P + 8) == N.ADA_ERR_ALIGNMENT
     assert call(s_tok=1032) == N.ADA_ERR_ALIGNMENT and call(q_sh=100) == N.ADA_ERR_ALIGNMENT
