@@ -776,28 +776,26 @@ inline Split split_for(int64_t rows, int64_t vocab) {
   return {c, rows * c <= 148};
 }
 
-// Shares of a row in the verification kernels (256 threads, `resident` CTAs on the card at once): the
-// fewest waves that fill at least nine tenths of their CTAs, up to four, else the fullest; at least
-// one packet a thread.
-inline void row_shares(int64_t rows, int64_t vocab, int pack, int64_t resident, int* chunks, int* packs) {
+// Shares of a row in the verification kernels (256 threads, `resident` CTAs on the card at once): what
+// takes least if a wave of CTAs takes `fixed` + the packets a thread of one of its shares reads, up to four
+// waves, at least one packet a thread.  Nothing fixed for the row statistics; for the draw the judging of
+// the drafts, about 8 us or 12 packets: 100 sequences of 3 rows of 151936 in one wave 49 us, in four full
+// ones 62.
+inline void row_shares(int64_t rows, int64_t vocab, int pack, int64_t resident, int64_t fixed, int* chunks,
+                       int* packs) {
   const int64_t units = cdiv(vocab, 256 * pack);  // packets a thread of a lone CTA
-  int64_t best = 1;
-  double best_fill = 0;
+  int64_t best = units, least = INT64_MAX;        // packets a thread of a share, its cost
   for (int w = 1; w <= 4; ++w) {
     int64_t c = rows > 0 ? w * resident / rows : 1;
     c = c < 1 ? 1 : (c > units ? units : c);
-    const int64_t per = cdiv(units, c);
-    c = cdiv(units, per);
-    const double fill = (double)(rows * units) / (double)(cdiv(rows * c, resident) * resident * per);
-    if (fill > best_fill * 1.02) {
-      best_fill = fill;
-      best = c;
+    const int64_t per = cdiv(units, c), cost = cdiv(rows * cdiv(units, per), resident) * (per + fixed);
+    if (cost < least) {
+      least = cost;
+      best = per;
     }
-    if (fill >= 0.9) break;
   }
-  const int64_t per = cdiv(units, best);
-  *packs = (int)per * 256;
-  *chunks = (int)cdiv(units, per);
+  *packs = (int)best * 256;
+  *chunks = (int)cdiv(units, best);
 }
 
 template <auto Kernel, typename... Args>
@@ -841,8 +839,8 @@ int verify_typed(VerifyParams P, cudaStream_t st) {
 // Workspace: the row statistics, then the draw's words.
 inline size_t verify_layout(VerifyParams& P, int64_t total_q, int64_t batch, int64_t vocab, int dtype, void* ws) {
   const int pack = 16 / dtype_size(dtype);
-  row_shares(total_q, vocab, pack, 4 * 148, &P.chunks, &P.chunk_packs);
-  row_shares(batch, vocab, pack, 3 * 148, &P.draw_chunks, &P.draw_packs);
+  row_shares(total_q, vocab, pack, 4 * 148, 0, &P.chunks, &P.chunk_packs);
+  row_shares(batch, vocab, pack, 3 * 148, 12, &P.draw_chunks, &P.draw_packs);
   const size_t part = (size_t)total_q * P.chunks * sizeof(float4);
   P.part = reinterpret_cast<float4*>(ws);
   P.best = reinterpret_cast<unsigned long long*>(reinterpret_cast<char*>(ws) + part);
