@@ -666,6 +666,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 3) draw_kernel(VerifyParams P) {
       pdl_wait();
       pdl_trigger();
       waited = true;
+      if (tid == 0) s_known = (int)(*const_cast<volatile unsigned long long*>(P.best + b) >> 32);
     }
     for (int i = warp; i < rows; i += WARPS) {
       Stats a = no_stats();
@@ -733,8 +734,6 @@ __global__ void __launch_bounds__(DRAW_THREADS, 3) draw_kernel(VerifyParams P) {
   const float* e = P.noise + b * P.ld_noise;
   const int struck = !P.draft && refused ? id_at[run] : -1;  // a certain draft: q = 1 there
   const int k0 = chunk * P.draw_packs;
-  if (tid == 0) s_known = (int)(*const_cast<volatile unsigned long long*>(P.best + b) >> 32);
-  __syncthreads();
   unsigned long long word =
       draw_share<T, VEC, DRAW_THREADS>(x, dr, e, P.n, k0, k0 + P.draw_packs, sc, st.m, st.s, dl, struck, &s_known);
   if (lane == 0) words[warp] = word;
