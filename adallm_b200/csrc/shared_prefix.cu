@@ -163,21 +163,17 @@ __device__ __forceinline__ int64_t tc_units(const Segment& x, const Params& P) {
 // of the same pages together.  It streams the piece's 16-key tiles through its own ring of RING slots
 // (TMA, 128-byte swizzle, one mbarrier a slot) and takes two tiles a step, so the steps' serial parts
 // (waits, maxima, the way of P through shared memory) are paid once for 32 keys:
-//   S^T = K . Q^T  mma.m16n8k32 on the e4m3 bytes as they lie (keys on M, rows on N), the queries as
-//     sums of e4m3 terms (see term_scale): K costs no conversion.  The head dimension is permuted so that
-//     lane (g, c) needs bytes [32c, 32c + 32) of keys g and g + 8, Q likewise.
+//   S^T = K . Q^T  mma.m16n8k16 (keys on M, rows on N), K widened to fp16 (exact) once for all rows, the
+//     scaled queries as fp16: exact down to 2^-25 of the row's maximum (bf16; fp16 2^-22), to 2^-32 of it
+//     below.  The head dimension is permuted so that lane (g, c) needs bytes [32c, 32c + 32) of keys g and
+//     g + 8, Q likewise.  (The warp-level e4m3 product is no way round the widening: it runs as
+//     conversions of both operands and two fp16 products, and queries need two or three e4m3 terms.)
 //   O^T += V^T . P^T  mma.m16n8k16 with V widened to fp16 and P rounded to fp16; the output dimension is
 //     permuted so that the lane needs bytes [16g, 16g + 16) of keys 2c, 2c + 1, 2c + 8, 2c + 9.
 // All shared-memory reads are 16 bytes a lane, conflict-free through the swizzle.  Statistics fp32; the
 // sums are rescaled only when a row's maximum moved.
-// Queries as sums of e4m3 terms.  A row is scaled by a power of two to a maximum in [128, 256); a term
-// keeps 4 significant bits and what it leaves is exact, so two terms hold every bf16 value down to 2^-10
-// of the row's maximum exactly (three hold fp16), smaller ones to 2^-18 of it.
-template <typename TQ> struct Terms;
-template <> struct Terms<__nv_bfloat16> { static constexpr int N = 2; };
-template <> struct Terms<__half> { static constexpr int N = 3; };
-// From the packed 16-bit maxima of |q| over a row's even and odd elements: the scale, and its inverse
-// (NaN for a row with infinities or NaN).
+// A row of queries is scaled by a power of two to a maximum in [128, 256).  From the packed 16-bit maxima
+// of |q| over its even and odd elements: the scale, and its inverse (NaN for a row with infinities or NaN).
 template <typename TQ> __device__ __forceinline__ void term_scale(uint32_t top, float& up, float& down) {
   const uint16_t top16 = (uint16_t)max(top & 0xFFFFu, top >> 16);
   const uint32_t most = __float_as_uint(to_f32(*reinterpret_cast<const TQ*>(&top16)));
@@ -191,29 +187,6 @@ __device__ __forceinline__ uint32_t top_of(uint32_t top, const uint4& u) {
   top = __vmaxu2(top, u.z & 0x7FFF7FFFu);
   return __vmaxu2(top, u.w & 0x7FFF7FFFu);
 }
-// The next term of 4 values (packed), which are left with the rest.
-__device__ __forceinline__ uint32_t next_term(float* f, bool last) {
-  const uint32_t a = f32x2_to_e4m3x2(f[0], f[1]), b = f32x2_to_e4m3x2(f[2], f[3]);
-  if (!last) {
-    const uint32_t ha = e4m3x2_to_f16x2((uint16_t)a), hb = e4m3x2_to_f16x2((uint16_t)b);
-    const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&ha));
-    const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
-    f[0] -= fa.x;
-    f[1] -= fa.y;
-    f[2] -= fb.x;
-    f[3] -= fb.y;
-  }
-  return a | (b << 16);
-}
-// D(16x8, f32) += A(16x32, e4m3, row) * B(32x8, e4m3, col)
-__device__ __forceinline__ void mma_16832_e4m3(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                               uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 constexpr int RING = 4;
 constexpr int WARPS = 4;
 constexpr int MIN_TILES = 4;  // of a split: below, a piece's fixed cost outweighs its keys
@@ -263,7 +236,7 @@ template <typename TQ, int NB>
 __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
     pieces_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, Params P) {
   using namespace sm100;
-  constexpr int ROWS = 8 * NB, TERMS = Terms<TQ>::N;
+  constexpr int ROWS = 8 * NB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   extern __shared__ uint8_t smem_raw[];
@@ -433,7 +406,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
 
     // ---- the rows: queries as the B operand (lane: row g of each block of 8, d in [32c, 32c + 32)), and
     // for the rows 2c, 2c + 1 that this lane's scores belong to their scale and key range [lo, hi)
-    uint32_t qf[NB][TERMS][8];
+    uint32_t qf[NB][16];
     float cs[NB][2];
     int lo[NB][2], hi[NB][2], lo_max = 0, hi_min = 0x7fffffff;
 #pragma unroll
@@ -452,9 +425,9 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] *= up;
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) {
-          qf[nb][term][2 * i] = next_term(f, term + 1 == TERMS);
-          qf[nb][term][2 * i + 1] = next_term(f + 4, term + 1 == TERMS);
+        for (int e = 0; e < 4; ++e) {
+          const __half2 h = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+          qf[nb][4 * i + e] = *reinterpret_cast<const uint32_t*>(&h);
         }
       }
       cs[nb][0] = P.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * c);
@@ -527,13 +500,15 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
         const uint32_t* kg = reinterpret_cast<const uint32_t*>(kk);
         const uint32_t* kg8 = reinterpret_cast<const uint32_t*>(kk + 2);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int ks = 0; ks < 8; ++ks) {
+          uint32_t a[4];
+          a[0] = e4m3x2_to_f16x2((uint16_t)(kg[ks] & 0xFFFFu));
+          a[1] = e4m3x2_to_f16x2((uint16_t)(kg8[ks] & 0xFFFFu));
+          a[2] = e4m3x2_to_f16x2((uint16_t)(kg[ks] >> 16));
+          a[3] = e4m3x2_to_f16x2((uint16_t)(kg8[ks] >> 16));
 #pragma unroll
-          for (int term = 0; term < TERMS; ++term)
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              mma_16832_e4m3(sc[nb][u], kg[2 * ks], kg8[2 * ks], kg[2 * ks + 1], kg8[2 * ks + 1], qf[nb][term][2 * ks],
-                             qf[nb][term][2 * ks + 1]);
+          for (int nb = 0; nb < NB; ++nb) mma_16816_f16(sc[nb][u], a, qf[nb] + 2 * ks);
+        }
       }
       const bool whole = ok2 == 3u && tt >= lo_max && tt + 2 * TILE <= hi_min;  // warp-uniform
 #pragma unroll
@@ -710,6 +685,26 @@ constexpr int THREADS = 16 * 32;
 constexpr int NE = 2, NV = 2, ND = 2;
 constexpr int REGS_LAUNCH = 128, REGS_ROWS = 192, REGS_REST = 64;  // a thread: 4 * 128 = 2 * 192 + 2 * 64
 static_assert(2 * REGS_ROWS + 2 * REGS_REST <= 4 * REGS_LAUNCH, "registers of the block");
+// Queries as sums of e4m3 terms.  Of a row scaled to a maximum in [128, 256) a
+// term keeps 4 significant bits and what it leaves is exact, so two terms hold every bf16 value down to 2^-10
+// of the row's maximum exactly (three hold fp16), smaller ones to 2^-18 of it.
+template <typename TQ> struct Terms;
+template <> struct Terms<__nv_bfloat16> { static constexpr int N = 2; };
+template <> struct Terms<__half> { static constexpr int N = 3; };
+// The next term of 4 values (packed), which are left with the rest.
+__device__ __forceinline__ uint32_t next_term(float* f, bool last) {
+  const uint32_t a = f32x2_to_e4m3x2(f[0], f[1]), b = f32x2_to_e4m3x2(f[2], f[3]);
+  if (!last) {
+    const uint32_t ha = e4m3x2_to_f16x2((uint16_t)a), hb = e4m3x2_to_f16x2((uint16_t)b);
+    const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&ha));
+    const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
+    f[0] -= fa.x;
+    f[1] -= fa.y;
+    f[2] -= fb.x;
+    f[3] -= fb.y;
+  }
+  return a | (b << 16);
+}
 // A piece: blocks [blk, blk + n) of a unit; n = 0: no more.
 struct Piece {
   int tok0, tokens, k0, len;
