@@ -200,12 +200,12 @@ __device__ __forceinline__ uint4 tile_ld16(const uint8_t* tile, int row, int chu
 // one piece for every warp of the grid, or twice the (segment, row block, head) units where those are
 // more.  work[s] = (tiles, row blocks * heads).  Each lane tries a length, from the bound that the tiles
 // alone give upwards; lengths past those (or of more segments than are worth trying) come from
-// pieces <= tiles / length + units.  Warp-wide.
+// pieces <= tiles / length + units.  CTA-wide: each warp counts a share of the segments.
 __device__ __forceinline__ int ceil_div_small(int a, float inverse) {  // a < 2^21: the half keeps it off the edges
   return (int)(((float)a - 0.5f) * inverse) + (a > 0);
 }
-__device__ __forceinline__ int split_tiles(const int2* work, int segs, int max_pieces) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ int split_tiles(const int2* work, int segs, int max_pieces, int (*counted)[32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t all = 0;
   int units = 0, most = 0;
   for (int s = lane; s < segs; s += 32) {
@@ -220,11 +220,16 @@ __device__ __forceinline__ int split_tiles(const int2* work, int segs, int max_p
   const int least = (int)min(all / max_pieces + 1, (int64_t)most);
   const int ct = max(MIN_TILES, least) + lane;
   bool fits = false;
-  if (segs <= 256 && most < (1 << 21)) {
+  if (segs <= 256 && most < (1 << 21)) {  // the same in every warp
     const float inverse = 1.f / (float)ct;
     int n = 0;
 #pragma unroll 4
-    for (int s = 0; s < segs; ++s) n += ceil_div_small(work[s].x, inverse) * work[s].y;
+    for (int s = warp; s < segs; s += WARPS) n += ceil_div_small(work[s].x, inverse) * work[s].y;
+    counted[warp][lane] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) n += counted[w][lane];
     fits = n <= max_pieces && n >= 0;
   }
   const unsigned who = __ballot_sync(0xffffffffu, fits);
@@ -248,7 +253,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
   int* first = reinterpret_cast<int*>(work + segs);  // pieces before each segment, by heads
   __shared__ uint64_t bars[WARPS][RING];
   __shared__ __align__(16) __half p_s[WARPS][NB][8][40];  // 32 keys a row; padded against bank conflicts
-  __shared__ int abort_flag, s_tiles, s_cut;
+  __shared__ int abort_flag, s_cut, counted[WARPS][32];
   uint64_t* bar = bars[warp];
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -271,8 +276,8 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
     if (s >= P.num_groups && x.len < x.tokens) s_cut = 1;  // rows inside the prefix: it needs a mask too
   }
   __syncthreads();
+  const int ct = split_tiles(work + skip, segs - skip, P.max_pieces, counted);
   if (warp == 0) {
-    const int ct = split_tiles(work + skip, segs - skip, P.max_pieces);
     int sum = 0;
     for (int s0 = 0; s0 < segs; s0 += 32) {
       const int s = s0 + lane;
@@ -286,13 +291,9 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
       if (s < segs) first[s] = sum + acc - n;
       sum += __shfl_sync(0xffffffffu, acc, 31);
     }
-    if (lane == 0) {
-      first[segs] = sum;
-      s_tiles = ct;
-    }
+    if (lane == 0) first[segs] = sum;
   }
   __syncthreads();
-  const int ct = s_tiles;
   const bool cut = s_cut != 0;
   // ---- for the merge: CTA i writes the tokens of sequences i, i + CTAs, ...
   for (int b = blockIdx.x; b < P.batch; b += gridDim.x) {
