@@ -116,11 +116,6 @@ __device__ __forceinline__ int sequence_of(const Params& P, int n) {  // row n's
   const int b = interval_of(P.cu_q, P.batch, n);
   return b < P.batch ? b : -1;
 }
-__device__ __forceinline__ int group_of(const Params& P, int b) {  // sequence b's, or -1
-  if (!P.cu_groups) return P.num_groups > 0 ? 0 : -1;
-  const int g = interval_of(P.cu_groups, P.num_groups, b);
-  return g < P.num_groups ? g : -1;
-}
 
 // A segment: rows [tok0, tok0 + tokens) x group heads over keys [k0, len) of a page list.
 struct Segment {
@@ -206,18 +201,16 @@ __device__ __forceinline__ int ceil_div_small(int a, float inverse) {  // a < 2^
 }
 __device__ __forceinline__ int split_tiles(const int2* work, int segs, int max_pieces, int (*counted)[32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t all = 0;
-  int units = 0, most = 0;
+  float about = 0.f;  // the tiles of all pieces' rows: where the lengths tried begin
+  int most = 0;
   for (int s = lane; s < segs; s += 32) {
-    all += (int64_t)work[s].x * work[s].y;
-    units += work[s].x ? work[s].y : 0;
+    about += (float)work[s].x * (float)work[s].y;
     most = max(most, work[s].x);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-  units = __reduce_add_sync(0xffffffffu, units);
+  for (int o = 16; o > 0; o >>= 1) about += __shfl_xor_sync(0xffffffffu, about, o);
   most = __reduce_max_sync(0xffffffffu, most);
-  const int least = (int)min(all / max_pieces + 1, (int64_t)most);
+  const int least = (int)fminf(__fdividef(about, (float)max_pieces) + 1.f, (float)most);
   const int ct = max(MIN_TILES, least) + lane;
   bool fits = false;
   if (segs <= 256 && most < (1 << 21)) {  // the same in every warp
@@ -234,6 +227,15 @@ __device__ __forceinline__ int split_tiles(const int2* work, int segs, int max_p
   }
   const unsigned who = __ballot_sync(0xffffffffu, fits);
   if (who) return __shfl_sync(0xffffffffu, ct, __ffs(who) - 1);
+  int64_t all = 0;
+  int units = 0;
+  for (int s = lane; s < segs; s += 32) {
+    all += (int64_t)work[s].x * work[s].y;
+    units += work[s].x ? work[s].y : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  units = __reduce_add_sync(0xffffffffu, units);
   return (int)max((int64_t)MIN_TILES, all / max(1, max_pieces - units) + 1);
 }
 
@@ -249,13 +251,16 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
   uint8_t* ring = base + warp * RING_BYTES;
   const int segs = P.num_groups + P.batch;
   Segment* seg = reinterpret_cast<Segment*>(base + WARPS * RING_BYTES);
-  int2* work = reinterpret_cast<int2*>(seg + segs);  // tiles, row blocks * heads (0: not this kernel's)
+  int2* work = reinterpret_cast<int2*>(seg + segs);  // tiles (0: not this kernel's), then splits; row blocks * heads
   int* first = reinterpret_cast<int*>(work + segs);  // pieces before each segment, by heads
+  int* begins = first + segs + 1;                    // first sequence of each group, and the end
   __shared__ uint64_t bars[WARPS][RING];
   __shared__ __align__(16) __half p_s[WARPS][NB][8][40];  // 32 keys a row; padded against bank conflicts
   __shared__ int abort_flag, s_cut, counted[WARPS][32];
   uint64_t* bar = bars[warp];
   if (threadIdx.x == 0) {
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
     abort_flag = 0;
     s_cut = P.window > 0;
   }
@@ -275,23 +280,30 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
     work[s] = make_int2(s >= skip ? x.tiles() : 0, (x.tokens * P.group + ROWS - 1) / ROWS * P.num_kv_heads);
     if (s >= P.num_groups && x.len < x.tokens) s_cut = 1;  // rows inside the prefix: it needs a mask too
   }
+  for (int i = threadIdx.x; i <= P.num_groups; i += WARPS * 32) begins[i] = group_begin(P, i);
   __syncthreads();
   const int ct = split_tiles(work + skip, segs - skip, P.max_pieces, counted);
-  if (warp == 0) {
-    int sum = 0;
-    for (int s0 = 0; s0 < segs; s0 += 32) {
-      const int s = s0 + lane;
-      const int n = s < segs ? (work[s].x + ct - 1) / ct * work[s].y : 0;
-      int acc = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, acc, o);
-        if (lane >= o) acc += up;
-      }
-      if (s < segs) first[s] = sum + acc - n;
-      sum += __shfl_sync(0xffffffffu, acc, 31);
+  if (warp == 0) {  // each lane a run of segments: their splits in place of their tiles, the pieces before them
+    const int run = (segs + 31) / 32, from = min(segs, lane * run), to = min(segs, from + run);
+    const float inverse = 1.f / (float)ct;
+    int mine = 0;
+    for (int s = from; s < to; ++s) {
+      const int tiles = work[s].x;
+      work[s].x = tiles < (1 << 21) ? ceil_div_small(tiles, inverse) : (tiles + ct - 1) / ct;
+      mine += work[s].x * work[s].y;
     }
-    if (lane == 0) first[segs] = sum;
+    int acc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, acc, o);
+      if (lane >= o) acc += up;
+    }
+    int before = acc - mine;
+    for (int s = from; s < to; ++s) {
+      first[s] = before;
+      before += work[s].x * work[s].y;
+    }
+    if (lane == 31) first[segs] = acc;
   }
   __syncthreads();
   const bool cut = s_cut != 0;
@@ -299,10 +311,13 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
   for (int b = blockIdx.x; b < P.batch; b += gridDim.x) {
     const Segment x = seg[P.num_groups + b];
     if (x.tokens == 0) continue;
-    const int g = group_of(P, b);
+    int g = -1;  // the last group that begins at or before b, unless b is behind them all
+    for (int i = 0; i <= P.num_groups; i += 32)
+      g += __popc(__ballot_sync(0xffffffffu, i + lane <= P.num_groups && begins[i + lane] <= b));
+    if (g == P.num_groups) g = -1;
     RowPlan r;
     r.own_first = first[P.num_groups + b];
-    r.own_splits = (x.tiles() + ct - 1) / ct;
+    r.own_splits = work[P.num_groups + b].x;
     r.pre_first = r.pre_splits = r.blocks = r.pad = 0;
     r.tc_from = r.tc_units = r.tc_total = r.tc_ctas = 0;
     int tok0_g = 0;
@@ -310,7 +325,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
       tok0_g = seg[g].tok0;
       if (!P.prefix_tc) {
         r.pre_first = first[g];
-        r.pre_splits = (seg[g].tiles() + ct - 1) / ct;
+        r.pre_splits = work[g].x;
       } else {  // prefix_kernel's units and blocks, as its Walk lays them out
         for (int i = 0; i < P.num_groups; ++i) {
           const int blocks = tc_blocks(seg[i]);
@@ -350,7 +365,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
     }
     const bool pre = s < P.num_groups;
     const Segment x = seg[s];
-    const int splits = (work[s].x + ct - 1) / ct, off = piece - first[s];
+    const int splits = work[s].x, off = piece - first[s];
     int kvh;
     const int flat = P.by_kv_heads.divmod(off, kvh);
     const int rb = flat / splits, sp = flat - rb * splits;
@@ -973,6 +988,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     mbar_init(fin, 1);
     *abort_flag = 0;
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
     fence_mbar_init();
   }
   if (warp == 13) tmem_alloc(tmem_slot, TMEM_COLS);
@@ -1552,8 +1569,10 @@ inline int row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 // pieces_kernel keeps the segments in shared memory behind its rings; its limit is set once, for the most
 // there may be, so that calls of different batches on different threads cannot lower it under one another.
 constexpr int MAX_SEGMENTS = 4096;
-constexpr int pieces_smem(int segs) { return 1024 + WARPS * RING_BYTES + segs * ((int)sizeof(Segment) + 12) + 4; }
-static_assert(pieces_smem(MAX_SEGMENTS) + 8 * 1024 <= 227 * 1024, "the segments have to fit beside the rings");
+constexpr int pieces_smem(int groups, int batch) {
+  return 1024 + WARPS * RING_BYTES + (groups + batch) * ((int)sizeof(Segment) + 12) + groups * 4 + 8;
+}
+static_assert(pieces_smem(MAX_SEGMENTS, 0) + 8 * 1024 <= 227 * 1024, "the segments have to fit beside the rings");
 constexpr int PIECES_PER_SM = 3 * WARPS;
 
 // prefix_kernel takes the prefixes from 33 rows a prefix and KV head on (with fewer, its 128-row tiles stay
@@ -1708,10 +1727,10 @@ extern "C" int ada_fp8_shared_prefix_decode(
     }
     ADA_CHECK_LAUNCH();
   }
-  const int smem = sp::pieces_smem(num_groups + batch);
+  const int smem = sp::pieces_smem(num_groups, batch);
 #define ADA_SP(TQ, NB)                                                                                              \
   do {                                                                                                              \
-    if (!sp::smem_ready<sp::pieces_kernel<TQ, NB>>(sp::pieces_smem(sp::MAX_SEGMENTS))) return ADA_ERR_CUDA;         \
+    if (!sp::smem_ready<sp::pieces_kernel<TQ, NB>>(sp::pieces_smem(sp::MAX_SEGMENTS, 0))) return ADA_ERR_CUDA;         \
     (void)ada::launch_k(sp::pieces_kernel<TQ, NB>, dim3((unsigned)(sms * (NB == 1 ? 3 : 2))), dim3(sp::WARPS * 32), \
                         smem, st, tmk, tmv, P);                                                                     \
   } while (0)
