@@ -152,6 +152,16 @@ __device__ __forceinline__ int64_t tc_units(const Segment& x, const Params& P) {
   return (((int64_t)x.tokens * P.group + (1 << TC_ROWS_LOG2) - 1) >> TC_ROWS_LOG2) * P.num_kv_heads;
 }
 
+// CTAs that share `total` blocks.  All SMs from three blocks an SM on; fewer blocks go to half of them, so that
+// pieces_kernel, which cannot share an SM with prefix_kernel, runs beside it on the others: 192 rows x 8 heads
+// behind 2,048 keys 35.2 -> 25.8 us, behind 4,096 38.4 -> 29.9; with 512 blocks (8,192 keys) there is nothing
+// to win (32.7 on all SMs, 32.1 on 64).
+__device__ __forceinline__ int64_t tc_ctas_of(int64_t total, int sms) {
+  if (total > 2 * sms) return sms;
+  const int half = max(1, sms / 2), each = max(1, ((int)total + half - 1) / half);
+  return ((int)total + each - 1) / each;
+}
+
 // ---- pieces of few rows: one warp each, warp-level MMA --------------------------------------------
 // Bound: HBM by its bytes; measured, the instructions of a tile.  A warp takes one piece (segment, block
 // of 8 * NB rows, split, KV head) at a time, KV head fastest, so that neighbouring warps read the heads
@@ -338,7 +348,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
           r.tc_total += units * blocks;
           r.tc_ctas += units;
         }
-        r.tc_ctas = min((int64_t)P.tc_ctas, r.tc_total);
+        r.tc_ctas = tc_ctas_of(r.tc_total, P.tc_ctas);
       }
     }
     for (int i = threadIdx.x; i < x.tokens; i += WARPS * 32) {
@@ -1428,7 +1438,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       cut = __any_sync(0xffffffffu, cut);
       while (w.g0 + 32 < P.num_groups) w.forward(P);
       const int64_t total = __shfl_sync(0xffffffffu, w.before + w.size, 31);
-      const int64_t ctas = min((int64_t)gridDim.x, total);
+      const int64_t ctas = tc_ctas_of(total, (int)gridDim.x);
       if (w.g0 > 0) w.begin(P);
       const bool work = (int64_t)blockIdx.x < ctas;
       w.pos = work ? range_begin(total, ctas, blockIdx.x) : 0;
@@ -1577,10 +1587,10 @@ constexpr int PIECES_PER_SM = 3 * WARPS;
 
 // prefix_kernel takes the prefixes from 33 rows a prefix and KV head on (with fewer, its 128-row tiles stay
 // emptier than the pieces' blocks of 8), where (rows) x (keys that the prefix tables reach) x (KV heads)
-// is at least 2^21: its launch, set-up and partials cost about 10 us, which the pieces need for that much.
-// 64 rows x 8 heads behind 2,048 keys: 24 us by pieces, 30 us with it; behind 32,768 keys the pieces' share
-// alone is 16 times as long.
-constexpr int64_t TC_ROWS = 33, TC_WORK = 1 << 21;
+// is at least 3 * 2^19, where its start-up and partials (about 15 us) are made up for.  By pieces and with it,
+// in us: 64 rows x 8 heads behind 2,048 keys 22.6, 21.8, behind 8,192 38.1, 32.7; 192 rows behind 1,024 32.0,
+// 24.1; 256 rows behind 512 27.3, 31.2.
+constexpr int64_t TC_ROWS = 33, TC_WORK = 3 << 19;
 
 struct Layout {
   int nb;
