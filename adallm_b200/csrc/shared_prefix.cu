@@ -293,6 +293,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
   for (int i = threadIdx.x; i <= P.num_groups; i += WARPS * 32) begins[i] = group_begin(P, i);
   __syncthreads();
   const int ct = split_tiles(work + skip, segs - skip, P.max_pieces, counted);
+  __syncthreads();  // every warp has counted: splits take the tiles' place
   if (warp == 0) {  // each lane a run of segments: their splits in place of their tiles, the pieces before them
     const int run = (segs + 31) / 32, from = min(segs, lane * run), to = min(segs, from + run);
     const float inverse = 1.f / (float)ct;

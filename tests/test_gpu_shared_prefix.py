@@ -372,3 +372,14 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="CUDA"):
         shared_prefix_decode(**good, workspace=torch.empty(need, dtype=torch.uint8))
     assert bool(torch.isfinite(shared_prefix_decode(**good).float()).all())
+
+
+def test_many_segments_give_the_same_every_time():
+    """More segments than the split length is searched over: all warps still agree on one."""
+    n = 320
+    case = osp.make_shared_prefix_case(28, [900, 1200, 40, 300, 1], [64] * 5, [1 + (37 * i) % 700 for i in range(n)],
+                                       [1] * n, 8, 8, 16)
+    out = _run(case)
+    a, k = _args(_to_gpu(case))
+    for _ in range(200):
+        assert torch.equal(shared_prefix_decode(*a, **k), out)
