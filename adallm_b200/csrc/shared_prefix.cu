@@ -45,8 +45,9 @@ struct Divisor {
 };
 
 // A token's partials.  Own keys: `own_splits` pieces, KV heads apart, from own_first + row block *
-// own_splits * KV heads + KV head on, row own_row + head of the segment; prefix likewise, or with prefix_kernel the pieces of the
-// `blocks` blocks from block `tc_from` + unit * blocks on (units: tc_units before the group).
+// own_splits * KV heads + KV head on, row own_row + head of the segment; prefix likewise, or with
+// prefix_kernel the pieces of the `blocks` blocks from block `tc_from` + unit * blocks on (units: tc_units
+// before the group).
 struct RowPlan {
   int own_first, own_splits, own_row, pre_row;
   int pre_first, pre_splits, blocks, pad;
@@ -163,7 +164,11 @@ __device__ __forceinline__ int64_t tc_ctas_of(int64_t total, int sms) {
 }
 
 // ---- pieces of few rows: one warp each, warp-level MMA --------------------------------------------
-// Bound: HBM by its bytes; measured, the instructions of a tile.  A warp takes one piece (segment, block
+// Bound: HBM by its bytes, latency by measurement.  8 x 8 samples of prompts of 869 to 3,454 keys, 16 KV
+// heads, window 1,024 (108 MB): 37 us, 2.9 TB/s = 0.44 of a measured copy; every further tile then costs its
+// bytes at 0.96 of that rate, but about 5 us pass before the first load (lengths, plan, page look-up: some
+// 1,500 instructions that run once, so fetching them is what takes the time) and 1 to 2 at either end of a
+// piece.  A warp takes one piece (segment, block
 // of 8 * NB rows, split, KV head) at a time, KV head fastest, so that neighbouring warps read the heads
 // of the same pages together.  It streams the piece's 16-key tiles through its own ring of RING slots
 // (TMA, 128-byte swizzle, one mbarrier a slot) and takes two tiles a step, so the steps' serial parts
@@ -173,7 +178,8 @@ __device__ __forceinline__ int64_t tc_ctas_of(int64_t total, int sms) {
 //     below.  The head dimension is permuted so that lane (g, c) needs bytes [32c, 32c + 32) of keys g and
 //     g + 8, Q likewise.  (The warp-level e4m3 product is no way round the widening: it runs as
 //     conversions of both operands and two fp16 products, and queries need two or three e4m3 terms.)
-//   O^T += V^T . P^T  mma.m16n8k16 with V widened to fp16 and P rounded to fp16; the output dimension is
+//   O^T += V^T . P^T  mma.m16n8k16 with V widened to fp16 (exact) and P rounded to fp16, 2^-11 of a weight
+//     (bf16 would leave 2^-8); the row sums add the unrounded weights in fp32.  The output dimension is
 //     permuted so that the lane needs bytes [16g, 16g + 16) of keys 2c, 2c + 1, 2c + 8, 2c + 9.
 // All shared-memory reads are 16 bytes a lane, conflict-free through the swizzle.  Statistics fp32; the
 // sums are rescaled only when a row's maximum moved.
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
   uint8_t* ring = base + warp * RING_BYTES;
   const int segs = P.num_groups + P.batch;
   Segment* seg = reinterpret_cast<Segment*>(base + WARPS * RING_BYTES);
-  int2* work = reinterpret_cast<int2*>(seg + segs);  // tiles (0: not this kernel's), then splits; row blocks * heads
+  int2* work = reinterpret_cast<int2*>(seg + segs);  // tiles (0: not this kernel's), then splits; blocks * heads
   int* first = reinterpret_cast<int*>(work + segs);  // pieces before each segment, by heads
   int* begins = first + segs + 1;                    // first sequence of each group, and the end
   __shared__ uint64_t bars[WARPS][RING];
@@ -686,25 +692,30 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
 }
 
 // ---- prefixes under many rows: tcgen05 ---------------------------------------------------------------
-// Bound: the tensor cores, 4 * 128 flops for every (row, key).  A unit is 256 rows (two 128-row
+// Bound: the tensor cores, 4 * 128 flops for every (row, key).  1,024 rows x 8 KV heads x 32,768 keys (137 GFLOP):
+// 142 us, 0.97 PFLOP/s = 0.59 of a measured bf16 product's rate; a block of 128 keys takes 3,550 cycles where its
+// MMAs take 2,048 and its exponentials as many: a tile's scores, maxima, weights and products follow one another,
+// and TMEM (O and S of both tiles fill it) has no room for a second S.  A unit is 256 rows (two 128-row
 // tiles, the TMEM lanes) of one prefix and KV head over blocks of 128 keys; the blocks of all units are
 // laid end to end and every CTA takes an equal range, so a range covers the end of one unit, whole
 // ones and the start of another, each giving one partial (piece = unit + CTA index: one of the two
 // moves on from each piece to the next).
 //   S_t = Q_t . K^T  kind::f8f6f4 on the e4m3 bytes as they lie in the cache, the queries as sums of e4m3
 //     terms (see Terms): K is never widened and the terms cost what the fp16 product would.
-//   P  = 2^(S c - m) in fp16, written over S in TMEM, the A operand of
-//   O_t += P_t . V  kind::f16; V is widened to fp16 by four warps, once for both tiles.
+//   P  = 2^(S c - m) in fp16 (2^-11 of a weight; the sums add them unrounded), over S in TMEM, the A operand of
+//   O_t += P_t . V  kind::f16; V is widened to fp16 (exact) by four warps, once for both tiles.
 // Roles (16 warps): 0-3 widen V; 4-7 and 8-11 take tile 0's and tile 1's rows (thread = row: queries to
 // terms, softmax, O to the workspace); 12 loads (TMA, eight 16-key tiles a block for K and V each);
 // 13 issues the MMAs; 14 walks the CTA's range and hands out its pieces.  The row warps take 192
-// registers a thread (a row of S at once), the others 64.  P.V of a block and S of the next are issued together for a tile, so one tile's
-// MMAs run under the other tile's softmax.  All tcgen05 operations come from one thread in order, so
-// s_full of block j + 1 also says that P.V of block j is complete: O may be rescaled.
+// registers a thread (a row of S at once), the others 64.  P.V of a block and S of the next are issued
+// together for a tile, so one tile's MMAs run under the other tile's softmax.  All tcgen05 operations come
+// from one thread in order, so s_full of block j + 1 also says that P.V of block j is complete: O may be
+// rescaled.
 // Barriers, phase = use: d_full/d_empty (pieces), k_full/k_empty (K slots), e_full/e_empty (e4m3 V
-// slots), v_full/v_empty (fp16 V slots), s_full[t], p_full[t][half] (a block's S, P of tile t), q_full[t], o_full[t] (a piece's Q, O).  A
-// tile's next S and its next P.V wait for q_full and p_full, which its warps give after they have
-// written the piece before.  Every wait is bounded and ends all roles through the abort flag.
+// slots), v_full/v_empty (fp16 V slots), s_full[t], p_full[t][half] (a block's S, P of tile t), q_full[t],
+// o_full[t] (a piece's Q, O).  A tile's next S and its next P.V wait for q_full and p_full, which its warps
+// give after they have written the piece before.  Every wait is bounded and ends all roles through the
+// abort flag.
 namespace tc {
 constexpr int BM = 128, BN = 128, TILES = 2, ROWS = TILES * BM;
 static_assert(BN == TC_KEYS && ROWS == 1 << TC_ROWS_LOG2, "shape of a unit");
@@ -1478,6 +1489,9 @@ inline bool registers_ready() {
 }  // namespace tc
 
 // ---- merge: one warp per (row, head), four dimensions a lane --------------------------------------
+// out = v_scale * sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over the row's pieces i, M = max m_i, in the
+// order of the pieces.  Bound: the partials' bytes, latency for few rows: 256 rows x 32 heads (48 MB of partials) 20.6 us from
+// a cold L2, 2.3 TB/s; 64 rows x 32 heads 10.3 us, a chain of three loads (plan, maxima, sums).
 template <typename TO>
 __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
   pdl_wait();
@@ -1574,7 +1588,8 @@ inline bool smem_ready(int bytes) {
 }
 
 // Blocks of 8 rows that a warp takes together: what the rows of a sequence fill on average, up to two
-// (a prefix of 16 rows ran faster as two blocks of 8 than as one of 16: 54 against 72 us for 8 x 8 samples).
+// (with 8 rows or fewer a sequence, 16 cost more than a prefix's K and V read half as often give back: 42
+// against 56 us for 8 x 8 samples of 2 rows, 23 against 31 for 16 sequences of 4).
 inline int row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 // pieces_kernel keeps the segments in shared memory behind its rings; its limit is set once, for the most
