@@ -383,3 +383,10 @@ def test_many_segments_give_the_same_every_time():
     a, k = _args(_to_gpu(case))
     for _ in range(200):
         assert torch.equal(shared_prefix_decode(*a, **k), out)
+
+
+@pytest.mark.parametrize("prefixes,sizes", [([3000], [4]), ([6000], [4]), ([700, 2500], [3, 1])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_long_prefixes(prefixes, sizes, dtype):
+    """Blocks of keys for half of the SMs (several each) and for all of them, ranges that cross units."""
+    _run(osp.make_shared_prefix_case(29, prefixes, sizes, [5, 64, 3, 90], [12, 3, 1, 9], 32, 8, 16, dtype))
