@@ -202,20 +202,6 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-_WORKSPACES: dict = {}
-
-
-def workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """Uninitialised scratch reused per (device, stream), for entries whose workspace has no initial
-    value; inside a CUDA-graph capture a fresh buffer of the graph's pool."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    buf = _WORKSPACES.get((device.index, stream))
-    if buf is None or buf.numel() < nbytes:
-        buf = _WORKSPACES[device.index, stream] = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return buf
-
-
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

@@ -76,7 +76,7 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     Exp(1); draft_logits [B, D, V] (target's dtype, any strides with unit stride in V) and
     draft_lse fp32 [B, D]: the logits each draft was drawn from and their log-normaliser at the
     sequence's temperature (``sample`` returns it); both None for drafts without a distribution.
-    workspace: at least verify_workspace_bytes(...) bytes (default: one kept per stream).
+    workspace: at least verify_workspace_bytes(...) bytes (default: allocated for the call).
     Returns (tokens int64 [B, D + 1], accepted int32 [B], logprobs fp32 [B, D + 1]): the accepted
     drafts and the drawn token with their log-probabilities under the target, then -1 and 0."""
     drafter = draft_logits is not None
@@ -115,7 +115,8 @@ def verify_drafts(target_logits: torch.Tensor, input_ids: torch.Tensor, cu_seqle
     device = target_logits.device
     stream = N.stream_ptr(device)
     if workspace is None:
-        workspace = N.workspace(device, stream, verify_workspace_bytes(n, b, v, dtype))
+        # one of its own: the launches of another thread's call on this stream may fall between this call's
+        workspace = torch.empty(verify_workspace_bytes(n, b, v, dtype), dtype=torch.uint8, device=device)
     else:
         N.require_cuda(workspace, what="verify_drafts")
     # (a single row may have any stride)

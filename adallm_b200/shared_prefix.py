@@ -47,8 +47,8 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     Row i of t attends to positions <= prefix + context - t + i, with window W > 0 to the last W
     of them.  Rows that see no key are zeros.
     Returns [N, Hq, 128] in q.dtype.  workspace: at least shared_prefix_workspace_bytes(...) bytes
-    (default: one kept per stream).  At most 4096 prefixes and sequences together.  err: optional int32 [1] device word; 0x90 is OR-ed in if a
-    tile wait ran out."""
+    (default: allocated for the call).  At most 4096 prefixes and sequences together.  err: optional
+    int32 [1] device word; 0x90 is OR-ed in if a tile wait ran out."""
     if not (q.is_cuda and k_cache.is_cuda and v_cache.is_cuda and prefix_tables.is_cuda and prefix_lens.is_cuda
             and block_tables.is_cuda and context_lens.is_cuda):
         raise RuntimeError("shared_prefix_decode requires CUDA tensors")
@@ -99,7 +99,8 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     stream = N.stream_ptr(device)
     need = shared_prefix_workspace_bytes(total_q, groups, batch, hq, hkv, d)
     if workspace is None:
-        workspace = N.workspace(device, stream, need)
+        # one of its own: the launches of another thread's call on this stream may fall between this call's
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
     else:
         N.require_cuda(workspace, what="shared_prefix_decode")
     if err is not None:

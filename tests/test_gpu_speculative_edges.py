@@ -1,11 +1,17 @@
-"""Shared-prefix decode, sampling and verification where calls meet and at the ends of their ranges.
-Two runs of one call have to be equal."""
+"""Shared-prefix decode, sampling and verification where calls meet: several threads on one stream,
+calls of different size in turn, and inputs at the ends of their ranges.
+
+Tolerances are those of the operators' own tests (tests/test_gpu_shared_prefix.py,
+tests/test_gpu_sampling.py); where two runs of one call are compared they have to be equal."""
+import functools
 import threading
 
+import numpy as np
 import pytest
 import torch
 
 from adallm_b200.attention import paged_decode, paged_prefill
+from adallm_b200.sampler import sample, verify_drafts
 from adallm_b200.shared_prefix import shared_prefix_decode
 from oracle import speculative as osp
 from tests.gpu_util import dev
@@ -55,3 +61,59 @@ def test_a_threads_first_cuda_call(entry):
     _in_threads(call)
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def _attention(seed, prefix, n, rows, reach=0):
+    c = osp.make_shared_prefix_case(seed, [prefix], [n], [3 + (7 * i) % 90 for i in range(n)], [rows] * n, 32, 8, 16)
+    c = {k: v.to(dev()) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    if reach:  # a table of this many pages: enough rows then go to the tensor-core kernel
+        c["prefix_tables"] = torch.nn.functional.pad(c["prefix_tables"], (0, reach), value=-1)
+    return lambda: (shared_prefix_decode(c["q"], c["k_cache"], c["v_cache"], c["prefix_tables"], c["prefix_lens"],
+                                         c["cu_groups"], c["block_tables"], c["context_lens"], c["scale"],
+                                         cu_seqlens_q=c["cu_seqlens_q"]),)
+
+
+def _verification(seed, batch, drafts, vocab):
+    g = torch.Generator().manual_seed(seed)
+    n = batch * (drafts + 1)
+    target = 3 * torch.randn((n, vocab), generator=g)
+    ids = target.roll(1, 0).argmax(-1)  # likely tokens: some are accepted
+    a = [t.to(dev()) for t in (target, ids, torch.arange(0, n + 1, drafts + 1, dtype=torch.int32), torch.full((batch,), 0.3),
+                               torch.rand((batch, drafts), generator=g),
+                               torch.empty((batch, vocab)).exponential_(1.0, generator=g))]
+    return lambda: verify_drafts(*a)
+
+
+def _calls():
+    return [_attention(1, 300, 5, 1), _verification(2, 3, 4, 5003), _attention(3, 900, 24, 3, reach=1 << 14),
+            _verification(4, 40, 2, 1009), _attention(5, 64, 60, 2), _verification(6, 1, 1, 90001)]
+
+
+def test_threads_on_one_stream_get_their_own_results():
+    calls = _calls()
+    alone = [tuple(t.clone() for t in f()) for f in calls]
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(len(calls)), []
+
+    def caller(i):
+        start.wait(timeout=60)
+        for _ in range(150):
+            got = calls[i]()
+            if not all(torch.equal(a, b) for a, b in zip(got, alone[i])):
+                wrong.append(i)
+
+    _in_threads(*(functools.partial(caller, i) for i in range(len(calls))))
+    torch.cuda.synchronize()
+    assert not wrong, wrong
+
+
+def test_calls_of_different_sizes_in_turn():
+    """No host wait between them: each one's launches follow the one's before on the stream."""
+    calls = _calls()
+    alone = [tuple(t.clone() for t in f()) for f in calls]
+    torch.cuda.synchronize()
+    order = np.random.default_rng(0).integers(0, len(calls), 400).tolist()
+    got = [(i, calls[i]()) for i in order]
+    torch.cuda.synchronize()
+    for i, out in got:
+        assert all(torch.equal(a, b) for a, b in zip(out, alone[i])), i
