@@ -1707,7 +1707,8 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.by_page = sp::Divisor::of(page_size);
   P.by_kv_heads = sp::Divisor::of(num_kv_heads);
   P.by_heads = sp::Divisor::of(num_heads);
-  P.window = window;
+  // a window as wide as all positions cuts nothing off; any other leaves the differences below in 32 bits
+  P.window = window < ((int64_t)max_pages + max_prefix_pages) * page_size ? window : 0;
   P.scale_log2 = scale * k_scale * sp::LOG2E;
   P.v_scale = v_scale;
   P.out = out;

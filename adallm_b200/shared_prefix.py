@@ -83,6 +83,7 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError("cu_groups must hold the first sequence of each group and the end (None for one group)")
     if total_q != batch if cu_seqlens_q is None else cu_seqlens_q.numel() != batch + 1:
         raise ValueError("cu_seqlens_q must have batch + 1 entries (None for one row per sequence)")
+    window = min(int(window), 0x7FFFFFFF)  # (past any position; the foreign call would take the low 32 bits)
     device = q.device
     if out is None:
         out = q.new_empty((total_q, hq, d))
@@ -109,7 +110,7 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], pages,
         prefix_tables.data_ptr(), pts[0], pt_pages, prefix_lens.data_ptr(), cu_g, groups,
         block_tables.data_ptr(), bts[0], bt_pages, context_lens.data_ptr(), cu_q, batch,
-        total_q, hq, hkv, d, page, float(scale), float(k_scale), float(v_scale), int(window), out.data_ptr(), out_code,
+        total_q, hq, hkv, d, page, float(scale), float(k_scale), float(v_scale), window, out.data_ptr(), out_code,
         os[0], os[1], workspace.data_ptr(), workspace.nbytes, N.ptr(err), stream)
     if st:
         N.check(st, "shared-prefix decode attention")

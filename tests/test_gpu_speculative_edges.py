@@ -117,3 +117,25 @@ def test_calls_of_different_sizes_in_turn():
     torch.cuda.synchronize()
     for i, out in got:
         assert all(torch.equal(a, b) for a, b in zip(out, alone[i])), i
+
+
+@pytest.mark.parametrize("reach", [0, 1 << 14])
+@pytest.mark.parametrize("rows", [[1, 2], [40, 33], [3, 0]])
+def test_windows_wider_than_all_positions(rows, reach):
+    """Prefixes and contexts with fewer keys than rows; from the reach of the tables on a window cuts nothing."""
+    c = osp.make_shared_prefix_case(7, [20], [2], [2, 30], rows, 32, 8, 16)
+    c = {k: v.to(dev()) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    c["prefix_tables"] = torch.nn.functional.pad(c["prefix_tables"], (0, reach), value=-1)
+
+    def run(window):
+        return shared_prefix_decode(c["q"], c["k_cache"], c["v_cache"], c["prefix_tables"], c["prefix_lens"],
+                                    c["cu_groups"], c["block_tables"], c["context_lens"], c["scale"],
+                                    cu_seqlens_q=c["cu_seqlens_q"], window=window)
+
+    want = run(0)
+    reached = (c["prefix_tables"].shape[1] + c["block_tables"].shape[1]) * 16
+    for window in (50, reached - 1, reached, 1 << 30, 2 ** 31 - 40, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 3, 1 << 62):
+        got = run(window)
+        assert float((got - want).float().abs().max()) <= 2 ** -8 * float(want.float().abs().max()), window
+        if window >= reached:
+            assert torch.equal(got, want), window
