@@ -504,7 +504,8 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
       l[nb][0] = l[nb][1] = 0.f;
     }
     bool failed = false;
-    for (int k = 0; k < nt; k += 2) {
+    int k = 0;
+    for (; k < nt; k += 2) {
       const bool two = k + 1 < nt;
       bool came = true;
 #pragma unroll
@@ -656,8 +657,14 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
       // the mask of the next step's block of 32 (its look-up is RING tiles old by then)
       if (((k + 2) & 31) == 0 && looked == k + 2) ok_mask = __ballot_sync(0xffffffffu, my_block >= 0);
     }
-    uses += nt;
     const float poison = failed ? __int_as_float(0x7fc00000) : 0.f;  // a tile never came: the result is not valid
+    if (failed && lane == 0) {  // leave no copy in flight: wait (bounded) for the tiles asked for and not taken
+      const uint64_t t0 = globaltimer();
+      for (int i = k; i < nt && i < k + RING; ++i)
+        while (!mbar_try_wait(&bar[(uses + i) % RING], ((uses + i) / RING) & 1) && globaltimer() - t0 < 1000000000ull) {
+        }
+    }
+    uses += nt;
 
     float2* ml = P.ml_part + (int64_t)piece * ROWS;
     float* op = P.o_part + (int64_t)piece * ROWS * D;
@@ -1287,7 +1294,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else {
     regs_down<REGS_REST>();
     if (warp == 12) {  // ---------------- loads ----------------
-      uint32_t j = 0;
+      uint32_t j = 0, keys = 0;  // blocks asked for: V, K
       bool ok = true;
       for (uint32_t d = 0; ok; ++d) {
         const Piece x = take(d);
@@ -1323,6 +1330,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           __syncwarp();
           if (mine) tma_load_4d(base + L::K + sk * 16384 + tile * TILE_BYTES, &tmk, &k_full[sk], 0, x.kvh, row0, blk);
+          keys = j + 1;
           ok = j < NE || wait_w(&e_empty[se], j / NE - 1, abort_v, P.err);
           if (!ok) break;
           if (lane == 0) {
@@ -1334,13 +1342,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (mine) tma_load_4d(base + L::E + se * 16384 + tile * TILE_BYTES, &tmv, &e_full[se], 0, x.kvh, row0, blk);
         }
       }
-      if (lane == 0 && *abort_v) {  // leave no copy in flight: wait (bounded) for the last use of every slot
+      if (lane == 0) {  // leave no copy in flight: wait (bounded) for the last use of every slot
         const uint64_t t0 = globaltimer();
         for (int i = 0; i < NK + NE; ++i) {
           uint64_t* bar = i < NK ? &k_full[i] : &e_full[i - NK];
-          const uint32_t ns = i < NK ? NK : NE, slot = i < NK ? i : i - NK;
-          if (j <= slot) continue;
-          const uint32_t use = (j - 1 - slot) / ns;
+          const uint32_t ns = i < NK ? NK : NE, slot = i < NK ? i : i - NK, asked = i < NK ? keys : j;
+          if (asked <= slot) continue;
+          const uint32_t use = (asked - 1 - slot) / ns;
           while (!mbar_try_wait(bar, use & 1) && globaltimer() - t0 < 1000000000ull) {
           }
         }

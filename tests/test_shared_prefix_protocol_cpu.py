@@ -1,0 +1,73 @@
+"""CPU models of what the shared-prefix kernels (csrc/shared_prefix.cu) leave behind when a wait runs out:
+no copy into shared memory may be in flight when a CTA ends.  Each model walks the kernel's own steps and slot arithmetic and stops at every wait in turn."""
+import pytest
+
+RING = 4  # pieces_kernel: 16-key tiles of a warp's ring
+
+
+def pieces_warp(tiles, stop, drain=True):
+    """One piece of `tiles` tiles whose waits run out at step `stop` (of two tiles), behind a ring that has
+    taken any number of tiles before.  Returns the copies in flight at the end, by tile."""
+    asked = set(range(min(RING, tiles)))  # the first RING tiles
+    taken = set()
+    k = 0
+    while k < tiles:
+        if k == stop:
+            break
+        taken |= {t for t in (k, k + 1) if t < tiles}
+        asked |= {t for t in (k + RING, k + RING + 1) if t < tiles and k + RING < tiles}
+        k += 2
+    else:
+        return asked - taken
+    waited = set(range(k, min(tiles, k + RING))) if drain else set()
+    assert waited <= asked, "a wait for a tile that was never asked for would only end by its limit"
+    for uses in range(2 * RING):  # the slots' phases: each slot is waited for once, one phase past the last taken
+        slots = [(uses + t) % RING for t in waited]
+        assert len(slots) == len(set(slots))
+        for t in waited:
+            before = [u for u in taken if (uses + u) % RING == (uses + t) % RING]
+            assert all((uses + u) // RING < (uses + t) // RING for u in before)
+            assert t < RING or (uses + t) // RING - 1 in [(uses + u) // RING for u in before]
+    return asked - taken - waited
+
+
+@pytest.mark.parametrize("tiles", range(1, 40))
+def test_pieces_leave_no_copy_in_flight(tiles):
+    for stop in range(0, tiles, 2):
+        assert not pieces_warp(tiles, stop)
+        assert pieces_warp(tiles, stop, drain=False)  # what the model is there to see
+
+
+def loader(blocks, stop, k_slots, v_slots, counts=2):
+    """prefix_kernel's loads of K and V blocks, stopped at wait number `stop` (None: never).  Returns the
+    copies in flight after the drain: ('k' or 'v', block).  counts=1: K drained by the count of V blocks."""
+    flight, keys, j, waits = set(), 0, 0, 0
+    while j < blocks:
+        if waits == stop:  # the K slot is not free
+            break
+        waits += 1
+        flight.add(("k", j))
+        keys = j + 1
+        if waits == stop:  # the V slot is not free
+            break
+        waits += 1
+        flight.add(("v", j))
+        j += 1
+    for i in range(k_slots + v_slots):
+        kind, n, slot = ("k", k_slots, i) if i < k_slots else ("v", v_slots, i - k_slots)
+        asked = keys if kind == "k" and counts == 2 else j
+        if asked <= slot:
+            continue
+        use = (asked - 1 - slot) // n
+        last = use * n + slot
+        assert last < asked <= last + n, "the last use of the slot"
+        flight -= {(kind, b) for b in range(slot, last + 1, n)}  # the phase before is complete, too
+    return flight
+
+
+@pytest.mark.parametrize("k_slots", [2, 3])
+@pytest.mark.parametrize("blocks", [1, 2, 3, 4, 7, 12])
+def test_the_loader_leaves_no_copy_in_flight(blocks, k_slots):
+    for stop in [None] + list(range(2 * blocks)):
+        assert not loader(blocks, stop, k_slots, 2)
+    assert any(loader(blocks, stop, k_slots, 2, counts=1) for stop in range(2 * blocks))
