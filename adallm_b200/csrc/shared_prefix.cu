@@ -86,6 +86,7 @@ struct Params {
   float* tc_o;         // [unit + CTA][256 rows][D]
   float2* tc_ml;       // [unit + CTA][256 rows]
   int64_t tc_rows;     // rows of the two
+  unsigned int* tc_lost;  // [CTA of prefix_kernel]: a wait ran out, its partials are not valid
 };
 
 // ---- metadata (lengths are cut to what the tables reach, row ranges to the rows there are) ----
@@ -693,7 +694,11 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
                 make_float2(acc[nb][mt][1], acc[nb][mt][3]);
       }
     }
-    if (failed) break;
+    if (failed) {  // nor is anything that this warp has left to do
+      for (piece += gridDim.x * WARPS; piece < pieces; piece += gridDim.x * WARPS)
+        if (lane < ROWS) P.ml_part[(int64_t)piece * ROWS + lane] = make_float2(poison, poison);
+      break;
+    }
   }
   if (P.prefix_tc) pdl_wait();  // so that the merge, which waits for this kernel, finds both done
 }
@@ -1273,11 +1278,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       // ---- the piece's partial
       if (ok) ok = wait_w(&o_full[t], done, abort_v, P.err);
+      if (!ok) break;  // (see tc_lost)
       ++done;
       tc_fence_after();
       const int64_t at = ((int64_t)x.unit + blockIdx.x) * ROWS + t * BM + r;
       if (at < P.tc_rows) {
-        if (valid) P.tc_ml[at] = ok ? make_float2(m, l) : make_float2(__int_as_float(0x7fc00000), 0.f);
+        if (valid) P.tc_ml[at] = make_float2(m, l);
         float* op = P.tc_o + at * D;
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
@@ -1479,6 +1485,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 13) tmem_dealloc(tmem, TMEM_COLS);
+  if (threadIdx.x == 0) P.tc_lost[blockIdx.x] = (unsigned)*abort_v;
 }
 
 // The row warps wait for registers that the others give back: only what the block was launched with is
@@ -1546,11 +1553,13 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
       }
     }
   };
+  unsigned int lost = 0;
   if (plan.blocks > 0) {
     const int r = plan.pre_row + hg;
     const int64_t unit = (int64_t)(r / tc::ROWS) * P.num_kv_heads + kvh, from = plan.tc_from + unit * plan.blocks;
     const int64_t c0 = tc::cta_of(plan.tc_total, plan.tc_ctas, from);
     const int64_t c1 = tc::cta_of(plan.tc_total, plan.tc_ctas, from + plan.blocks - 1);
+    for (int64_t c = c0 + lane; c <= c1; c += 32) lost |= P.tc_lost[c];
     gather((int)(c1 - c0 + 1), (plan.tc_units + unit + c0) * tc::ROWS + r % tc::ROWS, tc::ROWS, P.tc_ml, P.tc_o,
            P.tc_rows);
   }
@@ -1562,6 +1571,7 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
   };
   join(plan.pre_first, plan.pre_splits, plan.pre_row + hg);
   join(plan.own_first, plan.own_splits, plan.own_row + hg);
+  if (__any_sync(0xffffffffu, lost != 0)) L = __int_as_float(0x7fc00000);
   const float inv = L > 0.f ? P.v_scale / L : (L != L ? L : 0.f);  // a poisoned piece stays visible
   TO* op = reinterpret_cast<TO*>(P.out) + (int64_t)n * P.o_st + (int64_t)h * P.o_sh + 4 * lane;
   TO v[4] = {from_f32<TO>(O.x * inv), from_f32<TO>(O.y * inv), from_f32<TO>(O.z * inv), from_f32<TO>(O.w * inv)};
@@ -1620,7 +1630,7 @@ struct Layout {
   int nb;
   bool tc;  // enough rows for prefix_kernel
   int64_t pieces, tc_pieces;
-  size_t plan, ml, o, tc_ml, tc_o, bytes;  // offsets of the workspace's parts, its size
+  size_t plan, ml, o, tc_lost, tc_ml, tc_o, bytes;  // offsets of the workspace's parts, its size
 };
 inline Layout layout(int64_t total_q, int64_t groups, int64_t batch, int64_t heads, int64_t kv_heads) {
   Layout y;
@@ -1636,7 +1646,8 @@ inline Layout layout(int64_t total_q, int64_t groups, int64_t batch, int64_t hea
   y.plan = 0;
   y.ml = up((size_t)total_q * sizeof(RowPlan));
   y.o = up(y.ml + (size_t)y.pieces * rows * sizeof(float2));
-  y.tc_ml = up(y.o + (size_t)y.pieces * rows * D * sizeof(float));
+  y.tc_lost = up(y.o + (size_t)y.pieces * rows * D * sizeof(float));
+  y.tc_ml = up(y.tc_lost + (y.tc ? 148 * sizeof(unsigned int) : 0));
   y.tc_o = up(y.tc_ml + (size_t)y.tc_pieces * tc::ROWS * sizeof(float2));
   y.bytes = y.tc_o + (size_t)y.tc_pieces * tc::ROWS * D * sizeof(float);
   return y;
@@ -1730,6 +1741,7 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.max_pieces = (int32_t)(y.pieces < 0x7fffffff ? y.pieces : 0x7fffffff);
   const int64_t reach = (int64_t)max_prefix_pages * page_size;
   P.prefix_tc = y.tc && total_q * (int64_t)P.group * num_kv_heads * reach >= sp::TC_WORK ? 1 : 0;
+  P.tc_lost = reinterpret_cast<unsigned int*>(ws + y.tc_lost);
   P.tc_ml = reinterpret_cast<float2*>(ws + y.tc_ml);
   P.tc_o = reinterpret_cast<float*>(ws + y.tc_o);
   P.tc_rows = y.tc_pieces * sp::tc::ROWS;

@@ -1,5 +1,6 @@
 """CPU models of what the shared-prefix kernels (csrc/shared_prefix.cu) leave behind when a wait runs out:
-no copy into shared memory may be in flight when a CTA ends.  Each model walks the kernel's own steps and slot arithmetic and stops at every wait in turn."""
+no copy into shared memory may be in flight when a CTA ends, and every partial that was not computed has
+to be marked.  Each model walks the kernel's own steps and slot arithmetic and stops at every wait in turn."""
 import pytest
 
 RING = 4  # pieces_kernel: 16-key tiles of a warp's ring
@@ -71,3 +72,19 @@ def test_the_loader_leaves_no_copy_in_flight(blocks, k_slots):
     for stop in [None] + list(range(2 * blocks)):
         assert not loader(blocks, stop, k_slots, 2)
     assert any(loader(blocks, stop, k_slots, 2, counts=1) for stop in range(2 * blocks))
+
+
+@pytest.mark.parametrize("pieces,warps", [(1, 4), (7, 4), (50, 12), (12, 12)])
+def test_every_piece_of_a_warp_that_stops_is_marked(pieces, warps):
+    """Pieces go round the warps; one that stops marks the piece it is at and all that it had left."""
+    for who in range(warps):
+        mine = list(range(who, pieces, warps))
+        for at in range(len(mine)):
+            written = set(mine[:at])
+            marked = {mine[at]}
+            piece = mine[at] + warps
+            while piece < pieces:
+                marked.add(piece)
+                piece += warps
+            others = {p for p in range(pieces) if p % warps != who}
+            assert written | marked | others == set(range(pieces)) and not written & marked
