@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 3) draw_kernel(VerifyParams P) {
   // this one start: all inputs are settled, only its own results are waited for below.
   const int64_t b = blockIdx.x / P.draw_chunks;
   const int chunk = blockIdx.x % P.draw_chunks;
-  const int begin = max(0, __ldg(P.cu_q + b)), end = min(P.total_q, __ldg(P.cu_q + b + 1));
+  const int begin = min(max(0, __ldg(P.cu_q + b)), P.total_q), end = min(max(0, __ldg(P.cu_q + b + 1)), P.total_q);
   const int drafts = min(end - begin - 1, P.max_drafts);  // -1: an empty sequence
   const Scale sc(P.temps[b]);
   int64_t* tokens = P.tokens + b * (P.max_drafts + 1);
@@ -727,9 +727,10 @@ __global__ void __launch_bounds__(DRAW_THREADS, 3) draw_kernel(VerifyParams P) {
   // ---- the token after the accepted drafts: row `count`, row `run` of the last tile
   const T* x = reinterpret_cast<const T*>(P.target) + (int64_t)(begin + count) * P.ld;
   const Stats st = rows_s[run];
-  auto finish = [&](int winner) {
-    tokens[count] = winner != NONE ? winner : -1;
-    logprobs[count] = winner != NONE ? sc.diff(as_f32(x[winner]), st.m) / sc.t - logf(st.s) : 0.f;
+  auto finish = [&](int winner) {  // (a list that does not ascend leaves rows without statistics, and any winner)
+    const bool any = winner >= 0 && winner < P.n;
+    tokens[count] = any ? winner : -1;
+    logprobs[count] = any ? sc.diff(as_f32(x[winner]), st.m) / sc.t - logf(st.s) : 0.f;
   };
   if (sc.greedy || !(st.s > 0.f)) {
     if (chunk == 0 && tid == 0) finish(st.s > 0.f ? st.at : NONE);

@@ -139,3 +139,20 @@ def test_windows_wider_than_all_positions(rows, reach):
         assert float((got - want).float().abs().max()) <= 2 ** -8 * float(want.float().abs().max()), window
         if window >= reached:
             assert torch.equal(got, want), window
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 3, 8], [-3, 4, 6, 8], [0, 2 ** 31 - 1, -2 ** 31, 8], [8, 6, 2, 0], [5, 5, 9, 12]])
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+def test_verify_lists_that_do_not_ascend(cu, temperature):
+    """Such a list has no meaning, but the call stays inside its tensors: tokens of the vocabulary or -1,
+    whatever the workspace held before."""
+    g = torch.Generator().manual_seed(3)
+    v = 1003
+    a = [t.to(dev()) for t in (torch.randn((8, v), generator=g), torch.randint(0, v, (8,), generator=g),
+                               torch.tensor(cu, dtype=torch.int32), torch.full((3,), temperature),
+                               torch.rand((3, 2), generator=g), torch.empty((3, v)).exponential_(1.0, generator=g))]
+    for fill in (0x00, 0x7F, 0xFF):
+        room = torch.full((1 << 16,), fill, dtype=torch.uint8, device=dev())
+        tokens, accepted, _ = verify_drafts(*a, workspace=room)
+        assert bool(((tokens >= -1) & (tokens < v)).all())
+        assert bool(((accepted >= 0) & (accepted <= 2)).all())
