@@ -253,7 +253,13 @@ __device__ __forceinline__ int split_tiles(const int2* work, int segs, int max_p
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   units = __reduce_add_sync(0xffffffffu, units);
-  return (int)max((int64_t)MIN_TILES, all / max(1, max_pieces - units) + 1);
+  return (int)min(max((int64_t)MIN_TILES, all / max(1, max_pieces - units) + 1), (int64_t)1 << 27);
+}
+
+// Pieces of a lane's segments.  Lists that overlap can name any number: the count stops at 2^26 - 1 (a
+// workspace of as many pieces would be 256 GB), so that 32 lanes' sum stays in 32 bits and still ascends.
+__device__ __forceinline__ int more_pieces(int before, int2 splits_units) {
+  return (int)min(before + (int64_t)splits_units.x * splits_units.y, (int64_t)(1 << 26) - 1);
 }
 
 template <typename TQ, int NB>
@@ -308,7 +314,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
     for (int s = from; s < to; ++s) {
       const int tiles = work[s].x;
       work[s].x = tiles < (1 << 21) ? ceil_div_small(tiles, inverse) : (tiles + ct - 1) / ct;
-      mine += work[s].x * work[s].y;
+      mine = more_pieces(mine, work[s]);
     }
     int acc = mine;
 #pragma unroll
@@ -316,10 +322,11 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
       const int up = __shfl_up_sync(0xffffffffu, acc, o);
       if (lane >= o) acc += up;
     }
-    int before = acc - mine;
+    const int before = acc - mine;
+    mine = 0;
     for (int s = from; s < to; ++s) {
-      first[s] = before;
-      before += work[s].x * work[s].y;
+      first[s] = before + mine;
+      mine = more_pieces(mine, work[s]);
     }
     if (lane == 31) first[segs] = acc;
   }
@@ -371,8 +378,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
     for (int n = threadIdx.x; n < P.total_q; n += WARPS * 32)
       if (n < from || n >= to) P.plan[n] = none;
   }
-  // (group lists that overlap could name more than the workspace holds)
-  const int pieces = first[segs] < 0 ? P.max_pieces : min(first[segs], P.max_pieces);
+  const int pieces = min(first[segs], P.max_pieces);  // (lists that overlap could name more than the workspace holds)
   uint32_t uses = 0;  // tiles through the ring (slot = uses % RING, parity = (uses / RING) & 1)
   for (int piece = blockIdx.x * WARPS + warp; piece < pieces; piece += gridDim.x * WARPS) {
     int s = 0;  // the last segment with first[s] <= piece (it is not empty), 32 probes at a time
@@ -1165,7 +1171,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int lo = 0, hi = 0;
       if (valid) hi = x.len;
       if (valid && x.cut) {
-        const int b = sequence_of(P, n);
+        const int b = max(0, sequence_of(P, n));  // (-1: only from lists that do not ascend)
         const int pos = x.len + own_len(P, b) - (q_begin(P, b + 1) - n);
         hi = min(x.len, pos + 1);
         lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
@@ -1282,7 +1288,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       ++done;
       tc_fence_after();
       const int64_t at = ((int64_t)x.unit + blockIdx.x) * ROWS + t * BM + r;
-      if (at < P.tc_rows) {
+      if ((uint64_t)at < (uint64_t)P.tc_rows) {
         if (valid) P.tc_ml[at] = make_float2(m, l);
         float* op = P.tc_o + at * D;
 #pragma unroll 1
@@ -1524,7 +1530,7 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
     for (int s0 = 0; s0 < count; s0 += 32) {
       float2 ml = make_float2(-INFINITY, 0.f);
       const int64_t mine = row0 + (s0 + lane) * step;
-      if (s0 + lane < count && mine < limit) ml = mls[mine];
+      if (s0 + lane < count && (uint64_t)mine < (uint64_t)limit) ml = mls[mine];
       float most = ml.x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -1559,7 +1565,7 @@ __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
     const int64_t unit = (int64_t)(r / tc::ROWS) * P.num_kv_heads + kvh, from = plan.tc_from + unit * plan.blocks;
     const int64_t c0 = tc::cta_of(plan.tc_total, plan.tc_ctas, from);
     const int64_t c1 = tc::cta_of(plan.tc_total, plan.tc_ctas, from + plan.blocks - 1);
-    for (int64_t c = c0 + lane; c <= c1; c += 32) lost |= P.tc_lost[c];
+    for (int64_t c = max(c0, (int64_t)0) + lane; c <= c1 && c < P.tc_ctas; c += 32) lost |= P.tc_lost[c];
     gather((int)(c1 - c0 + 1), (plan.tc_units + unit + c0) * tc::ROWS + r % tc::ROWS, tc::ROWS, P.tc_ml, P.tc_o,
            P.tc_rows);
   }
@@ -1738,7 +1744,7 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.plan = reinterpret_cast<sp::RowPlan*>(ws + y.plan);
   P.ml_part = reinterpret_cast<float2*>(ws + y.ml);
   P.o_part = reinterpret_cast<float*>(ws + y.o);
-  P.max_pieces = (int32_t)(y.pieces < 0x7fffffff ? y.pieces : 0x7fffffff);
+  P.max_pieces = (int32_t)(y.pieces < (1 << 26) ? y.pieces : (1 << 26) - 1);
   const int64_t reach = (int64_t)max_prefix_pages * page_size;
   P.prefix_tc = y.tc && total_q * (int64_t)P.group * num_kv_heads * reach >= sp::TC_WORK ? 1 : 0;
   P.tc_lost = reinterpret_cast<unsigned int*>(ws + y.tc_lost);

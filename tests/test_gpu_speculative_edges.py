@@ -156,3 +156,29 @@ def test_verify_lists_that_do_not_ascend(cu, temperature):
         tokens, accepted, _ = verify_drafts(*a, workspace=room)
         assert bool(((tokens >= -1) & (tokens < v)).all())
         assert bool(((accepted >= 0) & (accepted <= 2)).all())
+
+
+@pytest.mark.parametrize("reach", [0, 1 << 14])
+def test_attention_lists_that_do_not_ascend(reach):
+    """Rows and sequences claimed several times over, or before and past all there are: the call stays inside
+    its tensors, and lists in order give what they gave."""
+    n = 12
+    c = osp.make_shared_prefix_case(9, [100, 60], [7, 5], [5 + i for i in range(n)], [4] * n, 32, 8, 16)
+    c = {k: v.to(dev()) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    c["prefix_tables"] = torch.nn.functional.pad(c["prefix_tables"], (0, reach), value=-1)
+
+    def run(**kw):
+        a = {**c, **kw}
+        return shared_prefix_decode(a["q"], a["k_cache"], a["v_cache"], a["prefix_tables"], a["prefix_lens"],
+                                    a["cu_groups"], a["block_tables"], a["context_lens"], a["scale"],
+                                    cu_seqlens_q=a["cu_seqlens_q"])
+
+    want = run()
+    i32 = dict(dtype=torch.int32, device=dev())
+    low, high = -2 ** 31, 2 ** 31 - 1
+    for cu_q in ([0, 48] * 6 + [0], [48] * 6 + [0] * 7, [low, high] * 6 + [low], list(range(24, -2, -2))):
+        assert run(cu_seqlens_q=torch.tensor(cu_q, **i32)).shape == want.shape
+    for cu_g in ([0, 12, 0], [12, 0, 12], [low, high, low], [5, 5, 3]):
+        assert run(cu_groups=torch.tensor(cu_g, **i32)).shape == want.shape
+    torch.cuda.synchronize()
+    assert torch.equal(run(), want)

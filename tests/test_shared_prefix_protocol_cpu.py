@@ -1,6 +1,9 @@
 """CPU models of what the shared-prefix kernels (csrc/shared_prefix.cu) leave behind when a wait runs out:
 no copy into shared memory may be in flight when a CTA ends, and every partial that was not computed has
-to be marked.  Each model walks the kernel's own steps and slot arithmetic and stops at every wait in turn."""
+to be marked.  Each model walks the kernel's own steps and slot arithmetic and stops at every wait in turn.
+And a model of the plan's counts for lists that name more pieces than there can be."""
+import random
+
 import pytest
 
 RING = 4  # pieces_kernel: 16-key tiles of a warp's ring
@@ -88,3 +91,33 @@ def test_every_piece_of_a_warp_that_stops_is_marked(pieces, warps):
                 piece += warps
             others = {p for p in range(pieces) if p % warps != who}
             assert written | marked | others == set(range(pieces)) and not written & marked
+
+
+def plan(work, cap=(1 << 26) - 1):
+    """pieces_kernel's scan: `work` is (splits, row blocks * heads) by segment; the pieces before each segment
+    and in all, each lane counting a run of segments in 32 bits."""
+    segs = len(work)
+    run = -(-segs // 32)
+    first, total = [0] * segs, 0
+    for lane in range(32):
+        mine = 0
+        for s in range(min(segs, lane * run), min(segs, lane * run + run)):
+            first[s] = total + mine
+            mine = min(mine + work[s][0] * work[s][1], cap) if cap else mine + work[s][0] * work[s][1]
+        total += mine
+    wrap = lambda v: (v + (1 << 31)) % (1 << 32) - (1 << 31)  # noqa: E731
+    return [wrap(v) for v in first] + [wrap(total)]
+
+
+@pytest.mark.parametrize("segs", [1, 3, 32, 33, 1000, 4096])
+def test_the_plan_ascends_whatever_the_lists_say(segs):
+    """Also where every sequence claims all rows there can be (2^30 row-heads): a count that wrapped around
+    would name pieces and rows before the workspace."""
+    rnd = random.Random(segs)
+    fair = [(rnd.randint(0, 9), rnd.randint(0, 40)) for _ in range(segs)]
+    assert plan(fair) == plan(fair, cap=None) and plan(fair)[-1] == sum(a * b for a, b in fair)
+    wild = [(rnd.choice((0, 1, 1 << 10, 1 << 24)), rnd.choice((0, 8, 1 << 20, 1 << 27))) for _ in range(segs)]
+    for work in (wild, [(1 << 24, 1 << 27)] * segs, [(1, 1 << 27)] * segs):
+        first = plan(work)
+        assert all(0 <= a <= b for a, b in zip(first, first[1:]))
+    assert segs < 32 or min(plan([(1, 1 << 27)] * segs, cap=None)) < 0
