@@ -58,6 +58,8 @@ struct RowPlan {
 struct Params {
   const void* q;
   int64_t q_st, q_sh;
+  const uint8_t* v;  // the V cache itself, for mark_nan, and its strides
+  int64_t v_page, v_tok, v_head;
   int64_t num_pages;
   const int32_t* pt;  // [groups][max_prefix_pages]
   int64_t pt_stride;
@@ -162,6 +164,64 @@ __device__ __forceinline__ int64_t tc_ctas_of(int64_t total, int sms) {
   if (total > 2 * sms) return sms;
   const int half = max(1, sms / 2), each = max(1, ((int)total + half - 1) / half);
   return ((int)total + each - 1) / each;
+}
+
+// ---- NaN among the values ----------------------------------------------------------------------------
+// A weight of 0 does not take a NaN out of P.V, so a NaN value would reach the rows that do not see its key
+// (a later draft's token, a key that has left the window).  Where rows see different keys, NaN values are
+// taken as 0 in shared memory, and the dimensions in which each row does see one are looked up in the cache
+// and marked over the stored sums.  prefix_kernel looks for them in every block of such a piece (a warp of
+// its own marks them); pieces_kernel, whose tiles are short, finds them in a piece's sums and runs the piece
+// once more.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {  // e4m3 NaN: 0x80 in the byte
+  return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~((nan_bytes(w) >> 7) * 0xFFu); }
+// Thread `who` of `whos`: its share of the 16-byte chunks of a tile without NaN; whether there were any.
+__device__ __forceinline__ bool clean(uint8_t* tile, int chunks, int who, int whos) {
+  bool any = false;
+#pragma unroll 1
+  for (int i = who; i < chunks; i += whos) {
+    const uint4 e = *reinterpret_cast<const uint4*>(tile + 16 * i);
+    if (!(nan_bytes(e.x) | nan_bytes(e.y) | nan_bytes(e.z) | nan_bytes(e.w))) continue;
+    any = true;
+    *reinterpret_cast<uint4*>(tile + 16 * i) =
+        make_uint4(without_nan(e.x), without_nan(e.y), without_nan(e.z), without_nan(e.w));
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the slot is loaded again
+  }
+  __syncwarp();
+  return any;
+}
+// Warp-wide: NaN over the dimensions [d0, d0 + dims) of each lane's sums `o` in which one of the keys [lo, hi)
+// that it sees has a NaN value; keys [from, to) of the page list are looked at.
+__device__ __forceinline__ void mark_nan(const Params& P, const int32_t* table, int kvh, int from, int to, int lo, int hi,
+                                         float* o, int d0, int dims) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int k0 = from; k0 < to; k0 += 32) {
+    int blk = -1, row = 0;  // of this lane's key
+    if (k0 + lane < to) {
+      const int at = P.by_page.div(k0 + lane);
+      row = k0 + lane - at * P.page;
+      blk = __ldg(table + at);
+    }
+    const bool there = blk >= 0 && blk < P.num_pages;
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(
+        P.v + (there ? blk * P.v_page + row * P.v_tok + kvh * P.v_head : 0));
+#pragma unroll 1
+    for (int w = 0; w < D / 4; ++w) {
+      const uint32_t bad = there ? nan_bytes(x[w]) : 0u;
+#pragma unroll 1
+      for (uint32_t who = __ballot_sync(0xffffffffu, bad != 0); who; who &= who - 1) {
+        const int key = k0 + __ffs(who) - 1;
+        const uint32_t b = __shfl_sync(0xffffffffu, bad, __ffs(who) - 1);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+          if (((b >> (8 * i + 7)) & 1u) && key >= lo && key < hi && 4 * w + i >= d0 && 4 * w + i < d0 + dims)
+            o[4 * w + i] = __int_as_float(0x7fc00000);
+      }
+    }
+  }
 }
 
 // ---- pieces of few rows: one warp each, warp-level MMA --------------------------------------------
@@ -380,6 +440,7 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
   }
   const int pieces = min(first[segs], P.max_pieces);  // (lists that overlap could name more than the workspace holds)
   uint32_t uses = 0;  // tiles through the ring (slot = uses % RING, parity = (uses / RING) & 1)
+  bool careful = false;  // this piece's NaN values are to be taken as 0
   for (int piece = blockIdx.x * WARPS + warp; piece < pieces; piece += gridDim.x * WARPS) {
     int s = 0;  // the last segment with first[s] <= piece (it is not empty), 32 probes at a time
     for (int step = segs <= 32 ? 1 : (segs <= 1024 ? 32 : 1024);; step >>= 5) {
@@ -524,6 +585,9 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
         failed = true;
         break;
       }
+      if (__builtin_expect(careful, 0))
+        for (int u = 0; u < (two ? 2 : 1); ++u)
+          clean(ring + ((uses + k + u) % RING) * 2 * TILE_BYTES + TILE_BYTES, TILE_BYTES / 16, lane, 32);
       const int tt = t_begin + TILE * k;
       const uint32_t ok2 = (ok_mask >> (k & 31)) & (two ? 3u : 1u);  // which of the two tiles are there
       float sc[NB][2][4];
@@ -664,6 +728,19 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
       // the mask of the next step's block of 32 (its look-up is RING tiles old by then)
       if (((k + 2) & 31) == 0 && looked == k + 2) ok_mask = __ballot_sync(0xffffffffu, my_block >= 0);
     }
+    if (__builtin_expect((t_begin < lo_max || hi_min < t_end) && !careful && !failed, 0)) {
+      float sum = 0.f;  // a key that some row does not see: a NaN may be another row's
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) sum += (acc[nb][mt][0] + acc[nb][mt][1]) + (acc[nb][mt][2] + acc[nb][mt][3]);
+      if (__any_sync(0xffffffffu, sum != sum)) {  // the piece once more, without NaN values
+        careful = true;
+        uses += nt;
+        piece -= gridDim.x * WARPS;
+        continue;
+      }
+    }
     const float poison = failed ? __int_as_float(0x7fc00000) : 0.f;  // a tile never came: the result is not valid
     if (failed && lane == 0) {  // leave no copy in flight: wait (bounded) for the tiles asked for and not taken
       const uint64_t t0 = globaltimer();
@@ -700,6 +777,16 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
                 make_float2(acc[nb][mt][1], acc[nb][mt][3]);
       }
     }
+    if (__builtin_expect(careful, 0)) {  // over the sums that this lane has just stored
+#pragma unroll 1
+      for (int r = 0; r < 2 * NB; ++r) {
+        const int row = (r >> 1) * 8 + 2 * c + (r & 1);
+        const int from = NB == 2 && r > 1 ? (r & 1 ? lo[NB - 1][1] : lo[NB - 1][0]) : (r & 1 ? lo[0][1] : lo[0][0]);
+        const int to = NB == 2 && r > 1 ? (r & 1 ? hi[NB - 1][1] : hi[NB - 1][0]) : (r & 1 ? hi[0][1] : hi[0][0]);
+        mark_nan(P, table, kvh, t_begin, t_end, from, rb * ROWS + row < rows ? to : 0, op + row * D, 16 * g, 16);
+      }
+      careful = false;
+    }
     if (failed) {  // nor is anything that this warp has left to do
       for (piece += gridDim.x * WARPS; piece < pieces; piece += gridDim.x * WARPS)
         if (lane < ROWS) P.ml_part[(int64_t)piece * ROWS + lane] = make_float2(poison, poison);
@@ -724,21 +811,22 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
 //   O_t += P_t . V  kind::f16; V is widened to fp16 (exact) by four warps, once for both tiles.
 // Roles (16 warps): 0-3 widen V; 4-7 and 8-11 take tile 0's and tile 1's rows (thread = row: queries to
 // terms, softmax, O to the workspace); 12 loads (TMA, eight 16-key tiles a block for K and V each);
-// 13 issues the MMAs; 14 walks the CTA's range and hands out its pieces.  The row warps take 192
+// 13 issues the MMAs; 14 walks the CTA's range and hands out its pieces; 15 marks NaN values.  The row warps take 192
 // registers a thread (a row of S at once), the others 64.  P.V of a block and S of the next are issued
 // together for a tile, so one tile's MMAs run under the other tile's softmax.  All tcgen05 operations come
 // from one thread in order, so s_full of block j + 1 also says that P.V of block j is complete: O may be
 // rescaled.
 // Barriers, phase = use: d_full/d_empty (pieces), k_full/k_empty (K slots), e_full/e_empty (e4m3 V
 // slots), v_full/v_empty (fp16 V slots), s_full[t], p_full[t][half] (a block's S, P of tile t), q_full[t],
-// o_full[t] (a piece's Q, O).  A tile's next S and its next P.V wait for q_full and p_full, which its warps
+// o_full[t] (a piece's Q, O), stored (a cut piece's partial; the rows are at most two pieces ahead of the
+// warp that waits for it).  A tile's next S and its next P.V wait for q_full and p_full, which its warps
 // give after they have written the piece before.  Every wait is bounded and ends all roles through the
 // abort flag.
 namespace tc {
 constexpr int BM = 128, BN = 128, TILES = 2, ROWS = TILES * BM;
 static_assert(BN == TC_KEYS && ROWS == 1 << TC_ROWS_LOG2, "shape of a unit");
 constexpr int THREADS = 16 * 32;
-constexpr int NE = 2, NV = 2, ND = 2;
+constexpr int NE = 2, NV = 2, ND = 2, NS = 4;
 constexpr int REGS_LAUNCH = 128, REGS_ROWS = 192, REGS_REST = 64;  // a thread: 4 * 128 = 2 * 192 + 2 * 64
 static_assert(2 * REGS_ROWS + 2 * REGS_REST <= 4 * REGS_LAUNCH, "registers of the block");
 // Queries as sums of e4m3 terms.  Of a row scaled to a maximum in [128, 256) a
@@ -774,8 +862,8 @@ template <int TERMS> struct Smem {
   static constexpr int E = K + NK * 16384;               // e4m3 V slots
   static constexpr int V = E + NE * 16384;               // fp16 V slots [2 halves of d][128 keys][128 B]
   static constexpr int BAR = V + NV * 32768;
-  static constexpr int NBAR = 2 * ND + 2 * NK + 2 * NE + 2 * NV + 5 * TILES + 1;
-  static constexpr int END = BAR + NBAR * 8 + ND * (int)sizeof(Piece) + NE * 4 + 8;
+  static constexpr int NBAR = 2 * ND + 2 * NK + 2 * NE + 2 * NV + 5 * TILES + 1 + NS;
+  static constexpr int END = BAR + NBAR * 8 + ND * (int)sizeof(Piece) + NE * 4 + 12;
   static constexpr int BYTES = 1024 + END;
 };
 static_assert(Smem<2>::BYTES <= 232448 && Smem<3>::BYTES <= 232448, "shared memory per CTA");
@@ -997,15 +1085,17 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* q_full = p_full + 2 * TILES;
   uint64_t* o_full = q_full + TILES;
   uint64_t* fin = o_full + TILES;
-  Piece* pieces = reinterpret_cast<Piece*>(fin + 1);
+  uint64_t* stored = fin + 1;
+  Piece* pieces = reinterpret_cast<Piece*>(stored + NS);
   int* e_ok = reinterpret_cast<int*>(pieces + ND);  // which of a V slot's page tiles are there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(e_ok + NE);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* abort_v = abort_flag;
+  volatile int* nan_v = abort_flag + 1;  // a NaN value was taken as 0
   if (threadIdx.x == 0) {
     for (int i = 0; i < ND; ++i) {
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], 14);
+      mbar_init(&d_empty[i], 15);
     }
     for (int i = 0; i < NK; ++i) {
       mbar_init(&k_full[i], 1);
@@ -1027,7 +1117,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&o_full[t], 1);
     }
     mbar_init(fin, 1);
+    for (int i = 0; i < NS; ++i) mbar_init(&stored[i], 8);
     *abort_flag = 0;
+    *nan_v = 0;
     prefetch_tmap(&tmk);
     prefetch_tmap(&tmv);
     fence_mbar_init();
@@ -1051,6 +1143,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     return x;
   };
 
+  // The keys [lo, hi) of a piece's prefix that row `row` of its group sees.
+  auto seen_keys = [&](int row, const Piece& x, int& lo, int& hi) {
+    const int n = x.tok0 + P.by_group.div(row), b = max(0, sequence_of(P, n));  // (-1: only from lists that do not ascend)
+    const int pos = x.len + own_len(P, b) - (q_begin(P, b + 1) - n);
+    hi = min(x.len, pos + 1);
+    lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
+  };
+
   if (warp < 4) {  // ---------------- V: e4m3 -> fp16 ----------------
     regs_down<REGS_REST>();
     const int ct = threadIdx.x;
@@ -1067,8 +1167,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           break;
         }
         const int key0 = x.k0 + (x.blk + i) * BN, there = e_ok[se];
-        const uint8_t* src = base + L::E + se * 16384;
+        uint8_t* src = base + L::E + se * 16384;
         uint8_t* dst = base + L::V + sv * 32768;
+        // (what this warp widens below; published by the arrive there, the product and its commit)
+        if (x.cut && clean(src, min(BN, x.len - key0) * 8, ct, 128)) *nan_v = 1;
 #pragma unroll 4
         for (int u = 0; u < 8; ++u) {
           const int id = ct + 128 * u, key = id >> 3, ch = id & 7;
@@ -1109,9 +1211,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Piece x = take(d);
       if (!x.n) break;
       const int row = x.rb * ROWS + t * BM + r, rows = x.tokens * P.group;
-      if (x.rb * ROWS + t * BM >= rows) continue;  // the unit has no rows in this tile
+      if (x.rb * ROWS + t * BM >= rows) {  // the unit has no rows in this tile
+        if (x.cut && lane == 0) mbar_arrive_plain(&stored[d % NS]);
+        continue;
+      }
       const bool valid = row < rows;
-      const int n = x.tok0 + P.by_group.div(row);
       // ---- the warp's 32 rows of queries as e4m3 terms, eight lanes a row.  The rows are copied into the
       // place of their first two terms and converted there; the loop is kept short, since this runs once
       // a piece and fetching unrolled code took longer than running it.
@@ -1170,12 +1274,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---- the keys that the row sees
       int lo = 0, hi = 0;
       if (valid) hi = x.len;
-      if (valid && x.cut) {
-        const int b = max(0, sequence_of(P, n));  // (-1: only from lists that do not ascend)
-        const int pos = x.len + own_len(P, b) - (q_begin(P, b + 1) - n);
-        hi = min(x.len, pos + 1);
-        lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
-      }
+      if (valid && x.cut) seen_keys(row, x, lo, hi);
       const int32_t* table = P.pt + (int64_t)x.g * P.pt_stride;
       const int tile0 = x.blk * (BN / TILE);  // of the piece's first block, from k0
       auto entry = [&](int tile) {            // is the page of this lane's key tile there?
@@ -1302,6 +1401,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       tc_fence_before();
+      if (x.cut) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive_plain(&stored[d % NS]);
+      }
     }
   } else {
     regs_down<REGS_REST>();
@@ -1484,6 +1587,23 @@ __global__ void __launch_bounds__(THREADS, 1)
           mbar_arrive_plain(&d_full[d % ND]);
         }
         if (!x.n) break;
+      }
+    } else {  // ---------------- NaN values (cut is the same for all pieces) ----------------
+      for (uint32_t d = 0;; ++d) {
+        const Piece x = take(d);
+        if (!x.n) break;
+        if (!x.cut) continue;
+        if (!wait_w(&stored[d % NS], d / NS, abort_v, P.err)) break;
+        if (!*nan_v) continue;
+        const int rows = min(ROWS, x.tokens * P.group - x.rb * ROWS);
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 32) {
+          int lo = 0, hi = 0;
+          const int64_t at = ((int64_t)x.unit + blockIdx.x) * ROWS + r0 + lane;
+          if (r0 + lane < rows && (uint64_t)at < (uint64_t)P.tc_rows) seen_keys(x.rb * ROWS + r0 + lane, x, lo, hi);
+          mark_nan(P, P.pt + x.g * P.pt_stride, x.kvh, x.k0 + x.blk * BN, min(x.len, x.k0 + (x.blk + x.n) * BN), lo, hi,
+                   P.tc_o + at * D, 0, D);
+        }
       }
     }
   }
@@ -1710,6 +1830,10 @@ extern "C" int ada_fp8_shared_prefix_decode(
   P.q = q;
   P.q_st = q_stride_t;
   P.q_sh = q_stride_h;
+  P.v = v_cache;
+  P.v_page = kv_stride_page;
+  P.v_tok = kv_stride_tok;
+  P.v_head = kv_stride_head;
   P.num_pages = num_pages;
   P.pt = prefix_tables;
   P.pt_stride = pt_stride;

@@ -182,3 +182,81 @@ def test_attention_lists_that_do_not_ascend(reach):
         assert run(cu_groups=torch.tensor(cu_g, **i32)).shape == want.shape
     torch.cuda.synchronize()
     assert torch.equal(run(), want)
+
+
+def _matches(out, ref, vmax):
+    """NaN where the definition is NaN, and elsewhere the tolerance of tests/test_gpu_shared_prefix.py."""
+    out = out.cpu()
+    assert torch.equal(out.isnan(), ref.isnan())
+    ulp = 2 ** -8 if out.dtype == torch.bfloat16 else 2 ** -11
+    off = ((out.double() - ref).abs() - ulp * ref.abs() - 2 ** -10 * vmax).nan_to_num(nan=-1.0)
+    assert float(off.max()) <= 0, float(off.max())
+
+
+@pytest.mark.parametrize("reach", [0, 1 << 14])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [4, 3, 1], [40, 30, 9]])
+@pytest.mark.parametrize("window", [0, 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_nan_keys_and_values_reach_the_rows_that_see_them_alone(rows, window, reach, dtype):
+    """Single elements and whole keys: before the windows, at their edges, among the newest tokens, in pages
+    that end inside a tile."""
+    c = osp.make_shared_prefix_case(11, [301], [3], [50, 90, 33], rows, 32, 8, 16, dtype)
+    vmax = float(c["v_cache"].float().nan_to_num(0.0).abs().max())
+    d = {k: v.to(dev()) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    d["prefix_tables"] = torch.nn.functional.pad(d["prefix_tables"], (0, reach), value=-1)
+
+    def place(table, key):
+        return int(table[key // 16]), key % 16
+
+    spots = [("v_cache", place(c["prefix_tables"][0], k), h, at) for k, h, at in
+             ((5, slice(None), slice(None)), (230, 2, 17), (250, 0, 127), (290, 7, 64), (300, 3, 5))]
+    spots += [("v_cache", place(c["block_tables"][0], k), h, at) for k, h, at in
+              ((49, 1, 0), (48, slice(None), slice(None)), (46, 5, 33), (20, 6, 100))]
+    spots += [("v_cache", place(c["block_tables"][2], 32), 4, 77), ("k_cache", place(c["block_tables"][1], 89), 2, 9),
+              ("k_cache", place(c["prefix_tables"][0], 7), slice(None), slice(None))]
+    if window == 0:  # without a window the rows see all of the prefix: leave it some finite output
+        spots = [s for s in spots if s[2] != slice(None)]
+    for some in (spots[:1], spots[4:7], spots):
+        for cache in ("k_cache", "v_cache"):
+            d[cache].copy_(c[cache].to(dev()))
+        host = {n: c[n].clone() for n in ("k_cache", "v_cache")}
+        for name, (block, row), head, at in some:
+            host[name].view(torch.uint8)[block, row, head, at] = osp.NAN_BYTE
+        for cache in host:
+            d[cache].copy_(host[cache].to(dev()))
+        out = shared_prefix_decode(d["q"], d["k_cache"], d["v_cache"], d["prefix_tables"], d["prefix_lens"],
+                                   d["cu_groups"], d["block_tables"], d["context_lens"], d["scale"],
+                                   cu_seqlens_q=d["cu_seqlens_q"], window=window)
+        ref = osp.shared_prefix_decode(c["q"], host["k_cache"], host["v_cache"], c["prefix_tables"], c["prefix_lens"],
+                                       c["cu_groups"], c["block_tables"], c["context_lens"], c["scale"],
+                                       cu_seqlens_q=c["cu_seqlens_q"], window=window)
+        assert not bool(ref.isnan().all())
+        _matches(out, ref, vmax)
+
+
+@pytest.mark.parametrize("reach", [0, 1 << 14])
+def test_nan_values_in_many_short_prefixes(reach):
+    """Several pieces a CTA and a warp, of which some hold NaN values behind the windows of some rows."""
+    groups, rng = 40, np.random.default_rng(5)
+    prefixes = rng.integers(1, 260, groups).tolist()
+    own = rng.integers(9, 60, groups).tolist()
+    c = osp.make_shared_prefix_case(12, prefixes, [1] * groups, own, rng.integers(20, 50, groups).tolist(), 8, 4, 16)
+    vmax = float(c["v_cache"].float().nan_to_num(0.0).abs().max())
+    for g in range(0, groups, 3):
+        key = int(rng.integers(0, prefixes[g]))
+        c["v_cache"].view(torch.uint8)[int(c["prefix_tables"][g, key // 16]), key % 16, g % 4, rng.integers(0, 128, 5)] = 0xFF
+    for g in range(1, groups, 4):
+        key = int(rng.integers(0, own[g]))
+        c["v_cache"].view(torch.uint8)[int(c["block_tables"][g, key // 16]), key % 16, g % 4, 64:] = 0x7F
+    d = {k: v.to(dev()) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    d["prefix_tables"] = torch.nn.functional.pad(d["prefix_tables"], (0, reach), value=-1)
+    for window in (0, 30, 100):
+        def run(a):
+            f = shared_prefix_decode if a is d else osp.shared_prefix_decode
+            return f(a["q"], a["k_cache"], a["v_cache"], a["prefix_tables"], a["prefix_lens"], a["cu_groups"],
+                     a["block_tables"], a["context_lens"], a["scale"], cu_seqlens_q=a["cu_seqlens_q"], window=window)
+
+        out, ref = run(d), run(c)
+        assert bool(ref.isnan().any())
+        _matches(out, ref, vmax)
+        assert torch.equal(torch.nan_to_num(run(d), 7.0), torch.nan_to_num(out, 7.0))

@@ -121,3 +121,36 @@ def test_the_plan_ascends_whatever_the_lists_say(segs):
         first = plan(work)
         assert all(0 <= a <= b for a, b in zip(first, first[1:]))
     assert segs < 32 or min(plan([(1, 1 << 27)] * segs, cap=None)) < 0
+
+
+def marker(pieces, bars, seed, ring=2):
+    """prefix_kernel's rows and the warp that marks NaN values behind them, over a ring of `ring` pieces and
+    `bars` barriers: how far the rows get ahead, and whether a wait could see a phase past the one it is for."""
+    rnd = random.Random(seed)
+    given = taken = stored = marked = 0  # pieces: handed out, taken by the rows, stored, taken by the marker
+    waiting, ahead, alias = None, 0, False
+    done = [0] * bars  # completed phases
+    while marked < pieces or waiting is not None:
+        step = rnd.choice(("give", "take", "store", "mark", "wait"))
+        if step == "give" and given < pieces and given < min(taken, marked) + ring:
+            given += 1
+        elif step == "take" and taken == stored and taken < given:
+            taken += 1
+        elif step == "store" and stored < taken:
+            done[stored % bars] += 1
+            stored += 1
+        elif step == "mark" and waiting is None and marked < given:
+            waiting, marked = marked, marked + 1
+        elif step == "wait" and waiting is not None:
+            phases = done[waiting % bars] - waiting // bars  # 1: complete; 2 would look like 0
+            ahead, alias = max(ahead, stored - waiting), alias or phases > 1
+            if phases >= 1:
+                waiting = None
+    return ahead, alias
+
+
+@pytest.mark.parametrize("pieces", [1, 2, 3, 9, 30])
+def test_the_marking_warp_never_mistakes_a_phase(pieces):
+    runs = [marker(pieces, 4, seed) for seed in range(300)]
+    assert max(a for a, _ in runs) <= 3 and not any(alias for _, alias in runs)
+    assert pieces < 9 or any(alias for _, alias in (marker(pieces, 1, seed) for seed in range(300)))
