@@ -208,8 +208,9 @@ struct Fold {
   // packet's weights against m.  Returns whether m moved.
   template <int N>
   __device__ __forceinline__ bool add(float* v, float most, int k, const Scale& sc, float* w) {
-    if (most > top) {
-      top = most;
+    const float reach = fminf(most, FLT_MAX);  // +inf is the largest float: no later maximum than one of that
+    if (reach > top) {
+      top = reach;
       top_pack = k;
     }
     const bool moved = __any_sync(0xffffffffu, most > m);
@@ -241,7 +242,7 @@ struct Fold {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
     if (sc.greedy) {
-      if (top_pack != NONE && top >= m) {  // (top may be +inf, m not)
+      if (top_pack != NONE && top >= m) {
         float v[pack_n<T>()];
         unpack<T>(load_pack<T, VEC>(x, top_pack, n), v);
 #pragma unroll

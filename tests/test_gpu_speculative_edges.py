@@ -260,3 +260,22 @@ def test_nan_values_in_many_short_prefixes(reach):
         assert bool(ref.isnan().any())
         _matches(out, ref, vmax)
         assert torch.equal(torch.nan_to_num(run(d), 7.0), torch.nan_to_num(out, 7.0))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 700])
+def test_greedy_takes_the_largest_float_before_a_later_infinity(rows):
+    """+inf is read as the largest float, so the two tie: in packets of one lane, of one warp and apart."""
+    v, top = 70001, torch.finfo(torch.float32).max
+    logits = torch.randn((rows, v), generator=torch.Generator().manual_seed(1)).to(dev())
+    first = (torch.arange(rows, device=dev()) * 7 + 5) % 1000
+    r = torch.arange(rows, device=dev())
+    zero, noise = torch.zeros(rows, device=dev()), torch.ones((rows, v), device=dev())
+    one = torch.arange(rows + 1, dtype=torch.int32, device=dev())
+    for step in (1, 4, 128, 1024, 4096, 8192, 16384, 65536):
+        x = logits.clone()
+        x[r, first] = top
+        x[r, first + step] = torch.inf
+        assert torch.equal(sample(x, zero, noise)[0], first), step
+        ids = torch.zeros(rows, dtype=torch.int64, device=dev())
+        tokens, _, _ = verify_drafts(x, ids, one, zero, zero[:, None][:, :0], noise)
+        assert torch.equal(tokens[:, 0], first), step
