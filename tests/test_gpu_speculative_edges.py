@@ -279,3 +279,38 @@ def test_greedy_takes_the_largest_float_before_a_later_infinity(rows):
         ids = torch.zeros(rows, dtype=torch.int64, device=dev())
         tokens, _, _ = verify_drafts(x, ids, one, zero, zero[:, None][:, :0], noise)
         assert torch.equal(tokens[:, 0], first), step
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t", [0.25, 0.9, 1.0, 2.0])
+def test_drafts_that_infinities_make_certain(dtype, t):
+    """A drafter that forces a token by +inf: its normaliser stays finite at every temperature, the draft's
+    probability is 1, and it is accepted as often as the target would draw it."""
+    g = torch.Generator().manual_seed(2)
+    n, v, at = 64, 1003, 7
+    target = torch.randn((2 * n, v), generator=g).to(dtype)
+    target[::2, at] = torch.linspace(-3, 9, n).to(dtype)  # from hardly ever to nearly always
+    draft = torch.randn((n, v), generator=g).to(dtype)
+    draft[:, at] = torch.inf
+    temps, u = torch.full((n,), t), torch.rand((n, 1), generator=g)
+    noise = torch.empty((n, v)).exponential_(1.0, generator=g)
+    drawn, logprobs, lse = sample(draft.to(dev()), temps.to(dev()), noise.to(dev()))
+    assert drawn.tolist() == [at] * n and not bool(logprobs.any()) and bool(torch.isfinite(lse).all())
+    ids = torch.zeros(2 * n, dtype=torch.int64)
+    ids[1::2] = at
+    sure = 0
+    for given in (lse, torch.full_like(lse, torch.inf) if t < 1 else lse):  # as a plain logsumexp has it
+        tokens, accepted, lp = verify_drafts(target.to(dev()), ids.to(dev()),
+                                             torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device=dev()),
+                                             temps.to(dev()), u.to(dev()), noise.to(dev()),
+                                             draft_logits=draft[:, None].to(dev()), draft_lse=given[:, None])
+        for i in range(n):
+            want, count, want_lp, margin = osp.verify(target[2 * i:2 * i + 2].double().numpy(), [0, at], t, u[i].tolist(),
+                                                      noise[i].numpy(), draft[i:i + 1].double().numpy(), [float(lse[i])], 1)
+            if margin < 2 ** -17:
+                continue
+            sure += 1
+            assert tokens[i].tolist() == want + [-1] * (2 - len(want)) and int(accepted[i]) == count, i
+            assert all(abs(a - b) <= 2 ** -20 * 60 + 2 ** -19 for a, b in zip(lp[i].tolist(), want_lp))
+        assert int(accepted.sum()) < n and (t > 1 or int(accepted.sum()) > 0)  # (at 2 no target is above 1 in 10)
+    assert sure > n
