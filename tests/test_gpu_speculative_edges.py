@@ -314,3 +314,41 @@ def test_drafts_that_infinities_make_certain(dtype, t):
             assert all(abs(a - b) <= 2 ** -20 * 60 + 2 ** -19 for a, b in zip(lp[i].tolist(), want_lp))
         assert int(accepted.sum()) < n and (t > 1 or int(accepted.sum()) > 0)  # (at 2 no target is above 1 in 10)
     assert sure > n
+
+
+@pytest.mark.parametrize("reach", [0, 1 << 18])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_huge_queries_take_the_key_with_the_largest_score(dtype, reach):
+    """Queries near the top of their type: the scores of a head are so far apart that its output is the value of
+    its best key.  A score is a sum of 128 products in 32 bits, off by 2^-20 of the sum of their sizes at most;
+    heads whose best two scores are closer than twice that and 64 powers of two are left out."""
+    c = osp.make_shared_prefix_case(26, [200], [3], [20, 33, 40], [20, 16, 9], 32, 8, 16, dtype)
+    top = 1e30 if dtype == torch.bfloat16 else 6e4
+    g = torch.Generator().manual_seed(4)
+    size = 2.0 ** -torch.randint(0, 4, c["q"].shape, generator=g).float()
+    c["q"] = (top * size * torch.sign(c["q"].float() + 1e-9)).to(dtype)
+    c["scale"] = 128 ** -0.5 * (1.0 if dtype == torch.bfloat16 else 64.0)
+    d = {k: v.to(dev()) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    pad = reach // 16 - d["prefix_tables"].shape[1]
+    d["prefix_tables"] = torch.nn.functional.pad(d["prefix_tables"], (0, max(pad, 0)), value=-1)
+    out = shared_prefix_decode(d["q"], d["k_cache"], d["v_cache"], d["prefix_tables"], d["prefix_lens"], d["cu_groups"],
+                               d["block_tables"], d["context_lens"], d["scale"], cu_seqlens_q=d["cu_seqlens_q"]).cpu()
+    ulp = 2 ** -8 if dtype == torch.bfloat16 else 2 ** -11
+    sure = 0
+    for b in range(3):
+        begin, end, own = int(c["cu_seqlens_q"][b]), int(c["cu_seqlens_q"][b + 1]), int(c["context_lens"][b])
+        keys = [(c["prefix_tables"][0, j // 16], j % 16) for j in range(200)]
+        keys += [(c["block_tables"][b, j // 16], j % 16) for j in range(own)]
+        k, v = (torch.stack([c[n][int(p), r].double() for p, r in keys]) for n in ("k_cache", "v_cache"))
+        for n in range(begin, end):
+            see = 200 + own - (end - begin) + (n - begin) + 1
+            q = c["q"][n].double().view(8, 4, 128)
+            s = torch.einsum("hgd,lhd->hgl", q, k[:see]) * c["scale"] / np.log(2)
+            err = 2.0 ** -20 * torch.einsum("hgd,lhd->hgl", q.abs(), k[:see].abs()).amax(-1) * c["scale"] / np.log(2)
+            best = s.topk(2, dim=-1)
+            clear = best.values[..., 0] - best.values[..., 1] > 2 * err + 64
+            want = v[best.indices[..., 0], torch.arange(8)[:, None]]
+            got = out[n].double().view(8, 4, 128)
+            assert bool(((got - want).abs() <= ulp * want.abs())[clear].all()), n
+            sure += int(clear.sum())
+    assert sure > 32 * 45 // 2
