@@ -309,8 +309,8 @@ template <typename T> __device__ __forceinline__ void share(int n, int rank, int
 }
 
 // ---- sampling: one cluster per row -------------------------------------------------------------
-// 64 rows of 151,936 bf16 logits (58 MB with the noise): 15.7 us, 3.7 TB/s = 0.57 of a measured copy, bound by
-// the instructions of a logit and the start and end of a 16 us kernel; one row 7.2 us, a chain of latencies
+// 64 rows of 151,936 bf16 logits (58 MB with the noise): 14.9 us, 3.9 TB/s = 0.60 of a measured copy, bound by
+// the instructions of a logit and the start and end of a 15 us kernel; one row 7.0 us, a chain of latencies
 // (launch, one read, the cluster's exchange).  The statistics and the race share one read of the row, which
 // is why the race filters by a score shared as raw numbers: the row's maximum is not known yet.
 struct SampleWord {
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 // (by then in L2).  In both any CTA takes any share of any row, so ragged numbers of drafts cost no
 // balance; in the second each CTA judges its sequence's drafts for itself (a few words) and the
 // shares meet in one 64-bit atomic maximum of (score, lowest index), whose order does not matter.
-// 230 rows of 151,936 bf16 logits for 64 sequences (128 MB): 38.7 us.  The statistics take 21 us, 3.3 TB/s = 0.51 of
+// 230 rows of 151,936 bf16 logits for 64 sequences (128 MB): 38.8 us.  The statistics take 21 us, 3.3 TB/s = 0.51 of
 // a measured copy, issue slots 0.66 busy (12 instructions a logit, fixed costs of a warp's share included);
 // the draw about 20, of which the judging, a chain of dependent reads, is 6 to 8 before its first load.
 struct VerifyParams {

@@ -226,7 +226,7 @@ __device__ __forceinline__ void mark_nan(const Params& P, const int32_t* table, 
 
 // ---- pieces of few rows: one warp each, warp-level MMA --------------------------------------------
 // Bound: HBM by its bytes, latency by measurement.  8 x 8 samples of prompts of 869 to 3,454 keys, 16 KV
-// heads, window 1,024 (108 MB): 37 us, 2.9 TB/s = 0.44 of a measured copy; every further tile then costs its
+// heads, window 1,024 (108 MB): 38 us, 2.8 TB/s = 0.43 of a measured copy; every further tile then costs its
 // bytes at 0.96 of that rate, but about 5 us pass before the first load (lengths, plan, page look-up: some
 // 1,500 instructions that run once, so fetching them is what takes the time) and 1 to 2 at either end of a
 // piece.  A warp takes one piece (segment, block
@@ -1631,8 +1631,8 @@ inline bool registers_ready() {
 
 // ---- merge: one warp per (row, head), four dimensions a lane --------------------------------------
 // out = v_scale * sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over the row's pieces i, M = max m_i, in the
-// order of the pieces.  Bound: the partials' bytes, latency for few rows: 256 rows x 32 heads (48 MB of partials) 20.6 us from
-// a cold L2, 2.3 TB/s; 64 rows x 32 heads 10.3 us, a chain of three loads (plan, maxima, sums).
+// order of the pieces.  Bound: the partials' bytes, latency for few rows: 256 rows x 32 heads (48 MB of partials)
+// 21.0 us from a cold L2, 2.3 TB/s; 64 rows x 32 heads 10.8 us, a chain of three loads (plan, maxima, sums).
 template <typename TO>
 __global__ void __launch_bounds__(128) merge_kernel(Params P, int piece_rows) {
   pdl_wait();
@@ -1731,9 +1731,9 @@ inline bool smem_ready(int bytes) {
   return true;
 }
 
-// Blocks of 8 rows that a warp takes together: what the rows of a sequence fill on average, up to two
-// (with 8 rows or fewer a sequence, 16 cost more than a prefix's K and V read half as often give back: 42
-// against 56 us for 8 x 8 samples of 2 rows, 23 against 31 for 16 sequences of 4).
+// Blocks of 8 rows that a warp takes together: two where the sequences have more than 8 rows on average, one
+// otherwise (then 16 cost more than a prefix's K and V read half as often give back: 42 against 56 us for
+// 8 x 8 samples of 2 rows, 23 against 31 for 16 sequences of 4).
 inline int row_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 // pieces_kernel keeps the segments in shared memory behind its rings; its limit is set once, for the most
@@ -1747,7 +1747,9 @@ constexpr int PIECES_PER_SM = 3 * WARPS;
 
 // prefix_kernel takes the prefixes from 33 rows a prefix and KV head on (with fewer, its 128-row tiles stay
 // emptier than the pieces' blocks of 8), where (rows) x (keys that the prefix tables reach) x (KV heads)
-// is at least 3 * 2^19, where its start-up and partials (about 15 us) are made up for.  By pieces and with it,
+// is at least 3 * 2^19, where its start-up and partials (about 15 us) are made up for.  The host knows the
+// tables' width, not the lengths: behind tables padded to a long reach (and under a window, which is not
+// counted either) a short prefix takes it too, and pays those 15 us.  By pieces and with it, tables cut to the prefix,
 // in us: 64 rows x 8 heads behind 2,048 keys 22.6, 21.8, behind 8,192 38.1, 32.7; 192 rows behind 1,024 32.0,
 // 24.1; 256 rows behind 512 27.3, 31.2.
 constexpr int64_t TC_ROWS = 33, TC_WORK = 3 << 19;

@@ -578,7 +578,9 @@ ADA_API int ada_argmax_noalloc(const void* logits, int64_t ld, int64_t rows, int
  * at row 0 of its first page, its new tokens included (store them first).  Rows cu_seqlens_q[b]
  * .. cu_seqlens_q[b+1] - 1 of q are its t_b newest tokens: query i stands at position
  * pos = prefix_len + context_len - t_b + i of the joined keys and sees keys j <= pos, with
- * window W > 0 only the last W of them (the meaning of the decode entry's window).
+ * window W > 0 only the last W of them (the meaning of the decode entry's window); any W from the
+ * positions that the tables reach on is no window.  A NaN key or value reaches the rows that see it,
+ * and no others.
  *
  * q, out   [total_q, num_heads, head_dim], token and head strides given, unit stride in D
  * k_cache, v_cache, num_pages, page_size, k_scale, v_scale: as the decode entry; table entries
@@ -589,10 +591,13 @@ ADA_API int ada_argmax_noalloc(const void* logits, int64_t ld, int64_t rows, int
  *          no group (num_groups 0, or outside [cu_groups[0], cu_groups[num_groups])) has no prefix
  * cu_seqlens_q int32 [batch + 1] ascending; NULL: one row per sequence (total_q == batch).  Rows
  *          of no sequence, and rows that see no key, are written as zeros
- * err      optional uint32 word: 0x90 is OR-ed in if a tile wait ran out (~2 s)
+ * err      optional uint32 word: 0x90 is OR-ed in if a tile wait ran out (~2 s); the rows concerned are NaN
  * Implemented: head_dim 128, num_heads / num_kv_heads <= 128, page_size % 16 == 0,
- * num_groups + batch <= 4096, scale * k_scale > 0.  workspace: ada_fp8_shared_prefix_decode_workspace_size bytes, 256-byte
- * aligned, no initial value; calls that share one must be ordered.
+ * num_groups + batch <= 4096, scale * k_scale > 0.  Lists that do not ascend give unspecified rows, but
+ * nothing outside the tensors is read or written.  workspace: ada_fp8_shared_prefix_decode_workspace_size
+ * bytes (28 MiB for 16 sequences of 32 / 8 heads, 0.6 GiB for 4,000), 256-byte aligned, no initial value.
+ * The call makes two or three launches that talk through it: calls that share one, also from several host
+ * threads, must be ordered as a whole.
  * ---------------------------------------------------------------------- */
 ADA_API size_t ada_fp8_shared_prefix_decode_workspace_size(int32_t total_q, int32_t num_groups, int32_t batch,
                                                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
@@ -614,8 +619,9 @@ ADA_API int ada_fp8_shared_prefix_decode(
  * z = logits / T;  lse[r] = ln sum exp(z);  tokens[r] = the lowest index of the largest
  * exp(z - lse) / noise;  logprobs[r] = z[token] - lse.  T <= 1e-10: greedy, tokens[r] = the first
  * maximum, lse and logprobs at temperature 1.  -inf and NaN logits have probability 0, +inf is
- * read as the largest float; a row with no possible token gives token -1, logprob 0, lse -inf.
- * logprobs, lse: either may be NULL.  One launch, no workspace.
+ * read as the largest float, where z stops as well; a row with no possible token gives token -1,
+ * logprob 0, lse -inf.  logprobs, lse: either may be NULL.  One launch, no workspace.  Implemented:
+ * rows <= 2^20, vocab <= 2^30.
  * ---------------------------------------------------------------------- */
 ADA_API int ada_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab,
                        const float* temperatures, const float* noise, int64_t ld_noise, int64_t* tokens,
@@ -637,8 +643,10 @@ ADA_API int ada_sample(const void* logits, int dtype, int64_t ld, int64_t rows, 
  * maximum.  tokens int64 and logprobs fp32 [batch, max_drafts + 1]: the accepted drafts and the
  * drawn token with their log-probabilities under p, then -1 and 0; accepted int32 [batch].
  * Logits are read as in ada_sample; where no token is possible the drawn one is -1.
- * workspace: ada_verify_drafts_workspace_size bytes, 16-byte aligned, no initial value; calls that
- * share one must be ordered.  Two launches.
+ * Implemented: batch <= 2^20, vocab <= 2^30, max_drafts <= 1024.  A cu_seqlens_q that does not ascend
+ * gives unspecified tokens (of the vocabulary, or -1).  workspace: ada_verify_drafts_workspace_size bytes,
+ * 16-byte aligned, no initial value.  Two launches that talk through it: calls that share one, also from
+ * several host threads, must be ordered as a whole.
  * ---------------------------------------------------------------------- */
 ADA_API size_t ada_verify_drafts_workspace_size(int32_t total_q, int32_t batch, int64_t vocab, int dtype);
 ADA_API int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t total_q, int64_t vocab,
