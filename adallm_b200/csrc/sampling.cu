@@ -293,10 +293,12 @@ __device__ __forceinline__ float2 unpack2(unsigned long long v) {
 }
 __device__ __forceinline__ float exponential(float e) { return fmaxf(e, 1e-10f); }
 
-// Probability of a draft's logit given its row's log-normaliser (NaN: 0, +inf: the largest float).  Below
-// temperature 1 the largest floats' quotient, and with it the normaliser, stops at the largest float.
+// Probability of a draft's logit given its row's log-normaliser (-inf and NaN: 0, +inf: the largest float).
+// Below temperature 1 the largest floats' quotients, of either sign, and with them the normaliser, stop at the
+// largest float.
+__device__ __forceinline__ float divided(float x, float t) { return fminf(fmaxf(x / t, -FLT_MAX), FLT_MAX); }
 __device__ __forceinline__ float draft_prob(float x, const Scale& sc, float lse) {
-  return x == x ? expf(fminf(x / sc.t, FLT_MAX) - (lse > FLT_MAX ? FLT_MAX : lse)) : 0.f;
+  return x >= -FLT_MAX ? expf(divided(x, sc.t) - (lse > FLT_MAX ? FLT_MAX : lse)) : 0.f;
 }
 
 // This CTA's packets [k0, k1) of a row of n elements, in shares of whole warps.
@@ -429,7 +431,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   const float ln_s = logf(w.s);
   tokens[r] = any && at != NONE ? at : -1;
   if (logprobs) logprobs[r] = any ? sc.diff(sc.greedy ? w.m : w.x, w.m) / sc.t - ln_s : 0.f;
-  if (lse) lse[r] = any ? fminf(w.m / sc.t, FLT_MAX) + ln_s : -INFINITY;
+  if (lse) lse[r] = any ? divided(w.m, sc.t) + ln_s : -INFINITY;
 }
 
 // ---- verification ---------------------------------------------------------------------------------

@@ -619,8 +619,8 @@ ADA_API int ada_fp8_shared_prefix_decode(
  * z = logits / T;  lse[r] = ln sum exp(z);  tokens[r] = the lowest index of the largest
  * exp(z - lse) / noise;  logprobs[r] = z[token] - lse.  T <= 1e-10: greedy, tokens[r] = the first
  * maximum, lse and logprobs at temperature 1.  -inf and NaN logits have probability 0, +inf is
- * read as the largest float, where z stops as well; a row with no possible token gives token -1,
- * logprob 0, lse -inf.  logprobs, lse: either may be NULL.  One launch, no workspace.  Implemented:
+ * read as the largest float; lse stops at the largest floats, and only a row with no possible token
+ * gives -inf (with token -1, logprob 0).  logprobs, lse: either may be NULL.  One launch, no workspace.  Implemented:
  * rows <= 2^20, vocab <= 2^30.
  * ---------------------------------------------------------------------- */
 ADA_API int ada_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab,

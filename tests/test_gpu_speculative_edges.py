@@ -4,6 +4,7 @@ calls of different size in turn, and inputs at the ends of their ranges.
 Tolerances are those of the operators' own tests (tests/test_gpu_shared_prefix.py,
 tests/test_gpu_sampling.py); where two runs of one call are compared they have to be equal."""
 import functools
+import math
 import threading
 
 import numpy as np
@@ -352,3 +353,32 @@ def test_huge_queries_take_the_key_with_the_largest_score(dtype, reach):
             assert bool(((got - want).abs() <= ulp * want.abs())[clear].all()), n
             sure += int(clear.sum())
     assert sure > 32 * 45 // 2
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("t", [1e-4, 0.3, 1.0, 3.0])
+def test_rows_masked_by_the_lowest_value_alone(dtype, t):
+    """Every logit the type's lowest: all tokens alike, so the noise decides, log-probability -ln n; the
+    normaliser is not the -inf of a row without a possible token, and a draft drawn from such a row never makes
+    the verified tokens anything but the target's (here certain ones)."""
+    n, v = 5, 300
+    g = torch.Generator().manual_seed(6)
+    low = torch.full((n, v), torch.finfo(dtype).min, dtype=dtype)
+    low[3, 10:] = -torch.inf
+    low[4] = -torch.inf
+    temps, noise = torch.full((n,), t, device=dev()), torch.empty((n, v)).exponential_(1.0, generator=g)
+    tokens, logprobs, lse = (x.cpu() for x in sample(low.to(dev()), temps, noise.to(dev())))
+    want = [int(noise[r].argmin()) for r in range(3)] + [int(noise[3, :10].argmin()), -1]
+    assert tokens.tolist() == want
+    off = logprobs - torch.tensor([-math.log(v)] * 3 + [-math.log(10), 0.0])
+    assert float(off.abs().max()) <= 2 ** -20 * math.log(v) + 2 ** -19
+    assert bool(torch.isfinite(lse[:4]).all()) and float(lse[4]) == -math.inf
+    target = torch.zeros((2 * n, v), dtype=dtype)
+    target[torch.arange(2 * n), torch.arange(2 * n)] = 20000.0
+    ids = torch.stack((torch.zeros(n, dtype=torch.long), tokens), 1).reshape(-1)
+    got, accepted, _ = verify_drafts(target.to(dev()), ids.to(dev()),
+                                     torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device=dev()), temps,
+                                     torch.rand((n, 1), generator=g).to(dev()), noise.to(dev()),
+                                     draft_logits=low[:, None].to(dev()), draft_lse=lse[:, None].to(dev()))
+    for r in range(n):
+        assert got[r].tolist() == ([2 * r, 2 * r + 1] if int(accepted[r]) else [2 * r, -1])
