@@ -208,9 +208,18 @@ __device__ __forceinline__ void mark_nan(const Params& P, const int32_t* table, 
     const bool there = blk >= 0 && blk < P.num_pages;
     const uint32_t* x = reinterpret_cast<const uint32_t*>(
         P.v + (there ? blk * P.v_page + row * P.v_tok + kvh * P.v_head : 0));
+    uint32_t any = 0;  // a first look, all of the key's loads in flight together: most keys have none
+    if (there) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint4 e = reinterpret_cast<const uint4*>(x)[i];
+        any |= nan_bytes(e.x) | nan_bytes(e.y) | nan_bytes(e.z) | nan_bytes(e.w);
+      }
+    }
+    if (!__any_sync(0xffffffffu, any)) continue;
 #pragma unroll 1
     for (int w = 0; w < D / 4; ++w) {
-      const uint32_t bad = there ? nan_bytes(x[w]) : 0u;
+      const uint32_t bad = any ? nan_bytes(x[w]) : 0u;
 #pragma unroll 1
       for (uint32_t who = __ballot_sync(0xffffffffu, bad != 0); who; who &= who - 1) {
         const int key = k0 + __ffs(who) - 1;
@@ -811,11 +820,11 @@ __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
 //   O_t += P_t . V  kind::f16; V is widened to fp16 (exact) by four warps, once for both tiles.
 // Roles (16 warps): 0-3 widen V; 4-7 and 8-11 take tile 0's and tile 1's rows (thread = row: queries to
 // terms, softmax, O to the workspace); 12 loads (TMA, eight 16-key tiles a block for K and V each);
-// 13 issues the MMAs; 14 walks the CTA's range and hands out its pieces; 15 marks NaN values.  The row warps take 192
-// registers a thread (a row of S at once), the others 64.  P.V of a block and S of the next are issued
-// together for a tile, so one tile's MMAs run under the other tile's softmax.  All tcgen05 operations come
-// from one thread in order, so s_full of block j + 1 also says that P.V of block j is complete: O may be
-// rescaled.
+// 13 issues the MMAs; 14 walks the CTA's range and hands out its pieces; 15 marks NaN values.  The row
+// warps take 192 registers a thread (a row of S at once), the others 64.  P.V of a block and S of the next
+// are issued together for a tile, so one tile's MMAs run under the other tile's softmax.  All tcgen05
+// operations come from one thread in order, so s_full of block j + 1 also says that P.V of block j is
+// complete: O may be rescaled.
 // Barriers, phase = use: d_full/d_empty (pieces), k_full/k_empty (K slots), e_full/e_empty (e4m3 V
 // slots), v_full/v_empty (fp16 V slots), s_full[t], p_full[t][half] (a block's S, P of tile t), q_full[t],
 // o_full[t] (a piece's Q, O), stored (a cut piece's partial; the rows are at most two pieces ahead of the
@@ -1749,8 +1758,8 @@ constexpr int PIECES_PER_SM = 3 * WARPS;
 // emptier than the pieces' blocks of 8), where (rows) x (keys that the prefix tables reach) x (KV heads)
 // is at least 3 * 2^19, where its start-up and partials (about 15 us) are made up for.  The host knows the
 // tables' width, not the lengths: behind tables padded to a long reach (and under a window, which is not
-// counted either) a short prefix takes it too, and pays those 15 us.  By pieces and with it, tables cut to the prefix,
-// in us: 64 rows x 8 heads behind 2,048 keys 22.6, 21.8, behind 8,192 38.1, 32.7; 192 rows behind 1,024 32.0,
+// counted either) a short prefix takes it too, and pays those 15 us.  By pieces and with it, tables cut to
+// the prefix, in us: 64 rows x 8 heads behind 2,048 keys 22.6, 21.8, behind 8,192 38.1, 32.7; 192 rows behind 1,024 32.0,
 // 24.1; 256 rows behind 512 27.3, 31.2.
 constexpr int64_t TC_ROWS = 33, TC_WORK = 3 << 19;
 
