@@ -79,6 +79,16 @@ _SIGS = {
     "ada_verify_drafts_workspace_size": (SZ, [I32, I32, I64, INT]),
     "ada_verify_drafts": (INT, [P, INT, I64, I32, I64, P, P, I32, I32, P, P, I64, P, I64, P, I64, I64, P, I64, I64, P,
                                 P, P, P, SZ, P]),
+    "ada_step_metadata": (INT, [P, P, I32, P, I64, I32, P, I64, P, I32, I64, P, P, P, P, P, P, P, P]),
+    "ada_rotary": (INT, [P, P, I64, I64, P, I64, I64, P, P, I64, I32, I32, I32, P, I64, I32, I32, INT, P]),
+    "ada_kv4_store": (INT, [P, P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I32, I32, I32, P, I64, I32, I32, P, P, P,
+                            I64, I64, I64, I32, F32, F32, INT, P]),
+    "ada_kv4_read": (INT, [P, P, I64, I64, I64, I32, I32, I32, P, I64, F32, F32, P, P, INT, P]),
+    "ada_kv4_paged_decode_workspace_size": (SZ, [I32, I32, I32]),
+    "ada_kv4_paged_decode": (INT, [P, INT, I64, I64, P, P, I64, I64, I64, P, I64, I32, P, I32, I32, I32, I32, I32, F32,
+                                   F32, F32, I32, P, INT, I64, I64, P, SZ, P]),
+    "ada_kv4_paged_prefill": (INT, [P, INT, I64, I64, P, P, I64, I64, I64, P, I64, I32, P, P, I32, I64, I32, I32, I32,
+                                    I32, I32, F32, F32, F32, I32, P, INT, I64, I64, P, P]),
     "ada_nvfp4_sf_bytes": (SZ, [I64, I64]),
     "ada_nvfp4_prepack_scales": (INT, [P, INT, I64, I64, I64, P, P]),
     "ada_nvfp4_linear_workspace_size": (SZ, [I64, I64, I64, INT]),
@@ -179,11 +189,16 @@ _ERROR_CODES = {0x50: "a peer's partial planes never arrived (tensor-parallel in
                 0x70: "a prefill attention tile load never completed",
                 0x80: "a router logit never arrived (fused MoE router wait)",
                 0x90: "a shared-prefix attention tile never completed"}
+# Bits of a step's metadata (several may be set).
+_STEP_BITS = [(0x100, "the free list of pages ran out"),
+              (0x200, "a block table is too narrow for its tokens"),
+              (0x400, "a step has more tokens than it is laid out for, or a slot passes 32 bits")]
 
 
 def describe_error_word(code: int) -> str:
     parts = [txt for bit, txt in _ERROR_BITS if code & bit]
-    hi = code & ~0xF
+    parts += [txt for bit, txt in _STEP_BITS if code & bit]
+    hi = code & ~0x70F
     if hi:
         parts.append(_ERROR_CODES.get(hi, f"code 0x{hi:x}"))
     return "; ".join(parts) or "ok"
@@ -200,6 +215,27 @@ def stream_ptr(device: torch.device | None = None) -> int:
     """The current stream's handle (the raw look-up: building a Stream object costs 2 us a call)."""
     index = device.index if device is not None else None
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def call(entry, device: torch.device, *args) -> int:
+    """entry(*args) with `device` current: a launch goes to the current device, its stream must be of it."""
+    if device.index == torch._C._cuda_getDevice():
+        return entry(*args)
+    with torch.cuda.device(device):
+        return entry(*args)
+
+
+def one_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    """The device that all tensors are on."""
+    device = first.device
+    if device.type != "cuda":
+        raise RuntimeError(f"{what} requires CUDA tensors")
+    for t in others:
+        if t is not None and t.device != device:
+            if not t.is_cuda:
+                raise RuntimeError(f"{what} requires CUDA tensors")
+            raise ValueError(f"{what}: all tensors must be on one device")
+    return device
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

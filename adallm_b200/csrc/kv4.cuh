@@ -1,0 +1,88 @@
+// The 4-bit paged KV cache: layout and conversions shared by its kernels.
+//
+// One block per (page, KV head), `page` rows of 128 elements (page a multiple of 16):
+//   bytes [0, 64 * page)           the rows' e2m1 codes, 64 bytes a row, even element in the low nibble
+//   bytes [64 * page, 72 * page)   the rows' e4m3 scales, 8 bytes a row, one for 16 elements
+// value = code * scale * (the tensor's scale).  A block is contiguous, so a tile of 16 rows is two
+// contiguous pieces (1,024 and 128 bytes) and a page of one head stays together in DRAM, where a
+// row of 72 bytes among other heads' would leave no 16-byte alignment to load with.
+// code * scale has at most 6 significant bits and lies in [2^-10, 2688]: exact in fp16 and in bf16.
+#pragma once
+
+#include "common.cuh"
+
+namespace ada {
+namespace kv4 {
+
+constexpr int D = 128;
+constexpr int BLOCK = 16;           // elements a scale
+constexpr int ROW = D / 2;          // bytes of codes a row
+constexpr int SROW = D / BLOCK;     // bytes of scales a row
+constexpr int ROW_BYTES = ROW + SROW;
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Largest scale's worth of elements; what lies beyond saturates (infinities too).
+constexpr float LIMIT = 2.f * 6.f * 448.f;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// e4m3 byte of max|x| / 6, saturated to 448; NaN when the block holds one (the block then reads as NaN).
+__device__ __forceinline__ uint32_t scale_code(float top) {
+  return f32x2_to_e4m3x2(__fdiv_rn(top, 6.f), 0.f) & 0xFFu;
+}
+__device__ __forceinline__ float scale_value(uint32_t code) {
+  const uint32_t h = e4m3x2_to_f16x2((uint16_t)code);
+  return __half2float(__ushort_as_half((unsigned short)(h & 0xFFFFu)));
+}
+
+// Eight elements -> eight codes: the nearest e2m1 to x / s, ties to even.  r = RN(1 / s); one
+// correction step makes q the correctly rounded fp32 quotient (s has 4 significant bits, x at most
+// 24, so a quotient that is not a midpoint of fp32 lies 2^-27 or more away from one, and the
+// step's own error is below 2^-45).  x * r alone puts exact ties, which bf16 values often are, on
+// either side.  A block whose scale is 0 (all below 2^-10 * 6) holds zeros.
+__device__ __forceinline__ uint32_t codes8(const float* x, float s) {
+  if (!(s > 0.f)) return 0u;
+  const float r = __frcp_rn(s);
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = fminf(fmaxf(x[i], -LIMIT), LIMIT);
+    const float q0 = v * r;
+    q[i] = fmaf(fmaf(-q0, s, v), r, q0);
+  }
+  return f32x8_to_e2m1x8(q);
+}
+
+// A query row enters the products multiplied by a power of two that brings its largest magnitude
+// `top` into [2^14, 2^15), so that bf16 rows of any size keep their bits in fp16 (what falls under fp16's
+// range is 2^-38 of the largest); the exponent is taken back in the factor of the scores, which stops
+// at 2^90: |score| < 2^34 then keeps every product finite, and a row of such a factor is decided by its
+// largest score alone.  A row of zeros, or with an infinity or NaN, is left as it is.
+__device__ __forceinline__ int query_exponent(float top) {
+  if (!(top > 0.f) || !(top < INFINITY)) return 0;
+  const int e = (int)(__float_as_uint(top) >> 23) - 127;  // (-127 for a subnormal)
+  return 14 - max(e, -100);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -127 < e < 128
+__device__ __forceinline__ float score_factor(float scale_log2, int exponent) {
+  return fminf(scale_log2 * pow2(-exponent), 1.2379400392853803e27f);
+}
+
+inline bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+// Checks of a cache's layout that every entry shares.
+inline int cache_ok(const void* kc, const void* vc, int64_t s_page, int64_t s_head, int64_t num_pages, int32_t heads,
+                    int32_t page) {
+  if (!kc || !vc || num_pages <= 0 || heads <= 0 || page <= 0) return ADA_ERR_INVALID_ARG;
+  if (page % 16) return ADA_ERR_UNSUPPORTED;
+  if (s_head < (int64_t)page * ROW_BYTES || s_page < (int64_t)page * ROW_BYTES) return ADA_ERR_INVALID_ARG;
+  if (misaligned16(kc) || misaligned16(vc) || (s_page & 15) || (s_head & 15)) return ADA_ERR_ALIGNMENT;
+  return ADA_OK;
+}
+
+}  // namespace kv4
+}  // namespace ada

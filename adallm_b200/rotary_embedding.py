@@ -4,9 +4,13 @@ Same constructor, cache and forward contract as the reference
 (adallm/ops/rotary_embedding.py:17-90): an fp32 cos/sin cache
 [max_position, 1, head_size] = [cos | sin] with optional linear scaling,
 NeoX rotate-half applied in fp32 and cast back, new q / k returned.
+
+``apply_rotary`` (``ada_rotary``) takes what the reference does not: interleaved pairs, a rotated part
+of the head narrower than the head, strided heads.  ``build_cos_sin_cache`` also makes YaRN's table.
 """
 from __future__ import annotations
 
+import math
 from functools import lru_cache
 
 import torch
@@ -15,9 +19,34 @@ from torch import nn
 from . import _native as N
 
 
+def _yarn_cos_sin_cache(rotary_dim: int, max_position: int, base: float, rope_scaling: dict, device=None):
+    """YaRN (Peng et al. 2023): pairs that turn more than beta_fast times over the trained length keep their
+    frequency, those below beta_slow turns are slowed by `factor`, a linear ramp lies between; cos and sin are
+    multiplied by the attention factor 0.1 ln(factor) + 1.  Angles in 64 bits, the table in fp32."""
+    factor = float(rope_scaling["factor"])
+    trained = float(rope_scaling.get("original_max_position_embeddings") or max_position / factor)
+    fast, slow = float(rope_scaling.get("beta_fast", 32.0)), float(rope_scaling.get("beta_slow", 1.0))
+    amplitude = rope_scaling.get("attention_factor")
+    amplitude = float(amplitude) if amplitude is not None else 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    half = rotary_dim // 2
+
+    def pair(turns):
+        return half * math.log(trained / (turns * 2 * math.pi)) / math.log(base)
+
+    low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rotary_dim - 1)
+    i = torch.arange(half, dtype=torch.float64, device=device)
+    keep = 1.0 - ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+    inv_freq = base ** (-i / half)
+    inv_freq = inv_freq * keep + inv_freq / factor * (1.0 - keep)
+    angle = torch.arange(max_position, dtype=torch.float64, device=device)[:, None] * inv_freq
+    return (torch.cat((angle.cos(), angle.sin()), -1) * amplitude).float().unsqueeze_(1)
+
+
 def build_cos_sin_cache(head_size: int, max_position: int, base: float, rope_scaling: dict | None = None,
                         device=None) -> torch.Tensor:
     """fp32 [max_position, 1, head_size]; same arithmetic as rotary_embedding.py:26-43."""
+    if rope_scaling is not None and rope_scaling.get("rope_type", rope_scaling.get("type")) == "yarn":
+        return _yarn_cos_sin_cache(head_size, max_position, base, rope_scaling, device)
     inv_freq = 1.0 / (base ** (torch.arange(0, head_size, 2, dtype=torch.float) / head_size))
     t = torch.arange(max_position, dtype=torch.float)
     if rope_scaling is not None:
@@ -53,19 +82,67 @@ def apply_rope(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, 
     return qo.view(query.shape), ko.view(key.shape)
 
 
+def apply_rotary(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, cos_sin_cache: torch.Tensor,
+                 interleaved: bool = False, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Rotate the first r = cos_sin_cache.shape[-1] elements of each head; the others are copied.
+
+    positions [T] (clamped to the table); query [T, Hq, D], key [T, Hkv, D] bf16/fp16, any strides over tokens and
+    heads that are multiples of 8; cos_sin_cache fp32 [max_position, (1,) r] = [cos | sin] of r / 2 pairs.  Pairs are
+    (i, i + r / 2), or (2i, 2i + 1) with interleaved.  Returns new contiguous tensors (q_out, k_out if given)."""
+    device = N.one_device("rotary_embedding", query, positions, key, cos_sin_cache, q_out, k_out)
+    code = N.DT.get(query.dtype)
+    if code is None or key.dtype is not query.dtype:
+        raise ValueError("rotary embedding expects bf16/fp16 q and k")
+    if query.dim() != 3 or key.dim() != 3:
+        raise ValueError("query and key must be [tokens, heads, head size]")
+    if query.stride(2) != 1:
+        query = query.contiguous()
+    if key.stride(2) != 1:
+        key = key.contiguous()
+    (t, hq, d), (tk, hk, dk) = query.shape, key.shape
+    if tk != t or positions.numel() != t or dk != d:
+        raise ValueError("positions, query and key must describe the same tokens")
+    if cos_sin_cache.dtype is not torch.float32 or not cos_sin_cache.is_contiguous():
+        raise ValueError("cos_sin_cache must be contiguous fp32")
+    if positions.dtype is not torch.int64 or not positions.is_contiguous():
+        positions = positions.to(torch.int64).contiguous()
+    if q_out is None:
+        q_out = query.new_empty((t, hq, d))
+    if k_out is None:
+        k_out = key.new_empty((t, hk, d))
+    for o, x in ((q_out, query), (k_out, key)):
+        if o.shape != x.shape or o.dtype is not x.dtype or not o.is_contiguous():
+            raise ValueError("q_out and k_out must be contiguous with their input's shape and type")
+    qs, ks = query.stride(), key.stride()
+    st = N.call(N.lib().ada_rotary, device, positions.data_ptr(), query.data_ptr(), qs[0], qs[1], key.data_ptr(), ks[0],
+                ks[1], q_out.data_ptr(), k_out.data_ptr(), t, hq, hk, d, cos_sin_cache.data_ptr(),
+                cos_sin_cache.shape[0], cos_sin_cache.shape[-1], interleaved, code, N.stream_ptr(device))
+    if st:
+        N.check(st, "rotary_embedding")
+    return q_out, k_out
+
+
 class RotaryEmbedding(nn.Module):
-    """Drop-in for adallm.ops.rotary_embedding.RotaryEmbedding."""
+    """Drop-in for adallm.ops.rotary_embedding.RotaryEmbedding; rotary_dim below head_size rotates a part of the
+    head, interleaved pairs neighbours."""
 
     def __init__(self, head_size: int, rotary_dim: int, max_position_embeddings: int, base: float,
-                 rope_scaling: dict | None = None) -> None:
+                 rope_scaling: dict | None = None, interleaved: bool = False) -> None:
         super().__init__()
         self.head_size = head_size
-        assert rotary_dim == head_size
-        self.register_buffer("cos_sin_cache", build_cos_sin_cache(head_size, max_position_embeddings, base,
+        self.rotary_dim = rotary_dim
+        self.interleaved = interleaved
+        assert rotary_dim <= head_size
+        self.register_buffer("cos_sin_cache", build_cos_sin_cache(rotary_dim, max_position_embeddings, base,
                                                                   rope_scaling), persistent=False)
 
     def forward(self, positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor):
-        return apply_rope(positions, query, key, self.cos_sin_cache)
+        if self.rotary_dim == self.head_size and not self.interleaved:
+            return apply_rope(positions, query, key, self.cos_sin_cache)
+        t, d = positions.numel(), self.head_size
+        q, k = apply_rotary(positions, query.reshape(t, -1, d), key.reshape(t, -1, d), self.cos_sin_cache,
+                            self.interleaved)
+        return q.view(query.shape), k.view(key.shape)
 
 
 @lru_cache(1)

@@ -657,6 +657,105 @@ ADA_API int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t
                               int64_t lse_stride_d, int64_t* tokens, int32_t* accepted, float* logprobs,
                               void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * A serving step's metadata from its requests' lengths, on the device
+ * Replaces the host loops of prepare_prefill / prepare_decode (adallm/runtime/model_runner.py:234-300)
+ * and the block manager's hand-out of pages to running requests.
+ * cached_lens, new_lens int32 [requests]: tokens in a request's pages, and its new ones (negative: 0).
+ * block_tables int32 [requests, >= max_pages] (row stride bt_stride): the pages of the cached tokens;
+ *   the pages that the new ones need are written behind them, taken off free_pages int32 [num_free] from
+ *   *free_start on, in request order.  *free_next: where the next step starts.
+ * num_tokens: tokens the outputs are laid out for, at least the sum of new_lens (more: padding, as a
+ *   captured step has).  positions int64, slot_mapping int32 [num_tokens]: of the new tokens, request
+ *   after request (slot = page * page_size + row); padding has position 0 and slot -1.
+ * cu_seqlens_q, cu_seqlens_k int32 [requests + 1]: prefix sums of the new tokens and of all tokens;
+ * context_lens int32 [requests]: cached + new.
+ * A token without a page (free list at its end, table too narrow, -1 in the table) gets slot -1.
+ * *err (may be NULL): 0x100 is OR-ed in if the free list ran out, 0x200 if a table was too narrow, 0x400
+ * if there are more tokens than num_tokens (those behind it are not listed) or a slot passes 32 bits.
+ * The same inputs give the same outputs, also after a run (only new pages are written); the outputs must
+ * not be the inputs (copy *free_next to *free_start, context_lens to cached_lens, behind the call).
+ * Implemented: requests <= 8192.  One launch, no workspace.
+ * ---------------------------------------------------------------------- */
+ADA_API int ada_step_metadata(const int32_t* cached_lens, const int32_t* new_lens, int32_t requests,
+                              int32_t* block_tables, int64_t bt_stride, int32_t max_pages,
+                              const int32_t* free_pages, int64_t num_free, const int32_t* free_start,
+                              int32_t page_size, int64_t num_tokens, int64_t* positions, int32_t* slot_mapping,
+                              int32_t* cu_seqlens_q, int32_t* cu_seqlens_k, int32_t* context_lens,
+                              int32_t* free_next, unsigned int* err, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions: half or interleaved pairs, a part of the head
+ * Widens RotaryEmbedding.forward (adallm/ops/rotary_embedding.py:45-56; ada_rope is its form).
+ * The first rotary_dim of head_dim elements are turned, the others copied.  Pairs are
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0; fp32, rounded once to the type.
+ * positions int64 [T], clamped to [0, max_position); cos_sin fp32 [max_position, rotary_dim] =
+ * [cos | sin] of the rotary_dim / 2 pairs (scaling for long contexts is in the table).
+ * q, k: element (t, h, d) at t * stride_t + h * stride_h + d; q_out [T, num_q_heads, head_dim], k_out
+ * [T, num_kv_heads, head_dim] contiguous, not over the inputs.
+ * Implemented: head_dim % 16 == 0 up to 1024, rotary_dim % 16 == 0, rows 16-byte aligned.
+ * ---------------------------------------------------------------------- */
+ADA_API int ada_rotary(const int64_t* positions, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                       int64_t k_stride_t, int64_t k_stride_h, void* q_out, void* k_out, int64_t num_tokens,
+                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const float* cos_sin,
+                       int64_t max_position, int32_t rotary_dim, int32_t interleaved, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * KV cache in 4 bits (no reference counterpart; beside the e4m3 cache's entries above)
+ * k_cache, v_cache: one block of page_size * 72 bytes per (page, KV head) at page * kv_stride_page + head *
+ * kv_stride_head (bytes, multiples of 16): page_size rows of 64 bytes of e2m1 codes (even element in
+ * the low nibble), then page_size rows of 8 e4m3 scales, one for 16 elements.
+ * value = code * scale * k_scale (v_scale).  head_dim 128, page_size % 16 == 0.
+ *
+ * ada_kv4_store packs the rows of k and v (strides as in ada_rotary) at slot_mapping int32 [T] (slot = page *
+ * page_size + row; slots outside the cache, -1 among them, are skipped; a slot given twice holds a mix
+ * of both rows).  Of x = element / k_scale in fp32: scale = e4m3(min(max |x| / 6, 448)) of a block of 16, code =
+ * the nearest e2m1 to x / scale, ties to even, saturating (infinities too); a block with a NaN reads as
+ * NaN.  With positions, q and k are rotated first as by ada_rotary (k rounded to the type before it
+ * is packed) and q is written to q_out; without (NULL), rows are stored as they are, and q may be NULL
+ * with num_q_heads 0.
+ * ada_kv4_read writes the values at slot_mapping as k, v [T, num_kv_heads, 128] (contiguous, bf16 or f16);
+ * zeros for slots outside the cache.
+ * ---------------------------------------------------------------------- */
+ADA_API int ada_kv4_store(const int64_t* positions, const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                          const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                          int64_t v_stride_h, void* q_out, int64_t num_tokens, int32_t num_q_heads,
+                          int32_t num_kv_heads, int32_t head_dim, const float* cos_sin, int64_t max_position,
+                          int32_t rotary_dim, int32_t interleaved, const int32_t* slot_mapping, uint8_t* k_cache,
+                          uint8_t* v_cache, int64_t kv_stride_page, int64_t kv_stride_head, int64_t num_pages,
+                          int32_t page_size, float k_scale, float v_scale, int dtype, void* stream);
+ADA_API int ada_kv4_read(const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
+                         int64_t kv_stride_head, int64_t num_pages, int32_t page_size, int32_t num_kv_heads,
+                         int32_t head_dim, const int32_t* slot_mapping, int64_t num_tokens, float k_scale,
+                         float v_scale, void* k, void* v, int dtype, void* stream);
+
+/* Decode attention over the 4-bit cache: arguments and masks as ada_fp8_paged_decode (window W > 0: the last W
+ * tokens; a zero-length sequence and one that sees no key give zeros), any number of heads a KV
+ * head.  Keys, values and probabilities enter the products in fp16, bf16 queries exactly (scaled by a power of two).
+ * workspace: ada_kv4_paged_decode_workspace_size bytes, 16-byte aligned, no initial value; calls that
+ * share one must be ordered as a whole. */
+ADA_API size_t ada_kv4_paged_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t num_kv_heads);
+ADA_API int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h,
+                                 const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
+                                 int64_t kv_stride_head, int64_t num_pages, const int32_t* block_tables,
+                                 int64_t bt_stride, int32_t max_pages, const int32_t* context_lens, int32_t batch,
+                                 int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                 float scale, float k_scale, float v_scale, int32_t window, void* out, int out_dtype,
+                                 int64_t out_stride_b, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* Causal prefill attention over the 4-bit cache: arguments and masks as ada_fp8_paged_prefill (window W > 0:
+ * the row's own position and the W before it); rows of q and out outside [0, total_q) and rows
+ * behind the last sequence are not touched.  *err (may be NULL): 0x70 if a tile wait ran out. */
+ADA_API int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h,
+                                  const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
+                                  int64_t kv_stride_head, int64_t num_pages, const int32_t* block_tables,
+                                  int64_t bt_stride, int32_t max_pages, const int32_t* cu_seqlens_q,
+                                  const int32_t* cu_seqlens_k, int32_t batch, int64_t total_q, int32_t max_seqlen_q,
+                                  int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                  float scale, float k_scale, float v_scale, int32_t window, void* out, int out_dtype,
+                                  int64_t out_stride_t, int64_t out_stride_h, unsigned int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
