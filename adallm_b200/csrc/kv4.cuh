@@ -84,5 +84,22 @@ inline int cache_ok(const void* kc, const void* vc, int64_t s_page, int64_t s_he
   return ADA_OK;
 }
 
+// Checks that the attention entries share.
+inline int attn_ok(const void* q, int qd, int64_t q_st, int64_t q_sh, const void* out, int od, int64_t o_st, int64_t o_sh,
+                   const void* kc, const void* vc, int64_t s_page, int64_t s_head, int64_t num_pages, const int32_t* bt,
+                   int64_t bt_stride, int32_t max_pages, int32_t hq, int32_t hkv, int32_t d, int32_t page, float scale,
+                   float k_scale, float v_scale, int32_t window) {
+  if (!q || !out || !bt || hq <= 0 || hkv <= 0 || max_pages <= 0) return ADA_ERR_INVALID_ARG;
+  if ((qd != ADA_DT_BF16 && qd != ADA_DT_F16) || (od != ADA_DT_BF16 && od != ADA_DT_F16)) return ADA_ERR_INVALID_ARG;
+  if (d != D) return ADA_ERR_UNSUPPORTED;
+  if (const int e = cache_ok(kc, vc, s_page, s_head, num_pages, hkv, page)) return e;
+  if (hq % hkv || window < 0 || bt_stride < max_pages) return ADA_ERR_INVALID_ARG;
+  if (!(scale * k_scale > 0.f) || !(v_scale > 0.f)) return ADA_ERR_INVALID_ARG;
+  if ((int64_t)max_pages * page > (1LL << 30)) return ADA_ERR_UNSUPPORTED;
+  if (misaligned16(q) || misaligned16(out) || ((q_st | q_sh | o_st | o_sh) & 7)) return ADA_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(bt) & 3) return ADA_ERR_ALIGNMENT;
+  return ADA_OK;
+}
+
 }  // namespace kv4
 }  // namespace ada

@@ -123,57 +123,10 @@ static void dispatch_attn(const AttnParams& P, dim3 grid, int qd, int od, cudaSt
     od == ADA_DT_BF16 ? launch_attn<__half, __nv_bfloat16>(P, grid, st) : launch_attn<__half, __half>(P, grid, st);
 }
 
-// Checks that both forms share.
-static int attn_ok(const AttnParams& P, int qd, int od, int32_t hq, int32_t hkv, int32_t d, float scale, float k_scale,
-                   float v_scale) {
-  if (!P.q || !P.out || !P.bt || hq <= 0 || hkv <= 0 || P.max_pages <= 0) return ADA_ERR_INVALID_ARG;
-  if ((qd != ADA_DT_BF16 && qd != ADA_DT_F16) || (od != ADA_DT_BF16 && od != ADA_DT_F16)) return ADA_ERR_INVALID_ARG;
-  if (d != D) return ADA_ERR_UNSUPPORTED;
-  if (const int e = cache_ok(P.kc, P.vc, P.s_page, P.s_head, P.num_pages, hkv, P.page)) return e;
-  if (hq % hkv || P.window < 0 || P.bt_stride < P.max_pages) return ADA_ERR_INVALID_ARG;
-  if (!(scale * k_scale > 0.f) || !(v_scale > 0.f)) return ADA_ERR_INVALID_ARG;
-  if ((int64_t)P.max_pages * P.page > (1LL << 30)) return ADA_ERR_UNSUPPORTED;
-  if (misaligned16(P.q) || misaligned16(P.out) || ((P.q_st | P.q_sh | P.o_st | P.o_sh) & 7)) return ADA_ERR_ALIGNMENT;
-  if ((reinterpret_cast<uintptr_t>(P.bt) | reinterpret_cast<uintptr_t>(P.lens) | reinterpret_cast<uintptr_t>(P.cu_q) |
-       reinterpret_cast<uintptr_t>(P.cu_k)) & 3)
-    return ADA_ERR_ALIGNMENT;
-  return ADA_OK;
-}
-
 }  // namespace kv4
 }  // namespace ada
 
 using namespace ada;
-
-extern "C" size_t ada_kv4_paged_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t num_kv_heads) {
-  return batch > 0 && num_heads > 0 && num_kv_heads > 0 ? 16 : 0;
-}
-
-extern "C" int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h,
-                                    const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
-                                    int64_t kv_stride_head, int64_t num_pages, const int32_t* block_tables,
-                                    int64_t bt_stride, int32_t max_pages, const int32_t* context_lens, int32_t batch,
-                                    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
-                                    float scale, float k_scale, float v_scale, int32_t window, void* out,
-                                    int out_dtype, int64_t out_stride_b, int64_t out_stride_h, void* workspace,
-                                    size_t workspace_bytes, void* stream) {
-  if (batch < 0) return ADA_ERR_INVALID_ARG;
-  if (batch == 0) return ADA_OK;
-  kv4::AttnParams P{q, q_stride_b, q_stride_h, out, out_stride_b, out_stride_h, k_cache, v_cache, kv_stride_page,
-                    kv_stride_head, num_pages, block_tables, bt_stride, max_pages, page_size, 1, window, context_lens,
-                    nullptr, nullptr, batch, scale * k_scale * kv4::LOG2E, v_scale};
-  if (!context_lens) return ADA_ERR_INVALID_ARG;
-  if (const int e = kv4::attn_ok(P, q_dtype, out_dtype, num_heads, num_kv_heads, head_dim, scale, k_scale, v_scale))
-    return e;
-  if (batch > 65535 || num_heads > 65535) return ADA_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < ada_kv4_paged_decode_workspace_size(batch, num_heads, num_kv_heads))
-    return ADA_ERR_WORKSPACE;
-  P.group = num_heads / num_kv_heads;
-  kv4::dispatch_attn(P, dim3(1, (unsigned)num_heads, (unsigned)batch), q_dtype, out_dtype,
-                     reinterpret_cast<cudaStream_t>(stream));
-  ADA_CHECK_LAUNCH();
-  return ADA_OK;
-}
 
 extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h,
                                      const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
@@ -190,8 +143,12 @@ extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_strid
                     kv_stride_head, num_pages, block_tables, bt_stride, max_pages, page_size, 1, window, nullptr,
                     cu_seqlens_q, cu_seqlens_k, total_q, scale * k_scale * kv4::LOG2E, v_scale};
   if (!cu_seqlens_q || !cu_seqlens_k) return ADA_ERR_INVALID_ARG;
-  if (const int e = kv4::attn_ok(P, q_dtype, out_dtype, num_heads, num_kv_heads, head_dim, scale, k_scale, v_scale))
+  if (const int e = kv4::attn_ok(q, q_dtype, q_stride_t, q_stride_h, out, out_dtype, out_stride_t, out_stride_h, k_cache,
+                                 v_cache, kv_stride_page, kv_stride_head, num_pages, block_tables, bt_stride, max_pages,
+                                 num_heads, num_kv_heads, head_dim, page_size, scale, k_scale, v_scale, window))
     return e;
+  if ((reinterpret_cast<uintptr_t>(cu_seqlens_q) | reinterpret_cast<uintptr_t>(cu_seqlens_k)) & 3)
+    return ADA_ERR_ALIGNMENT;
   if (batch > 65535 || num_heads > 65535) return ADA_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(err) & 3) return ADA_ERR_ALIGNMENT;
   P.group = num_heads / num_kv_heads;

@@ -1,0 +1,656 @@
+// Decode attention over the 4-bit paged KV cache (kv4.cuh), one query token a sequence.
+//
+//   out[b, h] = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale q . k_t),   t over the visible keys.
+//
+// Bound by HBM: 144 bytes a key and KV head against 4 * 128 * group operations.  A warp takes a
+// range of 16-key tiles; the tiles of all (sequence, KV head) items stand in one row and every warp
+// gets the same number of them, whatever the lengths, so one wave ends together.  What an item's
+// warps have found (maximum, sum, O) is joined in shared memory for the warps of a CTA and by a second
+// small kernel for several CTAs; items inside one warp or CTA are finished there.
+//
+// Tile: K 1,024 + 128 bytes and V the same, brought by cp.async (16 bytes a lane and step) into the
+// warp's own ring, so no barrier but the warp's.  Products on m16n8k16 with fp16 operands and fp32 sums:
+//   S^T = K Q^T    keys on M, heads on N.  The 128 elements are contracted in an order of our own:
+//                  lane (g, c) multiplies elements [32c, 32c + 32) of keys g and g + 8, which are 16
+//                  contiguous bytes of the row, with the same elements of Q (permuted once).
+//   O^T += V^T P^T elements on M, heads on N: lane (g, c) needs keys 2c, 2c+1, 2c+8, 2c+9 of the 16
+//                  elements of scale block g.  Row pairs' nibbles are joined in words of 8 before they are
+//                  widened, so a byte becomes an operand register (key, key + 1) by one conversion.
+// P^T comes from S^T by a transpose of 8x8 fragments (movmatrix).  A code times its scale is exact
+// in fp16.  The running maximum moves when a score passes it by 8 (log2): a vote a tile instead
+// of a reduction; p <= 2^8 in fp16 then, half a step 2^-11 of itself, and the sums are fp32.
+#include "kv4.cuh"
+
+namespace ada {
+namespace kv4 {
+namespace dec {
+
+constexpr int WARPS = 8;
+constexpr int STAGES = 4;
+constexpr int KEYS = 16;
+constexpr int V_OFF = KEYS * ROW;             // V codes
+constexpr int KS_OFF = 2 * KEYS * ROW;        // K scales
+constexpr int VS_OFF = KS_OFF + KEYS * SROW;  // V scales
+constexpr int TILE_BYTES = 2 * KEYS * ROW_BYTES;
+constexpr int HEADS = 8;                         // heads side by side (N of the MMA)
+constexpr int PART = HEADS * D + 2 * HEADS;      // floats of a partial: O, then (m, l) per head
+constexpr int WARP_SMEM = STAGES * TILE_BYTES + PART * 4;
+constexpr int MAX_BATCH = 8192;
+constexpr int MIN_TILES = 1;                     // fewest tiles a warp is given
+static_assert(STAGES * TILE_BYTES >= PART * 4, "a warp's last partial lies in its ring");
+
+struct Params {
+  const void* q;
+  int64_t q_sb, q_sh;
+  void* out;
+  int64_t o_sb, o_sh;
+  int q_bf16, o_bf16;
+  const uint8_t *kc, *vc;
+  int64_t s_page, s_head, num_pages;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int max_pages, page, window, batch;
+  int hkv, group, subs;  // subs: parts of at most 8 heads of a group
+  const int32_t* lens;
+  float scale_log2, v_scale;
+  int* cum;      // workspace: [batch + 1] tiles before a sequence (times items a sequence), then tiles a CTA
+  float* parts;  // workspace: [grid][2][PART]
+};
+
+struct Range {
+  int lo, hi, first;  // visible keys, first tile
+};
+__device__ __forceinline__ Range range_of(const Params& P, int b) {
+  const int ctx = (int)min((int64_t)__ldg(P.lens + b), (int64_t)P.max_pages * P.page);
+  const int full = __ldg(P.lens + b);
+  Range r;
+  r.hi = max(ctx, 0);
+  r.lo = P.window > 0 ? max(full - P.window, 0) : 0;
+  r.first = r.lo / KEYS;
+  return r;
+}
+__device__ __forceinline__ int tiles_of(const Range& r) {
+  return r.hi > r.lo ? (r.hi + KEYS - 1) / KEYS - r.first : 0;
+}
+
+// One (sequence, KV head, part of its heads), and where its tiles stand in the row of all.
+struct Item {
+  int b, h, base, end;  // h: KV head * subs + part
+};
+// The item of tile t (cum: tiles before a sequence, for one of its `items` items).
+__device__ __forceinline__ Item item_of(const int* cum, int batch, int items, int t) {
+  int lo = 0, hi = batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cum[mid + 1] * items > t)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  const int n = cum[lo + 1] - cum[lo];
+  const int h = (t - cum[lo] * items) / n;
+  const int base = cum[lo] * items + h * n;
+  return {lo, h, base, base + n};
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Four bytes of two codes each -> four f16x2.
+__device__ __forceinline__ void widen(uint32_t w, uint32_t* h) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+
+// Two rows lie in 128 bytes; a 16-byte chunk's place in them is moved by 2 * (line mod 4), so that
+// both the 16-byte reads of 8 keys' quarter rows and the 8-byte reads of every other key's blocks
+// fall on different banks.
+__device__ __forceinline__ int chunk_at(int line, int chunk) { return line * 128 + ((chunk ^ (2 * (line & 3))) << 4); }
+
+// Row of one head to memory: 16 elements of lane's scale block.
+__device__ __forceinline__ void write16(const Params& P, int b, int head, int e0, const float* f) {
+  if (P.o_bf16) {
+    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(P.out) + b * P.o_sb + head * P.o_sh + e0;
+    *reinterpret_cast<uint4*>(o) = pack8<__nv_bfloat16>(f);
+    *reinterpret_cast<uint4*>(o + 8) = pack8<__nv_bfloat16>(f + 8);
+  } else {
+    __half* o = reinterpret_cast<__half*>(P.out) + b * P.o_sb + head * P.o_sh + e0;
+    *reinterpret_cast<uint4*>(o) = pack8<__half>(f);
+    *reinterpret_cast<uint4*>(o + 8) = pack8<__half>(f + 8);
+  }
+}
+__device__ __forceinline__ void write4(const Params& P, int b, int head, int e0, float4 f) {
+  if (P.o_bf16) {
+    __nv_bfloat162 u[2] = {__floats2bfloat162_rn(f.x, f.y), __floats2bfloat162_rn(f.z, f.w)};
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + b * P.o_sb + head * P.o_sh + e0) =
+        *reinterpret_cast<uint2*>(u);
+  } else {
+    __half2 u[2] = {__floats2half2_rn(f.x, f.y), __floats2half2_rn(f.z, f.w)};
+    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(P.out) + b * P.o_sb + head * P.o_sh + e0) =
+        *reinterpret_cast<uint2*>(u);
+  }
+}
+
+// State of a warp's current piece of an item.
+struct Acc {
+  float o[8][4];  // M tile m: elements 16g + 2m (0, 1) and + 1 (2, 3), heads 2c (even) and 2c + 1
+  float m[2], l[2];
+};
+
+__global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_constant__ Params P) {
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ int warp_sum[WARPS];
+  __shared__ Item part_item[WARPS][2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  uint8_t* ring = sm + warp * WARP_SMEM;
+  float* slot0 = reinterpret_cast<float*>(ring + STAGES * TILE_BYTES);
+  int* cum = reinterpret_cast<int*>(sm + WARPS * WARP_SMEM);
+  const int items = P.hkv * P.subs;
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- tiles before each sequence
+  {
+    const int per = (P.batch + WARPS * 32 - 1) / (WARPS * 32);
+    const int b0 = min(tid * per, P.batch), b1 = min(b0 + per, P.batch);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) sum += tiles_of(range_of(P, b));
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    if (tid < WARPS) part_item[tid][0].end = part_item[tid][1].end = 0;  // no partial
+    __syncthreads();
+    int run = inc - sum;
+    for (int w = 0; w < warp; ++w) run += warp_sum[w];
+    for (int b = b0; b < b1; ++b) {
+      cum[b] = run;
+      run += tiles_of(range_of(P, b));
+    }
+    if (b0 < b1 && b1 == P.batch) cum[P.batch] = run;
+    __syncthreads();
+  }
+  const int total = cum[P.batch] * items;
+  const int workers = gridDim.x * WARPS;
+  const int per = max((total + workers - 1) / workers, MIN_TILES);
+  if (blockIdx.x == 0) {
+    for (int b = tid; b <= P.batch; b += WARPS * 32) P.cum[b] = cum[b];
+    if (tid == 0) P.cum[P.batch + 1] = per * WARPS;
+  }
+  const int64_t c0 = (int64_t)blockIdx.x * WARPS * per;  // this CTA's tiles
+  if (c0 >= total) return;
+  const int cta0 = (int)c0, cta1 = (int)min(c0 + (int64_t)WARPS * per, (int64_t)total);
+  const int r0 = min(cta0 + warp * per, total), r1 = min(r0 + per, total);
+
+  if (r0 < r1) {
+    // ---- the loads' cursor: tile `ld` of the row; its item, and the places of 32 of its tiles in the lanes
+    Item li = item_of(cum, P.batch, items, r0);
+    Range lr = range_of(P, li.b);
+    int ld = r0, from = -64;        // tiles [from, from + 32) of the row are in the lanes
+    int64_t at = -1;                // byte offset of the lane's tile in both caches (-1: not there)
+    int sat = 0;                    // its scales', from there
+    const int page_tiles = P.page / KEYS;
+    auto look = [&](int t) {  // tile t of the row, in item li: lane i takes tile t + i
+      from = t;
+      const int n = t + lane;
+      at = -1;
+      sat = 0;
+      if (n < li.end && n < r1) {
+        const int tile = lr.first + (n - li.base);
+        const int col = tile / page_tiles, row = tile - col * page_tiles;
+        const int64_t id = __ldg(P.bt + (int64_t)li.b * P.bt_stride + col);
+        if (id >= 0 && id < P.num_pages) {
+          at = id * P.s_page + (int64_t)(li.h / P.subs) * P.s_head + (int64_t)row * (KEYS * ROW);
+          sat = P.page * ROW - row * (KEYS * (ROW - SROW));
+        }
+      }
+    };
+    uint32_t there = 0;  // bit s: the tile in ring slot s is in the cache
+    const uint32_t ring_addr = smem_addr(ring);
+    auto load = [&](int slot) {
+      if (ld < r1) {
+        if (ld == li.end) {
+          li = item_of(cum, P.batch, items, ld);
+          lr = range_of(P, li.b);
+          from = -64;
+        }
+        if (ld >= from + 32 || from < 0) look(ld);
+        const int64_t a = __shfl_sync(0xffffffffu, at, ld - from);
+        const int s = __shfl_sync(0xffffffffu, sat, ld - from);
+        there &= ~(1u << slot);
+        if (a >= 0) {
+          there |= 1u << slot;
+          const uint8_t *k = P.kc + a, *v = P.vc + a;
+          const uint32_t dst = ring_addr + slot * TILE_BYTES;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int u = lane + 32 * i, line = u >> 3;
+            cp16(dst + chunk_at(line, u & 7), k + 16 * u);
+            cp16(dst + V_OFF + chunk_at(line, u & 7), v + 16 * u);
+          }
+          if (lane < 8) cp16(dst + KS_OFF + 16 * lane, k + s + 16 * lane);
+          else if (lane < 16) cp16(dst + VS_OFF + 16 * (lane - 8), v + s + 16 * (lane - 8));
+        }
+        ++ld;
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) load(i);
+
+    // ---- items of the range
+    int t = r0, slot = 0;
+    while (t < r1) {
+      const Item it = item_of(cum, P.batch, items, t);
+      const Range rg = range_of(P, it.b);
+      const int stop = min(it.end, r1);
+      const int kvh = it.h / P.subs, part = it.h - kvh * P.subs;
+      const int heads = min(P.group - part * HEADS, HEADS);
+      const int head0 = kvh * P.group + part * HEADS;
+      // queries: head g, elements [32c, 32c + 32)
+      uint32_t qf[16];
+      float fac[2];
+      {
+        float top = 0.f;
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (g < heads) {
+            const int64_t off = it.b * P.q_sb + (head0 + g) * P.q_sh + 32 * c + 8 * i;
+            if (P.q_bf16)
+              unpack8<__nv_bfloat16>(*reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(P.q) + off), f + 8 * i);
+            else
+              unpack8<__half>(*reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(P.q) + off), f + 8 * i);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[8 * i + j] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = max_nan(top, fabsf(f[i]));
+        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int ex = query_exponent(top);
+        const float mul = pow2(ex);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) qf[i] = pack_half2(f[2 * i] * mul, f[2 * i + 1] * mul);
+        const float mine = score_factor(P.scale_log2, ex);
+        fac[0] = __shfl_sync(0xffffffffu, mine, 8 * c);
+        fac[1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
+      }
+      Acc a;
+#pragma unroll
+      for (int m = 0; m < 8; ++m) a.o[m][0] = a.o[m][1] = a.o[m][2] = a.o[m][3] = 0.f;
+      a.m[0] = a.m[1] = -INFINITY;
+      a.l[0] = a.l[1] = 0.f;
+
+      for (; t < stop; ++t) {
+        cp_wait<STAGES - 2>();
+        __syncwarp();
+        const uint8_t* tile = ring + slot * TILE_BYTES;
+        const bool ok = (there >> slot) & 1;
+        const int key0 = (rg.first + (t - it.base)) * KEYS;
+        if (ok) {
+          const bool edge = key0 < rg.lo || key0 + KEYS > rg.hi;
+          // scores: keys g, g + 8 x heads 2c, 2c + 1
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+          {
+            const uint4 k0 = *reinterpret_cast<const uint4*>(tile + chunk_at(g >> 1, (g & 1) * 4 + c));
+            const uint4 k1 = *reinterpret_cast<const uint4*>(tile + chunk_at((g >> 1) + 4, (g & 1) * 4 + c));
+            const uint32_t s0 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(tile + KS_OFF + g * SROW + 2 * c));
+            const uint32_t s1 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(tile + KS_OFF + (g + 8) * SROW + 2 * c));
+            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t sa = prmt(s0, s0, w < 2 ? 0x1010 : 0x3232), sb = prmt(s1, s1, w < 2 ? 0x1010 : 0x3232);
+              uint32_t x[4], y[4];
+              widen(w0[w], x);
+              widen(w1[w], y);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint32_t A[4] = {mul2(x[2 * j], sa), mul2(y[2 * j], sb), mul2(x[2 * j + 1], sa), mul2(y[2 * j + 1], sb)};
+                mma_16816_f16(s, A, qf + 2 * (2 * w + j));
+              }
+            }
+          }
+          uint32_t vs0, vs1;  // scales of block g, keys (2c, 2c + 1) and (2c + 8, 2c + 9)
+          {
+            const uint8_t* p = tile + VS_OFF + 2 * c * SROW + g;
+            uint32_t b0 = p[0], b1 = p[SROW], b2 = p[8 * SROW], b3 = p[9 * SROW];
+            if (edge) {  // what is not seen counts as 0, also where it would be NaN
+              const int k = key0 + 2 * c;
+              b0 = k >= rg.lo && k < rg.hi ? b0 : 0;
+              b1 = k + 1 >= rg.lo && k + 1 < rg.hi ? b1 : 0;
+              b2 = k + 8 >= rg.lo && k + 8 < rg.hi ? b2 : 0;
+              b3 = k + 9 >= rg.lo && k + 9 < rg.hi ? b3 : 0;
+              const int ka = key0 + g, kb = ka + 8;
+              if (ka < rg.lo || ka >= rg.hi) s[0] = s[1] = -INFINITY;
+              if (kb < rg.lo || kb >= rg.hi) s[2] = s[3] = -INFINITY;
+            }
+            vs0 = e4m3x2_to_f16x2((uint16_t)(b0 | (b1 << 8)));
+            vs1 = e4m3x2_to_f16x2((uint16_t)(b2 | (b3 << 8)));
+          }
+          const float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+          if (__any_sync(0xffffffffu, (x0 - a.m[0]) * fac[0] > 8.f || (x1 - a.m[1]) * fac[1] > 8.f)) {
+            float n0 = x0, n1 = x1;
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+              n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+              n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+            }
+            n0 = fmaxf(n0, a.m[0]);
+            n1 = fmaxf(n1, a.m[1]);
+            const float f0 = n0 == -INFINITY ? 1.f : fast_exp2((a.m[0] - n0) * fac[0]);
+            const float f1 = n1 == -INFINITY ? 1.f : fast_exp2((a.m[1] - n1) * fac[1]);
+            a.m[0] = n0;
+            a.m[1] = n1;
+            a.l[0] *= f0;
+            a.l[1] *= f1;
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+              a.o[m][0] *= f0;
+              a.o[m][1] *= f1;
+              a.o[m][2] *= f0;
+              a.o[m][3] *= f1;
+            }
+          }
+          const float m0 = a.m[0] == -INFINITY ? 0.f : a.m[0], m1 = a.m[1] == -INFINITY ? 0.f : a.m[1];
+          const float p0 = fast_exp2((s[0] - m0) * fac[0]), p1 = fast_exp2((s[1] - m1) * fac[1]);
+          const float p2 = fast_exp2((s[2] - m0) * fac[0]), p3 = fast_exp2((s[3] - m1) * fac[1]);
+          a.l[0] += p0 + p2;
+          a.l[1] += p1 + p3;
+          const uint32_t pb[2] = {transpose8(pack_half2(p0, p1)), transpose8(pack_half2(p2, p3))};
+          // values: keys 2c, 2c + 1, 2c + 8, 2c + 9, block g
+          const int vch = (g >> 1), vin = (g & 1) * 8;
+          const uint2 va = *reinterpret_cast<const uint2*>(tile + V_OFF + chunk_at(c, vch) + vin);
+          const uint2 vb = *reinterpret_cast<const uint2*>(tile + V_OFF + chunk_at(c, 4 + vch) + vin);
+          const uint2 vc = *reinterpret_cast<const uint2*>(tile + V_OFF + chunk_at(c + 4, vch) + vin);
+          const uint2 vd = *reinterpret_cast<const uint2*>(tile + V_OFF + chunk_at(c + 4, 4 + vch) + vin);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t a0 = w ? va.y : va.x, b0 = w ? vb.y : vb.x, c0_ = w ? vc.y : vc.x, d0 = w ? vd.y : vd.x;
+            constexpr uint32_t LO = 0x0F0F0F0Fu;
+            uint32_t e0[4], e1[4], f0[4], f1[4];  // (even, odd) elements of the first and second key pair
+            widen((a0 & LO) | ((b0 << 4) & ~LO), e0);
+            widen(((a0 >> 4) & LO) | (b0 & ~LO), e1);
+            widen((c0_ & LO) | ((d0 << 4) & ~LO), f0);
+            widen(((c0_ >> 4) & LO) | (d0 & ~LO), f1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t A[4] = {mul2(e0[j], vs0), mul2(e1[j], vs0), mul2(f0[j], vs1), mul2(f1[j], vs1)};
+              mma_16816_f16(a.o[4 * w + j], A, pb);
+            }
+          }
+        }
+        __syncwarp();  // every lane has read the slot before this one
+        load(slot == 0 ? STAGES - 1 : slot - 1);
+        slot = slot == STAGES - 1 ? 0 : slot + 1;
+      }
+
+      // ---- the piece's end
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        a.l[0] += __shfl_xor_sync(0xffffffffu, a.l[0], o);
+        a.l[1] += __shfl_xor_sync(0xffffffffu, a.l[1], o);
+      }
+      const bool began = it.base >= r0, ended = it.end <= r1;
+      if (began && ended) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (2 * c + x >= heads) continue;
+          // (a NaN sum stays one)
+          const float inv = a.l[x] == 0.f ? 0.f : P.v_scale / a.l[x];
+          float f[16];
+#pragma unroll
+          for (int m = 0; m < 8; ++m) {
+            f[2 * m] = a.o[m][x] * inv;
+            f[2 * m + 1] = a.o[m][2 + x] * inv;
+          }
+          write16(P, it.b, head0 + 2 * c + x, 16 * g, f);
+        }
+      } else {
+        // the last piece's partial may lie in the ring: its own copies have arrived
+        const int which = began ? 1 : 0;
+        float* dst = which ? reinterpret_cast<float*>(ring) : slot0;
+        if (which) {
+          cp_wait<0>();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float* o = dst + (2 * c + x) * D + 16 * g;
+#pragma unroll
+          for (int m = 0; m < 8; m += 2)
+            *reinterpret_cast<float4*>(o + 2 * m) = make_float4(a.o[m][x], a.o[m][2 + x], a.o[m + 1][x], a.o[m + 1][2 + x]);
+          if (g == 0) {
+            dst[HEADS * D + 2 * (2 * c + x)] = a.m[x] == -INFINITY ? -INFINITY : a.m[x] * fac[x];
+            dst[HEADS * D + 2 * (2 * c + x) + 1] = a.l[x];
+          }
+        }
+        if (lane == 0) part_item[warp][which] = it;
+      }
+    }
+  }
+  __syncthreads();
+
+  // ---- pieces of one item in several warps: joined here (thread: head, 4 elements)
+  const int head = tid >> 5, e0 = 4 * lane;
+  int w = 0;
+  while (w < 2 * WARPS) {
+    const Item it = part_item[w >> 1][w & 1];
+    if (it.end == 0) {
+      ++w;
+      continue;
+    }
+    int last = w;  // the item's last partial of this CTA: its others are the first slots of the next warps
+    for (int n = ((w >> 1) + 1) * 2; n < 2 * WARPS; n += 2) {
+      const Item x = part_item[n >> 1][0];
+      if (x.end != it.end) break;
+      last = n;
+    }
+    auto piece = [&](int n) {
+      const uint8_t* r = sm + (n >> 1) * WARP_SMEM;
+      return reinterpret_cast<const float*>(n & 1 ? r : r + STAGES * TILE_BYTES);
+    };
+    float m = -INFINITY;
+    for (int n = w; n <= last; n = ((n >> 1) + 1) * 2) m = fmaxf(m, piece(n)[HEADS * D + 2 * head]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int n = w; n <= last; n = ((n >> 1) + 1) * 2) {
+      const float* p = piece(n);
+      const float pm = p[HEADS * D + 2 * head];
+      const float f = m == -INFINITY ? 1.f : fast_exp2(pm - m);
+      const float4 x = *reinterpret_cast<const float4*>(p + head * D + e0);
+      l = fmaf(f, p[HEADS * D + 2 * head + 1], l);
+      o.x = fmaf(f, x.x, o.x);
+      o.y = fmaf(f, x.y, o.y);
+      o.z = fmaf(f, x.z, o.z);
+      o.w = fmaf(f, x.w, o.w);
+    }
+    if (it.base >= cta0 && it.end <= cta1) {
+      const int kvh = it.h / P.subs, part = it.h - kvh * P.subs;
+      if (head < min(P.group - part * HEADS, HEADS)) {
+        const float inv = l == 0.f ? 0.f : P.v_scale / l;
+        write4(P, it.b, kvh * P.group + part * HEADS + head, e0, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+      }
+    } else {
+      float* dst = P.parts + ((int64_t)blockIdx.x * 2 + (it.base >= cta0 ? 1 : 0)) * PART;
+      *reinterpret_cast<float4*>(dst + head * D + e0) = o;
+      if (lane == 0) {
+        dst[HEADS * D + 2 * head] = m;
+        dst[HEADS * D + 2 * head + 1] = l;
+      }
+    }
+    w = last + 1;
+  }
+}
+
+// Items of several CTAs, and sequences without keys.  One CTA an item; thread: head, 4 elements.
+constexpr int MAX_CTAS = 512;
+__global__ void __launch_bounds__(HEADS * 32) merge_kernel(const __grid_constant__ Params P) {
+  __shared__ float weight[HEADS][MAX_CTAS];
+  pdl_wait();
+  pdl_trigger();
+  const int items = P.hkv * P.subs, b = blockIdx.x / items, h = blockIdx.x - b * items;
+  const int head = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = 4 * lane;
+  const int kvh = h / P.subs, part = h - kvh * P.subs;
+  const int before = __ldg(P.cum + b), n = __ldg(P.cum + b + 1) - before, chunk = __ldg(P.cum + P.batch + 1);
+  const bool mine = head < min(P.group - part * HEADS, HEADS);
+  const int row = kvh * P.group + part * HEADS + head;
+  if (n == 0) {
+    if (mine) write4(P, b, row, e0, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
+  const int base = before * items + h * n;
+  const int first = base / chunk, pieces = (base + n - 1) / chunk - first + 1;
+  if (pieces == 1) return;  // finished there
+  // the first CTA's partial is its second (the item begins there), the others' their first
+  auto at = [&](int i) { return P.parts + ((int64_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * PART; };
+  float m = -INFINITY, l = 0.f;
+  for (int i = lane; i < pieces; i += 32) m = fmaxf(m, at(i)[HEADS * D + 2 * head]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int i = lane; i < pieces; i += 32) {
+    const float* p = at(i) + HEADS * D + 2 * head;
+    const float f = m == -INFINITY ? 1.f : fast_exp2(p[0] - m);
+    weight[head][i] = f;
+    l = fmaf(f, p[1], l);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  __syncwarp();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < pieces; ++i) {
+    const float f = weight[head][i];
+    const float4 x = *reinterpret_cast<const float4*>(at(i) + head * D + e0);
+    o.x = fmaf(f, x.x, o.x);
+    o.y = fmaf(f, x.y, o.y);
+    o.z = fmaf(f, x.z, o.z);
+    o.w = fmaf(f, x.w, o.w);
+  }
+  const float inv = l == 0.f ? 0.f : P.v_scale / l;
+  if (mine) write4(P, b, row, e0, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+}
+
+static int grid_size(int dev) {
+  static std::atomic<int> sms[64];
+  int n = sms[dev];
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 0;
+    sms[dev] = n;
+  }
+  return n * 2 < MAX_CTAS ? n * 2 : MAX_CTAS;
+}
+
+}  // namespace dec
+}  // namespace kv4
+}  // namespace ada
+
+using namespace ada;
+namespace dec = ada::kv4::dec;
+
+// The lists (cum and the tiles a CTA), rounded up to 16 bytes, then two partials a CTA.
+static size_t decode_lists(int32_t batch) { return ((size_t)(batch + 2) * 4 + 15) & ~(size_t)15; }
+
+extern "C" size_t ada_kv4_paged_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t num_kv_heads) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0) return 0;
+  return decode_lists(batch) + (size_t)dec::MAX_CTAS * 2 * dec::PART * 4;
+}
+
+extern "C" int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h,
+                                    const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
+                                    int64_t kv_stride_head, int64_t num_pages, const int32_t* block_tables,
+                                    int64_t bt_stride, int32_t max_pages, const int32_t* context_lens, int32_t batch,
+                                    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                    float scale, float k_scale, float v_scale, int32_t window, void* out,
+                                    int out_dtype, int64_t out_stride_b, int64_t out_stride_h, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (batch < 0) return ADA_ERR_INVALID_ARG;
+  if (batch == 0) return ADA_OK;
+  if (!context_lens) return ADA_ERR_INVALID_ARG;
+  if (const int e = kv4::attn_ok(q, q_dtype, q_stride_b, q_stride_h, out, out_dtype, out_stride_b, out_stride_h, k_cache,
+                                 v_cache, kv_stride_page, kv_stride_head, num_pages, block_tables, bt_stride, max_pages,
+                                 num_heads, num_kv_heads, head_dim, page_size, scale, k_scale, v_scale, window))
+    return e;
+  if (reinterpret_cast<uintptr_t>(context_lens) & 3) return ADA_ERR_ALIGNMENT;
+  dec::Params P;
+  P.hkv = num_kv_heads;
+  P.group = num_heads / num_kv_heads;
+  P.subs = (P.group + dec::HEADS - 1) / dec::HEADS;
+  const int64_t items = (int64_t)num_kv_heads * P.subs;
+  const int64_t tiles = cdiv((int64_t)max_pages * page_size, dec::KEYS) + 1;
+  // the row of all tiles is counted in 32 bits
+  if (batch > dec::MAX_BATCH || batch * items * tiles > 0x7fffffffLL || batch * items > 0x7fffffffLL)
+    return ADA_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < ada_kv4_paged_decode_workspace_size(batch, num_heads, num_kv_heads))
+    return ADA_ERR_WORKSPACE;
+  if (kv4::misaligned16(workspace)) return ADA_ERR_ALIGNMENT;
+  P.q = q;
+  P.q_sb = q_stride_b;
+  P.q_sh = q_stride_h;
+  P.out = out;
+  P.o_sb = out_stride_b;
+  P.o_sh = out_stride_h;
+  P.q_bf16 = q_dtype == ADA_DT_BF16;
+  P.o_bf16 = out_dtype == ADA_DT_BF16;
+  P.kc = k_cache;
+  P.vc = v_cache;
+  P.s_page = kv_stride_page;
+  P.s_head = kv_stride_head;
+  P.num_pages = num_pages;
+  P.bt = block_tables;
+  P.bt_stride = bt_stride;
+  P.max_pages = max_pages;
+  P.page = page_size;
+  P.window = window;
+  P.batch = batch;
+  P.lens = context_lens;
+  P.scale_log2 = scale * k_scale * kv4::LOG2E;
+  P.v_scale = v_scale;
+  P.cum = static_cast<int*>(workspace);
+  P.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + decode_lists(batch));
+  static std::atomic<bool> ready[64];
+  constexpr size_t most = dec::WARPS * dec::WARP_SMEM + (dec::MAX_BATCH + 1) * 4;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ADA_ERR_CUDA;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(dec::split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
+      return ADA_ERR_CUDA;
+    ready[dev] = true;
+  }
+  const int grid = dec::grid_size(dev);
+  if (grid == 0) return ADA_ERR_CUDA;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const size_t smem = dec::WARPS * dec::WARP_SMEM + (size_t)(batch + 1) * 4;
+  (void)launch_k(dec::split_kernel, dim3((unsigned)grid), dim3(dec::WARPS * 32), smem, st, P);
+  ADA_CHECK_LAUNCH();
+  (void)launch_k(dec::merge_kernel, dim3((unsigned)(batch * items)), dim3(dec::HEADS * 32), 0, st, P);
+  ADA_CHECK_LAUNCH();
+  return ADA_OK;
+}
