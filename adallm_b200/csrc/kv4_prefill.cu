@@ -1,0 +1,652 @@
+// Causal prefill attention over the 4-bit paged KV cache (kv4.cuh).
+//
+// Semantics as the e4m3 form (prefill_attention.cu): sequence b's len_q new rows see keys
+// j <= i + len_k - len_q, with a window W > 0 also j >= i + len_k - len_q - W; a row without keys is
+// zeros.  Rows are (token, head) pairs of a KV head's group, head fastest, so 256 / group tokens
+// share every key block that a CTA widens.
+//
+// Bound by the exponentials and the tensor pipe alike: a block of 64 keys takes 256 x 64 of the former
+// (16 a cycle and SM: 1,024 cycles) and 2 x 256 x 64 x 128 multiply-adds (4,096 a cycle: 1,024).
+//
+// One CTA a (256-row query block, KV head, sequence); 14 warps:
+//   warp 0        producer: copies the codes and scales of each block's four 16-key tiles (contiguous
+//                 pieces of 1,024 and 128 bytes) into a staging ring;
+//   warp 1        MMA issuer and TMEM owner: S_t = Q_t K^T for the two 128-row tiles t (M 128, N 64) into
+//                 one of a tile's two S buffers, O_t += P_t V with P_t as the A operand in TMEM;
+//   warps 2-5     converters: codes x scales -> f16 K and V operand tiles (exact);
+//   warps 6-9, 10-13   softmax of tile 0 and 1, thread = row: brings its query row into shared memory
+//                 as f16 (times a power of two, kv4.cuh), then per block reads 64 scores from TMEM and
+//                 writes 64 f16 probabilities over them, where P V reads them: no shared memory and no
+//                 proxy fence in between.  A row's reference moves when a score passes it by
+//                 8 (log2); only then its O row is rescaled.
+//
+// A NaN scale of a value would reach every row through 0 * NaN, also those that do not see its key:
+// the converters widen it as 0 and mark (key, scale block), and rows that see a marked key turn
+// their 16 elements to NaN at the end.
+//
+// Barriers (block j, tile t): e_full[j % NSTG], e_empty, kv_full[j % NKV], kv_empty (commit after both P V),
+// s_full[t][j & 1] (commit), p_full[t][j & 1] (4 warps), o_done[t] (commit after P V), q_ready (8 warps), fin.
+// A refill waits for the release of the use before, so a barrier is never two phases ahead of a
+// waiter: S_{j+2} is issued after p_full of j; o_done of j comes after p_full of j, whose softmax
+// has already passed its wait for j - 1.  Before S_{j+1} overwrites the buffer that P_{j-1} lay in, the
+// issuer waits for o_done of j - 1.
+#include "kv4.cuh"
+#include "tc_attention.cuh"
+
+namespace ada {
+namespace kv4 {
+namespace pf4 {
+using namespace tca;
+using namespace sm100;
+
+constexpr int NT = 2, BM = 128, BN = 64, TILE = 16;
+constexpr int NSTG = 4, NKV = 3, NCONV = 4, NSOFT = 4;
+constexpr int THREADS = (2 + NCONV + NT * NSOFT) * 32;
+constexpr int Q_OFF = 0;                     // f16 Q, NT x [2 halves][128 rows][128 B]
+constexpr int K_OFF = Q_OFF + NT * 32768;    // f16 K, NKV x [2 halves][64 keys][128 B]
+constexpr int V_OFF = K_OFF + NKV * 16384;
+constexpr int E_OFF = V_OFF + NKV * 16384;   // staging: K codes, V codes, K scales, V scales of 64 keys
+constexpr int E_BYTES = 2 * BN * ROW_BYTES;
+constexpr int EV = BN * ROW, EKS = 2 * BN * ROW, EVS = EKS + BN * SROW;
+constexpr int BAR_OFF = E_OFF + NSTG * E_BYTES;
+constexpr int NBAR = 2 * NSTG + 2 * NKV + 5 * NT + 2;
+constexpr int FLAG_OFF = BAR_OFF + NBAR * 8;  // words: e_ok[NSTG], then per K/V slot [ok][4 warps' NaN flags][16 NaN masks]
+constexpr int SLOT_WORDS = 24;
+constexpr int SMEM = 1024 + FLAG_OFF + (NSTG + NKV * SLOT_WORDS + 4) * 4;
+constexpr uint32_t TMEM_COLS = 512, S_COL = 256;  // O of tile t at 128 t; S buffer b of tile t at 256 + 128 t + 64 b
+constexpr float MOVE_LOG2 = 8.f;
+static_assert(SMEM <= 232448, "shared memory per CTA");
+static_assert(E_BYTES % 16 == 0 && BAR_OFF % 16 == 0 && (FLAG_OFF % 8) == 0, "alignment");
+constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+// Up to this factor |score * factor| < 2^24, where the rounding of a row's reference is below 1 (log2).
+constexpr float SAFE_FACTOR = 9.765625e-4f;  // 2^-10
+
+struct Params {
+  const void* q;
+  int64_t q_st, q_sh;
+  void* out;
+  int64_t o_st, o_sh;
+  const uint8_t *kc, *vc;
+  int64_t s_page, s_head, num_pages;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int max_pages, page, window, group, qt, q_bf16, o_bf16;
+  const int32_t *cu_q, *cu_k;
+  int64_t rows;
+  float scale_log2, v_scale;
+  unsigned* err;
+};
+
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 64 columns of this thread's TMEM lane; load and wait are one statement, so no register of the load
+// can be touched before the wait.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr), "r"(taddr + 32)
+      : "memory");
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul2h(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Eight codes -> four f16x2 (low half = even element).
+__device__ __forceinline__ void widen8(uint32_t w, uint32_t* h) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+// 16 codes times their scale as 16 f16 (two chunks).
+__device__ __forceinline__ void widen16(uint2 codes, uint32_t scale2, uint4& lo, uint4& hi) {
+  uint32_t h[8];
+  widen8(codes.x, h);
+  widen8(codes.y, h + 4);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = mul2h(h[i], scale2);
+  lo = make_uint4(h[0], h[1], h[2], h[3]);
+  hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
+__device__ __forceinline__ uint32_t both_halves(uint32_t e4m3) {
+  const uint32_t h = e4m3x2_to_f16x2((uint16_t)e4m3);
+  return prmt(h, h, 0x1010);
+}
+
+// Keys [lo, hi) that new token t of a sequence sees.
+__device__ __forceinline__ void key_range(const Params& P, int t, int off, int len_k, int& lo, int& hi) {
+  hi = min(len_k, t + off + 1);
+  lo = P.window > 0 ? max(0, t + off - P.window) : 0;
+}
+
+__global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_constant__ Params P) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x, b = blockIdx.y;
+  const int qblk = gridDim.z - 1 - blockIdx.z;  // the longest causal rows of all heads and sequences first
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *qs = base + Q_OFF, *kf = base + K_OFF, *vf = base + V_OFF, *es = base + E_OFF;
+  uint64_t* e_full = reinterpret_cast<uint64_t*>(base + BAR_OFF);
+  uint64_t* e_empty = e_full + NSTG;
+  uint64_t* kv_full = e_empty + NSTG;
+  uint64_t* kv_empty = kv_full + NKV;
+  uint64_t* s_full = kv_empty + NKV;   // [NT][2]
+  uint64_t* p_full = s_full + 2 * NT;  // [NT][2]
+  uint64_t* o_done = p_full + 2 * NT;  // [NT]
+  uint64_t* q_ready = o_done + NT;
+  uint64_t* fin = q_ready + 1;
+  int* e_ok = reinterpret_cast<int*>(base + FLAG_OFF);
+  uint32_t* slots = reinterpret_cast<uint32_t*>(e_ok + NSTG);
+  uint32_t* tmem_slot = slots + NKV * SLOT_WORDS;
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* abort_v = abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NSTG; ++s) {
+      mbar_init(&e_full[s], 1);
+      mbar_init(&e_empty[s], NCONV);
+    }
+    for (int i = 0; i < NKV; ++i) {
+      mbar_init(&kv_full[i], NCONV);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2 * NT; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], NSOFT);
+    }
+    for (int t = 0; t < NT; ++t) mbar_init(&o_done[t], 1);
+    mbar_init(q_ready, NT * NSOFT);
+    mbar_init(fin, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  const int64_t q_begin = __ldg(P.cu_q + b);
+  const int len_q = (int)min(max((int64_t)__ldg(P.cu_q + b + 1) - q_begin, (int64_t)0), (int64_t)1 << 30);
+  const int len_k = (int)min(max((int64_t)__ldg(P.cu_k + b + 1) - __ldg(P.cu_k + b), (int64_t)0), (int64_t)1 << 30);
+  const int t0 = qblk * P.qt;
+  const bool active = t0 < len_q;
+  const int off = len_k - len_q;
+  int nblk = 0, kb0 = 0, k_end = 0;
+  if (active) {
+    const int t_last = min(t0 + P.qt, len_q) - 1;
+    int k_lo, k_hi, dlo, dhi;
+    key_range(P, t0, off, len_k, k_lo, dhi);
+    key_range(P, t_last, off, len_k, dlo, k_hi);
+    k_end = min(k_hi, P.max_pages * P.page);
+    kb0 = (k_lo / BN) * BN;
+    nblk = k_end > k_lo ? (k_end - kb0 + BN - 1) / BN : 0;
+  }
+
+  if (warp == 0) {  // ---------------- producer ----------------
+    // Lanes hold the places of 8 blocks' 32 tiles; lanes 0-15 each copy one piece of a block.
+    const int page_tiles = P.page / TILE;
+    const int64_t head = (int64_t)kvh * P.s_head;
+    auto place = [&](int first) -> int64_t {  // byte offset of the lane's tile's codes, -1: a hole
+      const int key0 = kb0 + TILE * (first + lane);
+      if (key0 >= k_end) return -1;
+      const int tile = key0 / TILE, col = tile / page_tiles;
+      const int64_t id = __ldg(P.bt + (int64_t)b * P.bt_stride + col);
+      return id < 0 || id >= P.num_pages ? -1 : id * P.s_page + head + (int64_t)(tile - col * page_tiles) * (TILE * ROW);
+    };
+    int64_t cur = nblk > 0 ? place(0) : -1, nxt = nblk > 8 ? place(32) : -1;
+    int issued = 0;
+    for (int j = 0; j < nblk; ++j) {
+      if (j > 0 && (j & 7) == 0) {
+        cur = nxt;
+        nxt = j + 8 < nblk ? place(32 * (j / 8 + 1)) : -1;
+      }
+      const int s = j % NSTG;
+      int go = 1;
+      if (lane == 0) go = !*abort_v && (j < NSTG || wait_b(&e_empty[s], ((j / NSTG) - 1) & 1, abort_v, P.err));
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      // piece: tile (lane & 3) of K codes, V codes, K scales, V scales
+      const int tile = lane & 3, kind = (lane >> 2) & 3;
+      const int64_t at = __shfl_sync(0xffffffffu, cur, 4 * (j & 7) + tile);
+      const uint32_t mask = __ballot_sync(0xffffffffu, at >= 0) & 15u;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (lane == 0) {
+        e_ok[s] = (int)mask;
+        mbar_arrive_expect_tx(&e_full[s], __popc(mask) * 2u * TILE * ROW_BYTES);
+      }
+      __syncwarp();
+      if (lane < 16 && at >= 0) {
+        const uint8_t* cache = (kind & 1) ? P.vc : P.kc;
+        uint8_t* st = es + s * E_BYTES;
+        if (kind < 2) {
+          bulk_load(st + kind * EV + tile * (TILE * ROW), cache + at, TILE * ROW, &e_full[s]);
+        } else {
+          const int row = (kb0 + j * BN + TILE * tile) % P.page;
+          bulk_load(st + (kind == 2 ? EKS : EVS) + tile * (TILE * SROW),
+                    cache + at - (int64_t)row * ROW + (int64_t)P.page * ROW + row * SROW, TILE * SROW, &e_full[s]);
+        }
+      }
+      issued = j + 1;
+    }
+    if (lane == 0) {
+      // leave no copy in flight when the CTA ends: wait (bounded) for the last use of each slot
+      for (int j = issued > NSTG ? issued - NSTG : 0; j < issued; ++j) {
+        uint32_t spins = 0;
+        const uint64_t t_start = globaltimer();
+        while (!mbar_try_wait(&e_full[j % NSTG], (j / NSTG) & 1)) {
+          if ((++spins & 63u) == 0 && globaltimer() - t_start > 2000000000ull) {
+            if (P.err) atomicOr(P.err, ERR_TILE_WAIT);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {  // ---------------- MMA issuer ----------------
+    if (lane == 0 && nblk > 0) {
+      const uint32_t q_addr = smem_u32(qs), k_addr = smem_u32(kf), v_addr = smem_u32(vf);
+      auto issue_s = [&](int j) {
+        const uint32_t kb = (uint32_t)(j % NKV);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint32_t d = tmem + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t hoff = (uint32_t)t * 32768u + (uint32_t)(kk / 4) * 16384u + (uint32_t)(kk % 4) * 32u;
+            const uint32_t koff = kb * 16384u + (uint32_t)(kk / 4) * 8192u + (uint32_t)(kk % 4) * 32u;
+            mma_f16(d, desc_kmajor_sw128(q_addr + hoff), desc_kmajor_sw128(k_addr + koff), IDESC_S, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[2 * t + (j & 1)]);
+        }
+      };
+      bool ok = wait_b(q_ready, 0, abort_v, P.err) && wait_b(&kv_full[0], 0, abort_v, P.err);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0);
+      }
+      for (int j = 0; ok && j < nblk; ++j) {
+        if (j + 1 < nblk) {
+          if (!wait_b(&kv_full[(j + 1) % NKV], ((j + 1) / NKV) & 1, abort_v, P.err)) break;
+          if (j > 0 && !(wait_b(&o_done[0], (j - 1) & 1, abort_v, P.err) && wait_b(&o_done[1], (j - 1) & 1, abort_v, P.err)))
+            break;
+          tc_fence_after();
+          issue_s(j + 1);
+        }
+        const uint32_t kb = (uint32_t)(j % NKV);
+        for (int t = 0; t < NT && ok; ++t) {
+          if (!wait_b(&p_full[2 * t + (j & 1)], (j >> 1) & 1, abort_v, P.err)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t p = tmem + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk) {
+            const uint64_t vd = smem_desc(v_addr + kb * 16384u + (uint32_t)kk * 16u * 128u, 8192, 1024, SWZ_128B);
+            mma_f16_ts(tmem + 128u * (uint32_t)t, p + 8u * (uint32_t)kk, vd, IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
+          }
+          tc_commit(&o_done[t]);
+        }
+        if (ok) tc_commit(&kv_empty[kb]);
+      }
+      // every MMA issued above has completed before the teardown
+      tc_commit(fin);
+      uint32_t spins = 0;
+      const uint64_t t_start = globaltimer();
+      while (!mbar_try_wait(fin, 0)) {
+        if ((++spins & 63u) == 0 && globaltimer() - t_start > 2000000000ull) {
+          if (P.err) atomicOr(P.err, ERR_TILE_WAIT);
+          break;
+        }
+      }
+    }
+  } else if (warp < 2 + NCONV) {  // ---------------- converters ----------------
+    const int ct = threadIdx.x - 64;
+    for (int j = 0; j < nblk; ++j) {
+      const int s = j % NSTG, kb = j % NKV;
+      if (!wait_b(&e_full[s], (j / NSTG) & 1, abort_v, P.err)) break;
+      if (j >= NKV && !wait_b(&kv_empty[kb], ((j / NKV) - 1) & 1, abort_v, P.err)) break;
+      const uint8_t* st = es + s * E_BYTES;
+      const int mask = e_ok[s];
+      uint32_t* flags = slots + kb * SLOT_WORDS;
+      uint32_t nan_any = 0;
+      // 64 keys x 8 blocks of 16 elements an operand: 4 units a thread
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int unit = ct + 128 * u, key = unit >> 3, blk = unit & 7;
+        const bool kok = (mask >> (key >> 4)) & 1;
+        const bool vok = kok & (kb0 + j * BN + key < len_k);
+        const uint2 kc = *reinterpret_cast<const uint2*>(st + 8 * unit);
+        const uint2 vc = *reinterpret_cast<const uint2*>(st + EV + 8 * unit);
+        const uint32_t ks = kok ? st[EKS + unit] : 0u;
+        uint32_t vs = vok ? st[EVS + unit] : 0u;
+        const bool nan = (vs & 0x7Fu) == 0x7Fu;
+        const uint32_t marked = __ballot_sync(0xffffffffu, nan);  // 4 keys x 8 blocks
+        if (nan) vs = 0;
+        nan_any |= marked;
+        if (lane == 0) flags[8 + 4 * u + (warp - 2)] = marked;
+        uint4 lo, hi;
+        const int c0 = ((blk & 3) * 2) ^ (key & 7), c1 = c0 ^ 1;
+        const int at = kb * 16384 + (blk >> 2) * 8192 + key * 128;
+        widen16(kc, both_halves(ks), lo, hi);
+        *reinterpret_cast<uint4*>(kf + at + (c0 << 4)) = lo;
+        *reinterpret_cast<uint4*>(kf + at + (c1 << 4)) = hi;
+        widen16(vc, both_halves(vs), lo, hi);
+        *reinterpret_cast<uint4*>(vf + at + (c0 << 4)) = lo;
+        *reinterpret_cast<uint4*>(vf + at + (c1 << 4)) = hi;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        flags[4 + (warp - 2)] = nan_any;
+        if (warp == 2) flags[0] = (uint32_t)mask;
+        mbar_arrive_plain(&kv_full[kb]);
+        mbar_arrive_plain(&e_empty[s]);
+      }
+    }
+  } else {  // ---------------- softmax: warpgroup t, thread = row r of tile t ----------------
+    const int t = (warp - 2 - NCONV) / NSOFT;
+    const int q4 = warp & 3;  // the TMEM lane quarter that this warp may access
+    const int r = 32 * q4 + lane, R = t * BM + r;
+    const uint32_t trow = tmem + ((uint32_t)(32 * q4) << 16);
+    const uint32_t o_col = 128u * (uint32_t)t, s_col = S_COL + 128u * (uint32_t)t;
+    const int tok = t0 + R / P.group;
+    const int64_t row = q_begin + tok;
+    const bool valid = active && R < P.qt * P.group && tok < len_q && row >= 0 && row < P.rows;
+    const int head = kvh * P.group + R % P.group;
+    int lo = 0, hi = 0;
+    if (valid) key_range(P, tok, off, len_k, lo, hi);
+    float factor = 0.f;
+    if (nblk > 0) {  // the query row -> f16, times a power of two
+      const int64_t at = row * P.q_st + head * P.q_sh;
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(P.q) + at);
+      uint4 raw[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) raw[c] = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+      float top = 0.f;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        float f[8];
+        if (P.q_bf16) unpack8<__nv_bfloat16>(raw[c], f); else unpack8<__half>(raw[c], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(f[i]));
+      }
+      const int ex = query_exponent(top);
+      const float mul = pow2(ex);
+      factor = score_factor(P.scale_log2, ex);
+      if (!valid) factor = fminf(factor, SAFE_FACTOR);  // (all its keys are masked)
+      uint8_t* dst = qs + t * 32768 + r * 128;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        float f[8];
+        if (P.q_bf16) unpack8<__nv_bfloat16>(raw[c], f); else unpack8<__half>(raw[c], f);
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) =
+            make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
+                       pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_plain(q_ready);
+    }
+    const bool safe = __all_sync(0xffffffffu, factor <= SAFE_FACTOR);
+    float m = -INFINITY;  // largest score that set the reference
+    float ref = 0.f;      // the reference, log2 units (0: none yet)
+    uint64_t l2[2] = {0ull, 0ull};
+    uint32_t nan_blocks = 0;
+    bool failed = false;
+    for (int j = 0; j < nblk; ++j) {
+      const int sb = j & 1;
+      // warp-uniform outcomes: the TMEM accesses below are warp-collective.  (kv_full orders the flags)
+      if (!__all_sync(0xffffffffu, wait_b(&kv_full[j % NKV], (j / NKV) & 1, abort_v, P.err) &&
+                                       wait_b(&s_full[2 * t + sb], (j >> 1) & 1, abort_v, P.err))) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      float x[64];
+      uint32_t* sr = reinterpret_cast<uint32_t*>(x);
+      tmem_ld64(trow + s_col + BN * sb, sr);
+      const uint32_t* flags = slots + (j % NKV) * SLOT_WORDS;
+      const uint32_t blk_ok = flags[0];
+      const uint4 marked = *reinterpret_cast<const uint4*>(flags + 4);
+      const int key0 = kb0 + j * BN, a = lo - key0, e = hi - key0;  // visible columns [a, e) of loaded tiles
+      if (!__all_sync(0xffffffffu, blk_ok == 15u && a <= 0 && e >= BN)) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          const bool vis = (i >= a) & (i < e) & (((blk_ok >> (i >> 4)) & 1u) != 0);
+          x[i] = vis ? x[i] : -INFINITY;
+        }
+      }
+      if (marked.x | marked.y | marked.z | marked.w) {
+        for (int i = max(a, 0); i < min(e, BN); ++i) nan_blocks |= (flags[8 + (i >> 2)] >> (8 * (i & 3))) & 0xFFu;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 64; i += 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], fmaxf(x[i + 2 * k], x[i + 2 * k + 1]));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      float alpha = 1.f;
+      if ((top - m) * factor > MOVE_LOG2) {
+        alpha = m == -INFINITY ? 0.f : safe ? fast_exp2(ref - top * factor) : fast_exp2((m - top) * factor);
+        m = top;
+        ref = top * factor;
+      }
+      uint32_t pk[32];
+      if (safe) {
+        const uint64_t c2 = pair(factor, factor), r2 = pair(-ref, -ref);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float p0, p1;
+          unpair(fma2(pair(x[2 * i], x[2 * i + 1]), c2, r2), p0, p1);
+          p0 = fast_exp2(p0);
+          p1 = fast_exp2(p1);
+          // fp32 probabilities feed the row's sum, fp16 ones P V
+          if (i == 0 && alpha != 1.f) {
+            float s0, s1, s2, s3;
+            unpair(l2[0], s0, s1);
+            unpair(l2[1], s2, s3);
+            l2[0] = pair(s0 * alpha, s1 * alpha);
+            l2[1] = pair(s2 * alpha, s3 * alpha);
+          }
+          l2[i & 1] = add2(l2[i & 1], pair(p0, p1));
+          pk[i] = pack_half2(p0, p1);
+        }
+      } else {
+        const float mm = m == -INFINITY ? 0.f : m;
+        float s0, s1, s2, s3;
+        unpair(l2[0], s0, s1);
+        unpair(l2[1], s2, s3);
+        s0 *= alpha, s1 *= alpha, s2 *= alpha, s3 *= alpha;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float p0 = fast_exp2((x[2 * i] - mm) * factor), p1 = fast_exp2((x[2 * i + 1] - mm) * factor);
+          s0 += p0;
+          s1 += p1;
+          pk[i] = pack_half2(p0, p1);
+        }
+        l2[0] = pair(s0, s1);
+        l2[1] = pair(s2, s3);
+      }
+      // the probabilities over the scores
+#pragma unroll
+      for (int i = 0; i < 2; ++i) tmem_st16(trow + s_col + BN * sb + 16 * i, pk + 16 * i);
+      // Waited for in every block, also where nothing is rescaled: a parity tells a phase from the one
+      // before it only to a waiter that has seen that one complete.
+      if (j > 0 && !__all_sync(0xffffffffu, wait_b(&o_done[t], (j - 1) & 1, abort_v, P.err))) {
+        failed = true;
+        break;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {  // O is stable: P V of the block before has completed
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16_async(trow + o_col + 16 * c, o);
+          tmem_wait_ld16(o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st16(trow + o_col + 16 * c, o);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_plain(&p_full[2 * t + sb]);
+    }
+    // ---- epilogue: O row / l
+    if (!failed && nblk > 0) {
+      failed = !__all_sync(0xffffffffu, wait_b(&o_done[t], (nblk - 1) & 1, abort_v, P.err));
+      tc_fence_after();
+    }
+    failed = __any_sync(0xffffffffu, failed || *abort_v != 0);
+    float s0, s1, s2, s3;
+    unpair(l2[0], s0, s1);
+    unpair(l2[1], s2, s3);
+    const float l = (s0 + s1) + (s2 + s3);
+    const float nan = __uint_as_float(0x7FC00000u);
+    const float inv = failed ? nan : l == 0.f ? 0.f : P.v_scale / l;
+    const int64_t o_at = row * P.o_st + head * P.o_sh;
+#pragma unroll 1
+    for (int c = 0; c < D / 16; ++c) {
+      uint32_t o[16];
+      if (nblk > 0 && !failed) {
+        tmem_ld16_async(trow + o_col + 16 * c, o);
+        tmem_wait_ld16(o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = 0u;
+      }
+      if (valid) {
+        const float f16 = (nan_blocks >> c) & 1 ? nan : inv;
+        float f[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = l == 0.f && !failed && f16 == 0.f ? 0.f : __uint_as_float(o[i]) * f16;
+        if (P.o_bf16) {
+          __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(P.out) + o_at + 16 * c;
+          *reinterpret_cast<uint4*>(op) = pack8<__nv_bfloat16>(f);
+          *reinterpret_cast<uint4*>(op + 8) = pack8<__nv_bfloat16>(f + 8);
+        } else {
+          __half* op = reinterpret_cast<__half*>(P.out) + o_at + 16 * c;
+          *reinterpret_cast<uint4*>(op) = pack8<__half>(f);
+          *reinterpret_cast<uint4*>(op + 8) = pack8<__half>(f + 8);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+}  // namespace pf4
+}  // namespace kv4
+}  // namespace ada
+
+using namespace ada;
+namespace pf4 = ada::kv4::pf4;
+
+extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h,
+                                     const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
+                                     int64_t kv_stride_head, int64_t num_pages, const int32_t* block_tables,
+                                     int64_t bt_stride, int32_t max_pages, const int32_t* cu_seqlens_q,
+                                     const int32_t* cu_seqlens_k, int32_t batch, int64_t total_q, int32_t max_seqlen_q,
+                                     int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                     float scale, float k_scale, float v_scale, int32_t window, void* out,
+                                     int out_dtype, int64_t out_stride_t, int64_t out_stride_h, unsigned int* err,
+                                     void* stream) {
+  if (batch < 0 || max_seqlen_q < 0 || total_q < 0) return ADA_ERR_INVALID_ARG;
+  if (batch == 0 || max_seqlen_q == 0 || total_q == 0) return ADA_OK;
+  if (!cu_seqlens_q || !cu_seqlens_k) return ADA_ERR_INVALID_ARG;
+  if (const int e = kv4::attn_ok(q, q_dtype, q_stride_t, q_stride_h, out, out_dtype, out_stride_t, out_stride_h, k_cache,
+                                 v_cache, kv_stride_page, kv_stride_head, num_pages, block_tables, bt_stride, max_pages,
+                                 num_heads, num_kv_heads, head_dim, page_size, scale, k_scale, v_scale, window))
+    return e;
+  if ((reinterpret_cast<uintptr_t>(cu_seqlens_q) | reinterpret_cast<uintptr_t>(cu_seqlens_k) |
+       reinterpret_cast<uintptr_t>(err)) & 3)
+    return ADA_ERR_ALIGNMENT;
+  const int group = num_heads / num_kv_heads;
+  if (group > pf4::NT * pf4::BM || batch > 65535 || max_seqlen_q > (1 << 30)) return ADA_ERR_UNSUPPORTED;
+  pf4::Params P;
+  P.q = q;
+  P.q_st = q_stride_t;
+  P.q_sh = q_stride_h;
+  P.out = out;
+  P.o_st = out_stride_t;
+  P.o_sh = out_stride_h;
+  P.kc = k_cache;
+  P.vc = v_cache;
+  P.s_page = kv_stride_page;
+  P.s_head = kv_stride_head;
+  P.num_pages = num_pages;
+  P.bt = block_tables;
+  P.bt_stride = bt_stride;
+  P.max_pages = max_pages;
+  P.page = page_size;
+  P.window = window < (1 << 30) ? window : 1 << 30;  // (past every position: sums stay in 32 bits)
+  P.group = group;
+  P.qt = pf4::NT * pf4::BM / group;
+  P.q_bf16 = q_dtype == ADA_DT_BF16;
+  P.o_bf16 = out_dtype == ADA_DT_BF16;
+  P.cu_q = cu_seqlens_q;
+  P.cu_k = cu_seqlens_k;
+  P.rows = total_q;
+  P.scale_log2 = scale * k_scale * kv4::LOG2E;
+  P.v_scale = v_scale;
+  P.err = err;
+  const int64_t qblocks = cdiv(max_seqlen_q < total_q ? (int64_t)max_seqlen_q : total_q, P.qt);
+  if (qblocks > 65535) return ADA_ERR_UNSUPPORTED;
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ADA_ERR_CUDA;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(pf4::prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pf4::SMEM) != cudaSuccess)
+      return ADA_ERR_CUDA;
+    ready[dev] = true;
+  }
+  (void)launch_k(pf4::prefill_kernel, dim3((unsigned)num_kv_heads, (unsigned)batch, (unsigned)qblocks), dim3(pf4::THREADS),
+                 pf4::SMEM, reinterpret_cast<cudaStream_t>(stream), P);
+  ADA_CHECK_LAUNCH();
+  return ADA_OK;
+}

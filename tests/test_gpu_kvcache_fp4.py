@@ -388,6 +388,11 @@ def test_results_do_not_change_between_runs():
     c = make(33, [5000, 70, 2222, 1], [1] * 4, 32, 8, 16)
     first = run_decode(c)
     assert all(torch.equal(first, run_decode(c)) for _ in range(5))
+    for lens, new in (([85], [70]), ([64, 128, 192, 300], [33, 128, 20, 250]), ([2000], [3])):  # one, two, more key blocks
+        c = make(36, lens, new, 12, 4, 32)
+        first = run_prefill(c)
+        assert_near(first, *want_of(c, decode=False))
+        assert all(torch.equal(first, run_prefill(c)) for _ in range(25))
 
 
 def test_refusals():
