@@ -61,7 +61,7 @@ __device__ __forceinline__ uint32_t codes8(const float* x, float s) {
 // `top` into [2^14, 2^15), so that bf16 rows of any size keep their bits in fp16 (what falls under fp16's
 // range is 2^-38 of the largest); the exponent is taken back in the factor of the scores, which stops
 // at 2^90: |score| < 2^34 then keeps every product finite, and a row of such a factor is decided by its
-// largest score alone.  A row of zeros, or with an infinity or NaN, is left as it is.
+// largest score alone.  (It is never 0: a masked score of -inf stays one.)  A row of zeros, or with an infinity or NaN, is left as it is.
 __device__ __forceinline__ int query_exponent(float top) {
   if (!(top > 0.f) || !(top < INFINITY)) return 0;
   const int e = (int)(__float_as_uint(top) >> 23) - 127;  // (-127 for a subnormal)
@@ -69,7 +69,7 @@ __device__ __forceinline__ int query_exponent(float top) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -127 < e < 128
 __device__ __forceinline__ float score_factor(float scale_log2, int exponent) {
-  return fminf(scale_log2 * pow2(-exponent), 1.2379400392853803e27f);
+  return fmaxf(fminf(scale_log2 * pow2(-exponent), 1.2379400392853803e27f), 1e-36f);
 }
 
 inline bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }

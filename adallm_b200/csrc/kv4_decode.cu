@@ -3,13 +3,15 @@
 //   out[b, h] = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale q . k_t),   t over the visible keys.
 //
 // Bound by HBM: 144 bytes a key and KV head against 4 * 128 * group operations.  A warp takes a
-// range of 16-key tiles; the tiles of all (sequence, KV head) items stand in one row and every warp
+// range of 32-key steps; the steps of all (sequence, KV head) items stand in one row and every warp
 // gets the same number of them, whatever the lengths, so one wave ends together.  What an item's
 // warps have found (maximum, sum, O) is joined in shared memory for the warps of a CTA and by a second
 // small kernel for several CTAs; items inside one warp or CTA are finished there.
 //
-// Tile: K 1,024 + 128 bytes and V the same, brought by cp.async (16 bytes a lane and step) into the
-// warp's own ring, so no barrier but the warp's.  Products on m16n8k16 with fp16 operands and fp32 sums:
+// Step: 32 keys, the K and V rows of two 16-key tiles (each in a page of its own when pages are
+// short), brought by cp.async into the warp's own ring of two: half a warp copies a tile, so the
+// places of both are one shuffle, and no barrier is needed but the warp's.  Products on m16n8k16 with
+// fp16 operands and fp32 sums:
 //   S^T = K Q^T    keys on M, heads on N.  The 128 elements are contracted in an order of our own:
 //                  lane (g, c) multiplies elements [32c, 32c + 32) of keys g and g + 8, which are 16
 //                  contiguous bytes of the row, with the same elements of Q (permuted once).
@@ -17,8 +19,11 @@
 //                  elements of scale block g.  Row pairs' nibbles are joined in words of 8 before they are
 //                  widened, so a byte becomes an operand register (key, key + 1) by one conversion.
 // P^T comes from S^T by a transpose of 8x8 fragments (movmatrix).  A code times its scale is exact
-// in fp16.  The running maximum moves when a score passes it by 8 (log2): a vote a tile instead
+// in fp16.  The running maximum moves when a score passes it by 8 (log2): a vote a step instead
 // of a reduction; p <= 2^8 in fp16 then, half a step 2^-11 of itself, and the sums are fp32.
+//
+// Instructions come next after HBM: widening takes 192 a lane and tile (a conversion, mostly a shift, and
+// a product for two elements), so everything else is kept per 32 keys.
 #include "kv4.cuh"
 
 namespace ada {
@@ -26,18 +31,20 @@ namespace kv4 {
 namespace dec {
 
 constexpr int WARPS = 8;
-constexpr int STAGES = 4;
-constexpr int KEYS = 16;
-constexpr int V_OFF = KEYS * ROW;             // V codes
-constexpr int KS_OFF = 2 * KEYS * ROW;        // K scales
-constexpr int VS_OFF = KS_OFF + KEYS * SROW;  // V scales
-constexpr int TILE_BYTES = 2 * KEYS * ROW_BYTES;
+constexpr int STAGES = 2;
+constexpr int TILE = 16;                      // keys that lie in one page
+constexpr int KEYS = 2 * TILE;                // keys a step
+// a ring slot: of each tile K codes, V codes, then K scales, V scales
+constexpr int V_OFF = TILE * ROW;
+constexpr int KS_OFF = 2 * TILE * ROW;
+constexpr int VS_OFF = KS_OFF + TILE * SROW;
+constexpr int TILE_BYTES = 2 * TILE * ROW_BYTES;
+constexpr int STEP_BYTES = 2 * TILE_BYTES;
 constexpr int HEADS = 8;                         // heads side by side (N of the MMA)
 constexpr int PART = HEADS * D + 2 * HEADS;      // floats of a partial: O, then (m, l) per head
-constexpr int WARP_SMEM = STAGES * TILE_BYTES + PART * 4;
+constexpr int WARP_SMEM = STAGES * STEP_BYTES + PART * 4;
 constexpr int MAX_BATCH = 8192;
-constexpr int MIN_TILES = 1;                     // fewest tiles a warp is given
-static_assert(STAGES * TILE_BYTES >= PART * 4, "a warp's last partial lies in its ring");
+static_assert(STAGES * STEP_BYTES >= PART * 4, "a warp's last partial lies in its ring");
 
 struct Params {
   const void* q;
@@ -58,7 +65,7 @@ struct Params {
 };
 
 struct Range {
-  int lo, hi, first;  // visible keys, first tile
+  int lo, hi, first;  // visible keys, first step
 };
 __device__ __forceinline__ Range range_of(const Params& P, int b) {
   const int ctx = (int)min((int64_t)__ldg(P.lens + b), (int64_t)P.max_pages * P.page);
@@ -69,7 +76,7 @@ __device__ __forceinline__ Range range_of(const Params& P, int b) {
   r.first = r.lo / KEYS;
   return r;
 }
-__device__ __forceinline__ int tiles_of(const Range& r) {
+__device__ __forceinline__ int steps_of(const Range& r) {
   return r.hi > r.lo ? (r.hi + KEYS - 1) / KEYS - r.first : 0;
 }
 
@@ -156,7 +163,7 @@ __device__ __forceinline__ void write4(const Params& P, int b, int head, int e0,
 // State of a warp's current piece of an item.
 struct Acc {
   float o[8][4];  // M tile m: elements 16g + 2m (0, 1) and + 1 (2, 3), heads 2c (even) and 2c + 1
-  float m[2], l[2];
+  float l[2];
 };
 
 __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_constant__ Params P) {
@@ -165,18 +172,18 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
   __shared__ Item part_item[WARPS][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   uint8_t* ring = sm + warp * WARP_SMEM;
-  float* slot0 = reinterpret_cast<float*>(ring + STAGES * TILE_BYTES);
+  float* slot0 = reinterpret_cast<float*>(ring + STAGES * STEP_BYTES);
   int* cum = reinterpret_cast<int*>(sm + WARPS * WARP_SMEM);
   const int items = P.hkv * P.subs;
   pdl_wait();
   pdl_trigger();
 
-  // ---- tiles before each sequence
+  // ---- steps before each sequence
   {
     const int per = (P.batch + WARPS * 32 - 1) / (WARPS * 32);
     const int b0 = min(tid * per, P.batch), b1 = min(b0 + per, P.batch);
     int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += tiles_of(range_of(P, b));
+    for (int b = b0; b < b1; ++b) sum += steps_of(range_of(P, b));
     int inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -190,14 +197,14 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
     for (int w = 0; w < warp; ++w) run += warp_sum[w];
     for (int b = b0; b < b1; ++b) {
       cum[b] = run;
-      run += tiles_of(range_of(P, b));
+      run += steps_of(range_of(P, b));
     }
     if (b0 < b1 && b1 == P.batch) cum[P.batch] = run;
     __syncthreads();
   }
   const int total = cum[P.batch] * items;
   const int workers = gridDim.x * WARPS;
-  const int per = max((total + workers - 1) / workers, MIN_TILES);
+  const int per = max((total + workers - 1) / workers, 1);
   if (blockIdx.x == 0) {
     for (int b = tid; b <= P.batch; b += WARPS * 32) P.cum[b] = cum[b];
     if (tid == 0) P.cum[P.batch + 1] = per * WARPS;
@@ -208,60 +215,68 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
   const int r0 = min(cta0 + warp * per, total), r1 = min(r0 + per, total);
 
   if (r0 < r1) {
-    // ---- the loads' cursor: tile `ld` of the row; its item, and the places of 32 of its tiles in the lanes
+    // ---- the loads' cursor: step `ld` of the row, its item, and 32 tiles (16 steps) from step `from` on in the
+    // lanes: the page's id (-1: not there) and the tile's place in it
     Item li = item_of(cum, P.batch, items, r0);
     Range lr = range_of(P, li.b);
-    int ld = r0, from = -64;        // tiles [from, from + 32) of the row are in the lanes
-    int64_t at = -1;                // byte offset of the lane's tile in both caches (-1: not there)
-    int sat = 0;                    // its scales', from there
-    const int page_tiles = P.page / KEYS;
-    auto look = [&](int t) {  // tile t of the row, in item li: lane i takes tile t + i
-      from = t;
-      const int n = t + lane;
-      at = -1;
-      sat = 0;
-      if (n < li.end && n < r1) {
-        const int tile = lr.first + (n - li.base);
-        const int col = tile / page_tiles, row = tile - col * page_tiles;
-        const int64_t id = __ldg(P.bt + (int64_t)li.b * P.bt_stride + col);
-        if (id >= 0 && id < P.num_pages) {
-          at = id * P.s_page + (int64_t)(li.h / P.subs) * P.s_head + (int64_t)row * (KEYS * ROW);
-          sat = P.page * ROW - row * (KEYS * (ROW - SROW));
-        }
+    int ld = r0, from = -64, id = -1, place = 0;
+    const int page_tiles = P.page / TILE;
+    const int half = lane >> 4, l16 = lane & 15;
+    const int64_t head_off = (int64_t)(li.h / P.subs) * P.s_head;
+    const uint8_t *klane = P.kc + head_off + 16 * l16, *vlane = P.vc + head_off + 16 * l16;
+    auto look = [&]() {
+      from = ld;
+      const int key = (lr.first + (ld - li.base)) * KEYS + lane * TILE;
+      id = -1;
+      place = 0;
+      if (key < lr.hi) {
+        const int tile = key / TILE, col = tile / page_tiles;
+        place = tile - col * page_tiles;
+        id = __ldg(P.bt + (int64_t)li.b * P.bt_stride + col);
+        if (id >= P.num_pages) id = -1;
       }
     };
-    uint32_t there = 0;  // bit s: the tile in ring slot s is in the cache
-    const uint32_t ring_addr = smem_addr(ring);
+    uint32_t there = 0;  // bits 2s, 2s + 1: the tiles in ring slot s are in the cache
+    const uint32_t lane_dst = smem_addr(ring) + half * TILE_BYTES + (l16 >> 3) * 128;
+    const uint32_t even = lane_dst + (((l16 & 7) ^ (2 * (l16 >> 3))) << 4);  // lines 0, 1 of each four, then 2, 3
+    const uint32_t odd = lane_dst + (((l16 & 7) ^ (2 * (l16 >> 3)) ^ 4) << 4);
+    const uint32_t scales = smem_addr(ring) + half * TILE_BYTES + KS_OFF + 16 * l16;
     auto load = [&](int slot) {
       if (ld < r1) {
         if (ld == li.end) {
           li = item_of(cum, P.batch, items, ld);
           lr = range_of(P, li.b);
           from = -64;
+          const int64_t off = (int64_t)(li.h / P.subs) * P.s_head;
+          klane = P.kc + off + 16 * l16;
+          vlane = P.vc + off + 16 * l16;
         }
-        if (ld >= from + 32 || from < 0) look(ld);
-        const int64_t a = __shfl_sync(0xffffffffu, at, ld - from);
-        const int s = __shfl_sync(0xffffffffu, sat, ld - from);
-        there &= ~(1u << slot);
-        if (a >= 0) {
-          there |= 1u << slot;
-          const uint8_t *k = P.kc + a, *v = P.vc + a;
-          const uint32_t dst = ring_addr + slot * TILE_BYTES;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int u = lane + 32 * i, line = u >> 3;
-            cp16(dst + chunk_at(line, u & 7), k + 16 * u);
-            cp16(dst + V_OFF + chunk_at(line, u & 7), v + 16 * u);
-          }
-          if (lane < 8) cp16(dst + KS_OFF + 16 * lane, k + s + 16 * lane);
-          else if (lane < 16) cp16(dst + VS_OFF + 16 * (lane - 8), v + s + 16 * (lane - 8));
+        if (ld >= from + 16) look();
+        const int src = 2 * (ld - from) + half;
+        const int my = __shfl_sync(0xffffffffu, id, src), at = __shfl_sync(0xffffffffu, place, src);
+        const uint32_t ok = __ballot_sync(0xffffffffu, my >= 0);
+        there = (there & ~(3u << (2 * slot))) | (((ok & 1u) | ((ok >> 15) & 2u)) << (2 * slot));
+        if (my >= 0) {
+          const int64_t page = (int64_t)my * P.s_page;
+          const uint8_t *k = klane + page + at * (TILE * ROW), *v = vlane + page + at * (TILE * ROW);
+          const uint32_t s = slot * STEP_BYTES;
+          cp16(even + s, k);
+          cp16(odd + s + 256, k + 256);
+          cp16(even + s + 512, k + 512);
+          cp16(odd + s + 768, k + 768);
+          cp16(even + s + V_OFF, v);
+          cp16(odd + s + V_OFF + 256, v + 256);
+          cp16(even + s + V_OFF + 512, v + 512);
+          cp16(odd + s + V_OFF + 768, v + 768);
+          // 8 pieces of K's scales, 8 of V's
+          cp16(scales + s, (l16 < 8 ? k : v - 128) + (P.page * ROW - at * (TILE * (ROW - SROW))));
         }
         ++ld;
       }
       cp_commit();
     };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load(i);
+    for (int i = 0; i < STAGES; ++i) load(i);
 
     // ---- items of the range
     int t = r0, slot = 0;
@@ -306,91 +321,104 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       Acc a;
 #pragma unroll
       for (int m = 0; m < 8; ++m) a.o[m][0] = a.o[m][1] = a.o[m][2] = a.o[m][3] = 0.f;
-      a.m[0] = a.m[1] = -INFINITY;
       a.l[0] = a.l[1] = 0.f;
+      float base0 = 0.f, base1 = 0.f;              // the running maxima
+      float pass0 = -INFINITY, pass1 = -INFINITY;  // scores beyond these move them; -inf: there is none yet
 
       for (; t < stop; ++t) {
-        cp_wait<STAGES - 2>();
+        cp_wait<STAGES - 1>();
         __syncwarp();
-        const uint8_t* tile = ring + slot * TILE_BYTES;
-        const bool ok = (there >> slot) & 1;
+        const uint8_t* step = ring + slot * STEP_BYTES;
+        const uint32_t ok = (there >> (2 * slot)) & 3u;
         const int key0 = (rg.first + (t - it.base)) * KEYS;
-        if (ok) {
-          const bool edge = key0 < rg.lo || key0 + KEYS > rg.hi;
-          // scores: keys g, g + 8 x heads 2c, 2c + 1
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-          {
-            const uint4 k0 = *reinterpret_cast<const uint4*>(tile + chunk_at(g >> 1, (g & 1) * 4 + c));
-            const uint4 k1 = *reinterpret_cast<const uint4*>(tile + chunk_at((g >> 1) + 4, (g & 1) * 4 + c));
-            const uint32_t s0 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(tile + KS_OFF + g * SROW + 2 * c));
-            const uint32_t s1 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(tile + KS_OFF + (g + 8) * SROW + 2 * c));
-            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+        const bool edge = key0 < rg.lo || key0 + KEYS > rg.hi || ok != 3u;
+        // scores: tile i, keys g, g + 8 x heads 2c, 2c + 1
+        float s[2][4];
+        uint32_t vs[2][2];  // scales of block g, keys (2c, 2c + 1) and (2c + 8, 2c + 9)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t sa = prmt(s0, s0, w < 2 ? 0x1010 : 0x3232), sb = prmt(s1, s1, w < 2 ? 0x1010 : 0x3232);
-              uint32_t x[4], y[4];
-              widen(w0[w], x);
-              widen(w1[w], y);
+        for (int i = 0; i < 2; ++i) {
+          const uint8_t* tile = step + i * TILE_BYTES;
+          s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(tile + chunk_at(g >> 1, (g & 1) * 4 + c));
+          const uint4 k1 = *reinterpret_cast<const uint4*>(tile + chunk_at((g >> 1) + 4, (g & 1) * 4 + c));
+          const uint32_t s0 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(tile + KS_OFF + g * SROW + 2 * c));
+          const uint32_t s1 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(tile + KS_OFF + (g + 8) * SROW + 2 * c));
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const uint32_t A[4] = {mul2(x[2 * j], sa), mul2(y[2 * j], sb), mul2(x[2 * j + 1], sa), mul2(y[2 * j + 1], sb)};
-                mma_16816_f16(s, A, qf + 2 * (2 * w + j));
-              }
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t sa = prmt(s0, s0, w < 2 ? 0x1010 : 0x3232), sb = prmt(s1, s1, w < 2 ? 0x1010 : 0x3232);
+            uint32_t x[4], y[4];
+            widen(w0[w], x);
+            widen(w1[w], y);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t A[4] = {mul2(x[2 * j], sa), mul2(y[2 * j], sb), mul2(x[2 * j + 1], sa), mul2(y[2 * j + 1], sb)};
+              mma_16816_f16(s[i], A, qf + 2 * (2 * w + j));
             }
           }
-          uint32_t vs0, vs1;  // scales of block g, keys (2c, 2c + 1) and (2c + 8, 2c + 9)
-          {
-            const uint8_t* p = tile + VS_OFF + 2 * c * SROW + g;
-            uint32_t b0 = p[0], b1 = p[SROW], b2 = p[8 * SROW], b3 = p[9 * SROW];
-            if (edge) {  // what is not seen counts as 0, also where it would be NaN
-              const int k = key0 + 2 * c;
-              b0 = k >= rg.lo && k < rg.hi ? b0 : 0;
-              b1 = k + 1 >= rg.lo && k + 1 < rg.hi ? b1 : 0;
-              b2 = k + 8 >= rg.lo && k + 8 < rg.hi ? b2 : 0;
-              b3 = k + 9 >= rg.lo && k + 9 < rg.hi ? b3 : 0;
-              const int ka = key0 + g, kb = ka + 8;
-              if (ka < rg.lo || ka >= rg.hi) s[0] = s[1] = -INFINITY;
-              if (kb < rg.lo || kb >= rg.hi) s[2] = s[3] = -INFINITY;
-            }
-            vs0 = e4m3x2_to_f16x2((uint16_t)(b0 | (b1 << 8)));
-            vs1 = e4m3x2_to_f16x2((uint16_t)(b2 | (b3 << 8)));
-          }
-          const float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
-          if (__any_sync(0xffffffffu, (x0 - a.m[0]) * fac[0] > 8.f || (x1 - a.m[1]) * fac[1] > 8.f)) {
-            float n0 = x0, n1 = x1;
+          const uint8_t* p = tile + VS_OFF + 2 * c * SROW + g;
+          vs[i][0] = p[0] | ((uint32_t)p[SROW] << 8);
+          vs[i][1] = p[8 * SROW] | ((uint32_t)p[9 * SROW] << 8);
+        }
+        if (edge) {  // what is not seen counts as 0, also where it would be NaN
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-              n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
-              n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
-            }
-            n0 = fmaxf(n0, a.m[0]);
-            n1 = fmaxf(n1, a.m[1]);
-            const float f0 = n0 == -INFINITY ? 1.f : fast_exp2((a.m[0] - n0) * fac[0]);
-            const float f1 = n1 == -INFINITY ? 1.f : fast_exp2((a.m[1] - n1) * fac[1]);
-            a.m[0] = n0;
-            a.m[1] = n1;
-            a.l[0] *= f0;
-            a.l[1] *= f1;
+          for (int i = 0; i < 2; ++i) {
+            const int k = key0 + i * TILE, hi = (ok >> i) & 1u ? rg.hi : 0;
+            auto seen = [&](int key) { return key >= rg.lo && key < hi; };
+            if (!seen(k + g)) s[i][0] = s[i][1] = -INFINITY;
+            if (!seen(k + g + 8)) s[i][2] = s[i][3] = -INFINITY;
 #pragma unroll
-            for (int m = 0; m < 8; ++m) {
-              a.o[m][0] *= f0;
-              a.o[m][1] *= f1;
-              a.o[m][2] *= f0;
-              a.o[m][3] *= f1;
+            for (int j = 0; j < 2; ++j) {
+              if (!seen(k + 2 * c + 8 * j)) vs[i][j] &= 0xFF00u;
+              if (!seen(k + 2 * c + 8 * j + 1)) vs[i][j] &= 0x00FFu;
             }
           }
-          const float m0 = a.m[0] == -INFINITY ? 0.f : a.m[0], m1 = a.m[1] == -INFINITY ? 0.f : a.m[1];
-          const float p0 = fast_exp2((s[0] - m0) * fac[0]), p1 = fast_exp2((s[1] - m1) * fac[1]);
-          const float p2 = fast_exp2((s[2] - m0) * fac[0]), p3 = fast_exp2((s[3] - m1) * fac[1]);
+        }
+        const float x0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
+        const float x1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+        if (__any_sync(0xffffffffu, x0 > pass0 || x1 > pass1)) {
+          float n0 = x0, n1 = x1;
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+          }
+          float f0 = 1.f, f1 = 1.f;
+          if (n0 > pass0) {
+            f0 = pass0 == -INFINITY ? 0.f : fast_exp2((base0 - n0) * fac[0]);
+            base0 = n0;
+            pass0 = n0 + 8.f / fac[0];
+          }
+          if (n1 > pass1) {
+            f1 = pass1 == -INFINITY ? 0.f : fast_exp2((base1 - n1) * fac[1]);
+            base1 = n1;
+            pass1 = n1 + 8.f / fac[1];
+          }
+          a.l[0] *= f0;
+          a.l[1] *= f1;
+#pragma unroll
+          for (int m = 0; m < 8; ++m) {
+            a.o[m][0] *= f0;
+            a.o[m][1] *= f1;
+            a.o[m][2] *= f0;
+            a.o[m][3] *= f1;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint8_t* tile = step + i * TILE_BYTES + V_OFF;
+          const float p0 = fast_exp2((s[i][0] - base0) * fac[0]), p1 = fast_exp2((s[i][1] - base1) * fac[1]);
+          const float p2 = fast_exp2((s[i][2] - base0) * fac[0]), p3 = fast_exp2((s[i][3] - base1) * fac[1]);
           a.l[0] += p0 + p2;
           a.l[1] += p1 + p3;
           const uint32_t pb[2] = {transpose8(pack_half2(p0, p1)), transpose8(pack_half2(p2, p3))};
+          const uint32_t vs0 = e4m3x2_to_f16x2((uint16_t)vs[i][0]), vs1 = e4m3x2_to_f16x2((uint16_t)vs[i][1]);
           // values: keys 2c, 2c + 1, 2c + 8, 2c + 9, block g
-          const int vch = (g >> 1), vin = (g & 1) * 8;
-          const uint2 va = *reinterpret_cast<const uint2*>(tile + V_OFF + chunk_at(c, vch) + vin);
-          const uint2 vb = *reinterpret_cast<const uint2*>(tile + V_OFF + chunk_at(c, 4 + vch) + vin);
-          const uint2 vc = *reinterpret_cast<const uint2*>(tile + V_OFF + chunk_at(c + 4, vch) + vin);
-          const uint2 vd = *reinterpret_cast<const uint2*>(tile + V_OFF + chunk_at(c + 4, 4 + vch) + vin);
+          const int vch = g >> 1, vin = (g & 1) * 8;
+          const uint2 va = *reinterpret_cast<const uint2*>(tile + chunk_at(c, vch) + vin);
+          const uint2 vb = *reinterpret_cast<const uint2*>(tile + chunk_at(c, 4 + vch) + vin);
+          const uint2 vc = *reinterpret_cast<const uint2*>(tile + chunk_at(c + 4, vch) + vin);
+          const uint2 vd = *reinterpret_cast<const uint2*>(tile + chunk_at(c + 4, 4 + vch) + vin);
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const uint32_t a0 = w ? va.y : va.x, b0 = w ? vb.y : vb.x, c0_ = w ? vc.y : vc.x, d0 = w ? vd.y : vd.x;
@@ -407,9 +435,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
             }
           }
         }
-        __syncwarp();  // every lane has read the slot before this one
-        load(slot == 0 ? STAGES - 1 : slot - 1);
-        slot = slot == STAGES - 1 ? 0 : slot + 1;
+        __syncwarp();  // every lane has read the slot
+        load(slot);
+        slot ^= 1;
       }
 
       // ---- the piece's end
@@ -448,7 +476,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
           for (int m = 0; m < 8; m += 2)
             *reinterpret_cast<float4*>(o + 2 * m) = make_float4(a.o[m][x], a.o[m][2 + x], a.o[m + 1][x], a.o[m + 1][2 + x]);
           if (g == 0) {
-            dst[HEADS * D + 2 * (2 * c + x)] = a.m[x] == -INFINITY ? -INFINITY : a.m[x] * fac[x];
+            const float top = x ? base1 : base0, pass = x ? pass1 : pass0;
+            dst[HEADS * D + 2 * (2 * c + x)] = pass == -INFINITY ? -INFINITY : top * fac[x];
             dst[HEADS * D + 2 * (2 * c + x) + 1] = a.l[x];
           }
         }
@@ -475,7 +504,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
     }
     auto piece = [&](int n) {
       const uint8_t* r = sm + (n >> 1) * WARP_SMEM;
-      return reinterpret_cast<const float*>(n & 1 ? r : r + STAGES * TILE_BYTES);
+      return reinterpret_cast<const float*>(n & 1 ? r : r + STAGES * STEP_BYTES);
     };
     float m = -INFINITY;
     for (int n = w; n <= last; n = ((n >> 1) + 1) * 2) m = fmaxf(m, piece(n)[HEADS * D + 2 * head]);
