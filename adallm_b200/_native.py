@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 
 import torch
 
@@ -89,6 +90,7 @@ _SIGS = {
                                    F32, F32, I32, P, INT, I64, I64, P, SZ, P]),
     "ada_kv4_paged_prefill": (INT, [P, INT, I64, I64, P, P, I64, I64, I64, P, I64, I32, P, P, I32, I64, I32, I32, I32,
                                     I32, I32, F32, F32, F32, I32, P, INT, I64, I64, P, P]),
+    "ada_call": (INT, [INT, C.c_char_p]),
     "ada_nvfp4_sf_bytes": (SZ, [I64, I64]),
     "ada_nvfp4_prepack_scales": (INT, [P, INT, I64, I64, I64, P, P]),
     "ada_nvfp4_linear_workspace_size": (SZ, [I64, I64, I64, INT]),
@@ -217,22 +219,43 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-def call(entry, device: torch.device, *args) -> int:
-    """entry(*args) with `device` current: a launch goes to the current device, its stream must be of it."""
-    if device.index == torch._C._cuda_getDevice():
-        return entry(*args)
-    with torch.cuda.device(device):
-        return entry(*args)
+class Packed:
+    """An entry called through ada_call: `pack` makes its arguments one buffer (ctypes takes longer to convert
+    them than the launch does), words as in the header, floats as doubles (`kinds`: q, or d where a float is)."""
+
+    def __init__(self, entry: int, kinds: str):
+        self.entry = entry
+        self.pack = struct.Struct("=" + kinds).pack
+        self._call = None
+
+    def __call__(self, device: int, *args) -> int:
+        """The entry's status.  A launch goes to the current device, and its stream must be of it."""
+        call = self._call
+        if call is None:
+            call = self._call = lib().ada_call
+        if device == _current_device():
+            return call(self.entry, self.pack(*args))
+        with torch.cuda.device(device):
+            return call(self.entry, self.pack(*args))
 
 
-def one_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    """The device that all tensors are on."""
-    device = first.device
-    if device.type != "cuda":
-        raise RuntimeError(f"{what} requires CUDA tensors")
-    for t in others:
-        if t is not None and t.device != device:
-            if not t.is_cuda:
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+step_metadata = Packed(1, "19q")
+rotary = Packed(2, "19q")
+kv4_store = Packed(3, "26q2d2q")
+kv4_read = Packed(4, "10q2d4q")
+kv4_paged_decode = Packed(5, "18q3d8q")
+kv4_paged_prefill = Packed(6, "21q3d7q")
+
+
+def one_device(what: str, *tensors: torch.Tensor) -> int:
+    """The index of the device that all tensors are on."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != device or device < 0:
+            if not all(t.is_cuda for t in tensors):
                 raise RuntimeError(f"{what} requires CUDA tensors")
             raise ValueError(f"{what}: all tensors must be on one device")
     return device

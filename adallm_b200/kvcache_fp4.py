@@ -15,7 +15,8 @@ import torch
 
 from . import _native as N
 
-I32 = torch.int32
+I32, U8 = torch.int32, torch.uint8
+LARGEST = 0x7FFFFFFF  # windows past any position
 HEAD_DIM = 128
 ROW_BYTES = 72
 
@@ -31,14 +32,15 @@ def empty_kvcache_fp4(num_pages: int, num_kv_heads: int, page_size: int, device=
 def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor):
     """(num_pages, KV heads, page size, page stride, head stride) of a cache."""
     shape, strides = k_cache.shape, k_cache.stride()
-    if k_cache.dtype is not torch.uint8 or v_cache.dtype is not torch.uint8:
+    if k_cache.dtype is not U8 or v_cache.dtype is not U8:
         raise ValueError("the 4-bit KV cache is held as uint8")
     if len(shape) != 3 or shape != v_cache.shape or strides != v_cache.stride() or strides[2] != 1:
         raise ValueError("k_cache and v_cache must share a [pages, Hkv, page * 72] layout")
-    page, rest = divmod(shape[2], ROW_BYTES)
-    if rest:
+    pages, hkv, block = shape
+    page = block // ROW_BYTES
+    if page * ROW_BYTES != block:
         raise ValueError("a block of the 4-bit KV cache has 72 bytes a row")
-    return shape[0], shape[1], page, strides[0], strides[1]
+    return pages, hkv, page, strides[0], strides[1]
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -55,29 +57,29 @@ def _slots(slot_mapping: torch.Tensor, tokens: int) -> torch.Tensor:
     return slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
 
 
-def _store(positions, query, key, value, cos_sin, k_cache, v_cache, slot_mapping, interleaved, k_scale, v_scale, q_out,
-           device):
+def _store(device, rotation, key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale):
+    """rotation: None, or (positions, query, cos_sin, interleaved, q_out)."""
     pages, hkv, page, s_page, s_head = _cache(k_cache, v_cache)
     key, value = _rows(key, "key"), _rows(value, "value")
-    tokens = key.shape[0]
-    code = N.DT.get(key.dtype)
-    if code is None or value.dtype is not key.dtype:
+    shape, ks, vs, dtype = key.shape, key.stride(), value.stride(), key.dtype
+    tokens = shape[0]
+    code = N.DT.get(dtype)
+    if code is None or value.dtype is not dtype:
         raise ValueError("key/value must be bf16 or fp16")
-    if key.shape != value.shape or key.shape[1] != hkv:
+    if shape != value.shape or shape[1] != hkv:
         raise ValueError("key and value must be [tokens, Hkv, 128] with the cache's heads")
     slots = _slots(slot_mapping, tokens)
-    ks, vs = key.stride(), value.stride()
-    if query is None:
-        q_args = (None, None, 0, 0)
-        hq, table_args = 0, (None, 0, 0, 0)
-    else:
-        qs = query.stride()
-        q_args = (positions.data_ptr(), query.data_ptr(), qs[0], qs[1])
+    pos = q = qs0 = qs1 = out = hq = table = reach = width = turn = 0
+    if rotation is not None:
+        positions, query, cos_sin, turn, q_out = rotation
+        pos, q, out, table = positions.data_ptr(), query.data_ptr(), q_out.data_ptr(), cos_sin.data_ptr()
+        qs0, qs1, _ = query.stride()
         hq = query.shape[1]
-        table_args = (cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[-1], interleaved)
-    st = N.call(N.lib().ada_kv4_store, device, *q_args, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1],
-                N.ptr(q_out), tokens, hq, hkv, HEAD_DIM, *table_args, slots.data_ptr(), k_cache.data_ptr(),
-                v_cache.data_ptr(), s_page, s_head, pages, page, k_scale, v_scale, code, N.stream_ptr(device))
+        size = cos_sin.shape
+        reach, width = size[0], size[-1]
+    st = N.kv4_store(device, pos, q, qs0, qs1, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], out, tokens,
+                     hq, hkv, HEAD_DIM, table, reach, width, turn, slots.data_ptr(), k_cache.data_ptr(),
+                     v_cache.data_ptr(), s_page, s_head, pages, page, k_scale, v_scale, code, N.raw_stream(device))
     if st:
         N.check(st, "store_kvcache_fp4")
 
@@ -90,7 +92,7 @@ def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     given twice holds a mix of both rows.  Of each 16 elements: scale = e4m3(max |x| / 6), codes = the nearest e2m1
     to x / scale; infinities saturate, a NaN makes its 16 elements read as NaN."""
     device = N.one_device("store_kvcache_fp4", key, value, k_cache, v_cache, slot_mapping)
-    _store(None, None, key, value, None, k_cache, v_cache, slot_mapping, False, k_scale, v_scale, None, device)
+    _store(device, None, key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
 
 
 def rotary_store_kvcache_fp4(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -102,10 +104,10 @@ def rotary_store_kvcache_fp4(positions: torch.Tensor, query: torch.Tensor, key: 
     query [T, Hq, 128], key/value [T, Hkv, 128]; the rest as in rotary_embedding.apply_rotary and
     store_kvcache_fp4.  Returns the rotated query (q_out, contiguous, if given)."""
     device = N.one_device("rotary_store_kvcache_fp4", key, query, value, positions, cos_sin_cache, k_cache, v_cache,
-                          slot_mapping, q_out)
+                          slot_mapping)
     query = _rows(query, "query")
-    shape = query.shape
-    if shape[0] != key.shape[0] or positions.numel() != shape[0] or query.dtype is not key.dtype:
+    shape, dtype = query.shape, query.dtype
+    if shape[0] != key.shape[0] or positions.numel() != shape[0] or dtype is not key.dtype:
         raise ValueError("positions, query and key must describe the same tokens in one type")
     if cos_sin_cache.dtype is not torch.float32 or not cos_sin_cache.is_contiguous():
         raise ValueError("cos_sin_cache must be contiguous fp32")
@@ -113,10 +115,10 @@ def rotary_store_kvcache_fp4(positions: torch.Tensor, query: torch.Tensor, key: 
         positions = positions.to(torch.int64).contiguous()
     if q_out is None:
         q_out = query.new_empty(shape)
-    elif q_out.shape != shape or q_out.dtype is not query.dtype or not q_out.is_contiguous():
-        raise ValueError("q_out must be contiguous with query's shape and type")
-    _store(positions, query, key, value, cos_sin_cache, k_cache, v_cache, slot_mapping, interleaved, k_scale, v_scale,
-           q_out, device)
+    elif q_out.shape != shape or q_out.dtype is not dtype or not q_out.is_contiguous() or q_out.get_device() != device:
+        raise ValueError("q_out must be contiguous with query's shape, type and device")
+    _store(device, (positions, query, cos_sin_cache, interleaved, q_out), key, value, k_cache, v_cache, slot_mapping,
+           k_scale, v_scale)
     return q_out
 
 
@@ -124,8 +126,7 @@ def read_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping:
                      dtype: torch.dtype = torch.bfloat16, k_scale: float = 1.0, v_scale: float = 1.0,
                      out: tuple | None = None) -> tuple:
     """The keys and values at the slots, [T, Hkv, 128] each in bf16/fp16; zeros for slots outside the cache."""
-    k_out, v_out = out if out is not None else (None, None)
-    device = N.one_device("read_kvcache_fp4", k_cache, v_cache, slot_mapping, k_out, v_out)
+    device = N.one_device("read_kvcache_fp4", k_cache, v_cache, slot_mapping)
     pages, hkv, page, s_page, s_head = _cache(k_cache, v_cache)
     code = N.DT.get(dtype)
     if code is None:
@@ -134,14 +135,15 @@ def read_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping:
     slots = _slots(slot_mapping, tokens)
     shape = (tokens, hkv, HEAD_DIM)
     if out is None:
-        k_out, v_out = torch.empty((2,) + shape, dtype=dtype, device=device).unbind(0)
+        k_out, v_out = torch.empty((2, tokens, hkv, HEAD_DIM), dtype=dtype, device=k_cache.device).unbind(0)
     else:
+        k_out, v_out = out
         for t in out:
-            if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
-                raise ValueError("out must be two contiguous [tokens, Hkv, 128] tensors of dtype")
-    st = N.call(N.lib().ada_kv4_read, device, k_cache.data_ptr(), v_cache.data_ptr(), s_page, s_head, pages, page, hkv,
-                HEAD_DIM, slots.data_ptr(), tokens, k_scale, v_scale, k_out.data_ptr(), v_out.data_ptr(), code,
-                N.stream_ptr(device))
+            if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != device:
+                raise ValueError("out must be two contiguous [tokens, Hkv, 128] tensors of dtype on the cache's device")
+    st = N.kv4_read(device, k_cache.data_ptr(), v_cache.data_ptr(), s_page, s_head, pages, page, hkv, HEAD_DIM,
+                    slots.data_ptr(), tokens, k_scale, v_scale, k_out.data_ptr(), v_out.data_ptr(), code,
+                    N.raw_stream(device))
     if st:
         N.check(st, "read_kvcache_fp4")
     return k_out, v_out
@@ -152,23 +154,23 @@ def paged_decode_fp4_workspace_bytes(batch: int, num_heads: int, num_kv_heads: i
     return int(N.lib().ada_kv4_paged_decode_workspace_size(batch, num_heads, num_kv_heads))
 
 
-def _attention(q, k_cache, v_cache, block_tables, out, *lists):
-    """Checks that decode and prefill share."""
-    layout = _cache(k_cache, v_cache)
+def _attention(device, q, block_tables, out, *lists):
+    """Checks that decode and prefill share: (q, its type's code, out, out's code)."""
     q = _rows(q, "q")
     code = N.DT.get(q.dtype)
-    if code is None or (out is not None and out.dtype not in N.DT):
-        raise ValueError("q and out must be bf16 or fp16")
+    if code is None:
+        raise ValueError("q must be bf16 or fp16")
     if block_tables.dtype is not I32 or block_tables.dim() != 2 or block_tables.stride(1) != 1:
         raise ValueError("block_tables must be int32 [sequences, pages] with unit stride")
-    for t, name in lists:
+    for t in lists:
         if t.dtype is not I32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be int32 with unit stride")
+            raise ValueError("context_lens, cu_seqlens_q and cu_seqlens_k must be int32 with unit stride")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.stride(2) != 1:
-        raise ValueError("out must have q's shape and unit stride in the head dimension")
-    return layout, q, code, out
+        return q, code, q.new_empty(q.shape), code
+    out_code = N.DT.get(out.dtype)
+    if out_code is None or out.shape != q.shape or out.stride(2) != 1 or out.get_device() != device:
+        raise ValueError("out must be bf16 or fp16 with q's shape and device and unit stride in the head dimension")
+    return q, code, out, out_code
 
 
 def paged_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -181,23 +183,29 @@ def paged_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     (ids outside the cache are masked); context_lens int32 [B], the new token included.  window W > 0: the last
     W tokens.  Returns [B, Hq, 128] in q.dtype; a sequence without keys gives zeros.  workspace: at
     least paged_decode_fp4_workspace_bytes(B, Hq, Hkv) bytes (default: allocated for the call)."""
-    device = N.one_device("paged_decode_fp4", q, k_cache, v_cache, block_tables, context_lens, out, workspace)
-    (pages, hkv, page, s_page, s_head), q, code, out = _attention(q, k_cache, v_cache, block_tables, out,
-                                                                  (context_lens, "context_lens"))
+    device = N.one_device("paged_decode_fp4", q, k_cache, v_cache, block_tables, context_lens)
+    pages, hkv, page, s_page, s_head = _cache(k_cache, v_cache)
+    q, code, out, out_code = _attention(device, q, block_tables, out, context_lens)
     batch, hq, d = q.shape
-    if context_lens.numel() != batch or block_tables.shape[0] != batch:
+    rows, max_pages = block_tables.shape
+    if context_lens.numel() != batch or rows != batch:
         raise ValueError("block_tables and context_lens must have one entry per sequence")
     if batch == 0:
         return out
     if workspace is None:
         # one of its own: the launches of another thread's call on this stream may fall between this call's
-        workspace = torch.empty(paged_decode_fp4_workspace_bytes(batch, hq, hkv), dtype=torch.uint8, device=device)
+        size = paged_decode_fp4_workspace_bytes(batch, hq, hkv)
+        workspace = k_cache.new_empty(size)
+    else:
+        size = workspace.nbytes
+        if workspace.get_device() != device or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous on q's device")
     qs, os = q.stride(), out.stride()
-    st = N.call(N.lib().ada_kv4_paged_decode, device, q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(),
-                v_cache.data_ptr(), s_page, s_head, pages, block_tables.data_ptr(), block_tables.stride(0),
-                block_tables.shape[1], context_lens.data_ptr(), batch, hq, hkv, d, page, scale, k_scale, v_scale,
-                min(int(window), 0x7FFFFFFF), out.data_ptr(), N.DT[out.dtype], os[0], os[1], workspace.data_ptr(),
-                workspace.nbytes, N.stream_ptr(device))
+    st = N.kv4_paged_decode(device, q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), s_page,
+                            s_head, pages, block_tables.data_ptr(), block_tables.stride(0), max_pages,
+                            context_lens.data_ptr(), batch, hq, hkv, d, page, scale, k_scale, v_scale,
+                            window if window < LARGEST else LARGEST, out.data_ptr(), out_code, os[0], os[1],
+                            workspace.data_ptr(), size, N.raw_stream(device))
     if st:
         N.check(st, "4-bit KV decode kernel")
     return out
@@ -213,24 +221,27 @@ def paged_prefill_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     sequence's cached prefix and new tokens; max_seqlen_q must be at least every sequence's new tokens.
     window W > 0: a row sees its own position and the W before it.  Rows behind the last sequence are left as
     they are in ``out`` (unset without it)."""
-    device = N.one_device("paged_prefill_fp4", q, k_cache, v_cache, block_tables, cu_seqlens_q, cu_seqlens_k, out, err)
-    (pages, hkv, page, s_page, s_head), q, code, out = _attention(q, k_cache, v_cache, block_tables, out,
-                                                                  (cu_seqlens_q, "cu_seqlens_q"),
-                                                                  (cu_seqlens_k, "cu_seqlens_k"))
+    device = N.one_device("paged_prefill_fp4", q, k_cache, v_cache, block_tables, cu_seqlens_q, cu_seqlens_k)
+    pages, hkv, page, s_page, s_head = _cache(k_cache, v_cache)
+    q, code, out, out_code = _attention(device, q, block_tables, out, cu_seqlens_q, cu_seqlens_k)
     total_q, hq, d = q.shape
+    rows, max_pages = block_tables.shape
     batch = cu_seqlens_q.numel() - 1
-    if cu_seqlens_k.numel() != batch + 1 or block_tables.shape[0] < batch:
+    if cu_seqlens_k.numel() != batch + 1 or rows < batch:
         raise ValueError("cu_seqlens_q, cu_seqlens_k and block_tables must describe the same sequences")
-    if err is not None and (err.dtype is not I32 or err.numel() != 1):
-        raise ValueError("err must be one int32")
+    word = 0
+    if err is not None:
+        if err.dtype is not I32 or err.numel() != 1 or err.get_device() != device:
+            raise ValueError("err must be one int32 on q's device")
+        word = err.data_ptr()
     if total_q == 0 or batch <= 0:
         return out
     qs, os = q.stride(), out.stride()
-    st = N.call(N.lib().ada_kv4_paged_prefill, device, q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(),
-                v_cache.data_ptr(), s_page, s_head, pages, block_tables.data_ptr(), block_tables.stride(0),
-                block_tables.shape[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch, total_q,
-                int(max_seqlen_q), hq, hkv, d, page, scale, k_scale, v_scale, min(int(window), 0x7FFFFFFF),
-                out.data_ptr(), N.DT[out.dtype], os[0], os[1], N.ptr(err), N.stream_ptr(device))
+    st = N.kv4_paged_prefill(device, q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), s_page,
+                             s_head, pages, block_tables.data_ptr(), block_tables.stride(0), max_pages,
+                             cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch, total_q, max_seqlen_q, hq, hkv, d,
+                             page, scale, k_scale, v_scale, window if window < LARGEST else LARGEST, out.data_ptr(),
+                             out_code, os[0], os[1], word, N.raw_stream(device))
     if st:
         N.check(st, "4-bit KV prefill kernel")
     return out

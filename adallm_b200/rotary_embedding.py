@@ -89,17 +89,22 @@ def apply_rotary(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor
     positions [T] (clamped to the table); query [T, Hq, D], key [T, Hkv, D] bf16/fp16, any strides over tokens and
     heads that are multiples of 8; cos_sin_cache fp32 [max_position, (1,) r] = [cos | sin] of r / 2 pairs.  Pairs are
     (i, i + r / 2), or (2i, 2i + 1) with interleaved.  Returns new contiguous tensors (q_out, k_out if given)."""
-    device = N.one_device("rotary_embedding", query, positions, key, cos_sin_cache, q_out, k_out)
-    code = N.DT.get(query.dtype)
-    if code is None or key.dtype is not query.dtype:
+    device = N.one_device("rotary_embedding", query, positions, key, cos_sin_cache)
+    dtype = query.dtype
+    code = N.DT.get(dtype)
+    if code is None or key.dtype is not dtype:
         raise ValueError("rotary embedding expects bf16/fp16 q and k")
     if query.dim() != 3 or key.dim() != 3:
         raise ValueError("query and key must be [tokens, heads, head size]")
-    if query.stride(2) != 1:
+    qs, ks = query.stride(), key.stride()
+    if qs[2] != 1:
         query = query.contiguous()
-    if key.stride(2) != 1:
+        qs = query.stride()
+    if ks[2] != 1:
         key = key.contiguous()
-    (t, hq, d), (tk, hk, dk) = query.shape, key.shape
+        ks = key.stride()
+    t, hq, d = q_shape = query.shape
+    tk, hk, dk = k_shape = key.shape
     if tk != t or positions.numel() != t or dk != d:
         raise ValueError("positions, query and key must describe the same tokens")
     if cos_sin_cache.dtype is not torch.float32 or not cos_sin_cache.is_contiguous():
@@ -107,16 +112,19 @@ def apply_rotary(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor
     if positions.dtype is not torch.int64 or not positions.is_contiguous():
         positions = positions.to(torch.int64).contiguous()
     if q_out is None:
-        q_out = query.new_empty((t, hq, d))
+        q_out = query.new_empty(q_shape)
+    elif q_out.shape != q_shape or q_out.dtype is not dtype or not q_out.is_contiguous() \
+            or q_out.get_device() != device:
+        raise ValueError("q_out must be contiguous with query's shape, type and device")
     if k_out is None:
-        k_out = key.new_empty((t, hk, d))
-    for o, x in ((q_out, query), (k_out, key)):
-        if o.shape != x.shape or o.dtype is not x.dtype or not o.is_contiguous():
-            raise ValueError("q_out and k_out must be contiguous with their input's shape and type")
-    qs, ks = query.stride(), key.stride()
-    st = N.call(N.lib().ada_rotary, device, positions.data_ptr(), query.data_ptr(), qs[0], qs[1], key.data_ptr(), ks[0],
-                ks[1], q_out.data_ptr(), k_out.data_ptr(), t, hq, hk, d, cos_sin_cache.data_ptr(),
-                cos_sin_cache.shape[0], cos_sin_cache.shape[-1], interleaved, code, N.stream_ptr(device))
+        k_out = key.new_empty(k_shape)
+    elif k_out.shape != k_shape or k_out.dtype is not dtype or not k_out.is_contiguous() \
+            or k_out.get_device() != device:
+        raise ValueError("k_out must be contiguous with key's shape, type and device")
+    table = cos_sin_cache.shape
+    st = N.rotary(device, positions.data_ptr(), query.data_ptr(), qs[0], qs[1], key.data_ptr(), ks[0], ks[1],
+                  q_out.data_ptr(), k_out.data_ptr(), t, hq, hk, d, cos_sin_cache.data_ptr(), table[0], table[-1],
+                  interleaved, code, N.raw_stream(device))
     if st:
         N.check(st, "rotary_embedding")
     return q_out, k_out

@@ -45,11 +45,11 @@ def step_metadata(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     gets slot -1.  err: optional int32 [1] device word; 0x100 (free list), 0x200 (table) and 0x400 (more
     tokens than num_tokens) are OR-ed in.  The inputs, block_tables apart, are left as they are: for the
     next step copy free_next to free_start and context_lens to cached_lens.  At most 8192 requests."""
-    device = N.one_device("step_metadata", cached_lens, new_lens, block_tables, free_pages, free_start, err)
-    for t, name in ((cached_lens, "cached_lens"), (new_lens, "new_lens"), (free_pages, "free_pages"),
-                    (free_start, "free_start")):
+    tensors = (cached_lens, new_lens, free_pages, free_start)
+    device = N.one_device("step_metadata", *tensors, block_tables)
+    for t in tensors:
         if t.dtype is not I32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be int32 with unit stride")
+            raise ValueError("cached_lens, new_lens, free_pages and free_start must be int32 with unit stride")
     requests = cached_lens.numel()
     if new_lens.numel() != requests or free_start.numel() != 1:
         raise ValueError("cached_lens and new_lens must have one entry per request, free_start one")
@@ -60,24 +60,27 @@ def step_metadata(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table
         raise ValueError("block_tables must have one row of unit stride per request")
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
-    if err is not None and (err.dtype is not I32 or err.numel() != 1):
-        raise ValueError("err must be one int32")
+    word = 0
+    if err is not None:
+        N.one_device("step_metadata", err, cached_lens)
+        if err.dtype is not I32 or err.numel() != 1:
+            raise ValueError("err must be one int32")
+        word = err.data_ptr()
     if out is None:
-        out = empty_step_metadata(requests, num_tokens, device)
+        out = empty_step_metadata(requests, num_tokens, cached_lens.device)
     else:
         if type(out) is not StepMetadata:
             out = StepMetadata(*out)
-        want = (num_tokens, num_tokens, requests + 1, requests + 1, requests, 1)
-        for t, n, name in zip(out, want, StepMetadata._fields):
-            if (t.numel() != n or t.dtype is not (torch.int64 if name == "positions" else I32)
-                    or not t.is_contiguous() or t.device != device):
-                raise ValueError(f"out.{name} must have {n} contiguous entries of its type on the inputs' device")
+        for t, n in zip(out, (num_tokens, num_tokens, requests + 1, requests + 1, requests, 1)):
+            if t.numel() != n or t.dtype is not (I32 if t is not out[0] else torch.int64) or not t.is_contiguous() \
+                    or t.get_device() != device:
+                raise ValueError("out must hold contiguous tensors as empty_step_metadata makes them")
     positions, slots, cu_q, cu_k, context, free_next = out
-    st = N.call(N.lib().ada_step_metadata, device, cached_lens.data_ptr(), new_lens.data_ptr(), requests,
-                block_tables.data_ptr(), max(row_stride, max_pages), max_pages, free_pages.data_ptr(),
-                free_pages.numel(), free_start.data_ptr(), page_size, num_tokens, positions.data_ptr(),
-                slots.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), context.data_ptr(), free_next.data_ptr(),
-                N.ptr(err), N.stream_ptr(device))
+    st = N.step_metadata(device, cached_lens.data_ptr(), new_lens.data_ptr(), requests, block_tables.data_ptr(),
+                         row_stride if row_stride > max_pages else max_pages, max_pages, free_pages.data_ptr(),
+                         free_pages.numel(), free_start.data_ptr(), page_size, num_tokens, positions.data_ptr(),
+                         slots.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), context.data_ptr(), free_next.data_ptr(),
+                         word, N.raw_stream(device))
     if st:
         N.check(st, "step_metadata")
     return out

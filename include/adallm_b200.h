@@ -756,6 +756,22 @@ ADA_API int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t
                                   float scale, float k_scale, float v_scale, int32_t window, void* out, int out_dtype,
                                   int64_t out_stride_t, int64_t out_stride_h, unsigned int* err, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The six entries above with their arguments as one array
+ * args: the entry's arguments in order, a 64-bit word each: pointers and integers as they are, floats as the
+ * bits of a double.  For bindings whose cost goes by the number of arguments.  A 32-bit argument out
+ * of its range gives ADA_ERR_UNSUPPORTED, an unknown entry ADA_ERR_INVALID_ARG; the rest is the entry's own.
+ * ---------------------------------------------------------------------- */
+enum {
+  ADA_CALL_STEP_METADATA = 1,
+  ADA_CALL_ROTARY = 2,
+  ADA_CALL_KV4_STORE = 3,
+  ADA_CALL_KV4_READ = 4,
+  ADA_CALL_KV4_PAGED_DECODE = 5,
+  ADA_CALL_KV4_PAGED_PREFILL = 6
+};
+ADA_API int ada_call(int entry, const int64_t* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -108,6 +108,28 @@ def test_metadata_refusals(lib):
         (dict(t=1 << 31), UNSUP)])
 
 
+def test_packed_calls_are_the_entries_themselves(lib):
+    """Every entry's refusals come back the same through ada_call, argument by argument."""
+    store = dict(STORE)
+    cases = [(N.kv4_paged_decode, lib.ada_kv4_paged_decode, DECODE), (N.kv4_paged_prefill, lib.ada_kv4_paged_prefill, PREFILL),
+             (N.kv4_store, lib.ada_kv4_store, store)]
+    for packed, entry, good in cases:
+        assert len(good) == len(entry.argtypes)
+        for name in good:
+            for value in (-1, 0, 3, 7.5 if isinstance(good[name], float) else 1 << 40):
+                change = {**good, name: value}
+                if value == 1 << 40 and entry.argtypes[list(good).index(name)] in (N.I32, N.INT):
+                    assert lib.ada_call(packed.entry, packed.pack(*(v or 0 for v in change.values()))) == UNSUP
+                    continue
+                if isinstance(good[name], float):
+                    value = change[name] = float(value)
+                change["page"] = 20  # (no call is good, but for those that have nothing to do)
+                want = entry(*change.values())
+                assert lib.ada_call(packed.entry, packed.pack(*(v or 0 for v in change.values()))) == want, (name, value)
+    assert lib.ada_call(0, b"\0" * 300) == BAD and lib.ada_call(7, b"\0" * 300) == BAD
+    assert lib.ada_call(1, None) == BAD
+
+
 def test_cpu_tensors_are_refused():
     k, v = kv.empty_kvcache_fp4(2, 2, 16)
     q = torch.zeros((1, 4, 128), dtype=torch.bfloat16)
