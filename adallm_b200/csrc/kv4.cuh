@@ -21,40 +21,81 @@ constexpr int SROW = D / BLOCK;     // bytes of scales a row
 constexpr int ROW_BYTES = ROW + SROW;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// Largest scale's worth of elements; what lies beyond saturates (infinities too).
-constexpr float LIMIT = 2.f * 6.f * 448.f;
-
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
+// x / d given r near 1 / d: one correction step.  Correctly rounded where x / d lies further than 2^-44 of
+// itself from a midpoint of fp32 or on none: for divisors of few bits (6; the e4m3 scales) always (2^-27 and
+// more), for others but for one quotient in 2^20, which is one step (2^-24) off then.
+__device__ __forceinline__ float quotient(float x, float d, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-q, d, x), r, q);
+}
+
+// The same where x may be an infinity or the quotient one.
+__device__ __forceinline__ float any_quotient(float x, float d, float r) {
+  const float q = x * r;
+  return fabsf(q) == INFINITY ? q : fmaf(fmaf(-q, d, x), r, q);
+}
+
 // e4m3 byte of max|x| / 6, saturated to 448; NaN when the block holds one (the block then reads as NaN).
 __device__ __forceinline__ uint32_t scale_code(float top) {
-  return f32x2_to_e4m3x2(__fdiv_rn(top, 6.f), 0.f) & 0xFFu;
+  return f32x2_to_e4m3x2(any_quotient(top, 6.f, 1.f / 6.f), 0.f) & 0xFFu;
 }
 __device__ __forceinline__ float scale_value(uint32_t code) {
   const uint32_t h = e4m3x2_to_f16x2((uint16_t)code);
   return __half2float(__ushort_as_half((unsigned short)(h & 0xFFFFu)));
 }
 
-// Eight elements -> eight codes: the nearest e2m1 to x / s, ties to even.  r = RN(1 / s); one
-// correction step makes q the correctly rounded fp32 quotient (s has 4 significant bits, x at most
-// 24, so a quotient that is not a midpoint of fp32 lies 2^-27 or more away from one, and the
-// step's own error is below 2^-45).  x * r alone puts exact ties, which bf16 values often are, on
-// either side.  A block whose scale is 0 (all below 2^-10 * 6) holds zeros.
-__device__ __forceinline__ uint32_t codes8(const float* x, float s) {
+// Eight elements -> eight codes: the nearest e2m1 to x / s, ties to even.  x * (1 / s) alone puts exact
+// ties, which bf16 values often are, on either side; the quotient is the correctly rounded one.  A block
+// whose scale is 0 (all below 2^-10 * 6) holds zeros.  top: the block's max |x|.
+__device__ __forceinline__ uint32_t codes8(float* x, float s, float top) {
   if (!(s > 0.f)) return 0u;
-  const float r = __frcp_rn(s);
+  if (top == INFINITY) {  // infinities saturate like the largest floats (inf - inf would not)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -3.4028234663852886e38f), 3.4028234663852886e38f);
+  }
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   float q[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = fminf(fmaxf(x[i], -LIMIT), LIMIT);
-    const float q0 = v * r;
-    q[i] = fmaf(fmaf(-q0, s, v), r, q0);
-  }
+  for (int i = 0; i < 8; ++i) q[i] = quotient(x[i], s, r);
   return f32x8_to_e2m1x8(q);
+}
+// Eight codes -> their values, four f16x2 (low half = even element).
+__device__ __forceinline__ void widen8(uint32_t w, uint32_t* h) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// A scale's value in both halves.
+__device__ __forceinline__ uint32_t scale_f16x2(uint32_t e4m3) {
+  const uint32_t h = e4m3x2_to_f16x2((uint16_t)e4m3);
+  return prmt(h, h, 0x1010);
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // A query row enters the products multiplied by a power of two that brings its largest magnitude
@@ -72,6 +113,25 @@ __device__ __forceinline__ float score_factor(float scale_log2, int exponent) {
   return fmaxf(fminf(scale_log2 * pow2(-exponent), 1.2379400392853803e27f), 1e-36f);
 }
 
+// Two floats in one register pair: the packed fp32 operations round each half like the single ones.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 inline bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 // Checks of a cache's layout that every entry shares.

@@ -100,31 +100,6 @@ __device__ __forceinline__ Item item_of(const int* cum, int batch, int items, in
   return {lo, h, base, base + n};
 }
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// Four bytes of two codes each -> four f16x2.
-__device__ __forceinline__ void widen(uint32_t w, uint32_t* h) {
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-      : "r"(w));
-}
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -348,11 +323,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
           for (int w = 0; w < 4; ++w) {
             const uint32_t sa = prmt(s0, s0, w < 2 ? 0x1010 : 0x3232), sb = prmt(s1, s1, w < 2 ? 0x1010 : 0x3232);
             uint32_t x[4], y[4];
-            widen(w0[w], x);
-            widen(w1[w], y);
+            widen8(w0[w], x);
+            widen8(w1[w], y);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const uint32_t A[4] = {mul2(x[2 * j], sa), mul2(y[2 * j], sb), mul2(x[2 * j + 1], sa), mul2(y[2 * j + 1], sb)};
+              const uint32_t A[4] = {mul_f16x2(x[2 * j], sa), mul_f16x2(y[2 * j], sb), mul_f16x2(x[2 * j + 1], sa), mul_f16x2(y[2 * j + 1], sb)};
               mma_16816_f16(s[i], A, qf + 2 * (2 * w + j));
             }
           }
@@ -424,13 +399,13 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
             const uint32_t a0 = w ? va.y : va.x, b0 = w ? vb.y : vb.x, c0_ = w ? vc.y : vc.x, d0 = w ? vd.y : vd.x;
             constexpr uint32_t LO = 0x0F0F0F0Fu;
             uint32_t e0[4], e1[4], f0[4], f1[4];  // (even, odd) elements of the first and second key pair
-            widen((a0 & LO) | ((b0 << 4) & ~LO), e0);
-            widen(((a0 >> 4) & LO) | (b0 & ~LO), e1);
-            widen((c0_ & LO) | ((d0 << 4) & ~LO), f0);
-            widen(((c0_ >> 4) & LO) | (d0 & ~LO), f1);
+            widen8((a0 & LO) | ((b0 << 4) & ~LO), e0);
+            widen8(((a0 >> 4) & LO) | (b0 & ~LO), e1);
+            widen8((c0_ & LO) | ((d0 << 4) & ~LO), f0);
+            widen8(((c0_ >> 4) & LO) | (d0 & ~LO), f1);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const uint32_t A[4] = {mul2(e0[j], vs0), mul2(e1[j], vs0), mul2(f0[j], vs1), mul2(f1[j], vs1)};
+              const uint32_t A[4] = {mul_f16x2(e0[j], vs0), mul_f16x2(e1[j], vs0), mul_f16x2(f0[j], vs1), mul_f16x2(f1[j], vs1)};
               mma_16816_f16(a.o[4 * w + j], A, pb);
             }
           }

@@ -100,55 +100,16 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t* r) {
       : "r"(taddr), "r"(taddr + 32)
       : "memory");
 }
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t mul2h(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-// Eight codes -> four f16x2 (low half = even element).
-__device__ __forceinline__ void widen8(uint32_t w, uint32_t* h) {
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-      : "r"(w));
-}
 // 16 codes times their scale as 16 f16 (two chunks).
 __device__ __forceinline__ void widen16(uint2 codes, uint32_t scale2, uint4& lo, uint4& hi) {
   uint32_t h[8];
   widen8(codes.x, h);
   widen8(codes.y, h + 4);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = mul2h(h[i], scale2);
+  for (int i = 0; i < 8; ++i) h[i] = mul_f16x2(h[i], scale2);
   lo = make_uint4(h[0], h[1], h[2], h[3]);
   hi = make_uint4(h[4], h[5], h[6], h[7]);
 }
-__device__ __forceinline__ uint32_t both_halves(uint32_t e4m3) {
-  const uint32_t h = e4m3x2_to_f16x2((uint16_t)e4m3);
-  return prmt(h, h, 0x1010);
-}
-
 // Keys [lo, hi) that new token t of a sequence sees.
 __device__ __forceinline__ void key_range(const Params& P, int t, int off, int len_k, int& lo, int& hi) {
   hi = min(len_k, t + off + 1);
@@ -366,10 +327,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         uint4 lo, hi;
         const int c0 = ((blk & 3) * 2) ^ (key & 7), c1 = c0 ^ 1;
         const int at = kb * 16384 + (blk >> 2) * 8192 + key * 128;
-        widen16(kc, both_halves(ks), lo, hi);
+        widen16(kc, scale_f16x2(ks), lo, hi);
         *reinterpret_cast<uint4*>(kf + at + (c0 << 4)) = lo;
         *reinterpret_cast<uint4*>(kf + at + (c1 << 4)) = hi;
-        widen16(vc, both_halves(vs), lo, hi);
+        widen16(vc, scale_f16x2(vs), lo, hi);
         *reinterpret_cast<uint4*>(vf + at + (c0 << 4)) = lo;
         *reinterpret_cast<uint4*>(vf + at + (c1 << 4)) = hi;
       }

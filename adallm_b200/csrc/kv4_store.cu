@@ -22,108 +22,204 @@ struct RotaryParams {
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // token, head strides (elements)
   void *q_out, *k_out;                         // contiguous [T, heads, D]; k_out may be null
   int hq, hk, hv, d;                           // heads of each (hv = 0: no values), head size
+  int64_t tokens;
   // store (null cache: none)
   uint8_t *kc, *vc;
   int64_t s_page, s_head;
   const int32_t* slots;
   int64_t num_slots;
   int page;
-  float k_scale, v_scale;
+  float k_scale, v_scale, k_inv, v_inv;
 };
 
-// One CTA per (token, y-th share of the heads).  A thread keeps one chunk of 8 elements (16 bytes)
-// and walks the heads, so a token's cos and sin are read once per thread.
-template <typename T>
-__global__ void __launch_bounds__(256) rotary_store_kernel(RotaryParams P) {
+// A thread's unit is two chunks of 8 elements (16 bytes each) whose pairs lie within it: chunks i and
+// i + r/16 of the turned part (half layout), or neighbours; it keeps U heads (blockIdx.y's share) and walks
+// the tokens, so what belongs to a head is worked out once.  Rows and table entries of the next
+// STAGES - 1 tokens are on their way by cp.async, each thread's rows into places of its own: with a token
+// at a time, or one ahead in registers, an SM has 20-40 KB in flight where HBM wants 66 (95 us
+// instead of 66 for 16,381 tokens of 40 heads).
+// (one head with the store, whose arithmetic needs the registers)
+constexpr int heads_a_thread(bool store) { return store ? 1 : 2; }
+constexpr int STAGES = 4;
+// Bytes of a stage: the CTA's rows, then the table's row.
+__host__ __device__ constexpr int stage_bytes(int threads, int heads, int rot) { return threads * heads * 32 + rot * 4; }
+
+template <typename T, bool STORE>
+__global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_constant__ RotaryParams P) {
+  constexpr int U = heads_a_thread(STORE);
+  extern __shared__ __align__(16) uint8_t sm[];
   pdl_wait();
   pdl_trigger();
-  const int chunks = P.d >> 3;
-  const int lanes = blockDim.x / chunks;  // heads side by side
-  const int c = threadIdx.x % chunks, e0 = 8 * c;
-  const int64_t t = blockIdx.x;
-  const int half = P.rot >> 1;
-  const bool turned = P.pos != nullptr && e0 < P.rot;
-  const bool second = !P.interleaved && e0 >= half;
-  const int other = second ? e0 - half : e0 + half;  // the partners' chunk (half layout)
-  float cs[8], sn[8];
-  if (turned) {
-    const int64_t p = min(max(__ldg(P.pos + t), (int64_t)0), P.max_pos - 1);
-    const float* row = P.table + p * P.rot;
-    if (P.interleaved) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cs[i] = __ldg(row + e0 / 2 + i);
-        sn[i] = __ldg(row + half + e0 / 2 + i);
+  const int units = P.d >> 4;
+  const int lanes = blockDim.x / units;  // heads side by side
+  const int hl = (int)threadIdx.x / units, unit = (int)threadIdx.x - hl * units;
+  const int half = P.rot >> 1, rc = P.rot >> 3;
+  const bool turned = P.pos != nullptr && 16 * unit < P.rot;
+  const bool apart = turned && !P.interleaved;  // the unit's chunks are half the turned part apart
+  const int c0 = apart ? unit : 2 * unit, c1 = apart ? unit + (rc >> 1) : 2 * unit + 1;
+  const int step = 8 * (c1 - c0);
+  const int pair0 = apart ? 8 * c0 : 8 * unit;          // the unit's 8 pairs
+  // chunk c's neighbour in its block of 16 (c ^ 1): the lane that holds it, and as which of its two
+  int lane0 = 0, lane1 = 0;
+  bool one0 = false, one1 = false;
+  if (STORE) {
+    const int base = (int)(threadIdx.x & 31) - unit;  // (8 units a head: a head's lanes are in one warp)
+    auto find = [&](int c, int& lane, bool& one) {
+      if (P.pos && !P.interleaved && c < rc) {
+        one = c >= (rc >> 1);
+        lane = base + (one ? c - (rc >> 1) : c);
+      } else {
+        one = c & 1;
+        lane = base + (c >> 1);
       }
-    } else {
-      const int j = second ? other : e0;
+    };
+    find(c0 ^ 1, lane0, one0);
+    find(c1 ^ 1, lane1, one1);
+  }
+  // the thread's heads
+  const T* src[U];
+  T* dst[U];
+  int64_t src_st[U], dst_st[U];
+  uint8_t* cache[U];
+  bool turn[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        cs[i] = __ldg(row + j + i);
-        sn[i] = __ldg(row + half + j + i);
-      }
+  for (int u = 0; u < U; ++u) {
+    const int h = (int)blockIdx.y * (U * lanes) + u * lanes + hl;
+    src[u] = nullptr;
+    dst[u] = nullptr;
+    cache[u] = nullptr;
+    src_st[u] = dst_st[u] = 0;
+    turn[u] = false;
+    if (h < P.hq) {
+      src[u] = reinterpret_cast<const T*>(P.q) + h * P.q_sh + 8 * c0;
+      dst[u] = reinterpret_cast<T*>(P.q_out) + (int64_t)h * P.d + 8 * c0;
+      src_st[u] = P.q_st;
+      dst_st[u] = (int64_t)P.hq * P.d;
+      turn[u] = turned;
+    } else if (h < P.hq + P.hk) {
+      const int n = h - P.hq;
+      src[u] = reinterpret_cast<const T*>(P.k) + n * P.k_sh + 8 * c0;
+      if (P.k_out) dst[u] = reinterpret_cast<T*>(P.k_out) + (int64_t)n * P.d + 8 * c0;
+      src_st[u] = P.k_st;
+      dst_st[u] = (int64_t)P.hk * P.d;
+      turn[u] = turned;
+      if (STORE) cache[u] = P.kc + n * P.s_head;
+    } else if (h < P.hq + P.hk + P.hv) {
+      const int n = h - P.hq - P.hk;
+      src[u] = reinterpret_cast<const T*>(P.v) + n * P.v_sh + 8 * c0;
+      src_st[u] = P.v_st;
+      if (STORE) cache[u] = P.vc + n * P.s_head;
     }
   }
-  int64_t slot = -1;
-  if (P.kc) slot = __ldg(P.slots + t);
-  const bool store = slot >= 0 && slot < P.num_slots;
-  const int64_t block = store ? slot / P.page : 0;
-  const int srow = store ? (int)(slot - block * P.page) : 0;
-  const int heads = P.hq + P.hk + P.hv;
-  for (int h0 = blockIdx.y * lanes; h0 < heads; h0 += gridDim.y * lanes) {
-    const int h = h0 + (int)threadIdx.x / chunks;
-    const bool there = h < heads;
-    const bool is_q = h < P.hq, is_v = h >= P.hq + P.hk;
-    const int head = is_q ? h : is_v ? h - P.hq - P.hk : h - P.hq;
-    float y[8];
-    if (there) {
-      const T* src = is_q   ? reinterpret_cast<const T*>(P.q) + t * P.q_st + head * P.q_sh
-                     : is_v ? reinterpret_cast<const T*>(P.v) + t * P.v_st + head * P.v_sh
-                            : reinterpret_cast<const T*>(P.k) + t * P.k_st + head * P.k_sh;
-      uint4 own = *reinterpret_cast<const uint4*>(src + e0);
-      if (turned && !is_v) {
-        float x[8];
-        unpack8<T>(own, x);
+
+  const unsigned tokens = (unsigned)P.tokens;
+  const int stage = stage_bytes(blockDim.x, U, P.rot), rows = blockDim.x * U * 32;
+  const int lines = P.pos ? P.rot >> 2 : 0;  // 16-byte pieces of a table row
+  // the token whose rows are fetched next, and its position
+  unsigned ft = blockIdx.x;
+  auto place = [&](unsigned t) { return lines && t < tokens ? __ldg(P.pos + t) : (int64_t)0; };
+  int64_t fpos = place(ft);
+  auto fetch = [&](int s) {
+    if (ft < tokens) {
+      const uint32_t at = smem_addr(sm) + s * stage + threadIdx.x * 16;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (src[u]) {
+          const T* p = src[u] + ft * src_st[u];
+          cp16(at + (2 * u) * blockDim.x * 16, p);
+          cp16(at + (2 * u + 1) * blockDim.x * 16, p + step);
+        }
+      }
+      const float* row = P.table + min(max(fpos, (int64_t)0), P.max_pos - 1) * P.rot;
+      for (int i = threadIdx.x; i < lines; i += blockDim.x) cp16(smem_addr(sm) + s * stage + rows + 16 * i, row + 4 * i);
+      ft += gridDim.x;
+      fpos = place(ft);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+  int s = 0;
+  int slot = -1;
+  if (STORE && blockIdx.x < tokens) slot = __ldg(P.slots + blockIdx.x);
+  for (unsigned t = blockIdx.x; t < tokens; t += gridDim.x) {
+    const bool store = STORE && slot >= 0 && slot < P.num_slots;
+    const int page = store ? (int)((unsigned)slot / (unsigned)P.page) : 0;
+    const int srow = store ? slot - page * P.page : 0;
+    if (STORE && t + gridDim.x < tokens) slot = __ldg(P.slots + t + gridDim.x);
+    cp_wait<STAGES - 2>();
+    __syncthreads();  // every thread's part of the table row is there, and the stage before is read
+    fetch(s == 0 ? STAGES - 1 : s - 1);
+    const uint8_t* mine = sm + s * stage + threadIdx.x * 16;
+    float cs[8], sn[8];
+    if (turned) {
+      const float* row = reinterpret_cast<const float*>(sm + s * stage + rows) + pair0;
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        *reinterpret_cast<float4*>(cs + i) = *reinterpret_cast<const float4*>(row + i);
+        *reinterpret_cast<float4*>(sn + i) = *reinterpret_cast<const float4*>(row + half + i);
+      }
+    }
+    s = s == STAGES - 1 ? 0 : s + 1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!src[u]) continue;
+      uint4 o0 = *reinterpret_cast<const uint4*>(mine + (2 * u) * blockDim.x * 16);
+      uint4 o1 = *reinterpret_cast<const uint4*>(mine + (2 * u + 1) * blockDim.x * 16);
+      if (turn[u]) {
+        float x[8], z[8], y[8], w[8];
+        unpack8<T>(o0, x);
+        unpack8<T>(o1, z);
+        // single operations: joined to fused ones, or packed (which the compiler joins), they round differently
         if (P.interleaved) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             y[2 * i] = __fsub_rn(__fmul_rn(x[2 * i], cs[i]), __fmul_rn(x[2 * i + 1], sn[i]));
             y[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i + 1], cs[i]), __fmul_rn(x[2 * i], sn[i]));
+            w[2 * i] = __fsub_rn(__fmul_rn(z[2 * i], cs[4 + i]), __fmul_rn(z[2 * i + 1], sn[4 + i]));
+            w[2 * i + 1] = __fadd_rn(__fmul_rn(z[2 * i + 1], cs[4 + i]), __fmul_rn(z[2 * i], sn[4 + i]));
           }
         } else {
-          float z[8];
-          unpack8<T>(*reinterpret_cast<const uint4*>(src + other), z);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            y[i] = second ? __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(z[i], sn[i]))
-                          : __fsub_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(z[i], sn[i]));
+          for (int i = 0; i < 8; ++i) {
+            y[i] = __fsub_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(z[i], sn[i]));
+            w[i] = __fadd_rn(__fmul_rn(z[i], cs[i]), __fmul_rn(x[i], sn[i]));
+          }
         }
-        own = pack8<T>(y);
+        o0 = pack8<T>(y);
+        o1 = pack8<T>(w);
       }
-      if (is_q) {
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(P.q_out) + (t * P.hq + head) * P.d + e0) = own;
-      } else if (!is_v && P.k_out) {
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(P.k_out) + (t * P.hk + head) * P.d + e0) = own;
+      if (dst[u]) {
+        T* p = dst[u] + t * dst_st[u];
+        *reinterpret_cast<uint4*>(p) = o0;
+        *reinterpret_cast<uint4*>(p + step) = o1;
       }
-      unpack8<T>(own, y);
-    } else {
+      if (!STORE || !store || cache[u] == nullptr) continue;  // (the same for a head's 8 lanes)
+      float y[2][8], top[2] = {0.f, 0.f};
+      unpack8<T>(o0, y[0]);
+      unpack8<T>(o1, y[1]);
+      const bool is_v = (int)blockIdx.y * (U * lanes) + u * lanes + hl >= P.hq + P.hk;
+      const float div = is_v ? P.v_scale : P.k_scale, inv = is_v ? P.v_inv : P.k_inv;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = 0.f;
-    }
-    if (!P.kc) continue;
-    const float div = is_v ? P.v_scale : P.k_scale;
-    float top = 0.f;
+      for (int k = 0; k < 2; ++k) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (div != 1.f) y[i] = __fdiv_rn(y[i], div);
-      top = max_nan(top, fabsf(y[i]));
+        for (int i = 0; i < 8; ++i) {
+          if (div != 1.f) y[k][i] = any_quotient(y[k][i], div, inv);
+          top[k] = max_nan(top[k], fabsf(y[k][i]));
+        }
+      }
+      const uint32_t head_lanes = 0xFFu << (threadIdx.x & 24);
+      const float a0 = __shfl_sync(head_lanes, top[0], lane0), a1 = __shfl_sync(head_lanes, top[1], lane0);
+      const float b0 = __shfl_sync(head_lanes, top[0], lane1), b1 = __shfl_sync(head_lanes, top[1], lane1);
+      uint8_t* codes = cache[u] + page * P.s_page + srow * ROW;
+      uint8_t* scales = cache[u] + page * P.s_page + P.page * ROW + srow * SROW;
+      const float m0 = max_nan(top[0], one0 ? a1 : a0), m1 = max_nan(top[1], one1 ? b1 : b0);
+      const uint32_t s0 = scale_code(m0), s1 = scale_code(m1);
+      *reinterpret_cast<uint32_t*>(codes + 4 * c0) = codes8(y[0], scale_value(s0), m0);
+      *reinterpret_cast<uint32_t*>(codes + 4 * c1) = codes8(y[1], scale_value(s1), m1);
+      if (!(c0 & 1)) scales[c0 >> 1] = (uint8_t)s0;
+      if (!(c1 & 1)) scales[c1 >> 1] = (uint8_t)s1;
     }
-    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));  // a scale's 16 elements are two neighbouring lanes'
-    if (!there || is_q || !store) continue;
-    const uint32_t sc = scale_code(top);
-    uint8_t* out = (is_v ? P.vc : P.kc) + block * P.s_page + head * P.s_head;
-    *reinterpret_cast<uint32_t*>(out + (int64_t)srow * ROW + 4 * c) = codes8(y, scale_value(sc));
-    if (!(c & 1)) out[(int64_t)P.page * ROW + srow * SROW + (c >> 1)] = (uint8_t)sc;
   }
 }
 
@@ -131,63 +227,95 @@ struct ReadParams {
   const uint8_t *kc, *vc;
   int64_t s_page, s_head;
   const int32_t* slots;
-  int64_t num_slots, items;
+  int64_t num_slots, tokens;
   int page, hk;
   float k_scale, v_scale;
   void *k, *v;  // contiguous [T, Hkv, D]
 };
 
-// One thread per (token, head, block of 16): its codes and scale of both caches.
+// A CTA reads READ_TOKENS tokens; a thread takes 8 elements (4 bytes of codes -> 16 of values) of one
+// head of K or V of each of them, all loads before the first store.
+constexpr int READ_TOKENS = 4;
 template <typename T>
-__global__ void __launch_bounds__(256) read_kernel(ReadParams P) {
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadParams P) {
   pdl_wait();
   pdl_trigger();
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= P.items) return;
-  const int b = (int)(i % SROW);
-  const int64_t th = i / SROW, t = th / P.hk;
-  const int head = (int)(th - t * P.hk);
-  const int64_t slot = __ldg(P.slots + t);
-  const bool there = slot >= 0 && slot < P.num_slots;
-  const int64_t blk = there ? slot / P.page : 0;
-  const int64_t row = there ? slot - blk * P.page : 0;
-  const int64_t at = blk * P.s_page + head * P.s_head;
+  const int64_t t0 = (int64_t)blockIdx.x * READ_TOKENS;
+  int64_t page_at[READ_TOKENS];
+  int row[READ_TOKENS];
+  bool there[READ_TOKENS];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const uint8_t* src = (w ? P.vc : P.kc) + at;
-    const float mul = w ? P.v_scale : P.k_scale;
-    uint2 codes = make_uint2(0, 0);
-    uint32_t sc = 0;
-    if (there) {
-      codes = *reinterpret_cast<const uint2*>(src + row * ROW + 8 * b);
-      sc = src[(int64_t)P.page * ROW + row * SROW + b];
+  for (int i = 0; i < READ_TOKENS; ++i) {
+    const int slot = t0 + i < P.tokens ? __ldg(P.slots + t0 + i) : -1;
+    there[i] = slot >= 0 && slot < P.num_slots;
+    const int page = there[i] ? (int)((unsigned)slot / (unsigned)P.page) : 0;
+    page_at[i] = page * P.s_page;
+    row[i] = there[i] ? slot - page * P.page : 0;
+  }
+  const int c = threadIdx.x & 15, e0 = 8 * c;
+  for (int h = threadIdx.x >> 4; h < 2 * P.hk; h += 16) {
+    const bool is_v = h >= P.hk;
+    const int head = is_v ? h - P.hk : h;
+    const uint8_t* src = (is_v ? P.vc : P.kc) + head * P.s_head;
+    const float mul = is_v ? P.v_scale : P.k_scale;
+    uint32_t codes[READ_TOKENS], sc[READ_TOKENS];
+#pragma unroll
+    for (int i = 0; i < READ_TOKENS; ++i) {
+      codes[i] = sc[i] = 0;
+      if (there[i]) {
+        codes[i] = *reinterpret_cast<const uint32_t*>(src + page_at[i] + row[i] * ROW + 4 * c);
+        sc[i] = src[page_at[i] + P.page * ROW + row[i] * SROW + (c >> 1)];
+      }
     }
-    const float s = scale_value(sc);
-    T* out = reinterpret_cast<T*>(w ? P.v : P.k) + th * D + BLOCK * b;
+    T* out = reinterpret_cast<T*>(is_v ? P.v : P.k) + (t0 * P.hk + head) * D + e0;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      uint32_t h[4];
-      e2m1x8_to_f16x8(p ? codes.y : codes.x, h);
+    for (int i = 0; i < READ_TOKENS; ++i) {
+      if (t0 + i >= P.tokens) break;
+      uint32_t w[4];
+      widen8(codes[i], w);
+      const uint32_t s = scale_f16x2(sc[i]);
       float f[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-        f[2 * j] = __fmul_rn(v.x * s, mul);  // code * scale is exact
-        f[2 * j + 1] = __fmul_rn(v.y * s, mul);
+        w[j] = mul_f16x2(w[j], s);  // exact
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        f[2 * j] = mul == 1.f ? v.x : __fmul_rn(v.x, mul);
+        f[2 * j + 1] = mul == 1.f ? v.y : __fmul_rn(v.y, mul);
       }
-      *reinterpret_cast<uint4*>(out + 8 * p) = pack8<T>(f);
+      *reinterpret_cast<uint4*>(out + (int64_t)i * P.hk * D) = pack8<T>(f);
     }
   }
 }
 
+template <typename T, bool STORE>
+inline int launch_rotary_as(const RotaryParams& P, cudaStream_t st) {
+  // heads side by side: as many as 256 threads hold, shared out evenly over the CTAs they take (by fours:
+  // whole warps for the store's shuffles, 8 units a head there)
+  constexpr int U = heads_a_thread(STORE);
+  const int units = P.d / 16, heads = P.hq + P.hk + P.hv, most = 256 / units;
+  const int shares = (int)cdiv(heads, U * most);
+  const int even = (int)cdiv(cdiv(heads, U * shares), 4) * 4, lanes = even <= most ? even : most;
+  const int ys = (int)cdiv(heads, U * lanes), threads = lanes * units;
+  const int smem = STAGES * stage_bytes(threads, U, P.pos ? P.rot : 0);
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ADA_ERR_CUDA;
+  if (smem > 48 * 1024 && !ready[dev]) {
+    if (cudaFuncSetAttribute(rotary_store_kernel<T, STORE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             STAGES * stage_bytes(256, U, 1024)) != cudaSuccess)
+      return ADA_ERR_CUDA;
+    ready[dev] = true;
+  }
+  // three CTAs an SM stay and walk the tokens
+  const int64_t walkers = 3 * 148 / ys > 0 ? 3 * 148 / ys : 1;
+  (void)launch_k(rotary_store_kernel<T, STORE>, dim3((unsigned)(P.tokens < walkers ? P.tokens : walkers), (unsigned)ys),
+                 dim3((unsigned)threads), (size_t)smem, st, P);
+  ADA_CHECK_LAUNCH();
+  return ADA_OK;
+}
 template <typename T>
-inline void launch_rotary(const RotaryParams& P, int64_t tokens, cudaStream_t st) {
-  const int chunks = P.d / 8;
-  const int lanes = 256 / chunks;
-  const int shares = (int)cdiv(P.hq + P.hk + P.hv, lanes);
-  // few tokens: the heads' shares on CTAs of their own; many: one CTA walks a token's heads
-  const int y = tokens * shares <= 1024 ? shares : 1;
-  (void)launch_k(rotary_store_kernel<T>, dim3((unsigned)tokens, (unsigned)y), dim3((unsigned)(lanes * chunks)), 0, st, P);
+inline int launch_rotary(const RotaryParams& P, cudaStream_t st) {
+  return P.kc ? launch_rotary_as<T, true>(P, st) : launch_rotary_as<T, false>(P, st);
 }
 
 // Checks that ada_rotary and the store share.
@@ -197,7 +325,7 @@ static int rotary_ok(const RotaryParams& P, int64_t tokens, int dtype) {
   if (P.pos) {
     if (!P.table || P.max_pos <= 0 || P.rot <= 0 || P.rot > P.d) return ADA_ERR_INVALID_ARG;
     if (P.rot % 16) return ADA_ERR_UNSUPPORTED;
-    if (reinterpret_cast<uintptr_t>(P.table) & 3) return ADA_ERR_ALIGNMENT;
+    if (misaligned16(P.table)) return ADA_ERR_ALIGNMENT;
     if (reinterpret_cast<uintptr_t>(P.pos) & 7) return ADA_ERR_ALIGNMENT;
   }
   if (P.d % 16 || P.d > 1024 || tokens > 0x7fffffff) return ADA_ERR_UNSUPPORTED;
@@ -237,17 +365,13 @@ extern "C" int ada_rotary(const int64_t* positions, const void* q, int64_t q_str
   P.hq = num_q_heads;
   P.hk = num_kv_heads;
   P.d = head_dim;
+  P.tokens = num_tokens;
   if (num_tokens == 0) return ADA_OK;
   if (!positions || (num_kv_heads > 0 && !k_out)) return ADA_ERR_INVALID_ARG;
   if (const int e = kv4::rotary_ok(P, num_tokens, dtype)) return e;
   if (num_q_heads + num_kv_heads == 0) return ADA_OK;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == ADA_DT_BF16)
-    kv4::launch_rotary<__nv_bfloat16>(P, num_tokens, st);
-  else
-    kv4::launch_rotary<__half>(P, num_tokens, st);
-  ADA_CHECK_LAUNCH();
-  return ADA_OK;
+  return dtype == ADA_DT_BF16 ? kv4::launch_rotary<__nv_bfloat16>(P, st) : kv4::launch_rotary<__half>(P, st);
 }
 
 extern "C" int ada_kv4_store(const int64_t* positions, const void* q, int64_t q_stride_t, int64_t q_stride_h,
@@ -267,7 +391,7 @@ extern "C" int ada_kv4_store(const int64_t* positions, const void* q, int64_t q_
   P.pos = positions;
   P.table = cos_sin;
   P.max_pos = max_position;
-  P.rot = rotary_dim;
+  P.rot = positions ? rotary_dim : 0;
   P.interleaved = interleaved != 0;
   P.q = q;
   P.k = k;
@@ -282,6 +406,7 @@ extern "C" int ada_kv4_store(const int64_t* positions, const void* q, int64_t q_
   P.hq = num_q_heads;
   P.hk = P.hv = num_kv_heads;
   P.d = head_dim;
+  P.tokens = num_tokens;
   P.kc = k_cache;
   P.vc = v_cache;
   P.s_page = kv_stride_page;
@@ -291,14 +416,11 @@ extern "C" int ada_kv4_store(const int64_t* positions, const void* q, int64_t q_
   P.page = page_size;
   P.k_scale = k_scale;
   P.v_scale = v_scale;
+  P.k_inv = 1.f / k_scale;
+  P.v_inv = 1.f / v_scale;
   if (const int e = kv4::rotary_ok(P, num_tokens, dtype)) return e;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == ADA_DT_BF16)
-    kv4::launch_rotary<__nv_bfloat16>(P, num_tokens, st);
-  else
-    kv4::launch_rotary<__half>(P, num_tokens, st);
-  ADA_CHECK_LAUNCH();
-  return ADA_OK;
+  return dtype == ADA_DT_BF16 ? kv4::launch_rotary<__nv_bfloat16>(P, st) : kv4::launch_rotary<__half>(P, st);
 }
 
 extern "C" int ada_kv4_read(const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
@@ -321,14 +443,14 @@ extern "C" int ada_kv4_read(const uint8_t* k_cache, const uint8_t* v_cache, int6
   P.s_head = kv_stride_head;
   P.slots = slot_mapping;
   P.num_slots = num_pages * page_size;
-  P.items = num_tokens * num_kv_heads * kv4::SROW;
+  P.tokens = num_tokens;
   P.page = page_size;
   P.hk = num_kv_heads;
   P.k_scale = k_scale;
   P.v_scale = v_scale;
   P.k = k;
   P.v = v;
-  const int64_t grid = cdiv(P.items, 256);
+  const int64_t grid = cdiv(num_tokens, (int64_t)kv4::READ_TOKENS);
   if (grid > 0x7fffffff) return ADA_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == ADA_DT_BF16)

@@ -693,7 +693,7 @@ ADA_API int ada_step_metadata(const int32_t* cached_lens, const int32_t* new_len
  * [cos | sin] of the rotary_dim / 2 pairs (scaling for long contexts is in the table).
  * q, k: element (t, h, d) at t * stride_t + h * stride_h + d; q_out [T, num_q_heads, head_dim], k_out
  * [T, num_kv_heads, head_dim] contiguous, not over the inputs.
- * Implemented: head_dim % 16 == 0 up to 1024, rotary_dim % 16 == 0, rows 16-byte aligned.
+ * Implemented: head_dim % 16 == 0 up to 1024, rotary_dim % 16 == 0, rows and cos_sin 16-byte aligned.
  * ---------------------------------------------------------------------- */
 ADA_API int ada_rotary(const int64_t* positions, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
                        int64_t k_stride_t, int64_t k_stride_h, void* q_out, void* k_out, int64_t num_tokens,
