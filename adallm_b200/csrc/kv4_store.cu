@@ -8,6 +8,8 @@
 //
 // Store: a row's rotated key, rounded to T as a model without the fusion has it, and its value are
 // divided by the tensor's scale and packed as kv4.cuh describes.
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace ada {
@@ -32,6 +34,41 @@ struct RotaryParams {
   float k_scale, v_scale, k_inv, v_inv;
 };
 
+// Largest magnitude of 8 elements; NaN if one is.
+template <typename T>
+__device__ __forceinline__ float largest(const uint4& x) {
+  const uint32_t w[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
+  uint32_t a, b;
+  if (std::is_same<T, __half>::value) {
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+  } else {
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+  }
+  const T* h = reinterpret_cast<const T*>(&a);
+  return max_nan(to_f32(h[0]), to_f32(h[1]));
+}
+// Codes of 8 elements over the tensor's scale `div` (inv near 1 / div) and the block's scale s; top: the block's largest
+// quotient.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_codes(const uint4& x, float div, float inv, float s, float top) {
+  float y[8];
+  unpack8<T>(x, y);
+  if (div != 1.f) {
+    if (top == INFINITY) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = any_quotient(y[i], div, inv);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = quotient(y[i], div, inv);
+    }
+  }
+  return codes8(y, s, top);
+}
+
 // A thread's unit is two chunks of 8 elements (16 bytes each) whose pairs lie within it: chunks i and
 // i + r/16 of the turned part (half layout), or neighbours; it keeps U heads (blockIdx.y's share) and walks
 // the tokens, so what belongs to a head is worked out once.  Rows and table entries of the next
@@ -39,13 +76,13 @@ struct RotaryParams {
 // at a time, or one ahead in registers, an SM has 20-40 KB in flight where HBM wants 66 (95 us
 // instead of 66 for 16,381 tokens of 40 heads).
 // (one head with the store, whose arithmetic needs the registers)
-constexpr int heads_a_thread(bool store) { return store ? 1 : 2; }
+constexpr int heads_a_thread(bool) { return 2; }
 constexpr int STAGES = 4;
 // Bytes of a stage: the CTA's rows, then the table's row.
 __host__ __device__ constexpr int stage_bytes(int threads, int heads, int rot) { return threads * heads * 32 + rot * 4; }
 
 template <typename T, bool STORE>
-__global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_constant__ RotaryParams P) {
+__global__ void __launch_bounds__(256, STORE ? 2 : 3) rotary_store_kernel(const __grid_constant__ RotaryParams P) {
   constexpr int U = heads_a_thread(STORE);
   extern __shared__ __align__(16) uint8_t sm[];
   pdl_wait();
@@ -53,25 +90,26 @@ __global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_const
   const int units = P.d >> 4;
   const int lanes = blockDim.x / units;  // heads side by side
   const int hl = (int)threadIdx.x / units, unit = (int)threadIdx.x - hl * units;
-  const int half = P.rot >> 1, rc = P.rot >> 3;
-  const bool turned = P.pos != nullptr && 16 * unit < P.rot;
-  const bool apart = turned && !P.interleaved;  // the unit's chunks are half the turned part apart
-  const int c0 = apart ? unit : 2 * unit, c1 = apart ? unit + (rc >> 1) : 2 * unit + 1;
+  const int half = P.rot >> 1;
+  // Half layout: units of the first rc / 2 hold chunks (i, i + rc / 2), whose pairs lie across them.  The
+  // others, and all of the interleaved layout, hold chunks half of what is left apart, so that
+  // neighbouring lanes read and write neighbouring 16 bytes either time.
+  const int rc = P.pos && !P.interleaved ? P.rot >> 3 : 0;
+  const int rest = (2 * units - rc) >> 1;
+  const bool apart = unit < (rc >> 1);
+  const int c0 = apart ? unit : rc + unit - (rc >> 1), c1 = apart ? unit + (rc >> 1) : c0 + rest;
   const int step = 8 * (c1 - c0);
-  const int pair0 = apart ? 8 * c0 : 8 * unit;          // the unit's 8 pairs
+  // interleaved: which of the chunks are turned, and their 4 pairs' entries
+  const bool turn0 = P.pos && P.interleaved && 8 * c0 < P.rot, turn1 = P.pos && P.interleaved && 8 * c1 < P.rot;
   // chunk c's neighbour in its block of 16 (c ^ 1): the lane that holds it, and as which of its two
   int lane0 = 0, lane1 = 0;
   bool one0 = false, one1 = false;
   if (STORE) {
     const int base = (int)(threadIdx.x & 31) - unit;  // (8 units a head: a head's lanes are in one warp)
     auto find = [&](int c, int& lane, bool& one) {
-      if (P.pos && !P.interleaved && c < rc) {
-        one = c >= (rc >> 1);
-        lane = base + (one ? c - (rc >> 1) : c);
-      } else {
-        one = c & 1;
-        lane = base + (c >> 1);
-      }
+      const int first = c < rc ? 0 : rc, n = c < rc ? rc >> 1 : rest;
+      one = c - first >= n;
+      lane = base + (first >> 1) + (c - first) - (one ? n : 0);
     };
     find(c0 ^ 1, lane0, one0);
     find(c1 ^ 1, lane1, one1);
@@ -84,7 +122,7 @@ __global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_const
   bool turn[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int h = (int)blockIdx.y * (U * lanes) + u * lanes + hl;
+    const int h = (int)blockIdx.y + (int)gridDim.y * (u * lanes + hl);  // (every share has queries, keys and values)
     src[u] = nullptr;
     dst[u] = nullptr;
     cache[u] = nullptr;
@@ -95,14 +133,14 @@ __global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_const
       dst[u] = reinterpret_cast<T*>(P.q_out) + (int64_t)h * P.d + 8 * c0;
       src_st[u] = P.q_st;
       dst_st[u] = (int64_t)P.hq * P.d;
-      turn[u] = turned;
+      turn[u] = apart || turn0 || turn1;
     } else if (h < P.hq + P.hk) {
       const int n = h - P.hq;
       src[u] = reinterpret_cast<const T*>(P.k) + n * P.k_sh + 8 * c0;
       if (P.k_out) dst[u] = reinterpret_cast<T*>(P.k_out) + (int64_t)n * P.d + 8 * c0;
       src_st[u] = P.k_st;
       dst_st[u] = (int64_t)P.hk * P.d;
-      turn[u] = turned;
+      turn[u] = apart || turn0 || turn1;
       if (STORE) cache[u] = P.kc + n * P.s_head;
     } else if (h < P.hq + P.hk + P.hv) {
       const int n = h - P.hq - P.hk;
@@ -152,12 +190,21 @@ __global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_const
     fetch(s == 0 ? STAGES - 1 : s - 1);
     const uint8_t* mine = sm + s * stage + threadIdx.x * 16;
     float cs[8], sn[8];
-    if (turned) {
-      const float* row = reinterpret_cast<const float*>(sm + s * stage + rows) + pair0;
+    const float* row = reinterpret_cast<const float*>(sm + s * stage + rows);
+    if (apart) {  // 8 pairs
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
-        *reinterpret_cast<float4*>(cs + i) = *reinterpret_cast<const float4*>(row + i);
-        *reinterpret_cast<float4*>(sn + i) = *reinterpret_cast<const float4*>(row + half + i);
+        *reinterpret_cast<float4*>(cs + i) = *reinterpret_cast<const float4*>(row + 8 * c0 + i);
+        *reinterpret_cast<float4*>(sn + i) = *reinterpret_cast<const float4*>(row + half + 8 * c0 + i);
+      }
+    } else {
+      if (turn0) {
+        *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(row + 4 * c0);
+        *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(row + half + 4 * c0);
+      }
+      if (turn1) {
+        *reinterpret_cast<float4*>(cs + 4) = *reinterpret_cast<const float4*>(row + 4 * c1);
+        *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(row + half + 4 * c1);
       }
     }
     s = s == STAGES - 1 ? 0 : s + 1;
@@ -171,7 +218,7 @@ __global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_const
         unpack8<T>(o0, x);
         unpack8<T>(o1, z);
         // single operations: joined to fused ones, or packed (which the compiler joins), they round differently
-        if (P.interleaved) {
+        if (!apart) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             y[2 * i] = __fsub_rn(__fmul_rn(x[2 * i], cs[i]), __fmul_rn(x[2 * i + 1], sn[i]));
@@ -186,8 +233,8 @@ __global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_const
             w[i] = __fadd_rn(__fmul_rn(z[i], cs[i]), __fmul_rn(x[i], sn[i]));
           }
         }
-        o0 = pack8<T>(y);
-        o1 = pack8<T>(w);
+        if (apart || turn0) o0 = pack8<T>(y);
+        if (apart || turn1) o1 = pack8<T>(w);
       }
       if (dst[u]) {
         T* p = dst[u] + t * dst_st[u];
@@ -195,28 +242,20 @@ __global__ void __launch_bounds__(256, 3) rotary_store_kernel(const __grid_const
         *reinterpret_cast<uint4*>(p + step) = o1;
       }
       if (!STORE || !store || cache[u] == nullptr) continue;  // (the same for a head's 8 lanes)
-      float y[2][8], top[2] = {0.f, 0.f};
-      unpack8<T>(o0, y[0]);
-      unpack8<T>(o1, y[1]);
-      const bool is_v = (int)blockIdx.y * (U * lanes) + u * lanes + hl >= P.hq + P.hk;
-      const float div = is_v ? P.v_scale : P.k_scale, inv = is_v ? P.v_inv : P.k_inv;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (div != 1.f) y[k][i] = any_quotient(y[k][i], div, inv);
-          top[k] = max_nan(top[k], fabsf(y[k][i]));
-        }
-      }
+      const float top[2] = {largest<T>(o0), largest<T>(o1)};
       const uint32_t head_lanes = 0xFFu << (threadIdx.x & 24);
       const float a0 = __shfl_sync(head_lanes, top[0], lane0), a1 = __shfl_sync(head_lanes, top[1], lane0);
       const float b0 = __shfl_sync(head_lanes, top[0], lane1), b1 = __shfl_sync(head_lanes, top[1], lane1);
+      const bool is_v = (int)blockIdx.y + (int)gridDim.y * (u * lanes + hl) >= P.hq + P.hk;
+      const float div = is_v ? P.v_scale : P.k_scale, inv = is_v ? P.v_inv : P.k_inv;
+      // (the largest quotient is the largest element's: rounding keeps the order)
+      const float m0 = any_quotient(max_nan(top[0], one0 ? a1 : a0), div, inv);
+      const float m1 = any_quotient(max_nan(top[1], one1 ? b1 : b0), div, inv);
+      const uint32_t s0 = scale_code(m0), s1 = scale_code(m1);
       uint8_t* codes = cache[u] + page * P.s_page + srow * ROW;
       uint8_t* scales = cache[u] + page * P.s_page + P.page * ROW + srow * SROW;
-      const float m0 = max_nan(top[0], one0 ? a1 : a0), m1 = max_nan(top[1], one1 ? b1 : b0);
-      const uint32_t s0 = scale_code(m0), s1 = scale_code(m1);
-      *reinterpret_cast<uint32_t*>(codes + 4 * c0) = codes8(y[0], scale_value(s0), m0);
-      *reinterpret_cast<uint32_t*>(codes + 4 * c1) = codes8(y[1], scale_value(s1), m1);
+      *reinterpret_cast<uint32_t*>(codes + 4 * c0) = pack_codes<T>(o0, div, inv, scale_value(s0), m0);
+      *reinterpret_cast<uint32_t*>(codes + 4 * c1) = pack_codes<T>(o1, div, inv, scale_value(s1), m1);
       if (!(c0 & 1)) scales[c0 >> 1] = (uint8_t)s0;
       if (!(c1 & 1)) scales[c1 >> 1] = (uint8_t)s1;
     }
@@ -306,8 +345,9 @@ inline int launch_rotary_as(const RotaryParams& P, cudaStream_t st) {
       return ADA_ERR_CUDA;
     ready[dev] = true;
   }
-  // three CTAs an SM stay and walk the tokens
-  const int64_t walkers = 3 * 148 / ys > 0 ? 3 * 148 / ys : 1;
+  // as many CTAs as the SMs hold (80 registers a thread, shared memory) stay and walk the tokens
+  const int by_regs = 65536 / ((STORE ? 128 : 80) * threads), by_smem = 232448 / (smem + 1024);
+  const int64_t walkers = cdiv(148 * (by_regs < by_smem ? by_regs : by_smem), ys);
   (void)launch_k(rotary_store_kernel<T, STORE>, dim3((unsigned)(P.tokens < walkers ? P.tokens : walkers), (unsigned)ys),
                  dim3((unsigned)threads), (size_t)smem, st, P);
   ADA_CHECK_LAUNCH();
