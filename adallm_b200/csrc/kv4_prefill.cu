@@ -78,14 +78,32 @@ struct Params {
   unsigned* err;
 };
 
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t accumulate) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// High word of every shared-memory descriptor here: 1,024 bytes between 8-row groups, 128-byte swizzle.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | ((uint32_t)SWZ_128B << 29);
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(DESC_HI), "r"(IDESC_S), "r"((int)accumulate)
       : "memory");
+}
+// A (f16, two a column) in TMEM.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(DESC_HI), "r"(IDESC_PV), "r"((int)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 // 64 columns of this thread's TMEM lane; load and wait are one statement, so no register of the load
 // can be touched before the wait.
@@ -117,7 +135,7 @@ __device__ __forceinline__ void key_range(const Params& P, int t, int off, int l
 }
 
 __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_constant__ Params P) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kvh = blockIdx.x, b = blockIdx.y;
   const int qblk = gridDim.z - 1 - blockIdx.z;  // the longest causal rows of all heads and sequences first
 
@@ -242,59 +260,74 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       }
     }
   } else if (warp == 1) {  // ---------------- MMA issuer ----------------
-    if (lane == 0 && nblk > 0) {
-      const uint32_t q_addr = smem_u32(qs), k_addr = smem_u32(kf), v_addr = smem_u32(vf);
-      auto issue_s = [&](int j) {
-        const uint32_t kb = (uint32_t)(j % NKV);
+    // The whole warp runs this loop, its values uniform, and one elected lane issues: the operands of the
+    // tcgen05 instructions then stay in uniform registers (from a divergent lane an MMA takes about 100
+    // cycles to issue: 24 of them a block were the bound, 629 us instead of 400 for 4 x 2,048 behind 2,048).
+    if (nblk > 0) {
+      const bool leader = elect_one();
+      const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
+      // low words of the descriptors: address / 16, leading offset / 16 (V: 8 KB between the halves of d)
+      const uint32_t q_lo = (smem_u32(qs) >> 4) | (1u << 16), k_lo = (smem_u32(kf) >> 4) | (1u << 16);
+      const uint32_t v_lo = (smem_u32(vf) >> 4) | ((8192u >> 4) << 16);
+      auto issue_s = [&](int j, uint32_t slot) {
+        if (leader) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const uint32_t d = tmem + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
+          for (int t = 0; t < NT; ++t) {
+            const uint32_t d = tm + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t hoff = (uint32_t)t * 32768u + (uint32_t)(kk / 4) * 16384u + (uint32_t)(kk % 4) * 32u;
-            const uint32_t koff = kb * 16384u + (uint32_t)(kk / 4) * 8192u + (uint32_t)(kk % 4) * 32u;
-            mma_f16(d, desc_kmajor_sw128(q_addr + hoff), desc_kmajor_sw128(k_addr + koff), IDESC_S, kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_ss(d, q_lo + (uint32_t)t * 2048u + (uint32_t)(kk / 4) * 1024u + (uint32_t)(kk % 4) * 2u,
+                     k_lo + slot * 1024u + (uint32_t)(kk / 4) * 512u + (uint32_t)(kk % 4) * 2u, kk > 0);
+            tc_commit(&s_full[2 * t + (j & 1)]);
           }
-          tc_commit(&s_full[2 * t + (j & 1)]);
         }
+        __syncwarp();
       };
+      uint32_t slot = 0;
       bool ok = wait_b(q_ready, 0, abort_v, P.err) && wait_b(&kv_full[0], 0, abort_v, P.err);
+      ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
-        issue_s(0);
+        issue_s(0, 0);
       }
       for (int j = 0; ok && j < nblk; ++j) {
+        const uint32_t next = slot + 1 == NKV ? 0 : slot + 1;
         if (j + 1 < nblk) {
-          if (!wait_b(&kv_full[(j + 1) % NKV], ((j + 1) / NKV) & 1, abort_v, P.err)) break;
-          if (j > 0 && !(wait_b(&o_done[0], (j - 1) & 1, abort_v, P.err) && wait_b(&o_done[1], (j - 1) & 1, abort_v, P.err)))
-            break;
+          ok = wait_b(&kv_full[next], ((j + 1) / NKV) & 1, abort_v, P.err);
+          if (j > 0)
+            ok = ok && wait_b(&o_done[0], (j - 1) & 1, abort_v, P.err) && wait_b(&o_done[1], (j - 1) & 1, abort_v, P.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           tc_fence_after();
-          issue_s(j + 1);
+          issue_s(j + 1, next);
         }
-        const uint32_t kb = (uint32_t)(j % NKV);
-        for (int t = 0; t < NT && ok; ++t) {
-          if (!wait_b(&p_full[2 * t + (j & 1)], (j >> 1) & 1, abort_v, P.err)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t p = tmem + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk) {
-            const uint64_t vd = smem_desc(v_addr + kb * 16384u + (uint32_t)kk * 16u * 128u, 8192, 1024, SWZ_128B);
-            mma_f16_ts(tmem + 128u * (uint32_t)t, p + 8u * (uint32_t)kk, vd, IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
+        for (int t = 0; t < NT; ++t) {
+          ok = __all_sync(0xffffffffu, ok && wait_b(&p_full[2 * t + (j & 1)], (j >> 1) & 1, abort_v, P.err));
+          if (ok) {
+            tc_fence_after();
+            if (leader) {
+              const uint32_t p = tm + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
+#pragma unroll
+              for (int kk = 0; kk < BN / 16; ++kk)
+                mma_ts(tm + 128u * (uint32_t)t, p + 8u * (uint32_t)kk, v_lo + slot * 1024u + (uint32_t)kk * 128u,
+                       j > 0 || kk > 0);
+              tc_commit(&o_done[t]);
+              if (t == NT - 1) tc_commit(&kv_empty[slot]);
+            }
+            __syncwarp();
           }
-          tc_commit(&o_done[t]);
         }
-        if (ok) tc_commit(&kv_empty[kb]);
+        slot = next;
       }
       // every MMA issued above has completed before the teardown
-      tc_commit(fin);
+      if (leader) tc_commit(fin);
+      __syncwarp();
       uint32_t spins = 0;
       const uint64_t t_start = globaltimer();
       while (!mbar_try_wait(fin, 0)) {
         if ((++spins & 63u) == 0 && globaltimer() - t_start > 2000000000ull) {
-          if (P.err) atomicOr(P.err, ERR_TILE_WAIT);
+          if (leader && P.err) atomicOr(P.err, ERR_TILE_WAIT);
           break;
         }
       }
@@ -419,54 +452,43 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       if (marked.x | marked.y | marked.z | marked.w) {
         for (int i = max(a, 0); i < min(e, BN); ++i) nan_blocks |= (flags[8 + (i >> 2)] >> (8 * (i & 3))) & 0xFFu;
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int i = 0; i < 64; i += 8) {
+      for (int i = 4; i < 60; i += 8) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], fmaxf(x[i + 2 * k], x[i + 2 * k + 1]));
+        for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], x[i + 2 * k], x[i + 2 * k + 1]);
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const float top = max3(max3(mx[0], x[60], x[61]), max3(mx[1], x[62], x[63]), fmaxf(mx[2], mx[3]));
       float alpha = 1.f;
       if ((top - m) * factor > MOVE_LOG2) {
         alpha = m == -INFINITY ? 0.f : safe ? fast_exp2(ref - top * factor) : fast_exp2((m - top) * factor);
         m = top;
         ref = top * factor;
       }
-      uint32_t pk[32];
-      if (safe) {
-        const uint64_t c2 = pair(factor, factor), r2 = pair(-ref, -ref);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float p0, p1;
-          unpair(fma2(pair(x[2 * i], x[2 * i + 1]), c2, r2), p0, p1);
-          p0 = fast_exp2(p0);
-          p1 = fast_exp2(p1);
-          // fp32 probabilities feed the row's sum, fp16 ones P V
-          if (i == 0 && alpha != 1.f) {
-            float s0, s1, s2, s3;
-            unpair(l2[0], s0, s1);
-            unpair(l2[1], s2, s3);
-            l2[0] = pair(s0 * alpha, s1 * alpha);
-            l2[1] = pair(s2 * alpha, s3 * alpha);
-          }
-          l2[i & 1] = add2(l2[i & 1], pair(p0, p1));
-          pk[i] = pack_half2(p0, p1);
-        }
-      } else {
+      if (!safe) {  // (warp-uniform) the difference first; the loop below then only takes the exponential
         const float mm = m == -INFINITY ? 0.f : m;
-        float s0, s1, s2, s3;
-        unpair(l2[0], s0, s1);
-        unpair(l2[1], s2, s3);
-        s0 *= alpha, s1 *= alpha, s2 *= alpha, s3 *= alpha;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float p0 = fast_exp2((x[2 * i] - mm) * factor), p1 = fast_exp2((x[2 * i + 1] - mm) * factor);
-          s0 += p0;
-          s1 += p1;
-          pk[i] = pack_half2(p0, p1);
+        for (int i = 0; i < 64; ++i) x[i] = (x[i] - mm) * factor;
+      }
+      if (alpha != 1.f) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float s0, s1;
+          unpair(l2[i], s0, s1);
+          l2[i] = pair(s0 * alpha, s1 * alpha);
         }
-        l2[0] = pair(s0, s1);
-        l2[1] = pair(s2, s3);
+      }
+      const float c1 = safe ? factor : 1.f, r1 = safe ? -ref : 0.f;
+      const uint64_t c2 = pair(c1, c1), r2 = pair(r1, r1);
+      uint32_t pk[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float p0, p1;
+        unpair(fma2(pair(x[2 * i], x[2 * i + 1]), c2, r2), p0, p1);
+        p0 = fast_exp2(p0);
+        p1 = fast_exp2(p1);
+        l2[i & 1] = add2(l2[i & 1], pair(p0, p1));  // fp32 probabilities feed the row's sum, fp16 ones P V
+        pk[i] = pack_half2(p0, p1);
       }
       // the probabilities over the scores
 #pragma unroll
