@@ -25,11 +25,14 @@
 // their 16 elements to NaN at the end.
 //
 // Barriers (block j, tile t): e_full[j % NSTG], e_empty, kv_full[j % NKV], kv_empty (commit after both P V),
-// s_full[t][j & 1] (commit), p_full[t][j & 1] (4 warps), o_done[t] (commit after P V), q_ready (8 warps), fin.
-// A refill waits for the release of the use before, so a barrier is never two phases ahead of a
-// waiter: S_{j+2} is issued after p_full of j; o_done of j comes after p_full of j, whose softmax
-// has already passed its wait for j - 1.  Before S_{j+1} overwrites the buffer that P_{j-1} lay in, the
-// issuer waits for o_done of j - 1.
+// s_full[t][j & 1] (commit, and an arrival of the issuer's own), p_full[t][j & 1] (4 warps),
+// o_done[t] (commit
+// after P V), o_last[t] (after the last one), q_ready (8 warps), fin.
+// A wait by parity needs the phase before to be known complete and the next one not begun.  Refills wait
+// for the release of the use before, in every phase; S_{j+2} is issued after p_full of j.  o_done of j - 1: the
+// issuer waits for it (in turn) before S_{j+1} overwrites the buffer that P_{j-1} lay in, so a softmax that
+// has S_j knows that of j - 2 complete, and that of j cannot begin before its own p_full.  The
+// end waits for o_last, which has one phase.
 #include "kv4.cuh"
 #include "tc_attention.cuh"
 
@@ -49,7 +52,7 @@ constexpr int E_OFF = V_OFF + NKV * 16384;   // staging: K codes, V codes, K sca
 constexpr int E_BYTES = 2 * BN * ROW_BYTES;
 constexpr int EV = BN * ROW, EKS = 2 * BN * ROW, EVS = EKS + BN * SROW;
 constexpr int BAR_OFF = E_OFF + NSTG * E_BYTES;
-constexpr int NBAR = 2 * NSTG + 2 * NKV + 5 * NT + 2;
+constexpr int NBAR = 2 * NSTG + 2 * NKV + 6 * NT + 2;
 constexpr int FLAG_OFF = BAR_OFF + NBAR * 8;  // words: e_ok[NSTG], then per K/V slot [ok][4 warps' NaN flags][16 NaN masks]
 constexpr int SLOT_WORDS = 24;
 constexpr int SMEM = 1024 + FLAG_OFF + (NSTG + NKV * SLOT_WORDS + 4) * 4;
@@ -149,7 +152,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
   uint64_t* s_full = kv_empty + NKV;   // [NT][2]
   uint64_t* p_full = s_full + 2 * NT;  // [NT][2]
   uint64_t* o_done = p_full + 2 * NT;  // [NT]
-  uint64_t* q_ready = o_done + NT;
+  uint64_t* o_last = o_done + NT;      // [NT]
+  uint64_t* q_ready = o_last + NT;
   uint64_t* fin = q_ready + 1;
   int* e_ok = reinterpret_cast<int*>(base + FLAG_OFF);
   uint32_t* slots = reinterpret_cast<uint32_t*>(e_ok + NSTG);
@@ -167,10 +171,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       mbar_init(&kv_empty[i], 1);
     }
     for (int i = 0; i < 2 * NT; ++i) {
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[i], 2);
       mbar_init(&p_full[i], NSOFT);
     }
-    for (int t = 0; t < NT; ++t) mbar_init(&o_done[t], 1);
+    for (int t = 0; t < NT; ++t) {
+      mbar_init(&o_done[t], 1);
+      mbar_init(&o_last[t], 1);
+    }
     mbar_init(q_ready, NT * NSOFT);
     mbar_init(fin, 1);
     *abort_flag = 0;
@@ -279,6 +286,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
               mma_ss(d, q_lo + (uint32_t)t * 2048u + (uint32_t)(kk / 4) * 1024u + (uint32_t)(kk % 4) * 2u,
                      k_lo + slot * 1024u + (uint32_t)(kk / 4) * 512u + (uint32_t)(kk % 4) * 2u, kk > 0);
             tc_commit(&s_full[2 * t + (j & 1)]);
+            mbar_arrive_plain(&s_full[2 * t + (j & 1)]);  // passes on what kv_full ordered: the flags
           }
         }
         __syncwarp();
@@ -313,6 +321,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 mma_ts(tm + 128u * (uint32_t)t, p + 8u * (uint32_t)kk, v_lo + slot * 1024u + (uint32_t)kk * 128u,
                        j > 0 || kk > 0);
               tc_commit(&o_done[t]);
+              if (j + 1 == nblk) tc_commit(&o_last[t]);
               if (t == NT - 1) tc_commit(&kv_empty[slot]);
             }
             __syncwarp();
@@ -428,9 +437,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     bool failed = false;
     for (int j = 0; j < nblk; ++j) {
       const int sb = j & 1;
-      // warp-uniform outcomes: the TMEM accesses below are warp-collective.  (kv_full orders the flags)
-      if (!__all_sync(0xffffffffu, wait_b(&kv_full[j % NKV], (j / NKV) & 1, abort_v, P.err) &&
-                                       wait_b(&s_full[2 * t + sb], (j >> 1) & 1, abort_v, P.err))) {
+      // warp-uniform outcome: the TMEM accesses below are warp-collective
+      if (!__all_sync(0xffffffffu, wait_b(&s_full[2 * t + sb], (j >> 1) & 1, abort_v, P.err))) {
         failed = true;
         break;
       }
@@ -493,13 +501,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       // the probabilities over the scores
 #pragma unroll
       for (int i = 0; i < 2; ++i) tmem_st16(trow + s_col + BN * sb + 16 * i, pk + 16 * i);
-      // Waited for in every block, also where nothing is rescaled: a parity tells a phase from the one
-      // before it only to a waiter that has seen that one complete.
-      if (j > 0 && !__all_sync(0xffffffffu, wait_b(&o_done[t], (j - 1) & 1, abort_v, P.err))) {
-        failed = true;
-        break;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {  // O is stable: P V of the block before has completed
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        // O is stable once P V of the block before has completed (that of the one before that has: S_j was
+        // issued behind it, so the parity is this phase's)
+        if (!__all_sync(0xffffffffu, wait_b(&o_done[t], (j - 1) & 1, abort_v, P.err))) {
+          failed = true;
+          break;
+        }
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {
@@ -518,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     }
     // ---- epilogue: O row / l
     if (!failed && nblk > 0) {
-      failed = !__all_sync(0xffffffffu, wait_b(&o_done[t], (nblk - 1) & 1, abort_v, P.err));
+      failed = !__all_sync(0xffffffffu, wait_b(&o_last[t], 0, abort_v, P.err));
       tc_fence_after();
     }
     failed = __any_sync(0xffffffffu, failed || *abort_v != 0);
