@@ -85,7 +85,7 @@ _SIGS = {
     "ada_kv4_store": (INT, [P, P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I32, I32, I32, P, I64, I32, I32, P, P, P,
                             I64, I64, I64, I32, F32, F32, INT, P]),
     "ada_kv4_read": (INT, [P, P, I64, I64, I64, I32, I32, I32, P, I64, F32, F32, P, P, INT, P]),
-    "ada_kv4_paged_decode_workspace_size": (SZ, [I32, I32, I32]),
+    "ada_kv4_paged_decode_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32]),
     "ada_kv4_paged_decode": (INT, [P, INT, I64, I64, P, P, I64, I64, I64, P, I64, I32, P, I32, I32, I32, I32, I32, F32,
                                    F32, F32, I32, P, INT, I64, I64, P, SZ, P]),
     "ada_kv4_paged_prefill": (INT, [P, INT, I64, I64, P, P, I64, I64, I64, P, I64, I32, P, P, I32, I64, I32, I32, I32,

@@ -67,11 +67,10 @@ struct Params {
 struct Range {
   int lo, hi, first;  // visible keys, first step
 };
-__device__ __forceinline__ Range range_of(const Params& P, int b) {
-  const int ctx = (int)min((int64_t)__ldg(P.lens + b), (int64_t)P.max_pages * P.page);
-  const int full = __ldg(P.lens + b);
+__device__ __forceinline__ Range range_of(const Params& P, int len) {
+  const int full = max(len, 0);
   Range r;
-  r.hi = max(ctx, 0);
+  r.hi = min(full, P.max_pages * P.page);
   r.lo = P.window > 0 ? max(full - P.window, 0) : 0;
   r.first = r.lo / KEYS;
   return r;
@@ -141,6 +140,8 @@ struct Acc {
   float l[2];
 };
 
+// ALONE: one CTA an item, which it finishes; otherwise the steps of all items shared out equally.
+template <bool ALONE>
 __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_constant__ Params P) {
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int warp_sum[WARPS];
@@ -148,52 +149,91 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   uint8_t* ring = sm + warp * WARP_SMEM;
   float* slot0 = reinterpret_cast<float*>(ring + STAGES * STEP_BYTES);
-  int* cum = reinterpret_cast<int*>(sm + WARPS * WARP_SMEM);
+  // steps before each sequence, and the lengths (a copy a warp for up to 32 sequences: no barrier)
+  int* lists = reinterpret_cast<int*>(sm + WARPS * WARP_SMEM);
+  const bool few = P.batch <= 32;
+  int* cum = few ? lists + warp * 72 : lists;
+  int* lens = few ? cum + 36 : lists + P.batch + 1;
   const int items = P.hkv * P.subs;
+  if (lane < 2) part_item[warp][lane].end = 0;  // no partial
   pdl_wait();
   pdl_trigger();
 
-  // ---- steps before each sequence
-  {
-    const int per = (P.batch + WARPS * 32 - 1) / (WARPS * 32);
-    const int b0 = min(tid * per, P.batch), b1 = min(b0 + per, P.batch);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += steps_of(range_of(P, b));
-    int inc = sum;
+  int cta0, cta1, r0, r1;
+  Item alone{0, 0, 0, 0};
+  int alone_len = 0;
+  if (ALONE) {
+    alone.b = blockIdx.x / items;
+    alone.h = blockIdx.x - alone.b * items;
+    alone_len = __ldg(P.lens + alone.b);
+    alone.end = steps_of(range_of(P, alone_len));
+    const int per = (alone.end + WARPS - 1) / WARPS;
+    cta0 = 0;
+    cta1 = alone.end;
+    r0 = min(warp * per, cta1);
+    r1 = min(r0 + per, cta1);
+  } else {
+    if (few) {
+      const int len = lane < P.batch ? __ldg(P.lens + lane) : 0;
+      const int n = lane < P.batch ? steps_of(range_of(P, len)) : 0;
+      int inc = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      cum[lane + 1] = inc;
+      lens[lane] = len;
+      if (lane == 0) cum[0] = 0;
+      __syncwarp();
+    } else {
+      const int per = (P.batch + WARPS * 32 - 1) / (WARPS * 32);
+      const int b0 = min(tid * per, P.batch), b1 = min(b0 + per, P.batch);
+      int sum = 0;
+      for (int b = b0; b < b1; ++b) {
+        lens[b] = __ldg(P.lens + b);
+        sum += steps_of(range_of(P, lens[b]));
+      }
+      int inc = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      if (lane == 31) warp_sum[warp] = inc;
+      __syncthreads();
+      int run = inc - sum;
+      for (int w = 0; w < warp; ++w) run += warp_sum[w];
+      for (int b = b0; b < b1; ++b) {
+        cum[b] = run;
+        run += steps_of(range_of(P, lens[b]));
+      }
+      if (b0 < b1 && b1 == P.batch) cum[P.batch] = run;
+      __syncthreads();
     }
-    if (lane == 31) warp_sum[warp] = inc;
-    if (tid < WARPS) part_item[tid][0].end = part_item[tid][1].end = 0;  // no partial
-    __syncthreads();
-    int run = inc - sum;
-    for (int w = 0; w < warp; ++w) run += warp_sum[w];
-    for (int b = b0; b < b1; ++b) {
-      cum[b] = run;
-      run += steps_of(range_of(P, b));
+    const int total = cum[P.batch] * items;
+    const int workers = gridDim.x * WARPS;
+    const int per = max((total + workers - 1) / workers, 1);
+    if (blockIdx.x == 0) {  // for the merge (with few sequences every warp has the lists, and the first writes them)
+      for (int b = few ? lane : tid; b <= P.batch; b += few ? 32 : WARPS * 32)
+        if (!few || warp == 0) P.cum[b] = cum[b];
+      if (tid == 0) P.cum[P.batch + 1] = per * WARPS;
     }
-    if (b0 < b1 && b1 == P.batch) cum[P.batch] = run;
-    __syncthreads();
+    const int64_t c0 = (int64_t)blockIdx.x * WARPS * per;  // this CTA's steps
+    if (c0 >= total) return;
+    cta0 = (int)c0;
+    cta1 = (int)min(c0 + (int64_t)WARPS * per, (int64_t)total);
+    r0 = min(cta0 + warp * per, total);
+    r1 = min(r0 + per, total);
   }
-  const int total = cum[P.batch] * items;
-  const int workers = gridDim.x * WARPS;
-  const int per = max((total + workers - 1) / workers, 1);
-  if (blockIdx.x == 0) {
-    for (int b = tid; b <= P.batch; b += WARPS * 32) P.cum[b] = cum[b];
-    if (tid == 0) P.cum[P.batch + 1] = per * WARPS;
-  }
-  const int64_t c0 = (int64_t)blockIdx.x * WARPS * per;  // this CTA's tiles
-  if (c0 >= total) return;
-  const int cta0 = (int)c0, cta1 = (int)min(c0 + (int64_t)WARPS * per, (int64_t)total);
-  const int r0 = min(cta0 + warp * per, total), r1 = min(r0 + per, total);
+  auto item_at = [&](int t) { return ALONE ? alone : item_of(cum, P.batch, items, t); };
+  auto range_at = [&](int b) { return range_of(P, ALONE ? alone_len : lens[b]); };
 
   if (r0 < r1) {
     // ---- the loads' cursor: step `ld` of the row, its item, and 32 tiles (16 steps) from step `from` on in the
     // lanes: the page's id (-1: not there) and the tile's place in it
-    Item li = item_of(cum, P.batch, items, r0);
-    Range lr = range_of(P, li.b);
+    Item li = item_at(r0);
+    Range lr = range_at(li.b);
     int ld = r0, from = -64, id = -1, place = 0;
     const int page_tiles = P.page / TILE;
     const int half = lane >> 4, l16 = lane & 15;
@@ -219,8 +259,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
     auto load = [&](int slot) {
       if (ld < r1) {
         if (ld == li.end) {
-          li = item_of(cum, P.batch, items, ld);
-          lr = range_of(P, li.b);
+          li = item_at(ld);
+          lr = range_at(li.b);
           from = -64;
           const int64_t off = (int64_t)(li.h / P.subs) * P.s_head;
           klane = P.kc + off + 16 * l16;
@@ -256,8 +296,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
     // ---- items of the range
     int t = r0, slot = 0;
     while (t < r1) {
-      const Item it = item_of(cum, P.batch, items, t);
-      const Range rg = range_of(P, it.b);
+      const Item it = item_at(t);
+      const Range rg = range_at(it.b);
       const int stop = min(it.end, r1);
       const int kvh = it.h / P.subs, part = it.h - kvh * P.subs;
       const int heads = min(P.group - part * HEADS, HEADS);
@@ -464,6 +504,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
 
   // ---- pieces of one item in several warps: joined here (thread: head, 4 elements)
   const int head = tid >> 5, e0 = 4 * lane;
+  if (ALONE && cta1 == 0) {  // no key
+    const int kvh = alone.h / P.subs, part = alone.h - kvh * P.subs;
+    if (head < min(P.group - part * HEADS, HEADS))
+      write4(P, alone.b, kvh * P.group + part * HEADS + head, e0, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
   int w = 0;
   while (w < 2 * WARPS) {
     const Item it = part_item[w >> 1][w & 1];
@@ -515,7 +561,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
 }
 
 // Items of several CTAs, and sequences without keys.  One CTA an item; thread: head, 4 elements.
-constexpr int MAX_CTAS = 512;
+constexpr int MAX_CTAS = 512, EARLY = 6;
 __global__ void __launch_bounds__(HEADS * 32) merge_kernel(const __grid_constant__ Params P) {
   __shared__ float weight[HEADS][MAX_CTAS];
   pdl_wait();
@@ -535,6 +581,10 @@ __global__ void __launch_bounds__(HEADS * 32) merge_kernel(const __grid_constant
   if (pieces == 1) return;  // finished there
   // the first CTA's partial is its second (the item begins there), the others' their first
   auto at = [&](int i) { return P.parts + ((int64_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * PART; };
+  float4 early[EARLY];  // the first partials, asked for along with the maxima
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i)
+    early[i] = i < pieces ? *reinterpret_cast<const float4*>(at(i) + head * D + e0) : make_float4(0.f, 0.f, 0.f, 0.f);
   float m = -INFINITY, l = 0.f;
   for (int i = lane; i < pieces; i += 32) m = fmaxf(m, at(i)[HEADS * D + 2 * head]);
 #pragma unroll
@@ -549,8 +599,17 @@ __global__ void __launch_bounds__(HEADS * 32) merge_kernel(const __grid_constant
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   __syncwarp();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i) {
+    if (i >= pieces) break;
+    const float f = weight[head][i];
+    o.x = fmaf(f, early[i].x, o.x);
+    o.y = fmaf(f, early[i].y, o.y);
+    o.z = fmaf(f, early[i].z, o.z);
+    o.w = fmaf(f, early[i].w, o.w);
+  }
 #pragma unroll 4
-  for (int i = 0; i < pieces; ++i) {
+  for (int i = EARLY; i < pieces; ++i) {
     const float f = weight[head][i];
     const float4 x = *reinterpret_cast<const float4*>(at(i) + head * D + e0);
     o.x = fmaf(f, x.x, o.x);
@@ -579,11 +638,25 @@ static int grid_size(int dev) {
 using namespace ada;
 namespace dec = ada::kv4::dec;
 
-// The lists (cum and the tiles a CTA), rounded up to 16 bytes, then two partials a CTA.
+// The lists (cum and the steps a CTA), rounded up to 16 bytes, then two partials a CTA.
 static size_t decode_lists(int32_t batch) { return ((size_t)(batch + 2) * 4 + 15) & ~(size_t)15; }
 
-extern "C" size_t ada_kv4_paged_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t num_kv_heads) {
-  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0) return 0;
+// One CTA an item, and one launch, where an item has at most 40 steps (five a warp) whatever its length and
+// all items are resident at once; otherwise equal shares and a second launch that joins them.  (One sequence
+// of 700 keys, 32/8 heads: 11.3 us shared out, 8.5 alone; 4 x 1,024 keys of a window, 32/16: 14.3 and 10.3.  With
+// 16 warps a CTA 9.6 and 10.7: an SM issues the item's instructions no faster.)
+static bool decode_alone(int64_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t max_pages, int32_t page_size,
+                         int32_t window) {
+  const int64_t group = num_heads / num_kv_heads, items = num_kv_heads * cdiv(group, (int64_t)dec::HEADS);
+  const int64_t all = (int64_t)max_pages * page_size;
+  const int64_t reach = window > 0 && window < all ? (int64_t)window + dec::KEYS - 1 : all;
+  return batch * items <= 2 * 148 && cdiv(reach, (int64_t)dec::KEYS) <= 5 * dec::WARPS;
+}
+
+extern "C" size_t ada_kv4_paged_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t num_kv_heads,
+                                                      int32_t max_pages, int32_t page_size, int32_t window) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_pages <= 0 || page_size <= 0) return 0;
+  if (decode_alone(batch, num_heads, num_kv_heads, max_pages, page_size, window)) return 0;
   return decode_lists(batch) + (size_t)dec::MAX_CTAS * 2 * dec::PART * 4;
 }
 
@@ -612,9 +685,13 @@ extern "C" int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride
   // the row of all tiles is counted in 32 bits
   if (batch > dec::MAX_BATCH || batch * items * tiles > 0x7fffffffLL || batch * items > 0x7fffffffLL)
     return ADA_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < ada_kv4_paged_decode_workspace_size(batch, num_heads, num_kv_heads))
-    return ADA_ERR_WORKSPACE;
-  if (kv4::misaligned16(workspace)) return ADA_ERR_ALIGNMENT;
+  const bool alone = decode_alone(batch, num_heads, num_kv_heads, max_pages, page_size, window);
+  if (!alone) {
+    if (!workspace || workspace_bytes < ada_kv4_paged_decode_workspace_size(batch, num_heads, num_kv_heads, max_pages,
+                                                                            page_size, window))
+      return ADA_ERR_WORKSPACE;
+    if (kv4::misaligned16(workspace)) return ADA_ERR_ALIGNMENT;
+  }
   P.q = q;
   P.q_sb = q_stride_b;
   P.q_sh = q_stride_h;
@@ -640,19 +717,28 @@ extern "C" int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride
   P.cum = static_cast<int*>(workspace);
   P.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + decode_lists(batch));
   static std::atomic<bool> ready[64];
-  constexpr size_t most = dec::WARPS * dec::WARP_SMEM + (dec::MAX_BATCH + 1) * 4;
+  constexpr size_t lists = (size_t)(2 * dec::MAX_BATCH + 1) * 4;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ADA_ERR_CUDA;
   if (!ready[dev]) {
-    if (cudaFuncSetAttribute(dec::split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
+    if (cudaFuncSetAttribute(dec::split_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)(dec::WARPS * dec::WARP_SMEM + lists)) != cudaSuccess ||
+        cudaFuncSetAttribute(dec::split_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             dec::WARPS * dec::WARP_SMEM) != cudaSuccess)
       return ADA_ERR_CUDA;
     ready[dev] = true;
   }
   const int grid = dec::grid_size(dev);
   if (grid == 0) return ADA_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const size_t smem = dec::WARPS * dec::WARP_SMEM + (size_t)(batch + 1) * 4;
-  (void)launch_k(dec::split_kernel, dim3((unsigned)grid), dim3(dec::WARPS * 32), smem, st, P);
+  if (alone) {
+    (void)launch_k(dec::split_kernel<true>, dim3((unsigned)(batch * items)), dim3(dec::WARPS * 32),
+                   dec::WARPS * dec::WARP_SMEM, st, P);
+    ADA_CHECK_LAUNCH();
+    return ADA_OK;
+  }
+  const size_t smem = dec::WARPS * dec::WARP_SMEM + (batch <= 32 ? dec::WARPS * 72 * 4 : (size_t)(2 * batch + 1) * 4);
+  (void)launch_k(dec::split_kernel<false>, dim3((unsigned)grid), dim3(dec::WARPS * 32), smem, st, P);
   ADA_CHECK_LAUNCH();
   (void)launch_k(dec::merge_kernel, dim3((unsigned)(batch * items)), dim3(dec::HEADS * 32), 0, st, P);
   ADA_CHECK_LAUNCH();

@@ -150,8 +150,11 @@ def read_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping:
 
 
 @functools.lru_cache(maxsize=512)
-def paged_decode_fp4_workspace_bytes(batch: int, num_heads: int, num_kv_heads: int) -> int:
-    return int(N.lib().ada_kv4_paged_decode_workspace_size(batch, num_heads, num_kv_heads))
+def paged_decode_fp4_workspace_bytes(batch: int, num_heads: int, num_kv_heads: int, max_pages: int, page_size: int,
+                                     window: int = 0) -> int:
+    """0 where one launch does it (short tables and windows)."""
+    return int(N.lib().ada_kv4_paged_decode_workspace_size(batch, num_heads, num_kv_heads, max_pages, page_size,
+                                                           min(window, LARGEST)))
 
 
 def _attention(device, q, block_tables, out, *lists):
@@ -182,7 +185,7 @@ def paged_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     q [B, Hq, 128] bf16/fp16; k_cache/v_cache uint8 [pages, Hkv, page * 72]; block_tables int32 [B, max_pages]
     (ids outside the cache are masked); context_lens int32 [B], the new token included.  window W > 0: the last
     W tokens.  Returns [B, Hq, 128] in q.dtype; a sequence without keys gives zeros.  workspace: at
-    least paged_decode_fp4_workspace_bytes(B, Hq, Hkv) bytes (default: allocated for the call)."""
+    least paged_decode_fp4_workspace_bytes(...) bytes (default: allocated for the call)."""
     device = N.one_device("paged_decode_fp4", q, k_cache, v_cache, block_tables, context_lens)
     pages, hkv, page, s_page, s_head = _cache(k_cache, v_cache)
     q, code, out, out_code = _attention(device, q, block_tables, out, context_lens)
@@ -192,12 +195,15 @@ def paged_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError("block_tables and context_lens must have one entry per sequence")
     if batch == 0:
         return out
+    at = 0
     if workspace is None:
-        # one of its own: the launches of another thread's call on this stream may fall between this call's
-        size = paged_decode_fp4_workspace_bytes(batch, hq, hkv)
-        workspace = k_cache.new_empty(size)
+        size = paged_decode_fp4_workspace_bytes(batch, hq, hkv, max_pages, page, window)
+        if size:
+            # one of its own: the launches of another thread's call on this stream may fall between this call's
+            workspace = k_cache.new_empty(size)
+            at = workspace.data_ptr()
     else:
-        size = workspace.nbytes
+        size, at = workspace.nbytes, workspace.data_ptr()
         if workspace.get_device() != device or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous on q's device")
     qs, os = q.stride(), out.stride()
@@ -205,7 +211,7 @@ def paged_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                             s_head, pages, block_tables.data_ptr(), block_tables.stride(0), max_pages,
                             context_lens.data_ptr(), batch, hq, hkv, d, page, scale, k_scale, v_scale,
                             window if window < LARGEST else LARGEST, out.data_ptr(), out_code, os[0], os[1],
-                            workspace.data_ptr(), size, N.raw_stream(device))
+                            at, size, N.raw_stream(device))
     if st:
         N.check(st, "4-bit KV decode kernel")
     return out

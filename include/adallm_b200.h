@@ -732,9 +732,11 @@ ADA_API int ada_kv4_read(const uint8_t* k_cache, const uint8_t* v_cache, int64_t
 /* Decode attention over the 4-bit cache: arguments and masks as ada_fp8_paged_decode (window W > 0: the last W
  * tokens; a zero-length sequence and one that sees no key give zeros), any number of heads a KV
  * head.  Keys, values and probabilities enter the products in fp16, bf16 queries exactly (scaled by a power of two).
- * workspace: ada_kv4_paged_decode_workspace_size bytes, 16-byte aligned, no initial value; calls that
- * share one must be ordered as a whole. */
-ADA_API size_t ada_kv4_paged_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t num_kv_heads);
+ * out may have any strides that are multiples of 8.  workspace: ada_kv4_paged_decode_workspace_size bytes (0 for
+ * short caches and windows: one launch), 16-byte aligned, no initial value; calls that share one must be
+ * ordered as a whole.  Implemented: batch <= 8192, batch x KV heads x 32-key steps of a table row below 2^31. */
+ADA_API size_t ada_kv4_paged_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t num_kv_heads,
+                                                   int32_t max_pages, int32_t page_size, int32_t window);
 ADA_API int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h,
                                  const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
                                  int64_t kv_stride_head, int64_t num_pages, const int32_t* block_tables,

@@ -198,12 +198,27 @@ def test_decode_matches_64_bits(lens, hq, hkv, page, window, dtype):
 def test_decode_scales_output_type_strides_and_workspace():
     c = make(3, [100, 600], [1, 1], 16, 4, 16)
     wide = torch.full((2, 20, 144), 7.0, dtype=F16, device=dev())
-    ws = torch.full((kv.paged_decode_fp4_workspace_bytes(2, 16, 4),), 0xFF, dtype=torch.uint8, device=dev())
+    ws = torch.full((max(16, kv.paged_decode_fp4_workspace_bytes(2, 16, 4, c["tables"].shape[1], 16)),), 0xFF, dtype=torch.uint8, device=dev())
     q = c["q"]
     c["q"] = torch.nn.functional.pad(q, (0, 8, 1, 1))[:, 1:17, :128]
     out = run_decode(c, 0, 0.37, 0.05, 0.2, out=wide[:, 2:18, 8:136], workspace=ws)
     assert_near(out, *want_of(c, 0, 0.37, 0.05, 0.2))
     assert (wide[:, :2] == 7).all() and (wide[:, 18:] == 7).all() and (wide[..., :8] == 7).all()
+
+
+def test_decode_forms_agree():
+    """The same sequences behind tables that select one launch and two (lengths 0, 1, whole steps, ragged)."""
+    for lens, window in (([1280, 0, 1, 31, 32, 33, 64, 777], 0), ([5000, 1279, 40, 0], 1200)):
+        c = make(41, lens, [1] * len(lens), 16, 4, 16)
+        if window == 0:
+            c["tables"] = c["tables"][:, :80].contiguous()
+        assert kv.paged_decode_fp4_workspace_bytes(len(lens), 16, 4, c["tables"].shape[1], 16, window) == 0
+        want, err = want_of(c, window)
+        assert_near(run_decode(c, window), want, err)
+        wide = dict(c, tables=torch.nn.functional.pad(c["tables"], (0, 200), value=-1))
+        if window == 0:
+            assert kv.paged_decode_fp4_workspace_bytes(len(lens), 16, 4, wide["tables"].shape[1], 16) > 0
+            assert_near(run_decode(wide), want, err)
 
 
 def test_decode_batch_of_thousands():
@@ -348,7 +363,7 @@ def test_split_prefill_and_decode_agree_with_one_prefill():
 
 
 def test_streams_graphs_and_two_calls_at_once():
-    a, b = (make(s, [900, 3, 250], [1, 1, 1], 32, 8, 16) for s in (31, 32))
+    a, b = (make(s, [2900, 3, 250], [1, 1, 1], 32, 8, 16) for s in (31, 32))
     wa, wb = run_decode(a), run_decode(b)
     pa = run_prefill(a)
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
@@ -361,7 +376,9 @@ def test_streams_graphs_and_two_calls_at_once():
         torch.cuda.synchronize()
         assert torch.equal(x, wa) and torch.equal(y, wb)
     # two graphs with one workspace, replayed in turn
-    ws = torch.empty(kv.paged_decode_fp4_workspace_bytes(3, 32, 8), dtype=torch.uint8, device=dev())
+    size = kv.paged_decode_fp4_workspace_bytes(3, 32, 8, a["tables"].shape[1], 16)
+    assert size > 0 and size == kv.paged_decode_fp4_workspace_bytes(3, 32, 8, b["tables"].shape[1], 16)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev())
     outs, graphs = [], []
     for c in (a, b):
         o = torch.zeros_like(c["q"])
@@ -415,7 +432,8 @@ def test_refusals():
     bad(dec, q, k, v, t, ctx, 0.1, k_scale=-1.0)
     bad(dec, q, k, v, t, ctx, 0.1, v_scale=0.0)
     bad(dec, q, k, v, t, ctx, 0.1, out=torch.empty((2, 8, 64), dtype=BF16, device=dev()))
-    bad(dec, q, k, v, t, ctx, 0.1, workspace=torch.empty(8, dtype=torch.uint8, device=dev()))
+    wide = torch.nn.functional.pad(t, (0, 200), value=-1)
+    bad(dec, q, k, v, wide, ctx, 0.1, workspace=torch.empty(8, dtype=torch.uint8, device=dev()))
     bad(dec, q, k, v, t.cpu(), ctx, 0.1, error=RuntimeError)
     cu = torch.tensor([0, 1, 2], dtype=i32, device=dev())
     bad(pre, q, k, v, t, cu.long(), cu, 1, 0.1)

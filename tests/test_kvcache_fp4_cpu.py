@@ -44,9 +44,11 @@ def test_decode_refusals(lib):
         (dict(scale=math.nan), BAD), (dict(ks=-1.0), BAD), (dict(vs=0.0), BAD), (dict(q=8), ALIGN), (dict(k=8), ALIGN),
         (dict(out=24), ALIGN), (dict(qsh=132), ALIGN), (dict(osb=4100), ALIGN), (dict(sh=1160, sp=9999), ALIGN),
         (dict(sp=8 * 1152 + 8), ALIGN), (dict(sh=1136), BAD), (dict(bt=18), ALIGN), (dict(ctx=17), ALIGN),
-        (dict(mp=1 << 27, bts=1 << 27), UNSUP), (dict(ws=None), WS), (dict(wsb=1), WS)])
-    assert lib.ada_kv4_paged_decode_workspace_size(0, 32, 8) == 0
-    assert lib.ada_kv4_paged_decode_workspace_size(16, 32, 8) > 0
+        (dict(mp=1 << 27, bts=1 << 27), UNSUP), (dict(mp=200, bts=200, ws=None), WS),
+        (dict(mp=200, bts=200, wsb=1), WS), (dict(mp=200, bts=200, ws=24), ALIGN), (dict(batch=8193), UNSUP)])
+    size = lib.ada_kv4_paged_decode_workspace_size
+    assert size(0, 32, 8, 100, 16, 0) == 0 and size(16, 32, 8, 100, 16, 0) > 0
+    assert size(1, 32, 8, 80, 16, 0) == 0 and size(1, 32, 8, 81, 16, 0) > 0 and size(37, 32, 8, 81, 16, 1000) == 0
 
 
 PREFILL = dict(q=16, qd=0, qst=1024, qsh=128, k=16, v=16, sp=8 * 1152, sh=1152, pages=4, bt=16, bts=4, mp=4, cq=16, ck=16,
