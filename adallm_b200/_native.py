@@ -89,7 +89,8 @@ _SIGS = {
     "ada_kv4_paged_decode": (INT, [P, INT, I64, I64, P, P, I64, I64, I64, P, I64, I32, P, I32, I32, I32, I32, I32, F32,
                                    F32, F32, I32, P, INT, I64, I64, P, SZ, P]),
     "ada_kv4_paged_prefill": (INT, [P, INT, I64, I64, P, P, I64, I64, I64, P, I64, I32, P, P, I32, I64, I32, I32, I32,
-                                    I32, I32, F32, F32, F32, I32, P, INT, I64, I64, P, P]),
+                                    I32, I32, F32, F32, F32, I32, P, INT, I64, I64, P, SZ, P, P]),
+    "ada_kv4_paged_prefill_workspace_size": (SZ, [I32, I64, I32, I32, I32, I32, I32]),
     "ada_call": (INT, [INT, C.c_char_p]),
     "ada_nvfp4_sf_bytes": (SZ, [I64, I64]),
     "ada_nvfp4_prepack_scales": (INT, [P, INT, I64, I64, I64, P, P]),
@@ -247,7 +248,7 @@ rotary = Packed(2, "19q")
 kv4_store = Packed(3, "26q2d2q")
 kv4_read = Packed(4, "10q2d4q")
 kv4_paged_decode = Packed(5, "18q3d8q")
-kv4_paged_prefill = Packed(6, "21q3d7q")
+kv4_paged_prefill = Packed(6, "21q3d9q")
 
 
 def one_device(what: str, *tensors: torch.Tensor) -> int:

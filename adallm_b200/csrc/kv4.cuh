@@ -161,5 +161,13 @@ inline int attn_ok(const void* q, int qd, int64_t q_st, int64_t q_sh, const void
   return ADA_OK;
 }
 
+// Prefill of a few new tokens a sequence, in kv4_decode.cu; workspace as sized there.
+size_t rows_workspace_size(int32_t batch);
+int rows_prefill(const void* q, int q_dtype, int64_t q_st, int64_t q_sh, const uint8_t* kc, const uint8_t* vc,
+                 int64_t s_page, int64_t s_head, int64_t num_pages, const int32_t* bt, int64_t bt_stride,
+                 int32_t max_pages, const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int64_t rows, int32_t most,
+                 int32_t hq, int32_t hkv, int32_t page, float scale_log2, float v_scale, int32_t window, void* out,
+                 int out_dtype, int64_t o_st, int64_t o_sh, void* workspace, cudaStream_t st);
+
 }  // namespace kv4
 }  // namespace ada

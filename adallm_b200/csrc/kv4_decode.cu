@@ -56,47 +56,77 @@ struct Params {
   int64_t s_page, s_head, num_pages;
   const int32_t* bt;
   int64_t bt_stride;
-  int max_pages, page, window, batch;
-  int hkv, group, subs;  // subs: parts of at most 8 heads of a group
-  const int32_t* lens;
+  int max_pages, page, batch;
+  int span;              // keys that a row sees at most (0: all before it)
+  int hkv, group, subs;  // subs: parts of 8 columns ((token, head) pairs of a KV head's group) a sequence has at most
+  const int32_t* lens;          // decode: keys of each sequence
+  const int32_t *cu_q, *cu_k;   // rows: prefix sums of new tokens and of keys
+  int most;                     // rows: tokens of a sequence that are computed
+  int64_t rows;                 // of q and out
   float scale_log2, v_scale;
-  int* cum;      // workspace: [batch + 1] tiles before a sequence (times items a sequence), then tiles a CTA
+  int* cum;      // workspace: [batch + 1] (steps x parts) before a sequence, then steps a CTA
   float* parts;  // workspace: [grid][2][PART]
 };
 
-struct Range {
-  int lo, hi, first;  // visible keys, first step
+// A sequence: its keys, its new tokens (1 for decode), and how many of them are computed.
+struct Seq {
+  int keys, fresh, tokens;
 };
-__device__ __forceinline__ Range range_of(const Params& P, int len) {
-  const int full = max(len, 0);
+template <bool ROWS>
+__device__ __forceinline__ Seq seq_of(const Params& P, int keys, int fresh) {
+  constexpr int MOST = 1 << 30;
+  if (!ROWS) return {min(max(keys, 0), MOST), 1, 1};
+  const int n = min(max(fresh, 0), MOST);
+  return {min(max(keys, 0), MOST), n, min(n, P.most)};
+}
+template <bool ROWS>
+__device__ __forceinline__ Seq load_seq(const Params& P, int b) {
+  if (!ROWS) return seq_of<ROWS>(P, __ldg(P.lens + b), 1);
+  // (differences of lists that do not ascend may wrap: any value is as good as another there)
+  const unsigned k0 = (unsigned)__ldg(P.cu_k + b), k1 = (unsigned)__ldg(P.cu_k + b + 1);
+  const unsigned q0 = (unsigned)__ldg(P.cu_q + b), q1 = (unsigned)__ldg(P.cu_q + b + 1);
+  return seq_of<ROWS>(P, (int)(k1 - k0), (int)(q1 - q0));
+}
+// Keys [lo, hi) that token i of a sequence sees (0 <= i < tokens).
+__device__ __forceinline__ int lo_of(const Params& P, const Seq& q, int i) {
+  return P.span > 0 ? max(q.keys - q.fresh + i + 1 - P.span, 0) : 0;
+}
+__device__ __forceinline__ int hi_of(const Params& P, const Seq& q, int i) {
+  return max(min(min(q.keys, P.max_pages * P.page), q.keys - q.fresh + i + 1), 0);
+}
+struct Range {
+  int lo, hi, first;  // keys that any token sees, first step
+};
+__device__ __forceinline__ Range range_of(const Params& P, const Seq& q) {
   Range r;
-  r.hi = min(full, P.max_pages * P.page);
-  r.lo = P.window > 0 ? max(full - P.window, 0) : 0;
+  r.lo = lo_of(P, q, 0);
+  r.hi = q.tokens > 0 ? hi_of(P, q, q.tokens - 1) : 0;
   r.first = r.lo / KEYS;
   return r;
 }
 __device__ __forceinline__ int steps_of(const Range& r) {
   return r.hi > r.lo ? (r.hi + KEYS - 1) / KEYS - r.first : 0;
 }
+template <bool ROWS>
+__device__ __forceinline__ int parts_of(const Params& P, const Seq& q) {
+  return ROWS ? (q.tokens * P.group + HEADS - 1) / HEADS : P.subs;
+}
 
-// One (sequence, KV head, part of its heads), and where its tiles stand in the row of all.
+// One (sequence, KV head, part of its columns), and where its steps stand in the row of all.
 struct Item {
-  int b, h, base, end;  // h: KV head * subs + part
+  int b, kvh, part, base, end;
 };
-// The item of tile t (cum: tiles before a sequence, for one of its `items` items).
-__device__ __forceinline__ Item item_of(const int* cum, int batch, int items, int t) {
+// The sequence of step t (cum: steps x parts before a sequence, for one KV head).
+__device__ __forceinline__ int seq_at(const int* cum, int batch, int hkv, int t) {
   int lo = 0, hi = batch - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (cum[mid + 1] * items > t)
+    if (cum[mid + 1] * hkv > t)
       hi = mid;
     else
       lo = mid + 1;
   }
-  const int n = cum[lo + 1] - cum[lo];
-  const int h = (t - cum[lo] * items) / n;
-  const int base = cum[lo] * items + h * n;
-  return {lo, h, base, base + n};
+  return lo;
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
@@ -111,25 +141,25 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 __device__ __forceinline__ int chunk_at(int line, int chunk) { return line * 128 + ((chunk ^ (2 * (line & 3))) << 4); }
 
 // Row of one head to memory: 16 elements of lane's scale block.
-__device__ __forceinline__ void write16(const Params& P, int b, int head, int e0, const float* f) {
+__device__ __forceinline__ void write16(const Params& P, int64_t row, int head, int e0, const float* f) {
   if (P.o_bf16) {
-    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(P.out) + b * P.o_sb + head * P.o_sh + e0;
+    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(P.out) + row * P.o_sb + head * P.o_sh + e0;
     *reinterpret_cast<uint4*>(o) = pack8<__nv_bfloat16>(f);
     *reinterpret_cast<uint4*>(o + 8) = pack8<__nv_bfloat16>(f + 8);
   } else {
-    __half* o = reinterpret_cast<__half*>(P.out) + b * P.o_sb + head * P.o_sh + e0;
+    __half* o = reinterpret_cast<__half*>(P.out) + row * P.o_sb + head * P.o_sh + e0;
     *reinterpret_cast<uint4*>(o) = pack8<__half>(f);
     *reinterpret_cast<uint4*>(o + 8) = pack8<__half>(f + 8);
   }
 }
-__device__ __forceinline__ void write4(const Params& P, int b, int head, int e0, float4 f) {
+__device__ __forceinline__ void write4(const Params& P, int64_t row, int head, int e0, float4 f) {
   if (P.o_bf16) {
     __nv_bfloat162 u[2] = {__floats2bfloat162_rn(f.x, f.y), __floats2bfloat162_rn(f.z, f.w)};
-    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + b * P.o_sb + head * P.o_sh + e0) =
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + row * P.o_sb + head * P.o_sh + e0) =
         *reinterpret_cast<uint2*>(u);
   } else {
     __half2 u[2] = {__floats2half2_rn(f.x, f.y), __floats2half2_rn(f.z, f.w)};
-    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(P.out) + b * P.o_sb + head * P.o_sh + e0) =
+    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(P.out) + row * P.o_sb + head * P.o_sh + e0) =
         *reinterpret_cast<uint2*>(u);
   }
 }
@@ -140,8 +170,21 @@ struct Acc {
   float l[2];
 };
 
+// Column n of a part: its row of q and out and its head; false where there is none.
+template <bool ROWS>
+__device__ __forceinline__ bool column(const Params& P, const Item& it, const Seq& q, int64_t q0, int n, int64_t& row,
+                                       int& head, int& token) {
+  const int col = it.part * HEADS + n;
+  token = ROWS ? col / P.group : 0;
+  head = it.kvh * P.group + (ROWS ? col - token * P.group : col);
+  row = ROWS ? q0 + token : it.b;
+  return ROWS ? token < q.tokens && row >= 0 && row < P.rows : col < P.group;
+}
+
 // ALONE: one CTA an item, which it finishes; otherwise the steps of all items shared out equally.
-template <bool ALONE>
+// ROWS: a few new tokens a sequence, whose rows are columns beside each other as the heads are (the keys are
+// read once for 8 of them), each with a last key of its own; otherwise one token, the newest.
+template <bool ALONE, bool ROWS>
 __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_constant__ Params P) {
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int warp_sum[WARPS];
@@ -152,38 +195,42 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
   // steps before each sequence, and the lengths (a copy a warp for up to 32 sequences: no barrier)
   int* lists = reinterpret_cast<int*>(sm + WARPS * WARP_SMEM);
   const bool few = P.batch <= 32;
-  int* cum = few ? lists + warp * 72 : lists;
-  int* lens = few ? cum + 36 : lists + P.batch + 1;
-  const int items = P.hkv * P.subs;
+  int* cum = few ? lists + warp * 108 : lists;
+  int* keys = few ? cum + 36 : lists + P.batch + 1;
+  int* fresh = few ? keys + 36 : keys + P.batch;  // (ROWS)
   if (lane < 2) part_item[warp][lane].end = 0;  // no partial
   pdl_wait();
   pdl_trigger();
 
   int cta0, cta1, r0, r1;
-  Item alone{0, 0, 0, 0};
-  int alone_len = 0;
+  Item alone{0, 0, 0, 0, 0};
+  Seq alone_seq{0, 0, 0};
   if (ALONE) {
+    const int items = P.hkv * P.subs, h = blockIdx.x % items;
     alone.b = blockIdx.x / items;
-    alone.h = blockIdx.x - alone.b * items;
-    alone_len = __ldg(P.lens + alone.b);
-    alone.end = steps_of(range_of(P, alone_len));
+    alone.kvh = h / P.subs;
+    alone.part = h - alone.kvh * P.subs;
+    alone_seq = load_seq<ROWS>(P, alone.b);
+    alone.end = steps_of(range_of(P, alone_seq));
     const int per = (alone.end + WARPS - 1) / WARPS;
     cta0 = 0;
     cta1 = alone.end;
     r0 = min(warp * per, cta1);
     r1 = min(r0 + per, cta1);
   } else {
+    auto cost = [&](const Seq& q) { return steps_of(range_of(P, q)) * parts_of<ROWS>(P, q); };
     if (few) {
-      const int len = lane < P.batch ? __ldg(P.lens + lane) : 0;
-      const int n = lane < P.batch ? steps_of(range_of(P, len)) : 0;
-      int inc = n;
+      Seq q{0, 0, 0};
+      if (lane < P.batch) q = load_seq<ROWS>(P, lane);
+      int inc = lane < P.batch ? cost(q) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += up;
       }
       cum[lane + 1] = inc;
-      lens[lane] = len;
+      keys[lane] = q.keys;
+      if (ROWS) fresh[lane] = q.fresh;
       if (lane == 0) cum[0] = 0;
       __syncwarp();
     } else {
@@ -191,8 +238,10 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       const int b0 = min(tid * per, P.batch), b1 = min(b0 + per, P.batch);
       int sum = 0;
       for (int b = b0; b < b1; ++b) {
-        lens[b] = __ldg(P.lens + b);
-        sum += steps_of(range_of(P, lens[b]));
+        const Seq q = load_seq<ROWS>(P, b);
+        keys[b] = q.keys;
+        if (ROWS) fresh[b] = q.fresh;
+        sum += cost(q);
       }
       int inc = sum;
 #pragma unroll
@@ -206,12 +255,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       for (int w = 0; w < warp; ++w) run += warp_sum[w];
       for (int b = b0; b < b1; ++b) {
         cum[b] = run;
-        run += steps_of(range_of(P, lens[b]));
+        run += cost(seq_of<ROWS>(P, keys[b], ROWS ? fresh[b] : 1));
       }
       if (b0 < b1 && b1 == P.batch) cum[P.batch] = run;
       __syncthreads();
     }
-    const int total = cum[P.batch] * items;
+    const int total = cum[P.batch] * P.hkv;
     const int workers = gridDim.x * WARPS;
     const int per = max((total + workers - 1) / workers, 1);
     if (blockIdx.x == 0) {  // for the merge (with few sequences every warp has the lists, and the first writes them)
@@ -226,8 +275,20 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
     r0 = min(cta0 + warp * per, total);
     r1 = min(r0 + per, total);
   }
-  auto item_at = [&](int t) { return ALONE ? alone : item_of(cum, P.batch, items, t); };
-  auto range_at = [&](int b) { return range_of(P, ALONE ? alone_len : lens[b]); };
+  auto seq_in = [&](int b) { return ALONE ? alone_seq : seq_of<ROWS>(P, keys[b], ROWS ? fresh[b] : 1); };
+  auto item_at = [&](int t) {  // (the step's item has steps, so there are parts)
+    if (ALONE) return alone;
+    Item it;
+    it.b = seq_at(cum, P.batch, P.hkv, t);
+    const Seq q = seq_in(it.b);
+    const int n = steps_of(range_of(P, q)), parts = parts_of<ROWS>(P, q), h = (t - cum[it.b] * P.hkv) / n;
+    it.kvh = h / parts;
+    it.part = h - it.kvh * parts;
+    it.base = cum[it.b] * P.hkv + h * n;
+    it.end = it.base + n;
+    return it;
+  };
+  auto range_at = [&](int b) { return range_of(P, seq_in(b)); };
 
   if (r0 < r1) {
     // ---- the loads' cursor: step `ld` of the row, its item, and 32 tiles (16 steps) from step `from` on in the
@@ -237,7 +298,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
     int ld = r0, from = -64, id = -1, place = 0;
     const int page_tiles = P.page / TILE;
     const int half = lane >> 4, l16 = lane & 15;
-    const int64_t head_off = (int64_t)(li.h / P.subs) * P.s_head;
+    const int64_t head_off = (int64_t)li.kvh * P.s_head;
     const uint8_t *klane = P.kc + head_off + 16 * l16, *vlane = P.vc + head_off + 16 * l16;
     auto look = [&]() {
       from = ld;
@@ -262,7 +323,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
           li = item_at(ld);
           lr = range_at(li.b);
           from = -64;
-          const int64_t off = (int64_t)(li.h / P.subs) * P.s_head;
+          const int64_t off = (int64_t)li.kvh * P.s_head;
           klane = P.kc + off + 16 * l16;
           vlane = P.vc + off + 16 * l16;
         }
@@ -299,10 +360,21 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       const Item it = item_at(t);
       const Range rg = range_at(it.b);
       const int stop = min(it.end, r1);
-      const int kvh = it.h / P.subs, part = it.h - kvh * P.subs;
-      const int heads = min(P.group - part * HEADS, HEADS);
-      const int head0 = kvh * P.group + part * HEADS;
-      // queries: head g, elements [32c, 32c + 32)
+      const Seq sq = seq_in(it.b);
+      const int64_t q0 = ROWS ? __ldg(P.cu_q + it.b) : 0;
+      int64_t row;
+      int head, token;
+      // ROWS: keys that this lane's columns 2c, 2c + 1 see, and where all columns of the part see the same
+      int lo0 = 0, hi0 = 0, lo1 = 0, hi1 = 0, lo_all = rg.lo, hi_all = rg.hi;
+      if (ROWS) {
+        if (column<ROWS>(P, it, sq, q0, 2 * c, row, head, token)) lo0 = lo_of(P, sq, token), hi0 = hi_of(P, sq, token);
+        if (column<ROWS>(P, it, sq, q0, 2 * c + 1, row, head, token))
+          lo1 = lo_of(P, sq, token), hi1 = hi_of(P, sq, token);
+        lo_all = lo_of(P, sq, min((it.part * HEADS + HEADS - 1) / P.group, sq.tokens - 1));
+        hi_all = hi_of(P, sq, it.part * HEADS / P.group);
+      }
+      // queries: column g, elements [32c, 32c + 32)
+      const bool mine = column<ROWS>(P, it, sq, q0, g, row, head, token);
       uint32_t qf[16];
       float fac[2];
       {
@@ -310,8 +382,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
         float f[32];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (g < heads) {
-            const int64_t off = it.b * P.q_sb + (head0 + g) * P.q_sh + 32 * c + 8 * i;
+          if (mine) {
+            const int64_t off = row * P.q_sb + head * P.q_sh + 32 * c + 8 * i;
             if (P.q_bf16)
               unpack8<__nv_bfloat16>(*reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(P.q) + off), f + 8 * i);
             else
@@ -346,7 +418,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
         const uint8_t* step = ring + slot * STEP_BYTES;
         const uint32_t ok = (there >> (2 * slot)) & 3u;
         const int key0 = (rg.first + (t - it.base)) * KEYS;
-        const bool edge = key0 < rg.lo || key0 + KEYS > rg.hi || ok != 3u;
+        const bool edge = key0 < lo_all || key0 + KEYS > hi_all || ok != 3u;
         // scores: tile i, keys g, g + 8 x heads 2c, 2c + 1
         float s[2][4];
         uint32_t vs[2][2];  // scales of block g, keys (2c, 2c + 1) and (2c + 8, 2c + 9)
@@ -380,13 +452,49 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
           for (int i = 0; i < 2; ++i) {
             const int k = key0 + i * TILE, hi = (ok >> i) & 1u ? rg.hi : 0;
             auto seen = [&](int key) { return key >= rg.lo && key < hi; };
-            if (!seen(k + g)) s[i][0] = s[i][1] = -INFINITY;
-            if (!seen(k + g + 8)) s[i][2] = s[i][3] = -INFINITY;
+            if (ROWS) {
+              const int ha = min(hi0, hi), hb = min(hi1, hi);
+              if (k + g < lo0 || k + g >= ha) s[i][0] = -INFINITY;
+              if (k + g < lo1 || k + g >= hb) s[i][1] = -INFINITY;
+              if (k + g + 8 < lo0 || k + g + 8 >= ha) s[i][2] = -INFINITY;
+              if (k + g + 8 < lo1 || k + g + 8 >= hb) s[i][3] = -INFINITY;
+            } else {
+              if (!seen(k + g)) s[i][0] = s[i][1] = -INFINITY;
+              if (!seen(k + g + 8)) s[i][2] = s[i][3] = -INFINITY;
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               if (!seen(k + 2 * c + 8 * j)) vs[i][j] &= 0xFF00u;
               if (!seen(k + 2 * c + 8 * j + 1)) vs[i][j] &= 0x00FFu;
             }
+          }
+        }
+        if (ROWS && edge) {
+          // A value's NaN would reach columns that do not see its key, through 0 * NaN: it counts as 0, and the
+          // columns that see it get their 16 elements' NaN here (rare: a vote says whether there is one).
+          uint32_t bad = 0;  // bit 4i + 2j + x: key 16i + 8j + 2c + x
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const uint32_t v = vs[n >> 2][(n >> 1) & 1] >> (8 * (n & 1));
+            if ((v & 0x7Fu) == 0x7Fu) bad |= 1u << n;
+          }
+          if (__any_sync(0xffffffffu, bad != 0)) {
+            const float nan = __uint_as_float(0x7FC00000u);
+            for (int o = 0; o < 4; ++o) {
+              const uint32_t theirs = __shfl_sync(0xffffffffu, bad, (lane & ~3) + o);
+              for (int n = 0; n < 8; ++n) {
+                const int key = key0 + 16 * (n >> 2) + 8 * ((n >> 1) & 1) + 2 * o + (n & 1);
+                if (!((theirs >> n) & 1u)) continue;
+#pragma unroll
+                for (int m = 0; m < 8; ++m) {
+                  if (key >= lo0 && key < hi0) a.o[m][0] = a.o[m][2] = nan;
+                  if (key >= lo1 && key < hi1) a.o[m][1] = a.o[m][3] = nan;
+                }
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+              if ((bad >> n) & 1u) vs[n >> 2][(n >> 1) & 1] &= n & 1 ? 0x00FFu : 0xFF00u;
           }
         }
         const float x0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
@@ -465,7 +573,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       if (began && ended) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          if (2 * c + x >= heads) continue;
+          if (!column<ROWS>(P, it, sq, q0, 2 * c + x, row, head, token)) continue;
           // (a NaN sum stays one)
           const float inv = a.l[x] == 0.f ? 0.f : P.v_scale / a.l[x];
           float f[16];
@@ -474,7 +582,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
             f[2 * m] = a.o[m][x] * inv;
             f[2 * m + 1] = a.o[m][2 + x] * inv;
           }
-          write16(P, it.b, head0 + 2 * c + x, 16 * g, f);
+          write16(P, row, head, 16 * g, f);
         }
       } else {
         // the last piece's partial may lie in the ring: its own copies have arrived
@@ -502,12 +610,18 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
   }
   __syncthreads();
 
-  // ---- pieces of one item in several warps: joined here (thread: head, 4 elements)
-  const int head = tid >> 5, e0 = 4 * lane;
+  // ---- pieces of one item in several warps: joined here (thread: column, 4 elements)
+  const int col = tid >> 5, e0 = 4 * lane;
+  auto finish = [&](const Item& it, float4 o, float l) {
+    const Seq q = seq_in(it.b);
+    int64_t row;
+    int head, token;
+    if (!column<ROWS>(P, it, q, ROWS ? __ldg(P.cu_q + it.b) : 0, col, row, head, token)) return;
+    const float inv = l == 0.f ? 0.f : P.v_scale / l;
+    write4(P, row, head, e0, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+  };
   if (ALONE && cta1 == 0) {  // no key
-    const int kvh = alone.h / P.subs, part = alone.h - kvh * P.subs;
-    if (head < min(P.group - part * HEADS, HEADS))
-      write4(P, alone.b, kvh * P.group + part * HEADS + head, e0, make_float4(0.f, 0.f, 0.f, 0.f));
+    finish(alone, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
     return;
   }
   int w = 0;
@@ -528,32 +642,28 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       return reinterpret_cast<const float*>(n & 1 ? r : r + STAGES * STEP_BYTES);
     };
     float m = -INFINITY;
-    for (int n = w; n <= last; n = ((n >> 1) + 1) * 2) m = fmaxf(m, piece(n)[HEADS * D + 2 * head]);
+    for (int n = w; n <= last; n = ((n >> 1) + 1) * 2) m = fmaxf(m, piece(n)[HEADS * D + 2 * col]);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int n = w; n <= last; n = ((n >> 1) + 1) * 2) {
       const float* p = piece(n);
-      const float pm = p[HEADS * D + 2 * head];
+      const float pm = p[HEADS * D + 2 * col];
       const float f = m == -INFINITY ? 1.f : fast_exp2(pm - m);
-      const float4 x = *reinterpret_cast<const float4*>(p + head * D + e0);
-      l = fmaf(f, p[HEADS * D + 2 * head + 1], l);
+      const float4 x = *reinterpret_cast<const float4*>(p + col * D + e0);
+      l = fmaf(f, p[HEADS * D + 2 * col + 1], l);
       o.x = fmaf(f, x.x, o.x);
       o.y = fmaf(f, x.y, o.y);
       o.z = fmaf(f, x.z, o.z);
       o.w = fmaf(f, x.w, o.w);
     }
     if (it.base >= cta0 && it.end <= cta1) {
-      const int kvh = it.h / P.subs, part = it.h - kvh * P.subs;
-      if (head < min(P.group - part * HEADS, HEADS)) {
-        const float inv = l == 0.f ? 0.f : P.v_scale / l;
-        write4(P, it.b, kvh * P.group + part * HEADS + head, e0, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-      }
+      finish(it, o, l);
     } else {
       float* dst = P.parts + ((int64_t)blockIdx.x * 2 + (it.base >= cta0 ? 1 : 0)) * PART;
-      *reinterpret_cast<float4*>(dst + head * D + e0) = o;
+      *reinterpret_cast<float4*>(dst + col * D + e0) = o;
       if (lane == 0) {
-        dst[HEADS * D + 2 * head] = m;
-        dst[HEADS * D + 2 * head + 1] = l;
+        dst[HEADS * D + 2 * col] = m;
+        dst[HEADS * D + 2 * col + 1] = l;
       }
     }
     w = last + 1;
@@ -562,21 +672,27 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
 
 // Items of several CTAs, and sequences without keys.  One CTA an item; thread: head, 4 elements.
 constexpr int MAX_CTAS = 512, EARLY = 6;
+template <bool ROWS>
 __global__ void __launch_bounds__(HEADS * 32) merge_kernel(const __grid_constant__ Params P) {
   __shared__ float weight[HEADS][MAX_CTAS];
   pdl_wait();
   pdl_trigger();
   const int items = P.hkv * P.subs, b = blockIdx.x / items, h = blockIdx.x - b * items;
-  const int head = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = 4 * lane;
-  const int kvh = h / P.subs, part = h - kvh * P.subs;
-  const int before = __ldg(P.cum + b), n = __ldg(P.cum + b + 1) - before, chunk = __ldg(P.cum + P.batch + 1);
-  const bool mine = head < min(P.group - part * HEADS, HEADS);
-  const int row = kvh * P.group + part * HEADS + head;
-  if (n == 0) {
-    if (mine) write4(P, b, row, e0, make_float4(0.f, 0.f, 0.f, 0.f));
+  const int head = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = 4 * lane;  // (head: the column)
+  Item it{b, h / P.subs, h % P.subs, 0, 0};
+  const int before = __ldg(P.cum + b), all = __ldg(P.cum + b + 1) - before, chunk = __ldg(P.cum + P.batch + 1);
+  const Seq q = load_seq<ROWS>(P, b);
+  const int parts = parts_of<ROWS>(P, q);
+  if (it.part >= parts) return;
+  int64_t row;
+  int row_head, token;
+  const bool mine = column<ROWS>(P, it, q, ROWS ? __ldg(P.cu_q + b) : 0, head, row, row_head, token);
+  if (all == 0) {
+    if (mine) write4(P, row, row_head, e0, make_float4(0.f, 0.f, 0.f, 0.f));
     return;
   }
-  const int base = before * items + h * n;
+  const int n = all / parts;
+  const int base = before * P.hkv + (it.kvh * parts + it.part) * n;
   const int first = base / chunk, pieces = (base + n - 1) / chunk - first + 1;
   if (pieces == 1) return;  // finished there
   // the first CTA's partial is its second (the item begins there), the others' their first
@@ -618,7 +734,7 @@ __global__ void __launch_bounds__(HEADS * 32) merge_kernel(const __grid_constant
     o.w = fmaf(f, x.w, o.w);
   }
   const float inv = l == 0.f ? 0.f : P.v_scale / l;
-  if (mine) write4(P, b, row, e0, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+  if (mine) write4(P, row, row_head, e0, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
 static int grid_size(int dev) {
@@ -629,6 +745,38 @@ static int grid_size(int dev) {
     sms[dev] = n;
   }
   return n * 2 < MAX_CTAS ? n * 2 : MAX_CTAS;
+}
+// Shared memory limits of this device's kernels, once.
+static int prepare() {
+  static std::atomic<bool> ready[64];
+  constexpr int lists = (3 * MAX_BATCH + 1) * 4;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ADA_ERR_CUDA;
+  if (ready[dev]) return ADA_OK;
+  if (cudaFuncSetAttribute(split_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           WARPS * WARP_SMEM + lists) != cudaSuccess ||
+      cudaFuncSetAttribute(split_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           WARPS * WARP_SMEM + lists) != cudaSuccess ||
+      cudaFuncSetAttribute(split_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * WARP_SMEM) !=
+          cudaSuccess)
+    return ADA_ERR_CUDA;
+  ready[dev] = true;
+  return ADA_OK;
+}
+// Steps shared out equally, then the items of several CTAs joined.
+template <bool ROWS>
+static int launch_shared(const Params& P, cudaStream_t st) {
+  if (const int e = prepare()) return e;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return ADA_ERR_CUDA;
+  const int grid = grid_size(dev);
+  if (grid == 0) return ADA_ERR_CUDA;
+  const size_t smem = WARPS * WARP_SMEM + (P.batch <= 32 ? WARPS * 108 * 4 : (size_t)((ROWS ? 3 : 2) * P.batch + 1) * 4);
+  (void)launch_k(split_kernel<false, ROWS>, dim3((unsigned)grid), dim3(WARPS * 32), smem, st, P);
+  ADA_CHECK_LAUNCH();
+  (void)launch_k(merge_kernel<ROWS>, dim3((unsigned)(P.batch * P.hkv * P.subs)), dim3(HEADS * 32), 0, st, P);
+  ADA_CHECK_LAUNCH();
+  return ADA_OK;
 }
 
 }  // namespace dec
@@ -709,38 +857,66 @@ extern "C" int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride
   P.bt_stride = bt_stride;
   P.max_pages = max_pages;
   P.page = page_size;
-  P.window = window;
   P.batch = batch;
+  P.span = window;
   P.lens = context_lens;
+  P.cu_q = P.cu_k = nullptr;
+  P.most = 1;
+  P.rows = batch;
   P.scale_log2 = scale * k_scale * kv4::LOG2E;
   P.v_scale = v_scale;
   P.cum = static_cast<int*>(workspace);
   P.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + decode_lists(batch));
-  static std::atomic<bool> ready[64];
-  constexpr size_t lists = (size_t)(2 * dec::MAX_BATCH + 1) * 4;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ADA_ERR_CUDA;
-  if (!ready[dev]) {
-    if (cudaFuncSetAttribute(dec::split_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(dec::WARPS * dec::WARP_SMEM + lists)) != cudaSuccess ||
-        cudaFuncSetAttribute(dec::split_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             dec::WARPS * dec::WARP_SMEM) != cudaSuccess)
-      return ADA_ERR_CUDA;
-    ready[dev] = true;
-  }
-  const int grid = dec::grid_size(dev);
-  if (grid == 0) return ADA_ERR_CUDA;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (alone) {
-    (void)launch_k(dec::split_kernel<true>, dim3((unsigned)(batch * items)), dim3(dec::WARPS * 32),
-                   dec::WARPS * dec::WARP_SMEM, st, P);
+    if (const int e = dec::prepare()) return e;
+    (void)launch_k(dec::split_kernel<true, false>, dim3((unsigned)(batch * items)), dim3(dec::WARPS * 32),
+                   dec::WARPS * dec::WARP_SMEM, reinterpret_cast<cudaStream_t>(stream), P);
     ADA_CHECK_LAUNCH();
     return ADA_OK;
   }
-  const size_t smem = dec::WARPS * dec::WARP_SMEM + (batch <= 32 ? dec::WARPS * 72 * 4 : (size_t)(2 * batch + 1) * 4);
-  (void)launch_k(dec::split_kernel<false>, dim3((unsigned)grid), dim3(dec::WARPS * 32), smem, st, P);
-  ADA_CHECK_LAUNCH();
-  (void)launch_k(dec::merge_kernel, dim3((unsigned)(batch * items)), dim3(dec::HEADS * 32), 0, st, P);
-  ADA_CHECK_LAUNCH();
-  return ADA_OK;
+  return dec::launch_shared<false>(P, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t ada::kv4::rows_workspace_size(int32_t batch) { return decode_lists(batch) + (size_t)dec::MAX_CTAS * 2 * dec::PART * 4; }
+
+// The prefill entry's form for a few new tokens a sequence (its arguments are checked there).
+int ada::kv4::rows_prefill(const void* q, int q_dtype, int64_t q_st, int64_t q_sh, const uint8_t* kc, const uint8_t* vc,
+                           int64_t s_page, int64_t s_head, int64_t num_pages, const int32_t* bt, int64_t bt_stride,
+                           int32_t max_pages, const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int64_t rows,
+                           int32_t most, int32_t hq, int32_t hkv, int32_t page, float scale_log2, float v_scale,
+                           int32_t window, void* out, int out_dtype, int64_t o_st, int64_t o_sh, void* workspace,
+                           cudaStream_t st) {
+  dec::Params P;
+  P.hkv = hkv;
+  P.group = hq / hkv;
+  P.subs = (most * P.group + dec::HEADS - 1) / dec::HEADS;
+  P.q = q;
+  P.q_sb = q_st;
+  P.q_sh = q_sh;
+  P.out = out;
+  P.o_sb = o_st;
+  P.o_sh = o_sh;
+  P.q_bf16 = q_dtype == ADA_DT_BF16;
+  P.o_bf16 = out_dtype == ADA_DT_BF16;
+  P.kc = kc;
+  P.vc = vc;
+  P.s_page = s_page;
+  P.s_head = s_head;
+  P.num_pages = num_pages;
+  P.bt = bt;
+  P.bt_stride = bt_stride;
+  P.max_pages = max_pages;
+  P.page = page;
+  P.batch = batch;
+  P.span = window > 0 ? (window < (1 << 30) ? window + 1 : 0) : 0;  // (its own position and W before it)
+  P.lens = nullptr;
+  P.cu_q = cu_q;
+  P.cu_k = cu_k;
+  P.most = most;
+  P.rows = rows;
+  P.scale_log2 = scale_log2;
+  P.v_scale = v_scale;
+  P.cum = static_cast<int*>(workspace);
+  P.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + decode_lists(batch));
+  return dec::launch_shared<true>(P, st);
 }

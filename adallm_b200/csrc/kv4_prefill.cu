@@ -578,6 +578,29 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
 using namespace ada;
 namespace pf4 = ada::kv4::pf4;
 
+constexpr int64_t FEW_ROWS = 32, FEW_KEYS = 256;
+
+// A few rows a KV head behind tables of more than 256 keys go to the decode kernel's form, which shares the
+// keys out over all SMs; this one has a CTA for 256 rows, which walks its keys alone.  Measured, 32/8 heads, 8
+// sequences of 2 new tokens: 60 cached keys 13.0 us shared out and 7.8 here, 500: 16.8 and 20.9, 8,000: 33 and 221; 32
+// sequences of 8: 60: 26 and 20, 500: 36 and 41, 8,000: 235 and 431 (16 tokens would be even).
+static bool prefill_few(int64_t batch, int64_t most, int32_t num_heads, int32_t num_kv_heads, int32_t max_pages,
+                        int32_t page_size) {
+  const int64_t rows = most * (num_heads / num_kv_heads), parts = cdiv(rows, (int64_t)8);
+  return rows <= FEW_ROWS && (int64_t)max_pages * page_size > FEW_KEYS && batch <= 8192 &&
+         batch * num_kv_heads * parts * (cdiv((int64_t)max_pages * page_size, (int64_t)32) + 1) <= 0x7fffffffLL;
+}
+
+extern "C" size_t ada_kv4_paged_prefill_workspace_size(int32_t batch, int64_t total_q, int32_t max_seqlen_q,
+                                                       int32_t num_heads, int32_t num_kv_heads, int32_t max_pages,
+                                                       int32_t page_size) {
+  if (batch <= 0 || total_q <= 0 || max_seqlen_q <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_pages <= 0 ||
+      page_size <= 0)
+    return 0;
+  const int64_t most = max_seqlen_q < total_q ? max_seqlen_q : total_q;
+  return prefill_few(batch, most, num_heads, num_kv_heads, max_pages, page_size) ? kv4::rows_workspace_size(batch) : 0;
+}
+
 extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h,
                                      const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
                                      int64_t kv_stride_head, int64_t num_pages, const int32_t* block_tables,
@@ -585,8 +608,8 @@ extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_strid
                                      const int32_t* cu_seqlens_k, int32_t batch, int64_t total_q, int32_t max_seqlen_q,
                                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                      float scale, float k_scale, float v_scale, int32_t window, void* out,
-                                     int out_dtype, int64_t out_stride_t, int64_t out_stride_h, unsigned int* err,
-                                     void* stream) {
+                                     int out_dtype, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+                                     size_t workspace_bytes, unsigned int* err, void* stream) {
   if (batch < 0 || max_seqlen_q < 0 || total_q < 0) return ADA_ERR_INVALID_ARG;
   if (batch == 0 || max_seqlen_q == 0 || total_q == 0) return ADA_OK;
   if (!cu_seqlens_q || !cu_seqlens_k) return ADA_ERR_INVALID_ARG;
@@ -599,6 +622,16 @@ extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_strid
     return ADA_ERR_ALIGNMENT;
   const int group = num_heads / num_kv_heads;
   if (group > pf4::NT * pf4::BM || batch > 65535 || max_seqlen_q > (1 << 30)) return ADA_ERR_UNSUPPORTED;
+  const int64_t most = max_seqlen_q < total_q ? (int64_t)max_seqlen_q : total_q;
+  if (prefill_few(batch, most, num_heads, num_kv_heads, max_pages, page_size)) {
+    if (!workspace || workspace_bytes < kv4::rows_workspace_size(batch)) return ADA_ERR_WORKSPACE;
+    if (kv4::misaligned16(workspace)) return ADA_ERR_ALIGNMENT;
+    return kv4::rows_prefill(q, q_dtype, q_stride_t, q_stride_h, k_cache, v_cache, kv_stride_page, kv_stride_head,
+                             num_pages, block_tables, bt_stride, max_pages, cu_seqlens_q, cu_seqlens_k, batch, total_q,
+                             (int32_t)most, num_heads, num_kv_heads, page_size, scale * k_scale * kv4::LOG2E, v_scale,
+                             window, out, out_dtype, out_stride_t, out_stride_h, workspace,
+                             reinterpret_cast<cudaStream_t>(stream));
+  }
   pf4::Params P;
   P.q = q;
   P.q_st = q_stride_t;
@@ -626,7 +659,7 @@ extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_strid
   P.scale_log2 = scale * k_scale * kv4::LOG2E;
   P.v_scale = v_scale;
   P.err = err;
-  const int64_t qblocks = cdiv(max_seqlen_q < total_q ? (int64_t)max_seqlen_q : total_q, P.qt);
+  const int64_t qblocks = cdiv(most, P.qt);
   if (qblocks > 65535) return ADA_ERR_UNSUPPORTED;
   static std::atomic<bool> ready[64];
   int dev = 0;

@@ -54,12 +54,13 @@ extern "C" int ada_call(int entry, const int64_t* a) {
                                   real(a[20]), i32(a[21]), at<void>(a[22]), i32(a[23]), a[24], a[25], at<void>(a[26]),
                                   static_cast<size_t>(a[27]), at<void>(a[28]));
     case ADA_CALL_KV4_PAGED_PREFILL:
-      if (!fits(a, "piqqppqqqpqippiqiiiiidddipiqqpp")) return ADA_ERR_UNSUPPORTED;
+      if (!fits(a, "piqqppqqqpqippiqiiiiidddipiqqpqpp")) return ADA_ERR_UNSUPPORTED;
       return ada_kv4_paged_prefill(at<void>(a[0]), i32(a[1]), a[2], a[3], at<uint8_t>(a[4]), at<uint8_t>(a[5]), a[6],
                                    a[7], a[8], at<int32_t>(a[9]), a[10], i32(a[11]), at<int32_t>(a[12]),
                                    at<int32_t>(a[13]), i32(a[14]), a[15], i32(a[16]), i32(a[17]), i32(a[18]),
                                    i32(a[19]), i32(a[20]), real(a[21]), real(a[22]), real(a[23]), i32(a[24]),
-                                   at<void>(a[25]), i32(a[26]), a[27], a[28], at<unsigned>(a[29]), at<void>(a[30]));
+                                   at<void>(a[25]), i32(a[26]), a[27], a[28], at<void>(a[29]), static_cast<size_t>(a[30]),
+                                   at<unsigned>(a[31]), at<void>(a[32]));
     default:
       return ADA_ERR_INVALID_ARG;
   }

@@ -217,16 +217,25 @@ def paged_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
+@functools.lru_cache(maxsize=512)
+def paged_prefill_fp4_workspace_bytes(batch: int, total_q: int, max_seqlen_q: int, num_heads: int, num_kv_heads: int,
+                                      max_pages: int, page_size: int) -> int:
+    """0 but for a few rows a KV head."""
+    return int(N.lib().ada_kv4_paged_prefill_workspace_size(batch, total_q, max_seqlen_q, num_heads, num_kv_heads,
+                                                            max_pages, page_size))
+
+
 def paged_prefill_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                       cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, max_seqlen_q: int, scale: float,
                       window: int = 0, k_scale: float = 1.0, v_scale: float = 1.0, out: torch.Tensor | None = None,
-                      err: torch.Tensor | None = None) -> torch.Tensor:
+                      err: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Causal prefill attention of the new tokens against the 4-bit paged cache.
 
     The arguments of attention.paged_prefill with a 4-bit cache: q [total_q, Hq, 128]; the cache holds every
     sequence's cached prefix and new tokens; max_seqlen_q must be at least every sequence's new tokens.
     window W > 0: a row sees its own position and the W before it.  Rows behind the last sequence are left as
-    they are in ``out`` (unset without it)."""
+    they are in ``out`` (unset without it).  workspace: at least paged_prefill_fp4_workspace_bytes(...) bytes, which a few
+    rows a KV head behind long tables need (default: allocated for the call)."""
     device = N.one_device("paged_prefill_fp4", q, k_cache, v_cache, block_tables, cu_seqlens_q, cu_seqlens_k)
     pages, hkv, page, s_page, s_head = _cache(k_cache, v_cache)
     q, code, out, out_code = _attention(device, q, block_tables, out, cu_seqlens_q, cu_seqlens_k)
@@ -242,12 +251,22 @@ def paged_prefill_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         word = err.data_ptr()
     if total_q == 0 or batch <= 0:
         return out
+    at = 0
+    if workspace is None:
+        size = paged_prefill_fp4_workspace_bytes(batch, total_q, max_seqlen_q, hq, hkv, max_pages, page)
+        if size:
+            workspace = k_cache.new_empty(size)
+            at = workspace.data_ptr()
+    else:
+        size, at = workspace.nbytes, workspace.data_ptr()
+        if workspace.get_device() != device or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous on q's device")
     qs, os = q.stride(), out.stride()
     st = N.kv4_paged_prefill(device, q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), s_page,
                              s_head, pages, block_tables.data_ptr(), block_tables.stride(0), max_pages,
                              cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch, total_q, max_seqlen_q, hq, hkv, d,
                              page, scale, k_scale, v_scale, window if window < LARGEST else LARGEST, out.data_ptr(),
-                             out_code, os[0], os[1], word, N.raw_stream(device))
+                             out_code, os[0], os[1], at, size, word, N.raw_stream(device))
     if st:
         N.check(st, "4-bit KV prefill kernel")
     return out

@@ -748,7 +748,14 @@ ADA_API int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b,
 
 /* Causal prefill attention over the 4-bit cache: arguments and masks as ada_fp8_paged_prefill (window W > 0:
  * the row's own position and the W before it); rows of q and out outside [0, total_q) and rows
- * behind the last sequence are not touched.  *err (may be NULL): 0x70 if a tile wait ran out. */
+ * behind the last sequence are not touched.  A few rows a KV head (max_seqlen_q x heads a KV head up to 32)
+ * behind tables of more than 256 keys take the decode form, which shares long caches out over all SMs.  workspace: as for decode, sized by
+ * ada_kv4_paged_prefill_workspace_size (0 for more rows).  *err (may be NULL): 0x70 if a tile wait ran out (the
+ * rows concerned are NaN).  A NaN key reaches every element of the rows that see it, a NaN value the 16 elements of its
+ * block, and neither any other row.  Implemented: up to 256 heads a KV head. */
+ADA_API size_t ada_kv4_paged_prefill_workspace_size(int32_t batch, int64_t total_q, int32_t max_seqlen_q,
+                                                    int32_t num_heads, int32_t num_kv_heads, int32_t max_pages,
+                                                    int32_t page_size);
 ADA_API int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h,
                                   const uint8_t* k_cache, const uint8_t* v_cache, int64_t kv_stride_page,
                                   int64_t kv_stride_head, int64_t num_pages, const int32_t* block_tables,
@@ -756,7 +763,8 @@ ADA_API int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t
                                   const int32_t* cu_seqlens_k, int32_t batch, int64_t total_q, int32_t max_seqlen_q,
                                   int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                   float scale, float k_scale, float v_scale, int32_t window, void* out, int out_dtype,
-                                  int64_t out_stride_t, int64_t out_stride_h, unsigned int* err, void* stream);
+                                  int64_t out_stride_t, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
+                                  unsigned int* err, void* stream);
 
 /* ------------------------------------------------------------------------
  * The six entries above with their arguments as one array

@@ -163,6 +163,11 @@ def make(seed, lens, new, hq, hkv, page, dtype=BF16, q_spread=1.5, k_spread=1.0,
                 cu_k=cu(lens))
 
 
+def behind_long_tables(c, pages=64):
+    """The same sequences with wider tables: what selects the forms that share keys out."""
+    return dict(c, tables=torch.nn.functional.pad(c["tables"], (0, pages), value=-1))
+
+
 def assert_near(out, want, err, dtype=None):
     half = torch.finfo(dtype or out.dtype).eps / 2
     tol = err + half * (want.abs() + err) + torch.finfo(dtype or out.dtype).smallest_normal
@@ -234,9 +239,11 @@ def test_holes_and_bad_page_ids_are_masked(decode):
     c["tables"][0, 5] = c["k"].shape[0]
     c["tables"][0, 7] = 2 ** 31 - 1
     c["tables"][1, :] = -1  # nothing there: zeros
-    out = run_decode(c) if decode else run_prefill(c)
-    assert_near(out, *want_of(c, decode=decode))
-    assert (out[1] == 0).all()
+    want, err = want_of(c, decode=decode)
+    for d in (c, behind_long_tables(c, 100)):
+        out = run_decode(d) if decode else run_prefill(d)
+        assert_near(out, want, err)
+        assert (out[1] == 0).all()
 
 
 def test_lengths_beyond_the_table():
@@ -295,14 +302,20 @@ PREFILL = [  # cached, new, hq, hkv, page, window, dtype
     ([0, 37, 300, 5], [50, 1, 129, 0], 32, 8, 16, 40, F16), ([100, 0], [77, 200], 32, 4, 64, 0, BF16),
     ([15], [70], 12, 4, 32, 0, F16), ([3], [130], 4, 4, 16, 17, BF16), ([1024], [512], 32, 8, 16, 0, BF16),
     ([0], [700], 16, 1, 16, 0, BF16), ([500, 0, 63], [65, 64, 1], 32, 16, 256, 128, F16), ([7], [300], 33, 1, 48, 0, BF16),
-    ([2000], [3], 32, 8, 16, 0, F16), ([0, 0, 0], [16, 17, 15], 32, 2, 16, 1, BF16)]
+    ([2000], [3], 32, 8, 16, 0, F16), ([0, 0, 0], [16, 17, 15], 32, 2, 16, 1, BF16),
+    # few rows a KV head: the keys shared out as for decode
+    ([700, 0, 33], [8, 5, 1], 16, 4, 16, 0, BF16), ([9000, 3], [4, 2], 32, 4, 64, 0, F16),
+    ([300, 20, 0], [7, 3, 1], 12, 4, 48, 13, F16), ([1, 30, 31, 32] * 12, [1, 2, 3, 4] * 12, 8, 8, 16, 0, BF16),
+    ([64, 500], [0, 2], 32, 2, 32, 1, BF16), ([100], [32], 2, 2, 16, 40, BF16)]
 
 
 @pytest.mark.parametrize("cached,new,hq,hkv,page,window,dtype", PREFILL)
 def test_prefill_matches_64_bits(cached, new, hq, hkv, page, window, dtype):
     lens = [a + b for a, b in zip(cached, new)]
     c = make(sum(lens) + hq, lens, new, hq, hkv, page, dtype)
-    assert_near(run_prefill(c, window), *want_of(c, window, decode=False))
+    want, err = want_of(c, window, decode=False)
+    assert_near(run_prefill(c, window), want, err)
+    assert_near(run_prefill(behind_long_tables(c), window), want, err)
 
 
 def test_prefill_scales_output_type_strides_and_rows_left_alone():
@@ -333,6 +346,44 @@ def test_prefill_lists_that_do_not_ascend_stay_inside():
     run_prefill(c, out=out, most=100)
     c["cu_q"] = torch.tensor([-50, 30, 90], dtype=torch.int32, device=dev())
     run_prefill(c, out=out, most=100)
+    c = behind_long_tables(c)
+    for cu in ([60, 20, 2 ** 30], [-50, 30, 90], [2 ** 31 - 1, -2 ** 31, 7]):  # and with few rows
+        c["cu_q"] = torch.tensor(cu, dtype=torch.int32, device=dev())
+        run_prefill(c, out=out, most=8)
+    c["cu_q"] = torch.tensor([0, 4, 8], dtype=torch.int32, device=dev())
+    c["cu_k"] = torch.tensor([0, 2 ** 31 - 1, -5], dtype=torch.int32, device=dev())
+    run_prefill(c, out=out, most=4)
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_few_rows_nan_reaches_the_rows_that_see_it(where):
+    """NaN at key 97 of 100 with 6 new (94..99), and in the middle: elements as the formula has them."""
+    for key, window in ((97, 0), (97, 2), (50, 0), (93, 5)):
+        c = behind_long_tables(make(26, [100, 90], [6, 2], 16, 4, 16))
+        cache = c[where]
+        cache[int(c["tables"][0, key // 16]), 1, 16 * 64 + (key % 16) * 8 + 3] = 0x7F
+        out = run_prefill(c, window)
+        rows = torch.arange(6, device=dev()) + 94
+        sees = (rows >= key) & ((rows <= key + window) if window else True)
+        bad = out.isnan()
+        want = torch.zeros_like(bad)
+        want[:6, 4:8, (48 if where == "v" else 0):(64 if where == "v" else 128)] = sees[:, None, None]
+        assert torch.equal(bad, want)
+
+
+def test_few_rows_without_keys_scales_and_workspace():
+    c = behind_long_tables(make(27, [3, 64, 0], [8, 2, 3], 8, 2, 16))
+    size = kv.paged_prefill_fp4_workspace_bytes(3, 13, 8, 8, 2, c["tables"].shape[1], 16)
+    assert size > 0 and kv.paged_prefill_fp4_workspace_bytes(3, 13, 9, 8, 2, c["tables"].shape[1], 16) == 0
+    out = torch.full((15, 8, 128), 7.0, dtype=F16, device=dev())
+    q = torch.nn.functional.pad(c["q"], (0, 0, 0, 0, 0, 2))
+    run_prefill(dict(c, q=q), 0, 0.5, 0.3, 0.2, out=out, workspace=torch.full((size,), 0xFF, dtype=torch.uint8, device=dev()))
+    assert (out[:5] == 0).all() and (out[10:13] == 0).all() and (out[13:] == 7).all()
+    want, err = kv4.attention(c["q"][5:10], c["k"], c["v"], c["tables"], [3, 2], [3, 64], 0.2, k_scale=0.5, v_scale=0.3)
+    assert_near(out[5:10], want, err)
+    short = torch.empty(size - 1, dtype=torch.uint8, device=dev())
+    with pytest.raises(ValueError):
+        run_prefill(c, workspace=short)
 
 
 @pytest.mark.parametrize("where", ["k", "v"])

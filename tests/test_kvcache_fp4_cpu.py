@@ -52,8 +52,8 @@ def test_decode_refusals(lib):
 
 
 PREFILL = dict(q=16, qd=0, qst=1024, qsh=128, k=16, v=16, sp=8 * 1152, sh=1152, pages=4, bt=16, bts=4, mp=4, cq=16, ck=16,
-               batch=1, total=5, most=5, hq=32, hkv=8, d=128, page=16, scale=0.1, ks=1.0, vs=1.0, window=0, out=32, od=0,
-               ost=4096, osh=128, err=None, stream=None)
+               batch=1, total=50, most=50, hq=32, hkv=8, d=128, page=16, scale=0.1, ks=1.0, vs=1.0, window=0, out=32, od=0,
+               ost=4096, osh=128, ws=None, wsb=0, err=None, stream=None)
 
 
 def test_prefill_refusals(lib):
@@ -64,7 +64,12 @@ def test_prefill_refusals(lib):
         (dict(q=None), BAD), (dict(k=None), BAD), (dict(bt=None), BAD), (dict(cq=None), BAD), (dict(ck=None), BAD),
         (dict(out=None), BAD), (dict(qd=2), BAD), (dict(d=256), UNSUP), (dict(page=8), UNSUP), (dict(hq=33), BAD),
         (dict(window=-1), BAD), (dict(scale=-0.1), BAD), (dict(vs=math.nan), BAD), (dict(q=8), ALIGN), (dict(v=4), ALIGN),
-        (dict(ost=4), ALIGN), (dict(cq=18), ALIGN), (dict(err=2), ALIGN), (dict(batch=70000), UNSUP)])
+        (dict(ost=4), ALIGN), (dict(cq=18), ALIGN), (dict(err=2), ALIGN), (dict(batch=70000), UNSUP),
+        (dict(most=8, mp=40, bts=40), WS), (dict(most=8, mp=40, bts=40, ws=16, wsb=100), WS),
+        (dict(most=8, mp=40, bts=40, ws=8, wsb=1 << 30), ALIGN), (dict(total=3, mp=40, bts=40), WS)])
+    size = lib.ada_kv4_paged_prefill_workspace_size
+    assert size(1, 50, 50, 32, 8, 40, 16) == 0 and size(1, 50, 8, 32, 8, 40, 16) > 0
+    assert size(1, 50, 8, 32, 8, 16, 16) == 0 and size(1, 0, 8, 32, 8, 40, 16) == 0
 
 
 STORE = dict(pos=16, q=32, qst=4096, qsh=128, k=48, kst=1024, ksh=128, v=64, vst=1024, vsh=128, qo=80, t=3, hq=32, hkv=8,
