@@ -17,6 +17,7 @@ import torch
 from torch import nn
 
 from . import _native as N
+from . import kvcache_fp4 as fp4
 from .context import get_context
 
 
@@ -133,7 +134,8 @@ class Attention(nn.Module):
     """Drop-in for adallm.ops.attention.Attention (decode branch).
 
     KV cache views k_cache / v_cache are attached by the runner exactly as the
-    reference's ModelRunner.allocate_kv_cache does (adallm/runtime/model_runner.py:154-169)."""
+    reference's ModelRunner.allocate_kv_cache does (adallm/runtime/model_runner.py:154-169); uint8
+    views [pages, Hkv, page * 72] hold the cache in 4 bits (kvcache_fp4)."""
 
     def __init__(self, num_heads, head_dim, scale, num_kv_heads, sliding_window: int | None = None):
         super().__init__()
@@ -151,22 +153,25 @@ class Attention(nn.Module):
         if context.is_prefill and context.block_tables is None:
             raise NotImplementedError("adallm_b200 runs the prefix-cache prefill and the decode branch; a prefill "
                                       "without a block table stays on the reference path")
+        bits4 = self.k_cache.dtype is torch.uint8
+        store, prefill, decode = ((fp4.store_kvcache_fp4, fp4.paged_prefill_fp4, fp4.paged_decode_fp4) if bits4 else
+                                  (store_kvcache, paged_prefill, paged_decode))
         if self.k_cache.numel() and self.v_cache.numel():
-            store_kvcache(k, v, self.k_cache, self.v_cache, context.slot_mapping, self.k_scale, self.v_scale)
+            store(k, v, self.k_cache, self.v_cache, context.slot_mapping, self.k_scale, self.v_scale)
         window = self.sliding_window if (self.sliding_window is not None and self.sliding_window > 0) else 0
         if context.is_prefill:
             try:
-                return paged_prefill(q.view(-1, self.num_heads, self.head_dim), self.k_cache, self.v_cache,
-                                     context.block_tables, context.cu_seqlens_q, context.cu_seqlens_k,
-                                     context.max_seqlen_q, self.scale, window, self.k_scale, self.v_scale)
+                return prefill(q.view(-1, self.num_heads, self.head_dim), self.k_cache, self.v_cache,
+                               context.block_tables, context.cu_seqlens_q, context.cu_seqlens_k,
+                               context.max_seqlen_q, self.scale, window, self.k_scale, self.v_scale)
             except Exception as exc:
                 if torch.cuda.is_current_stream_capturing() or isinstance(exc, ValueError):
                     raise
                 raise RuntimeError("FP8 paged prefill kernel failed; no fallback is allowed in this runtime.") from exc
         try:
-            return paged_decode(q.view(-1, self.num_heads, self.head_dim), self.k_cache, self.v_cache,
-                                context.block_tables, context.context_lens, self.scale, window,
-                                self.k_scale, self.v_scale)
+            return decode(q.view(-1, self.num_heads, self.head_dim), self.k_cache, self.v_cache,
+                          context.block_tables, context.context_lens, self.scale, window,
+                          self.k_scale, self.v_scale)
         except Exception as exc:
             if torch.cuda.is_current_stream_capturing():
                 raise
