@@ -7,6 +7,10 @@
 // contiguous pieces (1,024 and 128 bytes) and a page of one head stays together in DRAM, where a
 // row of 72 bytes among other heads' would leave no 16-byte alignment to load with.
 // code * scale has at most 6 significant bits and lies in [2^-10, 2688]: exact in fp16 and in bf16.
+//
+// The kernels read lists, tables and queries by plain loads and not by those through the read-only path (ld.global.nc),
+// whose data must not change while a kernel runs: theirs is written by the launch before, which
+// overlaps their start (step_metadata.cu's CTAs read tables that others of it extend).
 #pragma once
 
 #include "common.cuh"
@@ -27,7 +31,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// x / d given r near 1 / d: one correction step.  Correctly rounded where x / d lies further than 2^-44 of
+// x / d given r near 1 / d: one Newton step on the quotient's remainder (Markstein 1990).  Correctly rounded where x / d lies further than 2^-44 of
 // itself from a midpoint of fp32 or on none: for divisors of few bits (6; the e4m3 scales) always (2^-27 and
 // more), for others but for one quotient in 2^20, which is one step (2^-24) off then.
 __device__ __forceinline__ float quotient(float x, float d, float r) {
@@ -132,13 +136,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// A tensor's scale that both it and its reciprocal are good for as fp32 factors (no NaN, infinity or subnormal).
+inline bool scale_ok(float s) { return s >= 1e-30f && s <= 1e30f; }
 inline bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 // Checks of a cache's layout that every entry shares.
 inline int cache_ok(const void* kc, const void* vc, int64_t s_page, int64_t s_head, int64_t num_pages, int32_t heads,
                     int32_t page) {
   if (!kc || !vc || num_pages <= 0 || heads <= 0 || page <= 0) return ADA_ERR_INVALID_ARG;
-  if (page % 16) return ADA_ERR_UNSUPPORTED;
+  if (page % 16 || page > (1 << 24)) return ADA_ERR_UNSUPPORTED;  // (places in a block are counted in 32 bits)
   if (s_head < (int64_t)page * ROW_BYTES || s_page < (int64_t)page * ROW_BYTES) return ADA_ERR_INVALID_ARG;
   if (misaligned16(kc) || misaligned16(vc) || (s_page & 15) || (s_head & 15)) return ADA_ERR_ALIGNMENT;
   return ADA_OK;
@@ -154,7 +160,7 @@ inline int attn_ok(const void* q, int qd, int64_t q_st, int64_t q_sh, const void
   if (d != D) return ADA_ERR_UNSUPPORTED;
   if (const int e = cache_ok(kc, vc, s_page, s_head, num_pages, hkv, page)) return e;
   if (hq % hkv || window < 0 || bt_stride < max_pages) return ADA_ERR_INVALID_ARG;
-  if (!(scale * k_scale > 0.f) || !(v_scale > 0.f)) return ADA_ERR_INVALID_ARG;
+  if (!(scale > 0.f) || !(scale <= 1e30f) || !scale_ok(k_scale) || !scale_ok(v_scale)) return ADA_ERR_INVALID_ARG;
   if ((int64_t)max_pages * page > (1LL << 30)) return ADA_ERR_UNSUPPORTED;
   if (misaligned16(q) || misaligned16(out) || ((q_st | q_sh | o_st | o_sh) & 7)) return ADA_ERR_ALIGNMENT;
   if (reinterpret_cast<uintptr_t>(bt) & 3) return ADA_ERR_ALIGNMENT;

@@ -44,6 +44,7 @@ constexpr int HEADS = 8;                         // heads side by side (N of the
 constexpr int PART = HEADS * D + 2 * HEADS;      // floats of a partial: O, then (m, l) per head
 constexpr int WARP_SMEM = STAGES * STEP_BYTES + PART * 4;
 constexpr int MAX_BATCH = 8192;
+constexpr int64_t MOST_STEPS = 1 << 30;
 static_assert(STAGES * STEP_BYTES >= PART * 4, "a warp's last partial lies in its ring");
 
 struct Params {
@@ -81,10 +82,10 @@ __device__ __forceinline__ Seq seq_of(const Params& P, int keys, int fresh) {
 }
 template <bool ROWS>
 __device__ __forceinline__ Seq load_seq(const Params& P, int b) {
-  if (!ROWS) return seq_of<ROWS>(P, __ldg(P.lens + b), 1);
+  if (!ROWS) return seq_of<ROWS>(P, P.lens[b], 1);
   // (differences of lists that do not ascend may wrap: any value is as good as another there)
-  const unsigned k0 = (unsigned)__ldg(P.cu_k + b), k1 = (unsigned)__ldg(P.cu_k + b + 1);
-  const unsigned q0 = (unsigned)__ldg(P.cu_q + b), q1 = (unsigned)__ldg(P.cu_q + b + 1);
+  const unsigned k0 = (unsigned)P.cu_k[b], k1 = (unsigned)P.cu_k[b + 1];
+  const unsigned q0 = (unsigned)P.cu_q[b], q1 = (unsigned)P.cu_q[b + 1];
   return seq_of<ROWS>(P, (int)(k1 - k0), (int)(q1 - q0));
 }
 // Keys [lo, hi) that token i of a sequence sees (0 <= i < tokens).
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       if (key < lr.hi) {
         const int tile = key / TILE, col = tile / page_tiles;
         place = tile - col * page_tiles;
-        id = __ldg(P.bt + (int64_t)li.b * P.bt_stride + col);
+        id = P.bt[(int64_t)li.b * P.bt_stride + col];
         if (id >= P.num_pages) id = -1;
       }
     };
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       const Range rg = range_at(it.b);
       const int stop = min(it.end, r1);
       const Seq sq = seq_in(it.b);
-      const int64_t q0 = ROWS ? __ldg(P.cu_q + it.b) : 0;
+      const int64_t q0 = ROWS ? P.cu_q[it.b] : 0;
       int64_t row;
       int head, token;
       // ROWS: keys that this lane's columns 2c, 2c + 1 see, and where all columns of the part see the same
@@ -616,7 +617,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
     const Seq q = seq_in(it.b);
     int64_t row;
     int head, token;
-    if (!column<ROWS>(P, it, q, ROWS ? __ldg(P.cu_q + it.b) : 0, col, row, head, token)) return;
+    if (!column<ROWS>(P, it, q, ROWS ? P.cu_q[it.b] : 0, col, row, head, token)) return;
     const float inv = l == 0.f ? 0.f : P.v_scale / l;
     write4(P, row, head, e0, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
   };
@@ -680,13 +681,13 @@ __global__ void __launch_bounds__(HEADS * 32) merge_kernel(const __grid_constant
   const int items = P.hkv * P.subs, b = blockIdx.x / items, h = blockIdx.x - b * items;
   const int head = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = 4 * lane;  // (head: the column)
   Item it{b, h / P.subs, h % P.subs, 0, 0};
-  const int before = __ldg(P.cum + b), all = __ldg(P.cum + b + 1) - before, chunk = __ldg(P.cum + P.batch + 1);
+  const int before = P.cum[b], all = P.cum[b + 1] - before, chunk = P.cum[P.batch + 1];
   const Seq q = load_seq<ROWS>(P, b);
   const int parts = parts_of<ROWS>(P, q);
   if (it.part >= parts) return;
   int64_t row;
   int row_head, token;
-  const bool mine = column<ROWS>(P, it, q, ROWS ? __ldg(P.cu_q + b) : 0, head, row, row_head, token);
+  const bool mine = column<ROWS>(P, it, q, ROWS ? P.cu_q[b] : 0, head, row, row_head, token);
   if (all == 0) {
     if (mine) write4(P, row, row_head, e0, make_float4(0.f, 0.f, 0.f, 0.f));
     return;
@@ -791,7 +792,7 @@ static size_t decode_lists(int32_t batch) { return ((size_t)(batch + 2) * 4 + 15
 
 // One CTA an item, and one launch, where an item has at most 40 steps (five a warp) whatever its length and
 // all items are resident at once; otherwise equal shares and a second launch that joins them.  (One sequence
-// of 700 keys, 32/8 heads: 11.3 us shared out, 8.5 alone; 4 x 1,024 keys of a window, 32/16: 14.3 and 10.3.  With
+// of 700 keys, 32/8 heads: 11.3 us shared out, 8.4 alone; 4 x 1,024 keys of a window, 32/16: 14.3 and 10.3.  With
 // 16 warps a CTA 9.6 and 10.7: an SM issues the item's instructions no faster.)
 static bool decode_alone(int64_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t max_pages, int32_t page_size,
                          int32_t window) {
@@ -829,9 +830,9 @@ extern "C" int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride
   P.group = num_heads / num_kv_heads;
   P.subs = (P.group + dec::HEADS - 1) / dec::HEADS;
   const int64_t items = (int64_t)num_kv_heads * P.subs;
-  const int64_t tiles = cdiv((int64_t)max_pages * page_size, dec::KEYS) + 1;
-  // the row of all tiles is counted in 32 bits
-  if (batch > dec::MAX_BATCH || batch * items * tiles > 0x7fffffffLL || batch * items > 0x7fffffffLL)
+  const int64_t steps = cdiv((int64_t)max_pages * page_size, dec::KEYS) + 1;
+  // the row of all steps is counted in 32 bits
+  if (batch > dec::MAX_BATCH || batch * items > dec::MOST_STEPS || batch * items * steps > dec::MOST_STEPS)
     return ADA_ERR_UNSUPPORTED;
   const bool alone = decode_alone(batch, num_heads, num_kv_heads, max_pages, page_size, window);
   if (!alone) {

@@ -25,8 +25,7 @@
 // their 16 elements to NaN at the end.
 //
 // Barriers (block j, tile t): e_full[j % NSTG], e_empty, kv_full[j % NKV], kv_empty (commit after both P V),
-// s_full[t][j & 1] (commit, and an arrival of the issuer's own), p_full[t][j & 1] (4 warps),
-// o_done[t] (commit
+// s_full[t][j & 1] (commit, and an arrival of the issuer's own), p_full[t][j & 1] (4 warps), o_done[t] (commit
 // after P V), o_last[t] (after the last one), q_ready (8 warps), fin.
 // A wait by parity needs the phase before to be known complete and the next one not begun.  Refills wait
 // for the release of the use before, in every phase; S_{j+2} is issued after p_full of j.  o_done of j - 1: the
@@ -191,9 +190,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
   pdl_wait();
   pdl_trigger();
 
-  const int64_t q_begin = __ldg(P.cu_q + b);
-  const int len_q = (int)min(max((int64_t)__ldg(P.cu_q + b + 1) - q_begin, (int64_t)0), (int64_t)1 << 30);
-  const int len_k = (int)min(max((int64_t)__ldg(P.cu_k + b + 1) - __ldg(P.cu_k + b), (int64_t)0), (int64_t)1 << 30);
+  const int64_t q_begin = P.cu_q[b];
+  const int len_q = (int)min(max((int64_t)P.cu_q[b + 1] - q_begin, (int64_t)0), (int64_t)1 << 30);
+  const int len_k = (int)min(max((int64_t)P.cu_k[b + 1] - P.cu_k[b], (int64_t)0), (int64_t)1 << 30);
   const int t0 = qblk * P.qt;
   const bool active = t0 < len_q;
   const int off = len_k - len_q;
@@ -216,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       const int key0 = kb0 + TILE * (first + lane);
       if (key0 >= k_end) return -1;
       const int tile = key0 / TILE, col = tile / page_tiles;
-      const int64_t id = __ldg(P.bt + (int64_t)b * P.bt_stride + col);
+      const int64_t id = P.bt[(int64_t)b * P.bt_stride + col];
       return id < 0 || id >= P.num_pages ? -1 : id * P.s_page + head + (int64_t)(tile - col * page_tiles) * (TILE * ROW);
     };
     int64_t cur = nblk > 0 ? place(0) : -1, nxt = nblk > 8 ? place(32) : -1;
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
   } else if (warp == 1) {  // ---------------- MMA issuer ----------------
     // The whole warp runs this loop, its values uniform, and one elected lane issues: the operands of the
     // tcgen05 instructions then stay in uniform registers (from a divergent lane an MMA takes about 100
-    // cycles to issue: 24 of them a block were the bound, 629 us instead of 400 for 4 x 2,048 behind 2,048).
+    // cycles to issue, 24 of them a block: 629 us instead of 518 for 4 x 2,048 tokens behind 2,048, 32/8 heads).
     if (nblk > 0) {
       const bool leader = elect_one();
       const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(P.q) + at);
       uint4 raw[16];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) raw[c] = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < 16; ++c) raw[c] = valid ? src[c] : make_uint4(0, 0, 0, 0);
       float top = 0.f;
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
@@ -586,9 +585,11 @@ constexpr int64_t FEW_ROWS = 32, FEW_KEYS = 256;
 // sequences of 8: 60: 26 and 20, 500: 36 and 41, 8,000: 235 and 431 (16 tokens would be even).
 static bool prefill_few(int64_t batch, int64_t most, int32_t num_heads, int32_t num_kv_heads, int32_t max_pages,
                         int32_t page_size) {
-  const int64_t rows = most * (num_heads / num_kv_heads), parts = cdiv(rows, (int64_t)8);
-  return rows <= FEW_ROWS && (int64_t)max_pages * page_size > FEW_KEYS && batch <= 8192 &&
-         batch * num_kv_heads * parts * (cdiv((int64_t)max_pages * page_size, (int64_t)32) + 1) <= 0x7fffffffLL;
+  constexpr int64_t MOST = 1 << 30;  // steps of 32 keys, which that kernel counts in 32 bits
+  const int64_t rows = most * (num_heads / num_kv_heads), items = batch * num_kv_heads * cdiv(rows, (int64_t)8);
+  const int64_t keys = (int64_t)max_pages * page_size;
+  return rows <= FEW_ROWS && keys > FEW_KEYS && keys <= MOST && batch <= 8192 && items <= MOST &&
+         items * (cdiv(keys, (int64_t)32) + 1) <= MOST;
 }
 
 extern "C" size_t ada_kv4_paged_prefill_workspace_size(int32_t batch, int64_t total_q, int32_t max_seqlen_q,

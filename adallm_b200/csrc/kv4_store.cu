@@ -73,17 +73,15 @@ __device__ __forceinline__ uint32_t pack_codes(const uint4& x, float div, float 
 // i + r/16 of the turned part (half layout), or neighbours; it keeps U heads (blockIdx.y's share) and walks
 // the tokens, so what belongs to a head is worked out once.  Rows and table entries of the next
 // STAGES - 1 tokens are on their way by cp.async, each thread's rows into places of its own: with a token
-// at a time, or one ahead in registers, an SM has 20-40 KB in flight where HBM wants 66 (95 us
-// instead of 66 for 16,381 tokens of 40 heads).
-// (one head with the store, whose arithmetic needs the registers)
-constexpr int heads_a_thread(bool) { return 2; }
-constexpr int STAGES = 4;
+// at a time, or one ahead in registers, an SM has 20-40 KB in flight where HBM wants 66 (95 us, with this
+// 62.5, for 16,381 tokens of 40 heads: 83% of the copy rate).  The store's arithmetic (maxima, quotients,
+// conversions) takes longer than its bytes: 75 us for 8,195 tokens of 32/8 heads, 47 by its bytes.
+constexpr int U = 2, STAGES = 4;
 // Bytes of a stage: the CTA's rows, then the table's row.
 __host__ __device__ constexpr int stage_bytes(int threads, int heads, int rot) { return threads * heads * 32 + rot * 4; }
 
 template <typename T, bool STORE>
 __global__ void __launch_bounds__(256, STORE ? 2 : 3) rotary_store_kernel(const __grid_constant__ RotaryParams P) {
-  constexpr int U = heads_a_thread(STORE);
   extern __shared__ __align__(16) uint8_t sm[];
   pdl_wait();
   pdl_trigger();
@@ -155,7 +153,7 @@ __global__ void __launch_bounds__(256, STORE ? 2 : 3) rotary_store_kernel(const 
   const int lines = P.pos ? P.rot >> 2 : 0;  // 16-byte pieces of a table row
   // the token whose rows are fetched next, and its position
   unsigned ft = blockIdx.x;
-  auto place = [&](unsigned t) { return lines && t < tokens ? __ldg(P.pos + t) : (int64_t)0; };
+  auto place = [&](unsigned t) { return lines && t < tokens ? P.pos[t] : (int64_t)0; };
   int64_t fpos = place(ft);
   auto fetch = [&](int s) {
     if (ft < tokens) {
@@ -179,12 +177,12 @@ __global__ void __launch_bounds__(256, STORE ? 2 : 3) rotary_store_kernel(const 
   for (int i = 0; i < STAGES - 1; ++i) fetch(i);
   int s = 0;
   int slot = -1;
-  if (STORE && blockIdx.x < tokens) slot = __ldg(P.slots + blockIdx.x);
+  if (STORE && blockIdx.x < tokens) slot = P.slots[blockIdx.x];
   for (unsigned t = blockIdx.x; t < tokens; t += gridDim.x) {
     const bool store = STORE && slot >= 0 && slot < P.num_slots;
     const int page = store ? (int)((unsigned)slot / (unsigned)P.page) : 0;
     const int srow = store ? slot - page * P.page : 0;
-    if (STORE && t + gridDim.x < tokens) slot = __ldg(P.slots + t + gridDim.x);
+    if (STORE && t + gridDim.x < tokens) slot = P.slots[t + gridDim.x];
     cp_wait<STAGES - 2>();
     __syncthreads();  // every thread's part of the table row is there, and the stage before is read
     fetch(s == 0 ? STAGES - 1 : s - 1);
@@ -285,7 +283,7 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
   bool there[READ_TOKENS];
 #pragma unroll
   for (int i = 0; i < READ_TOKENS; ++i) {
-    const int slot = t0 + i < P.tokens ? __ldg(P.slots + t0 + i) : -1;
+    const int slot = t0 + i < P.tokens ? P.slots[t0 + i] : -1;
     there[i] = slot >= 0 && slot < P.num_slots;
     const int page = there[i] ? (int)((unsigned)slot / (unsigned)P.page) : 0;
     page_at[i] = page * P.s_page;
@@ -330,7 +328,6 @@ template <typename T, bool STORE>
 inline int launch_rotary_as(const RotaryParams& P, cudaStream_t st) {
   // heads side by side: as many as 256 threads hold, shared out evenly over the CTAs they take (by fours:
   // whole warps for the store's shuffles, 8 units a head there)
-  constexpr int U = heads_a_thread(STORE);
   const int units = P.d / 16, heads = P.hq + P.hk + P.hv, most = 256 / units;
   const int shares = (int)cdiv(heads, U * most);
   const int even = (int)cdiv(cdiv(heads, U * shares), 4) * 4, lanes = even <= most ? even : most;
@@ -345,7 +342,7 @@ inline int launch_rotary_as(const RotaryParams& P, cudaStream_t st) {
       return ADA_ERR_CUDA;
     ready[dev] = true;
   }
-  // as many CTAs as the SMs hold (80 registers a thread, shared memory) stay and walk the tokens
+  // as many CTAs as the SMs hold (128 or 80 registers a thread, shared memory) stay and walk the tokens
   const int by_regs = 65536 / ((STORE ? 128 : 80) * threads), by_smem = 232448 / (smem + 1024);
   const int64_t walkers = cdiv(148 * (by_regs < by_smem ? by_regs : by_smem), ys);
   (void)launch_k(rotary_store_kernel<T, STORE>, dim3((unsigned)(P.tokens < walkers ? P.tokens : walkers), (unsigned)ys),
@@ -422,7 +419,7 @@ extern "C" int ada_kv4_store(const int64_t* positions, const void* q, int64_t q_
                              uint8_t* v_cache, int64_t kv_stride_page, int64_t kv_stride_head, int64_t num_pages,
                              int32_t page_size, float k_scale, float v_scale, int dtype, void* stream) {
   if (head_dim != kv4::D) return ADA_ERR_UNSUPPORTED;
-  if (num_tokens < 0 || !(k_scale > 0.f) || !(v_scale > 0.f)) return ADA_ERR_INVALID_ARG;
+  if (num_tokens < 0 || !kv4::scale_ok(k_scale) || !kv4::scale_ok(v_scale)) return ADA_ERR_INVALID_ARG;
   if (num_tokens == 0) return ADA_OK;
   if (!k || !v || !slot_mapping || (reinterpret_cast<uintptr_t>(slot_mapping) & 3)) return ADA_ERR_INVALID_ARG;
   if (const int e = kv4::cache_ok(k_cache, v_cache, kv_stride_page, kv_stride_head, num_pages, num_kv_heads, page_size))
@@ -467,7 +464,7 @@ extern "C" int ada_kv4_read(const uint8_t* k_cache, const uint8_t* v_cache, int6
                             int64_t kv_stride_head, int64_t num_pages, int32_t page_size, int32_t num_kv_heads,
                             int32_t head_dim, const int32_t* slot_mapping, int64_t num_tokens, float k_scale,
                             float v_scale, void* k, void* v, int dtype, void* stream) {
-  if (num_tokens < 0 || !(k_scale > 0.f) || !(v_scale > 0.f)) return ADA_ERR_INVALID_ARG;
+  if (num_tokens < 0 || !kv4::scale_ok(k_scale) || !kv4::scale_ok(v_scale)) return ADA_ERR_INVALID_ARG;
   if (dtype != ADA_DT_BF16 && dtype != ADA_DT_F16) return ADA_ERR_INVALID_ARG;
   if (head_dim != kv4::D) return ADA_ERR_UNSUPPORTED;
   if (num_tokens == 0) return ADA_OK;

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(Params P) {
   const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
   Sums sum{0, 0, 0};
   for (int b = b0; b < b1; ++b) {
-    const int c = max(__ldg(P.cached + b), 0), n = max(__ldg(P.fresh + b), 0);
+    const int c = max(P.cached[b], 0), n = max(P.fresh[b], 0);
     const int all = add_sat(c, n);
     had[b] = c;
     sum = sum + Sums{n, all, pages_of(all, P.page) - pages_of(c, P.page)};
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(Params P) {
   for (int b = b0; b < b1; ++b) {
     cu_q[b] = run.q;
     cu_p[b] = run.p;
-    const int c = had[b], n = max(__ldg(P.fresh + b), 0);
+    const int c = had[b], n = max(P.fresh[b], 0);
     const int all = add_sat(c, n);
     if (first) {
       P.cu_q[b] = run.q;
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(Params P) {
   }
   __syncthreads();
   const int total = cu_q[B], taken = cu_p[B];
-  const int64_t start = __ldg(P.free_start);
+  const int64_t start = *P.free_start;
   if (first && tid == 0) {
     *P.free_next = (int)max(min(start + taken, P.num_free), min(start, P.num_free));
     if (total > P.tokens) err |= ERR_TOKENS;
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(Params P) {
     else if (col >= P.max_pages)
       err |= ERR_WIDTH;
     else
-      P.tables[b * P.t_stride + col] = __ldg(P.free_pages + at);
+      P.tables[b * P.t_stride + col] = P.free_pages[at];
   }
   // the tokens
   for (int64_t t = me; t < P.tokens; t += step) {
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(Params P) {
           id = P.tables[b * P.t_stride + col];
         } else {
           const int64_t at = start + cu_p[b] + (col - owned);
-          if (at >= 0 && at < P.num_free) id = __ldg(P.free_pages + at);
+          if (at >= 0 && at < P.num_free) id = P.free_pages[at];
         }
       } else {
         err |= ERR_WIDTH;

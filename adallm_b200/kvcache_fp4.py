@@ -14,6 +14,7 @@ import functools
 import torch
 
 from . import _native as N
+from .rotary_embedding import check_table
 
 I32, U8 = torch.int32, torch.uint8
 LARGEST = 0x7FFFFFFF  # windows past any position
@@ -76,7 +77,7 @@ def _store(device, rotation, key, value, k_cache, v_cache, slot_mapping, k_scale
         qs0, qs1, _ = query.stride()
         hq = query.shape[1]
         size = cos_sin.shape
-        reach, width = size[0], size[-1]
+        reach, width = size[0], size[-1]  # [positions, (1,) width]
     st = N.kv4_store(device, pos, q, qs0, qs1, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], out, tokens,
                      hq, hkv, HEAD_DIM, table, reach, width, turn, slots.data_ptr(), k_cache.data_ptr(),
                      v_cache.data_ptr(), s_page, s_head, pages, page, k_scale, v_scale, code, N.raw_stream(device))
@@ -90,7 +91,7 @@ def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
 
     slot = page * page_size + row; slots outside the cache (-1 among them) are skipped, and a slot
     given twice holds a mix of both rows.  Of each 16 elements: scale = e4m3(max |x| / 6), codes = the nearest e2m1
-    to x / scale; infinities saturate, a NaN makes its 16 elements read as NaN."""
+    to x / scale; infinities saturate, a NaN makes its 16 elements read as NaN.  k_scale and v_scale: 1e-30 to 1e30."""
     device = N.one_device("store_kvcache_fp4", key, value, k_cache, v_cache, slot_mapping)
     _store(device, None, key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
 
@@ -102,15 +103,14 @@ def rotary_store_kvcache_fp4(positions: torch.Tensor, query: torch.Tensor, key: 
     """apply_rotary on query and key, and store_kvcache_fp4 of the rotated key and the value, in one launch.
 
     query [T, Hq, 128], key/value [T, Hkv, 128]; the rest as in rotary_embedding.apply_rotary and
-    store_kvcache_fp4.  Returns the rotated query (q_out, contiguous, if given)."""
+    store_kvcache_fp4.  Returns the rotated query (q_out, contiguous, if given; no input may lie in it)."""
     device = N.one_device("rotary_store_kvcache_fp4", key, query, value, positions, cos_sin_cache, k_cache, v_cache,
                           slot_mapping)
     query = _rows(query, "query")
     shape, dtype = query.shape, query.dtype
     if shape[0] != key.shape[0] or positions.numel() != shape[0] or dtype is not key.dtype:
         raise ValueError("positions, query and key must describe the same tokens in one type")
-    if cos_sin_cache.dtype is not torch.float32 or not cos_sin_cache.is_contiguous():
-        raise ValueError("cos_sin_cache must be contiguous fp32")
+    check_table(cos_sin_cache)
     if positions.dtype is not torch.int64 or not positions.is_contiguous():
         positions = positions.to(torch.int64).contiguous()
     if q_out is None:

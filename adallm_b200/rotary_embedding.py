@@ -82,13 +82,22 @@ def apply_rope(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, 
     return qo.view(query.shape), ko.view(key.shape)
 
 
+def check_table(cos_sin_cache: torch.Tensor) -> None:
+    shape = cos_sin_cache.shape
+    if cos_sin_cache.dtype is not torch.float32 or not cos_sin_cache.is_contiguous():
+        raise ValueError("cos_sin_cache must be contiguous fp32")
+    if len(shape) < 2 or shape[0] * shape[-1] != cos_sin_cache.numel():
+        raise ValueError("cos_sin_cache must be [max_position, (1,) rotated width]")
+
+
 def apply_rotary(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, cos_sin_cache: torch.Tensor,
                  interleaved: bool = False, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
     """Rotate the first r = cos_sin_cache.shape[-1] elements of each head; the others are copied.
 
     positions [T] (clamped to the table); query [T, Hq, D], key [T, Hkv, D] bf16/fp16, any strides over tokens and
     heads that are multiples of 8; cos_sin_cache fp32 [max_position, (1,) r] = [cos | sin] of r / 2 pairs.  Pairs are
-    (i, i + r / 2), or (2i, 2i + 1) with interleaved.  Returns new contiguous tensors (q_out, k_out if given)."""
+    (i, i + r / 2), or (2i, 2i + 1) with interleaved.  Returns new contiguous tensors (q_out, k_out if given; no input may
+    lie in them)."""
     device = N.one_device("rotary_embedding", query, positions, key, cos_sin_cache)
     dtype = query.dtype
     code = N.DT.get(dtype)
@@ -107,8 +116,7 @@ def apply_rotary(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor
     tk, hk, dk = k_shape = key.shape
     if tk != t or positions.numel() != t or dk != d:
         raise ValueError("positions, query and key must describe the same tokens")
-    if cos_sin_cache.dtype is not torch.float32 or not cos_sin_cache.is_contiguous():
-        raise ValueError("cos_sin_cache must be contiguous fp32")
+    check_table(cos_sin_cache)
     if positions.dtype is not torch.int64 or not positions.is_contiguous():
         positions = positions.to(torch.int64).contiguous()
     if q_out is None:

@@ -77,7 +77,7 @@ def step_metadata(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table
                 raise ValueError("out must hold contiguous tensors as empty_step_metadata makes them")
     positions, slots, cu_q, cu_k, context, free_next = out
     st = N.step_metadata(device, cached_lens.data_ptr(), new_lens.data_ptr(), requests, block_tables.data_ptr(),
-                         row_stride if row_stride > max_pages else max_pages, max_pages, free_pages.data_ptr(),
+                         max_pages if requests == 1 else row_stride, max_pages, free_pages.data_ptr(),
                          free_pages.numel(), free_start.data_ptr(), page_size, num_tokens, positions.data_ptr(),
                          slots.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), context.data_ptr(), free_next.data_ptr(),
                          word, N.raw_stream(device))

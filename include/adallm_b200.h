@@ -705,7 +705,8 @@ ADA_API int ada_rotary(const int64_t* positions, const void* q, int64_t q_stride
  * k_cache, v_cache: one block of page_size * 72 bytes per (page, KV head) at page * kv_stride_page + head *
  * kv_stride_head (bytes, multiples of 16): page_size rows of 64 bytes of e2m1 codes (even element in
  * the low nibble), then page_size rows of 8 e4m3 scales, one for 16 elements.
- * value = code * scale * k_scale (v_scale).  head_dim 128, page_size % 16 == 0.
+ * value = code * scale * k_scale (v_scale).  head_dim 128, page_size % 16 == 0 up to 2^24; k_scale, v_scale
+ * 1e-30 to 1e30 here and in the attention below.
  *
  * ada_kv4_store packs the rows of k and v (strides as in ada_rotary) at slot_mapping int32 [T] (slot = page *
  * page_size + row; slots outside the cache, -1 among them, are skipped; a slot given twice holds a mix
@@ -734,7 +735,8 @@ ADA_API int ada_kv4_read(const uint8_t* k_cache, const uint8_t* v_cache, int64_t
  * head.  Keys, values and probabilities enter the products in fp16, bf16 queries exactly (scaled by a power of two).
  * out may have any strides that are multiples of 8.  workspace: ada_kv4_paged_decode_workspace_size bytes (0 for
  * short caches and windows: one launch), 16-byte aligned, no initial value; calls that share one must be
- * ordered as a whole.  Implemented: batch <= 8192, batch x KV heads x 32-key steps of a table row below 2^31. */
+ * ordered as a whole.  Implemented: batch <= 8192, batch x KV heads x 32-key steps of a table row up to
+ * 2^30, scale in (0, 1e30]. */
 ADA_API size_t ada_kv4_paged_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t num_kv_heads,
                                                    int32_t max_pages, int32_t page_size, int32_t window);
 ADA_API int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h,
@@ -749,9 +751,9 @@ ADA_API int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b,
 /* Causal prefill attention over the 4-bit cache: arguments and masks as ada_fp8_paged_prefill (window W > 0:
  * the row's own position and the W before it); rows of q and out outside [0, total_q) and rows
  * behind the last sequence are not touched.  A few rows a KV head (max_seqlen_q x heads a KV head up to 32)
- * behind tables of more than 256 keys take the decode form, which shares long caches out over all SMs.  workspace: as for decode, sized by
- * ada_kv4_paged_prefill_workspace_size (0 for more rows).  *err (may be NULL): 0x70 if a tile wait ran out (the
- * rows concerned are NaN).  A NaN key reaches every element of the rows that see it, a NaN value the 16 elements of its
+ * behind tables of more than 256 keys take the decode form, which shares long caches out over all SMs.
+ * workspace: as for decode, sized by ada_kv4_paged_prefill_workspace_size (0 for more rows).  *err (may be NULL): 0x70
+ * if a tile wait ran out (the rows concerned are NaN).  A NaN key reaches every element of the rows that see it, a NaN value the 16 elements of its
  * block, and neither any other row.  Implemented: up to 256 heads a KV head. */
 ADA_API size_t ada_kv4_paged_prefill_workspace_size(int32_t batch, int64_t total_q, int32_t max_seqlen_q,
                                                     int32_t num_heads, int32_t num_kv_heads, int32_t max_pages,

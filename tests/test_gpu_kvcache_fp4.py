@@ -7,6 +7,7 @@ import torch
 
 from adallm_b200 import kvcache_fp4 as kv
 from adallm_b200.rotary_embedding import apply_rotary
+from adallm_b200.step_metadata import step_metadata
 from oracle import kv4
 from tests.gpu_util import dev
 
@@ -133,6 +134,30 @@ def test_strided_caches():
     assert (pool[:, 0] == 0).all() and (pool[:, 2] == 0).all()
     a, b = kv.read_kvcache_fp4(kc, vc, slots, F16)
     assert torch.equal(a, kv4.stored(k).half()) and torch.equal(b, kv4.stored(v).half())
+
+
+def test_caches_past_32_bits():
+    """Pages and heads further apart than 32 bits count, and a page of more rows than 16 bits count."""
+    g = gen(9)
+    hkv, page, lens = 2, 16, [40, 17]
+    far = torch.empty(11 << 30, dtype=torch.uint8, device=dev())
+    t, slots = 57, torch.tensor([*range(40), *range(64, 81)], dtype=torch.int32, device=dev())
+    k, v, q = randn((t, hkv, 128), g), randn((t, hkv, 128), g), randn((2, 8, 128), g)
+    tables = torch.tensor([[0, 1, 2], [4, 5, -1]], dtype=torch.int32, device=dev())
+    ctx, i32 = torch.tensor(lens, dtype=torch.int32, device=dev()), dict(dtype=torch.int32, device=dev())
+    kc, vc = (far[o:].as_strided((6, hkv, page * 72), ((1 << 30) + 32, (5 << 30) + (1 << 21), 1)) for o in (0, 1 << 20))
+    near = [torch.zeros((6, hkv, page * 72), dtype=torch.uint8, device=dev()) for _ in range(2)]
+    outs = []
+    for c in ((kc, vc), near):
+        kv.store_kvcache_fp4(k, v, *c, slots)
+        outs.append((*kv.read_kvcache_fp4(*c, slots), kv.paged_decode_fp4(q, *c, tables, ctx, 0.1),
+                     kv.paged_prefill_fp4(q, *c, tables, torch.tensor([0, 1, 2], **i32), torch.tensor([0, 40, 57], **i32), 1, 0.1)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    rows = 80000  # one page
+    kc, vc = (far[o:o + rows * 72].view(1, 1, rows * 72) for o in (0, rows * 72))
+    slots = torch.arange(rows - t, rows, **i32)
+    kv.store_kvcache_fp4(k[:, :1], v[:, :1], kc, vc, slots)
+    assert torch.equal(kv.read_kvcache_fp4(kc, vc, slots, F16)[0], kv4.stored(k[:, :1]).half())
 
 
 # ---- attention ----
@@ -413,6 +438,50 @@ def test_split_prefill_and_decode_agree_with_one_prefill():
     assert_near(run_decode(last), want[332:], err[332:])
 
 
+def test_attention_directly_behind_the_metadata_that_extends_its_tables():
+    """No launch in between: the tables' new entries are seen, next to old ones that the first launch reads."""
+    g = gen(40)
+    d, i32, page, hq, hkv = dev(), dict(dtype=torch.int32, device=dev()), 16, 16, 4
+    cached, new = [16 * (i % 5) for i in range(12)], [1 + 40 * (i % 3) for i in range(12)]
+    lens = [a + b for a, b in zip(cached, new)]
+    kc, vc = kv4.make_cache(200, hkv, page, g, d), kv4.make_cache(200, hkv, page, g, d)
+    old = torch.full((12, 12), -1, **i32)
+    for b, n in enumerate(cached):
+        old[b, :n // page] = torch.arange(10 * b, 10 * b + n // page)
+    free, start = torch.arange(150, 200, **i32), torch.zeros(1, **i32)
+    q = randn((sum(new), hq, 128), g)
+    one, wide = randn((12, hq, 128), g), torch.full((12, 12 + 128), -1, **i32)
+    a, b = torch.tensor(cached, **i32), torch.tensor(new, **i32)
+    for tables in (wide[:, :12], wide):
+        for _ in range(5):
+            wide.fill_(-1)
+            wide[:, :12] = old
+            torch.cuda.synchronize()
+            m = step_metadata(a, b, tables, free, start, page, sum(new))
+            pre = kv.paged_prefill_fp4(q, kc, vc, tables, m.cu_seqlens_q, m.cu_seqlens_k, max(new), 0.1)
+            wide.fill_(-1)
+            wide[:, :12] = old
+            torch.cuda.synchronize()
+            m = step_metadata(a, b, tables, free, start, page, sum(new))
+            dec = kv.paged_decode_fp4(one, kc, vc, tables, m.context_lens, 0.1)
+            assert (tables >= 0).sum().item() == sum(-(-n // page) for n in lens)
+            assert_near(pre, *kv4.attention(q, kc, vc, tables, new, lens, 0.1))
+            assert_near(dec, *kv4.attention(one, kc, vc, tables, [1] * 12, lens, 0.1, decode=True))
+
+
+def test_output_over_the_queries():
+    c = make(42, [900, 33, 0, 500], [3, 1, 0, 2], 16, 4, 16)
+    for d in (c, behind_long_tables(c)):
+        want = run_prefill(d)
+        q = d["q"].clone()
+        out = run_prefill(dict(d, q=q), out=q)
+        assert out is q and torch.equal(q, want)
+    c = make(43, [900, 33, 0, 500], [1] * 4, 16, 4, 16)
+    want = run_decode(c)
+    q = c["q"].clone()
+    assert torch.equal(run_decode(dict(c, q=q), out=q), want)
+
+
 def test_streams_graphs_and_two_calls_at_once():
     a, b = (make(s, [2900, 3, 250], [1, 1, 1], 32, 8, 16) for s in (31, 32))
     wa, wb = run_decode(a), run_decode(b)
@@ -502,6 +571,9 @@ def test_refusals():
     bad(st, rows, rows, k, v, slots[:2])
     bad(st, rows, rows, k, v, slots.long())
     bad(st, rows, rows, k, v, slots, 0.0)
+    bad(st, rows, rows, k, v, slots, 1e-39)
+    pos, table = torch.zeros(3, dtype=torch.int64, device=dev()), torch.zeros(64, device=dev())
+    bad(kv.rotary_store_kvcache_fp4, pos, rows, rows, rows, table, k, v, slots)
     bad(kv.read_kvcache_fp4, k, v, slots, torch.float32)
     bad(kv.empty_kvcache_fp4, 1, 1, 8)
 

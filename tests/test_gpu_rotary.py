@@ -167,6 +167,9 @@ def test_empty_and_refusals():
                  (pos, q[..., :72].contiguous(), k[..., :72].contiguous(), table)):
         with pytest.raises(ValueError):
             apply_rotary(*args)
+    for bad in (table[0], table[:, None].expand(8, 2, 64).contiguous()):  # [width], [positions, 2, width]
+        with pytest.raises(ValueError):
+            apply_rotary(pos, q, k, bad)
     with pytest.raises(ValueError):  # in place: a pair's halves belong to two threads
         apply_rotary(pos, q, k, table, q_out=q)
     with pytest.raises(ValueError):

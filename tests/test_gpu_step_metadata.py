@@ -186,6 +186,7 @@ def test_refusals():
     bad(1, torch.ones(3, **i32))
     bad(2, torch.zeros((3, 4), **i32))
     bad(2, torch.zeros((2, 4), **i32).t().contiguous().t())
+    bad(2, torch.zeros((1, 4), **i32).expand(2, 4))  # rows that share their pages' memory
     bad(3, torch.arange(18, **i32)[::2])
     bad(4, torch.zeros(2, **i32))
     bad(5, 0)

@@ -41,7 +41,9 @@ def test_decode_refusals(lib):
         (dict(ctx=None), BAD), (dict(out=None), BAD), (dict(qd=2), BAD), (dict(od=-1), BAD), (dict(d=64), UNSUP),
         (dict(page=24), UNSUP), (dict(page=0), BAD), (dict(hq=31), BAD), (dict(hkv=0), BAD), (dict(hq=0), BAD),
         (dict(window=-1), BAD), (dict(bts=3), BAD), (dict(mp=0), BAD), (dict(pages=0), BAD), (dict(scale=0.0), BAD),
-        (dict(scale=math.nan), BAD), (dict(ks=-1.0), BAD), (dict(vs=0.0), BAD), (dict(q=8), ALIGN), (dict(k=8), ALIGN),
+        (dict(scale=math.nan), BAD), (dict(scale=math.inf), BAD), (dict(ks=-1.0), BAD), (dict(vs=0.0), BAD),
+        (dict(ks=math.inf), BAD), (dict(ks=1e-39), BAD), (dict(vs=math.inf), BAD),
+        (dict(page=1 << 25, sp=1 << 36, sh=1 << 32), UNSUP), (dict(hq=1 << 30, hkv=1 << 30, mp=1 << 26, bts=1 << 26), UNSUP), (dict(q=8), ALIGN), (dict(k=8), ALIGN),
         (dict(out=24), ALIGN), (dict(qsh=132), ALIGN), (dict(osb=4100), ALIGN), (dict(sh=1160, sp=9999), ALIGN),
         (dict(sp=8 * 1152 + 8), ALIGN), (dict(sh=1136), BAD), (dict(bt=18), ALIGN), (dict(ctx=17), ALIGN),
         (dict(mp=1 << 27, bts=1 << 27), UNSUP), (dict(mp=200, bts=200, ws=None), WS),
@@ -70,6 +72,7 @@ def test_prefill_refusals(lib):
     size = lib.ada_kv4_paged_prefill_workspace_size
     assert size(1, 50, 50, 32, 8, 40, 16) == 0 and size(1, 50, 8, 32, 8, 40, 16) > 0
     assert size(1, 50, 8, 32, 8, 16, 16) == 0 and size(1, 0, 8, 32, 8, 40, 16) == 0
+    assert size(8000, 8000, 1, 1 << 30, 1 << 30, 1 << 26, 16) == 0 and size(1, 1, 1, 8, 8, 1 << 30, 1 << 30) == 0
 
 
 STORE = dict(pos=16, q=32, qst=4096, qsh=128, k=48, kst=1024, ksh=128, v=64, vst=1024, vsh=128, qo=80, t=3, hq=32, hkv=8,
@@ -83,7 +86,8 @@ def test_store_refusals(lib):
         (dict(t=-1), BAD), (dict(q=None), BAD), (dict(qo=None), BAD), (dict(qo=32), BAD), (dict(k=None), BAD),
         (dict(v=None), BAD), (dict(slots=None), BAD), (dict(kc=None), BAD), (dict(table=None), BAD), (dict(maxp=0), BAD),
         (dict(rot=0), BAD), (dict(rot=144), BAD), (dict(rot=40), UNSUP), (dict(d=64), UNSUP), (dict(page=20), UNSUP),
-        (dict(ks=0.0), BAD), (dict(vs=math.nan), BAD), (dict(dt=2), BAD), (dict(q=8), ALIGN), (dict(kst=1020), ALIGN),
+        (dict(ks=0.0), BAD), (dict(vs=math.nan), BAD), (dict(ks=math.inf), BAD), (dict(vs=1e-39), BAD),
+        (dict(page=1 << 25, sp=1 << 36, sh=1 << 32), UNSUP), (dict(dt=2), BAD), (dict(q=8), ALIGN), (dict(kst=1020), ALIGN),
         (dict(vsh=4), ALIGN), (dict(kc=8), ALIGN), (dict(table=18), ALIGN), (dict(pos=12), ALIGN)])
 
 
@@ -101,7 +105,7 @@ def test_rotary_and_read_refusals(lib):
     assert lib.ada_kv4_read(*{**good, "t": 0}.values()) == 0
     refuse(lib.ada_kv4_read, good, [
         (dict(kc=None), BAD), (dict(slots=None), BAD), (dict(k=None), BAD), (dict(v=40), ALIGN), (dict(dt=2), BAD),
-        (dict(d=96), UNSUP), (dict(page=15), UNSUP), (dict(ks=0.0), BAD), (dict(t=-1), BAD)])
+        (dict(d=96), UNSUP), (dict(page=15), UNSUP), (dict(ks=0.0), BAD), (dict(vs=math.inf), BAD), (dict(t=-1), BAD)])
 
 
 def test_metadata_refusals(lib):
