@@ -9,14 +9,13 @@
 // (16 a cycle and SM: 1,024 cycles) and 2 x 256 x 64 x 128 multiply-adds (4,096 a cycle: 1,024).
 //
 // One CTA a (256-row query block, KV head, sequence); 14 warps:
-//   warp 0        producer: copies the codes and scales of each block's four 16-key tiles (contiguous
-//                 pieces of 1,024 and 128 bytes) into a staging ring;
-//   warp 1        MMA issuer and TMEM owner: S_t = Q_t K^T for the two 128-row tiles t (M 128, N 64) into
-//                 one of a tile's two S buffers, O_t += P_t V with P_t as the A operand in TMEM;
-//   warps 2-5     converters: codes x scales -> f16 K and V operand tiles (exact);
+//   warp 0        TMEM owner, issues S_t = Q_t K^T for the two 128-row tiles t (M 128, N 64);
+//   warp 1        issues O_t += P_t V with P_t as the A operand in TMEM;
+//   warps 2-5     converters: a 16-key tile of each block each (in one page): its codes and scales by cp.async
+//                 into a ring of the warp's own, codes x scales -> f16 K and V operand tiles (exact);
 //   warps 6-9, 10-13   softmax of tile 0 and 1, thread = row: brings its query row into shared memory
 //                 as f16 (times a power of two, kv4.cuh), then per block reads 64 scores from TMEM and
-//                 writes 64 f16 probabilities over them, where P V reads them: no shared memory and no
+//                 writes 64 f16 probabilities there, where P V reads them: no shared memory and no
 //                 proxy fence in between.  A row's reference moves when a score passes it by
 //                 8 (log2); only then its O row is rescaled.
 //
@@ -24,14 +23,18 @@
 // the converters widen it as 0 and mark (key, scale block), and rows that see a marked key turn
 // their 16 elements to NaN at the end.
 //
-// Barriers (block j, tile t): e_full[j % NSTG], e_empty, kv_full[j % NKV], kv_empty (commit after both P V),
-// s_full[t][j & 1] (commit, and an arrival of the issuer's own), p_full[t][j & 1] (4 warps), o_done[t] (commit
-// after P V), o_last[t] (after the last one), q_ready (8 warps), fin.
+// Barriers (block j, tile t): kv_empty[j % NKV] (commit after both P V); s_go[t][j % NKV]: S_j
+// may run (4 converters; 4 softmax warps, which have S_{j-1} in registers, or Q in place for j = 0); s_full[t][j & 1] (commit
+// after S_j, an arrival of its issuer's own, commit after P V of j - 2); p_full[t][j & 1] (4 warps); o_last[t] (commit
+// after the last P V); fin.  Few waits, as each takes 150-300 cycles also where it passes.
+// The scores have one place a tile and the probabilities two: S_{j+1} is issued as soon as the softmax has S_j
+// in registers, and runs under its exponentials; P_j stays where it is until P V has read it.
 // A wait by parity needs the phase before to be known complete and the next one not begun.  Refills wait
-// for the release of the use before, in every phase; S_{j+2} is issued after p_full of j.  o_done of j - 1: the
-// issuer waits for it (in turn) before S_{j+1} overwrites the buffer that P_{j-1} lay in, so a softmax that
-// has S_j knows that of j - 2 complete, and that of j cannot begin before its own p_full.  The
-// end waits for o_last, which has one phase.
+// for the release of the use before, in every phase.  An arrival for the next phase of s_go[t][j % NKV] follows kv_empty of j
+// or S_{j+2}; one for the next of s_full[t][j & 1] is P V of j, behind p_full of j, which follows this phase, or S_{j+2}, behind
+// the read of S_{j+1}; p_full of j + 2 needs s_full of j + 2 and so P V of j.  A softmax that rescales O waits
+// for P V of j - 1 by kv_empty, whose phase before the converters of block j - 1 have seen.  The end waits for o_last,
+// which has one phase.
 #include "kv4.cuh"
 #include "tc_attention.cuh"
 
@@ -47,18 +50,20 @@ constexpr int THREADS = (2 + NCONV + NT * NSOFT) * 32;
 constexpr int Q_OFF = 0;                     // f16 Q, NT x [2 halves][128 rows][128 B]
 constexpr int K_OFF = Q_OFF + NT * 32768;    // f16 K, NKV x [2 halves][64 keys][128 B]
 constexpr int V_OFF = K_OFF + NKV * 16384;
-constexpr int E_OFF = V_OFF + NKV * 16384;   // staging: K codes, V codes, K scales, V scales of 64 keys
-constexpr int E_BYTES = 2 * BN * ROW_BYTES;
-constexpr int EV = BN * ROW, EKS = 2 * BN * ROW, EVS = EKS + BN * SROW;
-constexpr int BAR_OFF = E_OFF + NSTG * E_BYTES;
-constexpr int NBAR = 2 * NSTG + 2 * NKV + 6 * NT + 2;
-constexpr int FLAG_OFF = BAR_OFF + NBAR * 8;  // words: e_ok[NSTG], then per K/V slot [ok][4 warps' NaN flags][16 NaN masks]
+constexpr int E_OFF = V_OFF + NKV * 16384;   // converter warps' rings: K codes, V codes, K scales, V scales of a tile
+constexpr int E_BYTES = 2 * TILE * ROW_BYTES;
+constexpr int EV = TILE * ROW, EKS = 2 * TILE * ROW, EVS = EKS + TILE * SROW;
+constexpr int BAR_OFF = E_OFF + NCONV * NSTG * E_BYTES;
+constexpr int NBAR = NKV + NT * (NKV + 5) + NT * NSOFT + 1;
+constexpr int FLAG_OFF = (BAR_OFF + NBAR * 8 + 15) & ~15;  // words a K/V slot: [4 tiles there][4 tiles' NaN flags][16 NaN masks]
 constexpr int SLOT_WORDS = 24;
-constexpr int SMEM = 1024 + FLAG_OFF + (NSTG + NKV * SLOT_WORDS + 4) * 4;
-constexpr uint32_t TMEM_COLS = 512, S_COL = 256;  // O of tile t at 128 t; S buffer b of tile t at 256 + 128 t + 64 b
+constexpr int SMEM = 1024 + FLAG_OFF + (NKV * SLOT_WORDS + 4) * 4;
+static_assert(NCONV * TILE == BN, "a converter warp a tile");
+// O of tile t at 128 t; its S at 256 + 128 t, its P buffer b (f16, two a column) 64 + 32 b behind
+constexpr uint32_t TMEM_COLS = 512, S_COL = 256, P_COL = BN;
 constexpr float MOVE_LOG2 = 8.f;
 static_assert(SMEM <= 232448, "shared memory per CTA");
-static_assert(E_BYTES % 16 == 0 && BAR_OFF % 16 == 0 && (FLAG_OFF % 8) == 0, "alignment");
+static_assert(E_BYTES % 16 == 0 && BAR_OFF % 16 == 0 && FLAG_OFF % 16 == 0 && SLOT_WORDS % 4 == 0, "alignment");
 constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 // Up to this factor |score * factor| < 2^24, where the rounding of a row's reference is below 1 (log2).
@@ -144,45 +149,32 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *qs = base + Q_OFF, *kf = base + K_OFF, *vf = base + V_OFF, *es = base + E_OFF;
-  uint64_t* e_full = reinterpret_cast<uint64_t*>(base + BAR_OFF);
-  uint64_t* e_empty = e_full + NSTG;
-  uint64_t* kv_full = e_empty + NSTG;
-  uint64_t* kv_empty = kv_full + NKV;
-  uint64_t* s_full = kv_empty + NKV;   // [NT][2]
-  uint64_t* p_full = s_full + 2 * NT;  // [NT][2]
-  uint64_t* o_done = p_full + 2 * NT;  // [NT]
-  uint64_t* o_last = o_done + NT;      // [NT]
-  uint64_t* q_ready = o_last + NT;
-  uint64_t* fin = q_ready + 1;
-  int* e_ok = reinterpret_cast<int*>(base + FLAG_OFF);
-  uint32_t* slots = reinterpret_cast<uint32_t*>(e_ok + NSTG);
+  uint64_t* kv_empty = reinterpret_cast<uint64_t*>(base + BAR_OFF);
+  uint64_t* s_go = kv_empty + NKV;      // [NT][NKV]
+  uint64_t* s_full = s_go + NT * NKV;   // [NT][2]
+  uint64_t* p_full = s_full + 2 * NT;   // [NT][2]
+  uint64_t* o_last = p_full + 2 * NT;   // [NT]
+  uint64_t* q_raw = o_last + NT;        // [NT][NSOFT]
+  uint64_t* fin = q_raw + NT * NSOFT;
+  uint32_t* slots = reinterpret_cast<uint32_t*>(base + FLAG_OFF);
   uint32_t* tmem_slot = slots + NKV * SLOT_WORDS;
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* abort_v = abort_flag;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NSTG; ++s) {
-      mbar_init(&e_full[s], 1);
-      mbar_init(&e_empty[s], NCONV);
-    }
-    for (int i = 0; i < NKV; ++i) {
-      mbar_init(&kv_full[i], NCONV);
-      mbar_init(&kv_empty[i], 1);
-    }
+    for (int i = 0; i < NKV; ++i) mbar_init(&kv_empty[i], 1);
+    for (int i = 0; i < NT * NKV; ++i) mbar_init(&s_go[i], NCONV + NSOFT);
     for (int i = 0; i < 2 * NT; ++i) {
-      mbar_init(&s_full[i], 2);
+      mbar_init(&s_full[i], 3);
       mbar_init(&p_full[i], NSOFT);
     }
-    for (int t = 0; t < NT; ++t) {
-      mbar_init(&o_done[t], 1);
-      mbar_init(&o_last[t], 1);
-    }
-    mbar_init(q_ready, NT * NSOFT);
-    mbar_init(fin, 1);
+    for (int t = 0; t < NT; ++t) mbar_init(&o_last[t], 1);
+    for (int i = 0; i < NT * NSOFT; ++i) mbar_init(&q_raw[i], 1);
+    mbar_init(fin, 2);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
+  if (warp == 0) tmem_alloc(tmem_slot, TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -207,126 +199,64 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     nblk = k_end > k_lo ? (k_end - kb0 + BN - 1) / BN : 0;
   }
 
-  if (warp == 0) {  // ---------------- producer ----------------
-    // Lanes hold the places of 8 blocks' 32 tiles; lanes 0-15 each copy one piece of a block.
-    const int page_tiles = P.page / TILE;
-    const int64_t head = (int64_t)kvh * P.s_head;
-    auto place = [&](int first) -> int64_t {  // byte offset of the lane's tile's codes, -1: a hole
-      const int key0 = kb0 + TILE * (first + lane);
-      if (key0 >= k_end) return -1;
-      const int tile = key0 / TILE, col = tile / page_tiles;
-      const int64_t id = P.bt[(int64_t)b * P.bt_stride + col];
-      return id < 0 || id >= P.num_pages ? -1 : id * P.s_page + head + (int64_t)(tile - col * page_tiles) * (TILE * ROW);
-    };
-    int64_t cur = nblk > 0 ? place(0) : -1, nxt = nblk > 8 ? place(32) : -1;
-    int issued = 0;
-    for (int j = 0; j < nblk; ++j) {
-      if (j > 0 && (j & 7) == 0) {
-        cur = nxt;
-        nxt = j + 8 < nblk ? place(32 * (j / 8 + 1)) : -1;
-      }
-      const int s = j % NSTG;
-      int go = 1;
-      if (lane == 0) go = !*abort_v && (j < NSTG || wait_b(&e_empty[s], ((j / NSTG) - 1) & 1, abort_v, P.err));
-      if (!__shfl_sync(0xffffffffu, go, 0)) break;
-      // piece: tile (lane & 3) of K codes, V codes, K scales, V scales
-      const int tile = lane & 3, kind = (lane >> 2) & 3;
-      const int64_t at = __shfl_sync(0xffffffffu, cur, 4 * (j & 7) + tile);
-      const uint32_t mask = __ballot_sync(0xffffffffu, at >= 0) & 15u;
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (lane == 0) {
-        e_ok[s] = (int)mask;
-        mbar_arrive_expect_tx(&e_full[s], __popc(mask) * 2u * TILE * ROW_BYTES);
-      }
-      __syncwarp();
-      if (lane < 16 && at >= 0) {
-        const uint8_t* cache = (kind & 1) ? P.vc : P.kc;
-        uint8_t* st = es + s * E_BYTES;
-        if (kind < 2) {
-          bulk_load(st + kind * EV + tile * (TILE * ROW), cache + at, TILE * ROW, &e_full[s]);
-        } else {
-          const int row = (kb0 + j * BN + TILE * tile) % P.page;
-          bulk_load(st + (kind == 2 ? EKS : EVS) + tile * (TILE * SROW),
-                    cache + at - (int64_t)row * ROW + (int64_t)P.page * ROW + row * SROW, TILE * SROW, &e_full[s]);
-        }
-      }
-      issued = j + 1;
-    }
-    if (lane == 0) {
-      // leave no copy in flight when the CTA ends: wait (bounded) for the last use of each slot
-      for (int j = issued > NSTG ? issued - NSTG : 0; j < issued; ++j) {
-        uint32_t spins = 0;
-        const uint64_t t_start = globaltimer();
-        while (!mbar_try_wait(&e_full[j % NSTG], (j / NSTG) & 1)) {
-          if ((++spins & 63u) == 0 && globaltimer() - t_start > 2000000000ull) {
-            if (P.err) atomicOr(P.err, ERR_TILE_WAIT);
-            break;
-          }
-        }
-      }
-    }
-  } else if (warp == 1) {  // ---------------- MMA issuer ----------------
-    // The whole warp runs this loop, its values uniform, and one elected lane issues: the operands of the
+  if (warp < 2) {  // ---------------- MMA issuers: S, P V ----------------
+    // The whole warp runs its loop, the values uniform, and one elected lane issues: the operands of the
     // tcgen05 instructions then stay in uniform registers (from a divergent lane an MMA takes about 100
     // cycles to issue, 24 of them a block: 629 us instead of 518 for 4 x 2,048 tokens behind 2,048, 32/8 heads).
+    // S and P V have a warp each: a wait that passes takes 150-200 cycles, and five of them in turn left the
+    // tensor pipe idle for half of a block.
     if (nblk > 0) {
       const bool leader = elect_one();
       const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
       // low words of the descriptors: address / 16, leading offset / 16 (V: 8 KB between the halves of d)
       const uint32_t q_lo = (smem_u32(qs) >> 4) | (1u << 16), k_lo = (smem_u32(kf) >> 4) | (1u << 16);
       const uint32_t v_lo = (smem_u32(vf) >> 4) | ((8192u >> 4) << 16);
-      auto issue_s = [&](int j, uint32_t slot) {
-        if (leader) {
+      uint32_t slot = 0;
+      bool ok = true;
+      if (warp == 0) {
+        for (int j = 0; ok && j < nblk; ++j) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const uint32_t d = tm + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              mma_ss(d, q_lo + (uint32_t)t * 2048u + (uint32_t)(kk / 4) * 1024u + (uint32_t)(kk % 4) * 2u,
-                     k_lo + slot * 1024u + (uint32_t)(kk / 4) * 512u + (uint32_t)(kk % 4) * 2u, kk > 0);
-            tc_commit(&s_full[2 * t + (j & 1)]);
-            mbar_arrive_plain(&s_full[2 * t + (j & 1)]);  // passes on what kv_full ordered: the flags
-          }
-        }
-        __syncwarp();
-      };
-      uint32_t slot = 0;
-      bool ok = wait_b(q_ready, 0, abort_v, P.err) && wait_b(&kv_full[0], 0, abort_v, P.err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        tc_fence_after();
-        issue_s(0, 0);
-      }
-      for (int j = 0; ok && j < nblk; ++j) {
-        const uint32_t next = slot + 1 == NKV ? 0 : slot + 1;
-        if (j + 1 < nblk) {
-          ok = wait_b(&kv_full[next], ((j + 1) / NKV) & 1, abort_v, P.err);
-          if (j > 0)
-            ok = ok && wait_b(&o_done[0], (j - 1) & 1, abort_v, P.err) && wait_b(&o_done[1], (j - 1) & 1, abort_v, P.err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(j + 1, next);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          ok = __all_sync(0xffffffffu, ok && wait_b(&p_full[2 * t + (j & 1)], (j >> 1) & 1, abort_v, P.err));
-          if (ok) {
+            ok = __all_sync(0xffffffffu, ok && wait_b(&s_go[NKV * t + slot], (j / NKV) & 1, abort_v, P.err));
+            if (!ok) break;
             tc_fence_after();
             if (leader) {
-              const uint32_t p = tm + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
+              const uint32_t d = tm + S_COL + 128u * (uint32_t)t;
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                mma_ss(d, q_lo + (uint32_t)t * 2048u + (uint32_t)(kk / 4) * 1024u + (uint32_t)(kk % 4) * 2u,
+                       k_lo + slot * 1024u + (uint32_t)(kk / 4) * 512u + (uint32_t)(kk % 4) * 2u, kk > 0);
+              tc_commit(&s_full[2 * t + (j & 1)]);
+              mbar_arrive_plain(&s_full[2 * t + (j & 1)]);  // passes on what s_go ordered: flags, and V for P V
+            }
+            __syncwarp();
+          }
+          slot = slot + 1 == NKV ? 0 : slot + 1;
+        }
+      } else {
+        if (leader) {  // the probabilities' places are free
+          for (int i = 0; i < 2 * NT; ++i) mbar_arrive_plain(&s_full[i]);
+        }
+        __syncwarp();
+        for (int j = 0; ok && j < nblk; ++j) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            ok = __all_sync(0xffffffffu, ok && wait_b(&p_full[2 * t + (j & 1)], (j >> 1) & 1, abort_v, P.err));
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+              const uint32_t p = tm + S_COL + 128u * (uint32_t)t + P_COL + 32u * (uint32_t)(j & 1);
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)
                 mma_ts(tm + 128u * (uint32_t)t, p + 8u * (uint32_t)kk, v_lo + slot * 1024u + (uint32_t)kk * 128u,
                        j > 0 || kk > 0);
-              tc_commit(&o_done[t]);
-              if (j + 1 == nblk) tc_commit(&o_last[t]);
+              tc_commit(j + 1 == nblk ? &o_last[t] : &s_full[2 * t + (j & 1)]);  // (P_{j+2} may come)
               if (t == NT - 1) tc_commit(&kv_empty[slot]);
             }
             __syncwarp();
           }
+          slot = slot + 1 == NKV ? 0 : slot + 1;
         }
-        slot = next;
       }
       // every MMA issued above has completed before the teardown
       if (leader) tc_commit(fin);
@@ -341,92 +271,161 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       }
     }
   } else if (warp < 2 + NCONV) {  // ---------------- converters ----------------
-    const int ct = threadIdx.x - 64;
+    // Warp w brings and converts tile w of every block.  Its ring holds the codes and scales of NSTG blocks, by
+    // cp.async: a bulk copy takes a warp 60-100 cycles to issue, and a block has 16 contiguous pieces, so a warp that
+    // did nothing else needed 1,400-1,700 cycles a block and was the bound.
+    const int w = warp - 2, page_tiles = P.page / TILE;
+    uint8_t* ring = es + w * (NSTG * E_BYTES);
+    const uint8_t *kc = P.kc + (int64_t)kvh * P.s_head, *vc = P.vc + (int64_t)kvh * P.s_head;
+    int64_t codes = -1;  // of the lane's block (32 of them from a multiple on): its tile's codes in the cache, -1: a hole
+    int scales = 0;      // from there to its scales
+    uint32_t there = 0;  // bit s: the tile in ring slot s
+    int slot = 0;        // that the next block goes to
+    auto fetch = [&](int j) {
+      if (j < nblk) {
+        if ((j & 31) == 0) {
+          const int key0 = kb0 + BN * (j + lane) + TILE * w;
+          codes = -1;
+          if (j + lane < nblk && key0 < k_end) {
+            const int tile = key0 / TILE, col = tile / page_tiles, at = tile - col * page_tiles;
+            const int64_t id = P.bt[(int64_t)b * P.bt_stride + col];
+            if (id >= 0 && id < P.num_pages) {
+              codes = id * P.s_page + at * (TILE * ROW);
+              scales = P.page * ROW - at * (TILE * (ROW - SROW));
+            }
+          }
+        }
+        const int64_t at = __shfl_sync(0xffffffffu, codes, j & 31);
+        const int to = __shfl_sync(0xffffffffu, scales, j & 31);
+        there = (there & ~(1u << slot)) | ((uint32_t)(at >= 0) << slot);
+        if (at >= 0) {
+          const uint32_t dst = smem_u32(ring + slot * E_BYTES) + 16 * lane;
+          cp16(dst, kc + at + 16 * lane);
+          cp16(dst + 512, kc + at + 512 + 16 * lane);
+          cp16(dst + EV, vc + at + 16 * lane);
+          cp16(dst + EV + 512, vc + at + 512 + 16 * lane);
+          if (lane < 16) cp16(dst + EKS, (lane < 8 ? kc : vc - TILE * SROW) + at + to + 16 * lane);
+        }
+      }
+      cp_commit();
+      slot = slot + 1 == NSTG ? 0 : slot + 1;
+    };
+#pragma unroll
+    for (int j = 0; j < NSTG - 1; ++j) fetch(j);
+    int from = 0, kb = 0;
     for (int j = 0; j < nblk; ++j) {
-      const int s = j % NSTG, kb = j % NKV;
-      if (!wait_b(&e_full[s], (j / NSTG) & 1, abort_v, P.err)) break;
+      cp_wait<NSTG - 2>();
+      __syncwarp();  // every lane's part has arrived, and the slot before has been read
+      fetch(j + NSTG - 1);
       if (j >= NKV && !wait_b(&kv_empty[kb], ((j / NKV) - 1) & 1, abort_v, P.err)) break;
-      const uint8_t* st = es + s * E_BYTES;
-      const int mask = e_ok[s];
+      const uint8_t* st = ring + from * E_BYTES;
+      const bool ok = (there >> from) & 1u;
       uint32_t* flags = slots + kb * SLOT_WORDS;
       uint32_t nan_any = 0;
-      // 64 keys x 8 blocks of 16 elements an operand: 4 units a thread
+      // 16 keys x 8 blocks of 16 elements an operand: 4 units a lane
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int unit = ct + 128 * u, key = unit >> 3, blk = unit & 7;
-        const bool kok = (mask >> (key >> 4)) & 1;
-        const bool vok = kok & (kb0 + j * BN + key < len_k);
-        const uint2 kc = *reinterpret_cast<const uint2*>(st + 8 * unit);
-        const uint2 vc = *reinterpret_cast<const uint2*>(st + EV + 8 * unit);
-        const uint32_t ks = kok ? st[EKS + unit] : 0u;
+        const int unit = lane + 32 * u, key = TILE * w + (unit >> 3), blk = unit & 7;
+        const bool vok = ok & (kb0 + j * BN + key < len_k);
+        const uint2 k8 = *reinterpret_cast<const uint2*>(st + 8 * unit);
+        const uint2 v8 = *reinterpret_cast<const uint2*>(st + EV + 8 * unit);
+        const uint32_t ks = ok ? st[EKS + unit] : 0u;
         uint32_t vs = vok ? st[EVS + unit] : 0u;
         const bool nan = (vs & 0x7Fu) == 0x7Fu;
         const uint32_t marked = __ballot_sync(0xffffffffu, nan);  // 4 keys x 8 blocks
         if (nan) vs = 0;
         nan_any |= marked;
-        if (lane == 0) flags[8 + 4 * u + (warp - 2)] = marked;
+        if (lane == 0) flags[8 + 4 * w + u] = marked;
         uint4 lo, hi;
         const int c0 = ((blk & 3) * 2) ^ (key & 7), c1 = c0 ^ 1;
         const int at = kb * 16384 + (blk >> 2) * 8192 + key * 128;
-        widen16(kc, scale_f16x2(ks), lo, hi);
+        widen16(k8, scale_f16x2(ks), lo, hi);
         *reinterpret_cast<uint4*>(kf + at + (c0 << 4)) = lo;
         *reinterpret_cast<uint4*>(kf + at + (c1 << 4)) = hi;
-        widen16(vc, scale_f16x2(vs), lo, hi);
+        widen16(v8, scale_f16x2(vs), lo, hi);
         *reinterpret_cast<uint4*>(vf + at + (c0 << 4)) = lo;
         *reinterpret_cast<uint4*>(vf + at + (c1 << 4)) = hi;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
-        flags[4 + (warp - 2)] = nan_any;
-        if (warp == 2) flags[0] = (uint32_t)mask;
-        mbar_arrive_plain(&kv_full[kb]);
-        mbar_arrive_plain(&e_empty[s]);
+        flags[w] = ok;
+        flags[4 + w] = nan_any;
+        mbar_arrive_plain(&s_go[kb]);
+        mbar_arrive_plain(&s_go[NKV + kb]);
       }
+      kb = kb + 1 == NKV ? 0 : kb + 1;
+      from = from + 1 == NSTG ? 0 : from + 1;
     }
+    cp_wait<0>();
   } else {  // ---------------- softmax: warpgroup t, thread = row r of tile t ----------------
     const int t = (warp - 2 - NCONV) / NSOFT;
     const int q4 = warp & 3;  // the TMEM lane quarter that this warp may access
     const int r = 32 * q4 + lane, R = t * BM + r;
     const uint32_t trow = tmem + ((uint32_t)(32 * q4) << 16);
-    const uint32_t o_col = 128u * (uint32_t)t, s_col = S_COL + 128u * (uint32_t)t;
+    const uint32_t o_col = 128u * (uint32_t)t, s_col = S_COL + 128u * (uint32_t)t, p_col = s_col + P_COL;
     const int tok = t0 + R / P.group;
     const int64_t row = q_begin + tok;
     const bool valid = active && R < P.qt * P.group && tok < len_q && row >= 0 && row < P.rows;
+    const uint32_t there = __ballot_sync(0xffffffffu, valid);
     const int head = kvh * P.group + R % P.group;
     int lo = 0, hi = 0;
     if (valid) key_range(P, tok, off, len_k, lo, hi);
     float factor = 0.f;
-    if (nblk > 0) {  // the query row -> f16, times a power of two
-      const int64_t at = row * P.q_st + head * P.q_sh;
-      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(P.q) + at);
-      uint4 raw[16];
-#pragma unroll
-      for (int c = 0; c < 16; ++c) raw[c] = valid ? src[c] : make_uint4(0, 0, 0, 0);
-      float top = 0.f;
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        float f[8];
-        if (P.q_bf16) unpack8<__nv_bfloat16>(raw[c], f); else unpack8<__half>(raw[c], f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(f[i]));
+    uint8_t* rows = qs + t * 32768 + 4096 * q4;  // the warp's 32 rows of the Q tile, [2 halves at 16 KB]
+    if (nblk > 0) {
+      // The query rows -> f16, times a power of two.  They arrive by bulk copies, each half in its place, and are
+      // converted there: the L1 beside this much shared memory holds some 16 KB of loads under way, four
+      // round trips for 64 KB of rows (16,000 cycles a CTA instead of XXXX).
+      if (lane == 0) mbar_arrive_expect_tx(&q_raw[t * NSOFT + q4], __popc(there) * 256u);
+      __syncwarp();
+      if (valid) {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(P.q) + row * P.q_st + head * P.q_sh;
+        bulk_load(rows + lane * 128, src, 128, &q_raw[t * NSOFT + q4]);
+        bulk_load(rows + lane * 128 + 16384, src + 64, 128, &q_raw[t * NSOFT + q4]);
       }
-      const int ex = query_exponent(top);
-      const float mul = pow2(ex);
+      const bool got = __all_sync(0xffffffffu, wait_b(&q_raw[t * NSOFT + q4], 0, abort_v, P.err));
+      const int c = lane & 15, half = lane >> 4;
+      int ex = 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += 8) {  // a half-warp a row, four rows side by side
+        uint4 raw[4];
+        float top[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i0 + 2 * i + half;
+          raw[i] = *reinterpret_cast<const uint4*>(rows + r * 128 + (c >> 3) * 16384 + ((c & 7) << 4));
+          if (!got || !((there >> r) & 1u)) raw[i] = make_uint4(0, 0, 0, 0);
+          float f[8];
+          if (P.q_bf16) unpack8<__nv_bfloat16>(raw[i], f); else unpack8<__half>(raw[i], f);
+          top[i] = fabsf(f[0]);
+#pragma unroll
+          for (int k = 1; k < 8; ++k) top[i] = max_nan(top[i], fabsf(f[k]));
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i0 + 2 * i + half, e = query_exponent(top[i]);
+          const int theirs = __shfl_sync(0xffffffffu, e, 16 * (lane & 1));
+          if ((lane >> 1) == i0 / 2 + i) ex = theirs;
+          const float mul = pow2(e);
+          float f[8];
+          if (P.q_bf16) unpack8<__nv_bfloat16>(raw[i], f); else unpack8<__half>(raw[i], f);
+          *reinterpret_cast<uint4*>(rows + r * 128 + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) =
+              make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
+                         pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
+        }
+      }
       factor = score_factor(P.scale_log2, ex);
       if (!valid) factor = fminf(factor, SAFE_FACTOR);  // (all its keys are masked)
-      uint8_t* dst = qs + t * 32768 + r * 128;
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        float f[8];
-        if (P.q_bf16) unpack8<__nv_bfloat16>(raw[c], f); else unpack8<__half>(raw[c], f);
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) =
-            make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
-                       pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
-      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive_plain(q_ready);
+      if (lane == 0) mbar_arrive_plain(&s_go[NKV * t]);
     }
     const bool safe = __all_sync(0xffffffffu, factor <= SAFE_FACTOR);
     float m = -INFINITY;  // largest score that set the reference
@@ -435,18 +434,21 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     uint32_t nan_blocks = 0;
     bool failed = false;
     for (int j = 0; j < nblk; ++j) {
-      const int sb = j & 1;
       // warp-uniform outcome: the TMEM accesses below are warp-collective
-      if (!__all_sync(0xffffffffu, wait_b(&s_full[2 * t + sb], (j >> 1) & 1, abort_v, P.err))) {
+      if (!__all_sync(0xffffffffu, wait_b(&s_full[2 * t + (j & 1)], (j >> 1) & 1, abort_v, P.err))) {
         failed = true;
         break;
       }
       tc_fence_after();
       float x[64];
       uint32_t* sr = reinterpret_cast<uint32_t*>(x);
-      tmem_ld64(trow + s_col + BN * sb, sr);
+      tmem_ld64(trow + s_col, sr);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_plain(&s_go[NKV * t + (j + 1) % NKV]);
       const uint32_t* flags = slots + (j % NKV) * SLOT_WORDS;
-      const uint32_t blk_ok = flags[0];
+      const uint4 loaded = *reinterpret_cast<const uint4*>(flags);
+      const uint32_t blk_ok = loaded.x | (loaded.y << 1) | (loaded.z << 2) | (loaded.w << 3);
       const uint4 marked = *reinterpret_cast<const uint4*>(flags + 4);
       const int key0 = kb0 + j * BN, a = lo - key0, e = hi - key0;  // visible columns [a, e) of loaded tiles
       if (!__all_sync(0xffffffffu, blk_ok == 15u && a <= 0 && e >= BN)) {
@@ -497,13 +499,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         l2[i & 1] = add2(l2[i & 1], pair(p0, p1));  // fp32 probabilities feed the row's sum, fp16 ones P V
         pk[i] = pack_half2(p0, p1);
       }
-      // the probabilities over the scores
+      // (P V of two blocks ago has read the buffer: s_full says so as well)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) tmem_st16(trow + s_col + BN * sb + 16 * i, pk + 16 * i);
+      for (int i = 0; i < 2; ++i) tmem_st16(trow + p_col + 32 * (j & 1) + 16 * i, pk + 16 * i);
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        // O is stable once P V of the block before has completed (that of the one before that has: S_j was
-        // issued behind it, so the parity is this phase's)
-        if (!__all_sync(0xffffffffu, wait_b(&o_done[t], (j - 1) & 1, abort_v, P.err))) {
+        // O is stable once P V of the block before has completed
+        if (!__all_sync(0xffffffffu, wait_b(&kv_empty[(j - 1) % NKV], ((j - 1) / NKV) & 1, abort_v, P.err))) {
           failed = true;
           break;
         }
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_plain(&p_full[2 * t + sb]);
+      if (lane == 0) mbar_arrive_plain(&p_full[2 * t + (j & 1)]);
     }
     // ---- epilogue: O row / l
     if (!failed && nblk > 0) {
@@ -535,39 +536,45 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     const float l = (s0 + s1) + (s2 + s3);
     const float nan = __uint_as_float(0x7FC00000u);
     const float inv = failed ? nan : l == 0.f ? 0.f : P.v_scale / l;
-    const int64_t o_at = row * P.o_st + head * P.o_sh;
+    // by way of the Q tile, which no MMA reads any more, so that a half-warp writes a row's 256 bytes at once
+    __syncwarp();
 #pragma unroll 1
-    for (int c = 0; c < D / 16; ++c) {
-      uint32_t o[16];
+    for (int d0 = 0; d0 < D; d0 += 64) {
+      float o[64];
       if (nblk > 0 && !failed) {
-        tmem_ld16_async(trow + o_col + 16 * c, o);
-        tmem_wait_ld16(o);
+        tmem_ld64(trow + o_col + d0, reinterpret_cast<uint32_t*>(o));
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = 0u;
+        for (int i = 0; i < 64; ++i) o[i] = 0.f;
       }
-      if (valid) {
-        const float f16 = (nan_blocks >> c) & 1 ? nan : inv;
-        float f[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = l == 0.f && !failed && f16 == 0.f ? 0.f : __uint_as_float(o[i]) * f16;
-        if (P.o_bf16) {
-          __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(P.out) + o_at + 16 * c;
-          *reinterpret_cast<uint4*>(op) = pack8<__nv_bfloat16>(f);
-          *reinterpret_cast<uint4*>(op + 8) = pack8<__nv_bfloat16>(f + 8);
-        } else {
-          __half* op = reinterpret_cast<__half*>(P.out) + o_at + 16 * c;
-          *reinterpret_cast<uint4*>(op) = pack8<__half>(f);
-          *reinterpret_cast<uint4*>(op + 8) = pack8<__half>(f + 8);
-        }
+      for (int c = 0; c < 4; ++c) {
+        const float by = (nan_blocks >> (d0 / 16 + c)) & 1 ? nan : inv;
+        float* f = o + 16 * c;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = by == 0.f ? 0.f : f[i] * by;  // (no key: O holds nothing)
+        uint8_t* dst = rows + lane * 128 + (d0 / 64) * 16384;
+        const int c0 = (2 * c) ^ (lane & 7);
+        *reinterpret_cast<uint4*>(dst + (c0 << 4)) = P.o_bf16 ? pack8<__nv_bfloat16>(f) : pack8<__half>(f);
+        *reinterpret_cast<uint4*>(dst + ((c0 ^ 1) << 4)) = P.o_bf16 ? pack8<__nv_bfloat16>(f + 8) : pack8<__half>(f + 8);
       }
+    }
+    __syncwarp();
+    const int64_t mine = row * P.o_st + head * P.o_sh;
+    const int c = lane & 15, half = lane >> 4;
+#pragma unroll 8
+    for (int i = 0; i < 16; ++i) {
+      const int r = 2 * i + half;
+      const int64_t at = __shfl_sync(0xffffffffu, mine, r);
+      const uint4 v = *reinterpret_cast<const uint4*>(rows + r * 128 + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
+      if ((there >> r) & 1u) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(P.out) + at + 8 * c) = v;
     }
   }
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
+  if (warp == 0) tmem_dealloc(tmem, TMEM_COLS);
 }
 
 }  // namespace pf4

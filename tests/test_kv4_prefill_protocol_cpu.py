@@ -2,15 +2,15 @@
 
 Roles are generators that yield (barrier, parity) to wait; barriers count arrivals like mbarriers, and a wait by
 parity succeeds exactly when the current phase has the other parity (so one that is two phases late hangs, and one
-whose phase before has not completed passes too early: both show).  MMAs complete at random times, S before an earlier P V as well.
+whose phase before has not completed passes too early: both show).  MMAs complete at random times, those of the two issuers in any order.
 Checked: no deadlock; every MMA reads the block it means; no buffer is overwritten before its reader is
-done; O is rescaled only between P V of the blocks around it; the end reads O complete.  Three planted mistakes
+done; O is rescaled only between P V of the blocks around it; the end reads O complete.  Four planted mistakes
 are caught."""
 import random
 
 import pytest
 
-NSTG, NKV = 4, 3
+NKV = 3
 
 
 class Barrier:
@@ -38,105 +38,99 @@ def check(ok, what):
 
 def simulate(nblk, seed, plant=None, rescale=0.3):
     r = random.Random(seed)
-    B = dict(e_full=[Barrier(1) for _ in range(NSTG)], e_empty=[Barrier(4) for _ in range(NSTG)],
-             kv_full=[Barrier(4) for _ in range(NKV)], kv_empty=[Barrier(1) for _ in range(NKV)],
-             s_full=[[Barrier(2), Barrier(2)] for _ in range(2)], p_full=[[Barrier(4), Barrier(4)] for _ in range(2)],
-             o_done=[Barrier(1), Barrier(1)], o_last=[Barrier(1), Barrier(1)], q_ready=Barrier(8))
-    stage, conv, slot = [None] * NSTG, [[None] * 4 for _ in range(NKV)], [None] * NKV
-    sbuf = [[None, None], [None, None]]      # ("S" | "P", block), P a count of warps
+    B = dict(kv_empty=[Barrier(1) for _ in range(NKV)], s_go=[[Barrier(8) for _ in range(NKV)] for _ in range(2)],
+             s_full=[[Barrier(3), Barrier(3)] for _ in range(2)], p_full=[[Barrier(4), Barrier(4)] for _ in range(2)],
+             o_last=[Barrier(1), Barrier(1)])
+    conv = [[None] * 4 for _ in range(NKV)]
+    sbuf = [None, None]                      # block of a tile's scores
+    read = [[-1] * 4 for _ in range(2)]      # last block that a warp has in registers
+    pbuf = [[[None] * 4, [None] * 4] for _ in range(2)]  # block of a warp's probabilities
     o_pv = [-1, -1]                          # last P V completed
-    queue = []                               # MMAs and commits, in order
-
-    def producer():
-        for j in range(nblk):
-            s = j % NSTG
-            if j >= NSTG:
-                yield B["e_empty"][s], ((j // NSTG) - 1) & 1
-            stage[s] = j
-            B["e_full"][s].arrive()
+    queues = [], []                          # MMAs and commits of the two issuers, each in order
 
     def converter(w):
         for j in range(nblk):
-            s, kb = j % NSTG, j % NKV
-            yield B["e_full"][s], (j // NSTG) & 1
+            kb = j % NKV
             if j >= NKV and plant != "kv_empty":
                 yield B["kv_empty"][kb], ((j // NKV) - 1) & 1
-            check(stage[s] == j, "staging overwritten")
-            check(not any(kind in ("S", "PV") and k % NKV == kb and k != j for kind, _, k in queue if kind != "commit"),
+            check(not any(kind in ("S", "PV") and k % NKV == kb and k != j for kind, _, k in queues[0] + queues[1]
+                      if kind != "commit"),
                   "operands overwritten under an MMA")
             conv[kb][w] = j
             yield None
-            B["kv_full"][kb].arrive()
-            B["e_empty"][s].arrive()
+            B["s_go"][0][kb].arrive()
+            B["s_go"][1][kb].arrive()
 
-    def issuer():
-        def s_of(j):
+    def issuer_s():
+        for j in range(nblk):
             for t in range(2):
-                queue.append(("S", t, j))
-                queue.append(("commit", B["s_full"][t][j & 1], None))
+                yield B["s_go"][t][j % NKV], (j // NKV) & 1
+                queues[0].append(("S", t, j))
+                queues[0].append(("commit", B["s_full"][t][j & 1], None))
                 B["s_full"][t][j & 1].arrive()
 
-        yield B["q_ready"], 0
-        yield B["kv_full"][0], 0
-        s_of(0)
+    def issuer_pv():
+        for t in range(2):
+            B["s_full"][t][0].arrive()
+            B["s_full"][t][1].arrive()
+        yield None
         for j in range(nblk):
-            if j + 1 < nblk:
-                yield B["kv_full"][(j + 1) % NKV], ((j + 1) // NKV) & 1
-                if j > 0 and plant != "issuer":
-                    yield B["o_done"][0], (j - 1) & 1
-                    yield B["o_done"][1], (j - 1) & 1
-                s_of(j + 1)
             for t in range(2):
                 yield B["p_full"][t][j & 1], (j >> 1) & 1
-                queue.append(("PV", t, j))
-                queue.append(("commit", B["o_done"][t], None))
+                if plant == "p_read":
+                    B["s_full"][t][j & 1].arrive()
+                queues[1].append(("PV", t, j))
                 if j + 1 == nblk:
-                    queue.append(("commit", B["o_last"][t], None))
-            queue.append(("commit", B["kv_empty"][j % NKV], None))
+                    queues[1].append(("commit", B["o_last"][t], None))
+                elif plant != "p_read":
+                    queues[1].append(("commit", B["s_full"][t][j & 1], None))
+            queues[1].append(("commit", B["kv_empty"][j % NKV], None))
 
     def softmax(t, w):
-        B["q_ready"].arrive()
+        B["s_go"][t][0].arrive()
         for j in range(nblk):
             yield B["s_full"][t][j & 1], (j >> 1) & 1
-            check(sbuf[t][j & 1] in (("S", j), ("P", j)), "scores of another block")
+            check(sbuf[t] == j, "scores of another block")
             check(conv[j % NKV] == [j] * 4, "flags of another block")
+            if plant != "s_read":
+                read[t][w] = j
+            B["s_go"][t][(j + 1) % NKV].arrive()
             yield None
-            sbuf[t][j & 1] = ("P", j)
+            read[t][w] = j
+            check(conv[j % NKV] == [j] * 4, "flags of another block")
+            check(j < 2 or o_pv[t] >= j - 2, "probabilities written over those that P V has yet to read")
+            pbuf[t][j & 1][w] = j
             if j > 0 and r.random() < rescale:
-                yield B["o_done"][t], (j - 1) & 1
+                yield B["kv_empty"][(j - 1) % NKV], ((j - 1) // NKV) & 1
                 check(o_pv[t] == j - 1, "O rescaled while P V runs")
             yield None
             B["p_full"][t][j & 1].arrive()
         if plant == "end":
-            yield B["o_done"][t], (nblk - 1) & 1
+            yield B["kv_empty"][(nblk - 2) % NKV], (max(nblk - 2, 0) // NKV) & 1
         else:
             yield B["o_last"][t], 0
         check(o_pv[t] == nblk - 1, "O read before the last P V")
 
     def tensor():
         while True:
+            # (the order of the two issuers' MMAs is not promised; a commit waits for its own issuer's)
+            queue = r.choice(queues)
             if queue and r.random() < 0.7:
-                # (the order of MMAs of different shapes is not promised: an S may pass P V before it)
-                at = 0
-                if r.random() < 0.3:
-                    at = next((i for i, q in enumerate(queue) if q[0] == "S"), 0)
-                kind, t, j = queue[at]
+                kind, t, j = queue.pop(0)
                 if kind == "commit":
                     t.arrive()
                 elif kind == "S":
                     check(conv[j % NKV] == [j] * 4, "S of another block's keys")
-                    check(sbuf[t][j & 1] is None or sbuf[t][j & 1] == ("P", j - 2), "S over scores in use")
-                    check(o_pv[t] >= j - 2, "S over probabilities that P V has yet to read")
-                    sbuf[t][j & 1] = ("S", j)
+                    check(read[t] == [j - 1] * 4, "S over scores in use")
+                    sbuf[t] = j
                 else:
                     check(conv[j % NKV] == [j] * 4, "P V of another block's values")
-                    check(sbuf[t][j & 1] == ("P", j), "P V of another block's probabilities")
+                    check(pbuf[t][j & 1] == [j] * 4, "P V of another block's probabilities")
                     check(o_pv[t] == j - 1, "P V out of order")
                     o_pv[t] = j
-                queue.pop(at)
             yield None
 
-    roles = {"producer": producer(), "issuer": issuer()}
+    roles = {"issuer_s": issuer_s(), "issuer_pv": issuer_pv()}
     roles |= {f"conv{w}": converter(w) for w in range(4)}
     roles |= {f"soft{t}{w}": softmax(t, w) for t in range(2) for w in range(4)}
     machine = tensor()
@@ -144,7 +138,7 @@ def simulate(nblk, seed, plant=None, rescale=0.3):
     idle = 0
     while roles:
         next(machine)
-        moved = bool(queue)
+        moved = any(queues)
         for k in r.sample(list(roles), len(roles)):
             w = waits[k]
             if w is not None and not w[0].done(w[1]):
@@ -169,7 +163,7 @@ def test_random_schedules(nblk):
         simulate(nblk, seed, rescale=1.0)
 
 
-@pytest.mark.parametrize("plant,nblk", [("end", 2), ("issuer", 6), ("kv_empty", 9)])
+@pytest.mark.parametrize("plant,nblk", [("end", 3), ("s_read", 6), ("kv_empty", 9), ("p_read", 9)])
 def test_planted_mistakes_are_caught(plant, nblk):
     caught = 0
     for seed in range(200):
