@@ -5,8 +5,12 @@
 // zeros.  Rows are (token, head) pairs of a KV head's group, head fastest, so 256 / group tokens
 // share every key block that a CTA widens.
 //
-// Bound by the exponentials and the tensor pipe alike: a block of 64 keys takes 256 x 64 of the former
-// (16 a cycle and SM: 1,024 cycles) and 2 x 256 x 64 x 128 multiply-adds (4,096 a cycle: 1,024).
+// Floor of a block of 64 keys: 256 x 64 exponentials (16 a cycle and SM: 1,024 cycles), 2 x 256 x 64 x 128
+// multiply-adds (4,096 a cycle: 1,024) and the operands' shared-memory reads (some 1,400).  It takes about 1,900: the
+// softmax of the two tiles' rows on one scheduler runs in step (its exponentials 1,300 cycles side by side, 850 alone) and
+// its loads, maxima and waits (600) come in between.  4 x 2,048 tokens behind 2,048, 32/8 heads: 423 us, 58% of
+// the measured matrix rate.  Tried and left out: two threads a row (524: they have to agree on the reference),
+// turns between the tiles (466), part of the exponentials as polynomials on the FMA pipe (426-454), 128 keys a block (564).
 //
 // One CTA a (256-row query block, KV head, sequence); 14 warps:
 //   warp 0        TMEM owner, issues S_t = Q_t K^T for the two 128-row tiles t (M 128, N 64);
@@ -23,18 +27,15 @@
 // the converters widen it as 0 and mark (key, scale block), and rows that see a marked key turn
 // their 16 elements to NaN at the end.
 //
-// Barriers (block j, tile t): kv_empty[j % NKV] (commit after both P V); s_go[t][j % NKV]: S_j
-// may run (4 converters; 4 softmax warps, which have S_{j-1} in registers, or Q in place for j = 0); s_full[t][j & 1] (commit
-// after S_j, an arrival of its issuer's own, commit after P V of j - 2); p_full[t][j & 1] (4 warps); o_last[t] (commit
-// after the last P V); fin.  Few waits, as each takes 150-300 cycles also where it passes.
-// The scores have one place a tile and the probabilities two: S_{j+1} is issued as soon as the softmax has S_j
-// in registers, and runs under its exponentials; P_j stays where it is until P V has read it.
+// Barriers (block j, tile t): kv_empty[j % NKV] (commit after both P V); s_go[t][j % NKV]: S_j may run (4 converters;
+// commit after P V of j - 2, whose probabilities lie in the same place); s_full[t][j & 1] (commit after S_j, an
+// arrival of its issuer's own); p_full[t][j & 1] (4 warps); o_last[t] (commit after the last P V); q_ready (8
+// warps); fin.  Few waits, as each takes 150-300 cycles also where it passes.
 // A wait by parity needs the phase before to be known complete and the next one not begun.  Refills wait
-// for the release of the use before, in every phase.  An arrival for the next phase of s_go[t][j % NKV] follows kv_empty of j
-// or S_{j+2}; one for the next of s_full[t][j & 1] is P V of j, behind p_full of j, which follows this phase, or S_{j+2}, behind
-// the read of S_{j+1}; p_full of j + 2 needs s_full of j + 2 and so P V of j.  A softmax that rescales O waits
-// for P V of j - 1 by kv_empty, whose phase before the converters of block j - 1 have seen.  The end waits for o_last,
-// which has one phase.
+// for the release of the use before, in every phase.  An arrival for the next phase of s_go[t][j % NKV] follows kv_empty of
+// j or P V of j + 1; S_{j+2} and with it the next phases of s_full and p_full follow P V of j.  A softmax that
+// rescales O waits for P V of j - 1 by kv_empty, whose phase before the converters of block j - 1 have seen.
+// The end waits for o_last, which has one phase.
 #include "kv4.cuh"
 #include "tc_attention.cuh"
 
@@ -54,13 +55,12 @@ constexpr int E_OFF = V_OFF + NKV * 16384;   // converter warps' rings: K codes,
 constexpr int E_BYTES = 2 * TILE * ROW_BYTES;
 constexpr int EV = TILE * ROW, EKS = 2 * TILE * ROW, EVS = EKS + TILE * SROW;
 constexpr int BAR_OFF = E_OFF + NCONV * NSTG * E_BYTES;
-constexpr int NBAR = NKV + NT * (NKV + 5) + NT * NSOFT + 1;
+constexpr int NBAR = NKV + NT * (NKV + 5) + 2;
 constexpr int FLAG_OFF = (BAR_OFF + NBAR * 8 + 15) & ~15;  // words a K/V slot: [4 tiles there][4 tiles' NaN flags][16 NaN masks]
 constexpr int SLOT_WORDS = 24;
 constexpr int SMEM = 1024 + FLAG_OFF + (NKV * SLOT_WORDS + 4) * 4;
 static_assert(NCONV * TILE == BN, "a converter warp a tile");
-// O of tile t at 128 t; its S at 256 + 128 t, its P buffer b (f16, two a column) 64 + 32 b behind
-constexpr uint32_t TMEM_COLS = 512, S_COL = 256, P_COL = BN;
+constexpr uint32_t TMEM_COLS = 512, S_COL = 256;  // O of tile t at 128 t; S buffer b of tile t at 256 + 128 t + 64 b
 constexpr float MOVE_LOG2 = 8.f;
 static_assert(SMEM <= 232448, "shared memory per CTA");
 static_assert(E_BYTES % 16 == 0 && BAR_OFF % 16 == 0 && FLAG_OFF % 16 == 0 && SLOT_WORDS % 4 == 0, "alignment");
@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
   uint64_t* s_full = s_go + NT * NKV;   // [NT][2]
   uint64_t* p_full = s_full + 2 * NT;   // [NT][2]
   uint64_t* o_last = p_full + 2 * NT;   // [NT]
-  uint64_t* q_raw = o_last + NT;        // [NT][NSOFT]
-  uint64_t* fin = q_raw + NT * NSOFT;
+  uint64_t* q_ready = o_last + NT;
+  uint64_t* fin = q_ready + 1;
   uint32_t* slots = reinterpret_cast<uint32_t*>(base + FLAG_OFF);
   uint32_t* tmem_slot = slots + NKV * SLOT_WORDS;
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
@@ -163,13 +163,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NKV; ++i) mbar_init(&kv_empty[i], 1);
-    for (int i = 0; i < NT * NKV; ++i) mbar_init(&s_go[i], NCONV + NSOFT);
+    for (int i = 0; i < NT * NKV; ++i) mbar_init(&s_go[i], NCONV + 1);
     for (int i = 0; i < 2 * NT; ++i) {
-      mbar_init(&s_full[i], 3);
+      mbar_init(&s_full[i], 2);
       mbar_init(&p_full[i], NSOFT);
     }
     for (int t = 0; t < NT; ++t) mbar_init(&o_last[t], 1);
-    for (int i = 0; i < NT * NSOFT; ++i) mbar_init(&q_raw[i], 1);
+    mbar_init(q_ready, NT * NSOFT);
     mbar_init(fin, 2);
     *abort_flag = 0;
     fence_mbar_init();
@@ -214,14 +214,22 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       uint32_t slot = 0;
       bool ok = true;
       if (warp == 0) {
-        for (int j = 0; ok && j < nblk; ++j) {
+        ok = wait_b(q_ready, 0, abort_v, P.err);
+        if (leader) {  // the first two places of each tile's scores are free
+          for (int t = 0; t < NT; ++t) {
+            mbar_arrive_plain(&s_go[NKV * t]);
+            mbar_arrive_plain(&s_go[NKV * t + 1]);
+          }
+        }
+        __syncwarp();
+        for (int j = 0; j < nblk; ++j) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             ok = __all_sync(0xffffffffu, ok && wait_b(&s_go[NKV * t + slot], (j / NKV) & 1, abort_v, P.err));
             if (!ok) break;
             tc_fence_after();
             if (leader) {
-              const uint32_t d = tm + S_COL + 128u * (uint32_t)t;
+              const uint32_t d = tm + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
 #pragma unroll
               for (int kk = 0; kk < D / 16; ++kk)
                 mma_ss(d, q_lo + (uint32_t)t * 2048u + (uint32_t)(kk / 4) * 1024u + (uint32_t)(kk % 4) * 2u,
@@ -231,13 +239,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             }
             __syncwarp();
           }
+          if (!ok) break;
           slot = slot + 1 == NKV ? 0 : slot + 1;
         }
       } else {
-        if (leader) {  // the probabilities' places are free
-          for (int i = 0; i < 2 * NT; ++i) mbar_arrive_plain(&s_full[i]);
-        }
-        __syncwarp();
         for (int j = 0; ok && j < nblk; ++j) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -245,12 +250,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             if (!ok) break;
             tc_fence_after();
             if (leader) {
-              const uint32_t p = tm + S_COL + 128u * (uint32_t)t + P_COL + 32u * (uint32_t)(j & 1);
+              const uint32_t p = tm + S_COL + 128u * (uint32_t)t + BN * (uint32_t)(j & 1);
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)
                 mma_ts(tm + 128u * (uint32_t)t, p + 8u * (uint32_t)kk, v_lo + slot * 1024u + (uint32_t)kk * 128u,
                        j > 0 || kk > 0);
-              tc_commit(j + 1 == nblk ? &o_last[t] : &s_full[2 * t + (j & 1)]);  // (P_{j+2} may come)
+              tc_commit(j + 1 == nblk ? &o_last[t] : &s_go[NKV * t + (slot + 2) % NKV]);  // (S_{j+2} may come)
               if (t == NT - 1) tc_commit(&kv_empty[slot]);
             }
             __syncwarp();
@@ -322,29 +327,42 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       const bool ok = (there >> from) & 1u;
       uint32_t* flags = slots + kb * SLOT_WORDS;
       uint32_t nan_any = 0;
-      // 16 keys x 8 blocks of 16 elements an operand: 4 units a lane
+      // 16 keys x 8 blocks of 16 elements an operand: 4 units a lane, two read before the first is written (the compiler
+      // cannot move a read over a write that may be to the same place; 1, 2, 4 at a time: 433, 423, 436 us)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int unit = lane + 32 * u, key = TILE * w + (unit >> 3), blk = unit & 7;
-        const bool vok = ok & (kb0 + j * BN + key < len_k);
-        const uint2 k8 = *reinterpret_cast<const uint2*>(st + 8 * unit);
-        const uint2 v8 = *reinterpret_cast<const uint2*>(st + EV + 8 * unit);
-        const uint32_t ks = ok ? st[EKS + unit] : 0u;
-        uint32_t vs = vok ? st[EVS + unit] : 0u;
-        const bool nan = (vs & 0x7Fu) == 0x7Fu;
-        const uint32_t marked = __ballot_sync(0xffffffffu, nan);  // 4 keys x 8 blocks
-        if (nan) vs = 0;
-        nan_any |= marked;
-        if (lane == 0) flags[8 + 4 * w + u] = marked;
-        uint4 lo, hi;
-        const int c0 = ((blk & 3) * 2) ^ (key & 7), c1 = c0 ^ 1;
-        const int at = kb * 16384 + (blk >> 2) * 8192 + key * 128;
-        widen16(k8, scale_f16x2(ks), lo, hi);
-        *reinterpret_cast<uint4*>(kf + at + (c0 << 4)) = lo;
-        *reinterpret_cast<uint4*>(kf + at + (c1 << 4)) = hi;
-        widen16(v8, scale_f16x2(vs), lo, hi);
-        *reinterpret_cast<uint4*>(vf + at + (c0 << 4)) = lo;
-        *reinterpret_cast<uint4*>(vf + at + (c1 << 4)) = hi;
+      for (int u0 = 0; u0 < 4; u0 += 2) {
+        uint2 k8[2], v8[2];
+        uint32_t ks[2], vs[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int unit = lane + 32 * (u0 + i);
+          k8[i] = *reinterpret_cast<const uint2*>(st + 8 * unit);
+          v8[i] = *reinterpret_cast<const uint2*>(st + EV + 8 * unit);
+          ks[i] = st[EKS + unit];
+          vs[i] = st[EVS + unit];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int u = u0 + i, unit = lane + 32 * u, key = TILE * w + (unit >> 3), blk = unit & 7;
+          if (!ok) ks[i] = 0;
+          if (!ok || kb0 + j * BN + key >= len_k) vs[i] = 0;
+          const bool nan = (vs[i] & 0x7Fu) == 0x7Fu;
+          const uint32_t marked = __ballot_sync(0xffffffffu, nan);  // 4 keys x 8 blocks
+          if (nan) vs[i] = 0;
+          nan_any |= marked;
+          if (lane == 0) flags[8 + 4 * w + u] = marked;
+          uint4 lo, hi;
+          // (blocks 4-7 lie 8 KB behind 0-3, in the same banks: they write their halves in the other order)
+          const int c0 = ((blk & 3) * 2 + (blk >> 2)) ^ (key & 7), c1 = c0 ^ 1;
+          if (blk & 4) k8[i] = make_uint2(k8[i].y, k8[i].x), v8[i] = make_uint2(v8[i].y, v8[i].x);
+          const int at = kb * 16384 + (blk >> 2) * 8192 + key * 128;
+          widen16(k8[i], scale_f16x2(ks[i]), lo, hi);
+          *reinterpret_cast<uint4*>(kf + at + (c0 << 4)) = lo;
+          *reinterpret_cast<uint4*>(kf + at + (c1 << 4)) = hi;
+          widen16(v8[i], scale_f16x2(vs[i]), lo, hi);
+          *reinterpret_cast<uint4*>(vf + at + (c0 << 4)) = lo;
+          *reinterpret_cast<uint4*>(vf + at + (c1 << 4)) = hi;
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -363,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     const int q4 = warp & 3;  // the TMEM lane quarter that this warp may access
     const int r = 32 * q4 + lane, R = t * BM + r;
     const uint32_t trow = tmem + ((uint32_t)(32 * q4) << 16);
-    const uint32_t o_col = 128u * (uint32_t)t, s_col = S_COL + 128u * (uint32_t)t, p_col = s_col + P_COL;
+    const uint32_t o_col = 128u * (uint32_t)t, s_col = S_COL + 128u * (uint32_t)t;
     const int tok = t0 + R / P.group;
     const int64_t row = q_begin + tok;
     const bool valid = active && R < P.qt * P.group && tok < len_q && row >= 0 && row < P.rows;
@@ -373,59 +391,50 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     if (valid) key_range(P, tok, off, len_k, lo, hi);
     float factor = 0.f;
     uint8_t* rows = qs + t * 32768 + 4096 * q4;  // the warp's 32 rows of the Q tile, [2 halves at 16 KB]
+    const int c16 = lane & 15, r2 = lane >> 4;   // a half-warp a row
+    auto chunk = [&](int rr, int c) {
+      return reinterpret_cast<uint4*>(rows + rr * 128 + (c >> 3) * 16384 + (((c & 7) ^ (rr & 7)) << 4));
+    };
     if (nblk > 0) {
-      // The query rows -> f16, times a power of two.  They arrive by bulk copies, each half in its place, and are
-      // converted there: the L1 beside this much shared memory holds some 16 KB of loads under way, four
-      // round trips for 64 KB of rows (16,000 cycles a CTA instead of XXXX).
-      if (lane == 0) mbar_arrive_expect_tx(&q_raw[t * NSOFT + q4], __popc(there) * 256u);
-      __syncwarp();
-      if (valid) {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(P.q) + row * P.q_st + head * P.q_sh;
-        bulk_load(rows + lane * 128, src, 128, &q_raw[t * NSOFT + q4]);
-        bulk_load(rows + lane * 128 + 16384, src + 64, 128, &q_raw[t * NSOFT + q4]);
+      // The query rows -> f16, times a power of two, in place: elements come by cp.async to where their f16 form
+      // will lie, so that a thread reads and writes its row without bank conflicts.  (By loads into registers the L1
+      // beside this much shared memory, some 16 KB, holds a quarter of them at a time: 16,000 cycles a CTA, here 9,000.)
+      const int64_t mine = row * P.q_st + head * P.q_sh;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int rr = 2 * i + r2;
+        const int64_t at = __shfl_sync(0xffffffffu, mine, rr);
+        if ((there >> rr) & 1u) cp16(smem_u32(chunk(rr, c16)), reinterpret_cast<const uint16_t*>(P.q) + at + 8 * c16);
       }
-      const bool got = __all_sync(0xffffffffu, wait_b(&q_raw[t * NSOFT + q4], 0, abort_v, P.err));
-      const int c = lane & 15, half = lane >> 4;
-      int ex = 0;
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += 8) {  // a half-warp a row, four rows side by side
-        uint4 raw[4];
-        float top[4];
+      cp_commit();
+      cp_wait<0>();
+      __syncwarp();
+      float top = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < 16; ++c) {
+        uint4 x = *chunk(lane, c);
+        if (!valid) x = make_uint4(0, 0, 0, 0);
+        float f[8];
+        if (P.q_bf16) unpack8<__nv_bfloat16>(x, f); else unpack8<__half>(x, f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i0 + 2 * i + half;
-          raw[i] = *reinterpret_cast<const uint4*>(rows + r * 128 + (c >> 3) * 16384 + ((c & 7) << 4));
-          if (!got || !((there >> r) & 1u)) raw[i] = make_uint4(0, 0, 0, 0);
-          float f[8];
-          if (P.q_bf16) unpack8<__nv_bfloat16>(raw[i], f); else unpack8<__half>(raw[i], f);
-          top[i] = fabsf(f[0]);
-#pragma unroll
-          for (int k = 1; k < 8; ++k) top[i] = max_nan(top[i], fabsf(f[k]));
-        }
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i0 + 2 * i + half, e = query_exponent(top[i]);
-          const int theirs = __shfl_sync(0xffffffffu, e, 16 * (lane & 1));
-          if ((lane >> 1) == i0 / 2 + i) ex = theirs;
-          const float mul = pow2(e);
-          float f[8];
-          if (P.q_bf16) unpack8<__nv_bfloat16>(raw[i], f); else unpack8<__half>(raw[i], f);
-          *reinterpret_cast<uint4*>(rows + r * 128 + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) =
-              make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
-                         pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
-        }
+        for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(f[i]));
+      }
+      const int ex = query_exponent(top);
+      const float mul = pow2(ex);
+#pragma unroll 4
+      for (int c = 0; c < 16; ++c) {
+        uint4 x = *chunk(lane, c);
+        if (!valid) x = make_uint4(0, 0, 0, 0);
+        float f[8];
+        if (P.q_bf16) unpack8<__nv_bfloat16>(x, f); else unpack8<__half>(x, f);
+        *chunk(lane, c) = make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
+                                     pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
       }
       factor = score_factor(P.scale_log2, ex);
       if (!valid) factor = fminf(factor, SAFE_FACTOR);  // (all its keys are masked)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive_plain(&s_go[NKV * t]);
+      if (lane == 0) mbar_arrive_plain(q_ready);
     }
     const bool safe = __all_sync(0xffffffffu, factor <= SAFE_FACTOR);
     float m = -INFINITY;  // largest score that set the reference
@@ -442,10 +451,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       tc_fence_after();
       float x[64];
       uint32_t* sr = reinterpret_cast<uint32_t*>(x);
-      tmem_ld64(trow + s_col, sr);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_plain(&s_go[NKV * t + (j + 1) % NKV]);
+      tmem_ld64(trow + s_col + BN * (j & 1), sr);
       const uint32_t* flags = slots + (j % NKV) * SLOT_WORDS;
       const uint4 loaded = *reinterpret_cast<const uint4*>(flags);
       const uint32_t blk_ok = loaded.x | (loaded.y << 1) | (loaded.z << 2) | (loaded.w << 3);
@@ -499,9 +505,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         l2[i & 1] = add2(l2[i & 1], pair(p0, p1));  // fp32 probabilities feed the row's sum, fp16 ones P V
         pk[i] = pack_half2(p0, p1);
       }
-      // (P V of two blocks ago has read the buffer: s_full says so as well)
+      // the probabilities over the scores
 #pragma unroll
-      for (int i = 0; i < 2; ++i) tmem_st16(trow + p_col + 32 * (j & 1) + 16 * i, pk + 16 * i);
+      for (int i = 0; i < 2; ++i) tmem_st16(trow + s_col + BN * (j & 1) + 16 * i, pk + 16 * i);
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
         // O is stable once P V of the block before has completed
         if (!__all_sync(0xffffffffu, wait_b(&kv_empty[(j - 1) % NKV], ((j - 1) / NKV) & 1, abort_v, P.err))) {
@@ -553,21 +559,18 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         float* f = o + 16 * c;
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = by == 0.f ? 0.f : f[i] * by;  // (no key: O holds nothing)
-        uint8_t* dst = rows + lane * 128 + (d0 / 64) * 16384;
-        const int c0 = (2 * c) ^ (lane & 7);
-        *reinterpret_cast<uint4*>(dst + (c0 << 4)) = P.o_bf16 ? pack8<__nv_bfloat16>(f) : pack8<__half>(f);
-        *reinterpret_cast<uint4*>(dst + ((c0 ^ 1) << 4)) = P.o_bf16 ? pack8<__nv_bfloat16>(f + 8) : pack8<__half>(f + 8);
+        *chunk(lane, d0 / 8 + 2 * c) = P.o_bf16 ? pack8<__nv_bfloat16>(f) : pack8<__half>(f);
+        *chunk(lane, d0 / 8 + 2 * c + 1) = P.o_bf16 ? pack8<__nv_bfloat16>(f + 8) : pack8<__half>(f + 8);
       }
     }
     __syncwarp();
     const int64_t mine = row * P.o_st + head * P.o_sh;
-    const int c = lane & 15, half = lane >> 4;
 #pragma unroll 8
     for (int i = 0; i < 16; ++i) {
-      const int r = 2 * i + half;
-      const int64_t at = __shfl_sync(0xffffffffu, mine, r);
-      const uint4 v = *reinterpret_cast<const uint4*>(rows + r * 128 + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
-      if ((there >> r) & 1u) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(P.out) + at + 8 * c) = v;
+      const int rr = 2 * i + r2;
+      const int64_t at = __shfl_sync(0xffffffffu, mine, rr);
+      const uint4 v = *chunk(rr, c16);
+      if ((there >> rr) & 1u) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(P.out) + at + 8 * c16) = v;
     }
   }
 
