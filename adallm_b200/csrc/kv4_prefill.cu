@@ -12,7 +12,8 @@
 // the measured matrix rate.  Tried and left out: two threads a row (524: they have to agree on the reference),
 // turns between the tiles (466), part of the exponentials as polynomials on the FMA pipe (426-454), 128 keys a block (564).
 //
-// One CTA a (256-row query block, KV head, sequence); 14 warps:
+// One CTA a (256-row query block, KV head, sequence), or several that share its keys where there are few
+// (merge_kernel joins them); 14 warps:
 //   warp 0        TMEM owner, issues S_t = Q_t K^T for the two 128-row tiles t (M 128, N 64);
 //   warp 1        issues O_t += P_t V with P_t as the A operand in TMEM;
 //   warps 2-5     converters: a 16-key tile of each block each (in one page): its codes and scales by cp.async
@@ -62,6 +63,8 @@ constexpr int SMEM = 1024 + FLAG_OFF + (NKV * SLOT_WORDS + 4) * 4;
 static_assert(NCONV * TILE == BN, "a converter warp a tile");
 constexpr uint32_t TMEM_COLS = 512, S_COL = 256;  // O of tile t at 128 t; S buffer b of tile t at 256 + 128 t + 64 b
 constexpr float MOVE_LOG2 = 8.f;
+// A partial (floats): O as [32 groups of 4 elements][256 rows][4], then (largest score, sum, factor, -) a row.
+constexpr int ROWS = NT * BM, STATS = ROWS * D, PART = STATS + 4 * ROWS;
 static_assert(SMEM <= 232448, "shared memory per CTA");
 static_assert(E_BYTES % 16 == 0 && BAR_OFF % 16 == 0 && FLAG_OFF % 16 == 0 && SLOT_WORDS % 4 == 0, "alignment");
 constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
@@ -83,6 +86,8 @@ struct Params {
   int64_t rows;
   float scale_log2, v_scale;
   unsigned* err;
+  int qblocks, splits;  // CTAs that share a query block's keys
+  float* parts;         // workspace (splits > 1): a partial a CTA
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -144,7 +149,11 @@ __device__ __forceinline__ void key_range(const Params& P, int t, int off, int l
 __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_constant__ Params P) {
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kvh = blockIdx.x, b = blockIdx.y;
-  const int qblk = gridDim.z - 1 - blockIdx.z;  // the longest causal rows of all heads and sequences first
+  int qblk = P.qblocks - 1 - blockIdx.z, split = 0;  // the longest causal rows of all heads and sequences first
+  if (P.splits > 1) {
+    qblk = P.qblocks - 1 - blockIdx.z / P.splits;
+    split = blockIdx.z % P.splits;
+  }
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -197,6 +206,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     k_end = min(k_hi, P.max_pages * P.page);
     kb0 = (k_lo / BN) * BN;
     nblk = k_end > k_lo ? (k_end - kb0 + BN - 1) / BN : 0;
+    if (P.splits > 1) {  // (2^24 blocks x 148: below 2^32)
+      const unsigned n = nblk, first = n * split / P.splits;
+      nblk = (int)(n * (split + 1) / P.splits - first);
+      kb0 += (int)first * BN;
+    }
   }
 
   if (warp < 2) {  // ---------------- MMA issuers: S, P V ----------------
@@ -539,38 +553,57 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     float s0, s1, s2, s3;
     unpair(l2[0], s0, s1);
     unpair(l2[1], s2, s3);
-    const float l = (s0 + s1) + (s2 + s3);
+    float l = (s0 + s1) + (s2 + s3);
     const float nan = __uint_as_float(0x7FC00000u);
     const float inv = failed ? nan : l == 0.f ? 0.f : P.v_scale / l;
-    // by way of the Q tile, which no MMA reads any more, so that a half-warp writes a row's 256 bytes at once
-    __syncwarp();
-#pragma unroll 1
-    for (int d0 = 0; d0 < D; d0 += 64) {
-      float o[64];
+    if (P.splits > 1) {  // to the workspace, unnormalised: lanes' 16 bytes side by side
+      if (failed) l = nan;
+      float* part = P.parts + ((((int64_t)b * gridDim.x + kvh) * P.qblocks + qblk) * P.splits + split) * PART;
+      reinterpret_cast<float4*>(part + STATS)[R] = make_float4(m, l, factor, 0.f);
       if (nblk > 0 && !failed) {
-        tmem_ld64(trow + o_col + d0, reinterpret_cast<uint32_t*>(o));
-      } else {
+#pragma unroll 1
+        for (int d0 = 0; d0 < D; d0 += 64) {
+          float o[64];
+          tmem_ld64(trow + o_col + d0, reinterpret_cast<uint32_t*>(o));
 #pragma unroll
-        for (int i = 0; i < 64; ++i) o[i] = 0.f;
+          for (int c = 0; c < 16; ++c) {
+            float4 v = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            if ((nan_blocks >> (d0 / 16 + c / 4)) & 1) v = make_float4(nan, nan, nan, nan);
+            reinterpret_cast<float4*>(part)[(d0 / 4 + c) * ROWS + R] = v;
+          }
+        }
       }
+    } else {
+      // by way of the Q tile, which no MMA reads any more, so that a half-warp writes a row's 256 bytes at once
+      __syncwarp();
+#pragma unroll 1
+      for (int d0 = 0; d0 < D; d0 += 64) {
+        float o[64];
+        if (nblk > 0 && !failed) {
+          tmem_ld64(trow + o_col + d0, reinterpret_cast<uint32_t*>(o));
+        } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float by = (nan_blocks >> (d0 / 16 + c)) & 1 ? nan : inv;
-        float* f = o + 16 * c;
+          for (int i = 0; i < 64; ++i) o[i] = 0.f;
+        }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = by == 0.f ? 0.f : f[i] * by;  // (no key: O holds nothing)
-        *chunk(lane, d0 / 8 + 2 * c) = P.o_bf16 ? pack8<__nv_bfloat16>(f) : pack8<__half>(f);
-        *chunk(lane, d0 / 8 + 2 * c + 1) = P.o_bf16 ? pack8<__nv_bfloat16>(f + 8) : pack8<__half>(f + 8);
+        for (int c = 0; c < 4; ++c) {
+          const float by = (nan_blocks >> (d0 / 16 + c)) & 1 ? nan : inv;
+          float* f = o + 16 * c;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) f[i] = by == 0.f ? 0.f : f[i] * by;  // (no key: O holds nothing)
+          *chunk(lane, d0 / 8 + 2 * c) = P.o_bf16 ? pack8<__nv_bfloat16>(f) : pack8<__half>(f);
+          *chunk(lane, d0 / 8 + 2 * c + 1) = P.o_bf16 ? pack8<__nv_bfloat16>(f + 8) : pack8<__half>(f + 8);
+        }
       }
-    }
-    __syncwarp();
-    const int64_t mine = row * P.o_st + head * P.o_sh;
+      __syncwarp();
+      const int64_t mine = row * P.o_st + head * P.o_sh;
 #pragma unroll 8
-    for (int i = 0; i < 16; ++i) {
-      const int rr = 2 * i + r2;
-      const int64_t at = __shfl_sync(0xffffffffu, mine, rr);
-      const uint4 v = *chunk(rr, c16);
-      if ((there >> rr) & 1u) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(P.out) + at + 8 * c16) = v;
+      for (int i = 0; i < 16; ++i) {
+        const int rr = 2 * i + r2;
+        const int64_t at = __shfl_sync(0xffffffffu, mine, rr);
+        const uint4 v = *chunk(rr, c16);
+        if ((there >> rr) & 1u) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(P.out) + at + 8 * c16) = v;
+      }
     }
   }
 
@@ -578,6 +611,46 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
   __syncthreads();
   tc_fence_after();
   if (warp == 0) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// Partials of the CTAs that share a query block: a CTA 32 rows (lane: row), a warp 16 elements of them.
+__global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Params P) {
+  pdl_wait();
+  pdl_trigger();
+  const int kvh = blockIdx.x, b = blockIdx.y, qblk = blockIdx.z / (ROWS / 32);
+  const int R = 32 * (blockIdx.z % (ROWS / 32)) + (threadIdx.x & 31), w = threadIdx.x >> 5;
+  const int64_t q_begin = P.cu_q[b];
+  const int len_q = (int)min(max((int64_t)P.cu_q[b + 1] - q_begin, (int64_t)0), (int64_t)1 << 30);
+  const int tok = qblk * P.qt + R / P.group, head = kvh * P.group + R % P.group;
+  const int64_t row = q_begin + tok;
+  if (R >= P.qt * P.group || tok >= len_q || row < 0 || row >= P.rows) return;
+  const float* part = P.parts + (((int64_t)b * gridDim.x + kvh) * P.qblocks + qblk) * P.splits * PART;
+  float top = -INFINITY;
+  for (int i = 0; i < P.splits; ++i) top = fmaxf(top, reinterpret_cast<const float4*>(part + i * PART + STATS)[R].x);
+  float l = 0.f, o[16];
+#pragma unroll
+  for (int c = 0; c < 16; ++c) o[c] = 0.f;
+  for (int i = 0; i < P.splits; ++i) {
+    const float* p = part + i * PART;
+    const float4 st = reinterpret_cast<const float4*>(p + STATS)[R];
+    if (st.y == 0.f) continue;  // saw no key (a NaN sum stays)
+    const float f = st.x == top ? 1.f : fast_exp2((st.x - top) * st.z);
+    l = fmaf(f, st.y, l);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float4 v = reinterpret_cast<const float4*>(p)[(4 * w + c) * ROWS + R];
+      o[4 * c] = fmaf(f, v.x, o[4 * c]);
+      o[4 * c + 1] = fmaf(f, v.y, o[4 * c + 1]);
+      o[4 * c + 2] = fmaf(f, v.z, o[4 * c + 2]);
+      o[4 * c + 3] = fmaf(f, v.w, o[4 * c + 3]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : P.v_scale / l;
+#pragma unroll
+  for (int c = 0; c < 16; ++c) o[c] = inv == 0.f ? 0.f : o[c] * inv;
+  uint16_t* out = reinterpret_cast<uint16_t*>(P.out) + row * P.o_st + head * P.o_sh + 16 * w;
+  reinterpret_cast<uint4*>(out)[0] = P.o_bf16 ? pack8<__nv_bfloat16>(o) : pack8<__half>(o);
+  reinterpret_cast<uint4*>(out)[1] = P.o_bf16 ? pack8<__nv_bfloat16>(o + 8) : pack8<__half>(o + 8);
 }
 
 }  // namespace pf4
@@ -602,6 +675,22 @@ static bool prefill_few(int64_t batch, int64_t most, int32_t num_heads, int32_t 
          items * (cdiv(keys, (int64_t)32) + 1) <= MOST;
 }
 
+// CTAs that a query block's keys are shared by: as many as are resident at once, each with four blocks of 64 keys or more
+// (a CTA costs 9 us around its blocks and the join 4-5; a row of new tokens sees half of them on average).  One
+// sequence, 32/8 heads, alone and shared: 60 tokens behind 700 keys 24.7 and 17.9 us, 100 behind 1,500: 44 and 23, 128
+// behind 8,000: 150 and 40, 512 behind 8,000: 157 and 90; 512 alone would take 20.3 instead of 18.0.  (Eight
+// blocks at least: 25.0 for the first, 25.6 for the second.)
+static int prefill_splits(int64_t batch, int64_t most, int32_t num_heads, int32_t num_kv_heads, int64_t reach,
+                          int32_t window) {
+  const int64_t group = num_heads / num_kv_heads, qt = group > 0 ? pf4::ROWS / group : 0;
+  if (qt == 0 || reach > (1 << 30)) return 1;
+  const int64_t ctas = batch * num_kv_heads * cdiv(most, qt);
+  const int64_t seen = window > 0 && window + qt < reach ? window + qt : reach;
+  const int64_t s = ctas > 0 && ctas <= 148 ? 148 / ctas : 1;
+  const int64_t by_keys = (seen - (most < seen ? most : seen) / 2) / (4 * pf4::BN);
+  return (int)(s < by_keys ? s : by_keys < 1 ? 1 : by_keys);
+}
+
 extern "C" size_t ada_kv4_paged_prefill_workspace_size(int32_t batch, int64_t total_q, int32_t max_seqlen_q,
                                                        int32_t num_heads, int32_t num_kv_heads, int32_t max_pages,
                                                        int32_t page_size) {
@@ -609,7 +698,10 @@ extern "C" size_t ada_kv4_paged_prefill_workspace_size(int32_t batch, int64_t to
       page_size <= 0)
     return 0;
   const int64_t most = max_seqlen_q < total_q ? max_seqlen_q : total_q;
-  return prefill_few(batch, most, num_heads, num_kv_heads, max_pages, page_size) ? kv4::rows_workspace_size(batch) : 0;
+  if (prefill_few(batch, most, num_heads, num_kv_heads, max_pages, page_size)) return kv4::rows_workspace_size(batch);
+  const int splits = prefill_splits(batch, most, num_heads, num_kv_heads, (int64_t)max_pages * page_size, 0);
+  if (splits == 1) return 0;
+  return (size_t)(batch * num_kv_heads * cdiv(most, (int64_t)(pf4::ROWS / (num_heads / num_kv_heads))) * splits) * pf4::PART * 4;
 }
 
 extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h,
@@ -672,6 +764,14 @@ extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_strid
   P.err = err;
   const int64_t qblocks = cdiv(most, P.qt);
   if (qblocks > 65535) return ADA_ERR_UNSUPPORTED;
+  P.splits = prefill_splits(batch, most, num_heads, num_kv_heads, (int64_t)max_pages * page_size, window);
+  P.qblocks = (int)qblocks;
+  P.parts = static_cast<float*>(workspace);
+  if (P.splits > 1) {
+    if (!workspace || workspace_bytes < (size_t)(batch * num_kv_heads * qblocks * P.splits) * pf4::PART * 4)
+      return ADA_ERR_WORKSPACE;
+    if (kv4::misaligned16(workspace)) return ADA_ERR_ALIGNMENT;
+  }
   static std::atomic<bool> ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ADA_ERR_CUDA;
@@ -680,8 +780,13 @@ extern "C" int ada_kv4_paged_prefill(const void* q, int q_dtype, int64_t q_strid
       return ADA_ERR_CUDA;
     ready[dev] = true;
   }
-  (void)launch_k(pf4::prefill_kernel, dim3((unsigned)num_kv_heads, (unsigned)batch, (unsigned)qblocks), dim3(pf4::THREADS),
-                 pf4::SMEM, reinterpret_cast<cudaStream_t>(stream), P);
+  (void)launch_k(pf4::prefill_kernel, dim3((unsigned)num_kv_heads, (unsigned)batch, (unsigned)(qblocks * P.splits)),
+                 dim3(pf4::THREADS), pf4::SMEM, reinterpret_cast<cudaStream_t>(stream), P);
   ADA_CHECK_LAUNCH();
+  if (P.splits > 1) {
+    (void)launch_k(pf4::merge_kernel, dim3((unsigned)num_kv_heads, (unsigned)batch, (unsigned)(qblocks * (pf4::ROWS / 32))),
+                   dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), P);
+    ADA_CHECK_LAUNCH();
+  }
   return ADA_OK;
 }

@@ -220,7 +220,7 @@ def paged_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 @functools.lru_cache(maxsize=512)
 def paged_prefill_fp4_workspace_bytes(batch: int, total_q: int, max_seqlen_q: int, num_heads: int, num_kv_heads: int,
                                       max_pages: int, page_size: int) -> int:
-    """0 but for a few rows a KV head."""
+    """0 where one launch does it: full grids, short tables."""
     return int(N.lib().ada_kv4_paged_prefill_workspace_size(batch, total_q, max_seqlen_q, num_heads, num_kv_heads,
                                                             max_pages, page_size))
 
@@ -234,8 +234,8 @@ def paged_prefill_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     The arguments of attention.paged_prefill with a 4-bit cache: q [total_q, Hq, 128]; the cache holds every
     sequence's cached prefix and new tokens; max_seqlen_q must be at least every sequence's new tokens.
     window W > 0: a row sees its own position and the W before it.  Rows behind the last sequence are left as
-    they are in ``out`` (unset without it).  workspace: at least paged_prefill_fp4_workspace_bytes(...) bytes, which a few
-    rows a KV head behind long tables need (default: allocated for the call)."""
+    they are in ``out`` (unset without it).  workspace: at least paged_prefill_fp4_workspace_bytes(...) bytes, which few
+    rows behind long tables need (default: allocated for the call)."""
     device = N.one_device("paged_prefill_fp4", q, k_cache, v_cache, block_tables, cu_seqlens_q, cu_seqlens_k)
     pages, hkv, page, s_page, s_head = _cache(k_cache, v_cache)
     q, code, out, out_code = _attention(device, q, block_tables, out, cu_seqlens_q, cu_seqlens_k)

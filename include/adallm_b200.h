@@ -752,7 +752,9 @@ ADA_API int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b,
  * the row's own position and the W before it); rows of q and out outside [0, total_q) and rows
  * behind the last sequence are not touched.  A few rows a KV head (max_seqlen_q x heads a KV head up to 32)
  * behind tables of more than 256 keys take the decode form, which shares long caches out over all SMs.
- * workspace: as for decode, sized by ada_kv4_paged_prefill_workspace_size (0 for more rows).  *err (may be NULL): 0x70
+ * where there are
+ * fewer CTAs of 256 rows than SMs, several share a block's keys and a second launch joins them.  workspace: as for decode,
+ * sized by ada_kv4_paged_prefill_workspace_size (0 where one launch does it; 20 MB at most but for few rows' tables).  *err (may be NULL): 0x70
  * if a tile wait ran out (the rows concerned are NaN).  A NaN key reaches every element of the rows that see it, a NaN value the 16 elements of its
  * block, and neither any other row.  Implemented: up to 256 heads a KV head. */
 ADA_API size_t ada_kv4_paged_prefill_workspace_size(int32_t batch, int64_t total_q, int32_t max_seqlen_q,

@@ -399,7 +399,7 @@ def test_few_rows_nan_reaches_the_rows_that_see_it(where):
 def test_few_rows_without_keys_scales_and_workspace():
     c = behind_long_tables(make(27, [3, 64, 0], [8, 2, 3], 8, 2, 16))
     size = kv.paged_prefill_fp4_workspace_bytes(3, 13, 8, 8, 2, c["tables"].shape[1], 16)
-    assert size > 0 and kv.paged_prefill_fp4_workspace_bytes(3, 13, 9, 8, 2, c["tables"].shape[1], 16) == 0
+    assert size > 0 and kv.paged_prefill_fp4_workspace_bytes(3, 13, 9, 8, 2, 16, 16) == 0
     out = torch.full((15, 8, 128), 7.0, dtype=F16, device=dev())
     q = torch.nn.functional.pad(c["q"], (0, 0, 0, 0, 0, 2))
     run_prefill(dict(c, q=q), 0, 0.5, 0.3, 0.2, out=out, workspace=torch.full((size,), 0xFF, dtype=torch.uint8, device=dev()))
@@ -409,6 +409,46 @@ def test_few_rows_without_keys_scales_and_workspace():
     short = torch.empty(size - 1, dtype=torch.uint8, device=dev())
     with pytest.raises(ValueError):
         run_prefill(c, workspace=short)
+
+
+SHARED = [  # cached, new, hq, hkv, page, window, dtype: few query blocks whose keys several CTAs share
+    ([3000], [40], 32, 8, 16, 0, BF16), ([2000, 0, 700], [64, 9, 100], 12, 4, 48, 0, F16), ([1030], [70], 64, 1, 64, 0, BF16),
+    ([5000], [33], 16, 16, 16, 900, F16), ([0, 2500], [300, 40], 8, 8, 16, 0, BF16), ([600], [33], 6, 6, 256, 0, F16)]
+
+
+@pytest.mark.parametrize("cached,new,hq,hkv,page,window,dtype", SHARED)
+def test_prefill_with_shared_keys(cached, new, hq, hkv, page, window, dtype):
+    lens = [a + b for a, b in zip(cached, new)]
+    c = make(sum(lens) + hq, lens, new, hq, hkv, page, dtype)
+    size = kv.paged_prefill_fp4_workspace_bytes(len(new), sum(new), max(new), hq, hkv, c["tables"].shape[1], page)
+    assert size > 0
+    want, err = want_of(c, window, decode=False)
+    out = torch.full((sum(new) + 3, hq, 128), 7.0, dtype=dtype, device=dev())
+    q = torch.nn.functional.pad(c["q"], (0, 0, 0, 0, 0, 3))
+    ws = torch.full((size,), 0xFF, dtype=torch.uint8, device=dev())
+    run_prefill(dict(c, q=q), window, out=out, workspace=ws)
+    assert_near(out[:-3], want, err)
+    assert (out[-3:] == 7).all() and torch.equal(run_prefill(c, window), out[:-3])
+    with pytest.raises(ValueError):
+        kv.paged_prefill_fp4(c["q"], c["k"], c["v"], c["tables"], c["cu_q"], c["cu_k"], max(new), 0.1,
+                             workspace=ws[:size // 2 // 16 * 16])
+
+
+def test_shared_keys_with_holes_nan_and_rows_without_keys():
+    c = make(50, [3000, 1500, 20], [60, 40, 50], 16, 4, 16)  # (the last sequence's first 30 rows see no key)
+    c["tables"][0, 10:100] = -1
+    c["tables"][1, :] = -1
+    want, err = want_of(c, decode=False)
+    out = run_prefill(c)
+    assert_near(out, want, err)
+    assert (out[60:130] == 0).all()
+    key, block = 2980, 5  # a value that the last 20 rows see
+    page = c["v"][int(c["tables"][0, key // 16])]
+    page[:, 16 * 64 + (key % 16) * 8 + block] = 0x7F
+    got = run_prefill(c)
+    nan = got.isnan()
+    assert nan[40:60, :, 80:96].all() and int(nan.sum()) == 20 * 16 * 16
+    assert_near(torch.where(nan, want.to(got.dtype), got), want, err)
 
 
 @pytest.mark.parametrize("where", ["k", "v"])

@@ -68,9 +68,10 @@ def test_prefill_refusals(lib):
         (dict(window=-1), BAD), (dict(scale=-0.1), BAD), (dict(vs=math.nan), BAD), (dict(q=8), ALIGN), (dict(v=4), ALIGN),
         (dict(ost=4), ALIGN), (dict(cq=18), ALIGN), (dict(err=2), ALIGN), (dict(batch=70000), UNSUP),
         (dict(most=8, mp=40, bts=40), WS), (dict(most=8, mp=40, bts=40, ws=16, wsb=100), WS),
-        (dict(most=8, mp=40, bts=40, ws=8, wsb=1 << 30), ALIGN), (dict(total=3, mp=40, bts=40), WS)])
+        (dict(most=8, mp=40, bts=40, ws=8, wsb=1 << 30), ALIGN), (dict(total=3, mp=40, bts=40), WS), (dict(mp=40, bts=40), WS),
+        (dict(mp=40, bts=40, ws=16, wsb=1 << 20), WS), (dict(mp=40, bts=40, ws=8, wsb=1 << 30), ALIGN)])
     size = lib.ada_kv4_paged_prefill_workspace_size
-    assert size(1, 50, 50, 32, 8, 40, 16) == 0 and size(1, 50, 8, 32, 8, 40, 16) > 0
+    assert size(1, 50, 50, 32, 8, 20, 16) == 0 and size(1, 50, 50, 32, 8, 40, 16) > 0 and size(1, 50, 8, 32, 8, 40, 16) > 0
     assert size(1, 50, 8, 32, 8, 16, 16) == 0 and size(1, 0, 8, 32, 8, 40, 16) == 0
     assert size(8000, 8000, 1, 1 << 30, 1 << 30, 1 << 26, 16) == 0 and size(1, 1, 1, 8, 8, 1 << 30, 1 << 30) == 0
 
