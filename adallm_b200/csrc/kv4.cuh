@@ -13,6 +13,8 @@
 // overlaps their start (step_metadata.cu's CTAs read tables that others of it extend).
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ada {
@@ -29,6 +31,29 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+// Largest magnitudes of the even and the odd elements of `acc` and 8 more, in a pair; NaN if one is.
+template <typename T>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (std::is_same<T, __half>::value)
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max_pairs(uint32_t acc, const uint4& x) {
+  constexpr uint32_t MAGNITUDE = 0x7FFF7FFFu;
+  return max2_nan<T>(max2_nan<T>(acc, max2_nan<T>(x.x & MAGNITUDE, x.y & MAGNITUDE)),
+                     max2_nan<T>(x.z & MAGNITUDE, x.w & MAGNITUDE));
+}
+// The larger of a pair; NaN if one is.
+template <typename T>
+__device__ __forceinline__ float larger(const uint32_t& pair) {
+  const T* h = reinterpret_cast<const T*>(&pair);
+  return max_nan(to_f32(h[0]), to_f32(h[1]));
 }
 
 // x / d given r near 1 / d: one Newton step on the quotient's remainder (Markstein 1990).  Correctly rounded where x / d lies further than 2^-44 of

@@ -8,7 +8,7 @@
 // Floor of a block of 64 keys: 256 x 64 exponentials (16 a cycle and SM: 1,024 cycles), 2 x 256 x 64 x 128
 // multiply-adds (4,096 a cycle: 1,024) and the operands' shared-memory reads (some 1,400).  It takes about 1,900: the
 // softmax of the two tiles' rows on one scheduler runs in step (its exponentials 1,300 cycles side by side, 850 alone) and
-// its loads, maxima and waits (600) come in between.  4 x 2,048 tokens behind 2,048, 32/8 heads: 423 us, 58% of
+// its loads, maxima and waits (600) come in between.  4 x 2,048 tokens behind 2,048, 32/8 heads: 417 us, 0.59 of
 // the measured matrix rate.  Tried and left out: two threads a row (524: they have to agree on the reference),
 // turns between the tiles (466), part of the exponentials as polynomials on the FMA pipe (426-454), 128 keys a block (564).
 //
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     if (nblk > 0) {
       // The query rows -> f16, times a power of two, in place: elements come by cp.async to where their f16 form
       // will lie, so that a thread reads and writes its row without bank conflicts.  (By loads into registers the L1
-      // beside this much shared memory, some 16 KB, holds a quarter of them at a time: 16,000 cycles a CTA, here 9,000.)
+      // beside this much shared memory, some 16 KB, holds a quarter of them at a time: 16,000 cycles a CTA, here 7,500.)
       const int64_t mine = row * P.q_st + head * P.q_sh;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -423,27 +423,29 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       cp_commit();
       cp_wait<0>();
       __syncwarp();
-      float top = 0.f;
+      int ex = 0;
+      auto convert = [&](auto type) {
+        using T = decltype(type);
+        uint32_t top2 = 0;  // of pairs of magnitudes
 #pragma unroll 4
-      for (int c = 0; c < 16; ++c) {
-        uint4 x = *chunk(lane, c);
-        if (!valid) x = make_uint4(0, 0, 0, 0);
-        float f[8];
-        if (P.q_bf16) unpack8<__nv_bfloat16>(x, f); else unpack8<__half>(x, f);
+        for (int c = 0; c < 16; ++c) top2 = max_pairs<T>(top2, *chunk(lane, c));
+        ex = query_exponent(valid ? larger<T>(top2) : 0.f);
+        const float mul = pow2(ex);
+#pragma unroll 1
+        for (int c = 0; c < 16; c += 4) {
+          uint4 x[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(f[i]));
-      }
-      const int ex = query_exponent(top);
-      const float mul = pow2(ex);
-#pragma unroll 4
-      for (int c = 0; c < 16; ++c) {
-        uint4 x = *chunk(lane, c);
-        if (!valid) x = make_uint4(0, 0, 0, 0);
-        float f[8];
-        if (P.q_bf16) unpack8<__nv_bfloat16>(x, f); else unpack8<__half>(x, f);
-        *chunk(lane, c) = make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
-                                     pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
-      }
+          for (int i = 0; i < 4; ++i) x[i] = valid ? *chunk(lane, c + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f[8];
+            unpack8<T>(x[i], f);
+            *chunk(lane, c + i) = make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
+                                             pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
+          }
+        }
+      };
+      if (P.q_bf16) convert(__nv_bfloat16()); else convert(__half());
       factor = score_factor(P.scale_log2, ex);
       if (!valid) factor = fminf(factor, SAFE_FACTOR);  // (all its keys are masked)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -472,10 +474,24 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       const uint4 marked = *reinterpret_cast<const uint4*>(flags + 4);
       const int key0 = kb0 + j * BN, a = lo - key0, e = hi - key0;  // visible columns [a, e) of loaded tiles
       if (!__all_sync(0xffffffffu, blk_ok == 15u && a <= 0 && e >= BN)) {
+        if (__all_sync(0xffffffffu, a >= BN || e <= 0)) {  // none of the warp's rows sees the block
+          uint32_t zero[16] = {};
+          tmem_st16(trow + s_col + BN * (j & 1), zero);
+          tmem_st16(trow + s_col + BN * (j & 1) + 16, zero);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_plain(&p_full[2 * t + (j & 1)]);
+          continue;
+        }
+        const int a1 = max(a, 0);
+        const unsigned n = (unsigned)max(min(e, BN) - a1, 0);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const bool vis = (i >= a) & (i < e) & (((blk_ok >> (i >> 4)) & 1u) != 0);
-          x[i] = vis ? x[i] : -INFINITY;
+        for (int i = 0; i < 64; ++i) x[i] = (unsigned)(i - a1) < n ? x[i] : -INFINITY;
+        if (blk_ok != 15u) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (!((blk_ok >> (i >> 4)) & 1u)) x[i] = -INFINITY;
         }
       }
       if (marked.x | marked.y | marked.z | marked.w) {
@@ -590,7 +606,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
           const float by = (nan_blocks >> (d0 / 16 + c)) & 1 ? nan : inv;
           float* f = o + 16 * c;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = by == 0.f ? 0.f : f[i] * by;  // (no key: O holds nothing)
+          for (int i = 0; i < 16; ++i) f[i] *= by;  // (without a key O is 0)
           *chunk(lane, d0 / 8 + 2 * c) = P.o_bf16 ? pack8<__nv_bfloat16>(f) : pack8<__half>(f);
           *chunk(lane, d0 / 8 + 2 * c + 1) = P.o_bf16 ? pack8<__nv_bfloat16>(f + 8) : pack8<__half>(f + 8);
         }

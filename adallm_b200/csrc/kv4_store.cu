@@ -8,8 +8,6 @@
 //
 // Store: a row's rotated key, rounded to T as a model without the fusion has it, and its value are
 // divided by the tensor's scale and packed as kv4.cuh describes.
-#include <type_traits>
-
 #include "kv4.cuh"
 
 namespace ada {
@@ -37,19 +35,7 @@ struct RotaryParams {
 // Largest magnitude of 8 elements; NaN if one is.
 template <typename T>
 __device__ __forceinline__ float largest(const uint4& x) {
-  const uint32_t w[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
-  uint32_t a, b;
-  if (std::is_same<T, __half>::value) {
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
-  } else {
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
-  }
-  const T* h = reinterpret_cast<const T*>(&a);
-  return max_nan(to_f32(h[0]), to_f32(h[1]));
+  return larger<T>(max_pairs<T>(0u, x));
 }
 // Codes of 8 elements over the tensor's scale `div` (inv near 1 / div) and the block's scale s; top: the block's largest
 // quotient.
