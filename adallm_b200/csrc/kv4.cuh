@@ -33,6 +33,31 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// Two floats in one register pair: the packed fp32 operations round each half like the single ones.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Largest magnitudes of the even and the odd elements of `acc` and 8 more, in a pair; NaN if one is.
 template <typename T>
 __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
@@ -56,18 +81,23 @@ __device__ __forceinline__ float larger(const uint32_t& pair) {
   return max_nan(to_f32(h[0]), to_f32(h[1]));
 }
 
-// x / d given r near 1 / d: one Newton step on the quotient's remainder (Markstein 1990).  Correctly rounded where x / d lies further than 2^-44 of
-// itself from a midpoint of fp32 or on none: for divisors of few bits (6; the e4m3 scales) always (2^-27 and
-// more), for others but for one quotient in 2^20, which is one step (2^-24) off then.
-__device__ __forceinline__ float quotient(float x, float d, float r) {
-  const float q = x * r;
-  return fmaf(fmaf(-q, d, x), r, q);
-}
-
-// The same where x may be an infinity or the quotient one.
+// x / d given r near 1 / d: one Newton step on the quotient's remainder (Markstein 1990).  Correctly rounded where x / d
+// lies further than 2^-44 of itself from a midpoint of fp32 or on none: for divisors of few bits (6; the e4m3 scales)
+// always (2^-27 and more), for others but for one quotient in 2^20, which is one step (2^-24) off then.  (x may be an
+// infinity, or the quotient one.)
 __device__ __forceinline__ float any_quotient(float x, float d, float r) {
   const float q = x * r;
   return fabsf(q) == INFINITY ? q : fmaf(fmaf(-q, d, x), r, q);
+}
+
+// The same of 8 finite elements, two an instruction.
+__device__ __forceinline__ void quotients(float* x, float d, float r) {
+  const uint64_t minus = pair(-d, -d), r2 = pair(r, r);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t a = pair(x[i], x[i + 1]), q = mul2(a, r2);
+    unpair(fma2(fma2(q, minus, a), r2, q), x[i], x[i + 1]);
+  }
 }
 
 // e4m3 byte of max|x| / 6, saturated to 448; NaN when the block holds one (the block then reads as NaN).
@@ -90,10 +120,8 @@ __device__ __forceinline__ uint32_t codes8(float* x, float s, float top) {
   }
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-  float q[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = quotient(x[i], s, r);
-  return f32x8_to_e2m1x8(q);
+  quotients(x, s, r);
+  return f32x8_to_e2m1x8(x);
 }
 // Eight codes -> their values, four f16x2 (low half = even element).
 __device__ __forceinline__ void widen8(uint32_t w, uint32_t* h) {
@@ -142,25 +170,6 @@ __device__ __forceinline__ float score_factor(float scale_log2, int exponent) {
   return fmaxf(fminf(scale_log2 * pow2(-exponent), 1.2379400392853803e27f), 1e-36f);
 }
 
-// Two floats in one register pair: the packed fp32 operations round each half like the single ones.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // A tensor's scale that both it and its reciprocal are good for as fp32 factors (no NaN, infinity or subnormal).
 inline bool scale_ok(float s) { return s >= 1e-30f && s <= 1e30f; }
 inline bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }

@@ -48,8 +48,7 @@ __device__ __forceinline__ uint32_t pack_codes(const uint4& x, float div, float 
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = any_quotient(y[i], div, inv);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = quotient(y[i], div, inv);
+      quotients(y, div, inv);
     }
   }
   return codes8(y, s, top);
@@ -61,7 +60,7 @@ __device__ __forceinline__ uint32_t pack_codes(const uint4& x, float div, float 
 // STAGES - 1 tokens are on their way by cp.async, each thread's rows into places of its own: with a token
 // at a time, or one ahead in registers, an SM has 20-40 KB in flight where HBM wants 66 (95 us, with this
 // 62.5, for 16,381 tokens of 40 heads: 83% of the copy rate).  The store's arithmetic (maxima, quotients,
-// conversions) takes longer than its bytes: 75 us for 8,195 tokens of 32/8 heads, 47 by its bytes.
+// conversions) takes longer than its bytes: 54 us for 8,195 tokens of 32/16 heads, 34 by its bytes.
 constexpr int U = 2, STAGES = 4;
 // Bytes of a stage: the CTA's rows, then the table's row.
 __host__ __device__ constexpr int stage_bytes(int threads, int heads, int rot) { return threads * heads * 32 + rot * 4; }
