@@ -141,6 +141,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 // fall on different banks.
 __device__ __forceinline__ int chunk_at(int line, int chunk) { return line * 128 + ((chunk ^ (2 * (line & 3))) << 4); }
 
+// A pair times one half of another (through the type, so that the instruction takes the half and no other makes a pair).
+__device__ __forceinline__ uint32_t by_half(uint32_t a, uint32_t s, bool high) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&s);
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), high ? __high2half2(h) : __low2half2(h));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // Row of one head to memory: 16 elements of lane's scale block.
 __device__ __forceinline__ void write16(const Params& P, int64_t row, int head, int e0, const float* f) {
   if (P.o_bf16) {
@@ -434,13 +441,13 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
           const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t sa = prmt(s0, s0, w < 2 ? 0x1010 : 0x3232), sb = prmt(s1, s1, w < 2 ? 0x1010 : 0x3232);
             uint32_t x[4], y[4];
             widen8(w0[w], x);
             widen8(w1[w], y);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const uint32_t A[4] = {mul_f16x2(x[2 * j], sa), mul_f16x2(y[2 * j], sb), mul_f16x2(x[2 * j + 1], sa), mul_f16x2(y[2 * j + 1], sb)};
+              const uint32_t A[4] = {by_half(x[2 * j], s0, w >= 2), by_half(y[2 * j], s1, w >= 2),
+                                     by_half(x[2 * j + 1], s0, w >= 2), by_half(y[2 * j + 1], s1, w >= 2)};
               mma_16816_f16(s[i], A, qf + 2 * (2 * w + j));
             }
           }
