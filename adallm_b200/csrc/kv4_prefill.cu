@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       cp_wait<NSTG - 2>();
       __syncwarp();  // every lane's part has arrived, and the slot before has been read
       fetch(j + NSTG - 1);
-      if (j >= NKV && !wait_b(&kv_empty[kb], ((j / NKV) - 1) & 1, abort_v, P.err)) break;
+      if (j >= NKV && !wait_w(&kv_empty[kb], ((j / NKV) - 1) & 1, abort_v, P.err)) break;
       const uint8_t* st = ring + from * E_BYTES;
       const bool ok = (there >> from) & 1u;
       uint32_t* flags = slots + kb * SLOT_WORDS;

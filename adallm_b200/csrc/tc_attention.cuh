@@ -83,5 +83,21 @@ __device__ __forceinline__ bool wait_b(uint64_t* bar, uint32_t parity, volatile 
   }
 }
 
+// The same for a whole warp, with one outcome for all lanes: what follows may be warp-collective.  (A lane that gave up
+// alone would be missing there, and the others would wait for it for good.)
+__device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t parity, volatile int* abort_v, unsigned int* err) {
+  if (__all_sync(0xffffffffu, try_wait_sleep(bar, parity))) return true;
+  const uint64_t t0 = sm100::globaltimer();
+  for (;;) {
+    if (__all_sync(0xffffffffu, try_wait_sleep(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_v)) return false;
+    if (__any_sync(0xffffffffu, sm100::globaltimer() - t0 > 2000000000ull)) {
+      *abort_v = 1;
+      if (err) atomicOr(err, ERR_TILE_WAIT);
+      return false;
+    }
+  }
+}
+
 }  // namespace tca
 }  // namespace ada
