@@ -365,8 +365,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int j = 0; j < nblk; ++j) {
       const int s = j % NSTG, kb = j % NKV;
-      if (!wait_b(&e_full[s], (j / NSTG) & 1, abort_v, P.err)) break;
-      if (j >= NKV && !wait_b(&kv_empty[kb], ((j / NKV) - 1) & 1, abort_v, P.err)) break;
+      if (!wait_w(&e_full[s], (j / NSTG) & 1, abort_v, P.err)) break;
+      if (j >= NKV && !wait_w(&kv_empty[kb], ((j / NKV) - 1) & 1, abort_v, P.err)) break;
       const uint8_t* st = es + s * E_BYTES;
       const int mask = e_ok[s];
       int blk_ok[4];

@@ -57,7 +57,8 @@ def give_up(events, seed, blocks=6):
                 return
 
 
-ROLES = [("kv4_prefill.cu", "converters"), ("kv4_prefill.cu", "softmax")]
+ROLES = [("kv4_prefill.cu", "converters"), ("kv4_prefill.cu", "softmax"), ("prefill_attention.cu", "converters"),
+         ("prefill_attention.cu", "softmax")]
 
 
 @pytest.mark.parametrize("name,role", ROLES)
