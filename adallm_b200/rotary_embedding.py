@@ -19,32 +19,59 @@ from torch import nn
 from . import _native as N
 
 
+_YARN_KEYS = {"rope_type", "type", "rope_theta", "factor", "original_max_position_embeddings", "beta_fast", "beta_slow",
+              "attention_factor", "mscale", "mscale_all_dim", "truncate"}
+
+
 def _yarn_cos_sin_cache(rotary_dim: int, max_position: int, base: float, rope_scaling: dict, device=None):
     """YaRN (Peng et al. 2023): pairs that turn more than beta_fast times over the trained length keep their
-    frequency, those below beta_slow turns are slowed by `factor`, a linear ramp lies between; cos and sin are
-    multiplied by the attention factor 0.1 ln(factor) + 1.  Angles in 64 bits, the table in fp32."""
-    factor = float(rope_scaling["factor"])
-    trained = float(rope_scaling.get("original_max_position_embeddings") or max_position / factor)
-    fast, slow = float(rope_scaling.get("beta_fast", 32.0)), float(rope_scaling.get("beta_slow", 1.0))
-    amplitude = rope_scaling.get("attention_factor")
-    amplitude = float(amplitude) if amplitude is not None else 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    frequency, those below beta_slow turns are slowed by `factor`, a linear ramp lies between (its ends on whole
+    pairs unless `truncate` is false); cos and sin are multiplied by the attention factor: 0.1 ln(factor) + 1, or with
+    mscale m and mscale_all_dim n (0.1 m ln(factor) + 1) / (0.1 n ln(factor) + 1).  Angles in 64 bits, the table in
+    fp32.  The table has factor x original_max_position_embeddings rows at least, as positions behind its last
+    row are clamped to it.  Keys that would change the table in a way not known here are refused."""
+    given = {k: v for k, v in rope_scaling.items() if v is not None}
+    unknown = sorted(set(given) - _YARN_KEYS)
+    if unknown:
+        raise ValueError(f"yarn rope_scaling: unknown {', '.join(unknown)}")
+    if float(given.get("rope_theta", base)) != float(base):
+        raise ValueError("yarn rope_scaling: rope_theta is not the table's base")
+    if "factor" not in given or "original_max_position_embeddings" not in given:
+        raise ValueError("yarn rope_scaling needs factor and original_max_position_embeddings")
+    factor, trained = float(given["factor"]), float(given["original_max_position_embeddings"])
+    fast, slow = float(given.get("beta_fast", 32.0)), float(given.get("beta_slow", 1.0))
+    if not (1.0 <= factor < math.inf and 1.0 <= trained < math.inf and 0.0 < slow <= fast < math.inf):
+        raise ValueError("yarn rope_scaling: factor and original_max_position_embeddings of at least 1, 0 < beta_slow <= "
+                         "beta_fast")
+    scales = [k for k in ("attention_factor", "mscale", "mscale_all_dim") if k in given]
+    if not all(0.0 < float(given[k]) < math.inf for k in scales):
+        raise ValueError("yarn rope_scaling: attention_factor, mscale and mscale_all_dim must be positive")
+    if ("mscale" in given) != ("mscale_all_dim" in given):
+        raise ValueError("yarn rope_scaling: mscale and mscale_all_dim go together")  # (one alone is read in two ways)
+    m, n = (0.1 * float(given.get(k, d)) * math.log(factor) + 1.0 for k, d in (("mscale", 1.0), ("mscale_all_dim", 0.0)))
+    amplitude = float(given.get("attention_factor", m / n))
     half = rotary_dim // 2
 
     def pair(turns):
         return half * math.log(trained / (turns * 2 * math.pi)) / math.log(base)
 
-    low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rotary_dim - 1)
+    low, high = pair(fast), pair(slow)
+    if given.get("truncate", True):
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, rotary_dim - 1)
     i = torch.arange(half, dtype=torch.float64, device=device)
     keep = 1.0 - ((i - low) / max(high - low, 0.001)).clamp(0, 1)
     inv_freq = base ** (-i / half)
     inv_freq = inv_freq * keep + inv_freq / factor * (1.0 - keep)
-    angle = torch.arange(max_position, dtype=torch.float64, device=device)[:, None] * inv_freq
+    rows = max(max_position, math.ceil(factor * trained))
+    angle = torch.arange(rows, dtype=torch.float64, device=device)[:, None] * inv_freq
     return (torch.cat((angle.cos(), angle.sin()), -1) * amplitude).float().unsqueeze_(1)
 
 
 def build_cos_sin_cache(head_size: int, max_position: int, base: float, rope_scaling: dict | None = None,
                         device=None) -> torch.Tensor:
-    """fp32 [max_position, 1, head_size]; same arithmetic as rotary_embedding.py:26-43."""
+    """fp32 [max_position, 1, head_size]; same arithmetic as rotary_embedding.py:26-43.  A yarn table has
+    factor x original_max_position_embeddings rows where that is more."""
     if rope_scaling is not None and rope_scaling.get("rope_type", rope_scaling.get("type")) == "yarn":
         return _yarn_cos_sin_cache(head_size, max_position, base, rope_scaling, device)
     inv_freq = 1.0 / (base ** (torch.arange(0, head_size, 2, dtype=torch.float) / head_size))
