@@ -86,6 +86,12 @@ def build_cos_sin_cache(head_size: int, max_position: int, base: float, rope_sca
     return cache if device is None else cache.to(device)
 
 
+def _heads(x: torch.Tensor, positions: torch.Tensor, d: int) -> torch.Tensor:
+    """x as [tokens, heads, d], the heads counted: without tokens there is nothing to infer them from."""
+    t = positions.numel()
+    return x.reshape(t, (x.numel() // t if t else math.prod(x.shape[positions.dim():])) // d, d)
+
+
 def apply_rope(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, cos_sin_cache: torch.Tensor,
                q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
     N.require_cuda(positions, query, key, cos_sin_cache, what="rotary_embedding")
@@ -93,8 +99,7 @@ def apply_rope(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, 
         raise ValueError("rotary embedding expects bf16/fp16 q and k")
     d = cos_sin_cache.shape[-1]
     t = positions.numel()
-    q3 = query.view(t, -1, d) if query.is_contiguous() else query.reshape(t, -1, d)
-    k3 = key.view(t, -1, d) if key.is_contiguous() else key.reshape(t, -1, d)
+    q3, k3 = _heads(query, positions, d), _heads(key, positions, d)
     if q3.stride(1) != d or k3.stride(1) != d or q3.stride(2) != 1 or k3.stride(2) != 1:
         q3, k3 = q3.contiguous(), k3.contiguous()
     if cos_sin_cache.dtype != torch.float32 or not cos_sin_cache.is_contiguous():
@@ -182,8 +187,8 @@ class RotaryEmbedding(nn.Module):
     def forward(self, positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor):
         if self.rotary_dim == self.head_size and not self.interleaved:
             return apply_rope(positions, query, key, self.cos_sin_cache)
-        t, d = positions.numel(), self.head_size
-        q, k = apply_rotary(positions, query.reshape(t, -1, d), key.reshape(t, -1, d), self.cos_sin_cache,
+        d = self.head_size
+        q, k = apply_rotary(positions, _heads(query, positions, d), _heads(key, positions, d), self.cos_sin_cache,
                             self.interleaved)
         return q.view(query.shape), k.view(key.shape)
 
