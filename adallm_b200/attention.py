@@ -157,7 +157,10 @@ class Attention(nn.Module):
         store, prefill, decode = ((fp4.store_kvcache_fp4, fp4.paged_prefill_fp4, fp4.paged_decode_fp4) if bits4 else
                                   (store_kvcache, paged_prefill, paged_decode))
         if self.k_cache.numel() and self.v_cache.numel():
-            store(k, v, self.k_cache, self.v_cache, context.slot_mapping, self.k_scale, self.v_scale)
+            slots = context.slot_mapping
+            if bits4 and slots.dtype != torch.int32:  # store_kvcache converts by itself, the 4-bit store takes int32
+                slots = slots.clamp(-1, 0x7FFFFFFF).to(torch.int32)
+            store(k, v, self.k_cache, self.v_cache, slots, self.k_scale, self.v_scale)
         window = self.sliding_window if (self.sliding_window is not None and self.sliding_window > 0) else 0
         if context.is_prefill:
             try:
