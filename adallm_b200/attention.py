@@ -154,6 +154,7 @@ class Attention(nn.Module):
             raise NotImplementedError("adallm_b200 runs the prefix-cache prefill and the decode branch; a prefill "
                                       "without a block table stays on the reference path")
         bits4 = self.k_cache.dtype is torch.uint8
+        bits = "4-bit" if bits4 else "FP8"
         store, prefill, decode = ((fp4.store_kvcache_fp4, fp4.paged_prefill_fp4, fp4.paged_decode_fp4) if bits4 else
                                   (store_kvcache, paged_prefill, paged_decode))
         if self.k_cache.numel() and self.v_cache.numel():
@@ -170,7 +171,7 @@ class Attention(nn.Module):
             except Exception as exc:
                 if torch.cuda.is_current_stream_capturing() or isinstance(exc, ValueError):
                     raise
-                raise RuntimeError("FP8 paged prefill kernel failed; no fallback is allowed in this runtime.") from exc
+                raise RuntimeError(f"{bits} paged prefill kernel failed; no fallback is allowed in this runtime.") from exc
         try:
             return decode(q.view(-1, self.num_heads, self.head_dim), self.k_cache, self.v_cache,
                           context.block_tables, context.context_lens, self.scale, window,
@@ -180,4 +181,4 @@ class Attention(nn.Module):
                 raise
             if isinstance(exc, ValueError):
                 raise
-            raise RuntimeError("FP8 KV decode kernel failed; no fallback is allowed in this runtime.") from exc
+            raise RuntimeError(f"{bits} KV decode kernel failed; no fallback is allowed in this runtime.") from exc

@@ -1,4 +1,4 @@
-"""Attention.forward over a 4-bit cache beside its e4m3 form: the slots it takes."""
+"""Attention.forward over a 4-bit cache beside its e4m3 form: the slots it takes, and the kernel that a failure names."""
 import pytest
 import torch
 
@@ -31,6 +31,27 @@ def test_slots_of_64_bits_reach_the_store_as_32(monkeypatch):
         module()(torch.zeros((4, 512), dtype=torch.bfloat16), rows, rows)
     assert all(s.dtype == I32 for s in seen)
     assert seen[0].tolist() == [3, -1, 2 ** 31 - 1, 7] and seen[1].tolist() == [3, -1, 2 ** 31 - 1, -1]
+
+
+@pytest.mark.parametrize("bits", ["4-bit", "FP8"])
+@pytest.mark.parametrize("prefill", [True, False])
+def test_a_failure_names_the_kernel_that_ran(monkeypatch, bits, prefill):
+    def fail(*args):
+        raise RuntimeError("launch")
+
+    where, tail = (A.fp4, "_fp4") if bits == "4-bit" else (A, "")
+    monkeypatch.setattr(where, "paged_prefill" + tail, fail)
+    monkeypatch.setattr(where, "paged_decode" + tail, fail)
+    for name in ("store_kvcache_fp4", "store_kvcache"):
+        monkeypatch.setattr(A.fp4 if name.endswith("4") else A, name, lambda *a: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    m = module()
+    if bits == "FP8":
+        m.k_cache = m.v_cache = torch.zeros((3, 16, 2, 128)).to(torch.float8_e4m3fn)
+    one = torch.zeros(1, dtype=I32)
+    set_context(prefill, one, one, 1, 0, one, one, one[None])
+    with pytest.raises(RuntimeError, match=f"^{bits} {'paged prefill' if prefill else 'KV decode'} kernel failed"):
+        m(torch.zeros((1, 512), dtype=torch.bfloat16), None, None)
 
 
 @pytest.mark.gpu
