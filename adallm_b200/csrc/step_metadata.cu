@@ -134,12 +134,14 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(Params P) {
   for (int64_t i = me; i < taken; i += step) {
     const int b = segment(cu_p, B, (int)i);
     const int64_t at = start + i, col = pages_of(had[b], P.page) + (i - cu_p[b]);
-    if (at < 0 || at >= P.num_free)
+    const bool listed = at >= 0 && at < P.num_free;
+    if (!listed)
       err |= ERR_PAGES;
     else if (col >= P.max_pages)
       err |= ERR_WIDTH;
-    else
-      P.tables[b * P.t_stride + col] = P.free_pages[at];
+    // a page that is not there is none in the table either: what stood there may be a page of another request by now,
+    // and the next step counts these columns as the request's own
+    if (col < P.max_pages) P.tables[b * P.t_stride + col] = listed ? P.free_pages[at] : -1;
   }
   // the tokens
   for (int64_t t = me; t < P.tokens; t += step) {

@@ -42,7 +42,7 @@ def step_metadata(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     free_start int32 [1] on in request order, and ``free_next`` says where the next step starts.
     num_tokens: what the outputs are laid out for, at least the sum of new_lens; further tokens are
     padding with position 0 and slot -1.  A token without a page (free list at its end, table too narrow)
-    gets slot -1.  err: optional int32 [1] device word; 0x100 (free list), 0x200 (table) and 0x400 (more
+    gets slot -1, and its table entry is -1 (so it stays without one in the steps behind).  err: optional int32 [1] device word; 0x100 (free list), 0x200 (table) and 0x400 (more
     tokens than num_tokens) are OR-ed in.  The inputs, block_tables apart, are left as they are: for the
     next step copy free_next to free_start and context_lens to cached_lens.  At most 8192 requests."""
     tensors = (cached_lens, new_lens, free_pages, free_start)

@@ -670,7 +670,8 @@ ADA_API int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t
  *   after request (slot = page * page_size + row); padding has position 0 and slot -1.
  * cu_seqlens_q, cu_seqlens_k int32 [requests + 1]: prefix sums of the new tokens and of all tokens;
  * context_lens int32 [requests]: cached + new.
- * A token without a page (free list at its end, table too narrow, -1 in the table) gets slot -1.
+ * A token without a page (free list at its end, table too narrow, -1 in the table) gets slot -1; a page
+ * that the free list does not have is -1 in the table, whatever stood there.
  * *err (may be NULL): 0x100 is OR-ed in if the free list ran out, 0x200 if a table was too narrow, 0x400
  * if there are more tokens than num_tokens (those behind it are not listed) or a slot passes 32 bits.
  * The same inputs give the same outputs, also after a run (only new pages are written); the outputs must

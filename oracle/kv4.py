@@ -152,6 +152,8 @@ def step_metadata(cached, new, tables, free, start, page, tokens):
         for col in range(-(-c // page), -(-(c + n) // page)):
             if not 0 <= at < len(free):
                 err |= 0x100
+                if col < width:
+                    tables[b][col] = -1
             elif col >= width:
                 err |= 0x200
                 ids[col] = -1
