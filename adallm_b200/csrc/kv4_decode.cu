@@ -421,8 +421,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       float base0 = 0.f, base1 = 0.f;              // the running maxima
       float pass0 = -INFINITY, pass1 = -INFINITY;  // scores beyond these move them; -inf: there is none yet
 
-      auto one = [&](auto at) {  // a step whose ring slot is a constant, and so its addresses (549 instead of 583 instructions, 224 -> 221 us)
-        constexpr int slot = decltype(at)::value;
+      // A step whose ring slot is a constant, and so its addresses (549 instead of 583 instructions, 224 -> 221 us for the
+      // long case).  ROWS keeps the slot a variable: with its masks the step stands there once (36 bytes of spill stores
+      // instead of 80: 32 x 8 tokens behind 500 keys 35.2 instead of 38.5 us, 8 x 2 behind 8,000 32.3 and 33.3, 32 x 8
+      // behind 8,000 235 and 233).
+      auto one = [&](auto at) {
+        const int slot = at;
         cp_wait<STAGES - 1>();
         __syncwarp();
         const uint8_t* step = ring + slot * STEP_BYTES;
@@ -572,7 +576,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
         load(slot);
       };
       for (; t < stop; ++t) {
-        if (slot == 0)
+        if (ROWS)
+          one(slot);
+        else if (slot == 0)
           one(std::integral_constant<int, 0>());
         else
           one(std::integral_constant<int, 1>());
