@@ -89,7 +89,9 @@ def build_cos_sin_cache(head_size: int, max_position: int, base: float, rope_sca
 def _heads(x: torch.Tensor, positions: torch.Tensor, d: int) -> torch.Tensor:
     """x as [tokens, heads, d], the heads counted: without tokens there is nothing to infer them from."""
     t = positions.numel()
-    return x.reshape(t, (x.numel() // t if t else math.prod(x.shape[positions.dim():])) // d, d)
+    if x.numel():
+        return x.reshape(t, -1, d)
+    return x.reshape(t, 0 if t else math.prod(x.shape[positions.dim():]) // d, d)
 
 
 def apply_rope(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, cos_sin_cache: torch.Tensor,
