@@ -190,16 +190,21 @@ extern "C" int ada_step_metadata(const int32_t* cached_lens, const int32_t* new_
   if (requests > 0 && max_pages > 0 && (!block_tables || bt_stride < max_pages)) return ADA_ERR_INVALID_ARG;
   if (num_free > 0 && !free_pages) return ADA_ERR_INVALID_ARG;
   if (num_tokens > 0 && (!positions || !slot_mapping)) return ADA_ERR_INVALID_ARG;
-  // CTAs read these while another writes its results
-  if (free_next == free_start || context_lens == cached_lens || context_lens == new_lens) {
-    if (requests > 0 || free_next == free_start) return ADA_ERR_INVALID_ARG;
-  }
   if (requests > meta::MAX_REQUESTS || num_tokens > 0x7fffffff) return ADA_ERR_UNSUPPORTED;
   const uintptr_t words = (uintptr_t)cached_lens | (uintptr_t)new_lens | (uintptr_t)block_tables |
                           (uintptr_t)free_pages | (uintptr_t)free_start | (uintptr_t)slot_mapping |
                           (uintptr_t)cu_seqlens_q | (uintptr_t)cu_seqlens_k | (uintptr_t)context_lens |
                           (uintptr_t)free_next | (uintptr_t)err;
   if ((words & 3) || ((uintptr_t)positions & 7)) return ADA_ERR_ALIGNMENT;
+  // every CTA reads the inputs, the first one writes its results meanwhile: no output may lie in an input
+  const struct { const void* p; int64_t n; } in[] = {{cached_lens, 4LL * requests}, {new_lens, 4LL * requests},
+                                                     {free_pages, 4 * num_free}, {free_start, 4}},
+      made[] = {{positions, 8 * num_tokens}, {slot_mapping, 4 * num_tokens}, {cu_seqlens_q, 4LL * (requests + 1)},
+                {cu_seqlens_k, 4LL * (requests + 1)}, {context_lens, 4LL * requests}, {free_next, 4}};
+  for (const auto& a : in)
+    for (const auto& b : made)
+      if (a.n > 0 && b.n > 0 && (uintptr_t)a.p < (uintptr_t)b.p + b.n && (uintptr_t)b.p < (uintptr_t)a.p + a.n)
+        return ADA_ERR_INVALID_ARG;
   meta::Params P;
   P.cached = cached_lens;
   P.fresh = new_lens;

@@ -674,8 +674,8 @@ ADA_API int ada_verify_drafts(const void* target, int dtype, int64_t ld, int32_t
  * that the free list does not have is -1 in the table, whatever stood there.
  * *err (may be NULL): 0x100 is OR-ed in if the free list ran out, 0x200 if a table was too narrow, 0x400
  * if there are more tokens than num_tokens (those behind it are not listed) or a slot passes 32 bits.
- * The same inputs give the same outputs, also after a run (only new pages are written); the outputs must
- * not be the inputs (copy *free_next to *free_start, context_lens to cached_lens, behind the call).
+ * The same inputs give the same outputs, also after a run (only new pages are written); an output that
+ * overlaps an input is refused (copy *free_next to *free_start, context_lens to cached_lens, behind the call).
  * Implemented: requests <= 8192.  One launch, no workspace.
  * ---------------------------------------------------------------------- */
 ADA_API int ada_step_metadata(const int32_t* cached_lens, const int32_t* new_lens, int32_t requests,
