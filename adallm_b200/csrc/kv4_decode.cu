@@ -419,7 +419,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       for (int m = 0; m < 8; ++m) a.o[m][0] = a.o[m][1] = a.o[m][2] = a.o[m][3] = 0.f;
       a.l[0] = a.l[1] = 0.f;
       float base0 = 0.f, base1 = 0.f;              // the running maxima
-      float pass0 = -INFINITY, pass1 = -INFINITY;  // scores beyond these move them; -inf: there is none yet
+      // scores beyond these move them; -inf: there is none yet (rounded down: the next score above may be 16 further,
+      // and p = 2^16 is an infinity in fp16)
+      float pass0 = -INFINITY, pass1 = -INFINITY;
 
       // A step whose ring slot is a constant, and so its addresses (549 instead of 583 instructions, 224 -> 221 us for the
       // long case).  ROWS keeps the slot a variable: with its masks the step stands there once (36 bytes of spill stores
@@ -524,12 +526,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
           if (n0 > pass0) {
             f0 = pass0 == -INFINITY ? 0.f : fast_exp2((base0 - n0) * fac[0]);
             base0 = n0;
-            pass0 = n0 + 8.f / fac[0];
+            pass0 = __fadd_rd(n0, 8.f / fac[0]);
           }
           if (n1 > pass1) {
             f1 = pass1 == -INFINITY ? 0.f : fast_exp2((base1 - n1) * fac[1]);
             base1 = n1;
-            pass1 = n1 + 8.f / fac[1];
+            pass1 = __fadd_rd(n1, 8.f / fac[1]);
           }
           a.l[0] *= f0;
           a.l[1] *= f1;
