@@ -471,9 +471,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       // The running max is the reference point of this row's O and l.  It is moved (and O, l
       // rescaled by alpha) only when the block's max exceeds it by more than 2^RESCALE_LOG2, so
       // the probabilities stay <= 2^8 (exact in fp16's range) and O / l is unchanged: the same
-      // reference point scales numerator and denominator.
+      // reference point scales numerator and denominator.  (Moved by the difference, which is exact:
+      // near 2^27 m + 8 may round up to the next score, 16 above m.)
       float alpha = 1.f;
-      if (mx > m + RESCALE_LOG2 || (m == -INFINITY && mx != -INFINITY)) {
+      if (mx - m > RESCALE_LOG2 || (m == -INFINITY && mx != -INFINITY)) {
         alpha = fast_exp2(m - mx);  // 0 when the row had no visible key yet
         m = mx;
       }

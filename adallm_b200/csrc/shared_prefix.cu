@@ -1339,9 +1339,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 fmaxf(fmaxf(mq[4], mq[5]), fmaxf(mq[6], mq[7])));
         const float mx = raw * c;
         // The reference of a row's O and l follows its maximum only when that grew by more than
-        // 2^RESCALE_LOG2: weights stay <= 2^8, exact enough in fp16, and O / l does not change.
+        // 2^RESCALE_LOG2: weights stay <= 2^8, exact enough in fp16, and O / l does not change.  (By the difference,
+        // which is exact: near 2^27 m + 8 may round up to the next score, 16 above m.)
         float alpha = 1.f;
-        if (mx > m + RESCALE_LOG2 || (m == -INFINITY && mx != -INFINITY)) {
+        if (mx - m > RESCALE_LOG2 || (m == -INFINITY && mx != -INFINITY)) {
           alpha = fast_exp2(m - mx);
           m = mx;
           m_raw = raw;

@@ -11,6 +11,8 @@ import pytest
 import torch
 
 from adallm_b200 import kvcache_fp4 as kv
+from adallm_b200.attention import paged_prefill
+from adallm_b200.shared_prefix import shared_prefix_decode
 from tests.gpu_util import dev
 
 pytestmark = pytest.mark.gpu
@@ -19,7 +21,7 @@ LN2 = float(torch.tensor(math.log(2.0)))
 WANT = (1.0 + 2.0 * 2.0 ** 16) / (1.0 + 2.0 ** 16)  # value 1 at the first key, 2 at the second
 
 
-def near(out, zero=None):
+def near(out):
     half = torch.finfo(out.dtype).eps / 2
     assert out.isfinite().all()
     assert ((out.double() - WANT).abs() <= (2.0 ** -11 + 2.0 ** -20 + half) * WANT).all(), (float(out.min()), float(out.max()))
@@ -65,4 +67,41 @@ def test_4_bit_prefill(sequences, keys, new):
     cu = torch.arange(sequences + 1, dtype=torch.int32, device=dev())
     out = kv.paged_prefill_fp4(queries4(sequences * new, 4), kc, vc, tables, cu * new, cu * keys, new, LN2,
                                out=torch.empty((sequences * new, 4, 128), dtype=F16, device=dev()))
+    near(out)
+
+
+def caches8(keys, page, at):
+    """e4m3 caches of one head: key rows of 0, but 256 in elements 0 to 15 and 1 or 2 in element 16 of the keys at `at`."""
+    pages = -(-keys // page)
+    k, v = (torch.zeros((pages * page, 1, 128), device=dev()) for _ in range(2))
+    for key, value in zip(at, (1.0, 2.0)):
+        k[key, :, :16], k[key, :, 16], v[key] = 256.0, value, value
+    return *(x.to(torch.float8_e4m3fn).view(pages, page, 1, 128) for x in (k, v)), torch.arange(
+        pages, dtype=torch.int32, device=dev())[None]
+
+
+def queries8(rows, heads):
+    q = torch.zeros((rows, heads, 128), dtype=BF16, device=dev())
+    q[..., :16], q[..., 16] = 2.0 ** 15, 16.0
+    return q
+
+
+@pytest.mark.parametrize("keys,new", [(600, 300), (3000, 64)])
+def test_e4m3_prefill(keys, new):
+    kc, vc, tables = caches8(keys, 16, (3, 100))
+    cu = torch.arange(2, dtype=torch.int32, device=dev())
+    out = paged_prefill(queries8(new, 4), kc, vc, tables, cu * new, cu * keys, new, LN2,
+                        out=torch.empty((new, 4, 128), dtype=F16, device=dev()))
+    near(out)
+
+
+@pytest.mark.parametrize("sequences,prefix", [(4, 700), (64, 8192), (200, 20000)])
+def test_shared_prefix(sequences, prefix):
+    """Both keys in the prefix; the sequences' own keys are the row of zeros behind it."""
+    kc, vc, tables = caches8(prefix + 16, 16, (3, 140))
+    own = torch.full((sequences, 1), prefix // 16, dtype=torch.int32, device=dev())
+    out = shared_prefix_decode(queries8(sequences, 4), kc, vc, tables[:, :prefix // 16],
+                               torch.tensor([prefix // 16 * 16], dtype=torch.int32, device=dev()), None, own,
+                               torch.ones(sequences, dtype=torch.int32, device=dev()), LN2,
+                               out=torch.empty((sequences, 4, 128), dtype=F16, device=dev()))
     near(out)
