@@ -170,6 +170,12 @@ __device__ __forceinline__ float score_factor(float scale_log2, int exponent) {
   return fmaxf(fminf(scale_log2 * pow2(-exponent), 1.2379400392853803e27f), 1e-36f);
 }
 
+// Probabilities enter the products in fp16 as 2^6 times the weight against a row's reference, which a score passes by 8
+// (log2) at most and, in the prefill kernel's rounding, 1 more: 2^15 then.  Their half step is 2^-11 of themselves from 2^-20
+// of the reference's weight on, and 2^-31 of that below (without the factor 2^-25: thousands of keys of less, behind one
+// that takes most, were all lost).  The sums, in fp32, carry the same factor.
+constexpr float P_LOG2 = 6.f;
+
 // A tensor's scale that both it and its reciprocal are good for as fp32 factors (no NaN, infinity or subnormal).
 inline bool scale_ok(float s) { return s >= 1e-30f && s <= 1e30f; }
 inline bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }

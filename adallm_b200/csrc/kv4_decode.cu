@@ -20,7 +20,7 @@
 //                  widened, so a byte becomes an operand register (key, key + 1) by one conversion.
 // P^T comes from S^T by a transpose of 8x8 fragments (movmatrix).  A code times its scale is exact
 // in fp16.  The running maximum moves when a score passes it by 8 (log2): a vote a step instead
-// of a reduction; p <= 2^8 in fp16 then, half a step 2^-11 of itself, and the sums are fp32.
+// of a reduction; p (kv4.cuh, P_LOG2) is fp16 in the product, half a step 2^-11 of itself, and the sums are fp32.
 //
 // Instructions come next after HBM: widening takes 128 a lane and tile (a conversion, at half the rate, and a
 // product for two elements), so everything else is kept per 32 keys.  32 sequences of 32,767 keys, 32/8 heads: 221 us,
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
       a.l[0] = a.l[1] = 0.f;
       float base0 = 0.f, base1 = 0.f;              // the running maxima
       // scores beyond these move them; -inf: there is none yet (rounded down: the next score above may be 16 further,
-      // and p = 2^16 is an infinity in fp16)
+      // and its p an infinity in fp16)
       float pass0 = -INFINITY, pass1 = -INFINITY;
 
       // A step whose ring slot is a constant, and so its addresses (549 instead of 583 instructions, 224 -> 221 us for the
@@ -546,8 +546,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) split_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint8_t* tile = step + i * TILE_BYTES + V_OFF;
-          const float p0 = fast_exp2((s[i][0] - base0) * fac[0]), p1 = fast_exp2((s[i][1] - base1) * fac[1]);
-          const float p2 = fast_exp2((s[i][2] - base0) * fac[0]), p3 = fast_exp2((s[i][3] - base1) * fac[1]);
+          const float p0 = fast_exp2(fmaf(s[i][0] - base0, fac[0], P_LOG2)), p1 = fast_exp2(fmaf(s[i][1] - base1, fac[1], P_LOG2));
+          const float p2 = fast_exp2(fmaf(s[i][2] - base0, fac[0], P_LOG2)), p3 = fast_exp2(fmaf(s[i][3] - base1, fac[1], P_LOG2));
           a.l[0] += p0 + p2;
           a.l[1] += p1 + p3;
           const uint32_t pb[2] = {transpose8(pack_half2(p0, p1)), transpose8(pack_half2(p2, p3))};

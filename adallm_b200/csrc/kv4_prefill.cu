@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     }
     const bool safe = __all_sync(0xffffffffu, factor <= SAFE_FACTOR);
     float m = -INFINITY;  // largest score that set the reference
-    float ref = 0.f;      // the reference, log2 units (0: none yet)
+    float shift = P_LOG2; // what the exponents get: P_LOG2, less the reference (log2) in safe rows
     uint64_t l2[2] = {0ull, 0ull};
     uint32_t nan_blocks = 0;
     bool failed = false;
@@ -506,9 +506,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
       const float top = max3(max3(mx[0], x[60], x[61]), max3(mx[1], x[62], x[63]), fmaxf(mx[2], mx[3]));
       float alpha = 1.f;
       if ((top - m) * factor > MOVE_LOG2) {
-        alpha = m == -INFINITY ? 0.f : safe ? fast_exp2(ref - top * factor) : fast_exp2((m - top) * factor);
+        const float to = safe ? fmaf(-top, factor, P_LOG2) : P_LOG2;
+        alpha = m == -INFINITY ? 0.f : fast_exp2(safe ? to - shift : (m - top) * factor);
         m = top;
-        ref = top * factor;
+        shift = to;
       }
       if (!safe) {  // (warp-uniform) the difference first; the loop below then only takes the exponential
         const float mm = m == -INFINITY ? 0.f : m;
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
           l2[i] = pair(s0 * alpha, s1 * alpha);
         }
       }
-      const float c1 = safe ? factor : 1.f, r1 = safe ? -ref : 0.f;
+      const float c1 = safe ? factor : 1.f, r1 = shift;
       const uint64_t c2 = pair(c1, c1), r2 = pair(r1, r1);
       uint32_t pk[32];
 #pragma unroll

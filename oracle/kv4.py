@@ -119,14 +119,14 @@ def bound(spread, size, keys, largest):
     """How far an output element may be from the exact one before it is rounded to its type.
 
     spread = sum p |v|, size = the row's largest scale * sum |q k|, largest = max |v|.
-      * probabilities enter P.V in fp16: half a step 2^-11 of each, so 2^-11 spread; below fp16's normal range
-        (reference maximum 1) half of 2^-24 each, 2^-25 keys largest
+      * probabilities enter P.V in fp16: half a step 2^-11 of each, so 2^-11 spread; they are held times
+        2^6 against the reference, so below fp16's normal range half of 2^-30 each, 2^-31 keys largest
       * a score is 128 products in 8 fp32 accumulations of 16: each at most 2^-23 of the partial sum, twice
         (truncation), 2^-19 size together; it moves p and the normaliser, 2 * 2^-19 size spread
       * the exponent's argument and exp2 (2^-22 each), fp32 sums of p and of P.V over the keys (2^-23 a step, at
         most keys / 16 steps in a row): (2^-20 + keys * 2^-26) spread."""
     return ((2.0 ** -11 + 2.0 ** -18 * size + 2.0 ** -20 + keys * 2.0 ** -26) * spread
-            + keys * 2.0 ** -25 * largest)
+            + keys * 2.0 ** -31 * largest)
 
 
 def rotate(x, positions, inv_freq, interleaved=False, amplitude=1.0):
