@@ -23,8 +23,10 @@
 // of a reduction; p (kv4.cuh, P_LOG2) is fp16 in the product, half a step 2^-11 of itself, and the sums are fp32.
 //
 // Instructions come next after HBM: widening takes 128 a lane and tile (a conversion, at half the rate, and a
-// product for two elements), so everything else is kept per 32 keys.  32 sequences of 32,767 keys, 32/8 heads: 221 us,
-// 0.84 of the copy rate; at the power cap (1.7 GHz) the instructions are the bound and it takes about 260.
+// product for two elements), so everything else is kept per 32 keys.  32 sequences of 32,767 keys, 32/8 heads: 220 us,
+// 0.84 of the copy rate; at the power cap (1.7 GHz) the instructions are the bound and it takes about 260.  (Past some 1,040
+// sequences, 690 with few rows, the lists take more than half of an SM's shared memory beside the rings: one CTA an SM is
+// resident then, and the equal shares of the grid are worked off in two waves.)
 #include "kv4.cuh"
 
 namespace ada {

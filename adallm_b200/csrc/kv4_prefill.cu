@@ -8,8 +8,8 @@
 // Floor of a block of 64 keys: 256 x 64 exponentials (16 a cycle and SM: 1,024 cycles), 2 x 256 x 64 x 128
 // multiply-adds (4,096 a cycle: 1,024) and the operands' shared-memory reads (some 1,400).  It takes about 1,900: the
 // softmax of the two tiles' rows on one scheduler runs in step (its exponentials 1,300 cycles side by side, 850 alone) and
-// its loads, maxima and waits (600) come in between.  4 x 2,048 tokens behind 2,048, 32/8 heads: 417 us, 0.59 of
-// the measured matrix rate.  Tried and left out: two threads a row (524: they have to agree on the reference),
+// its loads, maxima and waits (600) come in between.  4 x 2,048 tokens behind 2,048, 32/8 heads: 413 us, 0.59 of
+// the measured matrix rate (445 call after call, at the power cap).  Tried and left out: two threads a row (524: they have to agree on the reference),
 // turns between the tiles (466), part of the exponentials as polynomials on the FMA pipe (426-454), 128 keys a block (564).
 //
 // One CTA a (256-row query block, KV head, sequence), or several that share its keys where there are few
@@ -681,8 +681,8 @@ constexpr int64_t FEW_ROWS = 32, FEW_KEYS = 256;
 
 // A few rows a KV head behind tables of more than 256 keys go to the decode kernel's form, which shares the
 // keys out over all SMs; this one has a CTA for 256 rows, which walks its keys alone.  Measured, 32/8 heads, 8
-// sequences of 2 new tokens: 60 cached keys 13.0 us shared out and 7.8 here, 500: 16.8 and 20.9, 8,000: 33 and 221; 32
-// sequences of 8: 60: 26 and 20, 500: 36 and 41, 8,000: 235 and 431 (16 tokens would be even).
+// sequences of 2 new tokens: 60 cached keys 12.9 us shared out and 8.6 here, 500: 16.7 and 17.0, 8,000: 32.6 and 149; 32
+// sequences of 8: 60: 26 and 19.5, 500: 35.5 and 32, 8,000: 235 and 251; 16 tokens, 64 rows, behind 8,000: 455-470 and 258.
 static bool prefill_few(int64_t batch, int64_t most, int32_t num_heads, int32_t num_kv_heads, int32_t max_pages,
                         int32_t page_size) {
   constexpr int64_t MOST = 1 << 30;  // steps of 32 keys, which that kernel counts in 32 bits
@@ -694,8 +694,8 @@ static bool prefill_few(int64_t batch, int64_t most, int32_t num_heads, int32_t 
 
 // CTAs that a query block's keys are shared by: as many as are resident at once, each with four blocks of 64 keys or more
 // (a CTA costs 9 us around its blocks and the join 4-5; a row of new tokens sees half of them on average).  One
-// sequence, 32/8 heads, alone and shared: 60 tokens behind 700 keys 24.7 and 17.9 us, 100 behind 1,500: 44 and 23, 128
-// behind 8,000: 150 and 40, 512 behind 8,000: 157 and 90; 512 alone would take 20.3 instead of 18.0.  (Eight
+// sequence, 32/8 heads, alone and shared: 60 tokens behind 700 keys 23 and 19 us, 100 behind 1,500: 43 and 20, 128
+// behind 8,000: 155 and 41, 512 behind 8,000: 161 and 95; 512 alone would take 20.3 instead of 18.0.  (Eight
 // blocks at least: 25.0 for the first, 25.6 for the second.)
 static int prefill_splits(int64_t batch, int64_t most, int32_t num_heads, int32_t num_kv_heads, int64_t reach,
                           int32_t window) {

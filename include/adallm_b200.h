@@ -711,7 +711,8 @@ ADA_API int ada_rotary(const int64_t* positions, const void* q, int64_t q_stride
  *
  * ada_kv4_store packs the rows of k and v (strides as in ada_rotary) at slot_mapping int32 [T] (slot = page *
  * page_size + row; slots outside the cache, -1 among them, are skipped; a slot given twice holds a mix
- * of both rows).  Of x = element / k_scale in fp32: scale = e4m3(min(max |x| / 6, 448)) of a block of 16, code =
+ * of both rows).  Of x = element / k_scale in fp32 (correctly rounded for scales of
+ * six bits, as powers of two; else but for one quotient in 2^20, a step off): scale = e4m3(min(max |x| / 6, 448)) of a block of 16, code =
  * the nearest e2m1 to x / scale, ties to even, saturating (infinities too); a block with a NaN reads as
  * NaN.  With positions, q and k are rotated first as by ada_rotary (k rounded to the type before it
  * is packed) and q is written to q_out; without (NULL), rows are stored as they are, and q may be NULL
@@ -753,8 +754,7 @@ ADA_API int ada_kv4_paged_decode(const void* q, int q_dtype, int64_t q_stride_b,
  * the row's own position and the W before it); rows of q and out outside [0, total_q) and rows
  * behind the last sequence are not touched.  A few rows a KV head (max_seqlen_q x heads a KV head up to 32)
  * behind tables of more than 256 keys take the decode form, which shares long caches out over all SMs.
- * where there are
- * fewer CTAs of 256 rows than SMs, several share a block's keys and a second launch joins them.  workspace: as for decode,
+ * Where there are fewer CTAs of 256 rows than SMs, several share a block's keys and a second launch joins them.  workspace: as for decode,
  * sized by ada_kv4_paged_prefill_workspace_size (0 where one launch does it; 20 MB at most but for few rows' tables).  *err (may be NULL): 0x70
  * if a tile wait ran out (the rows concerned are NaN).  A NaN key reaches every element of the rows that see it, a NaN value the 16 elements of its
  * block, and neither any other row.  Implemented: up to 256 heads a KV head. */
