@@ -196,11 +196,12 @@ class RotaryEmbedding(nn.Module):
 
 
 @lru_cache(1)
-def _get_rope_cached(head_size, rotary_dim, max_position, base, rope_scaling_key):
+def _get_rope_cached(head_size, rotary_dim, max_position, base, rope_scaling_key, interleaved):
     rope_scaling = dict(rope_scaling_key) if rope_scaling_key is not None else None
-    return RotaryEmbedding(head_size, rotary_dim, max_position, base, rope_scaling=rope_scaling)
+    return RotaryEmbedding(head_size, rotary_dim, max_position, base, rope_scaling=rope_scaling, interleaved=interleaved)
 
 
-def get_rope(head_size: int, rotary_dim: int, max_position: int, base: float, rope_scaling: dict | None = None):
+def get_rope(head_size: int, rotary_dim: int, max_position: int, base: float, rope_scaling: dict | None = None,
+             interleaved: bool = False):
     key = None if rope_scaling is None else tuple(sorted(rope_scaling.items()))
-    return _get_rope_cached(head_size, rotary_dim, max_position, base, key)
+    return _get_rope_cached(head_size, rotary_dim, max_position, base, key, bool(interleaved))

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from adallm_b200.rotary_embedding import RotaryEmbedding
+from adallm_b200.rotary_embedding import RotaryEmbedding, get_rope
 
 FORMS = [(128, 128, False), (128, 64, False), (128, 128, True), (256, 64, True)]
 SHAPES = [((0,), (0, 4, 0), (0, 1, 0)), ((0,), (0, 0), (0, 0)), ((2, 0), (2, 0, 0), (2, 0, 0)), ((3, 0), (3, 0, 4, 0), (3, 0, 2, 0))]
@@ -50,3 +50,11 @@ def test_shapes_of_few_tokens(d, r, interleaved):
     no = q[:, :0].reshape(6, 0, d)
     if r < d or interleaved:  # (without key heads)
         assert torch.equal(m(pos, q, no)[0], want[0])
+
+
+@pytest.mark.parametrize("d,r,interleaved", FORMS)
+def test_get_rope_gives_every_form(d, r, interleaved):
+    m = get_rope(d, r, 16, 1e4, None, interleaved)
+    assert (m.head_size, m.rotary_dim, m.interleaved) == (d, r, interleaved) and m.cos_sin_cache.shape == (16, 1, r)
+    assert get_rope(d, r, 16, 1e4, None, interleaved) is m and get_rope(d, r, 16, 1e4, None, not interleaved) is not m
+    assert get_rope(d, r, 16, 1e4).interleaved is False
