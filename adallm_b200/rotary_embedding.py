@@ -28,27 +28,31 @@ def _yarn_cos_sin_cache(rotary_dim: int, max_position: int, base: float, rope_sc
     frequency, those below beta_slow turns are slowed by `factor`, a linear ramp lies between (its ends on whole
     pairs unless `truncate` is false); cos and sin are multiplied by the attention factor: 0.1 ln(factor) + 1, or with
     mscale m and mscale_all_dim n (0.1 m ln(factor) + 1) / (0.1 n ln(factor) + 1).  Angles in 64 bits, the table in
-    fp32.  The table has factor x original_max_position_embeddings rows at least, as positions behind its last
-    row are clamped to it.  Keys that would change the table in a way not known here are refused."""
+    fp32.  The table has factor x original_max_position_embeddings rows at least (where that is not given it is
+    max_position / factor), as positions behind its last row are clamped to it.  Keys that would change the table in
+    a way not known here are refused."""
     given = {k: v for k, v in rope_scaling.items() if v is not None}
     unknown = sorted(set(given) - _YARN_KEYS)
     if unknown:
         raise ValueError(f"yarn rope_scaling: unknown {', '.join(unknown)}")
     if float(given.get("rope_theta", base)) != float(base):
         raise ValueError("yarn rope_scaling: rope_theta is not the table's base")
-    if "factor" not in given or "original_max_position_embeddings" not in given:
-        raise ValueError("yarn rope_scaling needs factor and original_max_position_embeddings")
-    factor, trained = float(given["factor"]), float(given["original_max_position_embeddings"])
+    if "factor" not in given:
+        raise ValueError("yarn rope_scaling needs its factor")
+    factor = float(given["factor"])
+    if not 0.0 < factor < math.inf:
+        raise ValueError("yarn rope_scaling: factor must be positive")
+    trained = float(given.get("original_max_position_embeddings", max_position / factor))
     fast, slow = float(given.get("beta_fast", 32.0)), float(given.get("beta_slow", 1.0))
-    if not (1.0 <= factor < math.inf and 1.0 <= trained < math.inf and 0.0 < slow <= fast < math.inf):
-        raise ValueError("yarn rope_scaling: factor and original_max_position_embeddings of at least 1, 0 < beta_slow <= "
-                         "beta_fast")
+    if not (0.0 < trained < math.inf and 0.0 < slow <= fast < math.inf):
+        raise ValueError("yarn rope_scaling: original_max_position_embeddings must be positive, 0 < beta_slow <= beta_fast")
     scales = [k for k in ("attention_factor", "mscale", "mscale_all_dim") if k in given]
     if not all(0.0 < float(given[k]) < math.inf for k in scales):
         raise ValueError("yarn rope_scaling: attention_factor, mscale and mscale_all_dim must be positive")
     if ("mscale" in given) != ("mscale_all_dim" in given):
         raise ValueError("yarn rope_scaling: mscale and mscale_all_dim go together")  # (one alone is read in two ways)
-    m, n = (0.1 * float(given.get(k, d)) * math.log(factor) + 1.0 for k, d in (("mscale", 1.0), ("mscale_all_dim", 0.0)))
+    stretch = 0.1 * math.log(max(factor, 1.0))
+    m, n = (stretch * float(given.get(k, d)) + 1.0 for k, d in (("mscale", 1.0), ("mscale_all_dim", 0.0)))
     amplitude = float(given.get("attention_factor", m / n))
     half = rotary_dim // 2
 
@@ -63,7 +67,7 @@ def _yarn_cos_sin_cache(rotary_dim: int, max_position: int, base: float, rope_sc
     keep = 1.0 - ((i - low) / max(high - low, 0.001)).clamp(0, 1)
     inv_freq = base ** (-i / half)
     inv_freq = inv_freq * keep + inv_freq / factor * (1.0 - keep)
-    rows = max(max_position, math.ceil(factor * trained))
+    rows = max(max_position, math.ceil(factor * trained)) if "original_max_position_embeddings" in given else max_position
     angle = torch.arange(rows, dtype=torch.float64, device=device)[:, None] * inv_freq
     return (torch.cat((angle.cos(), angle.sin()), -1) * amplitude).float().unsqueeze_(1)
 

@@ -63,13 +63,16 @@ def test_tables_cover_the_scaled_length():
     odd = {**YARN, "factor": 1.5, "original_max_position_embeddings": 333}
     assert build_cos_sin_cache(64, 16, BASE, odd).shape[0] == 500
     assert build_cos_sin_cache(64, 16, BASE, {"rope_type": "linear", "factor": 4.0}).shape[0] == 16
+    # without the original length max_position is the scaled one
+    near(build_cos_sin_cache(64, 4096, BASE, {"type": "yarn", "factor": FACTOR}), want[:4096], scale(1))
+    assert all(build_cos_sin_cache(64, n, BASE, {"type": "yarn", "factor": f}).shape[0] == n for n in (1000, 4097)
+               for f in (1.1, 3.0, 7.7))
 
 
 @pytest.mark.parametrize("keys", [
     {"mscale": 1.0}, {"mscale_all_dim": 1.0}, {"mscale": 0.0, "mscale_all_dim": 1.0}, {"mscale": 1.0, "mscale_all_dim": -1.0},
     {"attention_factor": 0.0}, {"attention_factor": math.nan}, {"extrapolation_factor": 1.0}, {"short_factor": [1.0]},
-    {"factor": None}, {"factor": 0.5}, {"factor": math.inf}, {"original_max_position_embeddings": None},
-    {"original_max_position_embeddings": 0}, {"beta_fast": 1.0, "beta_slow": 2.0}, {"beta_slow": 0.0}, {"rope_theta": 5e5}])
+    {"factor": None}, {"factor": 0.0}, {"factor": math.inf}, {"original_max_position_embeddings": 0}, {"beta_fast": 1.0, "beta_slow": 2.0}, {"beta_slow": 0.0}, {"rope_theta": 5e5}])
 def test_refusals(keys):
     with pytest.raises(ValueError):
         build_cos_sin_cache(128, 4096, BASE, {**YARN, **keys})
