@@ -20,7 +20,8 @@ from . import _native as N
 
 
 _YARN_KEYS = {"rope_type", "type", "rope_theta", "factor", "original_max_position_embeddings", "beta_fast", "beta_slow",
-              "attention_factor", "mscale", "mscale_all_dim", "truncate"}
+              "attention_factor", "mscale", "mscale_all_dim", "truncate",
+              "partial_rotary_factor"}  # (the table's width is an argument)
 
 
 def _yarn_cos_sin_cache(rotary_dim: int, max_position: int, base: float, rope_scaling: dict, device=None):

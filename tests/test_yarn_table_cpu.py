@@ -46,7 +46,8 @@ def scale(m):
     ({"attention_factor": 1.25}, 1.25, {}), ({"attention_factor": 0.5, "mscale": 1.0, "mscale_all_dim": 1.0}, 0.5, {}),
     ({"truncate": False}, scale(1), dict(truncate=False)), ({"truncate": True}, scale(1), {}),
     ({"beta_fast": 16.0, "beta_slow": 2}, scale(1), dict(fast=16.0, slow=2.0)),
-    ({"beta_fast": None, "attention_factor": None, "mscale": None, "truncate": None, "rope_theta": BASE}, scale(1), {})])
+    ({"beta_fast": None, "attention_factor": None, "mscale": None, "truncate": None, "rope_theta": BASE}, scale(1), {}),
+    ({"partial_rotary_factor": 0.5}, scale(1), {})])
 @pytest.mark.parametrize("width", [64, 128])
 def test_every_key(keys, amplitude, ramp, width):
     rows = int(FACTOR) * TRAINED
